@@ -231,6 +231,142 @@ int spatten_decode_attend(const spatten_decode_args* a, void* workspace, size_t 
                           void* stream);
 
 /*
+ * Paged KV cache held in 8 bits, one fp32 scale per block of tokens and KV
+ * head (a block is a page). The cache that a model appends to and attends
+ * over while it generates; no counterpart in the reference, which has no
+ * decoding.
+ *
+ * Pool: k, v [num_pages, G, page_size, D] codes, k_scale, v_scale
+ * [num_pages, G] fp32, contiguous; a value is code * scale. Slot s of
+ * sequence b is row s % page_size of page page_table[b, s / page_size]
+ * (int32, row stride table_stride elements). A page number outside
+ * [0, num_pages) has no memory: nothing is appended there, and its slots
+ * are no keys. page_size is 16, 32, 64 or 128; D is 64 or 128.
+ *
+ * Codes are finite in both types: int8 (scale = max|x| / 127) or e4m3
+ * (scale = the smallest power of two with max|x| <= 448 * scale, so that
+ * dividing by it is exact).
+ *
+ * A batch's new tokens are packed: sequence b brings the rows cu_tokens[b]
+ * .. cu_tokens[b+1]-1 (int32 [B+1], ascending, within [0, T]) of q / k / v /
+ * out, and holds seq_lens[b] tokens in all (int32 [B]), these included, which
+ * are its last ones: row cu_tokens[b] + i is slot
+ * seq_lens[b] - (cu_tokens[b+1] - cu_tokens[b]) + i. max_tokens bounds the
+ * tokens of one sequence (rows beyond it are left alone), so that the launch
+ * needs no device value on the host; it sizes the grid. Rows behind the last
+ * sequence are neither read nor written. All of these may change between the
+ * replays of a captured call.
+ */
+#define SPATTEN_KV_INT8 0
+#define SPATTEN_KV_E4M3 1
+typedef struct {
+  int kv_type; /* SPATTEN_KV_* */
+  int num_pages, page_size, G, D;
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* page_table; /* [B, max_pages] */
+  int64_t table_stride;
+  int max_pages;
+} spatten_paged_cache;
+
+/*
+ * Appends the new tokens' keys and values. In fp32, rounded once at the end:
+ *   x = k row (times rsqrt(mean(x^2) + eps) * k_norm_w where given),
+ *   rotated where cos / sin are given: (x1 c - x2 s, x2 c + x1 s) with
+ *   x1, x2 the halves of the row (HF rotate_half) and c, s the first D/2
+ *   entries of row `position` of the tables; v rows as they are.
+ * Then per written page and head: S = the larger of the page's scale (0 for a
+ * page whose first slot is new) and the scale of the largest finite new
+ * magnitude; where S grew the page's earlier codes become
+ * round(code * S_old / S); the new codes are round(x / S), saturated, a NaN
+ * stored as 0. With q, q_out (may be q itself) receives the query rows, normed
+ * with q_norm_w and rotated the same way, rounded to dtype.
+ * position: positions[row] (int32 [T]) or, without it, the row's slot; clamped
+ * to the table's cs_rows rows. Two sequences must not append into the same
+ * page in one call (sharing pages that are only read is fine).
+ * q / k / v / q_out: [T, heads, D] with strides in elements (multiples of 8,
+ * pointers 16-byte aligned), D contiguous; q_norm_w, k_norm_w [D] of dtype;
+ * cos, sin fp32 (cs_dtype SPATTEN_DTYPE_F32) or of dtype.
+ */
+typedef struct {
+  spatten_paged_cache cache;
+  int dtype; /* SPATTEN_DTYPE_F16 or _BF16 */
+  int B, H, T, max_tokens; /* H: query heads (0 without q) */
+  const int32_t* cu_tokens;
+  const int32_t* seq_lens;
+  const void* q;
+  int64_t q_st, q_sh;
+  const void* k;
+  int64_t k_st, k_sh;
+  const void* v;
+  int64_t v_st, v_sh;
+  void* q_out;
+  int64_t qo_st, qo_sh;
+  const void* q_norm_w; /* optional, both or neither with q */
+  const void* k_norm_w;
+  float eps;
+  const void* cos; /* optional [cs_rows, >= D/2], row stride cs_stride */
+  const void* sin;
+  int cs_dtype, cs_rows;
+  int64_t cs_stride;
+  const int32_t* positions; /* optional */
+} spatten_paged_append_args;
+
+int spatten_paged_append(const spatten_paged_append_args* a, void* stream);
+
+/*
+ * Attention of the new tokens' queries over the cache: query i of sequence b
+ * sees slots n < seq_lens[b] - n_b + i + 1 (n_b: the sequence's new tokens),
+ * its own among them when they were appended before:
+ *   out[row, h] = softmax(sm_scale * q[row, h] . K[h / (H/G)]) . V[h / (H/G)]
+ * over fp32 scores and statistics; 0 for a row that sees no key. Serves one
+ * token per sequence, a few drafted ones, or the next piece of a prompt.
+ * q, out: [T, H, D] by strides as in spatten_paged_append; H % G == 0,
+ * H / G <= 128.
+ */
+typedef struct {
+  spatten_paged_cache cache;
+  int dtype;
+  int B, H, T, max_tokens;
+  const int32_t* cu_tokens;
+  const int32_t* seq_lens;
+  const void* q;
+  int64_t q_st, q_sh;
+  void* out;
+  int64_t o_st, o_sh;
+  float sm_scale;
+} spatten_paged_attend_args;
+
+/* Bytes of workspace the call needs (256-byte aligned); 0 for bad arguments. */
+size_t spatten_paged_attend_workspace_size(const spatten_paged_attend_args* a);
+int spatten_paged_attend(const spatten_paged_attend_args* a, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/*
+ * Reads cached tokens back in 16 bits:
+ *   k_out[b, j] = code * scale of slot idx[b, j] (idx int64 [B, N], row stride
+ *   idx_stride; NULL: slot j), zeros where the slot is outside
+ *   [0, seq_lens[b]) or its page has no memory; v_out the same.
+ * The gather of the tokens that a cascade keeps (spatten_topk_indices) out of
+ * the cache, or a dense copy of a sequence. k_out, v_out [B, N, G, D] of dtype,
+ * contiguous, 16-byte aligned; either may be NULL.
+ */
+typedef struct {
+  spatten_paged_cache cache;
+  int dtype;
+  int B, N;
+  const int32_t* seq_lens;
+  const int64_t* idx;
+  int64_t idx_stride;
+  void* k_out;
+  void* v_out;
+} spatten_paged_read_args;
+
+int spatten_paged_read(const spatten_paged_read_args* a, void* stream);
+
+/*
  * Fused Q/K/V projection of the active heads, with the quantisation the
  * attention kernel reads. Replaces, per layer of the cascade:
  *   slice_linear_weights (module.py:12-34): index_select of the active heads'

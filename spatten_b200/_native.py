@@ -17,6 +17,7 @@ ERR_UNSUPPORTED = 3
 DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 MODE_QUANT, MODE_DENSE, MODE_COMPAT = 0, 1, 2
 PROJ_QUANT, PROJ_DENSE = 0, 1
+KV_INT8, KV_E4M3 = 0, 1
 
 ABI_VERSION = 4
 MAX_V_PRUNE_COUNT = 16  # spatten_prog_attn_args.v_prune_count limit
@@ -81,6 +82,45 @@ class QkNormRopeArgs(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """Mirror of spatten_paged_cache (include/spatten_b200.h)."""
+    _fields_ = [
+        ("kv_type", c_int), ("num_pages", c_int), ("page_size", c_int), ("G", c_int), ("D", c_int),
+        ("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp),
+        ("page_table", c_vp), ("table_stride", c_i64), ("max_pages", c_int),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """Mirror of spatten_paged_append_args (include/spatten_b200.h)."""
+    _fields_ = [
+        ("cache", PagedCache), ("dtype", c_int), ("B", c_int), ("H", c_int), ("T", c_int), ("max_tokens", c_int),
+        ("cu_tokens", c_vp), ("seq_lens", c_vp),
+        ("q", c_vp), ("q_st", c_i64), ("q_sh", c_i64), ("k", c_vp), ("k_st", c_i64), ("k_sh", c_i64),
+        ("v", c_vp), ("v_st", c_i64), ("v_sh", c_i64), ("q_out", c_vp), ("qo_st", c_i64), ("qo_sh", c_i64),
+        ("q_norm_w", c_vp), ("k_norm_w", c_vp), ("eps", c_float), ("cos", c_vp), ("sin", c_vp),
+        ("cs_dtype", c_int), ("cs_rows", c_int), ("cs_stride", c_i64), ("positions", c_vp),
+    ]
+
+
+class PagedAttendArgs(ctypes.Structure):
+    """Mirror of spatten_paged_attend_args (include/spatten_b200.h)."""
+    _fields_ = [
+        ("cache", PagedCache), ("dtype", c_int), ("B", c_int), ("H", c_int), ("T", c_int), ("max_tokens", c_int),
+        ("cu_tokens", c_vp), ("seq_lens", c_vp),
+        ("q", c_vp), ("q_st", c_i64), ("q_sh", c_i64), ("out", c_vp), ("o_st", c_i64), ("o_sh", c_i64),
+        ("sm_scale", c_float),
+    ]
+
+
+class PagedReadArgs(ctypes.Structure):
+    """Mirror of spatten_paged_read_args (include/spatten_b200.h)."""
+    _fields_ = [
+        ("cache", PagedCache), ("dtype", c_int), ("B", c_int), ("N", c_int), ("seq_lens", c_vp),
+        ("idx", c_vp), ("idx_stride", c_i64), ("k_out", c_vp), ("v_out", c_vp),
+    ]
+
+
 class CompactOutProjArgs(ctypes.Structure):
     """Mirror of spatten_compact_out_proj_args (include/spatten_b200.h)."""
     _fields_ = [
@@ -108,6 +148,10 @@ SIGNATURES = {
     "spatten_decode_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(DecodeArgs)]),
     "spatten_decode_importance": (c_int, [ctypes.POINTER(DecodeArgs), c_vp, ctypes.c_size_t, c_vp]),
     "spatten_decode_attend": (c_int, [ctypes.POINTER(DecodeArgs), c_vp, ctypes.c_size_t, c_vp]),
+    "spatten_paged_append": (c_int, [ctypes.POINTER(PagedAppendArgs), c_vp]),
+    "spatten_paged_attend_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(PagedAttendArgs)]),
+    "spatten_paged_attend": (c_int, [ctypes.POINTER(PagedAttendArgs), c_vp, ctypes.c_size_t, c_vp]),
+    "spatten_paged_read": (c_int, [ctypes.POINTER(PagedReadArgs), c_vp]),
     "spatten_qkv_proj": (c_int, [ctypes.POINTER(QkvProjArgs), c_vp]),
     "spatten_qk_norm_rope": (c_int, [ctypes.POINTER(QkNormRopeArgs), c_vp]),
     "spatten_compact_out_proj": (c_int, [ctypes.POINTER(CompactOutProjArgs), c_vp]),

@@ -12,6 +12,7 @@
 #include "common.cuh"
 #include "decode.h"
 #include "kernels.h"
+#include "paged.h"
 #include "proj.h"
 
 namespace {
@@ -504,6 +505,171 @@ int spatten_compact_out_proj(const spatten_compact_out_proj_args* a, void* strea
   p.res = a->res; p.res_st = a->res_row_stride;
   p.out = a->out;
   return cuda_status(spatten::launch_out_proj(p, (cudaStream_t)stream), "compact_out_proj launch");
+}
+
+// Checks a paged cache and brings it into the kernels' form.
+static int fill_paged_cache(const char* who, const spatten_paged_cache& c, spatten::PagedCache& p) {
+  if (c.kv_type != SPATTEN_KV_INT8 && c.kv_type != SPATTEN_KV_E4M3)
+    return fail(SPATTEN_ERR_INVALID, "%s: kv_type %d", who, c.kv_type);
+  if (c.D != 64 && c.D != 128) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: D=%d (need 64 or 128)", who, c.D);
+  if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64 && c.page_size != 128)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: page_size %d (need 16, 32, 64 or 128)", who, c.page_size);
+  if (c.num_pages < 1 || c.G < 1 || c.max_pages < 1)
+    return fail(SPATTEN_ERR_INVALID, "%s: empty cache num_pages=%d G=%d max_pages=%d", who, c.num_pages, c.G,
+                c.max_pages);
+  if (c.G > 4096) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: %d KV heads (at most 4096)", who, c.G);
+  if ((int64_t)c.max_pages * c.page_size > (int64_t)1 << 30)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: page table of more than 2^30 slots", who);
+  if (c.table_stride < c.max_pages) return fail(SPATTEN_ERR_INVALID, "%s: page table stride < max_pages", who);
+  if (!c.k || !c.v || !c.k_scale || !c.v_scale || !c.page_table)
+    return fail(SPATTEN_ERR_INVALID, "%s: null cache pointer", who);
+  if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.k_scale, 4) || !aligned(c.v_scale, 4) ||
+      !aligned(c.page_table, 4))
+    return fail(SPATTEN_ERR_INVALID, "%s: k/v not 16-byte or scales/page table not 4-byte aligned", who);
+  p.P = c.num_pages; p.page = c.page_size; p.G = c.G; p.D = c.D; p.max_pages = c.max_pages;
+  p.k = static_cast<uint8_t*>(c.k); p.v = static_cast<uint8_t*>(c.v);
+  p.k_scale = c.k_scale; p.v_scale = c.v_scale;
+  p.table = c.page_table; p.table_st = c.table_stride;
+  return SPATTEN_OK;
+}
+
+static int fill_paged_batch(const char* who, int dtype, int B, int H, int T, int max_tokens, const int32_t* cu,
+                            const int32_t* lens, spatten::PagedBatch& p) {
+  if (dtype != SPATTEN_DTYPE_F16 && dtype != SPATTEN_DTYPE_BF16)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: dtype %d (need f16 or bf16)", who, dtype);
+  if (B < 0 || T < 0 || H < 0 || max_tokens < 0)
+    return fail(SPATTEN_ERR_INVALID, "%s: negative size B=%d H=%d T=%d max_tokens=%d", who, B, H, T, max_tokens);
+  if (B > 65535) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: B=%d (at most 65535)", who, B);
+  if (T > 1 << 30) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: more than 2^30 rows", who);
+  p.B = B; p.H = H; p.T = T;
+  p.max_tokens = max_tokens < T ? max_tokens : T;
+  p.cu = cu; p.lens = lens;
+  if (B == 0 || p.max_tokens == 0) return SPATTEN_OK;  // no work: empty tensors may carry null pointers
+  if (!cu || !lens) return fail(SPATTEN_ERR_INVALID, "%s: null cu_tokens/seq_lens", who);
+  if (!aligned(cu, 4) || !aligned(lens, 4))
+    return fail(SPATTEN_ERR_INVALID, "%s: cu_tokens/seq_lens not 4-byte aligned", who);
+  return SPATTEN_OK;
+}
+
+// a [T, heads, D] tensor of 16-bit values: 16-byte rows
+static int check_rows(const char* who, const char* name, const void* x, int64_t st, int64_t sh) {
+  if (!x) return fail(SPATTEN_ERR_INVALID, "%s: null %s", who, name);
+  if (!aligned(x, 16)) return fail(SPATTEN_ERR_INVALID, "%s: %s not 16-byte aligned", who, name);
+  if (st < 0 || sh < 0 || st % 8 || sh % 8)
+    return fail(SPATTEN_ERR_INVALID, "%s: %s strides must be non-negative multiples of 8 elements", who, name);
+  return SPATTEN_OK;
+}
+
+int spatten_paged_append(const spatten_paged_append_args* a, void* stream) {
+  static const char* who = "paged_append";
+  if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
+  spatten::PagedAppendParams p;
+  if (int e = fill_paged_cache(who, a->cache, p.c)) return e;
+  if (int e = fill_paged_batch(who, a->dtype, a->B, a->H, a->T, a->max_tokens, a->cu_tokens, a->seq_lens, p.b))
+    return e;
+  if (p.b.B == 0 || p.b.max_tokens == 0) return ok();
+  if (p.b.max_tokens / p.c.page + 2 > 65535)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: more than 65533 pages of new tokens in one sequence", who);
+  if (int e = check_rows(who, "k", a->k, a->k_st, a->k_sh)) return e;
+  if (int e = check_rows(who, "v", a->v, a->v_st, a->v_sh)) return e;
+  if (a->q) {
+    if (a->H < 1 || a->H > 65536) return fail(SPATTEN_ERR_INVALID, "%s: H=%d query heads", who, a->H);
+    if (int e = check_rows(who, "q", a->q, a->q_st, a->q_sh)) return e;
+    if (int e = check_rows(who, "q_out", a->q_out, a->qo_st, a->qo_sh)) return e;
+    if (!a->q_norm_w != !a->k_norm_w) return fail(SPATTEN_ERR_INVALID, "%s: one of q_norm_w, k_norm_w", who);
+  } else if (a->q_norm_w || a->q_out) {
+    return fail(SPATTEN_ERR_INVALID, "%s: q_norm_w or q_out without q", who);
+  }
+  if ((a->q_norm_w && !aligned(a->q_norm_w, 16)) || (a->k_norm_w && !aligned(a->k_norm_w, 16)))
+    return fail(SPATTEN_ERR_INVALID, "%s: norm weights not 16-byte aligned", who);
+  if (a->k_norm_w && !(a->eps >= 0.f)) return fail(SPATTEN_ERR_INVALID, "%s: eps must be >= 0", who);
+  if (!a->cos != !a->sin) return fail(SPATTEN_ERR_INVALID, "%s: one of cos, sin", who);
+  if (a->cos) {
+    if (a->cs_dtype != SPATTEN_DTYPE_F32 && a->cs_dtype != a->dtype)
+      return fail(SPATTEN_ERR_UNSUPPORTED, "%s: cos/sin dtype %d (need f32 or the rows' own)", who, a->cs_dtype);
+    if (a->cs_rows < 1 || a->cs_stride < p.c.D / 2 || a->cs_stride % 8)
+      return fail(SPATTEN_ERR_INVALID, "%s: cos/sin rows %d, stride %lld (need >= 1, a multiple of 8 >= D/2)", who,
+                  a->cs_rows, (long long)a->cs_stride);
+    if (!aligned(a->cos, 16) || !aligned(a->sin, 16))
+      return fail(SPATTEN_ERR_INVALID, "%s: cos/sin not 16-byte aligned", who);
+    if (a->positions && !aligned(a->positions, 4))
+      return fail(SPATTEN_ERR_INVALID, "%s: positions not 4-byte aligned", who);
+  }
+  p.q = a->q; p.q_st = a->q_st; p.q_sh = a->q_sh;
+  p.k = a->k; p.k_st = a->k_st; p.k_sh = a->k_sh;
+  p.v = a->v; p.v_st = a->v_st; p.v_sh = a->v_sh;
+  p.q_out = a->q_out; p.qo_st = a->qo_st; p.qo_sh = a->qo_sh;
+  p.wq = a->q_norm_w; p.wk = a->k_norm_w; p.eps = a->eps;
+  p.cos = a->cos; p.sin = a->sin;
+  p.cs_f32 = a->cs_dtype == SPATTEN_DTYPE_F32; p.cs_rows = a->cs_rows; p.cs_st = a->cs_stride;
+  p.positions = a->positions;
+  return cuda_status(spatten::launch_paged_append(p, a->dtype, a->cache.kv_type, (cudaStream_t)stream),
+                     "paged_append launch");
+}
+
+static int fill_paged_attend(const spatten_paged_attend_args* a, spatten::PagedAttendParams& p) {
+  static const char* who = "paged_attend";
+  if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
+  if (int e = fill_paged_cache(who, a->cache, p.c)) return e;
+  if (int e = fill_paged_batch(who, a->dtype, a->B, a->H, a->T, a->max_tokens, a->cu_tokens, a->seq_lens, p.b))
+    return e;
+  if (a->H < 1 || a->H % p.c.G) return fail(SPATTEN_ERR_INVALID, "%s: H=%d %% G=%d", who, a->H, p.c.G);
+  if (a->H / p.c.G > 128)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most 128)", who, a->H / p.c.G);
+  if (!(a->sm_scale == a->sm_scale)) return fail(SPATTEN_ERR_INVALID, "%s: sm_scale is NaN", who);
+  p.q = a->q; p.q_st = a->q_st; p.q_sh = a->q_sh;
+  p.out = a->out; p.o_st = a->o_st; p.o_sh = a->o_sh;
+  p.scale_log2 = a->sm_scale * spatten::kLog2e;
+  return SPATTEN_OK;
+}
+
+size_t spatten_paged_attend_workspace_size(const spatten_paged_attend_args* a) {
+  spatten::PagedAttendParams p;
+  if (fill_paged_attend(a, p) != SPATTEN_OK) return 0;
+  return align256(spatten::paged_attend_workspace(p, sm_count()));
+}
+
+int spatten_paged_attend(const spatten_paged_attend_args* a, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  static const char* who = "paged_attend";
+  spatten::PagedAttendParams p;
+  if (int e = fill_paged_attend(a, p)) return e;
+  if (p.b.B == 0 || p.b.max_tokens == 0) return ok();
+  if (int e = check_rows(who, "q", a->q, a->q_st, a->q_sh)) return e;
+  if (int e = check_rows(who, "out", a->out, a->o_st, a->o_sh)) return e;
+  const size_t need = align256(spatten::paged_attend_workspace(p, sm_count()));
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return fail(SPATTEN_ERR_INVALID, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
+    if (!aligned(workspace, 256)) return fail(SPATTEN_ERR_INVALID, "%s: workspace not 256-byte aligned", who);
+  }
+  return cuda_status(spatten::launch_paged_attend(p, a->dtype, a->cache.kv_type, workspace, sm_count(),
+                                                  (cudaStream_t)stream),
+                     "paged_attend launch");
+}
+
+int spatten_paged_read(const spatten_paged_read_args* a, void* stream) {
+  static const char* who = "paged_read";
+  if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
+  spatten::PagedReadParams p;
+  if (int e = fill_paged_cache(who, a->cache, p.c)) return e;
+  if (a->dtype != SPATTEN_DTYPE_F16 && a->dtype != SPATTEN_DTYPE_BF16)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: dtype %d (need f16 or bf16)", who, a->dtype);
+  if (a->B < 0 || a->N < 0) return fail(SPATTEN_ERR_INVALID, "%s: negative size B=%d N=%d", who, a->B, a->N);
+  if (a->B > 65535) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: B=%d (at most 65535)", who, a->B);
+  if (a->B == 0 || a->N == 0) return ok();
+  if ((int64_t)a->N * p.c.G * p.c.D > (int64_t)1 << 38)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: N=%d slots of %d heads", who, a->N, p.c.G);
+  if (!a->seq_lens || !aligned(a->seq_lens, 4)) return fail(SPATTEN_ERR_INVALID, "%s: null or misaligned seq_lens", who);
+  if (a->idx && (!aligned(a->idx, 8) || a->idx_stride < 0))
+    return fail(SPATTEN_ERR_INVALID, "%s: idx misaligned or of a negative stride", who);
+  if (!a->k_out && !a->v_out) return fail(SPATTEN_ERR_INVALID, "%s: neither k_out nor v_out", who);
+  if ((a->k_out && !aligned(a->k_out, 16)) || (a->v_out && !aligned(a->v_out, 16)))
+    return fail(SPATTEN_ERR_INVALID, "%s: output not 16-byte aligned", who);
+  p.B = a->B; p.N = a->N; p.lens = a->seq_lens; p.idx = a->idx; p.idx_st = a->idx_stride;
+  p.k_out = a->k_out; p.v_out = a->v_out;
+  return cuda_status(spatten::launch_paged_read(p, a->dtype, a->cache.kv_type, (cudaStream_t)stream),
+                     "paged_read launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,65 @@
+// Device helpers shared by the kernels over the paged 8-bit KV cache.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "paged.h"
+
+namespace spatten {
+
+// The packed rows [begin, begin + n) of sequence b, and the slot of the first:
+// every value that comes from the device is brought into range here.
+struct PagedSeq {
+  int begin;  // first row of q / k / v / out
+  int n;      // rows to process (at most max_tokens)
+  int len;    // slots held, at most the page table's
+  int old;    // slot of row `begin` (negative when seq_lens is below the row count)
+};
+
+SPATTEN_DEV PagedSeq paged_seq(const PagedBatch& p, const PagedCache& c, int b) {
+  PagedSeq s;
+  const int lo = min(max(__ldg(p.cu + b), 0), p.T), hi = min(max(__ldg(p.cu + b + 1), lo), p.T);
+  const int len = min(max(__ldg(p.lens + b), 0), 1 << 30);
+  s.begin = lo;
+  s.n = min(hi - lo, p.max_tokens);
+  s.old = len - (hi - lo);
+  s.len = (int)min((int64_t)len, (int64_t)c.max_pages * c.page);
+  return s;
+}
+
+// Page of slots [pi * page, ...) of sequence b, or -1 where it has no memory.
+SPATTEN_DEV int paged_page(const PagedCache& c, int b, int pi) {
+  if (pi >= c.max_pages) return -1;
+  const int pid = __ldg(c.table + (int64_t)b * c.table_st + pi);
+  return (pid >= 0 && pid < c.P) ? pid : -1;
+}
+
+// Two e4m3 codes (low byte first) as f16x2; every e4m3 value is an f16.
+SPATTEN_DEV uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  uint32_t r;
+  asm("{ .reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t; }" : "=r"(r) : "r"(two));
+  return r;
+}
+
+// Two floats as e4m3 codes, lo in the low byte: nearest even, saturated.
+SPATTEN_DEV uint32_t f32x2_to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Four codes (a 32-bit word, lowest byte first) as floats.
+template <int KV>
+SPATTEN_DEV void codes4_to_f32(uint32_t w, float (&f)[4]) {
+  if constexpr (KV == kKvInt8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(w >> (8 * i));
+  } else {
+    const uint32_t a = e4m3x2_to_f16x2(w & 0xFFFFu), b = e4m3x2_to_f16x2(w >> 16);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
+  }
+}
+
+}  // namespace spatten
