@@ -324,7 +324,7 @@ int spatten_paged_append(const spatten_paged_append_args* a, void* stream);
  * over fp32 scores and statistics; 0 for a row that sees no key. Serves one
  * token per sequence, a few drafted ones, or the next piece of a prompt.
  * q, out: [T, H, D] by strides as in spatten_paged_append; H % G == 0,
- * H / G <= 128.
+ * H / G <= 128, B <= 8192.
  */
 typedef struct {
   spatten_paged_cache cache;

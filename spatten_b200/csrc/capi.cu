@@ -616,6 +616,8 @@ static int fill_paged_attend(const spatten_paged_attend_args* a, spatten::PagedA
   if (a->H < 1 || a->H % p.c.G) return fail(SPATTEN_ERR_INVALID, "%s: H=%d %% G=%d", who, a->H, p.c.G);
   if (a->H / p.c.G > 128)
     return fail(SPATTEN_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most 128)", who, a->H / p.c.G);
+  if (a->B > spatten::paged_attend_max_batch())
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: B=%d (at most %d)", who, a->B, spatten::paged_attend_max_batch());
   if (!(a->sm_scale == a->sm_scale)) return fail(SPATTEN_ERR_INVALID, "%s: sm_scale is NaN", who);
   p.q = a->q; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.out = a->out; p.o_st = a->o_st; p.o_sh = a->o_sh;
@@ -625,7 +627,7 @@ static int fill_paged_attend(const spatten_paged_attend_args* a, spatten::PagedA
 
 size_t spatten_paged_attend_workspace_size(const spatten_paged_attend_args* a) {
   spatten::PagedAttendParams p;
-  if (fill_paged_attend(a, p) != SPATTEN_OK) return 0;
+  if (fill_paged_attend(a, p) != SPATTEN_OK || p.b.B == 0 || p.b.max_tokens == 0) return 0;
   return align256(spatten::paged_attend_workspace(p, sm_count()));
 }
 

@@ -71,6 +71,7 @@ struct PagedReadParams {
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, int kv, cudaStream_t st);
 cudaError_t launch_paged_read(const PagedReadParams& p, int dtype, int kv, cudaStream_t st);
+int paged_attend_max_batch();  // sequences of one call
 size_t paged_attend_workspace(const PagedAttendParams& p, int n_sm);
 cudaError_t launch_paged_attend(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,
                                 cudaStream_t st);
