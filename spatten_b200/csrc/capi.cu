@@ -518,6 +518,8 @@ static int fill_paged_cache(const char* who, const spatten_paged_cache& c, spatt
     return fail(SPATTEN_ERR_INVALID, "%s: empty cache num_pages=%d G=%d max_pages=%d", who, c.num_pages, c.G,
                 c.max_pages);
   if (c.G > 4096) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: %d KV heads (at most 4096)", who, c.G);
+  if ((int64_t)c.num_pages * c.G * c.page_size >= ((int64_t)1 << 32) - 1)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: a pool of 2^32 rows or more", who);
   if ((int64_t)c.max_pages * c.page_size > (int64_t)1 << 30)
     return fail(SPATTEN_ERR_UNSUPPORTED, "%s: page table of more than 2^30 slots", who);
   if (c.table_stride < c.max_pages) return fail(SPATTEN_ERR_INVALID, "%s: page table stride < max_pages", who);
@@ -622,6 +624,9 @@ static int fill_paged_attend(const spatten_paged_attend_args* a, spatten::PagedA
   p.q = a->q; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.out = a->out; p.o_st = a->o_st; p.o_sh = a->o_sh;
   p.scale_log2 = a->sm_scale * spatten::kLog2e;
+  if (!spatten::paged_attend_fits(p))
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: %d rows of %d heads over a page table of %lld slots", who, a->T, a->H,
+                (long long)p.c.max_pages * p.c.page);
   return SPATTEN_OK;
 }
 

@@ -72,6 +72,7 @@ struct PagedReadParams {
 cudaError_t launch_paged_append(const PagedAppendParams& p, int dtype, int kv, cudaStream_t st);
 cudaError_t launch_paged_read(const PagedReadParams& p, int dtype, int kv, cudaStream_t st);
 int paged_attend_max_batch();  // sequences of one call
+bool paged_attend_fits(const PagedAttendParams& p);  // units of work count in 32 bits
 size_t paged_attend_workspace(const PagedAttendParams& p, int n_sm);
 cudaError_t launch_paged_attend(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,
                                 cudaStream_t st);

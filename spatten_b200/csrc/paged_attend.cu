@@ -37,39 +37,88 @@ namespace spatten {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kTile = 32;        // keys per warp step: two 16-key blocks, each within one page
-constexpr float kSlack = 8.f;    // p and w stay below 2^8
+constexpr float kSlack = 8.f;       // p and w stay below 2^8
 constexpr float kNoScale = -200.f;  // log2 of a scale of 0: below that of any float
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 
 // sequences whose prefix sums fit the shared memory
 constexpr int kMaxBatch = 8192;
 
+// The parts of a row tile that a CTA begins and does not finish.
+struct Cut {
+  int parts;         // 0: none
+  int row0, nrows;   // first row of the tile among the sequence's, rows of the sequence
+  int begin, g;      // first packed row of the sequence, KV head
+  int pad[3];
+};
+
 struct Workspace {
-  int4* meta;   // [ctas]: parts of the row tile that starts in this CTA and is cut (0: none), b, g, row tile
+  Cut* cut;     // [ctas]
   float4* ml;   // [2 ctas][rows] (m, l, M): slot 2 c: a tile begun before CTA c; 2 c + 1: one begun in it
   float* o;     // [2 ctas][rows][D]
 };
 
-template <int KV>
-struct Codes;
+// ---------------------------------------------------------------------------
+// Codes as operands. Words are 4 consecutive dims of a key.
+// ---------------------------------------------------------------------------
+template <int KV, int D, int NB>
+struct Operands;
 
-// int8: x ^ 0x80 in the low byte of 0x6400 is the f16 1152 + x; the difference
-// is exact. Bytes come out in the order (0, 2), (1, 3).
-template <>
-struct Codes<kKvInt8> {
-  static constexpr int kPair = 2;  // distance of a pair's dims
+// int8. K goes into the integer products as it is: a query row becomes two
+// int8 terms, q ~ (256 q1 + q2) max|q| / 32512 (within 2^-16 of its largest
+// element), and 256 (q1 . k) + (q2 . k) is exact in 32 bits. For V, x ^ 0x80 in
+// the low byte of 0x6400 is the f16 1152 + x, and the difference is exact.
+template <int D, int NB>
+struct Operands<kKvInt8, D, NB> {
+  static constexpr int KW = D / 16;  // K words of a lane and key
+  uint32_t q[NB][KW][2];             // [.][word][term]
+
+  // f: the lane's dims of its query row, as the words hold them; returns what
+  // a score has to be multiplied by
+  SPATTEN_DEV float set(int nb, const float (&f)[KW][4], float top) {
+    const float up = top > 0.f ? 32512.f / top : 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      uint32_t a = 0, b = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int x = __float2int_rn(fminf(fmaxf(f[w][i] * up, -32512.f), 32512.f));
+        const int hi = (x + 128) >> 8, lo = x - 256 * hi;
+        a |= ((uint32_t)hi & 0xFFu) << (8 * i);
+        b |= ((uint32_t)lo & 0xFFu) << (8 * i);
+      }
+      q[nb][w][0] = a;
+      q[nb][w][1] = b;
+    }
+    return top * (1.f / 32512.f);
+  }
+  SPATTEN_DEV void scores(const uint32_t (&k0)[KW], const uint32_t (&k1)[KW], float (&s)[NB][4]) const {
+    int hi[NB][4], lo[NB][4];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) hi[nb][i] = lo[nb][i] = 0;
+#pragma unroll
+    for (int w = 0; w < KW; w += 2) {
+      const uint32_t a[4] = {k0[w], k1[w], k0[w + 1], k1[w + 1]};
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        mma_s8_16832(hi[nb], a, q[nb][w][0], q[nb][w + 1][0]);
+        mma_s8_16832(lo[nb], a, q[nb][w][1], q[nb][w + 1][1]);
+      }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nb][i] = (float)(256 * hi[nb][i] + lo[nb][i]);
+  }
   static SPATTEN_DEV uint32_t biased(uint32_t w) {
     const uint32_t u = (w & 0x00FF00FFu) ^ 0x64806480u;
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-  // a word of one row: the f16 pairs of its two k halves
-  static SPATTEN_DEV void row(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    lo = biased(w);
-    hi = biased(w >> 8);
-  }
-  // words of two rows: the row pairs of dims 0 .. 3
-  static SPATTEN_DEV void rows(uint32_t x, uint32_t y, uint32_t (&d)[4]) {
+  // words of two keys: the key pairs of dims 0 .. 3
+  static SPATTEN_DEV void values(uint32_t x, uint32_t y, uint32_t (&d)[4]) {
     const uint32_t t = __byte_perm(x, y, 0x5410), u = __byte_perm(x, y, 0x7632);
     d[0] = biased(t);
     d[1] = biased(t >> 8);
@@ -78,17 +127,45 @@ struct Codes<kKvInt8> {
   }
 };
 
-template <>
-struct Codes<kKvE4m3> {
-  static constexpr int kPair = 1;
-  static SPATTEN_DEV void row(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    lo = e4m3x2_to_f16x2(w & 0xFFFFu);
-    hi = e4m3x2_to_f16x2(w >> 16);
+// e4m3: every code is an f16. A query row is scaled by a power of two that
+// takes its largest element to [2^14, 2^15): f16 then holds bf16's range to
+// 2^-39 of that element.
+template <int D, int NB>
+struct Operands<kKvE4m3, D, NB> {
+  static constexpr int KW = D / 16;
+  uint32_t q[NB][KW][2];
+
+  SPATTEN_DEV float set(int nb, const float (&f)[KW][4], float top) {
+    const int e = top > 0.f ? 14 - max((int)(__float_as_uint(top) >> 23) - 127, -112) : 0;  // at most 126
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      q[nb][w][0] = pack2<__half>(f[w][0] * up, f[w][1] * up);
+      q[nb][w][1] = pack2<__half>(f[w][2] * up, f[w][3] * up);
+    }
+    return __uint_as_float((uint32_t)(127 - e) << 23);
   }
-  static SPATTEN_DEV void rows(uint32_t x, uint32_t y, uint32_t (&d)[4]) {
-    const uint32_t t = __byte_perm(x, y, 0x5140), u = __byte_perm(x, y, 0x7362);
-    row(t, d[0], d[1]);
-    row(u, d[2], d[3]);
+  static SPATTEN_DEV void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+  SPATTEN_DEV void scores(const uint32_t (&k0)[KW], const uint32_t (&k1)[KW], float (&s)[NB][4]) const {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[nb][i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w) {
+      uint32_t a[4];
+      widen(k0[w], a[0], a[2]);
+      widen(k1[w], a[1], a[3]);
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) mma_16816<__half>(s[nb], a, q[nb][w][0], q[nb][w][1]);
+    }
+  }
+  static SPATTEN_DEV void values(uint32_t x, uint32_t y, uint32_t (&d)[4]) {
+    widen(__byte_perm(x, y, 0x5140), d[0], d[1]);
+    widen(__byte_perm(x, y, 0x7362), d[2], d[3]);
   }
 };
 
@@ -117,53 +194,69 @@ SPATTEN_DEV float normaliser(float m, float l, float M) {
   return l == 0.f ? 0.f : exp2f(fminf(finite_or_0(M) - finite_or_0(m), 127.f)) / l;
 }
 
-// Row tiles of a sequence and 32-key tiles that its last row sees (one at
-// least, so that rows without a key are written).
+// Row tiles of a sequence, and key tiles that its last row sees (one at least,
+// so that rows without a key are written).
 SPATTEN_DEV int row_tiles(const PagedSeq& s, int R, int rows) { return (int)(((int64_t)s.n * R + rows - 1) / rows); }
-SPATTEN_DEV int key_tiles(const PagedSeq& s) { return max(1, (min(s.old + s.n, s.len) + kTile - 1) / kTile); }
+SPATTEN_DEV int key_tiles(const PagedSeq& s, int keys) {
+  return max(1, (min(s.old + s.n, s.len) + keys - 1) / keys);
+}
 
 template <int D, int NB>
 struct Shape {
   static constexpr int kRows = 8 * NB;
+  static constexpr int kBlocks = 2;              // 16-key blocks per step, each within one page
+  static constexpr int kKeys = 16 * kBlocks;
+  static constexpr int kCtas = NB == 1 ? 3 : 2;  // resident per SM: 168 / 255 registers per thread
   static constexpr int kOPad = D + 4;
-  static constexpr int kCtas = NB == 1 ? 3 : 2;  // resident per SM: 170 / 255 registers per thread
-  static constexpr size_t smem(int B) { return (size_t)(B + 1) * 8; }
 };
 
-// K words of a lane: [block][row gid, gid + 8][D / 16]; V words: [block][keys 2t, 2t+1, 2t+8, 2t+9][D / 32]
-template <int D>
+// A lane's words: of K rows gid and gid + 8, of V rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a block.
+template <int D, int BL>
 struct Tile {
-  uint32_t k[2][2][D / 16];
-  uint32_t v[2][4][D / 32];
+  uint32_t k[BL][2][D / 16];
+  uint32_t v[BL][4][D / 32];
 };
 
 template <int D>
-SPATTEN_DEV void load_k(Tile<D>& t, int kb, const uint8_t* base, int gid, int tig) {
+SPATTEN_DEV void load_k(uint32_t (&k)[2][D / 16], const uint8_t* p) {
 #pragma unroll
   for (int r = 0; r < 2; ++r)
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
-      const uint4 x = ldg_stream16(base + (gid + 8 * r) * D + 16 * (tig + 4 * j));
-      t.k[kb][r][4 * j] = x.x; t.k[kb][r][4 * j + 1] = x.y;
-      t.k[kb][r][4 * j + 2] = x.z; t.k[kb][r][4 * j + 3] = x.w;
+      const uint4 x = ldg_stream16(p + r * 8 * D + 64 * j);
+      k[r][4 * j] = x.x; k[r][4 * j + 1] = x.y; k[r][4 * j + 2] = x.z; k[r][4 * j + 3] = x.w;
     }
 }
 
 // rows at or behind `live` of the block read as zeros (their bytes may be anything)
 template <int D>
-SPATTEN_DEV void load_v(Tile<D>& t, int kb, const uint8_t* base, int gid, int tig, int live) {
+SPATTEN_DEV void load_v(uint32_t (&v)[4][D / 32], const uint8_t* p, int tig, int live) {
+  if (live >= 16) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int row = 2 * tig + (r & 1) + 4 * (r & 2);
-    const uint8_t* p = base + row * D + gid * (D / 8);
-    if constexpr (D == 128) {
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (row < live) x = ldg_stream16(p);
-      t.v[kb][r][0] = x.x; t.v[kb][r][1] = x.y; t.v[kb][r][2] = x.z; t.v[kb][r][3] = x.w;
-    } else {
-      uint2 x = make_uint2(0u, 0u);
-      if (row < live) x = ldg_stream8(p);
-      t.v[kb][r][0] = x.x; t.v[kb][r][1] = x.y;
+    for (int r = 0; r < 4; ++r) {
+      const uint8_t* x = p + ((r & 1) + 4 * (r & 2)) * D;
+      if constexpr (D == 128) {
+        const uint4 y = ldg_stream16(x);
+        v[r][0] = y.x; v[r][1] = y.y; v[r][2] = y.z; v[r][3] = y.w;
+      } else {
+        const uint2 y = ldg_stream8(x);
+        v[r][0] = y.x; v[r][1] = y.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = (r & 1) + 4 * (r & 2);
+      const uint8_t* x = p + row * D;
+      if constexpr (D == 128) {
+        uint4 y = make_uint4(0u, 0u, 0u, 0u);
+        if (2 * tig + row < live) y = ldg_stream16(x);
+        v[r][0] = y.x; v[r][1] = y.y; v[r][2] = y.z; v[r][3] = y.w;
+      } else {
+        uint2 y = make_uint2(0u, 0u);
+        if (2 * tig + row < live) y = ldg_stream8(x);
+        v[r][0] = y.x; v[r][1] = y.y;
+      }
     }
   }
 }
@@ -172,52 +265,53 @@ template <int KV, int D, int NB>
 __global__ void __launch_bounds__(32 * kWarps, Shape<D, NB>::kCtas)
 paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf16) {
   using SH = Shape<D, NB>;
-  using C = Codes<KV>;
-  constexpr int ROWS = SH::kRows, KS = D / 16, NT = 32 * kWarps;
-  extern __shared__ __align__(16) long long pre[];  // [B + 1] units before each sequence
+  using Ops = Operands<KV, D, NB>;
+  constexpr int ROWS = SH::kRows, KS = D / 16, NT = 32 * kWarps, BL = SH::kBlocks, KEYS = SH::kKeys;
+  constexpr int AHEAD = 32 / BL;    // tiles whose pages and scales a warp holds
+  extern __shared__ uint32_t pre[];  // [B + 1] units before each sequence
   __shared__ __align__(16) float sm_o[kWarps][ROWS][SH::kOPad];
   __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS], sm_M[kWarps][ROWS];
-  __shared__ long long scan[kWarps];
+  __shared__ uint32_t scan[kWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
   const int G = p.c.G, R = p.b.H / G, page = p.c.page;
 
-  // prefix sums of the sequences' units
-  long long carry = 0;
+  // prefix sums of the sequences' units (the host made sure of 32 bits)
+  uint32_t U = 0;
   if (tid == 0) pre[0] = 0;
   for (int base = 0; base < p.b.B; base += NT) {
     const int b = base + tid;
-    long long x = 0;
+    uint32_t x = 0;
     if (b < p.b.B) {
       const PagedSeq s = paged_seq(p.b, p.c, b);
-      if (s.n > 0) x = (long long)G * row_tiles(s, R, ROWS) * key_tiles(s);
+      if (s.n > 0) x = (uint32_t)G * row_tiles(s, R, ROWS) * key_tiles(s, KEYS);
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
     if (lane == 31) scan[warp] = x;
     __syncthreads();
-    long long before = carry;
+    uint32_t before = U;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (w < warp) before += scan[w];
-      carry += scan[w];
+      U += scan[w];
     }
     if (b < p.b.B) pre[b + 1] = before + x;
     __syncthreads();
   }
-  const long long U = carry;
-  const int cta = blockIdx.x;
-  const int ctas = (int)min((long long)gridDim.x, (U + kWarps - 1) / kWarps);  // a tile per warp at least
-  int4 meta = make_int4(0, 0, 0, 0);
+  const uint32_t cta = blockIdx.x;
+  const uint32_t ctas = min(gridDim.x, (U + kWarps - 1) / kWarps);  // a tile per warp at least
+  Cut cut = {};
   if (cta >= ctas) {
-    if (tid == 0) ws.meta[cta] = meta;
+    if (tid == 0) ws.cut[cta] = cut;
     return;
   }
-  long long u = U * cta / ctas;
-  const long long u1 = U * (cta + 1) / ctas;
+  const uint32_t per = U / ctas, more = U % ctas;  // the first `more` CTAs take one unit more
+  uint32_t u = cta * per + min(cta, more);
+  const uint32_t u1 = u + per + (cta < more ? 1 : 0);
   int b = 0;
   for (int hi = p.b.B; hi - b > 1;) {  // the sequence of unit u
     const int mid = (b + hi) >> 1;
@@ -227,19 +321,55 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   while (u < u1) {
     while (pre[b + 1] <= u) ++b;
     const PagedSeq sq = paged_seq(p.b, p.c, b);
-    const int KT = key_tiles(sq), RT = row_tiles(sq, R, ROWS);
-    const long long local = u - pre[b];
-    const int g = (int)(local / ((long long)RT * KT));
-    const int rem = (int)(local - (long long)g * RT * KT), rt = rem / KT, t0 = rem % KT;
-    const int t1 = (int)min((long long)KT, t0 + (u1 - u));
+    const uint32_t KT = key_tiles(sq, KEYS), RT = row_tiles(sq, R, ROWS);
+    const uint32_t local = u - pre[b], line = local / KT, t0 = local % KT;
+    const int g = line / RT, rt = line % RT;
+    const uint32_t t1 = min(KT, t0 + (u1 - u));
     const int nrows = sq.n * R, r0 = rt * ROWS;
     // slots that the tile's last and first row see
     const int lim_max = min(sq.old + min((r0 + ROWS - 1) / R, sq.n - 1) + 1, sq.len);
     const int lim_min = min(sq.old + r0 / R + 1, sq.len);
-    const int t_end = min(t1, (max(lim_max, 0) + kTile - 1) / kTile);
+    const uint32_t t_end = min(t1, (uint32_t)(max(lim_max, 0) + KEYS - 1) / KEYS);
+
+    // this warp's tiles t0 + warp, + 4, ..: lane i keeps the row offset and the
+    // scales of block i % BL of tile i / BL of the AHEAD tiles at hand, and
+    // those of the AHEAD tiles after them
+    const int nt = t_end > t0 + warp ? (t_end - t0 - warp + kWarps - 1) / kWarps : 0;
+    auto tile_slot = [&](int j) { return (int)(t0 + warp + kWarps * j) * KEYS; };
+    auto page_of = [&](int j) {
+      const int slot = tile_slot(j + lane / BL) + 16 * (lane % BL);
+      return slot < lim_max ? paged_page(p.c, b, slot / page) : -1;
+    };
+    auto row_of = [&](int j, int pid) {
+      const int slot = tile_slot(j + lane / BL) + 16 * (lane % BL);
+      return pid >= 0 ? ((uint32_t)pid * G + g) * page + (slot & (page - 1)) : kNoRow;
+    };
+    const uint8_t* kp = p.c.k + gid * D + 16 * tig;
+    const uint8_t* vp = p.c.v + 2 * tig * D + gid * (D / 8);
+    uint32_t row_l = kNoRow, row_n[BL];
+    int pid_n = -1;
+    float ks_l = 0.f, vs_l = 0.f;
+    Tile<D, BL> tile;
+    if (nt > 0) {
+      const int pid = page_of(0);
+      row_l = row_of(0, pid);
+      const int64_t blk = (int64_t)max(pid, 0) * G + g;
+      if (pid >= 0) {
+        ks_l = __ldg(p.c.k_scale + blk);
+        vs_l = __ldg(p.c.v_scale + blk);
+      }
+      if (nt > AHEAD) pid_n = page_of(AHEAD);
+    }
+#pragma unroll
+    for (int kb = 0; kb < BL; ++kb) {
+      row_n[kb] = __shfl_sync(0xffffffffu, row_l, kb);
+      if (row_n[kb] != kNoRow) load_k<D>(tile.k[kb], kp + (uint64_t)row_n[kb] * D);
+      const int live = row_n[kb] != kNoRow ? lim_max - (tile_slot(0) + 16 * kb) : 0;
+      load_v<D>(tile.v[kb], vp + (uint64_t)(live > 0 ? row_n[kb] : 0) * D, tig, live);
+    }
 
     // queries: row gid of each 8-row block, all dims of it in the four lanes of gid
-    uint32_t qf[NB][KS][2];
+    Ops ops;
     float cq[NB][2], m[NB][2], M[NB][2], l[NB][2];
     int lim[NB][2];
     float o[NB][KS][4];
@@ -248,44 +378,30 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       const int r = r0 + nb * 8 + gid;
       const bool live = r < nrows;
       const int64_t at = live ? (int64_t)(sq.begin + r / R) * p.q_st + (int64_t)(g * R + r % R) * p.q_sh : 0;
-      const uint16_t* qp = static_cast<const uint16_t*>(p.q) + at;
+      const uint16_t* qp = static_cast<const uint16_t*>(p.q) + at + 16 * tig;
       uint2 raw[KS];
-      float top = 0.f;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        raw[s] = live ? __ldg(reinterpret_cast<const uint2*>(qp + 16 * (tig + 4 * (s / 4)) + 4 * (s % 4)))
-                      : make_uint2(0u, 0u);
-        const uint32_t w[2] = {raw[s].x, raw[s].y};
+      for (int s = 0; s < KS; ++s)
+        raw[s] = live ? __ldg(reinterpret_cast<const uint2*>(qp + 64 * (s / 4) + 4 * (s % 4))) : make_uint2(0u, 0u);
+      float f[KS][4], top = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float2 f;
-          if (bf16) f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
-          else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          const uint32_t w = j ? raw[s].y : raw[s].x;
+          float2 x;
+          if (bf16) x = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+          else x = __half22float2(*reinterpret_cast<const __half2*>(&w));
+          f[s][2 * j] = x.x;
+          f[s][2 * j + 1] = x.y;
+          top = fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y)));
+          // fmaxf drops a NaN: it makes the row's factor NaN instead
+          if (!(x.x == x.x && x.y == x.y)) top = INFINITY;
         }
-      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^e: top in [2^14, 2^15), e at most 126
-      const int e = top > 0.f ? 14 - max((int)(__float_as_uint(top) >> 23) - 127, -112) : 0;
-      const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const uint32_t w[2] = {raw[s].x, raw[s].y};
-        float f[4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float2 x;
-          if (bf16) x = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
-          else x = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-          f[2 * j] = x.x * up;
-          f[2 * j + 1] = x.y * up;
-        }
-        // the pairs that Codes::row makes of a word
-        qf[nb][s][0] = pack2<__half>(f[0], f[C::kPair]);
-        qf[nb][s][1] = pack2<__half>(f[3 - C::kPair], f[3]);
-      }
-      const float c = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
+      // a row that is not finite has no scores: NaN
+      const float c = ops.set(nb, f, top) * (top <= 3.4e38f ? p.scale_log2 : NAN);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {  // this lane's rows of the products: 2 tig, 2 tig + 1
         cq[nb][j] = __shfl_sync(0xffffffffu, c, (2 * tig + j) * 4);
@@ -299,104 +415,69 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         for (int j = 0; j < 4; ++j) o[nb][s][j] = 0.f;
     }
 
-    // this warp's tiles t0 + warp, + 4, ..: lane i keeps the page and scales of
-    // the 16-key block i & 1 of tile i >> 1 of the 16 tiles at hand, and the
-    // page-table entry of the 16 tiles after them
-    const int nt = t_end > t0 + warp ? (t_end - t0 - warp + kWarps - 1) / kWarps : 0;
-    auto block_slot = [&](int j) { return (t0 + warp + kWarps * j) * kTile; };
-    auto entry = [&](int j) {
-      const int slot = block_slot(j + (lane >> 1)) + 16 * (lane & 1);
-      return slot < lim_max ? paged_page(p.c, b, slot / page) : -1;
-    };
-    int pid_l = -1, pid_n = -1;
-    float ks_l = 0.f, vs_l = 0.f;
-    auto scales = [&]() {
-      const int64_t blk = (int64_t)max(pid_l, 0) * G + g;
-      ks_l = pid_l >= 0 ? __ldg(p.c.k_scale + blk) : 0.f;
-      vs_l = pid_l >= 0 ? __ldg(p.c.v_scale + blk) : 0.f;
-    };
-    Tile<D> tile;
-    int pid[2] = {-1, -1};  // of the tile in registers (its V part may still be the one before)
-    auto at = [&](const uint8_t* x, int which, int slot) {
-      return x + (((int64_t)max(which, 0) * G + g) * page + (slot & (page - 1))) * D;
-    };
-    if (nt > 0) {
-      pid_l = entry(0);
-      pid_n = entry(16);
-      scales();
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        pid[kb] = __shfl_sync(0xffffffffu, pid_l, kb);
-        const int slot = block_slot(0) + 16 * kb;
-        if (pid[kb] >= 0) load_k<D>(tile, kb, at(p.c.k, pid[kb], slot), gid, tig);
-        load_v<D>(tile, kb, at(p.c.v, pid[kb], slot), gid, tig, pid[kb] >= 0 ? lim_max - slot : 0);
-      }
-    }
     for (int j = 0; j < nt; ++j) {
-      const int slot0 = block_slot(j);
-      if ((j & 15) == 0) vs_l = vs_l > 0.f ? fmaxf(log2f(vs_l), kNoScale) : kNoScale;  // from here on: its log2
-      float ks[2], lv[2];
-      const int now[2] = {pid[0], pid[1]};
+      const int slot0 = tile_slot(j), at = j % AHEAD;
+      if (at == 0) vs_l = vs_l > 0.f ? fmaxf(log2f(vs_l), kNoScale) : kNoScale;  // from here on: its log2
+      float ks[BL], lv[BL];
+      bool none = false;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        ks[kb] = __shfl_sync(0xffffffffu, ks_l, 2 * (j & 15) + kb);
-        lv[kb] = __shfl_sync(0xffffffffu, vs_l, 2 * (j & 15) + kb);
+      for (int kb = 0; kb < BL; ++kb) {
+        ks[kb] = __shfl_sync(0xffffffffu, ks_l, BL * at + kb);
+        lv[kb] = __shfl_sync(0xffffffffu, vs_l, BL * at + kb);
+        none |= row_n[kb] == kNoRow;
       }
-      // scores
-      float s[2][NB][4];
+      float s[BL][NB][4];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < BL; ++kb) {
+        ops.scores(tile.k[kb][0], tile.k[kb][1], s[kb]);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < NB; ++nb) {
+          const float f0 = cq[nb][0] * ks[kb], f1 = cq[nb][1] * ks[kb];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[kb][nb][i] = 0.f;
-        if (now[kb] < 0) continue;  // warp-uniform: no memory, masked below
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          uint32_t a[4];
-          C::row(tile.k[kb][0][k], a[0], a[2]);
-          C::row(tile.k[kb][1][k], a[1], a[3]);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma_16816<__half>(s[kb][nb], a, qf[nb][k][0], qf[nb][k][1]);
+          for (int i = 0; i < 4; ++i) s[kb][nb][i] *= i & 1 ? f1 : f0;
         }
+      }
+      if (slot0 + KEYS > lim_min || none) {  // warp-uniform
+#pragma unroll
+        for (int kb = 0; kb < BL; ++kb)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (row_n[kb] == kNoRow || slot0 + 16 * kb + gid + 4 * (i & 2) >= lim[nb][i & 1])
+                s[kb][nb][i] = -INFINITY;
       }
       // the next tile's keys on their way
-      int next[2] = {-1, -1};
-      const int slot1 = block_slot(j + 1);
+      const int slot1 = tile_slot(j + 1);
       if (j + 1 < nt) {
-        if (((j + 1) & 15) == 0) {
-          pid_l = pid_n;
-          pid_n = entry(j + 17);
-          scales();
+        const int at1 = (j + 1) % AHEAD;
+        if (at1 == 0) {
+          row_l = row_of(j + 1, pid_n);
+          const int64_t blk = (int64_t)max(pid_n, 0) * G + g;
+          ks_l = pid_n >= 0 ? __ldg(p.c.k_scale + blk) : 0.f;
+          vs_l = pid_n >= 0 ? __ldg(p.c.v_scale + blk) : 0.f;
+          if (nt > j + 1 + AHEAD) pid_n = page_of(j + 1 + AHEAD);
         }
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          next[kb] = __shfl_sync(0xffffffffu, pid_l, 2 * ((j + 1) & 15) + kb);
-          if (next[kb] >= 0) load_k<D>(tile, kb, at(p.c.k, next[kb], slot1 + 16 * kb), gid, tig);
+        for (int kb = 0; kb < BL; ++kb) {
+          row_n[kb] = __shfl_sync(0xffffffffu, row_l, BL * at1 + kb);
+          if (row_n[kb] != kNoRow) load_k<D>(tile.k[kb], kp + (uint64_t)row_n[kb] * D);
         }
       }
       // p = 2^(s - m), and w = 2^(s + log2 v_scale - M)
-      const bool masked = slot0 + kTile > lim_min || now[0] < 0 || now[1] < 0;
       float top[NB][2], topw[NB][2];  // largest s, and s + log2 v_scale, of this lane
       bool up = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float t[2];
+          top[nb][c] = topw[nb][c] = -INFINITY;
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            const float f = cq[nb][c] * ks[kb];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float& x = s[kb][nb][2 * i + c];
-              x *= f;
-              if (masked && (now[kb] < 0 || slot0 + 16 * kb + gid + 8 * i >= lim[nb][c])) x = -INFINITY;
-            }
-            t[kb] = fmaxf(s[kb][nb][c], s[kb][nb][2 + c]);
+          for (int kb = 0; kb < BL; ++kb) {
+            const float t = fmaxf(s[kb][nb][c], s[kb][nb][2 + c]);
+            top[nb][c] = fmaxf(top[nb][c], t);
+            topw[nb][c] = fmaxf(topw[nb][c], t + lv[kb]);
           }
-          top[nb][c] = fmaxf(t[0], t[1]);
-          topw[nb][c] = fmaxf(t[0] + lv[0], t[1] + lv[1]);
           up |= top[nb][c] > m[nb][c] + kSlack || topw[nb][c] > M[nb][c] + kSlack;
         }
       if (__any_sync(0xffffffffu, up)) {
@@ -422,34 +503,30 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
             M[nb][c] = Mn;
           }
       }
-      uint32_t pf[2][NB][2];
+      uint32_t pf[BL][NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        float mf[2], Mf[2];
+        const float m0 = finite_or_0(m[nb][0]), m1 = finite_or_0(m[nb][1]);
+        const float M0 = finite_or_0(M[nb][0]), M1 = finite_or_0(M[nb][1]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          mf[c] = finite_or_0(m[nb][c]);
-          Mf[c] = finite_or_0(M[nb][c]);
-        }
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < BL; ++kb)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float s0 = s[kb][nb][2 * i], s1 = s[kb][nb][2 * i + 1];
-            l[nb][0] += fast_exp2(s0 - mf[0]);
-            l[nb][1] += fast_exp2(s1 - mf[1]);
-            pf[kb][nb][i] = transpose8x8(
-                pack2<__half>(fast_exp2(s0 + (lv[kb] - Mf[0])), fast_exp2(s1 + (lv[kb] - Mf[1]))));
+            l[nb][0] += fast_exp2(s0 - m0);
+            l[nb][1] += fast_exp2(s1 - m1);
+            pf[kb][nb][i] =
+                transpose8x8(pack2<__half>(fast_exp2(s0 + (lv[kb] - M0)), fast_exp2(s1 + (lv[kb] - M1))));
           }
       }
       // values
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < BL; ++kb)
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
           uint32_t lo[4], hi[4];
-          C::rows(tile.v[kb][0][w], tile.v[kb][1][w], lo);
-          C::rows(tile.v[kb][2][w], tile.v[kb][3][w], hi);
+          Ops::values(tile.v[kb][0][w], tile.v[kb][1][w], lo);
+          Ops::values(tile.v[kb][2][w], tile.v[kb][3][w], hi);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
@@ -460,10 +537,9 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       // and the next tile's values
       if (j + 1 < nt) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          pid[kb] = next[kb];
-          const int slot = slot1 + 16 * kb;
-          load_v<D>(tile, kb, at(p.c.v, pid[kb], slot), gid, tig, pid[kb] >= 0 ? lim_max - slot : 0);
+        for (int kb = 0; kb < BL; ++kb) {
+          const int live = row_n[kb] != kNoRow ? lim_max - (slot1 + 16 * kb) : 0;
+          load_v<D>(tile.v[kb], vp + (uint64_t)(live > 0 ? row_n[kb] : 0) * D, tig, live);
         }
       }
     }
@@ -521,74 +597,101 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       }
     }
     if (t0 == 0 && !whole) {  // cut: the CTAs up to that of its last unit hold a part each
-      const long long end = u + KT;
-      meta = make_int4((int)((end * ctas + U - 1) / U) - cta, b, g, rt);
+      const uint32_t last = u + KT - 1, big = more * (per + 1);
+      cut.parts = (int)(last < big ? last / (per + 1) : more + (last - big) / per) - (int)cta + 1;
+      cut.row0 = r0; cut.nrows = nrows; cut.begin = sq.begin; cut.g = g;
     }
     __syncthreads();
     u += t1 - t0;
   }
-  if (tid == 0) ws.meta[cta] = meta;
+  if (tid == 0) ws.cut[cta] = cut;
 }
 
-// Joins the row tile that starts in CTA blockIdx.x and is cut: its parts are
-// slot 2 c + 1 of that CTA and slot 2 c of the following ones. A warp per row.
+// Joins the row tile that CTA blockIdx.x began and did not finish: its parts
+// are slot 2 c + 1 of that CTA and slot 2 c of the following ones. A warp per
+// row and, where the tile has fewer rows than the CTA has warps, per share of
+// the parts; D / 32 dims per lane.
 template <int D, int ROWS>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttendParams p, const Workspace ws, const bool bf16) {
+  constexpr int E = D / 32, NW = 8;
+  __shared__ float sh[NW][D + 4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int E = D / 32;
-  const int c0 = blockIdx.x, lane = threadIdx.x & 31;
-  const int4 meta = ws.meta[c0];
-  if (meta.x <= 1) return;
-  const int parts = meta.x, g = meta.z, R = p.b.H / p.c.G;
-  const PagedSeq sq = paged_seq(p.b, p.c, meta.y);
-  for (int row = threadIdx.x >> 5; row < ROWS; row += 8) {
-    const int r = meta.w * ROWS + row;
-    if (r >= sq.n * R) return;
-    auto at = [&](int i) { return ((int64_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * ROWS + row); };
-    float mm = -INFINITY, MM = -INFINITY;
-    for (int i = lane; i < parts; i += 32) {
-      const float4 x = ws.ml[at(i)];
-      mm = fmaxf(mm, x.x);
-      MM = fmaxf(MM, x.z);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-      MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, d));
-    }
-    float l = 0.f, acc[E];
+  const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Cut cut = ws.cut[c0];
+  if (cut.parts == 0) return;
+  const int R = p.b.H / p.c.G, rows = min(cut.nrows - cut.row0, ROWS);
+  int share = NW;  // warps per row
+  while (share > 1 && rows * share > NW) share >>= 1;
+  const int lines = NW / share;  // rows at a time
+  for (int base = 0; base < rows; base += lines) {
+    const int row = base + warp / share, part0 = warp % share;
+    const bool live = row < rows;
+    auto at = [&](int i) { return (int64_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * ROWS + row; };
+    float mm = -INFINITY, MM = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-      float f = 0.f;
-      if (i0 + lane < parts) {
-        const float4 x = ws.ml[at(i0 + lane)];
-        f = fast_exp2(x.z - finite_or_0(MM));
-        l += x.y * fast_exp2(x.x - finite_or_0(mm));
+    if (live) {
+      for (int i = lane; i < cut.parts; i += 32) {
+        const float4 x = ws.ml[at(i)];
+        mm = fmaxf(mm, x.x);
+        MM = fmaxf(MM, x.z);
       }
-      const int n = min(32, parts - i0);
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        const float w = __shfl_sync(0xffffffffu, f, i);
-        const float* src = ws.o + at(i0 + i) * D + lane * E;
-        if constexpr (E == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src);
-          acc[0] += x.x * w; acc[1] += x.y * w; acc[2] += x.z * w; acc[3] += x.w * w;
-        } else {
-          const float2 x = *reinterpret_cast<const float2*>(src);
-          acc[0] += x.x * w; acc[1] += x.y * w;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) {
+        mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+        MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, d));
+      }
+      for (int i0 = part0; i0 < cut.parts; i0 += 8 * share) {
+        float x[8][E];
+        float4 h[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int i = i0 + k * share;
+          if (i < cut.parts) {
+            const float* src = ws.o + at(i) * D + lane * E;
+            h[k] = ws.ml[at(i)];
+            if constexpr (E == 4) {
+              const float4 y = *reinterpret_cast<const float4*>(src);
+              x[k][0] = y.x; x[k][1] = y.y; x[k][2] = y.z; x[k][3] = y.w;
+            } else {
+              const float2 y = *reinterpret_cast<const float2*>(src);
+              x[k][0] = y.x; x[k][1] = y.y;
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (i0 + k * share >= cut.parts) break;
+          const float f = fast_exp2(h[k].z - finite_or_0(MM));
+          l += h[k].y * fast_exp2(h[k].x - finite_or_0(mm));
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += x[k][e] * f;
         }
       }
     }
+    if (share > 1) {  // the shares of a row join in its first warp
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    const float inv = normaliser(mm, l, MM);
-    uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(sq.begin + r / R) * p.o_st +
-                   (int64_t)(g * R + r % R) * p.o_sh + lane * E;
+      for (int e = 0; e < E; ++e) sh[warp][lane * E + e] = acc[e];
+      if (lane == 0) sh[warp][D] = l;
+      __syncthreads();
+      if (part0 == 0)
+        for (int w = 1; w < share; ++w) {
+          l += sh[warp + w][D];
 #pragma unroll
-    for (int e = 0; e < E; e += 2)
-      *reinterpret_cast<uint32_t*>(op + e) =
-          bf16 ? pack2<__nv_bfloat16>(acc[e] * inv, acc[e + 1] * inv) : pack2<__half>(acc[e] * inv, acc[e + 1] * inv);
+          for (int e = 0; e < E; ++e) acc[e] += sh[warp + w][lane * E + e];
+        }
+      __syncthreads();
+    }
+    if (live && part0 == 0) {
+      const int r = cut.row0 + row;
+      const float inv = normaliser(mm, l, MM);
+      uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(cut.begin + r / R) * p.o_st +
+                     (int64_t)(cut.g * R + r % R) * p.o_sh + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        *reinterpret_cast<uint32_t*>(op + e) =
+            bf16 ? pack2<__nv_bfloat16>(acc[e] * inv, acc[e + 1] * inv) : pack2<__half>(acc[e] * inv, acc[e + 1] * inv);
+    }
   }
 }
 
@@ -603,9 +706,9 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 template <int KV, int D, int NB>
 cudaError_t attend_launch(const PagedAttendParams& p, bool bf16, const Workspace& ws, int ctas, cudaStream_t st) {
   using SH = Shape<D, NB>;
-  const size_t smem = SH::smem(p.b.B);
+  const size_t smem = (size_t)(p.b.B + 1) * sizeof(uint32_t);
   cudaError_t e = cudaFuncSetAttribute(paged_attend_kernel<KV, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)SH::smem(kMaxBatch));
+                                       (kMaxBatch + 1) * (int)sizeof(uint32_t));
   if (e != cudaSuccess) return e;
   paged_attend_kernel<KV, D, NB><<<ctas, 32 * kWarps, smem, st>>>(p, ws, bf16);
   e = cudaGetLastError();
@@ -640,9 +743,15 @@ cudaError_t attend_dim(const PagedAttendParams& p, bool bf16, const Workspace& w
 
 int paged_attend_max_batch() { return kMaxBatch; }
 
+bool paged_attend_fits(const PagedAttendParams& p) {
+  const int rows = row_block(p);
+  const double lines = (double)p.b.T * (p.b.H / p.c.G) / rows + p.b.B;  // row tiles of all sequences, at most
+  return lines * p.c.G * ((double)p.c.max_pages * p.c.page / 32 + 1) < 4e9;
+}
+
 size_t paged_attend_workspace(const PagedAttendParams& p, int n_sm) {
   const size_t ctas = grid_ctas(p, n_sm), rows = row_block(p);
-  return align256(ctas * sizeof(int4)) + align256(2 * ctas * rows * sizeof(float4)) +
+  return align256(ctas * sizeof(Cut)) + align256(2 * ctas * rows * sizeof(float4)) +
          align256(2 * ctas * rows * p.c.D * sizeof(float));
 }
 
@@ -651,8 +760,8 @@ cudaError_t launch_paged_attend(const PagedAttendParams& p, int dtype, int kv, v
   const int ctas = grid_ctas(p, n_sm), rows = row_block(p);
   uint8_t* w = static_cast<uint8_t*>(ws);
   Workspace s;
-  s.meta = reinterpret_cast<int4*>(w);
-  w += align256(ctas * sizeof(int4));
+  s.cut = reinterpret_cast<Cut*>(w);
+  w += align256(ctas * sizeof(Cut));
   s.ml = reinterpret_cast<float4*>(w);
   w += align256((size_t)2 * ctas * rows * sizeof(float4));
   s.o = reinterpret_cast<float*>(w);
