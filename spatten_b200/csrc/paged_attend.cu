@@ -30,6 +30,8 @@
 // CTA take turns on its tiles and join in shared memory; a (sequence, head, row
 // tile) that a range's border cuts leaves (m, l, M, o) partials in the workspace,
 // which a second kernel joins in a fixed order.
+#include <cmath>
+
 #include "kernels.h"
 #include "paged_dev.cuh"
 
@@ -169,18 +171,6 @@ struct Operands<kKvE4m3, D, NB> {
   }
 };
 
-SPATTEN_DEV uint4 ldg_stream16(const uint8_t* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
-SPATTEN_DEV uint2 ldg_stream8(const uint8_t* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
-
 SPATTEN_DEV uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -204,60 +194,56 @@ SPATTEN_DEV int key_tiles(const PagedSeq& s, int keys) {
 template <int D, int NB>
 struct Shape {
   static constexpr int kRows = 8 * NB;
-  static constexpr int kBlocks = 2;              // 16-key blocks per step, each within one page
+  static constexpr int kBlocks = 1;              // 16-key blocks per step, each within one page
   static constexpr int kKeys = 16 * kBlocks;
-  static constexpr int kCtas = NB == 1 ? 3 : 2;  // resident per SM: 168 / 255 registers per thread
-  static constexpr int kOPad = D + 4;
+  static constexpr int kStages = 4;              // steps of a warp's ring
+  static constexpr int kCtas = 3;                // resident per SM
+  static constexpr int kBlockBytes = 16 * D;     // K or V codes of a block
+  static constexpr int kStageBytes = 2 * kBlocks * kBlockBytes;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kOPad = D + 4;            // floats of a row in the join, which reuses the ring
+  static_assert(kWarps * kRows * kOPad * 4 <= kRing, "the join fits the ring");
 };
 
-// A lane's words: of K rows gid and gid + 8, of V rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of a block.
-template <int D, int BL>
-struct Tile {
-  uint32_t k[BL][2][D / 16];
-  uint32_t v[BL][4][D / 32];
-};
-
+// 16-byte chunks of a block's rows, XOR-swizzled so that the fragment reads of
+// eight lanes (two rows of K, or two chunks of four rows of V) meet different banks.
 template <int D>
-SPATTEN_DEV void load_k(uint32_t (&k)[2][D / 16], const uint8_t* p) {
-#pragma unroll
-  for (int r = 0; r < 2; ++r)
-#pragma unroll
-    for (int j = 0; j < D / 64; ++j) {
-      const uint4 x = ldg_stream16(p + r * 8 * D + 64 * j);
-      k[r][4 * j] = x.x; k[r][4 * j + 1] = x.y; k[r][4 * j + 2] = x.z; k[r][4 * j + 3] = x.w;
-    }
+SPATTEN_DEV int swizzled(int row, int chunk) {
+  if constexpr (D == 128) return row * 128 + ((chunk ^ (row & 7)) << 4);
+  else return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
 
-// rows at or behind `live` of the block read as zeros (their bytes may be anything)
+// A block of 16 rows into the ring; rows at or behind `live` arrive as zeros
+// (their bytes may be anything).
 template <int D>
-SPATTEN_DEV void load_v(uint32_t (&v)[4][D / 32], const uint8_t* p, int tig, int live) {
-  if (live >= 16) {
+SPATTEN_DEV void load_block(uint8_t* dst, const uint8_t* src, int lane, int live) {
+  constexpr int CH = D / 16, RPI = 32 / CH;  // chunks per row, rows per warp instruction
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const uint8_t* x = p + ((r & 1) + 4 * (r & 2)) * D;
-      if constexpr (D == 128) {
-        const uint4 y = ldg_stream16(x);
-        v[r][0] = y.x; v[r][1] = y.y; v[r][2] = y.z; v[r][3] = y.w;
-      } else {
-        const uint2 y = ldg_stream8(x);
-        v[r][0] = y.x; v[r][1] = y.y;
-      }
-    }
+  for (int i = 0; i < 16 / RPI; ++i) {
+    const int row = i * RPI + lane / CH;
+    cp_async16(dst + swizzled<D>(row, lane % CH), src + i * 512 + lane * 16, row < live);
+  }
+}
+
+// Words of K row `row` for lane tig: dims (D / 4) tig .. + D / 4 - 1.
+template <int D>
+SPATTEN_DEV void read_k(uint32_t (&k)[D / 16], const uint8_t* blk, int row, int tig) {
+#pragma unroll
+  for (int j = 0; j < D / 64; ++j) {
+    const uint4 x = *reinterpret_cast<const uint4*>(blk + swizzled<D>(row, tig * (D / 64) + j));
+    k[4 * j] = x.x; k[4 * j + 1] = x.y; k[4 * j + 2] = x.z; k[4 * j + 3] = x.w;
+  }
+}
+
+// Words of V row `row` for lane gid: dims (D / 8) gid .. + D / 8 - 1.
+template <int D>
+SPATTEN_DEV void read_v(uint32_t (&v)[D / 32], const uint8_t* blk, int row, int gid) {
+  if constexpr (D == 128) {
+    const uint4 x = *reinterpret_cast<const uint4*>(blk + swizzled<D>(row, gid));
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
   } else {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = (r & 1) + 4 * (r & 2);
-      const uint8_t* x = p + row * D;
-      if constexpr (D == 128) {
-        uint4 y = make_uint4(0u, 0u, 0u, 0u);
-        if (2 * tig + row < live) y = ldg_stream16(x);
-        v[r][0] = y.x; v[r][1] = y.y; v[r][2] = y.z; v[r][3] = y.w;
-      } else {
-        uint2 y = make_uint2(0u, 0u);
-        if (2 * tig + row < live) y = ldg_stream8(x);
-        v[r][0] = y.x; v[r][1] = y.y;
-      }
-    }
+    const uint2 x = *reinterpret_cast<const uint2*>(blk + swizzled<D>(row, gid >> 1) + (gid & 1) * 8);
+    v[0] = x.x; v[1] = x.y;
   }
 }
 
@@ -268,8 +254,10 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   using Ops = Operands<KV, D, NB>;
   constexpr int ROWS = SH::kRows, KS = D / 16, NT = 32 * kWarps, BL = SH::kBlocks, KEYS = SH::kKeys;
   constexpr int AHEAD = 32 / BL;    // tiles whose pages and scales a warp holds
-  extern __shared__ uint32_t pre[];  // [B + 1] units before each sequence
-  __shared__ __align__(16) float sm_o[kWarps][ROWS][SH::kOPad];
+  constexpr int ST = SH::kStages;
+  extern __shared__ __align__(128) uint8_t dsm[];
+  float (*sm_o)[ROWS][SH::kOPad] = reinterpret_cast<float (*)[ROWS][SH::kOPad]>(dsm);  // over the rings
+  uint32_t* pre = reinterpret_cast<uint32_t*>(dsm + SH::kRing);  // [B + 1] units before each sequence
   __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS], sm_M[kWarps][ROWS];
   __shared__ uint32_t scan[kWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -332,8 +320,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     const uint32_t t_end = min(t1, (uint32_t)(max(lim_max, 0) + KEYS - 1) / KEYS);
 
     // this warp's tiles t0 + warp, + 4, ..: lane i keeps the row offset and the
-    // scales of block i % BL of tile i / BL of the AHEAD tiles at hand, and
-    // those of the AHEAD tiles after them
+    // scales of block i % BL of tile i / BL of the AHEAD tiles at hand, and the
+    // page of the AHEAD tiles after them
     const int nt = t_end > t0 + warp ? (t_end - t0 - warp + kWarps - 1) / kWarps : 0;
     auto tile_slot = [&](int j) { return (int)(t0 + warp + kWarps * j) * KEYS; };
     auto page_of = [&](int j) {
@@ -344,29 +332,37 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       const int slot = tile_slot(j + lane / BL) + 16 * (lane % BL);
       return pid >= 0 ? ((uint32_t)pid * G + g) * page + (slot & (page - 1)) : kNoRow;
     };
-    const uint8_t* kp = p.c.k + gid * D + 16 * tig;
-    const uint8_t* vp = p.c.v + 2 * tig * D + gid * (D / 8);
-    uint32_t row_l = kNoRow, row_n[BL];
+    uint8_t* ring = dsm + warp * ST * SH::kStageBytes;
+    uint32_t row_l = kNoRow, have_l = 0, have_n = 0;  // have: blocks with memory, a bit per lane
     int pid_n = -1;
-    float ks_l = 0.f, vs_l = 0.f;
-    Tile<D, BL> tile;
-    if (nt > 0) {
-      const int pid = page_of(0);
-      row_l = row_of(0, pid);
-      const int64_t blk = (int64_t)max(pid, 0) * G + g;
-      if (pid >= 0) {
-        ks_l = __ldg(p.c.k_scale + blk);
-        vs_l = __ldg(p.c.v_scale + blk);
-      }
-      if (nt > AHEAD) pid_n = page_of(AHEAD);
-    }
+    float ks_l = 0.f, vs_l = 0.f, ks_n = 0.f, vs_n = 0.f;
+    // tile j on its way into slot j % ST (an empty group past the end)
+    auto issue = [&](int j) {
+      if (j < nt) {
+        const int at = j % AHEAD;
+        if (at == 0) {
+          const int pid = j == 0 ? page_of(0) : pid_n;
+          row_l = row_of(j, pid);
+          have_n = __ballot_sync(0xffffffffu, pid >= 0);
+          const int64_t blk = (int64_t)max(pid, 0) * G + g;
+          ks_n = pid >= 0 ? __ldg(p.c.k_scale + blk) : 0.f;
+          vs_n = pid >= 0 ? __ldg(p.c.v_scale + blk) : 0.f;
+          if (nt > j + AHEAD) pid_n = page_of(j + AHEAD);
+        }
+        uint8_t* dst = ring + (j % ST) * SH::kStageBytes;
 #pragma unroll
-    for (int kb = 0; kb < BL; ++kb) {
-      row_n[kb] = __shfl_sync(0xffffffffu, row_l, kb);
-      if (row_n[kb] != kNoRow) load_k<D>(tile.k[kb], kp + (uint64_t)row_n[kb] * D);
-      const int live = row_n[kb] != kNoRow ? lim_max - (tile_slot(0) + 16 * kb) : 0;
-      load_v<D>(tile.v[kb], vp + (uint64_t)(live > 0 ? row_n[kb] : 0) * D, tig, live);
-    }
+        for (int kb = 0; kb < BL; ++kb) {
+          const uint32_t row = __shfl_sync(0xffffffffu, row_l, BL * at + kb);
+          const uint64_t off = row == kNoRow ? 0 : (uint64_t)row * D;
+          const int live = row == kNoRow ? 0 : lim_max - (tile_slot(j) + 16 * kb);
+          load_block<D>(dst + kb * SH::kBlockBytes, p.c.k + off, lane, row == kNoRow ? 0 : 16);
+          load_block<D>(dst + (BL + kb) * SH::kBlockBytes, p.c.v + off, lane, live);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int j = 0; j < ST - 1; ++j) issue(j);
 
     // queries: row gid of each 8-row block, all dims of it in the four lanes of gid
     Ops ops;
@@ -378,11 +374,14 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       const int r = r0 + nb * 8 + gid;
       const bool live = r < nrows;
       const int64_t at = live ? (int64_t)(sq.begin + r / R) * p.q_st + (int64_t)(g * R + r % R) * p.q_sh : 0;
-      const uint16_t* qp = static_cast<const uint16_t*>(p.q) + at + 16 * tig;
+      const uint16_t* qp = static_cast<const uint16_t*>(p.q) + at + (D / 4) * tig;
       uint2 raw[KS];
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-        raw[s] = live ? __ldg(reinterpret_cast<const uint2*>(qp + 64 * (s / 4) + 4 * (s % 4))) : make_uint2(0u, 0u);
+      for (int s = 0; s < KS; s += 2) {
+        const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(qp + 4 * s)) : make_uint4(0u, 0u, 0u, 0u);
+        raw[s] = make_uint2(x.x, x.y);
+        raw[s + 1] = make_uint2(x.z, x.w);
+      }
       float f[KS][4], top = 0.f;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
@@ -416,20 +415,31 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     }
 
     for (int j = 0; j < nt; ++j) {
+      cp_async_wait<ST - 2>();
+      __syncwarp();  // tile j has landed for every lane, and tile j - 1 is read
+      issue(j + ST - 1);
+      const uint8_t* stage = ring + (j % ST) * SH::kStageBytes;
       const int slot0 = tile_slot(j), at = j % AHEAD;
-      if (at == 0) vs_l = vs_l > 0.f ? fmaxf(log2f(vs_l), kNoScale) : kNoScale;  // from here on: its log2
+      if (at == 0) {
+        have_l = have_n;
+        ks_l = ks_n;
+        vs_l = vs_n > 0.f ? fmaxf(log2f(vs_n), kNoScale) : kNoScale;  // log2 of the scale
+      }
       float ks[BL], lv[BL];
       bool none = false;
 #pragma unroll
       for (int kb = 0; kb < BL; ++kb) {
         ks[kb] = __shfl_sync(0xffffffffu, ks_l, BL * at + kb);
         lv[kb] = __shfl_sync(0xffffffffu, vs_l, BL * at + kb);
-        none |= row_n[kb] == kNoRow;
+        none |= !((have_l >> (BL * at + kb)) & 1u);
       }
       float s[BL][NB][4];
 #pragma unroll
       for (int kb = 0; kb < BL; ++kb) {
-        ops.scores(tile.k[kb][0], tile.k[kb][1], s[kb]);
+        uint32_t k0[KS], k1[KS];
+        read_k<D>(k0, stage + kb * SH::kBlockBytes, gid, tig);
+        read_k<D>(k1, stage + kb * SH::kBlockBytes, gid + 8, tig);
+        ops.scores(k0, k1, s[kb]);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const float f0 = cq[nb][0] * ks[kb], f1 = cq[nb][1] * ks[kb];
@@ -444,25 +454,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
           for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (row_n[kb] == kNoRow || slot0 + 16 * kb + gid + 4 * (i & 2) >= lim[nb][i & 1])
+              if (!((have_l >> (BL * at + kb)) & 1u) || slot0 + 16 * kb + gid + 4 * (i & 2) >= lim[nb][i & 1])
                 s[kb][nb][i] = -INFINITY;
-      }
-      // the next tile's keys on their way
-      const int slot1 = tile_slot(j + 1);
-      if (j + 1 < nt) {
-        const int at1 = (j + 1) % AHEAD;
-        if (at1 == 0) {
-          row_l = row_of(j + 1, pid_n);
-          const int64_t blk = (int64_t)max(pid_n, 0) * G + g;
-          ks_l = pid_n >= 0 ? __ldg(p.c.k_scale + blk) : 0.f;
-          vs_l = pid_n >= 0 ? __ldg(p.c.v_scale + blk) : 0.f;
-          if (nt > j + 1 + AHEAD) pid_n = page_of(j + 1 + AHEAD);
-        }
-#pragma unroll
-        for (int kb = 0; kb < BL; ++kb) {
-          row_n[kb] = __shfl_sync(0xffffffffu, row_l, BL * at1 + kb);
-          if (row_n[kb] != kNoRow) load_k<D>(tile.k[kb], kp + (uint64_t)row_n[kb] * D);
-        }
       }
       // p = 2^(s - m), and w = 2^(s + log2 v_scale - M)
       float top[NB][2], topw[NB][2];  // largest s, and s + log2 v_scale, of this lane
@@ -521,12 +514,16 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       }
       // values
 #pragma unroll
-      for (int kb = 0; kb < BL; ++kb)
+      for (int kb = 0; kb < BL; ++kb) {
+        const uint8_t* blk = stage + (BL + kb) * SH::kBlockBytes;
+        uint32_t v[4][D / 32];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) read_v<D>(v[r], blk, 2 * tig + (r & 1) + 4 * (r & 2), gid);
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
           uint32_t lo[4], hi[4];
-          Ops::values(tile.v[kb][0][w], tile.v[kb][1][w], lo);
-          Ops::values(tile.v[kb][2][w], tile.v[kb][3][w], hi);
+          Ops::values(v[0][w], v[1][w], lo);
+          Ops::values(v[2][w], v[3][w], hi);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
@@ -534,15 +531,9 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
             for (int nb = 0; nb < NB; ++nb) mma_16816<__half>(o[nb][2 * w + h], a, pf[kb][nb][0], pf[kb][nb][1]);
           }
         }
-      // and the next tile's values
-      if (j + 1 < nt) {
-#pragma unroll
-        for (int kb = 0; kb < BL; ++kb) {
-          const int live = row_n[kb] != kNoRow ? lim_max - (slot1 + 16 * kb) : 0;
-          load_v<D>(tile.v[kb], vp + (uint64_t)(live > 0 ? row_n[kb] : 0) * D, tig, live);
-        }
       }
     }
+    __syncthreads();  // every ring is read
 
     // the warps join, sums by m and outputs by M
 #pragma unroll
@@ -699,16 +690,26 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttendParams
 // tile of 16 has room for half the bytes in flight), else sixteen.
 int row_block(const PagedAttendParams& p) { return (int64_t)p.b.max_tokens * (p.b.H / p.c.G) <= 8 ? 8 : 16; }
 
-int grid_ctas(const PagedAttendParams& p, int n_sm) { return n_sm * (row_block(p) == 8 ? 3 : 2); }
+double units_bound(const PagedAttendParams& p) {
+  const int rows = row_block(p);
+  const double lines = (double)p.b.T * (p.b.H / p.c.G) / rows + p.b.B;  // row tiles of all sequences, at most
+  return lines * p.c.G * ((double)p.c.max_pages * p.c.page / 16 + 1);
+}
+
+// One resident wave, and no more than could have a unit for each warp.
+int grid_ctas(const PagedAttendParams& p, int n_sm) {
+  const int wave = n_sm * 3;
+  return (int)fmin((double)wave, fmax(1.0, ceil(units_bound(p) / kWarps)));
+}
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 template <int KV, int D, int NB>
 cudaError_t attend_launch(const PagedAttendParams& p, bool bf16, const Workspace& ws, int ctas, cudaStream_t st) {
   using SH = Shape<D, NB>;
-  const size_t smem = (size_t)(p.b.B + 1) * sizeof(uint32_t);
+  const size_t smem = SH::kRing + (size_t)(p.b.B + 1) * sizeof(uint32_t);
   cudaError_t e = cudaFuncSetAttribute(paged_attend_kernel<KV, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (kMaxBatch + 1) * (int)sizeof(uint32_t));
+                                       SH::kRing + (kMaxBatch + 1) * (int)sizeof(uint32_t));
   if (e != cudaSuccess) return e;
   paged_attend_kernel<KV, D, NB><<<ctas, 32 * kWarps, smem, st>>>(p, ws, bf16);
   e = cudaGetLastError();
@@ -743,11 +744,7 @@ cudaError_t attend_dim(const PagedAttendParams& p, bool bf16, const Workspace& w
 
 int paged_attend_max_batch() { return kMaxBatch; }
 
-bool paged_attend_fits(const PagedAttendParams& p) {
-  const int rows = row_block(p);
-  const double lines = (double)p.b.T * (p.b.H / p.c.G) / rows + p.b.B;  // row tiles of all sequences, at most
-  return lines * p.c.G * ((double)p.c.max_pages * p.c.page / 32 + 1) < 4e9;
-}
+bool paged_attend_fits(const PagedAttendParams& p) { return units_bound(p) < 4e9; }
 
 size_t paged_attend_workspace(const PagedAttendParams& p, int n_sm) {
   const size_t ctas = grid_ctas(p, n_sm), rows = row_block(p);
