@@ -151,6 +151,8 @@ template <typename T, int KV, int D, int PAGE>
 __global__ void __launch_bounds__(AppendShape<D, PAGE>::NT) paged_append_kernel(const PagedAppendParams p, int nqb) {
   using S = AppendShape<D, PAGE>;
   constexpr int LPR = S::LPR, RPP = S::RPP, PASSES = S::PASSES, NW = S::NT / 32;
+  grid_dependents();
+  grid_wait();
   const int b = blockIdx.z, chunk = blockIdx.y, G = p.c.G;
   const PagedSeq sq = paged_seq(p.b, p.c, b);
   if (sq.n == 0) return;
@@ -250,8 +252,8 @@ cudaError_t append_launch(const PagedAppendParams& p, cudaStream_t st) {
     const int per = S::RPP * (mt < 16 ? 1 : 8);
     nqb = (int)((rows + per - 1) / per);
   }
-  paged_append_kernel<T, KV, D, PAGE><<<dim3(2 * p.c.G + nqb, chunks, p.b.B), S::NT, 0, st>>>(p, nqb);
-  return cudaGetLastError();
+  return launch_dependent(paged_append_kernel<T, KV, D, PAGE>, dim3(2 * p.c.G + nqb, chunks, p.b.B), S::NT, 0, st, p,
+                          nqb);
 }
 
 template <typename T, int KV, int D>
@@ -277,6 +279,8 @@ cudaError_t append_dim(const PagedAppendParams& p, cudaStream_t st) {
 // rows. Bound by HBM (1 byte in, 2 out).
 template <typename T, int KV>
 __global__ void __launch_bounds__(256) paged_read_kernel(const PagedReadParams p, int64_t total) {
+  grid_dependents();
+  grid_wait();
   const int lpr = p.c.D / 16, per_tok = p.c.G * lpr;
   const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (t >= total) return;
@@ -319,8 +323,7 @@ template <typename T, int KV>
 cudaError_t read_launch(const PagedReadParams& p, cudaStream_t st) {
   const int64_t total = (int64_t)p.N * p.c.G * (p.c.D / 16);
   const dim3 grid((unsigned)((total + 255) / 256), p.B);
-  paged_read_kernel<T, KV><<<grid, 256, 0, st>>>(p, total);
-  return cudaGetLastError();
+  return launch_dependent(paged_read_kernel<T, KV>, grid, 256, 0, st, p, total);
 }
 
 }  // namespace

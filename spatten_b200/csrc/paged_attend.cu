@@ -23,10 +23,12 @@
 //    that follows max(s + log2 v_scale). A block with a tiny scale and all the weight
 //    keeps its 11 bits beside blocks with large scales and no weight.
 //
-// Work split: the (sequence, KV head, row tile, 32-key tile) units are numbered
-// and cut into equal ranges, one per CTA, over one wave of resident CTAs, from
-// the lengths on the device: a ragged batch and one long sequence fill the GPU
-// alike, and a captured launch follows the lengths it finds. The four warps of a
+// Work split, over one wave of resident CTAs and from the lengths on the device,
+// so that a ragged batch and one long sequence fill the GPU alike and a captured
+// launch follows the lengths it finds. A line is a (sequence, KV head, row tile).
+// Few lines: each is cut into chunks of equal length, one per CTA. Many: the
+// lines' units (16-key tiles, plus kLineCost for a line's set-up) are numbered and
+// cut into equal ranges, one per CTA. The four warps of a
 // CTA take turns on its tiles and join in shared memory; a (sequence, head, row
 // tile) that a range's border cuts leaves (m, l, M, o) partials in the workspace,
 // which a second kernel joins in a fixed order.
@@ -39,6 +41,7 @@ namespace spatten {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr uint32_t kLineCost = 8;   // what a line's set-up takes, in tiles (3 us of 0.35 us tiles)
 constexpr float kSlack = 8.f;       // p and w stay below 2^8
 constexpr float kNoScale = -200.f;  // log2 of a scale of 0: below that of any float
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
@@ -259,21 +262,55 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   float (*sm_o)[ROWS][SH::kOPad] = reinterpret_cast<float (*)[ROWS][SH::kOPad]>(dsm);  // over the rings
   uint32_t* pre = reinterpret_cast<uint32_t*>(dsm + SH::kRing);  // [B + 1] units before each sequence
   __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS], sm_M[kWarps][ROWS];
-  __shared__ uint32_t scan[kWarps];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ uint32_t scan[2 * kWarps];
+  grid_dependents();
+  grid_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
-  const int G = p.c.G, R = p.b.H / G, page = p.c.page;
+  const int G = p.c.G, R = p.b.H / G, page = p.c.page, page_log = __ffs(page) - 1;
 
-  // prefix sums of the sequences' units (the host made sure of 32 bits)
-  uint32_t U = 0;
+  // tiles and lines in all (the host made sure of 32 bits)
+  uint32_t U = 0, lines = 0;
+  auto tiles_of = [&](int b, uint32_t& n) {  // key tiles of a line of sequence b, and its lines
+    n = 0;
+    if (b >= p.b.B) return 0u;
+    const PagedSeq s = paged_seq(p.b, p.c, b);
+    if (s.n > 0) n = (uint32_t)G * row_tiles(s, R, ROWS);
+    return (uint32_t)key_tiles(s, KEYS);
+  };
+  uint32_t n0, k0 = 0;  // of sequence `tid`
+  for (int base = 0; base < p.b.B; base += NT) {
+    uint32_t n;
+    const uint32_t k = tiles_of(base + tid, n);
+    if (base == 0) {
+      n0 = n;
+      k0 = k;
+    }
+    const uint32_t x = __reduce_add_sync(0xffffffffu, n * k), y = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) {
+      scan[warp] = x;
+      scan[kWarps + warp] = y;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      U += scan[w];
+      lines += scan[kWarps + w];
+    }
+    __syncthreads();
+  }
+  // chunk: tiles per unit. ceil(tiles / chunk) summed over the lines is at most
+  // U / chunk + lines, so with few lines every unit has a CTA.
+  const bool few = lines * 8 <= gridDim.x;
+  const uint32_t chunk = few ? max((U + gridDim.x - lines - 1) / (gridDim.x - lines), (uint32_t)kWarps) : 1;
+  const uint32_t lead = few ? 0 : kLineCost;
+  auto units_of = [&](uint32_t k) { return few ? (k + chunk - 1) / chunk : k + lead; };
+  // prefix sums of the sequences' units
+  U = 0;
   if (tid == 0) pre[0] = 0;
   for (int base = 0; base < p.b.B; base += NT) {
-    const int b = base + tid;
-    uint32_t x = 0;
-    if (b < p.b.B) {
-      const PagedSeq s = paged_seq(p.b, p.c, b);
-      if (s.n > 0) x = (uint32_t)G * row_tiles(s, R, ROWS) * key_tiles(s, KEYS);
-    }
+    uint32_t n = n0, k = k0;
+    if (base > 0) k = tiles_of(base + tid, n);
+    uint32_t x = n * units_of(k);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
@@ -287,11 +324,11 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       if (w < warp) before += scan[w];
       U += scan[w];
     }
-    if (b < p.b.B) pre[b + 1] = before + x;
+    if (base + tid < p.b.B) pre[base + tid + 1] = before + x;
     __syncthreads();
   }
   const uint32_t cta = blockIdx.x;
-  const uint32_t ctas = min(gridDim.x, (U + kWarps - 1) / kWarps);  // a tile per warp at least
+  const uint32_t ctas = min(gridDim.x, few ? U : (U + kWarps - 1) / kWarps);
   Cut cut = {};
   if (cta >= ctas) {
     if (tid == 0) ws.cut[cta] = cut;
@@ -309,15 +346,27 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   while (u < u1) {
     while (pre[b + 1] <= u) ++b;
     const PagedSeq sq = paged_seq(p.b, p.c, b);
-    const uint32_t KT = key_tiles(sq, KEYS), RT = row_tiles(sq, R, ROWS);
-    const uint32_t local = u - pre[b], line = local / KT, t0 = local % KT;
+    const uint32_t KT = key_tiles(sq, KEYS), KU = units_of(KT), RT = row_tiles(sq, R, ROWS);
+    const uint32_t local = u - pre[b], line = local / KU, v0 = local % KU, v1 = min(KU, v0 + (u1 - u));
     const int g = line / RT, rt = line % RT;
-    const uint32_t t1 = min(KT, t0 + (u1 - u));
+    const uint32_t t0 = few ? v0 * chunk : max(v0, lead) - lead, t1 = few ? min(KT, v1 * chunk) : max(v1, lead) - lead;
     const int nrows = sq.n * R, r0 = rt * ROWS;
     // slots that the tile's last and first row see
     const int lim_max = min(sq.old + min((r0 + ROWS - 1) / R, sq.n - 1) + 1, sq.len);
     const int lim_min = min(sq.old + r0 / R + 1, sq.len);
     const uint32_t t_end = min(t1, (uint32_t)(max(lim_max, 0) + KEYS - 1) / KEYS);
+
+    // queries: row gid of each 8-row block, all dims of it in the four lanes of gid
+    uint4 raw[NB][KS / 2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const int r = r0 + nb * 8 + gid;
+      const uint16_t* qp = static_cast<const uint16_t*>(p.q) + (D / 4) * tig;
+      if (r < nrows) qp += (int64_t)(sq.begin + r / R) * p.q_st + (int64_t)(g * R + r % R) * p.q_sh;
+#pragma unroll
+      for (int s = 0; s < KS / 2; ++s)
+        raw[nb][s] = r < nrows ? __ldg(reinterpret_cast<const uint4*>(qp) + s) : make_uint4(0u, 0u, 0u, 0u);
+    }
 
     // this warp's tiles t0 + warp, + 4, ..: lane i keeps the row offset and the
     // scales of block i % BL of tile i / BL of the AHEAD tiles at hand, and the
@@ -326,7 +375,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     auto tile_slot = [&](int j) { return (int)(t0 + warp + kWarps * j) * KEYS; };
     auto page_of = [&](int j) {
       const int slot = tile_slot(j + lane / BL) + 16 * (lane % BL);
-      return slot < lim_max ? paged_page(p.c, b, slot / page) : -1;
+      return slot < lim_max ? paged_page(p.c, b, slot >> page_log) : -1;
     };
     auto row_of = [&](int j, int pid) {
       const int slot = tile_slot(j + lane / BL) + 16 * (lane % BL);
@@ -364,30 +413,19 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
 #pragma unroll
     for (int j = 0; j < ST - 1; ++j) issue(j);
 
-    // queries: row gid of each 8-row block, all dims of it in the four lanes of gid
     Ops ops;
     float cq[NB][2], m[NB][2], M[NB][2], l[NB][2];
     int lim[NB][2];
     float o[NB][KS][4];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int r = r0 + nb * 8 + gid;
-      const bool live = r < nrows;
-      const int64_t at = live ? (int64_t)(sq.begin + r / R) * p.q_st + (int64_t)(g * R + r % R) * p.q_sh : 0;
-      const uint16_t* qp = static_cast<const uint16_t*>(p.q) + at + (D / 4) * tig;
-      uint2 raw[KS];
-#pragma unroll
-      for (int s = 0; s < KS; s += 2) {
-        const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(qp + 4 * s)) : make_uint4(0u, 0u, 0u, 0u);
-        raw[s] = make_uint2(x.x, x.y);
-        raw[s + 1] = make_uint2(x.z, x.w);
-      }
       float f[KS][4], top = 0.f;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint32_t w = j ? raw[s].y : raw[s].x;
+          const uint4 four = raw[nb][s / 2];
+          const uint32_t w = s & 1 ? (j ? four.w : four.z) : (j ? four.y : four.x);
           float2 x;
           if (bf16) x = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
           else x = __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -555,8 +593,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         }
       }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == KT;
-    const int slot = 2 * cta + (t0 == 0 ? 1 : 0);
+    const bool whole = v0 == 0 && v1 == KU;
+    const int slot = 2 * cta + (v0 == 0 ? 1 : 0);
     for (int i = tid; i < ROWS * (D / 4); i += NT) {
       const int row = i / (D / 4), d = (i % (D / 4)) * 4, r = r0 + row;
       if (r >= nrows) break;
@@ -587,102 +625,104 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         if (d == 0) ws.ml[(int64_t)slot * ROWS + row] = make_float4(mm, ll, MM, 0.f);
       }
     }
-    if (t0 == 0 && !whole) {  // cut: the CTAs up to that of its last unit hold a part each
-      const uint32_t last = u + KT - 1, big = more * (per + 1);
+    if (v0 == 0 && !whole) {  // cut: the CTAs up to that of its last unit hold a part each
+      const uint32_t last = u + KU - 1, big = more * (per + 1);
       cut.parts = (int)(last < big ? last / (per + 1) : more + (last - big) / per) - (int)cta + 1;
       cut.row0 = r0; cut.nrows = nrows; cut.begin = sq.begin; cut.g = g;
     }
     __syncthreads();
-    u += t1 - t0;
+    u += v1 - v0;
   }
   if (tid == 0) ws.cut[cta] = cut;
 }
 
-// Joins the row tile that CTA blockIdx.x began and did not finish: its parts
-// are slot 2 c + 1 of that CTA and slot 2 c of the following ones. A warp per
-// row and, where the tile has fewer rows than the CTA has warps, per share of
-// the parts; D / 32 dims per lane.
+// Joins the line that CTA blockIdx.x began and did not finish: its parts are
+// slot 2 c + 1 of that CTA and slot 2 c of the following ones. A warp per row
+// and, where the line has fewer rows than the CTA has warps, per share of the
+// parts; D / 32 dims per lane, eight parts in flight.
+constexpr int kJoinWarps = 16;
+
 template <int D, int ROWS>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttendParams p, const Workspace ws, const bool bf16) {
-  constexpr int E = D / 32, NW = 8;
-  __shared__ float sh[NW][D + 4];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const PagedAttendParams p, const Workspace ws,
+                                                                     const bool bf16) {
+  constexpr int E = D / 32, FLY = 8;
+  __shared__ float sh[kJoinWarps][D + 4];
+  grid_dependents();
+  grid_wait();
   const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Cut cut = ws.cut[c0];
   if (cut.parts == 0) return;
   const int R = p.b.H / p.c.G, rows = min(cut.nrows - cut.row0, ROWS);
-  int share = NW;  // warps per row
-  while (share > 1 && rows * share > NW) share >>= 1;
-  const int lines = NW / share;  // rows at a time
-  for (int base = 0; base < rows; base += lines) {
-    const int row = base + warp / share, part0 = warp % share;
-    const bool live = row < rows;
-    auto at = [&](int i) { return (int64_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * ROWS + row; };
-    float mm = -INFINITY, MM = -INFINITY, l = 0.f, acc[E];
+  int share = kJoinWarps;  // warps per row
+  while (share > 1 && rows * share > kJoinWarps) share >>= 1;
+  const int row = warp / share, part0 = warp % share;
+  const bool live = row < rows;
+  auto at = [&](int i) { return (int64_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * ROWS + row; };
+  float mm = -INFINITY, MM = -INFINITY, l = 0.f, acc[E], x[FLY][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    if (live) {
-      for (int i = lane; i < cut.parts; i += 32) {
-        const float4 x = ws.ml[at(i)];
-        mm = fmaxf(mm, x.x);
-        MM = fmaxf(MM, x.z);
-      }
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  auto fetch = [&](int i0) {
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) {
-        mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-        MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, d));
-      }
-      for (int i0 = part0; i0 < cut.parts; i0 += 8 * share) {
-        float x[8][E];
-        float4 h[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int i = i0 + k * share;
-          if (i < cut.parts) {
-            const float* src = ws.o + at(i) * D + lane * E;
-            h[k] = ws.ml[at(i)];
-            if constexpr (E == 4) {
-              const float4 y = *reinterpret_cast<const float4*>(src);
-              x[k][0] = y.x; x[k][1] = y.y; x[k][2] = y.z; x[k][3] = y.w;
-            } else {
-              const float2 y = *reinterpret_cast<const float2*>(src);
-              x[k][0] = y.x; x[k][1] = y.y;
-            }
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (i0 + k * share >= cut.parts) break;
-          const float f = fast_exp2(h[k].z - finite_or_0(MM));
-          l += h[k].y * fast_exp2(h[k].x - finite_or_0(mm));
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += x[k][e] * f;
-        }
+    for (int k = 0; k < FLY; ++k) {
+      const int i = i0 + k * share;
+      if (i >= cut.parts) break;
+      const float* src = ws.o + at(i) * D + lane * E;
+      if constexpr (E == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(src);
+        x[k][0] = y.x; x[k][1] = y.y; x[k][2] = y.z; x[k][3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(src);
+        x[k][0] = y.x; x[k][1] = y.y;
       }
     }
-    if (share > 1) {  // the shares of a row join in its first warp
-#pragma unroll
-      for (int e = 0; e < E; ++e) sh[warp][lane * E + e] = acc[e];
-      if (lane == 0) sh[warp][D] = l;
-      __syncthreads();
-      if (part0 == 0)
-        for (int w = 1; w < share; ++w) {
-          l += sh[warp + w][D];
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += sh[warp + w][lane * E + e];
-        }
-      __syncthreads();
+  };
+  if (live) {
+    fetch(part0);
+    for (int i = lane; i < cut.parts; i += 32) {
+      const float4 h = ws.ml[at(i)];
+      mm = fmaxf(mm, h.x);
+      MM = fmaxf(MM, h.z);
     }
-    if (live && part0 == 0) {
-      const int r = cut.row0 + row;
-      const float inv = normaliser(mm, l, MM);
-      uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(cut.begin + r / R) * p.o_st +
-                     (int64_t)(cut.g * R + r % R) * p.o_sh + lane * E;
 #pragma unroll
-      for (int e = 0; e < E; e += 2)
-        *reinterpret_cast<uint32_t*>(op + e) =
-            bf16 ? pack2<__nv_bfloat16>(acc[e] * inv, acc[e + 1] * inv) : pack2<__half>(acc[e] * inv, acc[e + 1] * inv);
+    for (int d = 16; d > 0; d >>= 1) {
+      mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+      MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, d));
     }
+    for (int i0 = part0; i0 < cut.parts; i0 += FLY * share) {
+      if (i0 != part0) fetch(i0);
+#pragma unroll
+      for (int k = 0; k < FLY; ++k) {
+        const int i = i0 + k * share;
+        if (i >= cut.parts) break;
+        const float4 h = ws.ml[at(i)];
+        const float f = fast_exp2(h.z - finite_or_0(MM));
+        l += h.y * fast_exp2(h.x - finite_or_0(mm));
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += x[k][e] * f;
+      }
+    }
+  }
+  if (share > 1) {  // the shares of a row join in its first warp
+#pragma unroll
+    for (int e = 0; e < E; ++e) sh[warp][lane * E + e] = acc[e];
+    if (lane == 0) sh[warp][D] = l;
+    __syncthreads();
+    if (part0 == 0)
+      for (int w = 1; w < share; ++w) {
+        l += sh[warp + w][D];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += sh[warp + w][lane * E + e];
+      }
+  }
+  if (live && part0 == 0) {
+    const int r = cut.row0 + row;
+    const float inv = normaliser(mm, l, MM);
+    uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(cut.begin + r / R) * p.o_st +
+                   (int64_t)(cut.g * R + r % R) * p.o_sh + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+      *reinterpret_cast<uint32_t*>(op + e) =
+          bf16 ? pack2<__nv_bfloat16>(acc[e] * inv, acc[e + 1] * inv) : pack2<__half>(acc[e] * inv, acc[e + 1] * inv);
   }
 }
 
@@ -693,7 +733,7 @@ int row_block(const PagedAttendParams& p) { return (int64_t)p.b.max_tokens * (p.
 double units_bound(const PagedAttendParams& p) {
   const int rows = row_block(p);
   const double lines = (double)p.b.T * (p.b.H / p.c.G) / rows + p.b.B;  // row tiles of all sequences, at most
-  return lines * p.c.G * ((double)p.c.max_pages * p.c.page / 16 + 1);
+  return lines * p.c.G * ((double)p.c.max_pages * p.c.page / 16 + 1 + kLineCost);
 }
 
 // One resident wave, and no more than could have a unit for each warp.
@@ -711,20 +751,9 @@ cudaError_t attend_launch(const PagedAttendParams& p, bool bf16, const Workspace
   cudaError_t e = cudaFuncSetAttribute(paged_attend_kernel<KV, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        SH::kRing + (kMaxBatch + 1) * (int)sizeof(uint32_t));
   if (e != cudaSuccess) return e;
-  paged_attend_kernel<KV, D, NB><<<ctas, 32 * kWarps, smem, st>>>(p, ws, bf16);
-  e = cudaGetLastError();
+  e = launch_dependent(paged_attend_kernel<KV, D, NB>, dim3(ctas), 32 * kWarps, smem, st, p, ws, bf16);
   if (e != cudaSuccess) return e;
-  // scheduled while the first kernel drains; it waits for its results itself
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, SH::kRows>, p, ws, bf16);
+  return launch_dependent(paged_join_kernel<D, SH::kRows>, dim3(ctas), 32 * kJoinWarps, 0, st, p, ws, bf16);
 }
 
 template <int KV, int D>

@@ -7,6 +7,30 @@
 
 namespace spatten {
 
+// Kernels over the cache follow one another many times a token, so each is
+// launched as a dependent of the one before it in the stream (launch_dependent):
+// its CTAs may start while the other's last ones run, and wait in grid_wait(),
+// before any access to memory, until that grid is complete and its results are
+// visible. grid_dependents() lets the next such launch start.
+SPATTEN_DEV void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+SPATTEN_DEV void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st,
+                             Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // The packed rows [begin, begin + n) of sequence b, and the slot of the first:
 // every value that comes from the device is brought into range here.
 struct PagedSeq {
