@@ -4,18 +4,18 @@
 //   int8:  S = max|x| / 127                     (IEEE division)
 //   e4m3:  S = 2^ceil(log2(max|x| / 448))       (dividing by it is exact)
 // A block's scale only grows: S' = max(S, that of the largest new magnitude);
-// where it grew, the earlier codes become round(code * S / S'). Every step is
-// a correctly rounded fp32 operation on its own (no contraction), and the
-// sum of squares of the norm is taken in 64 bits, so that every order of it
-// rounds to the same value: the codes do not depend on how lanes are arranged.
+// where it grew, the earlier codes become round(code * S / S'). Rotation and
+// quantisation are correctly rounded fp32 operations one by one (no
+// contraction); only the norm's sum of squares has an order of its own.
 //
 // One CTA per written block of K or V: the block's new rows stay in
-// registers (8 dims per thread and row) between the maximum and the
-// quantisation, so each input is read once and each code written once; the
-// earlier codes are only touched where the scale grew. The query rows'
-// norm and rotation ride in further CTAs of the same launch. A decode step is
-// bound by the chain of dependent loads (lengths, page table, scale), a prompt
-// by HBM.
+// registers between the maximum and the quantisation, so each input is read
+// once and each code written once; the earlier codes are only touched where the
+// scale grew. A thread holds 4 dims of a row's first half and the 4 that rotate
+// with them, so a rotation needs no exchange. The query rows' norm and rotation
+// ride in further CTAs of the same launch. A decode step is bound by the chain
+// of dependent loads (lengths, page table, scale), a prompt by HBM and the
+// instructions per element.
 #include "kernels.h"
 #include "paged_dev.cuh"
 
@@ -24,9 +24,11 @@ namespace {
 
 constexpr float kMaxFinite = 3.402823466e38f;
 
-SPATTEN_DEV float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a <= kMaxFinite ? a : 0.f;  // infinities and NaN do not enter a scale
+// The larger magnitude, NaN when either is.
+SPATTEN_DEV float max_abs_nan(float a, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(x)));
+  return r;
 }
 
 // The scale that a block whose largest finite magnitude is `amax` needs.
@@ -44,24 +46,21 @@ SPATTEN_DEV float scale_for(float amax) {
   }
 }
 
-// Eight values over the block's scale, as codes.
+// Eight finite values over the block's scale (not 0), as codes; rc = 1 / s.
 template <int KV>
-SPATTEN_DEV uint2 encode8(const float (&x)[8], float s) {
-  uint32_t w[2] = {0u, 0u};
-  if (s == 0.f) return make_uint2(0u, 0u);
-  if constexpr (KV == kKvInt8) {
-    const float rc = rcp_approx(s);
+SPATTEN_DEV uint2 encode8(const float (&x)[8], float s, float rc) {
+  uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int c = min(max(quant_div(x[i], s, rc), -127), 127);  // NaN converts to 0
-      w[i >> 2] |= ((uint32_t)c & 0xFFu) << (8 * (i & 3));
-    }
-  } else {
-    const float inv = 1.0f / s;  // a power of two
+  for (int j = 0; j < 2; ++j) {
+    if constexpr (KV == kKvInt8) {
+      int c[4];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float a = x[i] == x[i] ? x[i] * inv : 0.f, b = x[i + 1] == x[i + 1] ? x[i + 1] * inv : 0.f;
-      w[i >> 2] |= f32x2_to_e4m3x2(a, b) << (8 * (i & 3));
+      for (int i = 0; i < 4; ++i) c[i] = quant_div_fadd(x[4 * j + i], s, rc);
+      const uint32_t lo = __byte_perm(c[0], c[1], 0x0040), hi = __byte_perm(c[2], c[3], 0x0040);
+      w[j] = __byte_perm(lo, hi, 0x5410);
+    } else {
+      w[j] = f32x2_to_e4m3x2(x[4 * j] * rc, x[4 * j + 1] * rc) |
+             (f32x2_to_e4m3x2(x[4 * j + 2] * rc, x[4 * j + 3] * rc) << 16);
     }
   }
   return make_uint2(w[0], w[1]);
@@ -87,51 +86,50 @@ SPATTEN_DEV uint2 rescale8(uint2 c, float ratio) {
 }
 
 template <typename T>
-SPATTEN_DEV void load8(const T* p, float (&f)[8]) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+SPATTEN_DEV void unpack4(uint2 u, float* f) {
   const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(e[i]);
+  for (int i = 0; i < 4; ++i) f[i] = to_f32<T>(e[i]);
 }
 
-// Norm and rotation of one row spread over D / 8 lanes (lane li holds dims
-// 8 li ..), all lanes of the warp taking part.
+// A lane's dims of a row: 4 li .. of its first half (f[0 .. 3]) and of its second.
 template <typename T, int D>
-SPATTEN_DEV void norm_rotate(float (&x)[8], int li, const PagedAppendParams& p, const void* w, int pos) {
-  constexpr int LPR = D / 8;
-  if (w) {
-    double ss = 0.0;
+SPATTEN_DEV void load_halves(const T* row, int li, float (&f)[8]) {
+  unpack4<T>(*(reinterpret_cast<const uint2*>(row + 4 * li)), f);
+  unpack4<T>(*(reinterpret_cast<const uint2*>(row + D / 2 + 4 * li)), f + 4);
+}
+
+// Norm and rotation of one row spread over D / 8 lanes, all lanes of the warp
+// taking part; g: the lane's norm weights.
+template <typename T, int D>
+SPATTEN_DEV void norm_rotate(float (&x)[8], int li, const PagedAppendParams& p, const float* g, int pos) {
+  if (g) {
+    float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fma((double)x[i], (double)x[i], ss);
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float inv = rsqrtf(__fadd_rn((float)(ss * (1.0 / D)), p.eps));
-    float g[8];
-    load8<T>(static_cast<const T*>(w) + li * 8, g);
+    for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rsqrtf(__fadd_rn(ss * (1.0f / D), p.eps));
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], inv), g[i]);
   }
   if (p.cos) {
-    const bool first = li < LPR / 2;
-    const int64_t at = (int64_t)min(max(pos, 0), p.cs_rows - 1) * p.cs_st + (li % (LPR / 2)) * 8;
-    float c[8], s[8];
+    const int64_t at = (int64_t)min(max(pos, 0), p.cs_rows - 1) * p.cs_st + 4 * li;
+    float c[4], s[4];
     if (p.cs_f32) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.cos) + at) + j);
-        const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.sin) + at) + j);
-        c[4 * j] = a.x; c[4 * j + 1] = a.y; c[4 * j + 2] = a.z; c[4 * j + 3] = a.w;
-        s[4 * j] = b.x; s[4 * j + 1] = b.y; s[4 * j + 2] = b.z; s[4 * j + 3] = b.w;
-      }
+      const float4 a = *(reinterpret_cast<const float4*>(static_cast<const float*>(p.cos) + at));
+      const float4 b = *(reinterpret_cast<const float4*>(static_cast<const float*>(p.sin) + at));
+      c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w;
+      s[0] = b.x; s[1] = b.y; s[2] = b.z; s[3] = b.w;
     } else {
-      load8<T>(static_cast<const T*>(p.cos) + at, c);
-      load8<T>(static_cast<const T*>(p.sin) + at, s);
+      unpack4<T>(*(reinterpret_cast<const uint2*>(static_cast<const T*>(p.cos) + at)), c);
+      unpack4<T>(*(reinterpret_cast<const uint2*>(static_cast<const T*>(p.sin) + at)), s);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = __shfl_xor_sync(0xffffffffu, x[i], LPR / 2);  // the other half's value
-      const float a = __fmul_rn(x[i], c[i]), b = __fmul_rn(y, s[i]);
-      x[i] = first ? __fsub_rn(a, b) : __fadd_rn(a, b);
+    for (int i = 0; i < 4; ++i) {
+      const float a = x[i], b = x[4 + i];
+      x[i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
+      x[4 + i] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
     }
   }
 }
@@ -139,18 +137,20 @@ SPATTEN_DEV void norm_rotate(float (&x)[8], int li, const PagedAppendParams& p, 
 template <int D, int PAGE>
 struct AppendShape {
   static constexpr int LPR = D / 8;                               // lanes per row
-  static constexpr int NT = PAGE * D >= 8192 ? 256 : 128;         // threads
+  static constexpr int NT = PAGE * D >= 16384 ? 512 : PAGE * D >= 8192 ? 256 : 128;  // threads
   static constexpr int RPP = NT / LPR;                            // rows per pass
-  static constexpr int PASSES = PAGE / RPP;                       // at most 8: 64 values per thread
-  static_assert(PASSES >= 1 && PASSES <= 8 && PAGE % RPP == 0, "a block's rows fit the registers");
+  static constexpr int PASSES = PAGE / RPP;                       // at most 4: 32 values per thread
+  static constexpr int QROWS = 2;                                 // query rows of a thread in flight
+  static_assert(PASSES >= 1 && PASSES <= 4 && PAGE % RPP == 0, "a block's rows fit the registers");
 };
 
 // Grid (2 G + query CTAs, written blocks per sequence, B): unit x < G is K
 // head x, x < 2 G V head x - G, the others share the chunk's query rows.
 template <typename T, int KV, int D, int PAGE>
-__global__ void __launch_bounds__(AppendShape<D, PAGE>::NT) paged_append_kernel(const PagedAppendParams p, int nqb) {
+__global__ void __launch_bounds__(AppendShape<D, PAGE>::NT, 1024 / AppendShape<D, PAGE>::NT)
+paged_append_kernel(const PagedAppendParams p, int nqb) {
   using S = AppendShape<D, PAGE>;
-  constexpr int LPR = S::LPR, RPP = S::RPP, PASSES = S::PASSES, NW = S::NT / 32;
+  constexpr int LPR = S::LPR, RPP = S::RPP, PASSES = S::PASSES, NW = S::NT / 32, QR = S::QROWS;
   grid_dependents();
   grid_wait();
   const int b = blockIdx.z, chunk = blockIdx.y, G = p.c.G;
@@ -159,21 +159,29 @@ __global__ void __launch_bounds__(AppendShape<D, PAGE>::NT) paged_append_kernel(
   const int tid = threadIdx.x, lane = tid & 31, li = lane % LPR, rt = tid / LPR;
 
   if ((int)blockIdx.x >= 2 * G) {  // query rows of tokens [chunk * PAGE, ..): token-major, heads inside
-    const int t0 = chunk * PAGE, rows = min(PAGE, sq.n - t0) * p.b.H;
-    for (int r0 = ((int)blockIdx.x - 2 * G) * RPP; r0 < rows; r0 += nqb * RPP) {
-      const int r = r0 + rt;
-      const bool live = r < rows;
-      const int i = t0 + (live ? r : 0) / p.b.H, h = (live ? r : 0) % p.b.H;
-      const int64_t row = sq.begin + i;
-      float x[8];
-      load8<T>(static_cast<const T*>(p.q) + row * p.q_st + h * p.q_sh + li * 8, x);
-      const int pos = p.positions ? __ldg(p.positions + row) : sq.old + i;
-      norm_rotate<T, D>(x, li, p, p.wq, pos);
-      if (live) {
-        uint4 o;
-        o.x = pack2<T>(x[0], x[1]); o.y = pack2<T>(x[2], x[3]);
-        o.z = pack2<T>(x[4], x[5]); o.w = pack2<T>(x[6], x[7]);
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + row * p.qo_st + h * p.qo_sh + li * 8) = o;
+    const int t0 = chunk * PAGE, H = p.b.H, rows = min(PAGE, sq.n - t0) * H;
+    float w[8];
+    if (p.wq) load_halves<T, D>(static_cast<const T*>(p.wq), li, w);
+    for (int r0 = ((int)blockIdx.x - 2 * G) * RPP; r0 < rows; r0 += nqb * RPP * QR) {
+      float x[QR][8];
+      int tok[QR], h[QR];
+#pragma unroll
+      for (int j = 0; j < QR; ++j) {
+        const int r = min(r0 + j * nqb * RPP + rt, rows - 1);
+        tok[j] = t0 + r / H;
+        h[j] = r % H;
+        load_halves<T, D>(static_cast<const T*>(p.q) + (sq.begin + tok[j]) * p.q_st + h[j] * p.q_sh, li, x[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < QR; ++j) {
+        if (r0 + j * nqb * RPP >= rows) break;  // uniform
+        const int64_t row = sq.begin + tok[j];
+        norm_rotate<T, D>(x[j], li, p, p.wq ? w : nullptr, p.positions ? *(p.positions + row) : sq.old + tok[j]);
+        if (r0 + j * nqb * RPP + rt < rows) {
+          T* o = static_cast<T*>(p.q_out) + row * p.qo_st + h[j] * p.qo_sh + 4 * li;
+          *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(x[j][0], x[j][1]), pack2<T>(x[j][2], x[j][3]));
+          *reinterpret_cast<uint2*>(o + D / 2) = make_uint2(pack2<T>(x[j][4], x[j][5]), pack2<T>(x[j][6], x[j][7]));
+        }
       }
     }
     return;
@@ -190,52 +198,87 @@ __global__ void __launch_bounds__(AppendShape<D, PAGE>::NT) paged_append_kernel(
   if (pid < 0) return;
   const int64_t blk = (int64_t)pid * G + g;
   float* sp = (isk ? p.c.k_scale : p.c.v_scale) + blk;
-  uint8_t* codes = (isk ? p.c.k : p.c.v) + blk * (PAGE * D) + li * 8;
+  uint8_t* codes = (isk ? p.c.k : p.c.v) + blk * (PAGE * D);
   const float s_old = lo > 0 ? *sp : 0.f;
-  const T* src = static_cast<const T*>(isk ? p.k : p.v) + g * (isk ? p.k_sh : p.v_sh) + li * 8;
   const int64_t st = isk ? p.k_st : p.v_st;
+  const int64_t row0 = sq.begin + first - sq.old;  // packed row of the block's row 0
+  const T* src = static_cast<const T*>(isk ? p.k : p.v) + row0 * st + g * (isk ? p.k_sh : p.v_sh);
 
-  float x[PASSES][8];
-  float amax = 0.f;
+  float x[PASSES][8];  // rows that are not new: zeros
 #pragma unroll
   for (int j = 0; j < PASSES; ++j) {
     const int r = j * RPP + rt;
-    const bool live = r >= lo && r < hi;
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-    if (live) load8<T>(src + (int64_t)(sq.begin + first + r - sq.old) * st, x[j]);
+    if (r >= lo && r < hi) load_halves<T, D>(src + r * st, li, x[j]);
   }
+  float amax = 0.f;
+  if (isk && (p.wk || p.cos)) {
+    float w[8];
+    if (p.wk) load_halves<T, D>(static_cast<const T*>(p.wk), li, w);
 #pragma unroll
-  for (int j = 0; j < PASSES; ++j) {
-    const int r = j * RPP + rt;
-    const bool live = r >= lo && r < hi;
-    if (!__any_sync(0xffffffffu, live)) continue;
-    if (isk) {
-      const int64_t row = sq.begin + first + r - sq.old;
-      const int pos = p.positions ? (live ? __ldg(p.positions + row) : 0) : first + r;
-      norm_rotate<T, D>(x[j], li, p, p.wk, pos);
+    for (int j = 0; j < PASSES; ++j) {
+      const int r = j * RPP + rt;
+      const bool live = r >= lo && r < hi;
+      if (__any_sync(0xffffffffu, live))
+        norm_rotate<T, D>(x[j], li, p, p.wk ? w : nullptr,
+                          p.positions ? (live ? *(p.positions + row0 + r) : 0) : first + r);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, live ? finite_abs(x[j][i]) : 0.f);
   }
-  __shared__ float red[NW];
-  amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));  // magnitudes order as integers
-  if (lane == 0) red[tid >> 5] = amax;
-  __syncthreads();
 #pragma unroll
-  for (int w = 0; w < NW; ++w) amax = fmaxf(amax, red[w]);
+  for (int j = 0; j < PASSES; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = max_abs_nan(amax, x[j][i]);
+  __shared__ float red[NW];
+  // magnitudes order as integers, NaN above infinity above the rest
+  auto reduce = [&]() {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+    if (lane == 0) red[tid >> 5] = __uint_as_float(top);
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all = max(all, __float_as_uint(red[w]));
+    amax = __uint_as_float(all);
+  };
+  reduce();
+  bool odd = !(amax <= kMaxFinite);
+  if (odd) {  // they do not enter the scale: the largest of the rest
+    amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < PASSES; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(x[j][i]);
+        if (a <= kMaxFinite) amax = fmaxf(amax, a);
+      }
+    __syncthreads();
+    reduce();
+  }
   const float s = fmaxf(s_old, scale_for<KV>(amax));
+  if (odd) {  // a NaN is stored as 0, an infinity as the largest code of its sign
+    const float top = s * (KV == kKvInt8 ? 127.f : 448.f);
+#pragma unroll
+    for (int j = 0; j < PASSES; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(fabsf(x[j][i]) <= kMaxFinite)) x[j][i] = x[j][i] == x[j][i] ? copysignf(top, x[j][i]) : 0.f;
+  }
   if (s > s_old && lo > 0) {
     const float ratio = __fdiv_rn(s_old, s);
     for (int r = rt; r < lo; r += RPP) {
-      uint2* c = reinterpret_cast<uint2*>(codes + r * D);
+      uint2* c = reinterpret_cast<uint2*>(codes + r * D + 8 * li);
       *c = rescale8<KV>(*c, ratio);
     }
   }
+  const float rc = KV == kKvInt8 ? rcp_approx(s) : 1.0f / s;  // e4m3: a power of two
 #pragma unroll
   for (int j = 0; j < PASSES; ++j) {
     const int r = j * RPP + rt;
-    if (r >= lo && r < hi) *reinterpret_cast<uint2*>(codes + r * D) = encode8<KV>(x[j], s);
+    if (r >= lo && r < hi) {
+      const uint2 c = s > 0.f ? encode8<KV>(x[j], s, rc) : make_uint2(0u, 0u);
+      *reinterpret_cast<uint32_t*>(codes + r * D + 4 * li) = c.x;
+      *reinterpret_cast<uint32_t*>(codes + r * D + D / 2 + 4 * li) = c.y;
+    }
   }
   if (tid == 0) *sp = s;
 }
@@ -274,56 +317,78 @@ cudaError_t append_dim(const PagedAppendParams& p, cudaStream_t st) {
   return cudaErrorInvalidValue;
 }
 
-// Read back: a thread per 16 codes of one (token, head) of K and of V, heads
-// fastest, so that a warp writes consecutive 32-byte pieces and reads whole
-// rows. Bound by HBM (1 byte in, 2 out).
+// Read back. A CTA takes a run of tokens of one sequence; a thread takes 8 codes
+// of one (token, head) of K and of V at a time, heads fastest, so that a warp
+// reads whole rows and writes consecutive 16-byte pieces, and has four of them in
+// flight (index, page and codes each wait for the one before). Bound by HBM
+// (1 byte in, 2 out).
+constexpr int kReadThreads = 256, kReadFly = 4;
+
 template <typename T, int KV>
-__global__ void __launch_bounds__(256) paged_read_kernel(const PagedReadParams p, int64_t total) {
+__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const PagedReadParams p, int tokens) {
   grid_dependents();
   grid_wait();
-  const int lpr = p.c.D / 16, per_tok = p.c.G * lpr;
-  const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (t >= total) return;
-  const int b = blockIdx.y;
-  const int64_t j = t / per_tok;
-  const int u = (int)(t % per_tok), g = u / lpr, d = (u % lpr) * 16;
-  const int64_t slot = p.idx ? __ldg(p.idx + (int64_t)b * p.idx_st + j) : j;
-  int pid = -1;
-  if (slot >= 0 && slot < __ldg(p.lens + b) && slot < (int64_t)p.c.max_pages * p.c.page)
-    pid = paged_page(p.c, b, (int)(slot / p.c.page));
-  const int64_t blk = (int64_t)max(pid, 0) * p.c.G + g;
-  const int64_t src = (blk * p.c.page + (pid < 0 ? 0 : slot % p.c.page)) * p.c.D + d;
-  const int64_t dst = (((int64_t)b * p.N + j) * p.c.G + g) * p.c.D + d;
+  const int lpr = p.c.D / 8, per = p.c.G * lpr, b = blockIdx.y;
+  const int64_t j0 = (int64_t)blockIdx.x * tokens;
+  const int items = (int)min((int64_t)tokens, p.N - j0) * per;
+  const int64_t len = min((int64_t)*(p.lens + b), (int64_t)p.c.max_pages * p.c.page);
+  const int page_log = __ffs(p.c.page) - 1;
+  for (int i0 = threadIdx.x; i0 < items; i0 += kReadThreads * kReadFly) {
+    int64_t slot[kReadFly];
+    int u[kReadFly], pid[kReadFly];
 #pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    T* out = static_cast<T*>(which ? p.v_out : p.k_out);
-    if (!out) continue;
-    uint4 c = make_uint4(0u, 0u, 0u, 0u);
-    float s = 0.f;
-    if (pid >= 0) {
-      c = *reinterpret_cast<const uint4*>((which ? p.c.v : p.c.k) + src);
-      s = (which ? p.c.v_scale : p.c.k_scale)[blk];
+    for (int f = 0; f < kReadFly; ++f) {
+      const int i = min(i0 + f * kReadThreads, items - 1);
+      const int64_t j = j0 + i / per;
+      u[f] = i % per;
+      slot[f] = p.idx ? *(p.idx + (int64_t)b * p.idx_st + j) : j;
     }
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    uint32_t o[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[4];
-      codes4_to_f32<KV>(w[i], f);
-      o[2 * i] = pack2<T>(f[0] * s, f[1] * s);
-      o[2 * i + 1] = pack2<T>(f[2] * s, f[3] * s);
+    for (int f = 0; f < kReadFly; ++f)
+      pid[f] = slot[f] >= 0 && slot[f] < len ? paged_page(p.c, b, (int)(slot[f] >> page_log)) : -1;
+    uint2 c[kReadFly][2];
+    float s[kReadFly][2];
+#pragma unroll
+    for (int f = 0; f < kReadFly; ++f) {
+      const int64_t blk = (int64_t)max(pid[f], 0) * p.c.G + u[f] / lpr;
+      const int64_t src = (blk * p.c.page + (slot[f] & (p.c.page - 1))) * p.c.D + u[f] % lpr * 8;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        c[f][w] = make_uint2(0u, 0u);
+        s[f][w] = 0.f;
+        if (pid[f] >= 0 && (w ? p.v_out : p.k_out)) {
+          c[f][w] = *(reinterpret_cast<const uint2*>((w ? p.c.v : p.c.k) + src));
+          s[f][w] = *((w ? p.c.v_scale : p.c.k_scale) + blk);
+        }
+      }
     }
-    uint4* q = reinterpret_cast<uint4*>(out + dst);
-    q[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    q[1] = make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+    for (int f = 0; f < kReadFly; ++f) {
+      const int i = i0 + f * kReadThreads;
+      if (i >= items) break;
+      const int64_t dst = (((int64_t)b * p.N + j0) * per + i) * 8;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        T* out = static_cast<T*>(w ? p.v_out : p.k_out);
+        if (!out) continue;
+        float x[4], y[4];
+        codes4_to_f32<KV>(c[f][w].x, x);
+        codes4_to_f32<KV>(c[f][w].y, y);
+        const float m = s[f][w];
+        *reinterpret_cast<uint4*>(out + dst) =
+            make_uint4(pack2<T>(x[0] * m, x[1] * m), pack2<T>(x[2] * m, x[3] * m), pack2<T>(y[0] * m, y[1] * m),
+                       pack2<T>(y[2] * m, y[3] * m));
+      }
+    }
   }
 }
 
 template <typename T, int KV>
 cudaError_t read_launch(const PagedReadParams& p, cudaStream_t st) {
-  const int64_t total = (int64_t)p.N * p.c.G * (p.c.D / 16);
-  const dim3 grid((unsigned)((total + 255) / 256), p.B);
-  return launch_dependent(paged_read_kernel<T, KV>, grid, 256, 0, st, p, total);
+  const int per = p.c.G * (p.c.D / 8), run = kReadThreads * kReadFly;
+  const int tokens = per < run ? run / per : 1;
+  const dim3 grid((unsigned)((p.N + (int64_t)tokens - 1) / tokens), p.B);
+  return launch_dependent(paged_read_kernel<T, KV>, grid, kReadThreads, 0, st, p, tokens);
 }
 
 }  // namespace

@@ -32,6 +32,7 @@
 // CTA take turns on its tiles and join in shared memory; a (sequence, head, row
 // tile) that a range's border cuts leaves (m, l, M, o) partials in the workspace,
 // which a second kernel joins in a fixed order.
+#include <atomic>
 #include <cmath>
 
 #include "kernels.h"
@@ -365,7 +366,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       if (r < nrows) qp += (int64_t)(sq.begin + r / R) * p.q_st + (int64_t)(g * R + r % R) * p.q_sh;
 #pragma unroll
       for (int s = 0; s < KS / 2; ++s)
-        raw[nb][s] = r < nrows ? __ldg(reinterpret_cast<const uint4*>(qp) + s) : make_uint4(0u, 0u, 0u, 0u);
+        raw[nb][s] = r < nrows ? *(reinterpret_cast<const uint4*>(qp) + s) : make_uint4(0u, 0u, 0u, 0u);
     }
 
     // this warp's tiles t0 + warp, + 4, ..: lane i keeps the row offset and the
@@ -394,8 +395,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
           row_l = row_of(j, pid);
           have_n = __ballot_sync(0xffffffffu, pid >= 0);
           const int64_t blk = (int64_t)max(pid, 0) * G + g;
-          ks_n = pid >= 0 ? __ldg(p.c.k_scale + blk) : 0.f;
-          vs_n = pid >= 0 ? __ldg(p.c.v_scale + blk) : 0.f;
+          ks_n = pid >= 0 ? *(p.c.k_scale + blk) : 0.f;
+          vs_n = pid >= 0 ? *(p.c.v_scale + blk) : 0.f;
           if (nt > j + AHEAD) pid_n = page_of(j + AHEAD);
         }
         uint8_t* dst = ring + (j % ST) * SH::kStageBytes;
@@ -748,9 +749,16 @@ template <int KV, int D, int NB>
 cudaError_t attend_launch(const PagedAttendParams& p, bool bf16, const Workspace& ws, int ctas, cudaStream_t st) {
   using SH = Shape<D, NB>;
   const size_t smem = SH::kRing + (size_t)(p.b.B + 1) * sizeof(uint32_t);
-  cudaError_t e = cudaFuncSetAttribute(paged_attend_kernel<KV, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       SH::kRing + (kMaxBatch + 1) * (int)sizeof(uint32_t));
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
+    e = cudaFuncSetAttribute(paged_attend_kernel<KV, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             SH::kRing + (kMaxBatch + 1) * (int)sizeof(uint32_t));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   e = launch_dependent(paged_attend_kernel<KV, D, NB>, dim3(ctas), 32 * kWarps, smem, st, p, ws, bf16);
   if (e != cudaSuccess) return e;
   return launch_dependent(paged_join_kernel<D, SH::kRows>, dim3(ctas), 32 * kJoinWarps, 0, st, p, ws, bf16);

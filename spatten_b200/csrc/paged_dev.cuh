@@ -11,7 +11,9 @@ namespace spatten {
 // launched as a dependent of the one before it in the stream (launch_dependent):
 // its CTAs may start while the other's last ones run, and wait in grid_wait(),
 // before any access to memory, until that grid is complete and its results are
-// visible. grid_dependents() lets the next such launch start.
+// visible. grid_dependents() lets the next such launch start. Everything that a
+// grid before may have written is read by plain loads: a read-only (nc) load may
+// be moved ahead of the wait.
 SPATTEN_DEV void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 SPATTEN_DEV void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -42,8 +44,8 @@ struct PagedSeq {
 
 SPATTEN_DEV PagedSeq paged_seq(const PagedBatch& p, const PagedCache& c, int b) {
   PagedSeq s;
-  const int lo = min(max(__ldg(p.cu + b), 0), p.T), hi = min(max(__ldg(p.cu + b + 1), lo), p.T);
-  const int len = min(max(__ldg(p.lens + b), 0), 1 << 30);
+  const int lo = min(max(*(p.cu + b), 0), p.T), hi = min(max(*(p.cu + b + 1), lo), p.T);
+  const int len = min(max(*(p.lens + b), 0), 1 << 30);
   s.begin = lo;
   s.n = min(hi - lo, p.max_tokens);
   s.old = len - (hi - lo);
@@ -54,7 +56,7 @@ SPATTEN_DEV PagedSeq paged_seq(const PagedBatch& p, const PagedCache& c, int b) 
 // Page of slots [pi * page, ...) of sequence b, or -1 where it has no memory.
 SPATTEN_DEV int paged_page(const PagedCache& c, int b, int pi) {
   if (pi >= c.max_pages) return -1;
-  const int pid = __ldg(c.table + (int64_t)b * c.table_st + pi);
+  const int pid = *(c.table + (int64_t)b * c.table_st + pi);
   return (pid >= 0 && pid < c.P) ? pid : -1;
 }
 

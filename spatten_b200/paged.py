@@ -47,69 +47,75 @@ def new_paged_cache(num_pages, kv_heads, head_dim, page_size=64, kv_dtype=torch.
 
 
 def _index(t, name, dev, dim, dtype=torch.int32):
-    if t.device != dev:
-        raise ValueError(f"{name}: on {t.device}, the cache is on {dev}")
+    """Pointer of an index tensor; its checks."""
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, the cache is on cuda:{dev}")
     if t.dtype != dtype or t.dim() != dim:
         raise ValueError(f"{name}: {t.dtype} of {t.dim()} dimensions (need {dtype} of {dim})")
-    if t.numel() and t.stride(-1) != 1:
+    if t.stride()[-1] != 1 and t.numel() > 1:
         raise ValueError(f"{name}: last dimension must be contiguous")
     return t.data_ptr()
 
 
-def _fill_cache(a, cache, page_table, B):
+def _fill(a, cache, page_table, seq_lens):
+    """The cache and the sequences into ``a``; returns (device index, the
+    pool's shape)."""
     k, v, ks, vs = cache
-    dev = k.device
-    if dev.type != "cuda":
+    dev, dt, shape = k.get_device(), k.dtype, k.shape
+    if dev < 0:
         raise ValueError("paged cache: CUDA tensors expected (no CPU path)")
-    if k.dtype not in _KV or v.dtype != k.dtype:
-        raise TypeError(f"paged cache: codes {k.dtype} and {v.dtype} (need int8 or float8_e4m3fn)")
-    if k.dim() != 4 or v.shape != k.shape or ks.shape != k.shape[:2] or vs.shape != ks.shape or \
+    if dt not in _KV or v.dtype != dt:
+        raise TypeError(f"paged cache: codes {dt} and {v.dtype} (need int8 or float8_e4m3fn)")
+    if len(shape) != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2] or \
             ks.dtype != torch.float32 or vs.dtype != torch.float32:
         raise ValueError("paged cache: need k, v [P, G, page, D] and fp32 scales [P, G]")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("paged cache: contiguous tensors expected")
-    if not (v.device == ks.device == vs.device == dev):
+    if not v.get_device() == ks.get_device() == vs.get_device() == dev:
         raise ValueError("paged cache: tensors on several devices")
+    B = seq_lens.shape[0]
+    rows, cols = page_table.shape
+    if rows != B:
+        raise ValueError(f"page_table: {rows} rows for {B} sequences")
     c = a.cache
-    c.kv_type = _KV[k.dtype]
-    c.num_pages, c.G, c.page_size, c.D = k.shape
+    c.kv_type = _KV[dt]
+    c.num_pages, c.G, c.page_size, c.D = shape
     c.k, c.v, c.k_scale, c.v_scale = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
     c.page_table = _index(page_table, "page_table", dev, 2)
-    if page_table.shape[0] != B:
-        raise ValueError(f"page_table: {page_table.shape[0]} rows for {B} sequences")
-    c.max_pages = page_table.shape[1]
-    c.table_stride = page_table.stride(0) if B > 1 else c.max_pages
-    return dev
+    c.max_pages = cols
+    c.table_stride = page_table.stride()[0] if B > 1 else cols
+    a.B, a.seq_lens = B, _index(seq_lens, "seq_lens", dev, 1)
+    return dev, shape
 
 
-def _fill_batch(a, dev, cu_tokens, seq_lens, T, max_tokens):
-    a.cu_tokens, a.seq_lens = _index(cu_tokens, "cu_tokens", dev, 1), _index(seq_lens, "seq_lens", dev, 1)
-    a.B = seq_lens.shape[0]
+def _fill_tokens(a, dev, cu_tokens, T, max_tokens):
+    a.cu_tokens = _index(cu_tokens, "cu_tokens", dev, 1)
     if cu_tokens.shape[0] != a.B + 1:
         raise ValueError(f"cu_tokens: {cu_tokens.shape[0]} entries for {a.B} sequences")
     a.T, a.max_tokens = T, int(max_tokens)
 
 
-def _rows(x, name, dev, dt, T, heads, D):
+def _rows(x, name, dev, dt, shape):
     """Pointer and (token, head) strides of a [T, heads, D] tensor."""
-    if x.device != dev:
-        raise ValueError(f"{name}: on {x.device}, the cache is on {dev}")
+    if x.get_device() != dev:
+        raise ValueError(f"{name}: on {x.device}, the cache is on cuda:{dev}")
     if x.dtype != dt:
         raise TypeError(f"{name}: dtype {x.dtype} (need {dt})")
-    if tuple(x.shape) != (T, heads, D):
-        raise ValueError(f"{name}: shape {tuple(x.shape)} (need {(T, heads, D)})")
-    if x.numel() and x.stride(2) != 1:
+    if x.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(x.shape)} (need {shape})")
+    st, sh, sd = x.stride()
+    if sd != 1 and shape[0]:
         raise ValueError(f"{name}: last dimension must be contiguous")
-    return x.data_ptr(), x.stride(0) if T > 1 else 0, x.stride(1) if heads > 1 else 0
+    return x.data_ptr(), st if shape[0] > 1 else 0, sh if shape[1] > 1 else 0
 
 
 def _call(fn, dev, *args):
-    """``fn`` on the current stream of ``dev`` (the library works on the
-    current device)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return N.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+    """``fn`` on the current stream of device ``dev`` (the library works on
+    the current device)."""
+    if dev == torch._C._cuda_getDevice():
+        return N.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
     with torch.cuda.device(dev):
-        return N.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream))
+        return N.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
 
 
 def paged_append(cache, k, v, page_table, cu_tokens, seq_lens, max_tokens, q=None, cos=None, sin=None,
@@ -125,27 +131,26 @@ def paged_append(cache, k, v, page_table, cu_tokens, seq_lens, max_tokens, q=Non
     scale only grows; where it does, its earlier codes are rounded again.
     Two sequences must not append into the same page in one call."""
     a = N.PagedAppendArgs()
-    dev = _fill_cache(a, cache, page_table, seq_lens.shape[0])
-    G, D = cache.k.shape[1], cache.k.shape[3]
+    dev, (_, G, _, D) = _fill(a, cache, page_table, seq_lens)
     dt, T = k.dtype, k.shape[0]
     if dt not in _DT:
         raise TypeError(f"k: dtype {dt} (need float16 or bfloat16)")
     a.dtype = _DT[dt]
-    _fill_batch(a, dev, cu_tokens, seq_lens, T, max_tokens)
-    a.k, a.k_st, a.k_sh = _rows(k, "k", dev, dt, T, G, D)
-    a.v, a.v_st, a.v_sh = _rows(v, "v", dev, dt, T, G, D)
+    _fill_tokens(a, dev, cu_tokens, T, max_tokens)
+    a.k, a.k_st, a.k_sh = _rows(k, "k", dev, dt, (T, G, D))
+    a.v, a.v_st, a.v_sh = _rows(v, "v", dev, dt, (T, G, D))
     if q is not None:
-        H = q.shape[1]
-        a.H = H
-        a.q, a.q_st, a.q_sh = _rows(q, "q", dev, dt, T, H, D)
+        shape = (T, q.shape[1], D)
+        a.H = shape[1]
+        a.q, a.q_st, a.q_sh = _rows(q, "q", dev, dt, shape)
         if q_out is None:
-            q_out = torch.empty((T, H, D), dtype=dt, device=dev)
-        a.q_out, a.qo_st, a.qo_sh = _rows(q_out, "q_out", dev, dt, T, H, D)
+            q_out = q.new_empty(shape)
+        a.q_out, a.qo_st, a.qo_sh = _rows(q_out, "q_out", dev, dt, shape)
     elif q_out is not None or q_norm_w is not None:
         raise ValueError("q_out / q_norm_w without q")
     for w, name in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
-        if w is not None and (w.dtype != dt or w.device != dev or tuple(w.shape) != (D,) or not w.is_contiguous()):
-            raise ValueError(f"{name}: need a contiguous {dt} [{D}] on {dev}")
+        if w is not None and (w.dtype != dt or w.get_device() != dev or w.shape != (D,) or not w.is_contiguous()):
+            raise ValueError(f"{name}: need a contiguous {dt} [{D}] on cuda:{dev}")
     if k_norm_w is not None:
         a.k_norm_w, a.eps = k_norm_w.data_ptr(), float(eps)
     if q_norm_w is not None:
@@ -153,14 +158,15 @@ def paged_append(cache, k, v, page_table, cu_tokens, seq_lens, max_tokens, q=Non
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if cos is not None:
-        if cos.shape != sin.shape or cos.stride() != sin.stride() or cos.dtype != sin.dtype or cos.dim() != 2 or \
-                cos.shape[1] < D // 2 or cos.stride(1) != 1 or cos.device != dev or sin.device != dev:
-            raise ValueError(f"cos / sin: need two alike [rows, >= {D // 2}] tables on {dev}")
+        shape, st = cos.shape, cos.stride()
+        if sin.shape != shape or sin.stride() != st or sin.dtype != cos.dtype or len(shape) != 2 or \
+                shape[1] < D // 2 or st[1] != 1 or cos.get_device() != dev or sin.get_device() != dev:
+            raise ValueError(f"cos / sin: need two alike [rows, >= {D // 2}] tables on cuda:{dev}")
         if cos.dtype not in (torch.float32, dt):
             raise TypeError(f"cos / sin: dtype {cos.dtype} (need float32 or {dt})")
         a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
         a.cs_dtype = N.DTYPE_F32 if cos.dtype == torch.float32 else _DT[dt]
-        a.cs_rows, a.cs_stride = cos.shape[0], cos.stride(0) if cos.shape[0] > 1 else cos.shape[1] // 8 * 8
+        a.cs_rows, a.cs_stride = shape[0], st[0] if shape[0] > 1 else shape[1] // 8 * 8
         if positions is not None:
             a.positions = _index(positions, "positions", dev, 1)
             if positions.shape[0] != T:
@@ -178,22 +184,19 @@ def paged_attention(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_sc
     in HF's ``repeat_kv``. ``out`` rows behind the last sequence keep what they
     held."""
     a = N.PagedAttendArgs()
-    dev = _fill_cache(a, cache, page_table, seq_lens.shape[0])
-    T, H, D = q.shape
-    dt = q.dtype
+    dev, (_, _, _, D) = _fill(a, cache, page_table, seq_lens)
+    shape, dt = (q.shape[0], q.shape[1], D), q.dtype
     if dt not in _DT:
         raise TypeError(f"q: dtype {dt} (need float16 or bfloat16)")
-    a.dtype, a.H = _DT[dt], H
-    _fill_batch(a, dev, cu_tokens, seq_lens, T, max_tokens)
-    if D != cache.k.shape[3]:
-        raise ValueError(f"q: head dim {D}, the cache has {cache.k.shape[3]}")
-    a.q, a.q_st, a.q_sh = _rows(q, "q", dev, dt, T, H, D)
+    a.dtype, a.H = _DT[dt], shape[1]
+    _fill_tokens(a, dev, cu_tokens, shape[0], max_tokens)
+    a.q, a.q_st, a.q_sh = _rows(q, "q", dev, dt, shape)
     if out is None:
-        out = torch.empty((T, H, D), dtype=dt, device=dev)
-    a.out, a.o_st, a.o_sh = _rows(out, "out", dev, dt, T, H, D)
-    a.sm_scale = float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale)
+        out = q.new_empty(shape)
+    a.out, a.o_st, a.o_sh = _rows(out, "out", dev, dt, shape)
+    a.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
     n = N.lib.spatten_paged_attend_workspace_size(a)
-    ws = torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+    ws = q.new_empty((n,), dtype=torch.uint8) if n else None
     _call(N.lib.spatten_paged_attend, dev, a, ws.data_ptr() if n else None, n)
     return out
 
@@ -204,20 +207,20 @@ def paged_read(cache, page_table, seq_lens, idx=None, n_tokens=None, dtype=torch
     first ``n_tokens`` slots (default: what the page table spans). Zeros where
     a slot is outside the sequence."""
     a = N.PagedReadArgs()
-    B = seq_lens.shape[0]
-    dev = _fill_cache(a, cache, page_table, B)
+    dev, (_, G, page, D) = _fill(a, cache, page_table, seq_lens)
     if dtype not in _DT:
         raise TypeError(f"dtype {dtype} (need float16 or bfloat16)")
-    _, G, page, D = cache.k.shape
-    a.dtype, a.B, a.seq_lens = _DT[dtype], B, _index(seq_lens, "seq_lens", dev, 1)
+    B = a.B
+    a.dtype = _DT[dtype]
     if idx is not None:
         a.idx = _index(idx, "idx", dev, 2, torch.int64)
-        if idx.shape[0] != B:
-            raise ValueError(f"idx: {idx.shape[0]} rows for {B} sequences")
-        a.N, a.idx_stride = idx.shape[1], idx.stride(0)
+        rows, n = idx.shape
+        if rows != B:
+            raise ValueError(f"idx: {rows} rows for {B} sequences")
+        a.N, a.idx_stride = n, idx.stride()[0]
     else:
-        a.N = int(n_tokens) if n_tokens is not None else page_table.shape[1] * page
-    k, v = (torch.empty((B, max(a.N, 0), G, D), dtype=dtype, device=dev) for _ in range(2))
+        n = a.N = page_table.shape[1] * page if n_tokens is None else int(n_tokens)
+    k, v = (cache.k.new_empty((B, max(n, 0), G, D), dtype=dtype) for _ in range(2))
     a.k_out, a.v_out = k.data_ptr(), v.data_ptr()
     _call(N.lib.spatten_paged_read, dev, a)
     return k, v
