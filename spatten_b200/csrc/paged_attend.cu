@@ -640,13 +640,14 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
 // Joins the line that CTA blockIdx.x began and did not finish: its parts are
 // slot 2 c + 1 of that CTA and slot 2 c of the following ones. A warp per row
 // and, where the line has fewer rows than the CTA has warps, per share of the
-// parts; D / 32 dims per lane, eight parts in flight.
+// parts; D / 32 dims per lane. Bound by the latency of its loads: the (m, l, M)
+// of 64 parts (two per lane) and 8 outputs of the warp's share go out at once.
 constexpr int kJoinWarps = 16;
 
 template <int D, int ROWS>
-__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const PagedAttendParams p, const Workspace ws,
+__global__ void __launch_bounds__(32 * kJoinWarps, D == 128 ? 1 : 2) paged_join_kernel(const PagedAttendParams p, const Workspace ws,
                                                                      const bool bf16) {
-  constexpr int E = D / 32, FLY = 8;
+  constexpr int E = D / 32, FLY = 8, SPAN = 64;
   __shared__ float sh[kJoinWarps][D + 4];
   grid_dependents();
   grid_wait();
@@ -658,66 +659,82 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_kernel(const Paged
   while (share > 1 && rows * share > kJoinWarps) share >>= 1;
   const int row = warp / share, part0 = warp % share;
   const bool live = row < rows;
-  auto at = [&](int i) { return (int64_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * ROWS + row; };
-  float mm = -INFINITY, MM = -INFINITY, l = 0.f, acc[E], x[FLY][E];
+  auto at = [&](int i) { return (uint32_t)(2 * (c0 + i) + (i == 0)) * ROWS + row; };  // row of part i
+  float m = -INFINITY, M = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  auto fetch = [&](int i0) {
+  for (int base = 0; live && base < cut.parts; base += SPAN) {
+    const int end = min(base + SPAN, cut.parts);
+    float4 h[2];  // of parts base + lane and base + 32 + lane
 #pragma unroll
-    for (int k = 0; k < FLY; ++k) {
-      const int i = i0 + k * share;
-      if (i >= cut.parts) break;
-      const float* src = ws.o + at(i) * D + lane * E;
-      if constexpr (E == 4) {
-        const float4 y = *reinterpret_cast<const float4*>(src);
-        x[k][0] = y.x; x[k][1] = y.y; x[k][2] = y.z; x[k][3] = y.w;
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(src);
-        x[k][0] = y.x; x[k][1] = y.y;
-      }
+    for (int k = 0; k < 2; ++k) {
+      const int i = base + 32 * k + lane;
+      h[k] = i < end ? ws.ml[at(i)] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
     }
-  };
-  if (live) {
-    fetch(part0);
-    for (int i = lane; i < cut.parts; i += 32) {
-      const float4 h = ws.ml[at(i)];
-      mm = fmaxf(mm, h.x);
-      MM = fmaxf(MM, h.z);
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-      mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-      MM = fmaxf(MM, __shfl_xor_sync(0xffffffffu, MM, d));
-    }
-    for (int i0 = part0; i0 < cut.parts; i0 += FLY * share) {
-      if (i0 != part0) fetch(i0);
+    float f[2];
+    for (int i0 = base + part0; i0 == base + part0 || i0 < end; i0 += FLY * share) {
+      float x[FLY][E];
 #pragma unroll
       for (int k = 0; k < FLY; ++k) {
         const int i = i0 + k * share;
-        if (i >= cut.parts) break;
-        const float4 h = ws.ml[at(i)];
-        const float f = fast_exp2(h.z - finite_or_0(MM));
-        l += h.y * fast_exp2(h.x - finite_or_0(mm));
+        if (i < end) {
+          const float* src = ws.o + (at(i) * D + lane * E);
+          if constexpr (E == 4) {
+            const float4 y = *reinterpret_cast<const float4*>(src);
+            x[k][0] = y.x; x[k][1] = y.y; x[k][2] = y.z; x[k][3] = y.w;
+          } else {
+            const float2 y = *reinterpret_cast<const float2*>(src);
+            x[k][0] = y.x; x[k][1] = y.y;
+          }
+        }
+      }
+      if (i0 == base + part0) {  // the span's weights, while the outputs are under way
+        float mn = fmaxf(h[0].x, h[1].x), Mn = fmaxf(h[0].z, h[1].z);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += x[k][e] * f;
+        for (int d = 16; d > 0; d >>= 1) {
+          mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+          Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, d));
+        }
+        mn = fmaxf(m, mn);
+        Mn = fmaxf(M, Mn);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          f[k] = fast_exp2(h[k].z - finite_or_0(Mn));
+          sum += h[k].y * fast_exp2(h[k].x - finite_or_0(mn));
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        l = l * fast_exp2(m - finite_or_0(mn)) + sum;
+        const float r = fast_exp2(M - finite_or_0(Mn));
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= r;
+        m = mn;
+        M = Mn;
+      }
+#pragma unroll
+      for (int k = 0; k < FLY; ++k) {
+        const int i = i0 + k * share;
+        if (i >= end) break;  // warp-uniform
+        const float w = __shfl_sync(0xffffffffu, i - base < 32 ? f[0] : f[1], (i - base) & 31);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += x[k][e] * w;
       }
     }
   }
-  if (share > 1) {  // the shares of a row join in its first warp
+  if (share > 1) {  // the shares of a row join in its first warp; each has the whole l
 #pragma unroll
     for (int e = 0; e < E; ++e) sh[warp][lane * E + e] = acc[e];
-    if (lane == 0) sh[warp][D] = l;
     __syncthreads();
     if (part0 == 0)
       for (int w = 1; w < share; ++w) {
-        l += sh[warp + w][D];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += sh[warp + w][lane * E + e];
       }
   }
   if (live && part0 == 0) {
     const int r = cut.row0 + row;
-    const float inv = normaliser(mm, l, MM);
+    const float inv = normaliser(m, l, M);
     uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(cut.begin + r / R) * p.o_st +
                    (int64_t)(cut.g * R + r % R) * p.o_sh + lane * E;
 #pragma unroll

@@ -29,10 +29,39 @@ import torch
 
 from . import _native as N
 
-PagedKVCache = namedtuple("PagedKVCache", "k v k_scale v_scale")  # [P, G, page, D] x2, [P, G] x2
-
 _DT = {torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
 _KV = {torch.int8: N.KV_INT8, torch.float8_e4m3fn: N.KV_E4M3}
+
+
+class PagedKVCache(namedtuple("PagedKVCache", "k v k_scale v_scale")):
+    """The pool: k, v codes [P, G, page, D], k_scale, v_scale fp32 [P, G], all
+    contiguous. Its checks and the C form of it are made once, at its first
+    use (the tensors of a tuple do not change)."""
+
+    @property
+    def native(self):
+        """(device index, shape of the pool, C form without a page table)."""
+        try:
+            return self._native
+        except AttributeError:
+            pass
+        k, v, ks, vs = self
+        dev, dt, shape = k.get_device(), k.dtype, k.shape
+        if dev < 0:
+            raise ValueError("paged cache: CUDA tensors expected (no CPU path)")
+        if dt not in _KV or v.dtype != dt:
+            raise TypeError(f"paged cache: codes {dt} and {v.dtype} (need int8 or float8_e4m3fn)")
+        if len(shape) != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2] or \
+                ks.dtype != torch.float32 or vs.dtype != torch.float32:
+            raise ValueError("paged cache: need k, v [P, G, page, D] and fp32 scales [P, G]")
+        if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+            raise ValueError("paged cache: contiguous tensors expected")
+        if not v.get_device() == ks.get_device() == vs.get_device() == dev:
+            raise ValueError("paged cache: tensors on several devices")
+        P, G, page, D = shape
+        self._native = dev, (P, G, page, D), N.PagedCache(_KV[dt], P, page, G, D, k.data_ptr(), v.data_ptr(),
+                                                          ks.data_ptr(), vs.data_ptr())
+        return self._native
 
 
 def new_paged_cache(num_pages, kv_heads, head_dim, page_size=64, kv_dtype=torch.int8, device="cuda"):
@@ -60,29 +89,13 @@ def _index(t, name, dev, dim, dtype=torch.int32):
 def _fill(a, cache, page_table, seq_lens):
     """The cache and the sequences into ``a``; returns (device index, the
     pool's shape)."""
-    k, v, ks, vs = cache
-    dev, dt, shape = k.get_device(), k.dtype, k.shape
-    if dev < 0:
-        raise ValueError("paged cache: CUDA tensors expected (no CPU path)")
-    if dt not in _KV or v.dtype != dt:
-        raise TypeError(f"paged cache: codes {dt} and {v.dtype} (need int8 or float8_e4m3fn)")
-    if len(shape) != 4 or v.shape != shape or ks.shape != shape[:2] or vs.shape != shape[:2] or \
-            ks.dtype != torch.float32 or vs.dtype != torch.float32:
-        raise ValueError("paged cache: need k, v [P, G, page, D] and fp32 scales [P, G]")
-    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
-        raise ValueError("paged cache: contiguous tensors expected")
-    if not v.get_device() == ks.get_device() == vs.get_device() == dev:
-        raise ValueError("paged cache: tensors on several devices")
+    dev, shape, a.cache = cache.native
     B = seq_lens.shape[0]
     rows, cols = page_table.shape
     if rows != B:
         raise ValueError(f"page_table: {rows} rows for {B} sequences")
     c = a.cache
-    c.kv_type = _KV[dt]
-    c.num_pages, c.G, c.page_size, c.D = shape
-    c.k, c.v, c.k_scale, c.v_scale = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
-    c.page_table = _index(page_table, "page_table", dev, 2)
-    c.max_pages = cols
+    c.page_table, c.max_pages = _index(page_table, "page_table", dev, 2), cols
     c.table_stride = page_table.stride()[0] if B > 1 else cols
     a.B, a.seq_lens = B, _index(seq_lens, "seq_lens", dev, 1)
     return dev, shape
