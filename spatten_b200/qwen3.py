@@ -27,17 +27,25 @@ attention core with the progressive sparse attention kernel:
   count ``v_prune_num`` (<= 16), ``enable_prog_quant`` with ``quant_threshold``
   (the row max-probability below which the LSB plane of K is refetched).
 
-Prefill of unpadded batches only (the HF attention mask is not read: the
-mask is the causal one). The cascade state is shared by all layers of a
-model (``patch_qwen3``) and restarts at layer 0 of every forward.
+* Generation: with a ``PagedQwen3Cache`` as ``past_key_values`` the prefill's
+  keys and values of every layer go into a paged 8-bit cache (``paged.py``), and
+  later forwards (a token, a few, or the next piece of a prompt) append to it and
+  attend over it: QK-norm, RoPE and the append in one launch, the attention in
+  two. A layer that pruned its keys keeps attending over the ones it kept.
+
+Unpadded batches only (the HF attention mask is not read: the mask is the
+causal one). The cascade state is shared by all layers of a model
+(``patch_qwen3``) and restarts at layer 0 of every prefill.
 """
 import math
 from fractions import Fraction
 
 import torch
+from transformers.cache_utils import Cache
 from transformers.models.qwen3.modeling_qwen3 import Qwen3Attention, apply_rotary_pos_emb
 
 from . import _native as N
+from . import paged
 from .progressive import prog_attn, quant_k_planes, quant_q_int8
 from .select import gather_rows, topk_indices
 
@@ -92,6 +100,70 @@ def qk_norm_rope(q, k, q_norm, k_norm, cos, sin, Hq, Hk, D, quantize_q):
     return q_out, q8, qs, k_out
 
 
+class PagedQwen3Cache(Cache):
+    """Paged 8-bit KV cache of every layer, for ``past_key_values`` of a model
+    that ``patch_qwen3`` made. ``max_tokens`` slots per sequence are reserved in
+    each layer's pool, sequence b's pages in a row; the layers share one page
+    table. Layers may hold different numbers of tokens (token pruning)."""
+
+    def __init__(self, config, batch, max_tokens, page_size=64, kv_dtype=torch.int8, device="cuda"):
+        super().__init__(layers=[])
+        L, G, D = config.num_hidden_layers, config.num_key_value_heads, config.head_dim
+        self.batch, self.max_tokens = batch, int(max_tokens)
+        mp = -(-self.max_tokens // page_size)
+        self.pools = [paged.new_paged_cache(batch * mp, G, D, page_size, kv_dtype, device) for _ in range(L)]
+        self.page_table = torch.arange(batch * mp, dtype=torch.int32, device=device).view(batch, mp)
+        self.seq_lens = torch.zeros((L, batch), dtype=torch.int32, device=device)
+        self.held = [0] * L  # slots of each layer, as the host counts them
+        self.seen = [0] * L  # positions each layer has been given (kept or not)
+
+    def get_seq_length(self, layer_idx=0):
+        return self.seen[layer_idx]
+
+    def get_mask_sizes(self, query_length, layer_idx=0):
+        return self.seen[layer_idx or 0] + int(query_length), 0
+
+    def get_max_cache_shape(self, layer_idx=0):
+        return self.max_tokens
+
+    def reset(self):
+        """Forget every token; the pools stay."""
+        self.seq_lens.zero_()
+        self.held, self.seen = [0] * len(self.held), [0] * len(self.seen)
+
+    def packed(self, S):
+        """cu_tokens of a batch that brings S tokens per sequence."""
+        return torch.arange(0, (self.batch + 1) * S, S, dtype=torch.int32, device=self.seq_lens.device)
+
+    def grow(self, layer_idx, n, seen):
+        """Count n more slots (of ``seen`` more positions) in one layer."""
+        if self.held[layer_idx] + n > self.max_tokens:
+            raise ValueError(f"PagedQwen3Cache: {self.held[layer_idx]} + {n} tokens, room for {self.max_tokens}")
+        self.held[layer_idx] += n
+        self.seen[layer_idx] += seen
+        self.seq_lens[layer_idx].add_(n)
+        return self.seq_lens[layer_idx]
+
+    def store(self, layer_idx, k, v, seen):
+        """Append finished (normed and rotated) keys and values [B, K, G, D];
+        ``seen``: the positions that they were chosen from."""
+        B, K, G, D = k.shape
+        if B != self.batch:
+            raise ValueError(f"PagedQwen3Cache: batch {B}, made for {self.batch}")
+        lens = self.grow(layer_idx, K, seen)
+        paged.paged_append(self.pools[layer_idx], k.reshape(B * K, G, D), v.reshape(B * K, G, D), self.page_table,
+                           self.packed(K), lens, K)
+
+    def update(self, key_states, value_states, layer_idx, *args, **kwargs):
+        """HF's form of ``store`` ([B, G, K, D]); only a prefill's first call may
+        use it, as attention modules that read a dense cache expect all keys
+        back."""
+        if self.held[layer_idx]:
+            raise NotImplementedError("PagedQwen3Cache: read by SpattenQwen3Attention only")
+        self.store(layer_idx, key_states.transpose(1, 2), value_states.transpose(1, 2), key_states.shape[2])
+        return key_states, value_states
+
+
 class CascadeState:
     """Kept key positions [B, K] (int64, ascending) and their cumulative
     token importance [B, K] (fp32), handed from layer to layer."""
@@ -135,6 +207,31 @@ class SpattenQwen3Attention(Qwen3Attention):
                         f"v_prune_num={v_count}: at most {N.MAX_V_PRUNE_COUNT} keys per row by count")
         return v_thr, v_count
 
+    def _extend(self, hidden_states, position_embeddings, cache):
+        """Forward of further tokens over a ``PagedQwen3Cache`` that holds some."""
+        B, S, _ = hidden_states.shape
+        H, Hkv, d = self.num_heads, self.num_kv_heads, self.head_dim
+        dt = hidden_states.dtype
+        if dt not in _DT or d not in (64, 128):
+            raise NotImplementedError(f"PagedQwen3Cache: {dt}, head dim {d} (need fp16 / bf16, 64 or 128)")
+        if B != cache.batch:
+            raise ValueError(f"PagedQwen3Cache: batch {B}, made for {cache.batch}")
+        if float(self.k_norm.variance_epsilon) != float(self.q_norm.variance_epsilon):
+            raise ValueError("q_norm and k_norm must share their epsilon")
+        q = self.q_proj(hidden_states).view(B * S, H, d)
+        k = self.k_proj(hidden_states).view(B * S, Hkv, d)
+        v = self.v_proj(hidden_states).view(B * S, Hkv, d)
+        cos, sin = position_embeddings  # [B or 1, S, d]: a row per token
+        rows = torch.arange(cos.shape[0] * S, dtype=torch.int32, device=q.device)
+        positions = rows if cos.shape[0] == B else rows.repeat(B)
+        pool, cu = cache.pools[self.layer_idx], cache.packed(S)
+        lens = cache.grow(self.layer_idx, S, S)
+        q = paged.paged_append(pool, k, v, cache.page_table, cu, lens, S, q=q, cos=cos.reshape(-1, d),
+                               sin=sin.reshape(-1, d), positions=positions, q_norm_w=self.q_norm.weight,
+                               k_norm_w=self.k_norm.weight, eps=self.q_norm.variance_epsilon)
+        out = paged.paged_attention(q, pool, cache.page_table, cu, lens, S, sm_scale=self.scaling)
+        return self.o_proj(out.view(B, S, H * d)), None
+
     @torch.no_grad()
     def forward(self, hidden_states, position_embeddings, attention_mask=None, past_key_values=None,
                 **kwargs):
@@ -142,7 +239,10 @@ class SpattenQwen3Attention(Qwen3Attention):
             raise ValueError("SpattenQwen3Attention runs on the CUDA kernels only")
         B, S, _ = hidden_states.shape
         if past_key_values is not None and past_key_values.get_seq_length(self.layer_idx) > 0:
-            raise NotImplementedError("SpattenQwen3Attention: prefill only (the cache already holds keys)")
+            if isinstance(past_key_values, PagedQwen3Cache):
+                return self._extend(hidden_states, position_embeddings, past_key_values)
+            raise NotImplementedError("SpattenQwen3Attention: prefill only (the cache already holds keys); "
+                                      "a PagedQwen3Cache can be extended")
         H, Hkv, d = self.num_heads, self.num_kv_heads, self.head_dim
         dev = hidden_states.device
         cos, sin = position_embeddings
@@ -196,7 +296,9 @@ class SpattenQwen3Attention(Qwen3Attention):
         self.token_importance = cum
         st.kept_per_layer.append(K)
 
-        if past_key_values is not None:
+        if isinstance(past_key_values, PagedQwen3Cache):
+            past_key_values.store(self.layer_idx, k, v, S)
+        elif past_key_values is not None:
             # the cache concatenates into a new contiguous [B, Hkv, K, d] tensor
             # itself: the head-major views go in as they are (one copy, not two)
             past_key_values.update(kh, vh, self.layer_idx)
