@@ -85,12 +85,14 @@ const char* spatten_last_error(void) { return g_err.c_str(); }
 
 int spatten_device_error(unsigned int* code, int reset) {
   if (!code) return fail(SPATTEN_ERR_INVALID, "device_error: null output");
-  unsigned int proj = 0, out = 0;
+  unsigned int proj = 0, out = 0, paged = 0;
   if (int e = cuda_status(spatten::read_device_error(code, reset != 0), "device_error read")) return e;
   if (int e = cuda_status(spatten::read_proj_device_error(&proj, reset != 0), "device_error read")) return e;
   if (int e = cuda_status(spatten::read_out_proj_device_error(&out, reset != 0), "device_error read")) return e;
+  if (int e = cuda_status(spatten::read_paged_device_error(&paged, reset != 0), "device_error read")) return e;
   if (*code == 0) *code = proj;
   if (*code == 0) *code = out;
+  if (*code == 0) *code = paged;
   return ok();
 }
 

@@ -74,6 +74,12 @@ cudaError_t launch_paged_read(const PagedReadParams& p, int dtype, int kv, cudaS
 int paged_attend_max_batch();  // sequences of one call
 bool paged_attend_fits(const PagedAttendParams& p);  // units of work count in 32 bits
 size_t paged_attend_workspace(const PagedAttendParams& p, int n_sm);
+// the tcgen05 path (paged_attend_tc.cu), for many query rows per KV head
+bool paged_attend_tc_takes(const PagedAttendParams& p);
+size_t paged_attend_tc_workspace(const PagedAttendParams& p, int n_sm);
+cudaError_t launch_paged_attend_tc(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,
+                                   cudaStream_t st);
+cudaError_t read_paged_device_error(unsigned int* code, bool reset);
 cudaError_t launch_paged_attend(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,
                                 cudaStream_t st);
 

@@ -37,6 +37,7 @@
 
 #include "kernels.h"
 #include "paged_dev.cuh"
+#include "paged_join.cuh"
 
 namespace spatten {
 namespace {
@@ -50,23 +51,8 @@ constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 // sequences whose prefix sums fit the shared memory
 constexpr int kMaxBatch = 8192;
 
-// The parts of a row tile that a CTA begins and does not finish.
-struct Cut {
-  int parts;         // 0: none
-  int row0, nrows;   // first row of the tile among the sequence's, rows of the sequence
-  int begin, g;      // first packed row of the sequence, KV head
-  int pad[3];
-};
+using Workspace = PagedPartials;
 
-struct Workspace {
-  Cut* cut;     // [ctas]
-  float4* ml;   // [2 ctas][rows] (m, l, M): slot 2 c: a tile begun before CTA c; 2 c + 1: one begun in it
-  float* o;     // [2 ctas][rows][D]
-};
-
-// ---------------------------------------------------------------------------
-// Codes as operands. Words are 4 consecutive dims of a key.
-// ---------------------------------------------------------------------------
 template <int KV, int D, int NB>
 struct Operands;
 
@@ -179,13 +165,6 @@ SPATTEN_DEV uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-
-SPATTEN_DEV float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
-
-// What takes an output by M to the result: 2^(M - m) / l, 0 for a row without a key.
-SPATTEN_DEV float normaliser(float m, float l, float M) {
-  return l == 0.f ? 0.f : exp2f(fminf(finite_or_0(M) - finite_or_0(m), 127.f)) / l;
 }
 
 // Row tiles of a sequence, and key tiles that its last row sees (one at least,
@@ -330,7 +309,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   }
   const uint32_t cta = blockIdx.x;
   const uint32_t ctas = min(gridDim.x, few ? U : (U + kWarps - 1) / kWarps);
-  Cut cut = {};
+  PagedCut cut = {};
   if (cta >= ctas) {
     if (tid == 0) ws.cut[cta] = cut;
     return;
@@ -614,7 +593,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         acc.x += x.x * f; acc.y += x.y * f; acc.z += x.z * f; acc.w += x.w * f;
       }
       if (whole) {
-        const float inv = normaliser(mm, ll, MM);
+        const float inv = paged_normaliser(mm, ll, MM);
         uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(sq.begin + r / R) * p.o_st +
                        (int64_t)(g * R + r % R) * p.o_sh + d;
         uint2 v;
@@ -637,113 +616,6 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   if (tid == 0) ws.cut[cta] = cut;
 }
 
-// Joins the line that CTA blockIdx.x began and did not finish: its parts are
-// slot 2 c + 1 of that CTA and slot 2 c of the following ones. A warp per row
-// and, where the line has fewer rows than the CTA has warps, per share of the
-// parts; D / 32 dims per lane. Bound by the latency of its loads: the (m, l, M)
-// of 64 parts (two per lane) and 8 outputs of the warp's share go out at once.
-constexpr int kJoinWarps = 16;
-
-template <int D, int ROWS>
-__global__ void __launch_bounds__(32 * kJoinWarps, D == 128 ? 1 : 2) paged_join_kernel(const PagedAttendParams p, const Workspace ws,
-                                                                     const bool bf16) {
-  constexpr int E = D / 32, FLY = 8, SPAN = 64;
-  __shared__ float sh[kJoinWarps][D + 4];
-  grid_dependents();
-  grid_wait();
-  const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Cut cut = ws.cut[c0];
-  if (cut.parts == 0) return;
-  const int R = p.b.H / p.c.G, rows = min(cut.nrows - cut.row0, ROWS);
-  int share = kJoinWarps;  // warps per row
-  while (share > 1 && rows * share > kJoinWarps) share >>= 1;
-  const int row = warp / share, part0 = warp % share;
-  const bool live = row < rows;
-  auto at = [&](int i) { return (uint32_t)(2 * (c0 + i) + (i == 0)) * ROWS + row; };  // row of part i
-  float m = -INFINITY, M = -INFINITY, l = 0.f, acc[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int base = 0; live && base < cut.parts; base += SPAN) {
-    const int end = min(base + SPAN, cut.parts);
-    float4 h[2];  // of parts base + lane and base + 32 + lane
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int i = base + 32 * k + lane;
-      h[k] = i < end ? ws.ml[at(i)] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
-    }
-    float f[2];
-    for (int i0 = base + part0; i0 == base + part0 || i0 < end; i0 += FLY * share) {
-      float x[FLY][E];
-#pragma unroll
-      for (int k = 0; k < FLY; ++k) {
-        const int i = i0 + k * share;
-        if (i < end) {
-          const float* src = ws.o + (at(i) * D + lane * E);
-          if constexpr (E == 4) {
-            const float4 y = *reinterpret_cast<const float4*>(src);
-            x[k][0] = y.x; x[k][1] = y.y; x[k][2] = y.z; x[k][3] = y.w;
-          } else {
-            const float2 y = *reinterpret_cast<const float2*>(src);
-            x[k][0] = y.x; x[k][1] = y.y;
-          }
-        }
-      }
-      if (i0 == base + part0) {  // the span's weights, while the outputs are under way
-        float mn = fmaxf(h[0].x, h[1].x), Mn = fmaxf(h[0].z, h[1].z);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-          mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
-          Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, d));
-        }
-        mn = fmaxf(m, mn);
-        Mn = fmaxf(M, Mn);
-        float sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          f[k] = fast_exp2(h[k].z - finite_or_0(Mn));
-          sum += h[k].y * fast_exp2(h[k].x - finite_or_0(mn));
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        l = l * fast_exp2(m - finite_or_0(mn)) + sum;
-        const float r = fast_exp2(M - finite_or_0(Mn));
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] *= r;
-        m = mn;
-        M = Mn;
-      }
-#pragma unroll
-      for (int k = 0; k < FLY; ++k) {
-        const int i = i0 + k * share;
-        if (i >= end) break;  // warp-uniform
-        const float w = __shfl_sync(0xffffffffu, i - base < 32 ? f[0] : f[1], (i - base) & 31);
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += x[k][e] * w;
-      }
-    }
-  }
-  if (share > 1) {  // the shares of a row join in its first warp; each has the whole l
-#pragma unroll
-    for (int e = 0; e < E; ++e) sh[warp][lane * E + e] = acc[e];
-    __syncthreads();
-    if (part0 == 0)
-      for (int w = 1; w < share; ++w) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += sh[warp + w][lane * E + e];
-      }
-  }
-  if (live && part0 == 0) {
-    const int r = cut.row0 + row;
-    const float inv = normaliser(m, l, M);
-    uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(cut.begin + r / R) * p.o_st +
-                   (int64_t)(cut.g * R + r % R) * p.o_sh + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; e += 2)
-      *reinterpret_cast<uint32_t*>(op + e) =
-          bf16 ? pack2<__nv_bfloat16>(acc[e] * inv, acc[e + 1] * inv) : pack2<__half>(acc[e] * inv, acc[e + 1] * inv);
-  }
-}
-
 // Eight query rows per pass where that covers a sequence's rows (the register
 // tile of 16 has room for half the bytes in flight), else sixteen.
 int row_block(const PagedAttendParams& p) { return (int64_t)p.b.max_tokens * (p.b.H / p.c.G) <= 8 ? 8 : 16; }
@@ -759,8 +631,6 @@ int grid_ctas(const PagedAttendParams& p, int n_sm) {
   const int wave = n_sm * 3;
   return (int)fmin((double)wave, fmax(1.0, ceil(units_bound(p) / kWarps)));
 }
-
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 template <int KV, int D, int NB>
 cudaError_t attend_launch(const PagedAttendParams& p, bool bf16, const Workspace& ws, int ctas, cudaStream_t st) {
@@ -778,7 +648,7 @@ cudaError_t attend_launch(const PagedAttendParams& p, bool bf16, const Workspace
   }
   e = launch_dependent(paged_attend_kernel<KV, D, NB>, dim3(ctas), 32 * kWarps, smem, st, p, ws, bf16);
   if (e != cudaSuccess) return e;
-  return launch_dependent(paged_join_kernel<D, SH::kRows>, dim3(ctas), 32 * kJoinWarps, 0, st, p, ws, bf16);
+  return launch_paged_join<D, SH::kRows>(p, ws, ctas, bf16, st);
 }
 
 template <int KV, int D>
@@ -801,21 +671,15 @@ int paged_attend_max_batch() { return kMaxBatch; }
 bool paged_attend_fits(const PagedAttendParams& p) { return units_bound(p) < 4e9; }
 
 size_t paged_attend_workspace(const PagedAttendParams& p, int n_sm) {
-  const size_t ctas = grid_ctas(p, n_sm), rows = row_block(p);
-  return align256(ctas * sizeof(Cut)) + align256(2 * ctas * rows * sizeof(float4)) +
-         align256(2 * ctas * rows * p.c.D * sizeof(float));
+  if (paged_attend_tc_takes(p)) return paged_attend_tc_workspace(p, n_sm);
+  return paged_partials_bytes(grid_ctas(p, n_sm), row_block(p), p.c.D);
 }
 
 cudaError_t launch_paged_attend(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm, cudaStream_t st) {
   if (dtype != kF16 && dtype != kBF16) return cudaErrorInvalidValue;
-  const int ctas = grid_ctas(p, n_sm), rows = row_block(p);
-  uint8_t* w = static_cast<uint8_t*>(ws);
-  Workspace s;
-  s.cut = reinterpret_cast<Cut*>(w);
-  w += align256(ctas * sizeof(Cut));
-  s.ml = reinterpret_cast<float4*>(w);
-  w += align256((size_t)2 * ctas * rows * sizeof(float4));
-  s.o = reinterpret_cast<float*>(w);
+  if (paged_attend_tc_takes(p)) return launch_paged_attend_tc(p, dtype, kv, ws, n_sm, st);
+  const int ctas = grid_ctas(p, n_sm);
+  const Workspace s = paged_partials(ws, ctas, row_block(p));
   const bool bf16 = dtype == kBF16;
   return kv == kKvInt8 ? attend_dim<kKvInt8>(p, bf16, s, ctas, st) : attend_dim<kKvE4m3>(p, bf16, s, ctas, st);
 }

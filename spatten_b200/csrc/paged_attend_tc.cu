@@ -1,0 +1,627 @@
+// Attention over the paged 8-bit KV cache for many query rows per KV head
+// (pieces of prompts): the tcgen05 path of spatten_paged_attend.
+//
+// The R = H / G query heads of a KV head and the n new tokens of a sequence are
+// n R query rows over the same keys. A CTA takes 256 of them (two row tiles of
+// 128) and walks key tiles of 64:
+//   S [128 x 64] = Q' . K codes^T,  O [128 x D] += W . V codes   (kind::f16)
+// with f16 operands (every int8 and e4m3 code is an f16; q' = q 2^e, see
+// paged_attend.cu) and fp32 accumulators in tensor memory. One thread owns a
+// query row:
+//   t = S (sm_scale log2(e) 2^-e k_scale),  w = 2^(t + log2 v_scale - M),
+// with a reference M that follows max(t + log2 v_scale), so that W keeps 11 bits
+// whatever the blocks' scales are; O is rescaled in tensor memory when M moved by
+// more than 2^kSlack. The softmax's sum l needs p = 2^(t - m): within a block w
+// and p differ by the factor 2^(M - log2 v_scale - m), so l takes the block's sum
+// of w times it (one exponential per score), except where w could underflow
+// under it, which takes the exponentials of p.
+//
+// 13 warps, one CTA per SM:
+//   warps 0-3, 4-7  softmax of the two row tiles: S from tensor memory, W into
+//                   shared memory (swizzled), rescaling, the epilogue and the
+//                   next queries;
+//   warps 8-11      codes to f16: 16-byte loads two tiles ahead, widened into a
+//                   ring of K / V tiles in the layouts that the MMAs read (K
+//                   K-major, V MN-major: both [64-dim block][key][128 B]);
+//   warp 12         MMA issue: S of tile j + 1 before O of tile j.
+// A tile's codes are widened once for 256 rows, and two row tiles keep the
+// tensor cores busy through each other's softmax. What bounds it: shared-memory
+// traffic of the operands (a 128 x 64 x 16 step reads 6 KB) and the softmax's
+// exponentials (16 per clock and SM), at similar rates.
+//
+// Work split: as in paged_attend.cu, ranges of equal length over all CTAs, here in
+// keys: row tile rt of a sequence counts old + (rt + 1) 256 / R of them (the causal
+// triangle), cumulated in closed form, and the 64-key tile at position k belongs
+// to the CTA that holds unit k of its line. Every wait is bounded; a timeout
+// records a code in this file's device error word and the CTA winds down.
+#include <atomic>
+#include <cmath>
+
+#include "kernels.h"
+#include "paged_dev.cuh"
+#include "paged_join.cuh"
+#include "sm100.cuh"
+
+namespace spatten {
+namespace {
+
+using namespace sm100;
+
+constexpr int kRowTile = 128, kRowsCta = 256, kKeys = 64, kRing = 3;
+constexpr int kSoftWarps = 8, kWideWarps = 4, kThreads = 32 * (kSoftWarps + kWideWarps + 1);
+constexpr float kSlack = 8.f;
+constexpr float kNoScale = -200.f;  // log2 of a scale of 0
+constexpr unsigned kErr = 0x400;
+constexpr int kMaxBatch = 1024;
+
+template <int D>
+struct Lay {
+  static constexpr int kTileBytes = kKeys * D * 2;       // K or V, f16
+  static constexpr int kQBytes = kRowTile * D * 2;
+  static constexpr int kWBytes = kRowTile * kKeys * 2;
+  static constexpr int oQ = 0;                            // [2][D / 64][128][128 B]
+  static constexpr int oKV = oQ + 2 * kQBytes;            // [ring][K | V][D / 64][64][128 B]
+  static constexpr int oW = oKV + kRing * 2 * kTileBytes; // [2][128][128 B]
+  static constexpr int oScale = oW + 2 * kWBytes;         // [ring][ks 4, log2 vs 4, have]
+  static constexpr int kScaleStride = 48;
+  static constexpr int oBar = oScale + kRing * kScaleStride;
+  static constexpr int kNumBars = 2 * kRing + 4 + 4 + 2 + 2 + 2 + 1;
+  static constexpr int oTmem = oBar + kNumBars * 8;
+  static constexpr int oAbort = oTmem + 4;
+  static constexpr int oScan = oAbort + 4;                // [16]
+  static constexpr int oPre = oScan + 64;                 // [B + 1]
+  static constexpr int bytes(int B) { return oPre + (B + 1) * 4 + 1024; }
+};
+
+SPATTEN_DEV void tmem_st32f(uint32_t taddr, const float* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]),
+      "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]),
+      "f"(r[19]), "f"(r[20]), "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]),
+      "f"(r[28]), "f"(r[29]), "f"(r[30]), "f"(r[31]));
+}
+SPATTEN_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Four codes in order as two f16 pairs.
+template <int KV>
+SPATTEN_DEV uint2 widen4(uint32_t w) {
+  if constexpr (KV == kKvInt8) {
+    const uint32_t x = w ^ 0x80808080u;  // byte u under 0x64 is the f16 1024 + u = 1152 + code
+    uint32_t lo = __byte_perm(x, 0x64646464u, 0x4140), hi = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 b = __half2half2(__ushort_as_half(0x6480));
+    const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), b);
+    const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&hi), b);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&c));
+  } else {
+    return make_uint2(e4m3x2_to_f16x2(w & 0xFFFFu), e4m3x2_to_f16x2(w >> 16));
+  }
+}
+
+// A CTA's run of units, as segments of lines. Every role walks it by itself.
+struct Segments {
+  const PagedAttendParams& p;
+  const uint32_t* pre;
+  uint32_t u, u1;
+  int b, R;
+  // the current segment
+  PagedSeq sq;
+  int g, r0, nrows, lim_max, t0, t1;
+  bool first, whole;     // begins the line; is all of it
+  uint32_t u0, line;     // the segment's first unit; units of the line
+
+  SPATTEN_DEV static uint32_t tokens_per_tile(int R) { return (kRowsCta + R - 1) / R; }
+  // units of row tiles 0 .. rt - 1 of a sequence
+  SPATTEN_DEV static uint32_t before(const PagedSeq& s, uint32_t rt, uint32_t tok) {
+    return rt * max(s.old, 0) + tok * (rt * (rt + 1) / 2);
+  }
+  SPATTEN_DEV static uint32_t row_tiles(const PagedSeq& s, int R) { return ((uint32_t)s.n * R + kRowsCta - 1) / kRowsCta; }
+  SPATTEN_DEV static uint32_t units(const PagedSeq& s, int R) {
+    return s.n > 0 ? before(s, row_tiles(s, R), tokens_per_tile(R)) : 0;
+  }
+
+  SPATTEN_DEV bool next() {
+    if (u >= u1) return false;
+    while (pre[b + 1] <= u) ++b;
+    sq = paged_seq(p.b, p.c, b);
+    const uint32_t tok = tokens_per_tile(R), per = units(sq, R), local = u - pre[b];
+    g = local / per;
+    const uint32_t r = local % per;
+    uint32_t lo = 0, hi = row_tiles(sq, R);  // the row tile of unit r
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) >> 1;
+      if (before(sq, mid, tok) <= r) lo = mid; else hi = mid;
+    }
+    const uint32_t v0 = r - before(sq, lo, tok);
+    u0 = u;
+    line = before(sq, lo + 1, tok) - before(sq, lo, tok);
+    const uint32_t v1 = min(line, v0 + (u1 - u));
+    first = v0 == 0;
+    whole = first && v1 == line;
+    r0 = lo * kRowsCta;
+    nrows = sq.n * R;
+    lim_max = max(min(sq.old + min((r0 + kRowsCta - 1) / R, sq.n - 1) + 1, sq.len), 0);
+    const int kt = (lim_max + kKeys - 1) / kKeys;
+    t0 = min((int)((v0 + kKeys - 1) / kKeys), kt);
+    t1 = v1 == line ? kt : min((int)((v1 + kKeys - 1) / kKeys), kt);
+    u += v1 - v0;
+    return true;
+  }
+};
+
+template <int KV, int D>
+__global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const PagedAttendParams p, const PagedPartials ws,
+                                                                      const bool bf16) {
+  using L = Lay<D>;
+  extern __shared__ uint8_t smem_raw[];
+  grid_dependents();
+  grid_wait();
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  const uint32_t bars = smem_u32(sm + L::oBar);
+  const SBarArr kv_full{bars}, kv_empty{bars + 8 * kRing}, s_full{bars + 16 * kRing}, s_empty{bars + 16 * kRing + 32},
+      w_full{bars + 16 * kRing + 64}, o_done{bars + 16 * kRing + 80}, q_full{bars + 16 * kRing + 96};
+  const SBar drain{bars + 16 * kRing + 112};
+  volatile int* abort = reinterpret_cast<volatile int*>(sm + L::oAbort);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + L::oTmem);
+  uint32_t* pre = reinterpret_cast<uint32_t*>(sm + L::oPre);
+  uint32_t* scan = reinterpret_cast<uint32_t*>(sm + L::oScan);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = p.c.G, R = p.b.H / G;
+
+  if (tid == 0) {
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(kv_full[i], kWideWarps);
+      mbar_init(kv_empty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {  // [row tile][buffer]
+      mbar_init(s_full[i], 1);
+      mbar_init(s_empty[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(w_full[i], 4);
+      mbar_init(o_done[i], 1);
+      mbar_init(q_full[i], 4);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+    *abort = 0;
+    pre[0] = 0;
+  }
+  if (warp == kSoftWarps + kWideWarps) {
+    tmem_alloc(tslot, 512);
+    tmem_relinquish();
+  }
+  // prefix sums of the sequences' units (the host made sure of 32 bits)
+  uint32_t U = 0;
+  for (int base = 0; base < p.b.B; base += kThreads) {
+    const int b = base + tid;
+    uint32_t x = 0;
+    if (b < p.b.B) x = (uint32_t)G * Segments::units(paged_seq(p.b, p.c, b), R);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) scan[warp] = x;
+    __syncthreads();
+    uint32_t front = U;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) front += scan[w];
+      U += scan[w];
+    }
+    if (b < p.b.B) pre[b + 1] = front + x;
+    __syncthreads();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tslot;
+  const uint32_t cta = blockIdx.x, ctas = max(min(gridDim.x, (U + kKeys - 1) / kKeys), 1u);
+  const uint32_t per = U / ctas, more = U % ctas;
+  Segments seg{p, pre};
+  seg.R = R;
+  seg.b = 0;
+  seg.u = seg.u1 = 0;
+  if (cta < ctas) {
+    seg.u = cta * per + min(cta, more);
+    seg.u1 = seg.u + per + (cta < more ? 1 : 0);
+  }
+
+  if (warp < kSoftWarps) {
+    // ------------------------------------------------------------ softmax
+    const int rt = warp >> 2, row = tid & 127;  // row tile, row in it = tensor-memory lane
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = tl + rt * 2 * kKeys, to = tl + 4 * kKeys + rt * D;
+    PagedCut cut = {};
+    uint32_t c = 0, kv = 0;  // tiles of this row tile, tiles of the ring
+    bool alive = true;
+    while (seg.next()) {
+      const int r = seg.r0 + rt * kRowTile + row;
+      const bool live = r < seg.nrows, used = seg.nrows - seg.r0 > rt * kRowTile;
+      const int nt = seg.t1 - seg.t0, i = (live ? r : 0) / R, h = seg.g * R + (live ? r : 0) % R;
+      // the row's query, scaled into f16, as the A operand
+      float cq = 0.f;
+      if (used && nt > 0) {
+        const uint16_t* qp = static_cast<const uint16_t*>(p.q) + (int64_t)(seg.sq.begin + i) * p.q_st + (int64_t)h * p.q_sh;
+        float top = 0.f;
+        uint4 x[D / 8];
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          x[k] = live ? *(reinterpret_cast<const uint4*>(qp) + k) : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 f;
+            if (bf16) f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+            else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+            if (!(f.x == f.x && f.y == f.y)) top = INFINITY;
+          }
+        }
+        const int e = top > 0.f ? 14 - max((int)(__float_as_uint(top) >> 23) - 127, -112) : 0;
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        cq = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23) * (top <= 3.4e38f ? 1.f : NAN);
+        uint8_t* dst = sm + L::oQ + rt * L::kQBytes + row * 128;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) {
+          const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float2 f;
+            if (bf16) f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+            else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            o[j] = pack2<__half>(f.x * up, f.y * up);
+          }
+          *reinterpret_cast<uint4*>(dst + (k >> 3) * (kRowTile * 128) + (((k & 7) ^ (row & 7)) << 4)) =
+              make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        mbar_arrive_elect(q_full[rt]);
+      }
+      const int lim = live ? min(seg.sq.old + i + 1, seg.sq.len) : 0;
+      float m = -INFINITY, M = -INFINITY, l = 0.f;
+      if (!used) kv += max(nt, 0);
+      for (int t = seg.t0; used && t < seg.t1; ++t, ++kv) {
+        const int st = kv % kRing, buf = c & 1;
+        bool ok = mbar_wait(s_full[2 * rt + buf], (c >> 1) & 1, kErr | 1, abort);
+        ok = ok && mbar_wait(kv_full[st], (kv / kRing) & 1, kErr | 2, abort);  // (long complete) the tile's scales
+        if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+        tc_fence_after();
+        float s[kKeys];
+        tmem_ld32f(ts + buf * kKeys, s);
+        tmem_ld32f(ts + buf * kKeys + 32, s + 32);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_elect(s_empty[2 * rt + buf]);
+        const float4 ks = *reinterpret_cast<const float4*>(sm + L::oScale + st * L::kScaleStride);
+        const float4 lv4 = *reinterpret_cast<const float4*>(sm + L::oScale + st * L::kScaleStride + 16);
+        const uint32_t have = *reinterpret_cast<const uint32_t*>(sm + L::oScale + st * L::kScaleStride + 32);
+        const float a[4] = {cq * ks.x, cq * ks.y, cq * ks.z, cq * ks.w}, lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w};
+        const int key0 = t * kKeys;
+#pragma unroll
+        for (int k = 0; k < kKeys; ++k) s[k] *= a[k >> 4];
+        if (__any_sync(0xffffffffu, key0 + kKeys > lim) || have != 15u) {
+#pragma unroll
+          for (int k = 0; k < kKeys; ++k)
+            if (key0 + k >= lim || !((have >> (k >> 4)) & 1u)) s[k] = -INFINITY;
+        }
+        float top = -INFINITY, topw = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float x = s[16 * q];
+#pragma unroll
+          for (int k = 1; k < 16; ++k) x = fmaxf(x, s[16 * q + k]);
+          top = fmaxf(top, x);
+          topw = fmaxf(topw, x + lv[q]);
+        }
+        const bool up = top > m + kSlack || topw > M + kSlack;
+        const float Mn = up ? fmaxf(M, topw) : M, mn = up ? fmaxf(m, top) : m;
+        const float Mf = Mn == -INFINITY ? 0.f : Mn, mf = mn == -INFINITY ? 0.f : mn;
+        if (up) l *= fast_exp2(m - mf);
+        const float fo = up ? fast_exp2(M - Mf) : 1.f;
+        m = mn;
+        M = Mn;
+        uint32_t w[kKeys / 2];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float shift = lv[q] - Mf, e = Mf - lv[q] - mf;
+          float sum = 0.f, psum = 0.f;
+          const bool wide = e > 90.f;  // w may underflow where p does not
+          if (__any_sync(0xffffffffu, wide)) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) psum += fast_exp2(s[16 * q + k] - mf);
+          }
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) {
+            const float x = fast_exp2(s[16 * q + k] + shift), y = fast_exp2(s[16 * q + k + 1] + shift);
+            sum += x + y;
+            w[8 * q + (k >> 1)] = pack2<__half>(x, y);
+          }
+          l += wide ? psum : sum * fast_exp2(e);
+        }
+        // W and O are free once the MMA of the tile before is done
+        if (c > 0) {
+          ok = mbar_wait(o_done[rt], (c - 1) & 1, kErr | 3, abort);
+          if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+          tc_fence_after();
+        }
+        if (t > seg.t0 && __any_sync(0xffffffffu, fo != 1.f)) {
+#pragma unroll
+          for (int k = 0; k < D / 32; ++k) {
+            float o[32];
+            tmem_ld32f(to + 32 * k, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] *= fo;
+            tmem_st32f(to + 32 * k, o);
+          }
+          tmem_wait_st();
+        }
+        uint8_t* dst = sm + L::oW + rt * L::kWBytes + row * 128;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          *reinterpret_cast<uint4*>(dst + ((k ^ (row & 7)) << 4)) =
+              make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_elect(w_full[rt]);
+        ++c;
+      }
+      // epilogue: the row's O
+      if (used && nt > 0 && alive) {
+        const bool ok = mbar_wait(o_done[rt], (c - 1) & 1, kErr | 4, abort);
+        if (!__all_sync(0xffffffffu, ok)) alive = false;
+        tc_fence_after();
+      }
+      if (!alive) break;
+      if (used) {
+        const float inv = seg.whole ? paged_normaliser(m, l, M) : 1.f;
+        const uint32_t prow = (2 * cta + (seg.first ? 1 : 0)) * kRowsCta + rt * kRowTile + row;
+        uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(seg.sq.begin + i) * p.o_st + (int64_t)h * p.o_sh;
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          float o[32];
+          __syncwarp();
+          if (nt > 0) {
+            tmem_ld32f(to + 32 * k, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0.f;
+          }
+          if (!live) continue;
+          if (seg.whole) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              uint32_t x[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                x[q] = bf16 ? pack2<__nv_bfloat16>(o[j + 2 * q] * inv, o[j + 2 * q + 1] * inv)
+                            : pack2<__half>(o[j + 2 * q] * inv, o[j + 2 * q + 1] * inv);
+              *reinterpret_cast<uint4*>(op + 32 * k + j) = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<float4*>(ws.o + (size_t)prow * D + 32 * k + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+        }
+        if (live && !seg.whole) ws.ml[prow] = make_float4(m, l, M, 0.f);
+        tc_fence_before();
+      }
+      if (seg.first && !seg.whole) {  // the CTAs up to that of the line's last unit hold a part each
+        const uint32_t last = seg.u0 + seg.line - 1, big = more * (per + 1);
+        cut.parts = (int)(last < big ? last / (per + 1) : more + (last - big) / per) - (int)cta + 1;
+        cut.row0 = seg.r0; cut.nrows = seg.nrows; cut.begin = seg.sq.begin; cut.g = seg.g;
+      }
+    }
+    if (tid == 0) ws.cut[cta] = cut;
+  } else if (warp < kSoftWarps + kWideWarps) {
+    // ------------------------------------------------------------ codes to f16
+    constexpr int CH = D / 16, NC = D / 32, RPI = 128 / CH;  // chunks per key, chunks per thread of K (and V), keys per step
+    const int w = tid - 32 * kSoftWarps, col = w % CH, key = w / CH;
+    const int page_log = __ffs(p.c.page) - 1;
+    int t = 0;
+    bool more_tiles = true;
+    int pid[NC], pid_s = -1;  // pages of this thread's keys, and of block w & 3, of the tile to load next
+    auto pages = [&]() {
+      auto page_of = [&](int slot) { return slot < seg.lim_max ? paged_page(p.c, seg.b, slot >> page_log) : -1; };
+#pragma unroll
+      for (int i = 0; i < NC; ++i) pid[i] = page_of(t * kKeys + key + RPI * i);
+      pid_s = page_of(t * kKeys + 16 * (w & 3));
+    };
+    auto advance = [&]() {
+      ++t;
+      while (more_tiles && t >= seg.t1) {
+        more_tiles = seg.next();
+        t = seg.t0;
+      }
+      if (more_tiles) pages();
+    };
+    struct Hold {
+      uint4 k[NC], v[NC];
+      float ks, vs;
+      uint32_t have;
+      bool valid;
+    };
+    auto load = [&](Hold& x) {
+      x.valid = more_tiles;
+      if (!more_tiles) return;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int slot = t * kKeys + key + RPI * i;
+        const int64_t at =
+            (((int64_t)max(pid[i], 0) * G + seg.g) * p.c.page + (slot & (p.c.page - 1))) * D + col * 16;
+        x.k[i] = x.v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (pid[i] >= 0) x.k[i] = *reinterpret_cast<const uint4*>(p.c.k + at);
+        if (pid[i] >= 0 && slot < seg.lim_max) x.v[i] = *reinterpret_cast<const uint4*>(p.c.v + at);
+      }
+      x.ks = x.vs = 0.f;
+      if (w < 4 && pid_s >= 0) {
+        const int64_t blk = (int64_t)pid_s * G + seg.g;
+        x.ks = p.c.k_scale[blk];
+        x.vs = p.c.v_scale[blk];
+      }
+      x.have = __ballot_sync(0xffffffffu, pid_s >= 0) & 15u;
+      advance();
+    };
+    uint32_t n = 0;
+    auto store = [&](const Hold& x) {
+      const int st = n % kRing;
+      const bool ok = mbar_wait(kv_empty[st], ((n / kRing) & 1) ^ 1, kErr | 5, abort);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      uint8_t* kd = sm + L::oKV + st * 2 * L::kTileBytes + (col >> 2) * (kKeys * 128);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int row = key + RPI * i;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const uint4 c = v ? x.v[i] : x.k[i];
+          const uint2 a = widen4<KV>(c.x), b = widen4<KV>(c.y), d = widen4<KV>(c.z), e = widen4<KV>(c.w);
+          uint8_t* dst = kd + v * L::kTileBytes + row * 128;
+          const int sub = (col & 3) * 2;
+          *reinterpret_cast<uint4*>(dst + ((sub ^ (row & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+          *reinterpret_cast<uint4*>(dst + (((sub + 1) ^ (row & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
+        }
+      }
+      if (w < 4) {
+        float* sc = reinterpret_cast<float*>(sm + L::oScale + st * L::kScaleStride);
+        sc[w] = x.ks;
+        sc[4 + w] = x.vs > 0.f ? fmaxf(log2f(x.vs), kNoScale) : kNoScale;
+        if (w == 0) reinterpret_cast<uint32_t*>(sc)[8] = x.have;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      mbar_arrive_elect(kv_full[st]);
+      ++n;
+      return true;
+    };
+    t = -1;
+    seg.t1 = 0;  // before the first segment
+    advance();
+    Hold x, y;
+    load(x);
+    load(y);
+    while (true) {
+      if (!x.valid || !store(x)) break;
+      load(x);
+      if (!y.valid || !store(y)) break;
+      load(y);
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------ MMA issue
+    constexpr uint32_t idesc_s = instr_desc(1, 0, 0, 0, kRowTile, kKeys), idesc_o = instr_desc(1, 0, 0, 1, kRowTile, D);
+    const uint32_t qa = smem_u32(sm + L::oQ), wa = smem_u32(sm + L::oW);
+    uint32_t n = 0, c[2] = {0, 0}, nq[2] = {0, 0};
+    bool ok = true;
+    while (ok && seg.next()) {
+      const int nt = seg.t1 - seg.t0, tiles = seg.nrows - seg.r0 > kRowTile ? 2 : 1;
+      if (nt <= 0) continue;
+      for (int rt = 0; rt < tiles && ok; ++rt) ok = mbar_wait(q_full[rt], nq[rt]++ & 1, kErr | 6, abort);
+      for (int j = 0; j <= nt && ok; ++j) {
+        if (j < nt) {
+          const uint32_t g = n + j;
+          ok = mbar_wait(kv_full[g % kRing], (g / kRing) & 1, kErr | 7, abort);
+          const uint32_t ka = smem_u32(sm + L::oKV + (g % kRing) * 2 * L::kTileBytes);
+          for (int rt = 0; rt < tiles && ok; ++rt) {
+            const uint32_t x = c[rt] + j, buf = x & 1;
+            ok = mbar_wait(s_empty[2 * rt + buf], ((x >> 1) & 1) ^ 1, kErr | 8, abort);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              mma_f16(tmem + (2 * rt + buf) * kKeys,
+                      smem_desc_sw128(qa + rt * L::kQBytes + (k >> 2) * (kRowTile * 128) + (k & 3) * 32, 16, 1024),
+                      smem_desc_sw128(ka + (k >> 2) * (kKeys * 128) + (k & 3) * 32, 16, 1024), idesc_s, k > 0);
+            mma_commit(s_full[2 * rt + buf]);
+          }
+        }
+        if (j >= 1 && ok) {
+          const uint32_t g = n + j - 1;
+          const uint32_t va = smem_u32(sm + L::oKV + (g % kRing) * 2 * L::kTileBytes + L::kTileBytes);
+          for (int rt = 0; rt < tiles && ok; ++rt) {
+            ok = mbar_wait(w_full[rt], (c[rt] + j - 1) & 1, kErr | 9, abort);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              mma_f16(tmem + 4 * kKeys + rt * D, smem_desc_sw128(wa + rt * L::kWBytes + k * 32, 16, 1024),
+                      smem_desc_sw128(va + k * 2048, kKeys * 128, 1024), idesc_o, j > 1 || k > 0);
+            mma_commit(o_done[rt]);
+          }
+          if (ok) mma_commit(kv_empty[g % kRing]);
+        }
+      }
+      n += nt;
+      for (int rt = 0; rt < tiles; ++rt) c[rt] += nt;
+    }
+    // every MMA issued has completed before the tensor memory is freed
+    mma_commit(drain);
+    const long long start = clock64();
+    while (!mbar_try_wait(drain, 0) && clock64() - start < kWaitLimitCycles) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftWarps + kWideWarps) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int KV, int D>
+cudaError_t tc_launch(const PagedAttendParams& p, bool bf16, const PagedPartials& ws, int ctas, cudaStream_t st) {
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
+    e = cudaFuncSetAttribute(paged_attend_tc_kernel<KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Lay<D>::bytes(kMaxBatch));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  e = launch_dependent(paged_attend_tc_kernel<KV, D>, dim3(ctas), kThreads, Lay<D>::bytes(p.b.B), st, p, ws, bf16);
+  if (e != cudaSuccess) return e;
+  return launch_paged_join<D, kRowsCta>(p, ws, ctas, bf16, st);
+}
+
+}  // namespace
+
+// 64 rows per KV head and more: below, most of a row tile would be padding.
+bool paged_attend_tc_takes(const PagedAttendParams& p) {
+  const int R = p.b.H / p.c.G;
+  if ((int64_t)p.b.max_tokens * R < 64 || p.b.B > kMaxBatch) return false;
+  const double lines = (double)p.b.T * R / kRowsCta + p.b.B;  // at most
+  return lines * p.c.G * ((double)p.c.max_pages * p.c.page + kRowsCta) < 4e9;
+}
+
+size_t paged_attend_tc_workspace(const PagedAttendParams& p, int n_sm) {
+  return paged_partials_bytes(n_sm, kRowsCta, p.c.D);
+}
+
+cudaError_t launch_paged_attend_tc(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,
+                                   cudaStream_t st) {
+  const PagedPartials s = paged_partials(ws, n_sm, kRowsCta);
+  const bool bf16 = dtype == kBF16;
+  if (p.c.D == 128)
+    return kv == kKvInt8 ? tc_launch<kKvInt8, 128>(p, bf16, s, n_sm, st) : tc_launch<kKvE4m3, 128>(p, bf16, s, n_sm, st);
+  if (p.c.D == 64)
+    return kv == kKvInt8 ? tc_launch<kKvInt8, 64>(p, bf16, s, n_sm, st) : tc_launch<kKvE4m3, 64>(p, bf16, s, n_sm, st);
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t read_paged_device_error(unsigned int* code, bool reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(code, sm100::g_device_error, sizeof(unsigned int));
+  if (e != cudaSuccess || !reset) return e;
+  const unsigned int zero = 0;
+  return cudaMemcpyToSymbol(sm100::g_device_error, &zero, sizeof(unsigned int));
+}
+
+}  // namespace spatten
