@@ -245,17 +245,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
       float cq = 0.f;
       if (used && nt > 0) {
         const uint16_t* qp = static_cast<const uint16_t*>(p.q) + (int64_t)(seg.sq.begin + i) * p.q_st + (int64_t)h * p.q_sh;
+        // twice over the row (the second time from L1), to keep the loop's registers and code small
         float top = 0.f;
-        uint4 x[D / 8];
-#pragma unroll
+        auto pair = [&](uint32_t w) {
+          return bf16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u))
+                      : __half22float2(*reinterpret_cast<const __half2*>(&w));
+        };
+#pragma unroll 4
         for (int k = 0; k < D / 8; ++k) {
-          x[k] = live ? *(reinterpret_cast<const uint4*>(qp) + k) : make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+          const uint4 x = live ? *(reinterpret_cast<const uint4*>(qp) + k) : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float2 f;
-            if (bf16) f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
-            else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            const float2 f = pair(w[j]);
             top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
             if (!(f.x == f.x && f.y == f.y)) top = INFINITY;
           }
@@ -264,15 +266,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
         cq = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23) * (top <= 3.4e38f ? 1.f : NAN);
         uint8_t* dst = sm + L::oQ + rt * L::kQBytes + row * 128;
-#pragma unroll
+#pragma unroll 4
         for (int k = 0; k < D / 8; ++k) {
-          const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+          const uint4 x = live ? *(reinterpret_cast<const uint4*>(qp) + k) : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
           uint32_t o[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float2 f;
-            if (bf16) f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
-            else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            const float2 f = pair(w[j]);
             o[j] = pack2<__half>(f.x * up, f.y * up);
           }
           *reinterpret_cast<uint4*>(dst + (k >> 3) * (kRowTile * 128) + (((k & 7) ^ (row & 7)) << 4)) =
@@ -301,48 +302,68 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         const float4 ks = *reinterpret_cast<const float4*>(sm + L::oScale + st * L::kScaleStride);
         const float4 lv4 = *reinterpret_cast<const float4*>(sm + L::oScale + st * L::kScaleStride + 16);
         const uint32_t have = *reinterpret_cast<const uint32_t*>(sm + L::oScale + st * L::kScaleStride + 32);
-        const float a[4] = {cq * ks.x, cq * ks.y, cq * ks.z, cq * ks.w}, lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w};
+        float a[4] = {cq * ks.x, cq * ks.y, cq * ks.z, cq * ks.w};
+        const float lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w};
         const int key0 = t * kKeys;
+        const bool odd = key0 + kKeys > lim || have != 15u || !(fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) >= 0.f);
+        if (__builtin_expect(__any_sync(0xffffffffu, odd), 0)) {  // masked keys, factors below 0 or NaN: t itself
 #pragma unroll
-        for (int k = 0; k < kKeys; ++k) s[k] *= a[k >> 4];
-        if (__any_sync(0xffffffffu, key0 + kKeys > lim) || have != 15u) {
-#pragma unroll
-          for (int k = 0; k < kKeys; ++k)
+          for (int k = 0; k < kKeys; ++k) {
+            s[k] *= a[k >> 4];
             if (key0 + k >= lim || !((have >> (k >> 4)) & 1u)) s[k] = -INFINITY;
+          }
+          a[0] = a[1] = a[2] = a[3] = 1.f;
         }
         float top = -INFINITY, topw = -INFINITY;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float x = s[16 * q];
+          float x = s[16 * q], y = s[16 * q + 1];
 #pragma unroll
-          for (int k = 1; k < 16; ++k) x = fmaxf(x, s[16 * q + k]);
+          for (int k = 2; k < 16; k += 2) {
+            x = fmaxf(x, s[16 * q + k]);
+            y = fmaxf(y, s[16 * q + k + 1]);
+          }
+          x = fmaxf(x, y) * a[q];
           top = fmaxf(top, x);
           topw = fmaxf(topw, x + lv[q]);
         }
         const bool up = top > m + kSlack || topw > M + kSlack;
         const float Mn = up ? fmaxf(M, topw) : M, mn = up ? fmaxf(m, top) : m;
-        const float Mf = Mn == -INFINITY ? 0.f : Mn, mf = mn == -INFINITY ? 0.f : mn;
+        const float Mf = finite_or_0(Mn), mf = finite_or_0(mn);
         if (up) l *= fast_exp2(m - mf);
         const float fo = up ? fast_exp2(M - Mf) : 1.f;
         m = mn;
         M = Mn;
-        uint32_t w[kKeys / 2];
+        // w underflows where p does not: the sum of p itself
+        float e[4], psum = 0.f;
+        bool wide = false;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float shift = lv[q] - Mf, e = Mf - lv[q] - mf;
-          float sum = 0.f, psum = 0.f;
-          const bool wide = e > 90.f;  // w may underflow where p does not
-          if (__any_sync(0xffffffffu, wide)) {
+          e[q] = Mf - lv[q] - mf;
+          wide |= e[q] > 90.f;
+        }
+        if (__builtin_expect(__any_sync(0xffffffffu, wide), 0)) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) psum += fast_exp2(s[16 * q + k] - mf);
+          for (int k = 0; k < kKeys; ++k) {
+            const float x = fast_exp2(fmaf(s[k], a[k >> 4], -mf));
+            psum += e[k >> 4] > 90.f ? x : 0.f;
           }
+        }
+        uint32_t w[kKeys / 2];
+        l += psum;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 a2 = make_float2(a[q], a[q]), b2 = make_float2(lv[q] - Mf, lv[q] - Mf);
+          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int k = 0; k < 16; k += 2) {
-            const float x = fast_exp2(s[16 * q + k] + shift), y = fast_exp2(s[16 * q + k + 1] + shift);
-            sum += x + y;
-            w[8 * q + (k >> 1)] = pack2<__half>(x, y);
+            float2 x = __ffma2_rn(make_float2(s[16 * q + k], s[16 * q + k + 1]), a2, b2);
+            x.x = fast_exp2(x.x);
+            x.y = fast_exp2(x.y);
+            sum = __fadd2_rn(sum, x);
+            w[8 * q + (k >> 1)] = pack2<__half>(x.x, x.y);
           }
-          l += wide ? psum : sum * fast_exp2(e);
+          l += e[q] > 90.f ? 0.f : (sum.x + sum.y) * fast_exp2(e[q]);
         }
         // W and O are free once the MMA of the tile before is done
         if (c > 0) {
@@ -351,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
           tc_fence_after();
         }
         if (t > seg.t0 && __any_sync(0xffffffffu, fo != 1.f)) {
-#pragma unroll
+#pragma unroll 1
           for (int k = 0; k < D / 32; ++k) {
             float o[32];
             tmem_ld32f(to + 32 * k, o);
@@ -384,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         const float inv = seg.whole ? paged_normaliser(m, l, M) : 1.f;
         const uint32_t prow = (2 * cta + (seg.first ? 1 : 0)) * kRowsCta + rt * kRowTile + row;
         uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(seg.sq.begin + i) * p.o_st + (int64_t)h * p.o_sh;
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < D / 32; ++k) {
           float o[32];
           __syncwarp();
@@ -485,9 +506,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
           const uint4 c = v ? x.v[i] : x.k[i];
           const uint2 a = widen4<KV>(c.x), b = widen4<KV>(c.y), d = widen4<KV>(c.z), e = widen4<KV>(c.w);
           uint8_t* dst = kd + v * L::kTileBytes + row * 128;
-          const int sub = (col & 3) * 2;
-          *reinterpret_cast<uint4*>(dst + ((sub ^ (row & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
-          *reinterpret_cast<uint4*>(dst + (((sub + 1) ^ (row & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
+          // the lanes of the second 64-dim block take their halves the other way round: other banks
+          const bool odd = (col >> 2) & 1;
+          const int sub = (col & 3) * 2 + odd;
+          const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(d.x, d.y, e.x, e.y);
+          *reinterpret_cast<uint4*>(dst + ((sub ^ (row & 7)) << 4)) = odd ? hi : lo;
+          *reinterpret_cast<uint4*>(dst + (((sub ^ 1) ^ (row & 7)) << 4)) = odd ? lo : hi;
         }
       }
       if (w < 4) {
