@@ -16,14 +16,15 @@
 // of w times it (one exponential per score), except where w could underflow
 // under it, which takes the exponentials of p.
 //
-// 13 warps, one CTA per SM:
+// 16 warps, one CTA per SM:
 //   warps 0-3, 4-7  softmax of the two row tiles: S from tensor memory, W into
 //                   shared memory (swizzled), rescaling, the epilogue and the
 //                   next queries;
 //   warps 8-11      codes to f16: 16-byte loads two tiles ahead, widened into a
 //                   ring of K / V tiles in the layouts that the MMAs read (K
 //                   K-major, V MN-major: both [64-dim block][key][128 B]);
-//   warp 12         MMA issue: S of tile j + 1 before O of tile j.
+//   warps 12-15     MMA issue, one thread each: S and O of the two row tiles (one
+//                   thread for all took 3600 of a tile's 4450 cycles).
 // A tile's codes are widened once for 256 rows, and two row tiles keep the
 // tensor cores busy through each other's softmax. What bounds it: shared-memory
 // traffic of the operands (a 128 x 64 x 16 step reads 6 KB) and the softmax's
@@ -48,7 +49,8 @@ namespace {
 using namespace sm100;
 
 constexpr int kRowTile = 128, kRowsCta = 256, kKeys = 64, kRing = 3;
-constexpr int kSoftWarps = 8, kWideWarps = 4, kThreads = 32 * (kSoftWarps + kWideWarps + 1);
+constexpr int kSoftWarps = 8, kWideWarps = 4, kMmaWarps = 4,
+              kThreads = 32 * (kSoftWarps + kWideWarps + kMmaWarps);
 constexpr float kSlack = 8.f;
 constexpr float kNoScale = -200.f;  // log2 of a scale of 0
 constexpr unsigned kErr = 0x400;
@@ -65,7 +67,7 @@ struct Lay {
   static constexpr int oScale = oW + 2 * kWBytes;         // [ring][ks 4, log2 vs 4, have]
   static constexpr int kScaleStride = 48;
   static constexpr int oBar = oScale + kRing * kScaleStride;
-  static constexpr int kNumBars = 2 * kRing + 4 + 4 + 2 + 2 + 2 + 1;
+  static constexpr int kNumBars = 2 * kRing + 4 + 4 + 2 + 2 + 2 + 4;
   static constexpr int oTmem = oBar + kNumBars * 8;
   static constexpr int oAbort = oTmem + 4;
   static constexpr int oScan = oAbort + 4;                // [16]
@@ -161,8 +163,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
   uint8_t* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const uint32_t bars = smem_u32(sm + L::oBar);
   const SBarArr kv_full{bars}, kv_empty{bars + 8 * kRing}, s_full{bars + 16 * kRing}, s_empty{bars + 16 * kRing + 32},
-      w_full{bars + 16 * kRing + 64}, o_done{bars + 16 * kRing + 80}, q_full{bars + 16 * kRing + 96};
-  const SBar drain{bars + 16 * kRing + 112};
+      w_full{bars + 16 * kRing + 64}, o_done{bars + 16 * kRing + 80}, q_full{bars + 16 * kRing + 96},
+      drain{bars + 16 * kRing + 112};
   volatile int* abort = reinterpret_cast<volatile int*>(sm + L::oAbort);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + L::oTmem);
   uint32_t* pre = reinterpret_cast<uint32_t*>(sm + L::oPre);
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
   if (tid == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(kv_full[i], kWideWarps);
-      mbar_init(kv_empty[i], 1);
+      mbar_init(kv_empty[i], 2);  // the two row tiles
     }
     for (int i = 0; i < 4; ++i) {  // [row tile][buffer]
       mbar_init(s_full[i], 1);
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
       mbar_init(o_done[i], 1);
       mbar_init(q_full[i], 4);
     }
-    mbar_init(drain, 1);
+    for (int i = 0; i < kMmaWarps; ++i) mbar_init(drain[i], 1);
     fence_barrier_init();
     *abort = 0;
     pre[0] = 0;
@@ -540,55 +542,67 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
     }
   } else if (lane == 0) {
     // ------------------------------------------------------------ MMA issue
-    constexpr uint32_t idesc_s = instr_desc(1, 0, 0, 0, kRowTile, kKeys), idesc_o = instr_desc(1, 0, 0, 1, kRowTile, D);
-    const uint32_t qa = smem_u32(sm + L::oQ), wa = smem_u32(sm + L::oW);
-    uint32_t n = 0, c[2] = {0, 0}, nq[2] = {0, 0};
+    const int rt = (warp - kSoftWarps - kWideWarps) & 1;
+    const bool scores = warp < kSoftWarps + kWideWarps + 2;
+    uint32_t n = 0, c = 0, nq = 0;  // tiles of the ring, tiles and queries of this row tile
     bool ok = true;
-    while (ok && seg.next()) {
-      const int nt = seg.t1 - seg.t0, tiles = seg.nrows - seg.r0 > kRowTile ? 2 : 1;
-      if (nt <= 0) continue;
-      for (int rt = 0; rt < tiles && ok; ++rt) ok = mbar_wait(q_full[rt], nq[rt]++ & 1, kErr | 6, abort);
-      for (int j = 0; j <= nt && ok; ++j) {
-        if (j < nt) {
-          const uint32_t g = n + j;
-          ok = mbar_wait(kv_full[g % kRing], (g / kRing) & 1, kErr | 7, abort);
-          const uint32_t ka = smem_u32(sm + L::oKV + (g % kRing) * 2 * L::kTileBytes);
-          for (int rt = 0; rt < tiles && ok; ++rt) {
-            const uint32_t x = c[rt] + j, buf = x & 1;
-            ok = mbar_wait(s_empty[2 * rt + buf], ((x >> 1) & 1) ^ 1, kErr | 8, abort);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              mma_f16(tmem + (2 * rt + buf) * kKeys,
-                      smem_desc_sw128(qa + rt * L::kQBytes + (k >> 2) * (kRowTile * 128) + (k & 3) * 32, 16, 1024),
-                      smem_desc_sw128(ka + (k >> 2) * (kKeys * 128) + (k & 3) * 32, 16, 1024), idesc_s, k > 0);
-            mma_commit(s_full[2 * rt + buf]);
-          }
+    if (scores) {  // S = Q' K^T
+      constexpr uint32_t idesc = instr_desc(1, 0, 0, 0, kRowTile, kKeys);
+      const uint64_t q = smem_desc_sw128(smem_u32(sm + L::oQ + rt * L::kQBytes), 16, 1024);
+      while (ok && seg.next()) {
+        const int nt = seg.t1 - seg.t0;
+        if (nt <= 0) continue;
+        if (seg.nrows - seg.r0 <= rt * kRowTile) {
+          n += nt;
+          continue;
         }
-        if (j >= 1 && ok) {
-          const uint32_t g = n + j - 1;
-          const uint32_t va = smem_u32(sm + L::oKV + (g % kRing) * 2 * L::kTileBytes + L::kTileBytes);
-          for (int rt = 0; rt < tiles && ok; ++rt) {
-            ok = mbar_wait(w_full[rt], (c[rt] + j - 1) & 1, kErr | 9, abort);
-            if (!ok) break;
-            tc_fence_after();
+        ok = mbar_wait(q_full[rt], nq++ & 1, kErr | 6, abort);
+        for (int j = 0; j < nt && ok; ++j, ++n, ++c) {
+          const uint32_t st = n % kRing, buf = c & 1;
+          ok = mbar_wait(s_empty[2 * rt + buf], ((c >> 1) & 1) ^ 1, kErr | 8, abort) &&
+               mbar_wait(kv_full[st], (n / kRing) & 1, kErr | 7, abort);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t k = smem_desc_sw128(smem_u32(sm + L::oKV + st * 2 * L::kTileBytes), 16, 1024);
+          const uint32_t d = tmem + (2 * rt + buf) * kKeys;
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              mma_f16(tmem + 4 * kKeys + rt * D, smem_desc_sw128(wa + rt * L::kWBytes + k * 32, 16, 1024),
-                      smem_desc_sw128(va + k * 2048, kKeys * 128, 1024), idesc_o, j > 1 || k > 0);
-            mma_commit(o_done[rt]);
-          }
-          if (ok) mma_commit(kv_empty[g % kRing]);
+          for (int i = 0; i < D / 16; ++i)  // the descriptors' addresses count 16 bytes
+            mma_f16(d, q + (((i >> 2) * (kRowTile * 128) + (i & 3) * 32) >> 4),
+                    k + (((i >> 2) * (kKeys * 128) + (i & 3) * 32) >> 4), idesc, i > 0);
+          mma_commit(s_full[2 * rt + buf]);
         }
       }
-      n += nt;
-      for (int rt = 0; rt < tiles; ++rt) c[rt] += nt;
+    } else {  // O += W V
+      constexpr uint32_t idesc = instr_desc(1, 0, 0, 1, kRowTile, D);
+      const uint64_t a = smem_desc_sw128(smem_u32(sm + L::oW + rt * L::kWBytes), 16, 1024);
+      const uint32_t d = tmem + 4 * kKeys + rt * D;
+      while (ok && seg.next()) {
+        const int nt = seg.t1 - seg.t0;
+        const bool used = seg.nrows - seg.r0 > rt * kRowTile;
+        for (int j = 0; j < nt && ok; ++j, ++n) {
+          const uint32_t st = n % kRing;
+          ok = mbar_wait(kv_full[st], (n / kRing) & 1, kErr | 7, abort);
+          if (!ok) break;
+          if (!used) {  // (after the stage was filled: an arrival counts for its own phase)
+            mbar_arrive(kv_empty[st]);
+            continue;
+          }
+          ok = mbar_wait(w_full[rt], c & 1, kErr | 9, abort);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t v = smem_desc_sw128(smem_u32(sm + L::oKV + st * 2 * L::kTileBytes + L::kTileBytes), kKeys * 128, 1024);
+#pragma unroll
+          for (int i = 0; i < kKeys / 16; ++i) mma_f16(d, a + ((i * 32) >> 4), v + ((i * 2048) >> 4), idesc, j > 0 || i > 0);
+          mma_commit(o_done[rt]);
+          mma_commit(kv_empty[st]);
+          ++c;
+        }
+      }
     }
     // every MMA issued has completed before the tensor memory is freed
-    mma_commit(drain);
+    mma_commit(drain[2 * rt + (scores ? 0 : 1)]);
     const long long start = clock64();
-    while (!mbar_try_wait(drain, 0) && clock64() - start < kWaitLimitCycles) {
+    while (!mbar_try_wait(drain[2 * rt + (scores ? 0 : 1)], 0) && clock64() - start < kWaitLimitCycles) {
     }
   }
   tc_fence_before();
