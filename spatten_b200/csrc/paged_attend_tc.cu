@@ -448,7 +448,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
   } else if (warp < kSoftWarps + kWideWarps) {
     // ------------------------------------------------------------ codes to f16
     constexpr int CH = D / 16, NC = D / 32, RPI = 128 / CH;  // chunks per key, chunks per thread of K (and V), keys per step
-    const int w = tid - 32 * kSoftWarps, col = w % CH, key = w / CH;
+    // eight lanes of a store hold four 16-dim columns of two neighbouring keys: eight banks' worth
+    const int w = tid - 32 * kSoftWarps;
+    const int col = CH == 8 ? (w & 3) + ((w >> 1) & 4) : w & 3;
+    const int key = CH == 8 ? ((w >> 2) & 1) + 2 * (w >> 4) : w >> 2;
     const int page_log = __ffs(p.c.page) - 1;
     int t = 0;
     bool more_tiles = true;
@@ -508,12 +511,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
           const uint4 c = v ? x.v[i] : x.k[i];
           const uint2 a = widen4<KV>(c.x), b = widen4<KV>(c.y), d = widen4<KV>(c.z), e = widen4<KV>(c.w);
           uint8_t* dst = kd + v * L::kTileBytes + row * 128;
-          // the lanes of the second 64-dim block take their halves the other way round: other banks
-          const bool odd = (col >> 2) & 1;
-          const int sub = (col & 3) * 2 + odd;
-          const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(d.x, d.y, e.x, e.y);
-          *reinterpret_cast<uint4*>(dst + ((sub ^ (row & 7)) << 4)) = odd ? hi : lo;
-          *reinterpret_cast<uint4*>(dst + (((sub ^ 1) ^ (row & 7)) << 4)) = odd ? lo : hi;
+          const int sub = (col & 3) * 2;
+          *reinterpret_cast<uint4*>(dst + ((sub ^ (row & 7)) << 4)) = make_uint4(a.x, a.y, b.x, b.y);
+          *reinterpret_cast<uint4*>(dst + (((sub + 1) ^ (row & 7)) << 4)) = make_uint4(d.x, d.y, e.x, e.y);
         }
       }
       if (w < 4) {
