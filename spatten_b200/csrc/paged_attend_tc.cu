@@ -49,8 +49,13 @@ namespace {
 using namespace sm100;
 
 constexpr int kRowTile = 128, kRowsCta = 256, kKeys = 64, kRing = 3;
-constexpr int kSoftWarps = 8, kWideWarps = 4, kMmaWarps = 4,
+constexpr int kSoftWarps = 8, kWideWarps = 8, kMmaWarps = 4,
               kThreads = 32 * (kSoftWarps + kWideWarps + kMmaWarps);
+// registers per thread at launch, and of each role after setmaxnreg
+constexpr int kRegs = 96, kSoftRegs = 136, kWideRegs = 72, kMmaRegs = 64;
+static_assert(kSoftWarps * kSoftRegs + kWideWarps * kWideRegs + kMmaWarps * kMmaRegs ==
+                  (kSoftWarps + kWideWarps + kMmaWarps) * kRegs,
+              "the roles share what the block was launched with");
 constexpr float kSlack = 8.f;
 constexpr float kNoScale = -200.f;  // log2 of a scale of 0
 constexpr unsigned kErr = 0x400;
@@ -70,8 +75,8 @@ struct Lay {
   static constexpr int kNumBars = 2 * kRing + 4 + 4 + 2 + 2 + 2 + 4;
   static constexpr int oTmem = oBar + kNumBars * 8;
   static constexpr int oAbort = oTmem + 4;
-  static constexpr int oScan = oAbort + 4;                // [16]
-  static constexpr int oPre = oScan + 64;                 // [B + 1]
+  static constexpr int oScan = oAbort + 4;                // [32]
+  static constexpr int oPre = oScan + 128;                // [B + 1]
   static constexpr int bytes(int B) { return oPre + (B + 1) * 4 + 1024; }
 };
 
@@ -233,6 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
 
   if (warp < kSoftWarps) {
     // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs) : "memory");
     const int rt = warp >> 2, row = tid & 127;  // row tile, row in it = tensor-memory lane
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t ts = tl + rt * 2 * kKeys, to = tl + 4 * kKeys + rt * D;
@@ -447,7 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
     if (tid == 0) ws.cut[cta] = cut;
   } else if (warp < kSoftWarps + kWideWarps) {
     // ------------------------------------------------------------ codes to f16
-    constexpr int CH = D / 16, NC = D / 32, RPI = 128 / CH;  // chunks per key, chunks per thread of K (and V), keys per step
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideRegs) : "memory");
+    constexpr int CH = D / 16, NC = D / 64, RPI = 32 * kWideWarps / CH;  // chunks per key, chunks per thread of K (and V), keys per step
     // eight lanes of a store hold four 16-dim columns of two neighbouring keys: eight banks' worth
     const int w = tid - 32 * kSoftWarps;
     const int col = CH == 8 ? (w & 3) + ((w >> 1) & 4) : w & 3;
@@ -540,8 +547,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
       if (!y.valid || !store(y)) break;
       load(y);
     }
-  } else if (lane == 0) {
+  } else {
     // ------------------------------------------------------------ MMA issue
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs) : "memory");
+    if (lane == 0) {
     const int rt = (warp - kSoftWarps - kWideWarps) & 1;
     const bool scores = warp < kSoftWarps + kWideWarps + 2;
     uint32_t n = 0, c = 0, nq = 0;  // tiles of the ring, tiles and queries of this row tile
@@ -604,6 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
     const long long start = clock64();
     while (!mbar_try_wait(drain[2 * rt + (scores ? 0 : 1)], 0) && clock64() - start < kWaitLimitCycles) {
     }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -623,6 +633,12 @@ cudaError_t tc_launch(const PagedAttendParams& p, bool bf16, const PagedPartials
     e = cudaFuncSetAttribute(paged_attend_tc_kernel<KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              Lay<D>::bytes(kMaxBatch));
     if (e != cudaSuccess) return e;
+    // the split of the registers holds for this launch allocation only: setmaxnreg.inc would wait for
+    // registers that the block does not hold
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, paged_attend_tc_kernel<KV, D>);
+    if (e != cudaSuccess) return e;
+    if ((fa.numRegs + 7) / 8 * 8 != kRegs) return cudaErrorInvalidConfiguration;
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   e = launch_dependent(paged_attend_tc_kernel<KV, D>, dim3(ctas), kThreads, Lay<D>::bytes(p.b.B), st, p, ws, bf16);
