@@ -342,60 +342,58 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         const float fo = up ? fast_exp2(M - Mf) : 1.f;
         m = mn;
         M = Mn;
-        // w underflows where p does not: the sum of p itself
-        float e[4], psum = 0.f;
-        bool wide = false;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          e[q] = Mf - lv[q] - mf;
-          wide |= e[q] > 90.f;
-        }
-        if (__builtin_expect(__any_sync(0xffffffffu, wide), 0)) {
-#pragma unroll
-          for (int k = 0; k < kKeys; ++k) {
-            const float x = fast_exp2(fmaf(s[k], a[k >> 4], -mf));
-            psum += e[k >> 4] > 90.f ? x : 0.f;
-          }
-        }
-        uint32_t w[kKeys / 2];
-        l += psum;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float2 a2 = make_float2(a[q], a[q]), b2 = make_float2(lv[q] - Mf, lv[q] - Mf);
-          float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int k = 0; k < 16; k += 2) {
-            float2 x = __ffma2_rn(make_float2(s[16 * q + k], s[16 * q + k + 1]), a2, b2);
-            x.x = fast_exp2(x.x);
-            x.y = fast_exp2(x.y);
-            sum = __fadd2_rn(sum, x);
-            w[8 * q + (k >> 1)] = pack2<__half>(x.x, x.y);
-          }
-          l += e[q] > 90.f ? 0.f : (sum.x + sum.y) * fast_exp2(e[q]);
-        }
         // W and O are free once the MMA of the tile before is done
         if (c > 0) {
           ok = mbar_wait(o_done[rt], (c - 1) & 1, kErr | 3, abort);
           if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
           tc_fence_after();
         }
-        if (t > seg.t0 && __any_sync(0xffffffffu, fo != 1.f)) {
-#pragma unroll 1
-          for (int k = 0; k < D / 32; ++k) {
-            float o[32];
-            tmem_ld32f(to + 32 * k, o);
-            tmem_wait_ld();
+        float e[4];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] *= fo;
-            tmem_st32f(to + 32 * k, o);
+        for (int q = 0; q < 4; ++q) e[q] = Mf - lv[q] - mf;
+        const bool wide = fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) > 90.f;
+        if (__builtin_expect(__any_sync(0xffffffffu, wide || fo != 1.f), 0)) {
+          if (__any_sync(0xffffffffu, wide)) {  // w underflows where p does not: the sum of p itself
+#pragma unroll
+            for (int k = 0; k < kKeys; ++k) {
+              const float x = fast_exp2(fmaf(s[k], a[k >> 4], -mf));
+              l += e[k >> 4] > 90.f ? x : 0.f;
+            }
           }
-          tmem_wait_st();
+          if (t > seg.t0) {
+#pragma unroll 1
+            for (int k = 0; k < D / 32; ++k) {
+              float o[32];
+              tmem_ld32f(to + 32 * k, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] *= fo;
+              tmem_st32f(to + 32 * k, o);
+            }
+            tmem_wait_st();
+          }
         }
         uint8_t* dst = sm + L::oW + rt * L::kWBytes + row * 128;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          *reinterpret_cast<uint4*>(dst + ((k ^ (row & 7)) << 4)) =
-              make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        for (int q = 0; q < 4; ++q) {
+          const float2 a2 = make_float2(a[q], a[q]), b2 = make_float2(lv[q] - Mf, lv[q] - Mf);
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int at = 16 * q + 8 * h + 2 * k;
+              float2 x = __ffma2_rn(make_float2(s[at], s[at + 1]), a2, b2);
+              x.x = fast_exp2(x.x);
+              x.y = fast_exp2(x.y);
+              sum = __fadd2_rn(sum, x);
+              w[k] = pack2<__half>(x.x, x.y);
+            }
+            *reinterpret_cast<uint4*>(dst + (((2 * q + h) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          l += e[q] > 90.f ? 0.f : (sum.x + sum.y) * fast_exp2(e[q]);
+        }
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
