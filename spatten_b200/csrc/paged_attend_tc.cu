@@ -52,7 +52,7 @@ constexpr int kRowTile = 128, kRowsCta = 256, kKeys = 64, kRing = 3;
 constexpr int kSoftWarps = 8, kWideWarps = 8, kMmaWarps = 4,
               kThreads = 32 * (kSoftWarps + kWideWarps + kMmaWarps);
 // registers per thread at launch, and of each role after setmaxnreg
-constexpr int kRegs = 96, kSoftRegs = 136, kWideRegs = 72, kMmaRegs = 64;
+constexpr int kRegs = 96, kSoftRegs = 144, kWideRegs = 72, kMmaRegs = 48;
 static_assert(kSoftWarps * kSoftRegs + kWideWarps * kWideRegs + kMmaWarps * kMmaRegs ==
                   (kSoftWarps + kWideWarps + kMmaWarps) * kRegs,
               "the roles share what the block was launched with");
@@ -253,16 +253,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
       float cq = 0.f;
       if (used && nt > 0) {
         const uint16_t* qp = static_cast<const uint16_t*>(p.q) + (int64_t)(seg.sq.begin + i) * p.q_st + (int64_t)h * p.q_sh;
-        // twice over the row (the second time from L1), to keep the loop's registers and code small
         float top = 0.f;
+        uint4 x[D / 8];
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k)
+          x[k] = live ? *(reinterpret_cast<const uint4*>(qp) + k) : make_uint4(0u, 0u, 0u, 0u);
         auto pair = [&](uint32_t w) {
           return bf16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u))
                       : __half22float2(*reinterpret_cast<const __half2*>(&w));
         };
-#pragma unroll 4
+#pragma unroll
         for (int k = 0; k < D / 8; ++k) {
-          const uint4 x = live ? *(reinterpret_cast<const uint4*>(qp) + k) : make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 f = pair(w[j]);
@@ -274,10 +276,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
         cq = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23) * (top <= 3.4e38f ? 1.f : NAN);
         uint8_t* dst = sm + L::oQ + rt * L::kQBytes + row * 128;
-#pragma unroll 4
+#pragma unroll
         for (int k = 0; k < D / 8; ++k) {
-          const uint4 x = live ? *(reinterpret_cast<const uint4*>(qp) + k) : make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
           uint32_t o[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
       if (!alive) break;
       if (used) {
         const float inv = seg.whole ? paged_normaliser(m, l, M) : 1.f;
-        const uint32_t prow = (2 * cta + (seg.first ? 1 : 0)) * kRowsCta + rt * kRowTile + row;
+        const uint32_t slot = 2 * cta + (seg.first ? 1 : 0);
         uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(seg.sq.begin + i) * p.o_st + (int64_t)h * p.o_sh;
 #pragma unroll 1
         for (int k = 0; k < D / 32; ++k) {
@@ -436,10 +437,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
           } else {
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
-              *reinterpret_cast<float4*>(ws.o + (size_t)prow * D + 32 * k + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+              reinterpret_cast<float4*>(ws.o)[((size_t)slot * (D / 4) + 8 * k + j / 4) * kRowsCta + rt * kRowTile + row] =
+                  make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
           }
         }
-        if (live && !seg.whole) ws.ml[prow] = make_float4(m, l, M, 0.f);
+        if (live && !seg.whole) ws.ml[slot * kRowsCta + rt * kRowTile + row] = make_float4(m, l, M, 0.f);
         tc_fence_before();
       }
       if (seg.first && !seg.whole) {  // the CTAs up to that of the line's last unit hold a part each
@@ -621,6 +623,57 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
   }
 }
 
+// Joins the line that CTA blockIdx.x began and did not finish (parts: slot 2 c + 1
+// of that CTA, slot 2 c of the following ones; outputs as [D / 4][row] of four
+// dims): a warp takes 16 dims of 32 rows, a row per lane, so that the parts are
+// read whole and a lane writes 32 bytes.
+template <int D>
+__global__ void __launch_bounds__(32 * (D / 16)) paged_join_rows_kernel(const PagedAttendParams p, const PagedPartials ws,
+                                                                        const bool bf16) {
+  grid_dependents();
+  grid_wait();
+  const int c0 = blockIdx.x, dim = threadIdx.x >> 5, row = blockIdx.y * 32 + (threadIdx.x & 31);
+  const PagedCut cut = ws.cut[c0];
+  const int r = cut.row0 + row, R = p.b.H / p.c.G;
+  if (cut.parts == 0 || r >= cut.nrows) return;
+  float m = -INFINITY, M = -INFINITY, l = 0.f, acc[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll 2
+  for (int k = 0; k < cut.parts; ++k) {
+    const size_t slot = 2 * (size_t)(c0 + k) + (k == 0);
+    const float4 h = ws.ml[slot * kRowsCta + row];
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = reinterpret_cast<const float4*>(ws.o)[(slot * (D / 4) + 4 * dim + i) * kRowsCta + row];
+    const float mn = fmaxf(m, h.x), Mn = fmaxf(M, h.z);
+    l = l * fast_exp2(m - finite_or_0(mn)) + h.y * fast_exp2(h.x - finite_or_0(mn));
+    const float a = fast_exp2(M - finite_or_0(Mn)), b = fast_exp2(h.z - finite_or_0(Mn));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc[4 * i] = acc[4 * i] * a + x[i].x * b;
+      acc[4 * i + 1] = acc[4 * i + 1] * a + x[i].y * b;
+      acc[4 * i + 2] = acc[4 * i + 2] * a + x[i].z * b;
+      acc[4 * i + 3] = acc[4 * i + 3] * a + x[i].w * b;
+    }
+    m = mn;
+    M = Mn;
+  }
+  const float inv = paged_normaliser(m, l, M);
+  uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(cut.begin + r / R) * p.o_st +
+                 (int64_t)(cut.g * R + r % R) * p.o_sh + 16 * dim;
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    uint32_t x[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      x[q] = bf16 ? pack2<__nv_bfloat16>(acc[i + 2 * q] * inv, acc[i + 2 * q + 1] * inv)
+                  : pack2<__half>(acc[i + 2 * q] * inv, acc[i + 2 * q + 1] * inv);
+    *reinterpret_cast<uint4*>(op + i) = make_uint4(x[0], x[1], x[2], x[3]);
+  }
+}
+
 template <int KV, int D>
 cudaError_t tc_launch(const PagedAttendParams& p, bool bf16, const PagedPartials& ws, int ctas, cudaStream_t st) {
   static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
@@ -641,7 +694,7 @@ cudaError_t tc_launch(const PagedAttendParams& p, bool bf16, const PagedPartials
   }
   e = launch_dependent(paged_attend_tc_kernel<KV, D>, dim3(ctas), kThreads, Lay<D>::bytes(p.b.B), st, p, ws, bf16);
   if (e != cudaSuccess) return e;
-  return launch_paged_join<D, kRowsCta>(p, ws, ctas, bf16, st);
+  return launch_dependent(paged_join_rows_kernel<D>, dim3(ctas, kRowsCta / 32), 32 * (D / 16), 0, st, p, ws, bf16);
 }
 
 }  // namespace

@@ -26,8 +26,7 @@ SPATTEN_DEV float paged_normaliser(float m, float l, float M) {
   return l == 0.f ? 0.f : exp2f(fminf(finite_or_0(M) - finite_or_0(m), 127.f)) / l;
 }
 
-// Joins rows 16 blockIdx.y .. of the line that CTA blockIdx.x began and did not
-// finish: its parts are
+// Joins the line that CTA blockIdx.x began and did not finish: its parts are
 // slot 2 c + 1 of that CTA and slot 2 c of the following ones. A warp per row
 // and, where the line has fewer rows than the CTA has warps, per share of the
 // parts; D / 32 dims per lane. Bound by the latency of its loads: the (m, l, M)
@@ -44,13 +43,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps, D == 128 ? 1 : 2) paged_join_
   const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const PagedCut cut = ws.cut[c0];
   if (cut.parts == 0) return;
-  const int R = p.b.H / p.c.G, row0 = blockIdx.y * kJoinWarps;
-  const int rows = min(min(cut.nrows - cut.row0, ROWS) - row0, kJoinWarps);
-  if (rows <= 0) return;
+  const int R = p.b.H / p.c.G, rows = min(cut.nrows - cut.row0, ROWS);
   int share = kJoinWarps;  // warps per row
   while (share > 1 && rows * share > kJoinWarps) share >>= 1;
-  const int row = row0 + warp / share, part0 = warp % share;
-  const bool live = row - row0 < rows;
+  const int row = warp / share, part0 = warp % share;
+  const bool live = row < rows;
   auto at = [&](int i) { return (uint32_t)(2 * (c0 + i) + (i == 0)) * ROWS + row; };  // row of part i
   float m = -INFINITY, M = -INFINITY, l = 0.f, acc[E];
 #pragma unroll
@@ -139,8 +136,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps, D == 128 ? 1 : 2) paged_join_
 template <int D, int ROWS>
 cudaError_t launch_paged_join(const PagedAttendParams& p, const PagedPartials& ws, int ctas, bool bf16,
                               cudaStream_t st) {
-  const dim3 grid(ctas, (ROWS + kJoinWarps - 1) / kJoinWarps);
-  return launch_dependent(paged_join_kernel<D, ROWS>, grid, 32 * kJoinWarps, 0, st, p, ws, bf16);
+  static_assert(ROWS <= kJoinWarps, "a warp per row");
+  return launch_dependent(paged_join_kernel<D, ROWS>, dim3(ctas), 32 * kJoinWarps, 0, st, p, ws, bf16);
 }
 
 inline size_t paged_align256(size_t x) { return (x + 255) & ~size_t(255); }
