@@ -32,8 +32,8 @@
 //
 // Work split: as in paged_attend.cu, ranges of equal length over all CTAs, here in
 // keys: row tile rt of a sequence counts old + (rt + 1) 256 / R of them (the causal
-// triangle), cumulated in closed form, and the 64-key tile at position k belongs
-// to the CTA that holds unit k of its line. Every wait is bounded; a timeout
+// triangle) and kLineCost, cumulated in closed form, and the 64-key tile at
+// position k belongs to the CTA that holds unit kLineCost + k of its line. Every wait is bounded; a timeout
 // records a code in this file's device error word and the CTA winds down.
 #include <atomic>
 #include <cmath>
@@ -58,6 +58,7 @@ static_assert(kSoftWarps * kSoftRegs + kWideWarps * kWideRegs + kMmaWarps * kMma
               "the roles share what the block was launched with");
 constexpr float kSlack = 8.f;
 constexpr float kNoScale = -200.f;  // log2 of a scale of 0
+constexpr uint32_t kLineCost = 256;  // what a line's set-up takes, in keys (7 us, a 64-key tile 1.65 us)
 constexpr unsigned kErr = 0x400;
 constexpr int kMaxBatch = 1024;
 
@@ -121,7 +122,7 @@ struct Segments {
   SPATTEN_DEV static uint32_t tokens_per_tile(int R) { return (kRowsCta + R - 1) / R; }
   // units of row tiles 0 .. rt - 1 of a sequence
   SPATTEN_DEV static uint32_t before(const PagedSeq& s, uint32_t rt, uint32_t tok) {
-    return rt * max(s.old, 0) + tok * (rt * (rt + 1) / 2);
+    return rt * (max(s.old, 0) + kLineCost) + tok * (rt * (rt + 1) / 2);
   }
   SPATTEN_DEV static uint32_t row_tiles(const PagedSeq& s, int R) { return ((uint32_t)s.n * R + kRowsCta - 1) / kRowsCta; }
   SPATTEN_DEV static uint32_t units(const PagedSeq& s, int R) {
@@ -144,14 +145,15 @@ struct Segments {
     u0 = u;
     line = before(sq, lo + 1, tok) - before(sq, lo, tok);
     const uint32_t v1 = min(line, v0 + (u1 - u));
+    auto tile = [](uint32_t v) { return (int)((max(v, kLineCost) - kLineCost + kKeys - 1) / kKeys); };
     first = v0 == 0;
     whole = first && v1 == line;
     r0 = lo * kRowsCta;
     nrows = sq.n * R;
     lim_max = max(min(sq.old + min((r0 + kRowsCta - 1) / R, sq.n - 1) + 1, sq.len), 0);
     const int kt = (lim_max + kKeys - 1) / kKeys;
-    t0 = min((int)((v0 + kKeys - 1) / kKeys), kt);
-    t1 = v1 == line ? kt : min((int)((v1 + kKeys - 1) / kKeys), kt);
+    t0 = min(tile(v0), kt);
+    t1 = v1 == line ? kt : min(tile(v1), kt);
     u += v1 - v0;
     return true;
   }
@@ -249,44 +251,51 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
       const int r = seg.r0 + rt * kRowTile + row;
       const bool live = r < seg.nrows, used = seg.nrows - seg.r0 > rt * kRowTile;
       const int nt = seg.t1 - seg.t0, i = (live ? r : 0) / R, h = seg.g * R + (live ? r : 0) % R;
-      // the row's query, scaled into f16, as the A operand
-      float cq = 0.f;
+      float cq = 0.f;  // what a score of this row has to be multiplied by
       if (used && nt > 0) {
-        const uint16_t* qp = static_cast<const uint16_t*>(p.q) + (int64_t)(seg.sq.begin + i) * p.q_st + (int64_t)h * p.q_sh;
-        float top = 0.f;
-        uint4 x[D / 8];
-#pragma unroll
-        for (int k = 0; k < D / 8; ++k)
-          x[k] = live ? *(reinterpret_cast<const uint4*>(qp) + k) : make_uint4(0u, 0u, 0u, 0u);
+        // the warp's 32 rows, LQ lanes a row (16 bytes each), all loads in flight at once
+        constexpr int LQ = D / 8, RQ = 32 / LQ;
+        const int li = lane % LQ, in = lane / LQ, first = rt * kRowTile + (warp & 3) * 32;
         auto pair = [&](uint32_t w) {
           return bf16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u))
                       : __half22float2(*reinterpret_cast<const __half2*>(&w));
         };
+        uint4 x[LQ];
 #pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
+        for (int k = 0; k < LQ; ++k) {
+          const int y = seg.r0 + first + k * RQ + in;
+          const uint16_t* qp = static_cast<const uint16_t*>(p.q) + 8 * li;
+          x[k] = make_uint4(0u, 0u, 0u, 0u);
+          if (y < seg.nrows)
+            x[k] = *reinterpret_cast<const uint4*>(qp + (int64_t)(seg.sq.begin + y / R) * p.q_st +
+                                                   (int64_t)(seg.g * R + y % R) * p.q_sh);
+        }
+#pragma unroll
+        for (int k = 0; k < LQ; ++k) {
           const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+          float top = 0.f;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 f = pair(w[j]);
             top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
             if (!(f.x == f.x && f.y == f.y)) top = INFINITY;
           }
-        }
-        const int e = top > 0.f ? 14 - max((int)(__float_as_uint(top) >> 23) - 127, -112) : 0;
-        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-        cq = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23) * (top <= 3.4e38f ? 1.f : NAN);
-        uint8_t* dst = sm + L::oQ + rt * L::kQBytes + row * 128;
 #pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
-          const uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+          for (int d = LQ / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          const int e = top > 0.f ? 14 - max((int)(__float_as_uint(top) >> 23) - 127, -112) : 0;
+          const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+          const float back = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23) * (top <= 3.4e38f ? 1.f : NAN);
+          const float mine = __shfl_sync(0xffffffffu, back, (lane % RQ) * LQ);
+          if (lane / RQ == k) cq = mine;  // this thread's row is among the step's
           uint32_t o[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 f = pair(w[j]);
             o[j] = pack2<__half>(f.x * up, f.y * up);
           }
-          *reinterpret_cast<uint4*>(dst + (k >> 3) * (kRowTile * 128) + (((k & 7) ^ (row & 7)) << 4)) =
-              make_uint4(o[0], o[1], o[2], o[3]);
+          const int y = (warp & 3) * 32 + k * RQ + in;
+          *reinterpret_cast<uint4*>(sm + L::oQ + rt * L::kQBytes + (li >> 3) * (kRowTile * 128) + y * 128 +
+                                    (((li & 7) ^ (y & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -704,7 +713,7 @@ bool paged_attend_tc_takes(const PagedAttendParams& p) {
   const int R = p.b.H / p.c.G;
   if ((int64_t)p.b.max_tokens * R < 64 || p.b.B > kMaxBatch) return false;
   const double lines = (double)p.b.T * R / kRowsCta + p.b.B;  // at most
-  return lines * p.c.G * ((double)p.c.max_pages * p.c.page + kRowsCta) < 4e9;
+  return lines * p.c.G * ((double)p.c.max_pages * p.c.page + kRowsCta + kLineCost) < 4e9;
 }
 
 size_t paged_attend_tc_workspace(const PagedAttendParams& p, int n_sm) {
