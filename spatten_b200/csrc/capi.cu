@@ -626,6 +626,8 @@ static int fill_paged_attend(const spatten_paged_attend_args* a, spatten::PagedA
   p.q = a->q; p.q_st = a->q_st; p.q_sh = a->q_sh;
   p.out = a->out; p.o_st = a->o_st; p.o_sh = a->o_sh;
   p.scale_log2 = a->sm_scale * spatten::kLog2e;
+  p.rows_over = 0;
+  p.rows_upto = INT64_MAX;
   if (!spatten::paged_attend_fits(p))
     return fail(SPATTEN_ERR_UNSUPPORTED, "%s: %d rows of %d heads over a page table of %lld slots", who, a->T, a->H,
                 (long long)p.c.max_pages * p.c.page);

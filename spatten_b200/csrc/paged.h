@@ -57,6 +57,9 @@ struct PagedAttendParams {
   void* out;
   int64_t o_st, o_sh;
   float scale_log2;         // sm_scale * log2(e)
+  // the launch serves sequences with more than rows_over and at most rows_upto
+  // query rows per KV head
+  int64_t rows_over, rows_upto;
 };
 
 struct PagedReadParams {
@@ -75,6 +78,7 @@ int paged_attend_max_batch();  // sequences of one call
 bool paged_attend_fits(const PagedAttendParams& p);  // units of work count in 32 bits
 size_t paged_attend_workspace(const PagedAttendParams& p, int n_sm);
 // the tcgen05 path (paged_attend_tc.cu), for many query rows per KV head
+constexpr int kTcRows = 64;  // it takes sequences with more rows than this
 bool paged_attend_tc_takes(const PagedAttendParams& p);
 size_t paged_attend_tc_workspace(const PagedAttendParams& p, int n_sm);
 cudaError_t launch_paged_attend_tc(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,

@@ -254,7 +254,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     n = 0;
     if (b >= p.b.B) return 0u;
     const PagedSeq s = paged_seq(p.b, p.c, b);
-    if (s.n > 0) n = (uint32_t)G * row_tiles(s, R, ROWS);
+    if (paged_serves(p, s, R)) n = (uint32_t)G * row_tiles(s, R, ROWS);
     return (uint32_t)key_tiles(s, KEYS);
   };
   uint32_t n0, k0 = 0;  // of sequence `tid`
@@ -618,7 +618,11 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
 
 // Eight query rows per pass where that covers a sequence's rows (the register
 // tile of 16 has room for half the bytes in flight), else sixteen.
-int row_block(const PagedAttendParams& p) { return (int64_t)p.b.max_tokens * (p.b.H / p.c.G) <= 8 ? 8 : 16; }
+int row_block(const PagedAttendParams& p) {
+  // beside the tcgen05 launch: what is left is mostly single tokens
+  const int64_t tokens = p.rows_upto <= kTcRows ? 1 : p.b.max_tokens;
+  return tokens * (p.b.H / p.c.G) <= 8 ? 8 : 16;
+}
 
 double units_bound(const PagedAttendParams& p) {
   const int rows = row_block(p);
@@ -668,20 +672,54 @@ cudaError_t attend_dim(const PagedAttendParams& p, bool bf16, const Workspace& w
 
 int paged_attend_max_batch() { return kMaxBatch; }
 
-bool paged_attend_fits(const PagedAttendParams& p) { return units_bound(p) < 4e9; }
+namespace {
+
+// Which kernels a call takes. Sequences of more than kTcRows query rows per KV
+// head (pieces of prompts) go to the tcgen05 kernel, the others to the one above:
+// at 4 sequences x 8 heads over 4096 keys, 64 rows take 43.5 us there and 41.8 us
+// here, 96 rows 44 us and 55 us. The host knows the largest sequence only; where
+// the rows show that some must be shorter, both are launched and each serves its
+// own, so that single tokens beside a prompt's piece keep the kernel made for
+// them (the other launch costs about 4 us).
+struct Plan {
+  PagedAttendParams tc, few;
+  bool use_tc, use_few;
+};
+
+Plan plan_for(const PagedAttendParams& p) {
+  Plan x = {p, p, false, true};
+  x.tc.rows_over = x.few.rows_over = 0;
+  x.tc.rows_upto = x.few.rows_upto = INT64_MAX;
+  if (!paged_attend_tc_takes(p)) return x;
+  x.use_tc = true;
+  x.use_few = p.b.B > 1 && p.b.T < (int64_t)p.b.B * p.b.max_tokens;
+  if (x.use_few) x.tc.rows_over = x.few.rows_upto = kTcRows;
+  return x;
+}
+
+}  // namespace
+
+bool paged_attend_fits(const PagedAttendParams& p) { return units_bound(plan_for(p).few) < 4e9; }
 
 size_t paged_attend_workspace(const PagedAttendParams& p, int n_sm) {
-  if (paged_attend_tc_takes(p)) return paged_attend_tc_workspace(p, n_sm);
-  return paged_partials_bytes(grid_ctas(p, n_sm), row_block(p), p.c.D);
+  const Plan x = plan_for(p);
+  return (x.use_tc ? paged_attend_tc_workspace(p, n_sm) : 0) +
+         (x.use_few ? paged_partials_bytes(grid_ctas(x.few, n_sm), row_block(x.few), p.c.D) : 0);
 }
 
 cudaError_t launch_paged_attend(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm, cudaStream_t st) {
   if (dtype != kF16 && dtype != kBF16) return cudaErrorInvalidValue;
-  if (paged_attend_tc_takes(p)) return launch_paged_attend_tc(p, dtype, kv, ws, n_sm, st);
-  const int ctas = grid_ctas(p, n_sm);
-  const Workspace s = paged_partials(ws, ctas, row_block(p));
+  const Plan x = plan_for(p);
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  if (x.use_tc) {
+    const cudaError_t e = launch_paged_attend_tc(x.tc, dtype, kv, w, n_sm, st);
+    if (e != cudaSuccess || !x.use_few) return e;
+    w += paged_attend_tc_workspace(p, n_sm);
+  }
+  const int ctas = grid_ctas(x.few, n_sm);
+  const Workspace s = paged_partials(w, ctas, row_block(x.few));
   const bool bf16 = dtype == kBF16;
-  return kv == kKvInt8 ? attend_dim<kKvInt8>(p, bf16, s, ctas, st) : attend_dim<kKvE4m3>(p, bf16, s, ctas, st);
+  return kv == kKvInt8 ? attend_dim<kKvInt8>(x.few, bf16, s, ctas, st) : attend_dim<kKvE4m3>(x.few, bf16, s, ctas, st);
 }
 
 }  // namespace spatten

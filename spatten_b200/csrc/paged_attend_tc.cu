@@ -126,7 +126,7 @@ struct Segments {
   }
   SPATTEN_DEV static uint32_t row_tiles(const PagedSeq& s, int R) { return ((uint32_t)s.n * R + kRowsCta - 1) / kRowsCta; }
   SPATTEN_DEV static uint32_t units(const PagedSeq& s, int R) {
-    return s.n > 0 ? before(s, row_tiles(s, R), tokens_per_tile(R)) : 0;
+    return before(s, row_tiles(s, R), tokens_per_tile(R));
   }
 
   SPATTEN_DEV bool next() {
@@ -207,7 +207,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
   for (int base = 0; base < p.b.B; base += kThreads) {
     const int b = base + tid;
     uint32_t x = 0;
-    if (b < p.b.B) x = (uint32_t)G * Segments::units(paged_seq(p.b, p.c, b), R);
+    if (b < p.b.B) {
+      const PagedSeq s = paged_seq(p.b, p.c, b);
+      if (paged_serves(p, s, R)) x = (uint32_t)G * Segments::units(s, R);
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
@@ -708,10 +711,9 @@ cudaError_t tc_launch(const PagedAttendParams& p, bool bf16, const PagedPartials
 
 }  // namespace
 
-// 64 rows per KV head and more: below, most of a row tile would be padding.
 bool paged_attend_tc_takes(const PagedAttendParams& p) {
   const int R = p.b.H / p.c.G;
-  if ((int64_t)p.b.max_tokens * R < 64 || p.b.B > kMaxBatch) return false;
+  if ((int64_t)p.b.max_tokens * R <= kTcRows || p.b.B > kMaxBatch) return false;
   const double lines = (double)p.b.T * R / kRowsCta + p.b.B;  // at most
   return lines * p.c.G * ((double)p.c.max_pages * p.c.page + kRowsCta + kLineCost) < 4e9;
 }

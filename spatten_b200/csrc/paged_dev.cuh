@@ -53,6 +53,12 @@ SPATTEN_DEV PagedSeq paged_seq(const PagedBatch& p, const PagedCache& c, int b) 
   return s;
 }
 
+// Whether a launch serves the sequence, given its query rows per KV head.
+SPATTEN_DEV bool paged_serves(const PagedAttendParams& p, const PagedSeq& s, int R) {
+  const int64_t rows = (int64_t)s.n * R;
+  return rows > p.rows_over && rows <= p.rows_upto;
+}
+
 // Page of slots [pi * page, ...) of sequence b, or -1 where it has no memory.
 SPATTEN_DEV int paged_page(const PagedCache& c, int b, int pi) {
   if (pi >= c.max_pages) return -1;
