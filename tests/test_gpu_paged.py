@@ -11,7 +11,14 @@ Tolerances (u = 2^-24):
 * attention, per output: half a step of the result, and of A = sum p |v|:
   the rounding of p to fp16 (2^-11) and of the scores, D u S each way with S =
   sum |q k| of the scores, into an exponent (times 2 for numerator and
-  denominator), and 2^-16 for the fp32 sums over the keys.
+  denominator), and 2^-16 for the fp32 sums over the keys. And of the row's
+  largest A: a weight p v_scale is an fp16 relative to the row's largest, and
+  one below fp16's normal range is off by up to half its smallest step, 2^-25 of
+  that, times a code of at most 127; the largest weight meets a code of 64 or
+  more in one of its key's dims (normal values, D >= 64), so n keys make at
+  most n 2^-25 (127 / 64) < n 2^-24 of the row's largest A. It counts where an
+  output's own terms are that much smaller than its row's: a dim in which the key
+  with all the weight holds a 0.
 """
 import itertools
 
@@ -232,7 +239,7 @@ def _check_attend(out, q, cache, table, cu, lens, sm):
     D = q.shape[-1]
     T = cu[-1]
     tol = torch.finfo(out.dtype).eps / 2 * want.abs() + A * (2.0 ** -11 + 2 * D * U * S + 2.0 ** -16) + \
-        torch.finfo(out.dtype).smallest_normal
+        max(lens) * U * A.amax(-1, keepdim=True) + torch.finfo(out.dtype).smallest_normal
     bad = ((out.cpu().double() - want).abs() > tol)[:T]
     assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
     return want
@@ -514,3 +521,145 @@ def test_refusals():
         paged.paged_read(c, t, ln, idx=_i32([[0]]))
     with pytest.raises(TypeError):
         paged.paged_read(c, t, ln, dtype=torch.float32)
+
+
+def _device_error():
+    import ctypes
+    from spatten_b200 import _native as N
+    code = ctypes.c_uint(1)
+    N.check(N.lib.spatten_device_error(ctypes.byref(code), 0))
+    return code.value
+
+
+@pytest.mark.parametrize("kv,dt,D,page,G,R,news,lens,pad", [
+    # every sequence as long as the largest: the tensor-memory kernel serves all of them
+    (I8, BF16, 128, 64, 2, 4, [40, 40], [200, 41], 0),
+    (E4, F16, 64, 32, 3, 3, [90, 90, 90], [90, 300, 91], 0),
+    # mixed with shorter ones, one row tile and two, borders of both
+    (I8, F16, 128, 32, 1, 4, [33, 32, 31, 64, 65], [64, 200, 31, 64, 513], 7),
+    (E4, BF16, 128, 16, 2, 5, [1, 60, 0, 26, 2], [500, 77, 9, 26, 130], 3),
+    (I8, BF16, 64, 128, 2, 16, [9, 1, 17], [300, 129, 17], 1),
+    (E4, F16, 128, 64, 1, 128, [1, 2, 3], [64, 65, 130], 0),
+    (I8, F16, 128, 64, 1, 100, [3, 1], [200, 64], 0),
+])
+def test_attention_pieces(kv, dt, D, page, G, R, news, lens, pad):
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(21)
+    B, H = len(news), G * R
+    mp = max(lens) // page + 1
+    P = B * mp + 2
+    table, cu = _table(B, mp, P, g), _cum(news)
+    cache = _filled(kv, P, G, page, D, g)
+    q = torch.randn(cu[-1] + pad, H, D, generator=g).to(dt).cuda()
+    out = torch.full_like(q, 3.0)
+    paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), max(news), out=out)
+    _check_attend(out, q, cache, table, cu, lens, D ** -0.5)
+    assert (out[cu[-1]:] == 3).all()
+    again = paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), max(news))
+    assert torch.equal(again[:cu[-1]], out[:cu[-1]])
+    assert _device_error() == 0
+
+
+@pytest.mark.parametrize("kv", [I8, E4])
+def test_attention_pieces_masked_places(kv):
+    """As test_attention_masked_places, with enough rows for the
+    tensor-memory kernel; a row that is not finite stays alone; a negative
+    scale of the scores."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(22)
+    G, R, D, page = 2, 4, 128, 32
+    news, lens = [50, 40, 0, 70], [0, 25, 40, 260]
+    cu, B = _cum(news), 4
+    table = _table(B, 9, 40, g)
+    table[3, 1], table[3, 4], table[1, 0] = -1, 1000, -3
+    cache = _filled(kv, 40, G, page, D, g)
+    used = torch.zeros(40, dtype=torch.bool)
+    for b in range(B):
+        for s in range(lens[b]):
+            if 0 <= table[b, s // page] < 40:
+                used[table[b, s // page]] = True
+        last = int(table[b, lens[b] // page])
+        if 0 <= last < 40:
+            for t in cache[:2]:
+                t.view(I8)[last, :, lens[b] % page:] = 0x7F
+    for t in cache[2:]:
+        t[(~used).cuda()] = float("nan")
+    q = torch.randn(cu[-1], G * R, D, generator=g).to(BF16).cuda()
+    for sm in (D ** -0.5, -0.05):
+        out = paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), max(news), sm_scale=sm)
+        want, A, S = O.attend(q.cpu(), _cpu(cache), table, cu, lens, sm)
+        S = S.abs().clamp(min=1.0) if sm < 0 else S
+        tol = 2.0 ** -8 * want.abs() + A * (2.0 ** -11 + 2 * D * U * (abs(sm) * 127 * 4 * D) + 2.0 ** -16) + 1e-38
+        assert ((out.cpu().double() - want).abs() <= tol).all()
+        assert (out[:50] == 0).all() and (out[50:50 + 15] == 0).all()  # nothing held; the first 15 of 40 with 25 slots
+    bad = q.clone()
+    bad[100, 3, 5], bad[101, 6, 0] = float("nan"), float("inf")
+    got = paged.paged_attention(bad, cache, table.cuda(), _i32(cu), _i32(lens), max(news), sm_scale=-0.05)
+    assert torch.isnan(got[100, 3]).all() and torch.isnan(got[101, 6]).all()
+    same = torch.ones(out.shape[:2], dtype=torch.bool)
+    same[100, 3] = same[101, 6] = False
+    assert torch.equal(got[same.cuda()], out[same.cuda()])
+    assert _device_error() == 0
+
+
+def test_attention_pieces_extremes():
+    """test_attention_extremes with 80 queries per KV head."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(23)
+    G, R, D, page, n, T = 1, 4, 128, 16, 200, 20
+    table = _table(1, 13, 15, g)
+    cache = _filled(I8, 15, G, page, D, g, spread=False)
+    cache.v_scale[:, 0] = 2.0 ** torch.linspace(-100, 100, 15)[torch.randperm(15, generator=g)].round().cuda()
+    cache.v_scale[int(table[0, 2])] = 0.0
+    cache.k_scale[int(table[0, 4])] = 0.0
+    q = torch.randn(T, R, D, generator=g).to(BF16).cuda()
+    for x in (q, (q.float() * 300).to(BF16)):
+        out = paged.paged_attention(x, cache, table.cuda(), _i32([0, T]), _i32([n]), T)
+        _check_attend(out, x, cache, table, [0, T], [n], D ** -0.5)
+
+
+def test_attention_many_sequences():
+    """More sequences than the threads that number them, for both kernels, and
+    more than one launch can take."""
+    from spatten_b200 import _native as N
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(24)
+    G, D, page, P = 1, 64, 16, 50
+    cache = _filled(I8, P, G, page, D, g)
+    for B, R, hi in ((700, 1, 2), (700, 3, 30), (1100, 16, 5)):
+        news = torch.randint(0, hi, (B,), generator=g).tolist()
+        news[B // 2] = hi
+        lens = [n + int(x) for n, x in zip(news, torch.randint(0, 20, (B,), generator=g))]
+        table = torch.randint(0, P, (B, 4), generator=g).to(torch.int32)  # pages shared by the sequences
+        cu = _cum(news)
+        q = torch.randn(cu[-1], R, D, generator=g).to(F16).cuda()
+        out = paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), hi)
+        _check_attend(out, q, cache, table, cu, lens, D ** -0.5)
+    B = 8193
+    with pytest.raises(N.SpattenError, match="at most 8192"):
+        paged.paged_attention(q[:1], cache, torch.zeros(B, 1, dtype=torch.int32, device="cuda"), _i32([0] * B + [1]),
+                              _i32([1] * B), 1)
+
+
+def test_attention_captured_over_changing_pieces():
+    """One captured call, replayed while the sequences' new tokens, lengths and
+    pages change: sequences move between the two kernels."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(25)
+    G, R, D, page, B, T, mx = 2, 4, 128, 32, 3, 150, 100
+    cache = _filled(E4, 60, G, page, D, g)
+    q = torch.randn(T, G * R, D, generator=g).to(BF16).cuda()
+    td, cu, ln = (torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((B, 12), B + 1, B))
+    paged.paged_attention(q, cache, td, cu, ln, mx)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = paged.paged_attention(q, cache, td, cu, ln, mx)
+    for news, lens in (([1, 100, 20], [300, 100, 50]), ([70, 1, 1], [70, 384, 2]), ([16, 17, 0], [16, 40, 9])):
+        table = _table(B, 12, 60, g)
+        td.copy_(table)
+        cu.copy_(_i32(_cum(news)))
+        ln.copy_(_i32(lens))
+        gr.replay()
+        torch.cuda.synchronize()
+        _check_attend(out, q, cache, table, _cum(news), lens, D ** -0.5)
