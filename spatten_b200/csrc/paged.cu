@@ -47,20 +47,44 @@ SPATTEN_DEV float scale_for(float amax) {
 }
 
 // Eight finite values over the block's scale (not 0), as codes; rc = 1 / s.
+// int8: y = x rc lands within 2 ulp of x / s, so its rounding can only differ
+// from the division's near a tie; the distance to the rounded value is kept as a
+// maximum over the eight, and near a tie (or for the NaN that a subnormal scale's
+// reciprocal makes) they take the division. y + 1.5 2^23 holds the rounded
+// integer's low byte in its own.
 template <int KV>
-SPATTEN_DEV uint2 encode8(const float (&x)[8], float s, float rc) {
+SPATTEN_DEV uint2 encode8(const float2 (&x)[4], float s, float rc) {
   uint32_t w[2];
+  if constexpr (KV == kKvInt8) {
+    constexpr float kRound = 12582912.0f;
+    const float2 r2 = make_float2(rc, rc), up = make_float2(kRound, kRound), down = make_float2(-kRound, -kRound);
+    float far = 0.f;
+    uint32_t b[8];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if constexpr (KV == kKvInt8) {
-      int c[4];
+    for (int i = 0; i < 4; ++i) {
+      const float2 y = __fmul2_rn(x[i], r2), f = __fadd2_rn(y, up), t = __fadd2_rn(f, down);
+      const float2 d = __fadd2_rn(y, make_float2(-t.x, -t.y));
+      far = max_abs_nan(max_abs_nan(far, d.x), d.y);
+      b[2 * i] = __float_as_uint(f.x);
+      b[2 * i + 1] = __float_as_uint(f.y);
+    }
+    if (!(far <= 0.49990f)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) c[i] = quant_div_fadd(x[4 * j + i], s, rc);
-      const uint32_t lo = __byte_perm(c[0], c[1], 0x0040), hi = __byte_perm(c[2], c[3], 0x0040);
-      w[j] = __byte_perm(lo, hi, 0x5410);
-    } else {
-      w[j] = f32x2_to_e4m3x2(x[4 * j] * rc, x[4 * j + 1] * rc) |
-             (f32x2_to_e4m3x2(x[4 * j + 2] * rc, x[4 * j + 3] * rc) << 16);
+      for (int i = 0; i < 4; ++i) {
+        b[2 * i] = (uint32_t)__float2int_rn(__fdiv_rn(x[i].x, s));
+        b[2 * i + 1] = (uint32_t)__float2int_rn(__fdiv_rn(x[i].y, s));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      w[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040), __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040),
+                         0x5410);
+  } else {
+    const float2 r2 = make_float2(rc, rc);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float2 a = __fmul2_rn(x[2 * j], r2), b = __fmul2_rn(x[2 * j + 1], r2);
+      w[j] = f32x2_to_e4m3x2(a.x, a.y) | (f32x2_to_e4m3x2(b.x, b.y) << 16);
     }
   }
   return make_uint2(w[0], w[1]);
@@ -86,51 +110,65 @@ SPATTEN_DEV uint2 rescale8(uint2 c, float ratio) {
 }
 
 template <typename T>
-SPATTEN_DEV void unpack4(uint2 u, float* f) {
+SPATTEN_DEV float2 unpack2(uint32_t u) {
   const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = to_f32<T>(e[i]);
+  return make_float2(to_f32<T>(e[0]), to_f32<T>(e[1]));
 }
 
-// A lane's dims of a row: 4 li .. of its first half (f[0 .. 3]) and of its second.
+// A lane's dims of a row: 4 li .. of its first half (f[0], f[1]) and of its second.
 template <typename T, int D>
-SPATTEN_DEV void load_halves(const T* row, int li, float (&f)[8]) {
-  unpack4<T>(*(reinterpret_cast<const uint2*>(row + 4 * li)), f);
-  unpack4<T>(*(reinterpret_cast<const uint2*>(row + D / 2 + 4 * li)), f + 4);
+SPATTEN_DEV void load_halves(const T* row, int li, float2 (&f)[4]) {
+  const uint2 a = *reinterpret_cast<const uint2*>(row + 4 * li), b = *reinterpret_cast<const uint2*>(row + D / 2 + 4 * li);
+  f[0] = unpack2<T>(a.x);
+  f[1] = unpack2<T>(a.y);
+  f[2] = unpack2<T>(b.x);
+  f[3] = unpack2<T>(b.y);
 }
 
-// Norm and rotation of one row spread over D / 8 lanes, all lanes of the warp
-// taking part; g: the lane's norm weights.
-template <typename T, int D>
-SPATTEN_DEV void norm_rotate(float (&x)[8], int li, const PagedAppendParams& p, const float* g, int pos) {
-  if (g) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-    for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float inv = rsqrtf(__fadd_rn(ss * (1.0f / D), p.eps));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], inv), g[i]);
+// A lane's part of the rotation by a position: cos, sin and -sin of its pairs.
+struct Turn {
+  float2 c[2], s[2], n[2];
+};
+
+template <typename T>
+SPATTEN_DEV void load_turn(Turn& r, const PagedAppendParams& p, int pos, int li) {
+  const int64_t at = (int64_t)min(max(pos, 0), p.cs_rows - 1) * p.cs_st + 4 * li;
+  if (p.cs_f32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p.cos) + at);
+    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p.sin) + at);
+    r.c[0] = make_float2(a.x, a.y); r.c[1] = make_float2(a.z, a.w);
+    r.s[0] = make_float2(b.x, b.y); r.s[1] = make_float2(b.z, b.w);
+  } else {
+    const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.cos) + at);
+    const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.sin) + at);
+    r.c[0] = unpack2<T>(a.x); r.c[1] = unpack2<T>(a.y);
+    r.s[0] = unpack2<T>(b.x); r.s[1] = unpack2<T>(b.y);
   }
-  if (p.cos) {
-    const int64_t at = (int64_t)min(max(pos, 0), p.cs_rows - 1) * p.cs_st + 4 * li;
-    float c[4], s[4];
-    if (p.cs_f32) {
-      const float4 a = *(reinterpret_cast<const float4*>(static_cast<const float*>(p.cos) + at));
-      const float4 b = *(reinterpret_cast<const float4*>(static_cast<const float*>(p.sin) + at));
-      c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w;
-      s[0] = b.x; s[1] = b.y; s[2] = b.z; s[3] = b.w;
-    } else {
-      unpack4<T>(*(reinterpret_cast<const uint2*>(static_cast<const T*>(p.cos) + at)), c);
-      unpack4<T>(*(reinterpret_cast<const uint2*>(static_cast<const T*>(p.sin) + at)), s);
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = x[i], b = x[4 + i];
-      x[i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i]));
-      x[4 + i] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, s[i]));
-    }
+  for (int i = 0; i < 2; ++i) r.n[i] = make_float2(-r.s[i].x, -r.s[i].y);
+}
+
+// Norm (g: the lane's weights) of one row spread over D / 8 lanes, all lanes of
+// the warp taking part.
+template <int D>
+SPATTEN_DEV void norm_row(float2 (&x)[4], float eps, const float2 (&g)[4]) {
+  float2 q = __fmul2_rn(x[0], x[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) q = __ffma2_rn(x[i], x[i], q);
+  float ss = q.x + q.y;
+#pragma unroll
+  for (int o = D / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const float inv = rsqrtf(__fadd_rn(ss * (1.0f / D), eps));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __fmul2_rn(__fmul2_rn(x[i], make_float2(inv, inv)), g[i]);
+}
+
+SPATTEN_DEV void turn_row(float2 (&x)[4], const Turn& r) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 a = x[i], b = x[2 + i];
+    x[i] = __fadd2_rn(__fmul2_rn(a, r.c[i]), __fmul2_rn(b, r.n[i]));
+    x[2 + i] = __fadd2_rn(__fmul2_rn(b, r.c[i]), __fmul2_rn(a, r.s[i]));
   }
 }
 
@@ -140,17 +178,16 @@ struct AppendShape {
   static constexpr int NT = PAGE * D >= 16384 ? 512 : PAGE * D >= 8192 ? 256 : 128;  // threads
   static constexpr int RPP = NT / LPR;                            // rows per pass
   static constexpr int PASSES = PAGE / RPP;                       // at most 4: 32 values per thread
-  static constexpr int QROWS = 2;                                 // query rows of a thread in flight
   static_assert(PASSES >= 1 && PASSES <= 4 && PAGE % RPP == 0, "a block's rows fit the registers");
 };
 
 // Grid (2 G + query CTAs, written blocks per sequence, B): unit x < G is K
 // head x, x < 2 G V head x - G, the others share the chunk's query rows.
-template <typename T, int KV, int D, int PAGE>
+template <typename T, int KV, int D, int PAGE, int HEADS>
 __global__ void __launch_bounds__(AppendShape<D, PAGE>::NT, 1024 / AppendShape<D, PAGE>::NT)
 paged_append_kernel(const PagedAppendParams p, int nqb) {
   using S = AppendShape<D, PAGE>;
-  constexpr int LPR = S::LPR, RPP = S::RPP, PASSES = S::PASSES, NW = S::NT / 32, QR = S::QROWS;
+  constexpr int LPR = S::LPR, RPP = S::RPP, PASSES = S::PASSES, NW = S::NT / 32;
   grid_dependents();
   grid_wait();
   const int b = blockIdx.z, chunk = blockIdx.y, G = p.c.G;
@@ -158,29 +195,33 @@ paged_append_kernel(const PagedAppendParams p, int nqb) {
   if (sq.n == 0) return;
   const int tid = threadIdx.x, lane = tid & 31, li = lane % LPR, rt = tid / LPR;
 
-  if ((int)blockIdx.x >= 2 * G) {  // query rows of tokens [chunk * PAGE, ..): token-major, heads inside
-    const int t0 = chunk * PAGE, H = p.b.H, rows = min(PAGE, sq.n - t0) * H;
-    float w[8];
+  if ((int)blockIdx.x >= 2 * G) {
+    // query rows of tokens [chunk * PAGE, ..): a row of lanes takes HEADS heads of a token, which share
+    // its rotation and are in flight together
+    const int t0 = chunk * PAGE, H = p.b.H, groups = (H + HEADS - 1) / HEADS;
+    const int items = min(PAGE, sq.n - t0) * groups;
+    float2 w[4];
     if (p.wq) load_halves<T, D>(static_cast<const T*>(p.wq), li, w);
-    for (int r0 = ((int)blockIdx.x - 2 * G) * RPP; r0 < rows; r0 += nqb * RPP * QR) {
-      float x[QR][8];
-      int tok[QR], h[QR];
+    for (int i0 = ((int)blockIdx.x - 2 * G) * RPP; i0 < items; i0 += nqb * RPP) {
+      const bool live = i0 + rt < items;
+      const int item = live ? i0 + rt : items - 1, tok = t0 + item / groups, h0 = item % groups * HEADS;
+      const int64_t row = sq.begin + tok;
+      const T* src = static_cast<const T*>(p.q) + row * p.q_st + h0 * p.q_sh;
+      T* dst = static_cast<T*>(p.q_out) + row * p.qo_st + h0 * p.qo_sh + 4 * li;
+      Turn turn;
+      if (p.cos) load_turn<T>(turn, p, p.positions ? p.positions[row] : sq.old + tok, li);
+      float2 x[HEADS][4];
 #pragma unroll
-      for (int j = 0; j < QR; ++j) {
-        const int r = min(r0 + j * nqb * RPP + rt, rows - 1);
-        tok[j] = t0 + r / H;
-        h[j] = r % H;
-        load_halves<T, D>(static_cast<const T*>(p.q) + (sq.begin + tok[j]) * p.q_st + h[j] * p.q_sh, li, x[j]);
-      }
+      for (int h = 0; h < HEADS; ++h) load_halves<T, D>(src + min(h, H - 1 - h0) * p.q_sh, li, x[h]);
 #pragma unroll
-      for (int j = 0; j < QR; ++j) {
-        if (r0 + j * nqb * RPP >= rows) break;  // uniform
-        const int64_t row = sq.begin + tok[j];
-        norm_rotate<T, D>(x[j], li, p, p.wq ? w : nullptr, p.positions ? *(p.positions + row) : sq.old + tok[j]);
-        if (r0 + j * nqb * RPP + rt < rows) {
-          T* o = static_cast<T*>(p.q_out) + row * p.qo_st + h[j] * p.qo_sh + 4 * li;
-          *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(x[j][0], x[j][1]), pack2<T>(x[j][2], x[j][3]));
-          *reinterpret_cast<uint2*>(o + D / 2) = make_uint2(pack2<T>(x[j][4], x[j][5]), pack2<T>(x[j][6], x[j][7]));
+      for (int h = 0; h < HEADS; ++h) {
+        if (p.wq) norm_row<D>(x[h], p.eps, w);
+        if (p.cos) turn_row(x[h], turn);
+        if (live && h0 + h < H) {
+          T* o = dst + h * p.qo_sh;
+          *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(x[h][0].x, x[h][0].y), pack2<T>(x[h][1].x, x[h][1].y));
+          *reinterpret_cast<uint2*>(o + D / 2) =
+              make_uint2(pack2<T>(x[h][2].x, x[h][2].y), pack2<T>(x[h][3].x, x[h][3].y));
         }
       }
     }
@@ -204,31 +245,34 @@ paged_append_kernel(const PagedAppendParams p, int nqb) {
   const int64_t row0 = sq.begin + first - sq.old;  // packed row of the block's row 0
   const T* src = static_cast<const T*>(isk ? p.k : p.v) + row0 * st + g * (isk ? p.k_sh : p.v_sh);
 
-  float x[PASSES][8];  // rows that are not new: zeros
+  float2 x[PASSES][4];  // rows that are not new: zeros
 #pragma unroll
   for (int j = 0; j < PASSES; ++j) {
     const int r = j * RPP + rt;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
+    for (int i = 0; i < 4; ++i) x[j][i] = make_float2(0.f, 0.f);
     if (r >= lo && r < hi) load_halves<T, D>(src + r * st, li, x[j]);
   }
   float amax = 0.f;
   if (isk && (p.wk || p.cos)) {
-    float w[8];
+    float2 w[4];
     if (p.wk) load_halves<T, D>(static_cast<const T*>(p.wk), li, w);
 #pragma unroll
     for (int j = 0; j < PASSES; ++j) {
       const int r = j * RPP + rt;
       const bool live = r >= lo && r < hi;
-      if (__any_sync(0xffffffffu, live))
-        norm_rotate<T, D>(x[j], li, p, p.wk ? w : nullptr,
-                          p.positions ? (live ? *(p.positions + row0 + r) : 0) : first + r);
+      if (__any_sync(0xffffffffu, live)) {
+        Turn turn;
+        if (p.cos) load_turn<T>(turn, p, p.positions ? (live ? p.positions[row0 + r] : 0) : first + r, li);
+        if (p.wk) norm_row<D>(x[j], p.eps, w);
+        if (p.cos) turn_row(x[j], turn);
+      }
     }
   }
 #pragma unroll
   for (int j = 0; j < PASSES; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max_abs_nan(amax, x[j][i]);
+    for (int i = 0; i < 4; ++i) amax = max_abs_nan(max_abs_nan(amax, x[j][i].x), x[j][i].y);
   __shared__ float red[NW];
   // magnitudes order as integers, NaN above infinity above the rest
   auto reduce = [&]() {
@@ -248,7 +292,7 @@ paged_append_kernel(const PagedAppendParams p, int nqb) {
     for (int j = 0; j < PASSES; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(x[j][i]);
+        const float a = fabsf(i & 1 ? x[j][i >> 1].y : x[j][i >> 1].x);
         if (a <= kMaxFinite) amax = fmaxf(amax, a);
       }
     __syncthreads();
@@ -260,8 +304,10 @@ paged_append_kernel(const PagedAppendParams p, int nqb) {
 #pragma unroll
     for (int j = 0; j < PASSES; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (!(fabsf(x[j][i]) <= kMaxFinite)) x[j][i] = x[j][i] == x[j][i] ? copysignf(top, x[j][i]) : 0.f;
+      for (int i = 0; i < 8; ++i) {
+        float& y = i & 1 ? x[j][i >> 1].y : x[j][i >> 1].x;
+        if (!(fabsf(y) <= kMaxFinite)) y = y == y ? copysignf(top, y) : 0.f;
+      }
   }
   if (s > s_old && lo > 0) {
     const float ratio = __fdiv_rn(s_old, s);
@@ -283,20 +329,25 @@ paged_append_kernel(const PagedAppendParams p, int nqb) {
   if (tid == 0) *sp = s;
 }
 
-template <typename T, int KV, int D, int PAGE>
-cudaError_t append_launch(const PagedAppendParams& p, cudaStream_t st) {
+template <typename T, int KV, int D, int PAGE, int HEADS>
+cudaError_t append_heads(const PagedAppendParams& p, int passes, cudaStream_t st) {
   using S = AppendShape<D, PAGE>;
   const int mt = p.b.max_tokens;
   const int chunks = (int)(((int64_t)mt + PAGE - 2) / PAGE + 1);  // mt tokens touch at most this many blocks
   int nqb = 0;
   if (p.q) {
-    // a few tokens: one pass per CTA (latency); prompts: eight, to amortise the set-up
-    const int64_t rows = (int64_t)(mt < PAGE ? mt : PAGE) * p.b.H;
-    const int per = S::RPP * (mt < 16 ? 1 : 8);
-    nqb = (int)((rows + per - 1) / per);
+    const int64_t items = (int64_t)(mt < PAGE ? mt : PAGE) * ((p.b.H + HEADS - 1) / HEADS);
+    nqb = (int)((items + S::RPP * passes - 1) / (S::RPP * passes));
   }
-  return launch_dependent(paged_append_kernel<T, KV, D, PAGE>, dim3(2 * p.c.G + nqb, chunks, p.b.B), S::NT, 0, st, p,
-                          nqb);
+  return launch_dependent(paged_append_kernel<T, KV, D, PAGE, HEADS>, dim3(2 * p.c.G + nqb, chunks, p.b.B), S::NT, 0,
+                          st, p, nqb);
+}
+
+// A few tokens: a head per row of lanes, one pass per CTA (latency). Prompts:
+// four heads share a token's rotation, four passes share the set-up.
+template <typename T, int KV, int D, int PAGE>
+cudaError_t append_launch(const PagedAppendParams& p, cudaStream_t st) {
+  return p.b.max_tokens < 16 ? append_heads<T, KV, D, PAGE, 1>(p, 1, st) : append_heads<T, KV, D, PAGE, 4>(p, 4, st);
 }
 
 template <typename T, int KV, int D>
