@@ -574,7 +574,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         const int nt = seg.t1 - seg.t0;
         if (nt <= 0) continue;
         if (seg.nrows - seg.r0 <= rt * kRowTile) {
-          n += nt;
+          // not in use: this thread lets the ring go for its row tile, tile by tile (a wait for a phase
+          // further on would take an earlier one of the same parity for it)
+          for (int j = 0; j < nt && ok; ++j, ++n) {
+            ok = mbar_wait(kv_full[n % kRing], (n / kRing) & 1, kErr | 7, abort);
+            if (ok) mbar_arrive(kv_empty[n % kRing]);
+          }
           continue;
         }
         ok = mbar_wait(q_full[rt], nq++ & 1, kErr | 6, abort);
@@ -599,16 +604,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
       const uint32_t d = tmem + 4 * kKeys + rt * D;
       while (ok && seg.next()) {
         const int nt = seg.t1 - seg.t0;
-        const bool used = seg.nrows - seg.r0 > rt * kRowTile;
+        if (seg.nrows - seg.r0 <= rt * kRowTile) {
+          n += max(nt, 0);
+          continue;
+        }
         for (int j = 0; j < nt && ok; ++j, ++n) {
           const uint32_t st = n % kRing;
-          ok = mbar_wait(kv_full[st], (n / kRing) & 1, kErr | 7, abort);
-          if (!ok) break;
-          if (!used) {  // (after the stage was filled: an arrival counts for its own phase)
-            mbar_arrive(kv_empty[st]);
-            continue;
-          }
-          ok = mbar_wait(w_full[rt], c & 1, kErr | 9, abort);
+          // W first: with it the tile's stage is full and stays so until the arrival below
+          ok = mbar_wait(w_full[rt], c & 1, kErr | 9, abort) &&
+               mbar_wait(kv_full[st], (n / kRing) & 1, kErr | 7, abort);
           if (!ok) break;
           tc_fence_after();
           const uint64_t v = smem_desc_sw128(smem_u32(sm + L::oKV + st * 2 * L::kTileBytes + L::kTileBytes), kKeys * 128, 1024);

@@ -663,3 +663,23 @@ def test_attention_captured_over_changing_pieces():
         gr.replay()
         torch.cuda.synchronize()
         _check_attend(out, q, cache, table, _cum(news), lens, D ** -0.5)
+
+
+@pytest.mark.parametrize("kv,D,R,n,last", [(I8, 128, 2, 150, 150), (E4, 64, 2, 150, 129), (I8, 128, 3, 171, 40)])
+def test_attention_pieces_many_lines(kv, D, R, n, last):
+    """More lines of query rows than CTAs, every other with one row tile of two
+    in use, so that a CTA goes from one kind to the other."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(26)
+    G, page, B = 8, 64, 12
+    news = [n] * (B - 1) + [last]
+    lens = [x + 64 * b + 30 for b, x in enumerate(news)]
+    mp = max(lens) // page + 1
+    table, cu = _table(B, mp, B * mp, g), _cum(news)
+    cache = _filled(kv, B * mp, G, page, D, g)
+    q = torch.randn(cu[-1], G * R, D, generator=g).to(F16).cuda()
+    out = paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), max(news))
+    _check_attend(out, q, cache, table, cu, lens, D ** -0.5)
+    for _ in range(5):
+        assert torch.equal(paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), max(news)), out)
+    assert _device_error() == 0
