@@ -20,7 +20,7 @@
 //   warps 0-3, 4-7  softmax of the two row tiles: S from tensor memory, W into
 //                   shared memory (swizzled), rescaling, the epilogue and the
 //                   next queries;
-//   warps 8-11      codes to f16: 16-byte loads two tiles ahead, widened into a
+//   warps 8-11      codes to f16: 16-byte loads a tile ahead, widened into a
 //                   ring of K / V tiles in the layouts that the MMAs read (K
 //                   K-major, V MN-major: both [64-dim block][key][128 B]);
 //   warps 12-15     MMA issue, one thread each: S and O of the two row tiles (one
@@ -52,7 +52,7 @@ constexpr int kRowTile = 128, kRowsCta = 256, kKeys = 64, kRing = 3;
 constexpr int kSoftWarps = 8, kWideWarps = 8, kMmaWarps = 4,
               kThreads = 32 * (kSoftWarps + kWideWarps + kMmaWarps);
 // registers per thread at launch, and of each role after setmaxnreg
-constexpr int kRegs = 96, kSoftRegs = 144, kWideRegs = 72, kMmaRegs = 48;
+constexpr int kRegs = 96, kSoftRegs = 144, kWideRegs = 64, kMmaRegs = 64;
 static_assert(kSoftWarps * kSoftRegs + kWideWarps * kWideRegs + kMmaWarps * kMmaRegs ==
                   (kSoftWarps + kWideWarps + kMmaWarps) * kRegs,
               "the roles share what the block was launched with");
@@ -550,15 +550,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
     t = -1;
     seg.t1 = 0;  // before the first segment
     advance();
-    Hold x, y;
+    Hold x;
     load(x);
-    load(y);
-    while (true) {
-      if (!x.valid || !store(x)) break;
-      load(x);
-      if (!y.valid || !store(y)) break;
-      load(y);
-    }
+    while (x.valid && store(x)) load(x);
   } else {
     // ------------------------------------------------------------ MMA issue
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs) : "memory");
