@@ -564,6 +564,14 @@ static int check_rows(const char* who, const char* name, const void* x, int64_t 
   return SPATTEN_OK;
 }
 
+// ... that is written: distinct rows
+static int check_out_rows(const char* who, const char* name, const void* x, int64_t st, int64_t sh, int T, int H,
+                          int D) {
+  if (int e = check_rows(who, name, x, st, sh)) return e;
+  if ((T > 1 && st < D) || (H > 1 && sh < D)) return fail(SPATTEN_ERR_INVALID, "%s: rows of %s overlap", who, name);
+  return SPATTEN_OK;
+}
+
 int spatten_paged_append(const spatten_paged_append_args* a, void* stream) {
   static const char* who = "paged_append";
   if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
@@ -579,7 +587,7 @@ int spatten_paged_append(const spatten_paged_append_args* a, void* stream) {
   if (a->q) {
     if (a->H < 1 || a->H > 65536) return fail(SPATTEN_ERR_INVALID, "%s: H=%d query heads", who, a->H);
     if (int e = check_rows(who, "q", a->q, a->q_st, a->q_sh)) return e;
-    if (int e = check_rows(who, "q_out", a->q_out, a->qo_st, a->qo_sh)) return e;
+    if (int e = check_out_rows(who, "q_out", a->q_out, a->qo_st, a->qo_sh, a->T, a->H, p.c.D)) return e;
     if (!a->q_norm_w != !a->k_norm_w) return fail(SPATTEN_ERR_INVALID, "%s: one of q_norm_w, k_norm_w", who);
   } else if (a->q_norm_w || a->q_out) {
     return fail(SPATTEN_ERR_INVALID, "%s: q_norm_w or q_out without q", who);
@@ -647,7 +655,7 @@ int spatten_paged_attend(const spatten_paged_attend_args* a, void* workspace, si
   if (int e = fill_paged_attend(a, p)) return e;
   if (p.b.B == 0 || p.b.max_tokens == 0) return ok();
   if (int e = check_rows(who, "q", a->q, a->q_st, a->q_sh)) return e;
-  if (int e = check_rows(who, "out", a->out, a->o_st, a->o_sh)) return e;
+  if (int e = check_out_rows(who, "out", a->out, a->o_st, a->o_sh, a->T, a->H, p.c.D)) return e;
   const size_t need = align256(spatten::paged_attend_workspace(p, sm_count()));
   if (need > 0) {
     if (!workspace || workspace_bytes < need)

@@ -82,7 +82,7 @@ def test_bad_cache(kind, field, value, code):
     ("v_st", 260, N.ERR_INVALID), ("k_sh", -128, N.ERR_INVALID), ("q_out", 0, N.ERR_INVALID),
     ("q", 0, N.ERR_INVALID), ("H", 0, N.ERR_INVALID), ("q_norm_w", 1 << 20, N.ERR_INVALID),
     ("k_norm_w", 1 << 20, N.ERR_INVALID), ("cos", 0, N.ERR_INVALID), ("cs_dtype", N.DTYPE_F16, N.ERR_UNSUPPORTED),
-    ("cs_rows", 0, N.ERR_INVALID), ("cs_stride", 60, N.ERR_INVALID), ("positions", (1 << 20) + 1, N.ERR_INVALID),
+    ("qo_st", 0, N.ERR_INVALID), ("qo_sh", 64, N.ERR_INVALID), ("cs_rows", 0, N.ERR_INVALID), ("cs_stride", 60, N.ERR_INVALID), ("positions", (1 << 20) + 1, N.ERR_INVALID),
 ])
 def test_bad_append(field, value, code):
     assert N.lib.spatten_paged_append(_append(**{field: value}), None) == code
@@ -101,6 +101,7 @@ def test_bad_append_norm():
     ("H", 2 * 129, N.ERR_UNSUPPORTED), ("q", 0, N.ERR_INVALID), ("out", (1 << 20) + 8, N.ERR_INVALID),
     ("q_st", 1020, N.ERR_INVALID), ("o_sh", 4, N.ERR_INVALID), ("sm_scale", float("nan"), N.ERR_INVALID),
     ("cu_tokens", 0, N.ERR_INVALID), ("B", 70000, N.ERR_UNSUPPORTED), ("T", -2, N.ERR_INVALID),
+    ("B", 8193, N.ERR_UNSUPPORTED), ("o_st", 0, N.ERR_INVALID), ("o_sh", 64, N.ERR_INVALID),
 ])
 def test_bad_attend(field, value, code):
     assert N.lib.spatten_paged_attend(_attend(**{field: value}), None, 0, None) == code
