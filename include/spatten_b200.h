@@ -243,15 +243,16 @@ int spatten_decode_attend(const spatten_decode_args* a, void* workspace, size_t 
  * [0, num_pages) has no memory: nothing is appended there, and its slots
  * are no keys. page_size is 16, 32, 64 or 128; D is 64 or 128.
  *
- * Codes are finite in both types: int8 (scale = max|x| / 127) or e4m3
- * (scale = the smallest power of two with max|x| <= 448 * scale, so that
- * dividing by it is exact).
+ * Scales are not negative, and codes are finite in both types: int8
+ * (scale = max|x| / 127) or e4m3 (scale = the smallest power of two with
+ * max|x| <= 448 * scale, so that dividing by it is exact).
  *
  * A batch's new tokens are packed: sequence b brings the rows cu_tokens[b]
  * .. cu_tokens[b+1]-1 (int32 [B+1], ascending, within [0, T]) of q / k / v /
  * out, and holds seq_lens[b] tokens in all (int32 [B]), these included, which
  * are its last ones: row cu_tokens[b] + i is slot
- * seq_lens[b] - (cu_tokens[b+1] - cu_tokens[b]) + i. max_tokens bounds the
+ * seq_lens[b] - (cu_tokens[b+1] - cu_tokens[b]) + i. A sequence whose bounds
+ * descend or leave [0, T] brings no rows. max_tokens bounds the
  * tokens of one sequence (rows beyond it are left alone), so that the launch
  * needs no device value on the host; it sizes the grid. Rows behind the last
  * sequence are neither read nor written. All of these may change between the

@@ -243,12 +243,15 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   uint32_t* pre = reinterpret_cast<uint32_t*>(dsm + SH::kRing);  // [B + 1] units before each sequence
   __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS], sm_M[kWarps][ROWS];
   __shared__ uint32_t scan[2 * kWarps];
+  __shared__ unsigned long long scan_most[kWarps];
   grid_dependents();
   grid_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
   const int G = p.c.G, R = p.b.H / G, page = p.c.page, page_log = __ffs(page) - 1;
 
-  // tiles and lines in all (the host made sure of 32 bits)
+  // tiles and lines in all. The host made sure of 32 bits for sequences
+  // that share no rows; others may need more, and then nothing is done.
+  unsigned long long most = 0;
   uint32_t U = 0, lines = 0;
   auto tiles_of = [&](int b, uint32_t& n) {  // key tiles of a line of sequence b, and its lines
     n = 0;
@@ -266,18 +269,24 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       k0 = k;
     }
     const uint32_t x = __reduce_add_sync(0xffffffffu, n * k), y = __reduce_add_sync(0xffffffffu, n);
+    unsigned long long z = (unsigned long long)n * (k + kLineCost);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
     if (lane == 0) {
       scan[warp] = x;
       scan[kWarps + warp] = y;
+      scan_most[warp] = z;
     }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       U += scan[w];
       lines += scan[kWarps + w];
+      most += scan_most[w];
     }
     __syncthreads();
   }
+  if (most >> 32) U = lines = 0;
   // chunk: tiles per unit. ceil(tiles / chunk) summed over the lines is at most
   // U / chunk + lines, so with few lines every unit has a CTA.
   const bool few = lines * 8 <= gridDim.x;
@@ -307,6 +316,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     if (base + tid < p.b.B) pre[base + tid + 1] = before + x;
     __syncthreads();
   }
+  if (most >> 32) U = 0;
   const uint32_t cta = blockIdx.x;
   const uint32_t ctas = min(gridDim.x, few ? U : (U + kWarps - 1) / kWarps);
   PagedCut cut = {};

@@ -76,8 +76,8 @@ struct Lay {
   static constexpr int kNumBars = 2 * kRing + 4 + 4 + 2 + 2 + 2 + 4;
   static constexpr int oTmem = oBar + kNumBars * 8;
   static constexpr int oAbort = oTmem + 4;
-  static constexpr int oScan = oAbort + 4;                // [32]
-  static constexpr int oPre = oScan + 128;                // [B + 1]
+  static constexpr int oScan = (oAbort + 4 + 7) & ~7;     // [32] 64-bit
+  static constexpr int oPre = oScan + 256;                // [B + 1]
   static constexpr int bytes(int B) { return oPre + (B + 1) * 4 + 1024; }
 };
 
@@ -120,30 +120,32 @@ struct Segments {
   uint32_t u0, line;     // the segment's first unit; units of the line
 
   SPATTEN_DEV static uint32_t tokens_per_tile(int R) { return (kRowsCta + R - 1) / R; }
-  // units of row tiles 0 .. rt - 1 of a sequence
-  SPATTEN_DEV static uint32_t before(const PagedSeq& s, uint32_t rt, uint32_t tok) {
-    return rt * (max(s.old, 0) + kLineCost) + tok * (rt * (rt + 1) / 2);
+  // units of row tiles 0 .. rt - 1 of a sequence (`old` within the page table)
+  template <typename U = uint32_t>
+  SPATTEN_DEV static U before(const PagedAttendParams& p, const PagedSeq& s, uint32_t rt, uint32_t tok) {
+    const uint32_t old = min(max(s.old, 0), p.c.max_pages * p.c.page);
+    return U(rt) * (old + kLineCost) + tok * (U(rt) * (rt + 1) / 2);
   }
   SPATTEN_DEV static uint32_t row_tiles(const PagedSeq& s, int R) { return ((uint32_t)s.n * R + kRowsCta - 1) / kRowsCta; }
-  SPATTEN_DEV static uint32_t units(const PagedSeq& s, int R) {
-    return before(s, row_tiles(s, R), tokens_per_tile(R));
+  SPATTEN_DEV static unsigned long long units(const PagedAttendParams& p, const PagedSeq& s, int R) {
+    return before<unsigned long long>(p, s, row_tiles(s, R), tokens_per_tile(R));
   }
 
   SPATTEN_DEV bool next() {
     if (u >= u1) return false;
     while (pre[b + 1] <= u) ++b;
     sq = paged_seq(p.b, p.c, b);
-    const uint32_t tok = tokens_per_tile(R), per = units(sq, R), local = u - pre[b];
+    const uint32_t tok = tokens_per_tile(R), per = before(p, sq, row_tiles(sq, R), tok), local = u - pre[b];
     g = local / per;
     const uint32_t r = local % per;
     uint32_t lo = 0, hi = row_tiles(sq, R);  // the row tile of unit r
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) >> 1;
-      if (before(sq, mid, tok) <= r) lo = mid; else hi = mid;
+      if (before(p, sq, mid, tok) <= r) lo = mid; else hi = mid;
     }
-    const uint32_t v0 = r - before(sq, lo, tok);
+    const uint32_t v0 = r - before(p, sq, lo, tok);
     u0 = u;
-    line = before(sq, lo + 1, tok) - before(sq, lo, tok);
+    line = before(p, sq, lo + 1, tok) - before(p, sq, lo, tok);
     const uint32_t v1 = min(line, v0 + (u1 - u));
     auto tile = [](uint32_t v) { return (int)((max(v, kLineCost) - kLineCost + kKeys - 1) / kKeys); };
     first = v0 == 0;
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
   volatile int* abort = reinterpret_cast<volatile int*>(sm + L::oAbort);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + L::oTmem);
   uint32_t* pre = reinterpret_cast<uint32_t*>(sm + L::oPre);
-  uint32_t* scan = reinterpret_cast<uint32_t*>(sm + L::oScan);
+  unsigned long long* scan = reinterpret_cast<unsigned long long*>(sm + L::oScan);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = p.c.G, R = p.b.H / G;
 
@@ -202,30 +204,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
     tmem_alloc(tslot, 512);
     tmem_relinquish();
   }
-  // prefix sums of the sequences' units (the host made sure of 32 bits)
-  uint32_t U = 0;
+  // prefix sums of the sequences' units. The host made sure of 32 bits
+  // for sequences that share no rows; others may need more, and then nothing is done.
+  unsigned long long U64 = 0;
   for (int base = 0; base < p.b.B; base += kThreads) {
     const int b = base + tid;
-    uint32_t x = 0;
+    unsigned long long x = 0;
     if (b < p.b.B) {
       const PagedSeq s = paged_seq(p.b, p.c, b);
-      if (paged_serves(p, s, R)) x = (uint32_t)G * Segments::units(s, R);
+      if (paged_serves(p, s, R)) x = (unsigned long long)G * Segments::units(p, s, R);
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+      const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
     if (lane == 31) scan[warp] = x;
     __syncthreads();
-    uint32_t front = U;
+    unsigned long long front = U64;
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) front += scan[w];
-      U += scan[w];
+      U64 += scan[w];
     }
-    if (b < p.b.B) pre[b + 1] = front + x;
+    if (b < p.b.B) pre[b + 1] = (uint32_t)(front + x);
     __syncthreads();
   }
+  const uint32_t U = U64 >> 32 ? 0 : (uint32_t)U64;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -713,7 +717,7 @@ bool paged_attend_tc_takes(const PagedAttendParams& p) {
   const int R = p.b.H / p.c.G;
   if ((int64_t)p.b.max_tokens * R <= kTcRows || p.b.B > kMaxBatch) return false;
   const double lines = (double)p.b.T * R / kRowsCta + p.b.B;  // at most
-  return lines * p.c.G * ((double)p.c.max_pages * p.c.page + kRowsCta + kLineCost) < 4e9;
+  return lines * p.c.G * ((double)p.c.max_pages * p.c.page + p.b.max_tokens + kRowsCta + kLineCost) < 4e9;
 }
 
 size_t paged_attend_tc_workspace(const PagedAttendParams& p, int n_sm) {

@@ -44,11 +44,12 @@ struct PagedSeq {
 
 SPATTEN_DEV PagedSeq paged_seq(const PagedBatch& p, const PagedCache& c, int b) {
   PagedSeq s;
-  const int lo = min(max(*(p.cu + b), 0), p.T), hi = min(max(*(p.cu + b + 1), lo), p.T);
+  const int lo = *(p.cu + b), hi = *(p.cu + b + 1);
   const int len = min(max(*(p.lens + b), 0), 1 << 30);
-  s.begin = lo;
-  s.n = min(hi - lo, p.max_tokens);
-  s.old = len - (hi - lo);
+  const int n = lo >= 0 && lo <= hi && hi <= p.T ? hi - lo : 0;  // rows out of order or range: none
+  s.begin = n ? lo : 0;
+  s.n = min(n, p.max_tokens);
+  s.old = len - n;
   s.len = (int)min((int64_t)len, (int64_t)c.max_pages * c.page);
   return s;
 }

@@ -38,6 +38,9 @@ class PagedKVCache(namedtuple("PagedKVCache", "k v k_scale v_scale")):
     contiguous. Its checks and the C form of it are made once, at its first
     use (the tensors of a tuple do not change)."""
 
+    def __reduce__(self):  # copies and pickles make their own C form
+        return PagedKVCache, tuple(self)
+
     @property
     def native(self):
         """(device index, shape of the pool, C form without a page table)."""

@@ -683,3 +683,49 @@ def test_attention_pieces_many_lines(kv, D, R, n, last):
     for _ in range(5):
         assert torch.equal(paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), max(news)), out)
     assert _device_error() == 0
+
+
+@pytest.mark.parametrize("R,n", [(2, 5), (8, 40)])
+def test_index_tensors_out_of_range(R, n):
+    """cu_tokens that leave the rows, descend or claim every row many times,
+    lengths below zero and far beyond the page table: sequences that are in
+    order come out right, nothing is touched outside."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(31)
+    G, D, page, T = 2, 64, 16, 3 * n
+    big = 2 ** 31 - 1
+    cu = [0, n, n, -7, 2 * n, 2 * n - 3, big]
+    lens = [n + 50, 9, -big, 3, big, n]
+    table = _table(6, 8, 60, g)
+    table[5] = -1
+    cache = _filled(I8, 60, G, page, D, g)
+    q = torch.randn(T, G * R, D, generator=g).to(F16).cuda()
+    out = paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), n)
+    _check_attend(out[:n], q[:n], cache, table[:1], cu[:2], lens[:1], D ** -0.5)
+    before = _cpu(cache)
+    x = torch.randn(T, 2 * G, D, generator=g).to(F16).cuda()
+    own = torch.full_like(table, -1)
+    own[0] = table[0]
+    paged.paged_append(cache, x[:, :G], x[:, G:], own.cuda(), _i32(cu), _i32(lens), n)
+    want = O.append(before, x[:n, :G].cpu(), x[:n, G:].cpu(), own[:1], [0, n], lens[:1])
+    _check_append(cache, before, want)
+    k, _ = paged.paged_read(cache, table.cuda(), _i32(lens), n_tokens=140)
+    assert (k[2] == 0).all() and (k[4, 128:] == 0).all()
+    # every sequence claims every row: more work than the numbering holds in earnest, none of it out of range
+    B = 600
+    many = _i32([0 if b % 2 == 0 else T for b in range(B + 1)])
+    out = paged.paged_attention(q, cache, table[:1].expand(B, -1).contiguous().cuda(), many, _i32([n + 50] * B), T)
+    assert out.shape == q.shape and _device_error() == 0
+
+
+def test_copies_of_a_cache():
+    import copy
+    from spatten_b200 import paged
+    c = paged.new_paged_cache(3, 1, 64, page_size=16)
+    t, ln = _i32([[0]]), _i32([4])
+    paged.paged_read(c, t, ln)  # its C form exists
+    d = copy.deepcopy(c)
+    x = torch.ones(4, 1, 64, dtype=F16, device="cuda")
+    paged.paged_append(d, x, x, t, _i32([0, 4]), ln, 4)
+    assert (c.k == 0).all() and (d.k[0, 0, :4] == 127).all()
+    assert copy.copy(d).k.data_ptr() == d.k.data_ptr()
