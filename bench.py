@@ -888,7 +888,52 @@ def ours_arm(args, torch, rank, world, local_rank):
 
 
 MICRO_KERNELS = ("quant_q", "quant_k", "topk_decode", "topk_cascade", "gather", "op", "compat",
-                 "f32", "qk_norm_rope", "qkv_proj", "out_proj", "layer_norm")
+                 "f32", "qk_norm_rope", "qkv_proj", "out_proj", "layer_norm", "paged_append", "paged_read", "paged_attend",
+                 "paged_attend_e4m3", "paged_pieces")
+
+
+def paged_micro(torch, dev, name, g):
+    """(call, info) of a paged-cache micro case: Qwen3-8B's attention heads (32
+    query, 8 KV, 128 wide), pages of 64 tokens in shuffled order."""
+    from spatten_b200 import paged
+    H, G, d, page = 32, 8, 128, 64
+    rn = lambda *shape: torch.randn(*shape, generator=g, device=dev, dtype=torch.bfloat16)  # noqa: E731
+
+    def batch(b, held, new, kv=torch.int8):
+        mp = -(-held // page)
+        c = paged.new_paged_cache(b * mp, G, d, page, kv, dev)
+        for t in c[:2]:
+            t.view(torch.int8).random_(-100, 100, generator=g)
+        for t in c[2:]:
+            t.fill_(0.02)
+        i32 = dict(dtype=torch.int32, device=dev)
+        return (c, torch.randperm(b * mp, device=dev).to(torch.int32).view(b, mp),
+                torch.arange(0, (b + 1) * new, new, **i32), torch.full((b,), held, **i32))
+
+    if name == "paged_append":
+        c, table, cu, lens = batch(4, 8192, 8192)
+        qkv = rn(4 * 8192, H + 2 * G, d)
+        w = torch.ones(d, dtype=torch.bfloat16, device=dev)
+        ang = torch.arange(8192, device=dev)[:, None] * 1e6 ** (-torch.arange(0, d, 2, device=dev) / d)
+        cos, sin = ang.cos(), ang.sin()
+        return (lambda: paged.paged_append(c, qkv[:, H:H + G], qkv[:, H + G:], table, cu, lens, 8192, q=qkv[:, :H],
+                                           cos=cos, sin=sin, q_norm_w=w, k_norm_w=w)), \
+            dict(case="4 prompts of 8192 tokens: QK-norm, rotation, int8 append", bytes=4 * 8192 * d * (4 * H + 6 * G))
+    if name == "paged_read":
+        c, table, cu, lens = batch(64, 8192, 1)
+        idx = torch.rand(64, 8192, generator=g, device=dev).topk(2048, dim=1).indices.sort(1).values
+        return (lambda: paged.paged_read(c, table, lens, idx=idx)), \
+            dict(case="2048 kept of 8192 tokens, 64 sequences", bytes=64 * 2048 * (G * d * 6 + 8))
+    if name == "paged_pieces":
+        c, table, cu, lens = batch(2, 8192, 1024)
+        q = rn(2 * 1024, H, d)
+        return (lambda: paged.paged_attention(q, c, table, cu, lens, 1024)), \
+            dict(case="1024 new tokens over 8192, 2 sequences", flops=4 * 2 * 1024 * (8192 - 511.5) * H * d)
+    kv = torch.int8 if name == "paged_attend" else torch.float8_e4m3fn
+    c, table, cu, lens = batch(16, 32768, 1, kv)
+    q = rn(16, H, d)
+    return (lambda: paged.paged_attention(q, c, table, cu, lens, 1)), \
+        dict(case=f"one token per sequence over 32768, 16 sequences, {name}", bytes=16 * 32768 * G * d * 2)
 
 
 def micro_bench(torch, dev, name, steps):
@@ -989,6 +1034,8 @@ def micro_bench(torch, dev, name, steps):
         fn = lambda: add_layer_norm(x, w, b, 1e-12, residual=res)  # noqa: E731
         info = dict(case="BERT-base residual add + LayerNorm, 32 x 461 rows x 768 fp16",
                     bytes=3 * x.numel() * 2 + 2 * 768 * 2)
+    elif name.startswith("paged_"):
+        fn, info = paged_micro(torch, dev, name, g)
     else:
         raise ValueError(f"--micro {name}: one of {', '.join(MICRO_KERNELS)}")
     for _ in range(3):
