@@ -24,10 +24,10 @@ namespace {
 
 constexpr float kMaxFinite = 3.402823466e38f;
 
-// The larger magnitude, NaN when either is.
-SPATTEN_DEV float max_abs_nan(float a, float x) {
+// The largest magnitude, NaN when one is.
+SPATTEN_DEV float max_abs_nan(float a, float x, float y) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(x)));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(x), "f"(y));
   return r;
 }
 
@@ -47,28 +47,26 @@ SPATTEN_DEV float scale_for(float amax) {
 }
 
 // Eight finite values over the block's scale (not 0), as codes; rc = 1 / s.
-// int8: y = x rc lands within 2 ulp of x / s, so its rounding can only differ
-// from the division's near a tie; the distance to the rounded value is kept as a
-// maximum over the eight, and near a tie (or for the NaN that a subnormal scale's
-// reciprocal makes) they take the division. y + 1.5 2^23 holds the rounded
-// integer's low byte in its own.
+// int8: x rc (1 - 2^-20) and x rc (1 + 2^-20) enclose the rounded x / s, whose
+// rounding is theirs where they agree; where one of the eight disagrees (near a
+// tie, or with the infinity that a subnormal scale's reciprocal makes), they take
+// the division. x rc + 1.5 2^23 holds the rounded integer's low byte in its own.
 template <int KV>
 SPATTEN_DEV uint2 encode8(const float2 (&x)[4], float s, float rc) {
   uint32_t w[2];
   if constexpr (KV == kKvInt8) {
     constexpr float kRound = 12582912.0f;
-    const float2 r2 = make_float2(rc, rc), up = make_float2(kRound, kRound), down = make_float2(-kRound, -kRound);
-    float far = 0.f;
-    uint32_t b[8];
+    const float below = rc * (1.f - 0x1p-20f), above = rc * (1.f + 0x1p-20f);
+    const float2 r0 = make_float2(below, below), r1 = make_float2(above, above), up = make_float2(kRound, kRound);
+    uint32_t b[8], differ = 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 y = __fmul2_rn(x[i], r2), f = __fadd2_rn(y, up), t = __fadd2_rn(f, down);
-      const float2 d = __fadd2_rn(y, make_float2(-t.x, -t.y));
-      far = max_abs_nan(max_abs_nan(far, d.x), d.y);
+      const float2 f = __ffma2_rn(x[i], r0, up), t = __ffma2_rn(x[i], r1, up);
       b[2 * i] = __float_as_uint(f.x);
       b[2 * i + 1] = __float_as_uint(f.y);
+      differ |= (b[2 * i] ^ __float_as_uint(t.x)) | (b[2 * i + 1] ^ __float_as_uint(t.y));
     }
-    if (!(far <= 0.49990f)) {
+    if (differ || !(above <= kMaxFinite)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         b[2 * i] = (uint32_t)__float2int_rn(__fdiv_rn(x[i].x, s));
@@ -125,9 +123,9 @@ SPATTEN_DEV void load_halves(const T* row, int li, float2 (&f)[4]) {
   f[3] = unpack2<T>(b.y);
 }
 
-// A lane's part of the rotation by a position: cos, sin and -sin of its pairs.
+// A lane's part of the rotation by a position: cos and sin of its pairs.
 struct Turn {
-  float2 c[2], s[2], n[2];
+  float2 c[2], s[2];
 };
 
 template <typename T>
@@ -144,8 +142,6 @@ SPATTEN_DEV void load_turn(Turn& r, const PagedAppendParams& p, int pos, int li)
     r.c[0] = unpack2<T>(a.x); r.c[1] = unpack2<T>(a.y);
     r.s[0] = unpack2<T>(b.x); r.s[1] = unpack2<T>(b.y);
   }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) r.n[i] = make_float2(-r.s[i].x, -r.s[i].y);
 }
 
 // Norm (g: the lane's weights) of one row spread over D / 8 lanes, all lanes of
@@ -167,7 +163,7 @@ SPATTEN_DEV void turn_row(float2 (&x)[4], const Turn& r) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float2 a = x[i], b = x[2 + i];
-    x[i] = __fadd2_rn(__fmul2_rn(a, r.c[i]), __fmul2_rn(b, r.n[i]));
+    x[i] = __fadd2_rn(__fmul2_rn(a, r.c[i]), __fmul2_rn(b, make_float2(-r.s[i].x, -r.s[i].y)));
     x[2 + i] = __fadd2_rn(__fmul2_rn(b, r.c[i]), __fmul2_rn(a, r.s[i]));
   }
 }
@@ -257,13 +253,21 @@ paged_append_kernel(const PagedAppendParams p, int nqb) {
   if (isk && (p.wk || p.cos)) {
     float2 w[4];
     if (p.wk) load_halves<T, D>(static_cast<const T*>(p.wk), li, w);
+    // a pass ahead where there are several: a row's rotation is a load of its own
+    Turn ahead;
+    auto used = [&](int j) { return j < PASSES && hi > j * RPP && lo < (j + 1) * RPP; };
+    auto fetch = [&](int j) {
+      const int r = j * RPP + rt;
+      load_turn<T>(ahead, p, p.positions ? (r >= lo && r < hi ? p.positions[row0 + r] : 0) : first + r, li);
+    };
+    constexpr int EARLY = HEADS > 1 ? 1 : 0;
+    if (EARLY && p.cos && used(0)) fetch(0);
 #pragma unroll
     for (int j = 0; j < PASSES; ++j) {
-      const int r = j * RPP + rt;
-      const bool live = r >= lo && r < hi;
-      if (__any_sync(0xffffffffu, live)) {
-        Turn turn;
-        if (p.cos) load_turn<T>(turn, p, p.positions ? (live ? p.positions[row0 + r] : 0) : first + r, li);
+      Turn turn = ahead;
+      if (p.cos && used(j + EARLY)) fetch(j + EARLY);
+      if (!EARLY) turn = ahead;
+      if (used(j)) {
         if (p.wk) norm_row<D>(x[j], p.eps, w);
         if (p.cos) turn_row(x[j], turn);
       }
@@ -272,7 +276,7 @@ paged_append_kernel(const PagedAppendParams p, int nqb) {
 #pragma unroll
   for (int j = 0; j < PASSES; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) amax = max_abs_nan(max_abs_nan(amax, x[j][i].x), x[j][i].y);
+    for (int i = 0; i < 4; ++i) amax = max_abs_nan(amax, x[j][i].x, x[j][i].y);
   __shared__ float red[NW];
   // magnitudes order as integers, NaN above infinity above the rest
   auto reduce = [&]() {
@@ -344,10 +348,11 @@ cudaError_t append_heads(const PagedAppendParams& p, int passes, cudaStream_t st
 }
 
 // A few tokens: a head per row of lanes, one pass per CTA (latency). Prompts:
-// four heads share a token's rotation, four passes share the set-up.
+// four heads share a token's rotation (two at a time: 168 -> 182 us at 4 prompts
+// of 8192 tokens), two passes the set-up (one: 173 us).
 template <typename T, int KV, int D, int PAGE>
 cudaError_t append_launch(const PagedAppendParams& p, cudaStream_t st) {
-  return p.b.max_tokens < 16 ? append_heads<T, KV, D, PAGE, 1>(p, 1, st) : append_heads<T, KV, D, PAGE, 4>(p, 4, st);
+  return p.b.max_tokens < 16 ? append_heads<T, KV, D, PAGE, 1>(p, 1, st) : append_heads<T, KV, D, PAGE, 4>(p, 2, st);
 }
 
 template <typename T, int KV, int D>
