@@ -2,22 +2,27 @@
 //
 // One pass over the cache. The R = H / G query heads of a KV head and the n
 // new tokens of a sequence make n R query rows that share the keys; a row tile
-// is 8 or 16 of them. Per 16 keys, on the tensor cores with f16 operands (every
-// int8 and e4m3 code is an f16) and fp32 sums:
+// is 8 or 16 of them. Per 16 keys, on the tensor cores:
 //   S^T [16 keys x 8 rows]  = K codes . q'^T,
-//   O^T [D x 8 rows]       += V codes^T . P^T.
-// Both operands of the cache go from global memory into the fragments'
-// registers: the order of the contracted dims (of S) and of the output dims (of
-// O) is free, so each lane owns 16 consecutive bytes of a row, no shared memory
-// is needed, and every byte is read once per row tile. P^T turns from the
-// layout of S^T into that of an operand with one 8x8 transpose (movmatrix).
+//   O^T [D x 8 rows]       += V codes^T . P^T   (f16, every code is one; fp32 sums).
+// A warp's tiles come through a ring of its own (cp.async, three tiles in
+// flight; through registers the largest case below took 782 us). The order of the contracted dims (of S) and of the output
+// dims (of O) is free, so each lane reads 16 consecutive bytes of a row and takes
+// them as fragments as they are, and every byte is read once per row tile. P^T
+// turns from the layout of S^T into that of an operand with one 8x8 transpose
+// (movmatrix).
+//
+// Bound by HBM where there are keys enough: 64 sequences x 8 heads x 32768 keys
+// of int8, 671 us = 6.40 TB/s, 0.98 of the measured copy rate; one sequence of
+// 131001, 53 us = 5.07 TB/s; 48 ragged ones of up to 8192, 80 us = 5.2 TB/s. One of 777
+// takes 8.4 us, which is the chain of dependent loads and the second launch.
 //
 // Numerics:
-//  * q' = q 2^e with the row's largest element in [2^14, 2^15): f16 then holds
-//    bf16's range to 2^-39 of the row's largest element.
-//  * s = (q' . codes) (sm_scale log2(e) 2^-e k_scale) in fp32, p = 2^(s - m) with
-//    a reference m that follows the row's maximum (updated when it is exceeded
-//    by more than 2^kSlack); l sums p in fp32.
+//  * q' is the query row in what K's product takes: two int8 terms beside int8
+//    codes, a scaled f16 beside e4m3 (Operands).
+//  * s = (q' . codes) (sm_scale log2(e) k_scale / the row's factor) in fp32, p =
+//    2^(s - m) with a reference m that follows the row's maximum (updated when it is
+//    exceeded by more than kSlack); l sums p in fp32.
 //  * P is rounded to f16 for the second product (2^-11 of each weight), after
 //    v_scale has gone into it: w = 2^(s + log2 v_scale - M), M a second reference
 //    that follows max(s + log2 v_scale). A block with a tiny scale and all the weight
@@ -26,8 +31,8 @@
 // Work split, over one wave of resident CTAs and from the lengths on the device,
 // so that a ragged batch and one long sequence fill the GPU alike and a captured
 // launch follows the lengths it finds. A line is a (sequence, KV head, row tile).
-// Few lines: each is cut into chunks of equal length, one per CTA. Many: the
-// lines' units (16-key tiles, plus kLineCost for a line's set-up) are numbered and
+// Few lines: each is cut into chunks of equal length, one per CTA (16 sequences x 8
+// heads over up to 1000 keys: 22 -> 18 us). Many: the lines' units (16-key tiles, plus kLineCost for a line's set-up) are numbered and
 // cut into equal ranges, one per CTA. The four warps of a
 // CTA take turns on its tiles and join in shared memory; a (sequence, head, row
 // tile) that a range's border cuts leaves (m, l, M, o) partials in the workspace,
@@ -43,7 +48,10 @@ namespace spatten {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr uint32_t kLineCost = 8;   // what a line's set-up takes, in tiles (3 us of 0.35 us tiles)
+// What a line's set-up takes, in tiles (its chain of dependent loads and the
+// join of the warps). Measured: 8 tiles are 7 % slower at 64 sequences of up to
+// 2000 keys, 24 tiles 2 % at 48 of up to 8192.
+constexpr uint32_t kLineCost = 16;
 constexpr float kSlack = 8.f;       // p and w stay below 2^8
 constexpr float kNoScale = -200.f;  // log2 of a scale of 0: below that of any float
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
@@ -289,7 +297,10 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   if (most >> 32) U = lines = 0;
   // chunk: tiles per unit. ceil(tiles / chunk) summed over the lines is at most
   // U / chunk + lines, so with few lines every unit has a CTA.
-  const bool few = lines * 8 <= gridDim.x;
+  // It takes U lines / (grid (grid - lines)) tiles more than an equal share, and
+  // saves most CTAs a line's set-up.
+  const bool few = lines * 2 <= gridDim.x &&
+                   (float)U * lines <= (float)kLineCost * gridDim.x * (gridDim.x - lines);
   const uint32_t chunk = few ? max((U + gridDim.x - lines - 1) / (gridDim.x - lines), (uint32_t)kWarps) : 1;
   const uint32_t lead = few ? 0 : kLineCost;
   auto units_of = [&](uint32_t k) { return few ? (k + chunk - 1) / chunk : k + lead; };
