@@ -16,25 +16,34 @@
 // of w times it (one exponential per score), except where w could underflow
 // under it, which takes the exponentials of p.
 //
-// 16 warps, one CTA per SM:
-//   warps 0-3, 4-7  softmax of the two row tiles: S from tensor memory, W into
-//                   shared memory (swizzled), rescaling, the epilogue and the
-//                   next queries;
-//   warps 8-11      codes to f16: 16-byte loads a tile ahead, widened into a
+// 20 warps, one CTA per SM:
+//   warps 0-3, 4-7  softmax of the two row tiles: S from tensor memory, W into the
+//                   columns that S came from, rescaling, the epilogue and the next
+//                   queries;
+//   warps 8-15      codes to f16: 16-byte loads a tile ahead, widened into a
 //                   ring of K / V tiles in the layouts that the MMAs read (K
 //                   K-major, V MN-major: both [64-dim block][key][128 B]);
-//   warps 12-15     MMA issue, one thread each: S and O of the two row tiles (one
+//   warps 16-19     MMA issue, one thread each: S and O of the two row tiles (one
 //                   thread for all took 3600 of a tile's 4450 cycles).
 // A tile's codes are widened once for 256 rows, and two row tiles keep the
-// tensor cores busy through each other's softmax. What bounds it: shared-memory
-// traffic of the operands (a 128 x 64 x 16 step reads 6 KB) and the softmax's
-// exponentials (16 per clock and SM), at similar rates.
+// tensor cores busy through each other's softmax. S has two buffers per row tile, so
+// that the next S and the product with W run under a tile's exponentials; with W
+// in one shared-memory buffer a tile's exponentials had to wait for the product of
+// the tile before (512 new tokens over 32768: 376 us instead of 320).
+//
+// 512 new tokens over 32768 (32 heads, 8 KV heads, D = 128, int8): 320 us, 854
+// TFLOP/s, 0.51 of the measured bf16 rate; 1024 over 8192, 2 sequences, e4m3: 360 us,
+// 714 TFLOP/s; a prompt of 4096: 270 us, 507 TFLOP/s. What bounds it: one thread per
+// row takes a tile's 64 scores through a chain of load, maximum, exponentials and
+// store that two warps per scheduler do not hide; then a line's set-up (queries,
+// the first tile, the epilogue).
 //
 // Work split: as in paged_attend.cu, ranges of equal length over all CTAs, here in
 // keys: row tile rt of a sequence counts old + (rt + 1) 256 / R of them (the causal
 // triangle) and kLineCost, cumulated in closed form, and the 64-key tile at
-// position k belongs to the CTA that holds unit kLineCost + k of its line. Every wait is bounded; a timeout
-// records a code in this file's device error word and the CTA winds down.
+// position k belongs to the CTA that holds unit kLineCost + k of its line. Every
+// wait is bounded; a timeout records a code in this file's device error word and
+// the CTA winds down.
 #include <atomic>
 #include <cmath>
 
@@ -48,7 +57,7 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kRowTile = 128, kRowsCta = 256, kKeys = 64, kRing = 3;
+constexpr int kRowTile = 128, kRowsCta = 256, kKeys = 64, kRing = 4;
 constexpr int kSoftWarps = 8, kWideWarps = 8, kMmaWarps = 4,
               kThreads = 32 * (kSoftWarps + kWideWarps + kMmaWarps);
 // registers per thread at launch, and of each role after setmaxnreg
@@ -66,14 +75,12 @@ template <int D>
 struct Lay {
   static constexpr int kTileBytes = kKeys * D * 2;       // K or V, f16
   static constexpr int kQBytes = kRowTile * D * 2;
-  static constexpr int kWBytes = kRowTile * kKeys * 2;
   static constexpr int oQ = 0;                            // [2][D / 64][128][128 B]
   static constexpr int oKV = oQ + 2 * kQBytes;            // [ring][K | V][D / 64][64][128 B]
-  static constexpr int oW = oKV + kRing * 2 * kTileBytes; // [2][128][128 B]
-  static constexpr int oScale = oW + 2 * kWBytes;         // [ring][ks 4, log2 vs 4, have]
+  static constexpr int oScale = oKV + kRing * 2 * kTileBytes;  // [ring][ks 4, log2 vs 4, have]
   static constexpr int kScaleStride = 48;
   static constexpr int oBar = oScale + kRing * kScaleStride;
-  static constexpr int kNumBars = 2 * kRing + 4 + 4 + 2 + 2 + 2 + 4;
+  static constexpr int kNumBars = 2 * kRing + 4 + 4 + 4 + 2 + 4;
   static constexpr int oTmem = oBar + kNumBars * 8;
   static constexpr int oAbort = oTmem + 4;
   static constexpr int oScan = (oAbort + 4 + 7) & ~7;     // [32] 64-bit
@@ -81,6 +88,14 @@ struct Lay {
   static constexpr int bytes(int B) { return oPre + (B + 1) * 4 + 1024; }
 };
 
+SPATTEN_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 SPATTEN_DEV void tmem_st32f(uint32_t taddr, const float* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -172,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
   uint8_t* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const uint32_t bars = smem_u32(sm + L::oBar);
   const SBarArr kv_full{bars}, kv_empty{bars + 8 * kRing}, s_full{bars + 16 * kRing}, s_empty{bars + 16 * kRing + 32},
-      w_full{bars + 16 * kRing + 64}, o_done{bars + 16 * kRing + 80}, q_full{bars + 16 * kRing + 96},
+      w_full{bars + 16 * kRing + 64}, q_full{bars + 16 * kRing + 96},
       drain{bars + 16 * kRing + 112};
   volatile int* abort = reinterpret_cast<volatile int*>(sm + L::oAbort);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + L::oTmem);
@@ -188,13 +203,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
     }
     for (int i = 0; i < 4; ++i) {  // [row tile][buffer]
       mbar_init(s_full[i], 1);
-      mbar_init(s_empty[i], 4);
-    }
-    for (int i = 0; i < 2; ++i) {
       mbar_init(w_full[i], 4);
-      mbar_init(o_done[i], 1);
-      mbar_init(q_full[i], 4);
+      mbar_init(s_empty[i], 1);  // the product with W, which lies in S's columns, is done
     }
+    for (int i = 0; i < 2; ++i) mbar_init(q_full[i], 4);
     for (int i = 0; i < kMmaWarps; ++i) mbar_init(drain[i], 1);
     fence_barrier_init();
     *abort = 0;
@@ -321,9 +333,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         tmem_ld32f(ts + buf * kKeys, s);
         tmem_ld32f(ts + buf * kKeys + 32, s + 32);
         tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        mbar_arrive_elect(s_empty[2 * rt + buf]);
         const float4 ks = *reinterpret_cast<const float4*>(sm + L::oScale + st * L::kScaleStride);
         const float4 lv4 = *reinterpret_cast<const float4*>(sm + L::oScale + st * L::kScaleStride + 16);
         const uint32_t have = *reinterpret_cast<const uint32_t*>(sm + L::oScale + st * L::kScaleStride + 32);
@@ -359,12 +368,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         const float fo = up ? fast_exp2(M - Mf) : 1.f;
         m = mn;
         M = Mn;
-        // W and O are free once the MMA of the tile before is done
-        if (c > 0) {
-          ok = mbar_wait(o_done[rt], (c - 1) & 1, kErr | 3, abort);
-          if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
-          tc_fence_after();
-        }
         float e[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) e[q] = Mf - lv[q] - mf;
@@ -377,7 +380,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
               l += e[k >> 4] > 90.f ? x : 0.f;
             }
           }
-          if (t > seg.t0) {
+          if (t > seg.t0) {  // O is at rest once the product of the tile before is done
+            ok = mbar_wait(s_empty[2 * rt + (buf ^ 1)], ((c - 1) >> 1) & 1, kErr | 3, abort);
+            if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+            tc_fence_after();
 #pragma unroll 1
             for (int k = 0; k < D / 32; ++k) {
               float o[32];
@@ -390,14 +396,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
             tmem_wait_st();
           }
         }
-        uint8_t* dst = sm + L::oW + rt * L::kWBytes + row * 128;
+        uint32_t w[16];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const float2 a2 = make_float2(a[q], a[q]), b2 = make_float2(lv[q] - Mf, lv[q] - Mf);
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const int at = 16 * q + 8 * h + 2 * k;
@@ -405,21 +410,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
               x.x = fast_exp2(x.x);
               x.y = fast_exp2(x.y);
               sum = __fadd2_rn(sum, x);
-              w[k] = pack2<__half>(x.x, x.y);
+              w[8 * (q & 1) + 4 * h + k] = pack2<__half>(x.x, x.y);
             }
-            *reinterpret_cast<uint4*>(dst + (((2 * q + h) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
           }
+          if (q & 1) tmem_st16(ts + buf * kKeys + 8 * (q - 1), w);
           l += e[q] > 90.f ? 0.f : (sum.x + sum.y) * fast_exp2(e[q]);
         }
-        fence_proxy_async_smem();
+        tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        mbar_arrive_elect(w_full[rt]);
+        mbar_arrive_elect(w_full[2 * rt + buf]);
         ++c;
       }
       // epilogue: the row's O
       if (used && nt > 0 && alive) {
-        const bool ok = mbar_wait(o_done[rt], (c - 1) & 1, kErr | 4, abort);
+        const bool ok = mbar_wait(s_empty[2 * rt + ((c - 1) & 1)], ((c - 1) >> 1) & 1, kErr | 4, abort);
         if (!__all_sync(0xffffffffu, ok)) alive = false;
         tc_fence_after();
       }
@@ -598,7 +603,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
       }
     } else {  // O += W V
       constexpr uint32_t idesc = instr_desc(1, 0, 0, 1, kRowTile, D);
-      const uint64_t a = smem_desc_sw128(smem_u32(sm + L::oW + rt * L::kWBytes), 16, 1024);
       const uint32_t d = tmem + 4 * kKeys + rt * D;
       while (ok && seg.next()) {
         const int nt = seg.t1 - seg.t0;
@@ -607,16 +611,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
           continue;
         }
         for (int j = 0; j < nt && ok; ++j, ++n) {
-          const uint32_t st = n % kRing;
+          const uint32_t st = n % kRing, buf = c & 1;
           // W first: with it the tile's stage is full and stays so until the arrival below
-          ok = mbar_wait(w_full[rt], c & 1, kErr | 9, abort) &&
+          ok = mbar_wait(w_full[2 * rt + buf], (c >> 1) & 1, kErr | 9, abort) &&
                mbar_wait(kv_full[st], (n / kRing) & 1, kErr | 7, abort);
           if (!ok) break;
           tc_fence_after();
           const uint64_t v = smem_desc_sw128(smem_u32(sm + L::oKV + st * 2 * L::kTileBytes + L::kTileBytes), kKeys * 128, 1024);
 #pragma unroll
-          for (int i = 0; i < kKeys / 16; ++i) mma_f16(d, a + ((i * 32) >> 4), v + ((i * 2048) >> 4), idesc, j > 0 || i > 0);
-          mma_commit(o_done[rt]);
+          for (int i = 0; i < kKeys / 16; ++i) mma_f16_ts(d, tmem + (2 * rt + buf) * kKeys + 8 * i, v + ((i * 2048) >> 4), idesc, j > 0 || i > 0);
+          mma_commit(s_empty[2 * rt + buf]);
           mma_commit(kv_empty[st]);
           ++c;
         }
