@@ -32,8 +32,8 @@
 // the tile before (512 new tokens over 32768: 376 us instead of 320).
 //
 // 512 new tokens over 32768 (32 heads, 8 KV heads, D = 128, int8): 320 us, 854
-// TFLOP/s, 0.51 of the measured bf16 rate; 1024 over 8192, 2 sequences, e4m3: 360 us,
-// 714 TFLOP/s; a prompt of 4096: 270 us, 507 TFLOP/s. What bounds it: one thread per
+// TFLOP/s, 0.51 of the measured bf16 rate; 1024 over 8192, 2 sequences, e4m3: 355 us,
+// 726 TFLOP/s; a prompt of 4096: 222 us, 620 TFLOP/s. What bounds it: one thread per
 // row takes a tile's 64 scores through a chain of load, maximum, exponentials and
 // store that two warps per scheduler do not hide; then a line's set-up (queries,
 // the first tile, the epilogue).
@@ -61,13 +61,17 @@ constexpr int kRowTile = 128, kRowsCta = 256, kKeys = 64, kRing = 4;
 constexpr int kSoftWarps = 8, kWideWarps = 8, kMmaWarps = 4,
               kThreads = 32 * (kSoftWarps + kWideWarps + kMmaWarps);
 // registers per thread at launch, and of each role after setmaxnreg
-constexpr int kRegs = 96, kSoftRegs = 144, kWideRegs = 64, kMmaRegs = 64;
+constexpr int kRegs = 96, kSoftRegs = 152, kWideRegs = 64, kMmaRegs = 48;
 static_assert(kSoftWarps * kSoftRegs + kWideWarps * kWideRegs + kMmaWarps * kMmaRegs ==
                   (kSoftWarps + kWideWarps + kMmaWarps) * kRegs,
               "the roles share what the block was launched with");
 constexpr float kSlack = 8.f;
 constexpr float kNoScale = -200.f;  // log2 of a scale of 0
-constexpr uint32_t kLineCost = 256;  // what a line's set-up takes, in keys (7 us, a 64-key tile 1.65 us)
+// What a line's set-up takes, in keys: the queries, the first tile's way through
+// the pipeline and the epilogue, about 10 us at 1.2 us per 64-key tile. Measured on
+// a prompt of 4096 tokens and a piece of 862 over 7000: 256 keys 268 and 150 us,
+// 512 222 and 152 us, 896 229 and 160 us.
+constexpr uint32_t kLineCost = 512;
 constexpr unsigned kErr = 0x400;
 constexpr int kMaxBatch = 1024;
 
