@@ -11,7 +11,11 @@ PyTorch-facing API:
 * ``spatten_b200.bert``        -- ``SpattenBertSelfAttention``,
   ``spatten_encoder_forward``, ``slice_linear_weights``, ``patch_bert``.
 * ``spatten_b200.qwen3``       -- ``SpattenQwen3Attention``, ``patch_qwen3``:
-  Qwen3 prefill with cascade token pruning of the KV cache.
+  Qwen3 prefill with cascade token pruning of the KV cache, and generation over
+  a paged one (``PagedQwen3Cache``).
+* ``spatten_b200.decode``      -- a decode step over a progressive-quantised cache.
+* ``spatten_b200.paged``       -- a paged KV cache in 8 bits: ``paged_append``,
+  ``paged_attention``, ``paged_read``.
 * ``spatten_b200.distributed`` -- batch / head sharding over ranks and the
   importance all-reduce.
 * ``spatten_b200.torch_ops``   -- the same operators under ``torch.ops.spatten``.

@@ -116,3 +116,26 @@ def test_torch_ops_match_python():
                        paged.paged_attention(q, c[1], t, cu, ln, 20, sm_scale=0.1))
     for a, b in zip(torch.ops.spatten.paged_read(*c[0], t, ln, idx), paged.paged_read(c[1], t, ln, idx=idx)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("knobs", [{}, {"enable_token_prune": True, "token_keep_ratio": 0.7}])
+def test_generate(qwen3_model, knobs):
+    """HF's generate over the paged cache: the tokens that a loop of forwards
+    over another paged cache picks."""
+    from transformers import Qwen3ForCausalLM
+    from spatten_b200.qwen3 import PagedQwen3Cache, patch_qwen3
+    torch.manual_seed(0)
+    lm = patch_qwen3(Qwen3ForCausalLM(qwen3_model.config).to("cuda", torch.bfloat16).eval(), **knobs)
+    cfg = lm.config
+    ids = torch.randint(0, cfg.vocab_size, (2, 33), device="cuda")
+    cache = PagedQwen3Cache(cfg, 2, 64, page_size=16)
+    out = lm.generate(ids, attention_mask=torch.ones_like(ids), past_key_values=cache, max_new_tokens=9, do_sample=False,
+                      eos_token_id=None, pad_token_id=0)
+    assert out.shape == (2, 42) and torch.equal(out[:, :33], ids) and cache.get_seq_length() == 41
+    want, new, cache = ids, ids, PagedQwen3Cache(cfg, 2, 64, page_size=16)
+    with torch.no_grad():
+        for _ in range(9):
+            logits = lm(input_ids=new, past_key_values=cache, use_cache=True, logits_to_keep=1).logits
+            new = logits[:, -1:].argmax(-1)
+            want = torch.cat([want, new], 1)
+    assert torch.equal(out, want)
