@@ -14,8 +14,10 @@
 // scale grew. A thread holds 4 dims of a row's first half and the 4 that rotate
 // with them, so a rotation needs no exchange. The query rows' norm and rotation
 // ride in further CTAs of the same launch. A decode step is bound by the chain
-// of dependent loads (lengths, page table, scale), a prompt by HBM and the
-// instructions per element.
+// of dependent loads (lengths, page table, scale): 2.6 us for one token, 5.2 us for
+// 64 sequences. A prompt is bound by HBM and the issue slots (63 % of them used):
+// 4 prompts of 8192 tokens (32 query, 8 KV heads, D = 128, bf16 to int8), 166 us =
+// 4.46 TB/s, 0.68 of the measured copy rate.
 #include "kernels.h"
 #include "paged_dev.cuh"
 
@@ -377,7 +379,8 @@ cudaError_t append_dim(const PagedAppendParams& p, cudaStream_t st) {
 // of one (token, head) of K and of V at a time, heads fastest, so that a warp
 // reads whole rows and writes consecutive 16-byte pieces, and has four of them in
 // flight (index, page and codes each wait for the one before). Bound by HBM
-// (1 byte in, 2 out).
+// (1 byte in, 2 out): 2048 of 8192 tokens of 64 sequences, 154 us = 5.23 TB/s, 0.80 of
+// the measured copy rate.
 constexpr int kReadThreads = 256, kReadFly = 4;
 
 template <typename T, int KV>

@@ -13,9 +13,9 @@
 // (movmatrix).
 //
 // Bound by HBM where there are keys enough: 64 sequences x 8 heads x 32768 keys
-// of int8, 671 us = 6.40 TB/s, 0.98 of the measured copy rate; one sequence of
-// 131001, 53 us = 5.07 TB/s; 48 ragged ones of up to 8192, 80 us = 5.2 TB/s. One of 777
-// takes 8.4 us, which is the chain of dependent loads and the second launch.
+// of int8, 667 us = 6.44 TB/s, 0.99 of the measured copy rate; one sequence of
+// 131001, 53 us = 5.0 TB/s; 48 ragged ones of up to 8192, 79 us = 5.2 TB/s. One of
+// 777 takes 8.7 us, which is the chain of dependent loads and the second launch.
 //
 // Numerics:
 //  * q' is the query row in what K's product takes: two int8 terms beside int8

@@ -30,12 +30,13 @@ SPATTEN_DEV float paged_normaliser(float m, float l, float M) {
 // slot 2 c + 1 of that CTA and slot 2 c of the following ones. A warp per row
 // and, where the line has fewer rows than the CTA has warps, per share of the
 // parts; D / 32 dims per lane. Bound by the latency of its loads: the (m, l, M)
-// of 64 parts (two per lane) and 8 outputs of the warp's share go out at once.
+// of 64 parts (two per lane) and 8 outputs of the warp's share go out at once. It
+// adds 5 us to a launch of its own, less under the programmatic dependence.
 constexpr int kJoinWarps = 16;
 
 template <int D, int ROWS>
-__global__ void __launch_bounds__(32 * kJoinWarps, D == 128 ? 1 : 2) paged_join_kernel(const PagedAttendParams p, const PagedPartials ws,
-                                                                     const bool bf16) {
+__global__ void __launch_bounds__(32 * kJoinWarps, D == 128 ? 1 : 2)
+paged_join_kernel(const PagedAttendParams p, const PagedPartials ws, const bool bf16) {
   constexpr int E = D / 32, FLY = 8, SPAN = 64;
   __shared__ float sh[kJoinWarps][D + 4];
   grid_dependents();

@@ -82,7 +82,8 @@ def test_bad_cache(kind, field, value, code):
     ("v_st", 260, N.ERR_INVALID), ("k_sh", -128, N.ERR_INVALID), ("q_out", 0, N.ERR_INVALID),
     ("q", 0, N.ERR_INVALID), ("H", 0, N.ERR_INVALID), ("q_norm_w", 1 << 20, N.ERR_INVALID),
     ("k_norm_w", 1 << 20, N.ERR_INVALID), ("cos", 0, N.ERR_INVALID), ("cs_dtype", N.DTYPE_F16, N.ERR_UNSUPPORTED),
-    ("qo_st", 0, N.ERR_INVALID), ("qo_sh", 64, N.ERR_INVALID), ("cs_rows", 0, N.ERR_INVALID), ("cs_stride", 60, N.ERR_INVALID), ("positions", (1 << 20) + 1, N.ERR_INVALID),
+    ("qo_st", 0, N.ERR_INVALID), ("qo_sh", 64, N.ERR_INVALID),
+    ("cs_rows", 0, N.ERR_INVALID), ("cs_stride", 60, N.ERR_INVALID), ("positions", (1 << 20) + 1, N.ERR_INVALID),
 ])
 def test_bad_append(field, value, code):
     assert N.lib.spatten_paged_append(_append(**{field: value}), None) == code
