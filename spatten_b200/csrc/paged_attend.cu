@@ -696,9 +696,10 @@ int paged_attend_max_batch() { return kMaxBatch; }
 namespace {
 
 // Which kernels a call takes. Sequences of more than kTcRows query rows per KV
-// head (pieces of prompts) go to the tcgen05 kernel, the others to the one above:
-// at 4 sequences x 8 heads over 4096 keys, 64 rows take 43.5 us there and 41.8 us
-// here, 96 rows 44 us and 55 us. The host knows the largest sequence only; where
+// head (pieces of prompts) go to the tcgen05 kernel, the others to the one above.
+// 64 rows take 40 us there and 42 us here at 4 sequences x 8 heads over 4096 keys,
+// but 24 and 15 us at one over 800; 96 rows 40 and 55 us at the former. The
+// host knows the largest sequence only; where
 // the rows show that some must be shorter, both are launched and each serves its
 // own, so that single tokens beside a prompt's piece keep the kernel made for
 // them (the other launch costs about 4 us).
