@@ -104,7 +104,11 @@ class PagedQwen3Cache(Cache):
     """Paged 8-bit KV cache of every layer, for ``past_key_values`` of a model
     that ``patch_qwen3`` made. ``max_tokens`` slots per sequence are reserved in
     each layer's pool, sequence b's pages in a row; the layers share one page
-    table. Layers may hold different numbers of tokens (token pruning)."""
+    table. Layers may hold different numbers of tokens (token pruning).
+
+    HF's generation modes that change a cache are served: drafted tokens
+    (``crop``), beams (``reorder_cache``), and changes of the batch
+    (``batch_repeat_interleave``, ``batch_select_indices``)."""
 
     def __init__(self, config, batch, max_tokens, page_size=64, kv_dtype=torch.int8, device="cuda"):
         super().__init__(layers=[])
@@ -112,10 +116,23 @@ class PagedQwen3Cache(Cache):
         self.batch, self.max_tokens = batch, int(max_tokens)
         mp = -(-self.max_tokens // page_size)
         self.pools = [paged.new_paged_cache(batch * mp, G, D, page_size, kv_dtype, device) for _ in range(L)]
-        self.page_table = torch.arange(batch * mp, dtype=torch.int32, device=device).view(batch, mp)
+        self.page_table = self._pages(batch, mp, device)
         self.seq_lens = torch.zeros((L, batch), dtype=torch.int32, device=device)
         self.held = [0] * L  # slots of each layer, as the host counts them
         self.seen = [0] * L  # positions each layer has been given (kept or not)
+        self.pruned = [0] * L  # positions of a prompt of which each layer kept only some (0: all kept)
+
+    @staticmethod
+    def _pages(batch, per_sequence, device):
+        return torch.arange(batch * per_sequence, dtype=torch.int32, device=device).view(batch, per_sequence)
+
+    @property
+    def max_batch_size(self):
+        return self.batch
+
+    @property
+    def max_cache_len(self):
+        return self.max_tokens
 
     def get_seq_length(self, layer_idx=0):
         return self.seen[layer_idx]
@@ -129,7 +146,78 @@ class PagedQwen3Cache(Cache):
     def reset(self):
         """Forget every token; the pools stay."""
         self.seq_lens.zero_()
-        self.held, self.seen = [0] * len(self.held), [0] * len(self.seen)
+        L = len(self.pools)
+        self.held, self.seen, self.pruned = [0] * L, [0] * L, [0] * L
+
+    def crop(self, max_length):
+        """Forget the positions from ``max_length`` on (negative: that many of
+        the last ones), in every layer; their slots are written again by the next
+        tokens. A pruned prompt can only be forgotten as a whole: which of its
+        positions a layer kept is not known here."""
+        keep = max_length if max_length >= 0 else max(self.seen[0] + max_length, 0)
+        drop = [max(n - keep, 0) for n in self.seen]
+        if not any(drop):
+            return
+        if keep == 0:
+            return self.reset()
+        for n, d, fixed in zip(self.seen, drop, self.pruned):
+            if d and n - d < fixed:
+                raise NotImplementedError(f"PagedQwen3Cache: crop to {keep} inside a pruned prompt of {fixed} tokens")
+        if len(set(drop)) == 1:
+            self.seq_lens.sub_(drop[0])
+        else:  # layers that were given different numbers of tokens
+            for lens, d in zip(self.seq_lens, drop):
+                lens.sub_(d)
+        self.held = [n - d for n, d in zip(self.held, drop)]
+        self.seen = [n - d for n, d in zip(self.seen, drop)]
+
+    def _rows_of(self, idx):
+        rows = torch.arange(self.batch)[idx.cpu()].tolist() if idx.dtype == torch.bool else idx.tolist()
+        if not rows or not all(0 <= r < self.batch for r in rows):
+            raise ValueError(f"PagedQwen3Cache: sequences {rows} of {self.batch}")
+        return rows
+
+    def _by_sequence(self, t, pages=None):
+        """A pool's tensor as [batch, pages, ..] of each sequence's first pages
+        (codes as int8: copies need no more)."""
+        t = t.view(torch.int8) if t.dtype.itemsize == 1 else t
+        return t.view(self.batch, -1, *t.shape[1:])[:, :pages]
+
+    def reorder_cache(self, beam_idx):
+        """Sequence b becomes a copy of sequence beam_idx[b], on pages of its own
+        (the next tokens of two beams differ)."""
+        rows = self._rows_of(beam_idx)
+        if len(rows) != self.batch:
+            raise ValueError(f"PagedQwen3Cache: {len(rows)} beams for {self.batch} sequences")
+        moved = [b for b, r in enumerate(rows) if r != b]
+        if not moved:
+            return
+        dev = self.seq_lens.device
+        dst, src = torch.tensor([moved, [rows[b] for b in moved]], device=dev)
+        for pool, held in zip(self.pools, self.held):
+            for t in pool:
+                t = self._by_sequence(t, -(-held // pool.k.shape[2]))
+                t.index_copy_(0, dst, t.index_select(0, src))
+        self.seq_lens.index_copy_(1, dst, self.seq_lens.index_select(1, src))
+
+    def _select(self, rows):
+        """Sequence b of a new batch is a copy of sequence rows[b]."""
+        idx = torch.tensor(rows, device=self.seq_lens.device)
+        self.pools = [paged.PagedKVCache(*(self._by_sequence(t).index_select(0, idx).flatten(0, 1).view(t.dtype)
+                                           for t in pool)) for pool in self.pools]
+        self.seq_lens = self.seq_lens.index_select(1, idx)
+        self.batch = len(rows)
+        self.page_table = self._pages(self.batch, self.page_table.shape[1], idx.device)
+
+    def batch_repeat_interleave(self, repeats):
+        """``repeats`` copies of each sequence, beside one another."""
+        if repeats < 1:
+            raise ValueError(f"PagedQwen3Cache: {repeats} copies")
+        self._select([b for b in range(self.batch) for _ in range(repeats)])
+
+    def batch_select_indices(self, indices):
+        """The sequences ``indices`` (numbers or a mask) alone."""
+        self._select(self._rows_of(indices))
 
     def packed(self, S):
         """cu_tokens of a batch that brings S tokens per sequence."""
@@ -151,6 +239,8 @@ class PagedQwen3Cache(Cache):
         if B != self.batch:
             raise ValueError(f"PagedQwen3Cache: batch {B}, made for {self.batch}")
         lens = self.grow(layer_idx, K, seen)
+        if K < seen:
+            self.pruned[layer_idx] = self.seen[layer_idx]
         paged.paged_append(self.pools[layer_idx], k.reshape(B * K, G, D), v.reshape(B * K, G, D), self.page_table,
                            self.packed(K), lens, K)
 
