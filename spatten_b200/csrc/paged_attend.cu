@@ -18,9 +18,9 @@
 // 777 takes 8.7 us, which is the chain of dependent loads and the second launch.
 //
 // Numerics:
-//  * q' is the query row in what K's product takes: two int8 terms beside int8
-//    codes, a scaled f16 beside e4m3 (Operands).
-//  * s = (q' . codes) (sm_scale log2(e) k_scale / the row's factor) in fp32, p =
+//  * q' is the query row times a power of two, in what K's product takes: f16, or
+//    an integer of three int8 terms beside int8 codes (Operands).
+//  * s = (q' . codes) (sm_scale log2(e) k_scale / that power) in fp32, p =
 //    2^(s - m) with a reference m that follows the row's maximum (updated when it is
 //    exceeded by more than kSlack); l sums p in fp32.
 //  * P is rounded to f16 for the second product (2^-11 of each weight), after
@@ -39,6 +39,7 @@
 // which a second kernel joins in a fixed order.
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "kernels.h"
 #include "paged_dev.cuh"
@@ -61,111 +62,112 @@ constexpr int kMaxBatch = 8192;
 
 using Workspace = PagedPartials;
 
+// What the products take. Every code of either type is an f16 (an int8's byte x ^
+// 0x80 in the low byte of 0x6400 is the f16 1152 + x, and the difference is exact),
+// and f16 queries keep what they have (query_scale).
+//
+// Beside int8 codes, one block of eight query rows has another form, in which the
+// codes go into integer products as they are: three int8 terms a query, q' =
+// 65536 q1 + 256 q2 + q3 rounded to an integer of at most 2^22, with exact sums.
+// Without the widening of K, 64 sequences x 8 heads x 32768 keys take 670 us, bound
+// by HBM alone; with it 699, and 815 instead of 735 on a GPU that its power limit
+// slows down. The rounding is 2^-22 of the row's largest element, and within
+// what a sum of D fp32 products is off by where that element is at most kOutlier
+// times the row's mean magnitude; a tile with a row beyond takes the f16 form. (With
+// two row blocks the widening is shared by 16 rows, and f16 is faster than two terms
+// were: drafts of 24 sequences 22.0 -> 20.6 us.)
+constexpr float kOutlier = 16.f;
+
 template <int KV, int D, int NB>
-struct Operands;
-
-// int8. K goes into the integer products as it is: a query row becomes two
-// int8 terms, q ~ (256 q1 + q2) max|q| / 32512 (within 2^-16 of its largest
-// element), and 256 (q1 . k) + (q2 . k) is exact in 32 bits. For V, x ^ 0x80 in
-// the low byte of 0x6400 is the f16 1152 + x, and the difference is exact.
-template <int D, int NB>
-struct Operands<kKvInt8, D, NB> {
+struct Operands {
   static constexpr int KW = D / 16;  // K words of a lane and key
-  uint32_t q[NB][KW][2];             // [.][word][term]
+  static constexpr bool kTerms = KV == kKvInt8 && NB == 1;
+  uint32_t q[NB][KW][kTerms ? 3 : 2];
 
-  // f: the lane's dims of its query row, as the words hold them; returns what
-  // a score has to be multiplied by
-  SPATTEN_DEV float set(int nb, const float (&f)[KW][4], float top) {
-    const float up = top > 0.f ? 32512.f / top : 0.f;
+  // f: the lane's dims of its query row, as the words hold them, times `up`
+  SPATTEN_DEV void set(int nb, const float (&f)[KW][4], float up) {
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)  // in pairs as widen() brings them
+        q[nb][w][h] = KV == kKvInt8 ? pack2<__half>(f[w][h] * up, f[w][2 + h] * up)
+                                    : pack2<__half>(f[w][2 * h] * up, f[w][2 * h + 1] * up);
+  }
+  // the integer form: digits of f times kTermsUp `up`
+  static constexpr float kTermsUp = 128.f;
+  SPATTEN_DEV void set_terms(const float (&f)[KW][4], float up) {
 #pragma unroll
     for (int w = 0; w < KW; ++w) {
-      uint32_t a = 0, b = 0;
+      uint32_t d[3] = {0u, 0u, 0u};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int x = __float2int_rn(fminf(fmaxf(f[w][i] * up, -32512.f), 32512.f));
-        const int hi = (x + 128) >> 8, lo = x - 256 * hi;
-        a |= ((uint32_t)hi & 0xFFu) << (8 * i);
-        b |= ((uint32_t)lo & 0xFFu) << (8 * i);
+        int x = __float2int_rn(f[w][i] * up * kTermsUp);
+#pragma unroll
+        for (int t = 2; t >= 0; --t) {
+          const int low = (int)(int8_t)x;
+          d[t] |= ((uint32_t)low & 0xFFu) << (8 * i);
+          x = (x - low) >> 8;
+        }
       }
-      q[nb][w][0] = a;
-      q[nb][w][1] = b;
+#pragma unroll
+      for (int t = 0; t < 3; ++t) q[0][w][t] = d[t];
     }
-    return top * (1.f / 32512.f);
-  }
-  SPATTEN_DEV void scores(const uint32_t (&k0)[KW], const uint32_t (&k1)[KW], float (&s)[NB][4]) const {
-    int hi[NB][4], lo[NB][4];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) hi[nb][i] = lo[nb][i] = 0;
-#pragma unroll
-    for (int w = 0; w < KW; w += 2) {
-      const uint32_t a[4] = {k0[w], k1[w], k0[w + 1], k1[w + 1]};
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        mma_s8_16832(hi[nb], a, q[nb][w][0], q[nb][w + 1][0]);
-        mma_s8_16832(lo[nb], a, q[nb][w][1], q[nb][w + 1][1]);
-      }
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[nb][i] = (float)(256 * hi[nb][i] + lo[nb][i]);
   }
   static SPATTEN_DEV uint32_t biased(uint32_t w) {
     const uint32_t u = (w & 0x00FF00FFu) ^ 0x64806480u;
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
     return *reinterpret_cast<const uint32_t*>(&h);
   }
+  // a word's codes: int8's bytes (0, 2) and (1, 3), e4m3's (0, 1) and (2, 3)
+  static SPATTEN_DEV void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (KV == kKvInt8) {
+      lo = biased(w);
+      hi = biased(w >> 8);
+    } else {
+      asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }"
+          : "=r"(lo), "=r"(hi) : "r"(w));
+    }
+  }
+  template <bool TERMS>
+  SPATTEN_DEV void scores(const uint32_t (&k0)[KW], const uint32_t (&k1)[KW], float (&s)[NB][4]) const {
+    if constexpr (TERMS) {
+      int d[3][4];
+#pragma unroll
+      for (int t = 0; t < 3; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[t][i] = 0;
+#pragma unroll
+      for (int w = 0; w < KW; w += 2) {
+        const uint32_t a[4] = {k0[w], k1[w], k0[w + 1], k1[w + 1]};
+#pragma unroll
+        for (int t = 0; t < 3; ++t) mma_s8_16832(d[t], a, q[0][w][t], q[0][w + 1][t]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[0][i] = fmaf((float)(256 * d[0][i] + d[1][i]), 256.f, (float)d[2][i]);
+    } else {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[nb][i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        uint32_t a[4];
+        widen(k0[w], a[0], a[2]);
+        widen(k1[w], a[1], a[3]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma_16816<__half>(s[nb], a, q[nb][w][0], q[nb][w][1]);
+      }
+    }
+  }
   // words of two keys: the key pairs of dims 0 .. 3
   static SPATTEN_DEV void values(uint32_t x, uint32_t y, uint32_t (&d)[4]) {
-    const uint32_t t = __byte_perm(x, y, 0x5410), u = __byte_perm(x, y, 0x7632);
-    d[0] = biased(t);
-    d[1] = biased(t >> 8);
-    d[2] = biased(u);
-    d[3] = biased(u >> 8);
-  }
-};
-
-// e4m3: every code is an f16. A query row is scaled by a power of two that
-// takes its largest element to [2^14, 2^15): f16 then holds bf16's range to
-// 2^-39 of that element.
-template <int D, int NB>
-struct Operands<kKvE4m3, D, NB> {
-  static constexpr int KW = D / 16;
-  uint32_t q[NB][KW][2];
-
-  SPATTEN_DEV float set(int nb, const float (&f)[KW][4], float top) {
-    const int e = top > 0.f ? 14 - max((int)(__float_as_uint(top) >> 23) - 127, -112) : 0;  // at most 126
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-    for (int w = 0; w < KW; ++w) {
-      q[nb][w][0] = pack2<__half>(f[w][0] * up, f[w][1] * up);
-      q[nb][w][1] = pack2<__half>(f[w][2] * up, f[w][3] * up);
+    if constexpr (KV == kKvInt8) {
+      widen(__byte_perm(x, y, 0x5410), d[0], d[1]);
+      widen(__byte_perm(x, y, 0x7632), d[2], d[3]);
+    } else {
+      widen(__byte_perm(x, y, 0x5140), d[0], d[1]);
+      widen(__byte_perm(x, y, 0x7362), d[2], d[3]);
     }
-    return __uint_as_float((uint32_t)(127 - e) << 23);
-  }
-  static SPATTEN_DEV void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }"
-        : "=r"(lo), "=r"(hi) : "r"(w));
-  }
-  SPATTEN_DEV void scores(const uint32_t (&k0)[KW], const uint32_t (&k1)[KW], float (&s)[NB][4]) const {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[nb][i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < KW; ++w) {
-      uint32_t a[4];
-      widen(k0[w], a[0], a[2]);
-      widen(k1[w], a[1], a[3]);
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) mma_16816<__half>(s[nb], a, q[nb][w][0], q[nb][w][1]);
-    }
-  }
-  static SPATTEN_DEV void values(uint32_t x, uint32_t y, uint32_t (&d)[4]) {
-    widen(__byte_perm(x, y, 0x5140), d[0], d[1]);
-    widen(__byte_perm(x, y, 0x7362), d[2], d[3]);
   }
 };
 
@@ -418,6 +420,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     float cq[NB][2], m[NB][2], M[NB][2], l[NB][2];
     int lim[NB][2];
     float o[NB][KS][4];
+    bool terms = false;  // the integer form of the scores
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       float f[KS][4], top = 0.f;
@@ -438,11 +441,26 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // a row that is not finite has no scores: NaN
-      const float c = ops.set(nb, f, top) * (top <= 3.4e38f ? p.scale_log2 : NAN);
+      QueryScale qs = query_scale(top, p.scale_log2);
+      if constexpr (Ops::kTerms) {
+        float sum = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum += fabsf(f[s][j]);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        terms = __all_sync(0xffffffffu, !(top * D > kOutlier * sum));  // (rows that are not finite: either)
+      }
+      if (terms) {
+        if constexpr (Ops::kTerms) ops.set_terms(f, qs.up);
+        qs.factor *= 1.f / Ops::kTermsUp;
+      } else {
+        ops.set(nb, f, qs.up);
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {  // this lane's rows of the products: 2 tig, 2 tig + 1
-        cq[nb][j] = __shfl_sync(0xffffffffu, c, (2 * tig + j) * 4);
+        cq[nb][j] = __shfl_sync(0xffffffffu, qs.factor, (2 * tig + j) * 4);
         lim[nb][j] = min(sq.old + (r0 + nb * 8 + 2 * tig + j) / R + 1, sq.len);
         m[nb][j] = M[nb][j] = -INFINITY;
         l[nb][j] = 0.f;
@@ -453,124 +471,132 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         for (int j = 0; j < 4; ++j) o[nb][s][j] = 0.f;
     }
 
-    for (int j = 0; j < nt; ++j) {
-      cp_async_wait<ST - 2>();
-      __syncwarp();  // tile j has landed for every lane, and tile j - 1 is read
-      issue(j + ST - 1);
-      const uint8_t* stage = ring + (j % ST) * SH::kStageBytes;
-      const int slot0 = tile_slot(j), at = j % AHEAD;
-      if (at == 0) {
-        have_l = have_n;
-        ks_l = ks_n;
-        vs_l = vs_n > 0.f ? fmaxf(log2f(vs_n), kNoScale) : kNoScale;  // log2 of the scale
-      }
-      float ks[BL], lv[BL];
-      bool none = false;
-#pragma unroll
-      for (int kb = 0; kb < BL; ++kb) {
-        ks[kb] = __shfl_sync(0xffffffffu, ks_l, BL * at + kb);
-        lv[kb] = __shfl_sync(0xffffffffu, vs_l, BL * at + kb);
-        none |= !((have_l >> (BL * at + kb)) & 1u);
-      }
-      float s[BL][NB][4];
-#pragma unroll
-      for (int kb = 0; kb < BL; ++kb) {
-        uint32_t k0[KS], k1[KS];
-        read_k<D>(k0, stage + kb * SH::kBlockBytes, gid, tig);
-        read_k<D>(k1, stage + kb * SH::kBlockBytes, gid + 8, tig);
-        ops.scores(k0, k1, s[kb]);
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          const float f0 = cq[nb][0] * ks[kb], f1 = cq[nb][1] * ks[kb];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[kb][nb][i] *= i & 1 ? f1 : f0;
+    auto tiles = [&](auto form) {
+      constexpr bool TERMS = decltype(form)::value;
+      for (int j = 0; j < nt; ++j) {
+        cp_async_wait<ST - 2>();
+        __syncwarp();  // tile j has landed for every lane, and tile j - 1 is read
+        issue(j + ST - 1);
+        const uint8_t* stage = ring + (j % ST) * SH::kStageBytes;
+        const int slot0 = tile_slot(j), at = j % AHEAD;
+        if (at == 0) {
+          have_l = have_n;
+          ks_l = ks_n;
+          vs_l = vs_n > 0.f ? fmaxf(log2f(vs_n), kNoScale) : kNoScale;  // log2 of the scale
         }
-      }
-      if (slot0 + KEYS > lim_min || none) {  // warp-uniform
+        float ks[BL], lv[BL];
+        bool none = false;
 #pragma unroll
-        for (int kb = 0; kb < BL; ++kb)
+        for (int kb = 0; kb < BL; ++kb) {
+          ks[kb] = __shfl_sync(0xffffffffu, ks_l, BL * at + kb);
+          lv[kb] = __shfl_sync(0xffffffffu, vs_l, BL * at + kb);
+          none |= !((have_l >> (BL * at + kb)) & 1u);
+        }
+        float s[BL][NB][4];
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
+        for (int kb = 0; kb < BL; ++kb) {
+          uint32_t k0[KS], k1[KS];
+          read_k<D>(k0, stage + kb * SH::kBlockBytes, gid, tig);
+          read_k<D>(k1, stage + kb * SH::kBlockBytes, gid + 8, tig);
+          ops.template scores<TERMS>(k0, k1, s[kb]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!((have_l >> (BL * at + kb)) & 1u) || slot0 + 16 * kb + gid + 4 * (i & 2) >= lim[nb][i & 1])
-                s[kb][nb][i] = -INFINITY;
-      }
-      // p = 2^(s - m), and w = 2^(s + log2 v_scale - M)
-      float top[NB][2], topw[NB][2];  // largest s, and s + log2 v_scale, of this lane
-      bool up = false;
+          for (int nb = 0; nb < NB; ++nb) {
+            const float f0 = cq[nb][0] * ks[kb], f1 = cq[nb][1] * ks[kb];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          top[nb][c] = topw[nb][c] = -INFINITY;
-#pragma unroll
-          for (int kb = 0; kb < BL; ++kb) {
-            const float t = fmaxf(s[kb][nb][c], s[kb][nb][2 + c]);
-            top[nb][c] = fmaxf(top[nb][c], t);
-            topw[nb][c] = fmaxf(topw[nb][c], t + lv[kb]);
+            for (int i = 0; i < 4; ++i) s[kb][nb][i] *= i & 1 ? f1 : f0;
           }
-          up |= top[nb][c] > m[nb][c] + kSlack || topw[nb][c] > M[nb][c] + kSlack;
         }
-      if (__any_sync(0xffffffffu, up)) {
+        if (slot0 + KEYS > lim_min || none) {  // warp-uniform
+#pragma unroll
+          for (int kb = 0; kb < BL; ++kb)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (!((have_l >> (BL * at + kb)) & 1u) || slot0 + 16 * kb + gid + 4 * (i & 2) >= lim[nb][i & 1])
+                  s[kb][nb][i] = -INFINITY;
+        }
+        // p = 2^(s - m), and w = 2^(s + log2 v_scale - M)
+        float top[NB][2], topw[NB][2];  // largest s, and s + log2 v_scale, of this lane
+        bool up = false;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = top[nb][c], y = topw[nb][c];
+            top[nb][c] = topw[nb][c] = -INFINITY;
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) {
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-              y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+            for (int kb = 0; kb < BL; ++kb) {
+              const float t = fmaxf(s[kb][nb][c], s[kb][nb][2 + c]);
+              top[nb][c] = fmaxf(top[nb][c], t);
+              topw[nb][c] = fmaxf(topw[nb][c], t + lv[kb]);
             }
-            const float mn = fmaxf(m[nb][c], x), Mn = fmaxf(M[nb][c], y);
-            l[nb][c] *= fast_exp2(m[nb][c] - finite_or_0(mn));
-            const float f = fast_exp2(M[nb][c] - finite_or_0(Mn));
+            up |= top[nb][c] > m[nb][c] + kSlack || topw[nb][c] > M[nb][c] + kSlack;
+          }
+        if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-              o[nb][k][c] *= f;
-              o[nb][k][2 + c] *= f;
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float x = top[nb][c], y = topw[nb][c];
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) {
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+              }
+              const float mn = fmaxf(m[nb][c], x), Mn = fmaxf(M[nb][c], y);
+              l[nb][c] *= fast_exp2(m[nb][c] - finite_or_0(mn));
+              const float f = fast_exp2(M[nb][c] - finite_or_0(Mn));
+#pragma unroll
+              for (int k = 0; k < KS; ++k) {
+                o[nb][k][c] *= f;
+                o[nb][k][2 + c] *= f;
+              }
+              m[nb][c] = mn;
+              M[nb][c] = Mn;
             }
-            m[nb][c] = mn;
-            M[nb][c] = Mn;
-          }
-      }
-      uint32_t pf[BL][NB][2];
+        }
+        uint32_t pf[BL][NB][2];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const float m0 = finite_or_0(m[nb][0]), m1 = finite_or_0(m[nb][1]);
-        const float M0 = finite_or_0(M[nb][0]), M1 = finite_or_0(M[nb][1]);
+        for (int nb = 0; nb < NB; ++nb) {
+          const float m0 = finite_or_0(m[nb][0]), m1 = finite_or_0(m[nb][1]);
+          const float M0 = finite_or_0(M[nb][0]), M1 = finite_or_0(M[nb][1]);
 #pragma unroll
-        for (int kb = 0; kb < BL; ++kb)
+          for (int kb = 0; kb < BL; ++kb)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float s0 = s[kb][nb][2 * i], s1 = s[kb][nb][2 * i + 1];
-            l[nb][0] += fast_exp2(s0 - m0);
-            l[nb][1] += fast_exp2(s1 - m1);
-            pf[kb][nb][i] =
-                transpose8x8(pack2<__half>(fast_exp2(s0 + (lv[kb] - M0)), fast_exp2(s1 + (lv[kb] - M1))));
-          }
-      }
-      // values
+            for (int i = 0; i < 2; ++i) {
+              const float s0 = s[kb][nb][2 * i], s1 = s[kb][nb][2 * i + 1];
+              l[nb][0] += fast_exp2(s0 - m0);
+              l[nb][1] += fast_exp2(s1 - m1);
+              pf[kb][nb][i] =
+                  transpose8x8(pack2<__half>(fast_exp2(s0 + (lv[kb] - M0)), fast_exp2(s1 + (lv[kb] - M1))));
+            }
+        }
+        // values
 #pragma unroll
-      for (int kb = 0; kb < BL; ++kb) {
-        const uint8_t* blk = stage + (BL + kb) * SH::kBlockBytes;
-        uint32_t v[4][D / 32];
+        for (int kb = 0; kb < BL; ++kb) {
+          const uint8_t* blk = stage + (BL + kb) * SH::kBlockBytes;
+          uint32_t v[4][D / 32];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) read_v<D>(v[r], blk, 2 * tig + (r & 1) + 4 * (r & 2), gid);
+          for (int r = 0; r < 4; ++r) read_v<D>(v[r], blk, 2 * tig + (r & 1) + 4 * (r & 2), gid);
 #pragma unroll
-        for (int w = 0; w < D / 32; ++w) {
-          uint32_t lo[4], hi[4];
-          Ops::values(v[0][w], v[1][w], lo);
-          Ops::values(v[2][w], v[3][w], hi);
+          for (int w = 0; w < D / 32; ++w) {
+            uint32_t lo[4], hi[4];
+            Ops::values(v[0][w], v[1][w], lo);
+            Ops::values(v[2][w], v[3][w], hi);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) mma_16816<__half>(o[nb][2 * w + h], a, pf[kb][nb][0], pf[kb][nb][1]);
+              for (int nb = 0; nb < NB; ++nb) mma_16816<__half>(o[nb][2 * w + h], a, pf[kb][nb][0], pf[kb][nb][1]);
+            }
           }
         }
       }
+    };
+    if constexpr (Ops::kTerms) {
+      if (terms) tiles(std::true_type{}); else tiles(std::false_type{});
+    } else {
+      tiles(std::false_type{});
     }
     __syncthreads();  // every ring is read
 

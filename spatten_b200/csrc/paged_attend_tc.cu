@@ -6,7 +6,7 @@
 // 128) and walks key tiles of 64:
 //   S [128 x 64] = Q' . K codes^T,  O [128 x D] += W . V codes   (kind::f16)
 // with f16 operands (every int8 and e4m3 code is an f16; q' = q 2^e, see
-// paged_attend.cu) and fp32 accumulators in tensor memory. One thread owns a
+// query_scale) and fp32 accumulators in tensor memory. One thread owns a
 // query row:
 //   t = S (sm_scale log2(e) 2^-e k_scale),  w = 2^(t + log2 v_scale - M),
 // with a reference M that follows max(t + log2 v_scale), so that W keeps 11 bits
@@ -305,16 +305,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
           }
 #pragma unroll
           for (int d = LQ / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-          const int e = top > 0.f ? 14 - max((int)(__float_as_uint(top) >> 23) - 127, -112) : 0;
-          const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-          const float back = p.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23) * (top <= 3.4e38f ? 1.f : NAN);
-          const float mine = __shfl_sync(0xffffffffu, back, (lane % RQ) * LQ);
+          const QueryScale qs = query_scale(top, p.scale_log2);
+          const float mine = __shfl_sync(0xffffffffu, qs.factor, (lane % RQ) * LQ);
           if (lane / RQ == k) cq = mine;  // this thread's row is among the step's
           uint32_t o[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 f = pair(w[j]);
-            o[j] = pack2<__half>(f.x * up, f.y * up);
+            o[j] = pack2<__half>(f.x * qs.up, f.y * qs.up);
           }
           const int y = (warp & 3) * 32 + k * RQ + in;
           *reinterpret_cast<uint4*>(sm + L::oQ + rt * L::kQBytes + (li >> 3) * (kRowTile * 128) + y * 128 +

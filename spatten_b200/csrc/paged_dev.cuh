@@ -95,4 +95,20 @@ SPATTEN_DEV void codes4_to_f32(uint32_t w, float (&f)[4]) {
   }
 }
 
+// A query row as f16 for the product with the codes, times the power of two that
+// takes its largest magnitude `top` to [2^14, 2^15): bf16 and fp16 values keep all
+// their bits down to 2^-28 of that element, and some down to 2^-39 (powers of two
+// that fp32 does not hold are left out: a row below 2^-112 stays smaller). A row
+// that is not finite has no scores: its factor is NaN.
+struct QueryScale {
+  float up;      // the power
+  float factor;  // what its scores are multiplied by, beside the key's scale
+};
+
+SPATTEN_DEV QueryScale query_scale(float top, float scale_log2) {
+  const int e = top > 0.f ? 14 - max((int)(__float_as_uint(top) >> 23) - 127, -112) : 0;  // at most 126
+  const float back = __uint_as_float((uint32_t)(127 - e) << 23);
+  return {__uint_as_float((uint32_t)(127 + e) << 23), scale_log2 * back * (top <= 3.4e38f ? 1.f : NAN)};
+}
+
 }  // namespace spatten
