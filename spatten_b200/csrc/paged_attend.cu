@@ -55,6 +55,7 @@ constexpr int kWarps = 4;
 constexpr uint32_t kLineCost = 16;
 constexpr float kSlack = 8.f;       // p and w stay below 2^8
 constexpr float kNoScale = -200.f;  // log2 of a scale of 0: below that of any float
+constexpr float kNone = -3.402823466e38f;  // reference of a row without a key: finite, so that -inf less it is -inf
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 
 // sequences whose prefix sums fit the shared memory
@@ -206,36 +207,66 @@ SPATTEN_DEV int swizzled(int row, int chunk) {
   else return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
 
+// Offsets of a lane's pieces in a block of the ring: its rows' swizzles make two of
+// each kind, the others are constant distances away.
+template <int D>
+struct LaneOffsets {
+  uint32_t load[2], k[2], v[2];
+  SPATTEN_DEV LaneOffsets(int lane) {
+    constexpr int CH = D / 16;
+    const int gid = lane >> 2, tig = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      load[i] = swizzled<D>(i * (32 / CH) + lane / CH, lane % CH) - i * 512;
+      k[i] = swizzled<D>(gid, tig * (D / 64) + (D == 128 ? i : 0));
+      v[i] = D == 128 ? swizzled<D>(2 * tig + i, gid) : swizzled<D>(2 * tig + i, gid >> 1) + (gid & 1) * 8;
+    }
+  }
+};
+
 // A block of 16 rows into the ring; rows at or behind `live` arrive as zeros
 // (their bytes may be anything).
 template <int D>
-SPATTEN_DEV void load_block(uint8_t* dst, const uint8_t* src, int lane, int live) {
+SPATTEN_DEV void load_block(uint32_t dst, const LaneOffsets<D>& lo, const uint8_t* src, int lane, int live) {
   constexpr int CH = D / 16, RPI = 32 / CH;  // chunks per row, rows per warp instruction
 #pragma unroll
   for (int i = 0; i < 16 / RPI; ++i) {
     const int row = i * RPI + lane / CH;
-    cp_async16(dst + swizzled<D>(row, lane % CH), src + i * 512 + lane * 16, row < live);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst + lo.load[i & 1] + i * 512),
+                 "l"(src + i * 512), "r"(row < live ? 16 : 0));
   }
 }
 
-// Words of K row `row` for lane tig: dims (D / 4) tig .. + D / 4 - 1.
+SPATTEN_DEV uint4 lds128(uint32_t a) {
+  uint4 x;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(a));
+  return x;
+}
+SPATTEN_DEV uint2 lds64(uint32_t a) {
+  uint2 x;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(a));
+  return x;
+}
+
+// Words of K row gid + 8 h for lane tig: dims (D / 4) tig .. + D / 4 - 1.
 template <int D>
-SPATTEN_DEV void read_k(uint32_t (&k)[D / 16], const uint8_t* blk, int row, int tig) {
+SPATTEN_DEV void read_k(uint32_t (&k)[D / 16], uint32_t blk, const LaneOffsets<D>& lo, int h) {
 #pragma unroll
   for (int j = 0; j < D / 64; ++j) {
-    const uint4 x = *reinterpret_cast<const uint4*>(blk + swizzled<D>(row, tig * (D / 64) + j));
+    const uint4 x = lds128(blk + lo.k[j] + 8 * h * D);
     k[4 * j] = x.x; k[4 * j + 1] = x.y; k[4 * j + 2] = x.z; k[4 * j + 3] = x.w;
   }
 }
 
-// Words of V row `row` for lane gid: dims (D / 8) gid .. + D / 8 - 1.
+// Words of V row 2 tig + (r & 1) + 8 (r >> 1) for lane gid: dims (D / 8) gid .. + D / 8 - 1.
 template <int D>
-SPATTEN_DEV void read_v(uint32_t (&v)[D / 32], const uint8_t* blk, int row, int gid) {
+SPATTEN_DEV void read_v(uint32_t (&v)[D / 32], uint32_t blk, const LaneOffsets<D>& lo, int r) {
+  const uint32_t at = blk + lo.v[r & 1] + 8 * (r >> 1) * D;
   if constexpr (D == 128) {
-    const uint4 x = *reinterpret_cast<const uint4*>(blk + swizzled<D>(row, gid));
+    const uint4 x = lds128(at);
     v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
   } else {
-    const uint2 x = *reinterpret_cast<const uint2*>(blk + swizzled<D>(row, gid >> 1) + (gid & 1) * 8);
+    const uint2 x = lds64(at);
     v[0] = x.x; v[1] = x.y;
   }
 }
@@ -258,6 +289,9 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   grid_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
   const int G = p.c.G, R = p.b.H / G, page = p.c.page, page_log = __ffs(page) - 1;
+  const LaneOffsets<D> lo(lane);
+  const uint8_t* const k_lane = p.c.k + lane * 16;
+  const uint8_t* const v_lane = p.c.v + lane * 16;
 
   // tiles and lines in all. The host made sure of 32 bits for sequences
   // that share no rows; others may need more, and then nothing is done.
@@ -384,7 +418,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       const int slot = tile_slot(j + lane / BL) + 16 * (lane % BL);
       return pid >= 0 ? ((uint32_t)pid * G + g) * page + (slot & (page - 1)) : kNoRow;
     };
-    uint8_t* ring = dsm + warp * ST * SH::kStageBytes;
+    const uint32_t ring = smem_u32(dsm) + warp * ST * SH::kStageBytes;
     uint32_t row_l = kNoRow, have_l = 0, have_n = 0;  // have: blocks with memory, a bit per lane
     int pid_n = -1;
     float ks_l = 0.f, vs_l = 0.f, ks_n = 0.f, vs_n = 0.f;
@@ -401,14 +435,14 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
           vs_n = pid >= 0 ? *(p.c.v_scale + blk) : 0.f;
           if (nt > j + AHEAD) pid_n = page_of(j + AHEAD);
         }
-        uint8_t* dst = ring + (j % ST) * SH::kStageBytes;
+        const uint32_t dst = ring + (j % ST) * SH::kStageBytes;
 #pragma unroll
         for (int kb = 0; kb < BL; ++kb) {
           const uint32_t row = __shfl_sync(0xffffffffu, row_l, BL * at + kb);
           const uint64_t off = row == kNoRow ? 0 : (uint64_t)row * D;
           const int live = row == kNoRow ? 0 : lim_max - (tile_slot(j) + 16 * kb);
-          load_block<D>(dst + kb * SH::kBlockBytes, p.c.k + off, lane, row == kNoRow ? 0 : 16);
-          load_block<D>(dst + (BL + kb) * SH::kBlockBytes, p.c.v + off, lane, live);
+          load_block<D>(dst + kb * SH::kBlockBytes, lo, k_lane + off, lane, row == kNoRow ? 0 : 16);
+          load_block<D>(dst + (BL + kb) * SH::kBlockBytes, lo, v_lane + off, lane, live);
         }
       }
       cp_async_commit();
@@ -462,7 +496,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
       for (int j = 0; j < 2; ++j) {  // this lane's rows of the products: 2 tig, 2 tig + 1
         cq[nb][j] = __shfl_sync(0xffffffffu, qs.factor, (2 * tig + j) * 4);
         lim[nb][j] = min(sq.old + (r0 + nb * 8 + 2 * tig + j) / R + 1, sq.len);
-        m[nb][j] = M[nb][j] = -INFINITY;
+        m[nb][j] = M[nb][j] = kNone;
         l[nb][j] = 0.f;
       }
 #pragma unroll
@@ -477,7 +511,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         cp_async_wait<ST - 2>();
         __syncwarp();  // tile j has landed for every lane, and tile j - 1 is read
         issue(j + ST - 1);
-        const uint8_t* stage = ring + (j % ST) * SH::kStageBytes;
+        const uint32_t stage = ring + (j % ST) * SH::kStageBytes;
         const int slot0 = tile_slot(j), at = j % AHEAD;
         if (at == 0) {
           have_l = have_n;
@@ -496,8 +530,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
 #pragma unroll
         for (int kb = 0; kb < BL; ++kb) {
           uint32_t k0[KS], k1[KS];
-          read_k<D>(k0, stage + kb * SH::kBlockBytes, gid, tig);
-          read_k<D>(k1, stage + kb * SH::kBlockBytes, gid + 8, tig);
+          read_k<D>(k0, stage + kb * SH::kBlockBytes, lo, 0);
+          read_k<D>(k1, stage + kb * SH::kBlockBytes, lo, 1);
           ops.template scores<TERMS>(k0, k1, s[kb]);
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
@@ -544,8 +578,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
                 y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
               }
               const float mn = fmaxf(m[nb][c], x), Mn = fmaxf(M[nb][c], y);
-              l[nb][c] *= fast_exp2(m[nb][c] - finite_or_0(mn));
-              const float f = fast_exp2(M[nb][c] - finite_or_0(Mn));
+              l[nb][c] *= fast_exp2(m[nb][c] - mn);
+              const float f = fast_exp2(M[nb][c] - Mn);
 #pragma unroll
               for (int k = 0; k < KS; ++k) {
                 o[nb][k][c] *= f;
@@ -558,8 +592,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         uint32_t pf[BL][NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const float m0 = finite_or_0(m[nb][0]), m1 = finite_or_0(m[nb][1]);
-          const float M0 = finite_or_0(M[nb][0]), M1 = finite_or_0(M[nb][1]);
+          const float m0 = m[nb][0], m1 = m[nb][1], M0 = M[nb][0], M1 = M[nb][1];
 #pragma unroll
           for (int kb = 0; kb < BL; ++kb)
 #pragma unroll
@@ -574,10 +607,10 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         // values
 #pragma unroll
         for (int kb = 0; kb < BL; ++kb) {
-          const uint8_t* blk = stage + (BL + kb) * SH::kBlockBytes;
+          const uint32_t blk = stage + (BL + kb) * SH::kBlockBytes;
           uint32_t v[4][D / 32];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) read_v<D>(v[r], blk, 2 * tig + (r & 1) + 4 * (r & 2), gid);
+          for (int r = 0; r < 4; ++r) read_v<D>(v[r], blk, lo, r);
 #pragma unroll
           for (int w = 0; w < D / 32; ++w) {
             uint32_t lo[4], hi[4];
@@ -614,9 +647,9 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         for (int k = 0; k < KS; k += 2)
           dst[k / 2] = make_float4(o[nb][k][c], o[nb][k][2 + c], o[nb][k + 1][c], o[nb][k + 1][2 + c]);
         if (gid == 0) {
-          sm_m[warp][row] = m[nb][c];
+          sm_m[warp][row] = m[nb][c] == kNone ? -INFINITY : m[nb][c];
           sm_l[warp][row] = sum;
-          sm_M[warp][row] = M[nb][c];
+          sm_M[warp][row] = M[nb][c] == kNone ? -INFINITY : M[nb][c];
         }
       }
     __syncthreads();
