@@ -23,10 +23,12 @@
 //  * s = (q' . codes) (sm_scale log2(e) k_scale / that power) in fp32, p =
 //    2^(s - m) with a reference m that follows the row's maximum (updated when it is
 //    exceeded by more than kSlack); l sums p in fp32.
-//  * P is rounded to f16 for the second product (2^-11 of each weight), after
+//  * P is rounded to f16 for the second product (2^-12 of each weight), after
 //    v_scale has gone into it: w = 2^(s + log2 v_scale - M), M a second reference
-//    that follows max(s + log2 v_scale). A block with a tiny scale and all the weight
-//    keeps its 11 bits beside blocks with large scales and no weight.
+//    that follows max(s + log2 v_scale), kRoom below it. A block with a tiny scale and
+//    all the weight keeps its 11 bits beside blocks with large scales and no weight,
+//    and a weight down to 2^-21 of the row's largest beside that one (2^-32: half of
+//    f16's smallest step).
 //
 // Work split, over one wave of resident CTAs and from the lengths on the device,
 // so that a ragged batch and one long sequence fill the GPU alike and a captured
@@ -53,8 +55,6 @@ constexpr int kWarps = 4;
 // join of the warps). Measured: 8 tiles are 7 % slower at 64 sequences of up to
 // 2000 keys, 24 tiles 2 % at 48 of up to 8192.
 constexpr uint32_t kLineCost = 16;
-constexpr float kSlack = 8.f;       // p and w stay below 2^8
-constexpr float kNoScale = -200.f;  // log2 of a scale of 0: below that of any float
 constexpr float kNone = -3.402823466e38f;  // reference of a row without a key: finite, so that -inf less it is -inf
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 
@@ -564,7 +564,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
               top[nb][c] = fmaxf(top[nb][c], t);
               topw[nb][c] = fmaxf(topw[nb][c], t + lv[kb]);
             }
-            up |= top[nb][c] > m[nb][c] + kSlack || topw[nb][c] > M[nb][c] + kSlack;
+            up |= top[nb][c] > m[nb][c] + kSlack || topw[nb][c] > M[nb][c] + (kRoom + kSlack);
           }
         if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -577,7 +577,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
                 y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
               }
-              const float mn = fmaxf(m[nb][c], x), Mn = fmaxf(M[nb][c], y);
+              const float mn = fmaxf(m[nb][c], x), Mn = fmaxf(M[nb][c], y - kRoom);
               l[nb][c] *= fast_exp2(m[nb][c] - mn);
               const float f = fast_exp2(M[nb][c] - Mn);
 #pragma unroll

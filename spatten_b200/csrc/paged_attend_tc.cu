@@ -9,9 +9,9 @@
 // query_scale) and fp32 accumulators in tensor memory. One thread owns a
 // query row:
 //   t = S (sm_scale log2(e) 2^-e k_scale),  w = 2^(t + log2 v_scale - M),
-// with a reference M that follows max(t + log2 v_scale), so that W keeps 11 bits
-// whatever the blocks' scales are; O is rescaled in tensor memory when M moved by
-// more than 2^kSlack. The softmax's sum l needs p = 2^(t - m): within a block w
+// with a reference M that follows max(t + log2 v_scale), kRoom below it, so that W
+// keeps 11 bits whatever the blocks' scales are; O is rescaled in tensor memory when
+// that maximum grew by more than kSlack. The softmax's sum l needs p = 2^(t - m): within a block w
 // and p differ by the factor 2^(M - log2 v_scale - m), so l takes the block's sum
 // of w times it (one exponential per score), except where w could underflow
 // under it, which takes the exponentials of p.
@@ -65,8 +65,6 @@ constexpr int kRegs = 96, kSoftRegs = 152, kWideRegs = 64, kMmaRegs = 48;
 static_assert(kSoftWarps * kSoftRegs + kWideWarps * kWideRegs + kMmaWarps * kMmaRegs ==
                   (kSoftWarps + kWideWarps + kMmaWarps) * kRegs,
               "the roles share what the block was launched with");
-constexpr float kSlack = 8.f;
-constexpr float kNoScale = -200.f;  // log2 of a scale of 0
 // What a line's set-up takes, in keys: the queries, the first tile's way through
 // the pipeline and the epilogue, about 10 us at 1.2 us per 64-key tile. Measured on
 // a prompt of 4096 tokens and a piece of 862 over 7000: 256 keys 268 and 150 us,
@@ -363,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
           top = fmaxf(top, x);
           topw = fmaxf(topw, x + lv[q]);
         }
-        const bool up = top > m + kSlack || topw > M + kSlack;
-        const float Mn = up ? fmaxf(M, topw) : M, mn = up ? fmaxf(m, top) : m;
+        const bool up = top > m + kSlack || topw > M + (kRoom + kSlack);
+        const float Mn = up ? fmaxf(M, topw - kRoom) : M, mn = up ? fmaxf(m, top) : m;
         const float Mf = finite_or_0(Mn), mf = finite_or_0(mn);
         if (up) l *= fast_exp2(m - mf);
         const float fo = up ? fast_exp2(M - Mf) : 1.f;

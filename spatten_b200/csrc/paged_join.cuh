@@ -19,6 +19,13 @@ struct PagedPartials {
   float* o;       // [2 ctas][rows][D], by M
 };
 
+// The references of a row's exponentials follow its maxima where these have grown by
+// more than kSlack: p = 2^(s - m) stays below 2^kSlack, and the f16 weights 2^(s +
+// log2 v_scale - M), whose M is kRoom lower than its maximum, use f16's range up to
+// 2^(kRoom + kSlack) = 2^15.
+constexpr float kSlack = 8.f, kRoom = 7.f;
+constexpr float kNoScale = -200.f;  // log2 of a scale of 0: below that of any float
+
 SPATTEN_DEV float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
 
 // What takes an output by M to the result: 2^(M - m) / l, 0 for a row without a key.

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import paged as O
-from tests.test_gpu_paged import BF16, E4, F16, I8, _check_attend, _filled, _i32, _table
+from tests.test_gpu_paged import BF16, E4, F16, I8, U, _check_attend, _cpu, _filled, _i32, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,44 @@ def test_rows_of_all_kinds_side_by_side(kv, D, R, T):
     part[0] = alone.view(-1, D)[0]
     q.view(-1, D)[0] = 0
     _check_attend(part.view_as(out), q, cache, table, [0, T], [n], D ** -0.5)
+
+
+@pytest.mark.parametrize("kv", [I8, E4])
+@pytest.mark.parametrize("T", [1, 4, 30])
+@pytest.mark.parametrize("below", [18.0, 25.5, 29.0])
+def test_many_weak_keys_beside_a_strong_one(kv, T, below):
+    """A key with nearly all the weight whose values are zeros, and keys of
+    2^-below of its weight that make the whole output. A weight is an fp16 of
+    which the row's largest is 2^7 or more, so one below 2^-21 of it is off by at
+    most half of fp16's smallest step, 2^-25 / 2^7 = 2^-32 of the largest."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(43)
+    R, D, page, n, strong = 4, 128, 16, 600, 37
+    top = 127 if kv == I8 else 448
+    table = _table(1, 38, 40, g)
+    cache = paged.new_paged_cache(40, 1, D, page_size=page, kv_dtype=kv)
+
+    def put(t, x):
+        t.view(I8).copy_(x.round().to(I8) if kv == I8 else x.to(E4).view(I8))
+    q = torch.randn(D, generator=g)
+    k = torch.randn(40, 1, page, D, generator=g) * top / 5
+    v = torch.rand(40, 1, page, D, generator=g) * (top - 1) + 1
+    pid, row = int(table[0, strong // page]), strong % page
+    k[pid] = 0
+    k[pid, 0, row] = q / q.abs().max() * top
+    v[pid, 0, row] = 0
+    put(cache.k, k.clamp(-top, top))
+    put(cache.v, v)
+    cache.v_scale.fill_(2.0 ** (below - 14))
+    cache.k_scale.fill_(2.0 ** -20 / top)  # the weak keys' scores: near 0
+    cache.k_scale[pid] = 1.0 / top
+    q = q.to(F16)
+    score = float((q.double() * O.code_values(cache.k[pid, 0, row].cpu()) / top).sum())
+    sm = below * 0.6931471805599453 / score
+    q = q.expand(T, R, D).contiguous().cuda()
+    out = paged.paged_attention(q, cache, table.cuda(), _i32([0, T]), _i32([n]), T, sm_scale=sm)
+    want, A, S = O.attend(q.cpu(), _cpu(cache), table, [0, T], [n], sm)
+    tol = 2.0 ** -11 * want.abs() + A * (2.0 ** -11 + 2 * D * U * S + 2.0 ** -16) + \
+        n * 2.0 ** -32 * top * 2.0 ** (below - 14) + torch.finfo(F16).smallest_normal
+    assert ((out.cpu().double() - want).abs() <= tol).all()
+    assert (tol < 0.3 * want.abs()).all()  # they are seen
