@@ -288,7 +288,9 @@ typedef struct {
  * to the table's cs_rows rows. Two sequences must not append into the same
  * page in one call (sharing pages that are only read is fine).
  * q / k / v / q_out: [T, heads, D] with strides in elements (multiples of 8,
- * pointers 16-byte aligned), D contiguous; q_norm_w, k_norm_w [D] of dtype;
+ * pointers 16-byte aligned), D contiguous; the rows of an output apart (a
+ * token's heads before the next token's, or a head's tokens before the next
+ * head's); q_norm_w, k_norm_w [D] of dtype;
  * cos, sin fp32 (cs_dtype SPATTEN_DTYPE_F32) or of dtype.
  */
 typedef struct {

@@ -568,7 +568,10 @@ static int check_rows(const char* who, const char* name, const void* x, int64_t 
 static int check_out_rows(const char* who, const char* name, const void* x, int64_t st, int64_t sh, int T, int H,
                           int D) {
   if (int e = check_rows(who, name, x, st, sh)) return e;
-  if ((T > 1 && st < D) || (H > 1 && sh < D)) return fail(SPATTEN_ERR_INVALID, "%s: rows of %s overlap", who, name);
+  bool apart = (T < 2 || st >= D) && (H < 2 || sh >= D);
+  if (apart && T > 1 && H > 1)  // all heads of a token before the next token's, or the other way round
+    apart = (st - D) / (H - 1) >= sh || (sh - D) / (T - 1) >= st;
+  if (!apart) return fail(SPATTEN_ERR_INVALID, "%s: rows of %s overlap", who, name);
   return SPATTEN_OK;
 }
 
