@@ -29,3 +29,16 @@ def test_rows_of_an_output_do_not_interleave(T, H, st, sh, ok):
     assert N.lib.spatten_paged_attend(a, None, 0, None) == N.ERR_INVALID
     err = N.lib.spatten_last_error().decode()
     assert ("rows of out overlap" in err) == (not ok) and ("workspace of" in err) == ok, err
+
+
+@pytest.mark.parametrize("max_pages", [4, 0])
+def test_batches_without_sequences(max_pages):
+    """Tensors of an empty batch have no memory: their pointers are null."""
+    none = dict(page_table=0, max_pages=max_pages, table_stride=max_pages).items()
+    empty = dict(B=0, T=0, max_tokens=0, cu_tokens=1 << 20, seq_lens=0)
+    assert N.lib.spatten_paged_append(_append(cache=none, q=0, k=0, v=0, q_out=0, **empty), None) == N.OK
+    a = _attend(cache=none, q=0, out=0, **empty)
+    assert N.lib.spatten_paged_attend_workspace_size(a) == 0
+    assert N.lib.spatten_paged_attend(a, None, 0, None) == N.OK
+    assert N.lib.spatten_paged_read(_read(cache=none, B=0, seq_lens=0, idx=0, k_out=0, v_out=0), None) == N.OK
+    assert N.lib.spatten_paged_read(_read(cache=none), None) == N.ERR_INVALID  # three sequences need one
