@@ -84,7 +84,7 @@ def _index(t, name, dev, dim, dtype=torch.int32):
         raise ValueError(f"{name}: on {t.device}, the cache is on cuda:{dev}")
     if t.dtype != dtype or t.dim() != dim:
         raise ValueError(f"{name}: {t.dtype} of {t.dim()} dimensions (need {dtype} of {dim})")
-    if t.stride()[-1] != 1 and t.numel() > 1:
+    if t.stride()[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: last dimension must be contiguous")
     return t.data_ptr()
 

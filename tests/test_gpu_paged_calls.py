@@ -29,3 +29,31 @@ def test_no_sequences(cols):
     out = torch.full((3, 2, 64), 5.0, dtype=F16, device="cuda")
     paged.paged_attention(out.clone(), c, t, _i32([0]), _i32([]), 1, out=out)
     assert (out == 5).all()
+
+
+def test_columns_of_other_tensors():
+    """Index tensors with one column: the stride of a dimension of one entry
+    says nothing."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(61)
+    G, D, page, lens = 2, 64, 16, [5, 16, 1]
+    cache = _filled(I8, 8, G, page, D, g)
+    table = _table(3, 1, 8, g)
+    wide = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    wide[1] = table[:, 0].cuda()
+    column = wide[1:].t()  # [3, 1], strides (1, 3)
+    assert column.stride() == (1, 3)
+    q = torch.randn(3, G, D, generator=g).to(BF16).cuda()
+    cu = _cum([1] * 3)
+    out = paged.paged_attention(q, cache, column, _i32(cu), _i32(lens), 1)
+    _check_attend(out, q, cache, table, cu, lens, D ** -0.5)
+    idx = torch.tensor([[9, 3, 9], [4, 15, 0]], device="cuda")[1:].t()
+    for got, want in zip(paged.paged_read(cache, column, _i32(lens), idx=idx),
+                         paged.paged_read(cache, table.cuda(), _i32(lens), idx=idx.contiguous())):
+        assert torch.equal(got, want)
+    before = _cpu(cache)
+    x = torch.randn(3, 2 * G, D, generator=g).to(BF16).cuda()
+    paged.paged_append(cache, x[:, :G], x[:, G:], column, _i32(cu), _i32(lens), 1)
+    want = O.append(before, x[:, :G].cpu(), x[:, G:].cpu(), table, cu, lens)
+    for got, c in zip(_cpu(cache)[:2], want[1]):
+        assert ((O.code_values(got) - c).abs() <= 1).all()
