@@ -241,7 +241,8 @@ int spatten_decode_attend(const spatten_decode_args* a, void* workspace, size_t 
  * sequence b is row s % page_size of page page_table[b, s / page_size]
  * (int32, row stride table_stride elements). A page number outside
  * [0, num_pages) has no memory: nothing is appended there, and its slots
- * are no keys. page_size is 16, 32, 64 or 128; D is 64 or 128.
+ * are no keys. A row stride of 0 (one row for all sequences) will do where
+ * nothing is appended. page_size is 16, 32, 64 or 128; D is 64 or 128.
  *
  * Scales are not negative, and codes are finite in both types: int8
  * (scale = max|x| / 127) or e4m3 (scale = the smallest power of two with

@@ -510,8 +510,9 @@ int spatten_compact_out_proj(const spatten_compact_out_proj_args* a, void* strea
 }
 
 // Checks a paged cache and brings it into the kernels' form (B: sequences; the page
-// table of none may be empty).
-static int fill_paged_cache(const char* who, const spatten_paged_cache& c, int B, spatten::PagedCache& p) {
+// table of none may be empty; sequences that are only read may share a row of it).
+static int fill_paged_cache(const char* who, const spatten_paged_cache& c, int B, bool writes,
+                            spatten::PagedCache& p) {
   if (c.kv_type != SPATTEN_KV_INT8 && c.kv_type != SPATTEN_KV_E4M3)
     return fail(SPATTEN_ERR_INVALID, "%s: kv_type %d", who, c.kv_type);
   if (c.D != 64 && c.D != 128) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: D=%d (need 64 or 128)", who, c.D);
@@ -525,7 +526,8 @@ static int fill_paged_cache(const char* who, const spatten_paged_cache& c, int B
     return fail(SPATTEN_ERR_UNSUPPORTED, "%s: a pool of 2^32 rows or more", who);
   if ((int64_t)c.max_pages * c.page_size > (int64_t)1 << 30)
     return fail(SPATTEN_ERR_UNSUPPORTED, "%s: page table of more than 2^30 slots", who);
-  if (c.table_stride < c.max_pages) return fail(SPATTEN_ERR_INVALID, "%s: page table stride < max_pages", who);
+  if (c.table_stride < c.max_pages && (writes || c.table_stride != 0))
+    return fail(SPATTEN_ERR_INVALID, "%s: page table stride < max_pages", who);
   if (!c.k || !c.v || !c.k_scale || !c.v_scale || (!c.page_table && B != 0))
     return fail(SPATTEN_ERR_INVALID, "%s: null cache pointer", who);
   if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.k_scale, 4) || !aligned(c.v_scale, 4) ||
@@ -580,7 +582,7 @@ int spatten_paged_append(const spatten_paged_append_args* a, void* stream) {
   static const char* who = "paged_append";
   if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
   spatten::PagedAppendParams p;
-  if (int e = fill_paged_cache(who, a->cache, a->B, p.c)) return e;
+  if (int e = fill_paged_cache(who, a->cache, a->B, true, p.c)) return e;
   if (int e = fill_paged_batch(who, a->dtype, a->B, a->H, a->T, a->max_tokens, a->cu_tokens, a->seq_lens, p.b))
     return e;
   if (p.b.B == 0 || p.b.max_tokens == 0) return ok();
@@ -626,7 +628,7 @@ int spatten_paged_append(const spatten_paged_append_args* a, void* stream) {
 static int fill_paged_attend(const spatten_paged_attend_args* a, spatten::PagedAttendParams& p) {
   static const char* who = "paged_attend";
   if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
-  if (int e = fill_paged_cache(who, a->cache, a->B, p.c)) return e;
+  if (int e = fill_paged_cache(who, a->cache, a->B, false, p.c)) return e;
   if (int e = fill_paged_batch(who, a->dtype, a->B, a->H, a->T, a->max_tokens, a->cu_tokens, a->seq_lens, p.b))
     return e;
   if (a->H < 1 || a->H % p.c.G) return fail(SPATTEN_ERR_INVALID, "%s: H=%d %% G=%d", who, a->H, p.c.G);
@@ -675,7 +677,7 @@ int spatten_paged_read(const spatten_paged_read_args* a, void* stream) {
   static const char* who = "paged_read";
   if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
   spatten::PagedReadParams p;
-  if (int e = fill_paged_cache(who, a->cache, a->B, p.c)) return e;
+  if (int e = fill_paged_cache(who, a->cache, a->B, false, p.c)) return e;
   if (a->dtype != SPATTEN_DTYPE_F16 && a->dtype != SPATTEN_DTYPE_BF16)
     return fail(SPATTEN_ERR_UNSUPPORTED, "%s: dtype %d (need f16 or bf16)", who, a->dtype);
   if (a->B < 0 || a->N < 0) return fail(SPATTEN_ERR_INVALID, "%s: negative size B=%d N=%d", who, a->B, a->N);

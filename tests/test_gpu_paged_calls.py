@@ -57,3 +57,23 @@ def test_columns_of_other_tensors():
     want = O.append(before, x[:, :G].cpu(), x[:, G:].cpu(), table, cu, lens)
     for got, c in zip(_cpu(cache)[:2], want[1]):
         assert ((O.code_values(got) - c).abs() <= 1).all()
+
+
+def test_one_table_for_every_sequence():
+    """Samples of one prompt that only read it: an expanded page table."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(62)
+    G, R, D, page, lens = 2, 4, 128, 32, [100, 33, 100]
+    cache = _filled(I8, 6, G, page, D, g)
+    table = _table(1, 4, 6, g).cuda()
+    for new in ([1, 1, 1], [30, 20, 25]):
+        cu = _cum(new)
+        q = torch.randn(cu[-1], G * R, D, generator=g).to(BF16).cuda()
+        out = paged.paged_attention(q, cache, table.expand(3, -1), _i32(cu), _i32(lens), max(new))
+        _check_attend(out, q, cache, table.cpu().expand(3, -1), cu, lens, D ** -0.5)
+    for a, b in zip(paged.paged_read(cache, table.expand(3, -1), _i32(lens)),
+                    paged.paged_read(cache, table.repeat(3, 1), _i32(lens))):
+        assert torch.equal(a, b)
+    x = torch.zeros(3, G, D, dtype=BF16, device="cuda")
+    with pytest.raises(RuntimeError, match="stride"):
+        paged.paged_append(cache, x, x, table.expand(3, -1), _i32([0, 1, 2, 3]), _i32(lens), 1)

@@ -42,3 +42,16 @@ def test_batches_without_sequences(max_pages):
     assert N.lib.spatten_paged_attend(a, None, 0, None) == N.OK
     assert N.lib.spatten_paged_read(_read(cache=none, B=0, seq_lens=0, idx=0, k_out=0, v_out=0), None) == N.OK
     assert N.lib.spatten_paged_read(_read(cache=none), None) == N.ERR_INVALID  # three sequences need one
+
+
+def test_one_table_for_every_sequence():
+    """A row stride of 0: sequences that share their pages may read them, not
+    append to them."""
+    shared = dict(table_stride=0).items()
+    a = _attend(cache=shared)
+    assert N.lib.spatten_paged_attend(a, None, 0, None) == N.ERR_INVALID
+    assert "workspace of" in N.lib.spatten_last_error().decode()  # that is all it misses
+    assert N.lib.spatten_paged_read(_read(cache=shared, k_out=0, v_out=0), None) == N.ERR_INVALID
+    assert "neither k_out" in N.lib.spatten_last_error().decode()
+    assert N.lib.spatten_paged_append(_append(cache=shared), None) == N.ERR_INVALID
+    assert "stride" in N.lib.spatten_last_error().decode()
