@@ -223,14 +223,25 @@ class PagedQwen3Cache(Cache):
         """cu_tokens of a batch that brings S tokens per sequence."""
         return torch.arange(0, (self.batch + 1) * S, S, dtype=torch.int32, device=self.seq_lens.device)
 
-    def grow(self, layer_idx, n, seen):
-        """Count n more slots (of ``seen`` more positions) in one layer."""
-        if self.held[layer_idx] + n > self.max_tokens:
+    def append(self, layer_idx, n, seen, cu, k, v, **kw):
+        """``paged_append`` of n tokens per sequence (rows k, v, packed by cu =
+        ``packed(n)``) to one layer, counted as ``seen`` more positions; nothing
+        counts when the call is refused."""
+        held = self.held[layer_idx] + n
+        if held > self.max_tokens:
             raise ValueError(f"PagedQwen3Cache: {self.held[layer_idx]} + {n} tokens, room for {self.max_tokens}")
-        self.held[layer_idx] += n
+        lens = self.seq_lens[layer_idx]
+        lens.add_(n)
+        try:
+            q = paged.paged_append(self.pools[layer_idx], k, v, self.page_table, cu, lens, n, **kw)
+        except Exception:
+            lens.sub_(n)
+            raise
+        self.held[layer_idx] = held
         self.seen[layer_idx] += seen
-        self.seq_lens[layer_idx].add_(n)
-        return self.seq_lens[layer_idx]
+        if n < seen:
+            self.pruned[layer_idx] = self.seen[layer_idx]
+        return q
 
     def store(self, layer_idx, k, v, seen):
         """Append finished (normed and rotated) keys and values [B, K, G, D];
@@ -238,11 +249,7 @@ class PagedQwen3Cache(Cache):
         B, K, G, D = k.shape
         if B != self.batch:
             raise ValueError(f"PagedQwen3Cache: batch {B}, made for {self.batch}")
-        lens = self.grow(layer_idx, K, seen)
-        if K < seen:
-            self.pruned[layer_idx] = self.seen[layer_idx]
-        paged.paged_append(self.pools[layer_idx], k.reshape(B * K, G, D), v.reshape(B * K, G, D), self.page_table,
-                           self.packed(K), lens, K)
+        self.append(layer_idx, K, seen, self.packed(K), k.reshape(B * K, G, D), v.reshape(B * K, G, D))
 
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
         """HF's form of ``store`` ([B, G, K, D]); only a prefill's first call may
@@ -314,12 +321,12 @@ class SpattenQwen3Attention(Qwen3Attention):
         cos, sin = position_embeddings  # [B or 1, S, d]: a row per token
         rows = torch.arange(cos.shape[0] * S, dtype=torch.int32, device=q.device)
         positions = rows if cos.shape[0] == B else rows.repeat(B)
-        pool, cu = cache.pools[self.layer_idx], cache.packed(S)
-        lens = cache.grow(self.layer_idx, S, S)
-        q = paged.paged_append(pool, k, v, cache.page_table, cu, lens, S, q=q, cos=cos.reshape(-1, d),
-                               sin=sin.reshape(-1, d), positions=positions, q_norm_w=self.q_norm.weight,
-                               k_norm_w=self.k_norm.weight, eps=self.q_norm.variance_epsilon)
-        out = paged.paged_attention(q, pool, cache.page_table, cu, lens, S, sm_scale=self.scaling)
+        cu = cache.packed(S)
+        q = cache.append(self.layer_idx, S, S, cu, k, v, q=q, cos=cos.reshape(-1, d), sin=sin.reshape(-1, d),
+                         positions=positions, q_norm_w=self.q_norm.weight, k_norm_w=self.k_norm.weight,
+                         eps=self.q_norm.variance_epsilon)
+        out = paged.paged_attention(q, cache.pools[self.layer_idx], cache.page_table, cu,
+                                    cache.seq_lens[self.layer_idx], S, sm_scale=self.scaling)
         return self.o_proj(out.view(B, S, H * d)), None
 
     @torch.no_grad()

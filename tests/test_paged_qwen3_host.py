@@ -132,3 +132,23 @@ def test_sizes_that_hf_asks_for():
     assert c.max_batch_size == 2 and c.max_cache_len == 18 and c.get_max_cache_shape() == 18
     c.reset()
     assert c.get_seq_length() == 0 and c.held == [0, 0] and c.pruned == [0, 0] and (c.seq_lens == 0).all()
+
+
+def test_a_refused_append_counts_nothing(monkeypatch):
+    """An append that refuses its arguments (here: a cache without a GPU, rows of
+    another type) leaves the counts as they were, on the host and beside the
+    pools; and so does a forward that finds no room."""
+    from spatten_b200 import paged
+    c = _cache(held=(10, 6), seen=(10, 10))
+    was = list(c.held), list(c.seen), list(c.pruned), c.seq_lens.clone()
+    x = torch.zeros(2, 3, 2, 64, dtype=torch.float16)
+    for k, seen in ((x, 3), (x, 5), (x.float(), 3), (torch.zeros(2, 9, 2, 64, dtype=torch.float16), 9)):
+        for layer in range(2):
+            with pytest.raises((ValueError, TypeError)):
+                c.store(layer, k, k, seen)
+            assert (c.held, c.seen, c.pruned) == was[:3] and torch.equal(c.seq_lens, was[3])
+    # the call itself finds the new lengths
+    calls = []
+    monkeypatch.setattr(paged, "paged_append", lambda *a, **kw: calls.append((a[5].tolist(), a[6])))
+    c.store(1, x, x, 5)
+    assert calls == [([9, 9], 3)] and c.held == [10, 9] and c.seen == [10, 15] and c.pruned == [0, 15]
