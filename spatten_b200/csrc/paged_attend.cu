@@ -57,6 +57,7 @@ constexpr int kWarps = 4;
 constexpr uint32_t kLineCost = 16;
 constexpr float kNone = -3.402823466e38f;  // reference of a row without a key: finite, so that -inf less it is -inf
 constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+constexpr int kKeys = 16;  // of a tile, which lies within one page
 
 // sequences whose prefix sums fit the shared memory
 constexpr int kMaxBatch = 8192;
@@ -181,19 +182,15 @@ SPATTEN_DEV uint32_t transpose8x8(uint32_t x) {
 // Row tiles of a sequence, and key tiles that its last row sees (one at least,
 // so that rows without a key are written).
 SPATTEN_DEV int row_tiles(const PagedSeq& s, int R, int rows) { return (int)(((int64_t)s.n * R + rows - 1) / rows); }
-SPATTEN_DEV int key_tiles(const PagedSeq& s, int keys) {
-  return max(1, (min(s.old + s.n, s.len) + keys - 1) / keys);
-}
+SPATTEN_DEV int key_tiles(const PagedSeq& s) { return max(1, (min(s.old + s.n, s.len) + kKeys - 1) / kKeys); }
 
 template <int D, int NB>
 struct Shape {
   static constexpr int kRows = 8 * NB;
-  static constexpr int kBlocks = 1;              // 16-key blocks per step, each within one page
-  static constexpr int kKeys = 16 * kBlocks;
-  static constexpr int kStages = 4;              // steps of a warp's ring
+  static constexpr int kStages = 4;              // tiles of a warp's ring
   static constexpr int kCtas = 3;                // resident per SM
-  static constexpr int kBlockBytes = 16 * D;     // K or V codes of a block
-  static constexpr int kStageBytes = 2 * kBlocks * kBlockBytes;
+  static constexpr int kBlockBytes = kKeys * D;  // K or V codes of a tile
+  static constexpr int kStageBytes = 2 * kBlockBytes;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kOPad = D + 4;            // floats of a row in the join, which reuses the ring
   static_assert(kWarps * kRows * kOPad * 4 <= kRing, "the join fits the ring");
@@ -276,8 +273,8 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, NB>::kCtas)
 paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf16) {
   using SH = Shape<D, NB>;
   using Ops = Operands<KV, D, NB>;
-  constexpr int ROWS = SH::kRows, KS = D / 16, NT = 32 * kWarps, BL = SH::kBlocks, KEYS = SH::kKeys;
-  constexpr int AHEAD = 32 / BL;    // tiles whose pages and scales a warp holds
+  constexpr int ROWS = SH::kRows, KS = D / 16, NT = 32 * kWarps;
+  constexpr int AHEAD = 32;  // tiles whose pages and scales a warp holds
   constexpr int ST = SH::kStages;
   extern __shared__ __align__(128) uint8_t dsm[];
   float (*sm_o)[ROWS][SH::kOPad] = reinterpret_cast<float (*)[ROWS][SH::kOPad]>(dsm);  // over the rings
@@ -289,7 +286,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   grid_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
   const int G = p.c.G, R = p.b.H / G, page = p.c.page, page_log = __ffs(page) - 1;
-  const LaneOffsets<D> lo(lane);
+  const LaneOffsets<D> offs(lane);
   const uint8_t* const k_lane = p.c.k + lane * 16;
   const uint8_t* const v_lane = p.c.v + lane * 16;
 
@@ -302,7 +299,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     if (b >= p.b.B) return 0u;
     const PagedSeq s = paged_seq(p.b, p.c, b);
     if (paged_serves(p, s, R)) n = (uint32_t)G * row_tiles(s, R, ROWS);
-    return (uint32_t)key_tiles(s, KEYS);
+    return (uint32_t)key_tiles(s);
   };
   uint32_t n0, k0 = 0;  // of sequence `tid`
   for (int base = 0; base < p.b.B; base += NT) {
@@ -383,7 +380,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
   while (u < u1) {
     while (pre[b + 1] <= u) ++b;
     const PagedSeq sq = paged_seq(p.b, p.c, b);
-    const uint32_t KT = key_tiles(sq, KEYS), KU = units_of(KT), RT = row_tiles(sq, R, ROWS);
+    const uint32_t KT = key_tiles(sq), KU = units_of(KT), RT = row_tiles(sq, R, ROWS);
     const uint32_t local = u - pre[b], line = local / KU, v0 = local % KU, v1 = min(KU, v0 + (u1 - u));
     const int g = line / RT, rt = line % RT;
     const uint32_t t0 = few ? v0 * chunk : max(v0, lead) - lead, t1 = few ? min(KT, v1 * chunk) : max(v1, lead) - lead;
@@ -391,7 +388,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     // slots that the tile's last and first row see
     const int lim_max = min(sq.old + min((r0 + ROWS - 1) / R, sq.n - 1) + 1, sq.len);
     const int lim_min = min(sq.old + r0 / R + 1, sq.len);
-    const uint32_t t_end = min(t1, (uint32_t)(max(lim_max, 0) + KEYS - 1) / KEYS);
+    const uint32_t t_end = min(t1, (uint32_t)(max(lim_max, 0) + kKeys - 1) / kKeys);
 
     // queries: row gid of each 8-row block, all dims of it in the four lanes of gid
     uint4 raw[NB][KS / 2];
@@ -406,20 +403,20 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     }
 
     // this warp's tiles t0 + warp, + 4, ..: lane i keeps the row offset and the
-    // scales of block i % BL of tile i / BL of the AHEAD tiles at hand, and the
-    // page of the AHEAD tiles after them
+    // scales of tile i of the AHEAD tiles at hand, and the page of the one AHEAD
+    // tiles on
     const int nt = t_end > t0 + warp ? (t_end - t0 - warp + kWarps - 1) / kWarps : 0;
-    auto tile_slot = [&](int j) { return (int)(t0 + warp + kWarps * j) * KEYS; };
+    auto tile_slot = [&](int j) { return (int)(t0 + warp + kWarps * j) * kKeys; };
     auto page_of = [&](int j) {
-      const int slot = tile_slot(j + lane / BL) + 16 * (lane % BL);
+      const int slot = tile_slot(j + lane);
       return slot < lim_max ? paged_page(p.c, b, slot >> page_log) : -1;
     };
     auto row_of = [&](int j, int pid) {
-      const int slot = tile_slot(j + lane / BL) + 16 * (lane % BL);
+      const int slot = tile_slot(j + lane);
       return pid >= 0 ? ((uint32_t)pid * G + g) * page + (slot & (page - 1)) : kNoRow;
     };
     const uint32_t ring = smem_u32(dsm) + warp * ST * SH::kStageBytes;
-    uint32_t row_l = kNoRow, have_l = 0, have_n = 0;  // have: blocks with memory, a bit per lane
+    uint32_t row_l = kNoRow, have_l = 0, have_n = 0;  // have: tiles with memory, a bit per lane
     int pid_n = -1;
     float ks_l = 0.f, vs_l = 0.f, ks_n = 0.f, vs_n = 0.f;
     // tile j on its way into slot j % ST (an empty group past the end)
@@ -436,14 +433,10 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
           if (nt > j + AHEAD) pid_n = page_of(j + AHEAD);
         }
         const uint32_t dst = ring + (j % ST) * SH::kStageBytes;
-#pragma unroll
-        for (int kb = 0; kb < BL; ++kb) {
-          const uint32_t row = __shfl_sync(0xffffffffu, row_l, BL * at + kb);
-          const uint64_t off = row == kNoRow ? 0 : (uint64_t)row * D;
-          const int live = row == kNoRow ? 0 : lim_max - (tile_slot(j) + 16 * kb);
-          load_block<D>(dst + kb * SH::kBlockBytes, lo, k_lane + off, lane, row == kNoRow ? 0 : 16);
-          load_block<D>(dst + (BL + kb) * SH::kBlockBytes, lo, v_lane + off, lane, live);
-        }
+        const uint32_t row = __shfl_sync(0xffffffffu, row_l, at);
+        const uint64_t off = row == kNoRow ? 0 : (uint64_t)row * D;
+        load_block<D>(dst, offs, k_lane + off, lane, row == kNoRow ? 0 : kKeys);
+        load_block<D>(dst + SH::kBlockBytes, offs, v_lane + off, lane, row == kNoRow ? 0 : lim_max - tile_slot(j));
       }
       cp_async_commit();
     };
@@ -518,37 +511,25 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
           ks_l = ks_n;
           vs_l = vs_n > 0.f ? fmaxf(log2f(vs_n), kNoScale) : kNoScale;  // log2 of the scale
         }
-        float ks[BL], lv[BL];
-        bool none = false;
+        const float ks = __shfl_sync(0xffffffffu, ks_l, at), lv = __shfl_sync(0xffffffffu, vs_l, at);
+        const bool none = !((have_l >> at) & 1u);
+        float s[NB][4];
+        uint32_t k0[KS], k1[KS];
+        read_k<D>(k0, stage, offs, 0);
+        read_k<D>(k1, stage, offs, 1);
+        ops.template scores<TERMS>(k0, k1, s);
 #pragma unroll
-        for (int kb = 0; kb < BL; ++kb) {
-          ks[kb] = __shfl_sync(0xffffffffu, ks_l, BL * at + kb);
-          lv[kb] = __shfl_sync(0xffffffffu, vs_l, BL * at + kb);
-          none |= !((have_l >> (BL * at + kb)) & 1u);
+        for (int nb = 0; nb < NB; ++nb) {
+          const float f0 = cq[nb][0] * ks, f1 = cq[nb][1] * ks;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[nb][i] *= i & 1 ? f1 : f0;
         }
-        float s[BL][NB][4];
+        if (slot0 + kKeys > lim_min || none) {  // warp-uniform
 #pragma unroll
-        for (int kb = 0; kb < BL; ++kb) {
-          uint32_t k0[KS], k1[KS];
-          read_k<D>(k0, stage + kb * SH::kBlockBytes, lo, 0);
-          read_k<D>(k1, stage + kb * SH::kBlockBytes, lo, 1);
-          ops.template scores<TERMS>(k0, k1, s[kb]);
+          for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const float f0 = cq[nb][0] * ks[kb], f1 = cq[nb][1] * ks[kb];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[kb][nb][i] *= i & 1 ? f1 : f0;
-          }
-        }
-        if (slot0 + KEYS > lim_min || none) {  // warp-uniform
-#pragma unroll
-          for (int kb = 0; kb < BL; ++kb)
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (!((have_l >> (BL * at + kb)) & 1u) || slot0 + 16 * kb + gid + 4 * (i & 2) >= lim[nb][i & 1])
-                  s[kb][nb][i] = -INFINITY;
+            for (int i = 0; i < 4; ++i)
+              if (none || slot0 + gid + 4 * (i & 2) >= lim[nb][i & 1]) s[nb][i] = -INFINITY;
         }
         // p = 2^(s - m), and w = 2^(s + log2 v_scale - M)
         float top[NB][2], topw[NB][2];  // largest s, and s + log2 v_scale, of this lane
@@ -557,13 +538,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            top[nb][c] = topw[nb][c] = -INFINITY;
-#pragma unroll
-            for (int kb = 0; kb < BL; ++kb) {
-              const float t = fmaxf(s[kb][nb][c], s[kb][nb][2 + c]);
-              top[nb][c] = fmaxf(top[nb][c], t);
-              topw[nb][c] = fmaxf(topw[nb][c], t + lv[kb]);
-            }
+            top[nb][c] = fmaxf(s[nb][c], s[nb][2 + c]);
+            topw[nb][c] = top[nb][c] + lv;
             up |= top[nb][c] > m[nb][c] + kSlack || topw[nb][c] > M[nb][c] + (kRoom + kSlack);
           }
         if (__any_sync(0xffffffffu, up)) {
@@ -589,39 +565,32 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
               M[nb][c] = Mn;
             }
         }
-        uint32_t pf[BL][NB][2];
+        uint32_t pf[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const float m0 = m[nb][0], m1 = m[nb][1], M0 = M[nb][0], M1 = M[nb][1];
 #pragma unroll
-          for (int kb = 0; kb < BL; ++kb)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float s0 = s[kb][nb][2 * i], s1 = s[kb][nb][2 * i + 1];
-              l[nb][0] += fast_exp2(s0 - m0);
-              l[nb][1] += fast_exp2(s1 - m1);
-              pf[kb][nb][i] =
-                  transpose8x8(pack2<__half>(fast_exp2(s0 + (lv[kb] - M0)), fast_exp2(s1 + (lv[kb] - M1))));
-            }
+          for (int i = 0; i < 2; ++i) {
+            const float s0 = s[nb][2 * i], s1 = s[nb][2 * i + 1];
+            l[nb][0] += fast_exp2(s0 - m0);
+            l[nb][1] += fast_exp2(s1 - m1);
+            pf[nb][i] = transpose8x8(pack2<__half>(fast_exp2(s0 + (lv - M0)), fast_exp2(s1 + (lv - M1))));
+          }
         }
         // values
+        uint32_t v[4][D / 32];
 #pragma unroll
-        for (int kb = 0; kb < BL; ++kb) {
-          const uint32_t blk = stage + (BL + kb) * SH::kBlockBytes;
-          uint32_t v[4][D / 32];
+        for (int r = 0; r < 4; ++r) read_v<D>(v[r], stage + SH::kBlockBytes, offs, r);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) read_v<D>(v[r], blk, lo, r);
+        for (int w = 0; w < D / 32; ++w) {
+          uint32_t lo[4], hi[4];
+          Ops::values(v[0][w], v[1][w], lo);
+          Ops::values(v[2][w], v[3][w], hi);
 #pragma unroll
-          for (int w = 0; w < D / 32; ++w) {
-            uint32_t lo[4], hi[4];
-            Ops::values(v[0][w], v[1][w], lo);
-            Ops::values(v[2][w], v[3][w], hi);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t a[4] = {lo[2 * h], lo[2 * h + 1], hi[2 * h], hi[2 * h + 1]};
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb) mma_16816<__half>(o[nb][2 * w + h], a, pf[kb][nb][0], pf[kb][nb][1]);
-            }
+            for (int nb = 0; nb < NB; ++nb) mma_16816<__half>(o[nb][2 * w + h], a, pf[nb][0], pf[nb][1]);
           }
         }
       }
