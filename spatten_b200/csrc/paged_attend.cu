@@ -477,7 +477,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
           for (int j = 0; j < 4; ++j) sum += fabsf(f[s][j]);
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        terms = __all_sync(0xffffffffu, !(top * D > kOutlier * sum));  // (rows that are not finite: either)
+        terms = __all_sync(0xffffffffu, !(top > kOutlier / D * sum));  // (rows that are not finite: either)
       }
       if (terms) {
         if constexpr (Ops::kTerms) ops.set_terms(f, qs.up);
