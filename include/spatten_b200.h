@@ -246,14 +246,16 @@ int spatten_decode_attend(const spatten_decode_args* a, void* workspace, size_t 
  *
  * Scales are not negative, and codes are finite in both types: int8
  * (scale = max|x| / 127) or e4m3 (scale = the smallest power of two with
- * max|x| <= 448 * scale, so that dividing by it is exact).
+ * max|x| <= 448 * scale, 2^-126 at the least, so that dividing by it is exact).
  *
  * A batch's new tokens are packed: sequence b brings the rows cu_tokens[b]
  * .. cu_tokens[b+1]-1 (int32 [B+1], ascending, within [0, T]) of q / k / v /
  * out, and holds seq_lens[b] tokens in all (int32 [B]), these included, which
  * are its last ones: row cu_tokens[b] + i is slot
  * seq_lens[b] - (cu_tokens[b+1] - cu_tokens[b]) + i. A sequence whose bounds
- * descend or leave [0, T] brings no rows. max_tokens bounds the
+ * descend or leave [0, T] brings no rows. (Sequences that claim the same
+ * rows write them in any order; attention leaves out as it was where their
+ * claims add up to more work than 32 bits number.) max_tokens bounds the
  * tokens of one sequence (rows beyond it are left alone), so that the launch
  * needs no device value on the host; it sizes the grid. Rows behind the last
  * sequence are neither read nor written. All of these may change between the
@@ -325,7 +327,8 @@ int spatten_paged_append(const spatten_paged_append_args* a, void* stream);
  * sees slots n < seq_lens[b] - n_b + i + 1 (n_b: the sequence's new tokens),
  * its own among them when they were appended before:
  *   out[row, h] = softmax(sm_scale * q[row, h] . K[h / (H/G)]) . V[h / (H/G)]
- * over fp32 scores and statistics; 0 for a row that sees no key. Serves one
+ * over fp32 scores and statistics, with q exact or to 2^-22 of its row's
+ * largest magnitude and the weights of V in fp16; 0 for a row that sees no key. Serves one
  * token per sequence, a few drafted ones, or the next piece of a prompt.
  * q, out: [T, H, D] by strides as in spatten_paged_append; H % G == 0,
  * H / G <= 128, B <= 8192.

@@ -351,7 +351,12 @@ cudaError_t append_heads(const PagedAppendParams& p, int passes, cudaStream_t st
 
 // A few tokens: a head per row of lanes, one pass per CTA (latency). Prompts:
 // four heads share a token's rotation (two at a time: 168 -> 182 us at 4 prompts
-// of 8192 tokens), two passes the set-up (one: 173 us).
+// of 8192 tokens), two passes the set-up (one: 173 us). The first form against the
+// second (32/8 heads x 128): one sequence of 1, 15, 32 and 64 tokens 2.6, 2.6, 3.3 and
+// 4.2 us against 2.7, 3.7, 3.8 and 4.5; 8 sequences of 15, 32 and 64 3.7, 5.1 and 7.8
+// against 4.7, 5.8 and 6.7; 64 of 1, 4, 8, 15 and 32 5.4, 8.1, 9.9, 15.3 and 23.4
+// against 5.8, 8.1, 9.1, 13.0 and 16.9. The border lies between where 64 sequences
+// and where one would have it.
 template <typename T, int KV, int D, int PAGE>
 cudaError_t append_launch(const PagedAppendParams& p, cudaStream_t st) {
   return p.b.max_tokens < 16 ? append_heads<T, KV, D, PAGE, 1>(p, 1, st) : append_heads<T, KV, D, PAGE, 4>(p, 2, st);

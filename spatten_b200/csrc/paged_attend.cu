@@ -6,16 +6,21 @@
 //   S^T [16 keys x 8 rows]  = K codes . q'^T,
 //   O^T [D x 8 rows]       += V codes^T . P^T   (f16, every code is one; fp32 sums).
 // A warp's tiles come through a ring of its own (cp.async, three tiles in
-// flight; through registers the largest case below took 782 us). The order of the contracted dims (of S) and of the output
-// dims (of O) is free, so each lane reads 16 consecutive bytes of a row and takes
-// them as fragments as they are, and every byte is read once per row tile. P^T
-// turns from the layout of S^T into that of an operand with one 8x8 transpose
-// (movmatrix).
+// flight; through registers the largest case below took 782 us). The order of the
+// contracted dims (of S) and of the output dims (of O) is free, so each lane reads 16
+// consecutive bytes of a row and takes them as fragments as they are, and every byte
+// is read once per row tile. P^T turns from the layout of S^T into that of an operand
+// with one 8x8 transpose (movmatrix).
 //
 // Bound by HBM where there are keys enough: 64 sequences x 8 heads x 32768 keys
-// of int8, 667 us = 6.44 TB/s, 0.99 of the measured copy rate; one sequence of
-// 131001, 53 us = 5.0 TB/s; 48 ragged ones of up to 8192, 79 us = 5.2 TB/s. One of
-// 777 takes 8.7 us, which is the chain of dependent loads and the second launch.
+// of int8, 660 to 680 us = 6.3 to 6.5 TB/s in short runs at full clocks; in a long run
+// the GPU meets its power limit (990 W, 1.55 GHz instead of 1.97) and a call
+// takes 676 to 726 us from one GPU to the next, 0.91 to 0.97 of the measured copy
+// rate. One sequence of 131001, 53 us = 5.0 TB/s; 48 ragged ones of up to 8192, 79 us
+// = 5.2 TB/s. One of 777 takes 8.8 us, which is the chain of dependent loads and the
+// second launch. Beyond 16 rows each row tile walks the keys by itself: 32 sequences
+// over 8192 keys of e4m3 take 100, 184, 274 and 379 us at 16, 32, 48 and 64 rows (the
+// cache's bytes once: 82 us).
 //
 // Numerics:
 //  * q' is the query row times a power of two, in what K's product takes: f16, or
@@ -23,8 +28,10 @@
 //  * s = (q' . codes) (sm_scale log2(e) k_scale / that power) in fp32, p =
 //    2^(s - m) with a reference m that follows the row's maximum (updated when it is
 //    exceeded by more than kSlack); l sums p in fp32.
-//  * P is rounded to f16 for the second product (2^-12 of each weight), after
-//    v_scale has gone into it: w = 2^(s + log2 v_scale - M), M a second reference
+//  * P is rounded to f16 for the second product (2^-12 of each weight, as much as
+//    an fp16 output's own rounding: 2.7e-4 off the 64-bit result where fp32 weights
+//    are 2.0e-4; a second f16 term would double that product), after v_scale has gone
+//    into it: w = 2^(s + log2 v_scale - M), M a second reference
 //    that follows max(s + log2 v_scale), kRoom below it. A block with a tiny scale and
 //    all the weight keeps its 11 bits beside blocks with large scales and no weight,
 //    and a weight down to 2^-21 of the row's largest beside that one (2^-32: half of
@@ -34,11 +41,11 @@
 // so that a ragged batch and one long sequence fill the GPU alike and a captured
 // launch follows the lengths it finds. A line is a (sequence, KV head, row tile).
 // Few lines: each is cut into chunks of equal length, one per CTA (16 sequences x 8
-// heads over up to 1000 keys: 22 -> 18 us). Many: the lines' units (16-key tiles, plus kLineCost for a line's set-up) are numbered and
-// cut into equal ranges, one per CTA. The four warps of a
-// CTA take turns on its tiles and join in shared memory; a (sequence, head, row
-// tile) that a range's border cuts leaves (m, l, M, o) partials in the workspace,
-// which a second kernel joins in a fixed order.
+// heads over up to 1000 keys: 22 -> 18 us). Many: the lines' units (16-key tiles,
+// plus kLineCost for a line's set-up) are numbered and cut into equal ranges, one per
+// CTA. The four warps of a CTA take turns on its tiles and join in shared memory; a
+// (sequence, head, row tile) that a range's border cuts leaves (m, l, M, o) partials
+// in the workspace, which a second kernel joins in a fixed order.
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -71,8 +78,8 @@ using Workspace = PagedPartials;
 // Beside int8 codes, one block of eight query rows has another form, in which the
 // codes go into integer products as they are: three int8 terms a query, q' =
 // 65536 q1 + 256 q2 + q3 rounded to an integer of at most 2^22, with exact sums.
-// Without the widening of K, 64 sequences x 8 heads x 32768 keys take 670 us, bound
-// by HBM alone; with it 699, and 815 instead of 735 on a GPU that its power limit
+// Without the widening of K, 64 sequences x 8 heads x 32768 keys take 666 us, bound
+// by HBM alone; with it 697, and 818 instead of 734 on a GPU that its power limit
 // slows down. The rounding is 2^-22 of the row's largest element, and within
 // what a sum of D fp32 products is off by where that element is at most kOutlier
 // times the row's mean magnitude; a tile with a row beyond takes the f16 form. (With
@@ -725,12 +732,17 @@ namespace {
 
 // Which kernels a call takes. Sequences of more than kTcRows query rows per KV
 // head (pieces of prompts) go to the tcgen05 kernel, the others to the one above.
-// 64 rows take 40 us there and 42 us here at 4 sequences x 8 heads over 4096 keys,
-// but 24 and 15 us at one over 800; 96 rows 40 and 55 us at the former. The
-// host knows the largest sequence only; where
+// 64 rows (8 KV heads x 128, int8) take 40 us there and 43 us here at 4 sequences
+// over 4096 keys, 61 and 71 us at one over 32768, 349 and 476 us at 32 over 8192, but
+// 49 and 44 us at 16 over 1000 (e4m3) and 24 and 15 us at one over 800; 96 rows 40
+// and 57, 60 and 94, 331 and 702, 50 and 56, 24 and 15 us. So the sides meet at 40
+// rows where sequences are many and long and beyond 128 where they are few and short;
+// the border is in between, as lengths are not known on the host, which
+// knows the largest sequence's rows only. Where
 // the rows show that some must be shorter, both are launched and each serves its
 // own, so that single tokens beside a prompt's piece keep the kernel made for
-// them (the other launch costs about 4 us).
+// them (512 new tokens over 4096 take 63 us, 47 single ones over 4000 76, together
+// 150).
 struct Plan {
   PagedAttendParams tc, few;
   bool use_tc, use_few;

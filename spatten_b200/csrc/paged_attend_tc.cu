@@ -32,8 +32,8 @@
 // the tile before (512 new tokens over 32768: 376 us instead of 320).
 //
 // 512 new tokens over 32768 (32 heads, 8 KV heads, D = 128, int8): 320 us, 854
-// TFLOP/s, 0.51 of the measured bf16 rate; 1024 over 8192, 2 sequences, e4m3: 355 us,
-// 726 TFLOP/s; a prompt of 4096: 222 us, 620 TFLOP/s. What bounds it: one thread per
+// TFLOP/s, 0.51 of the measured bf16 rate; 1024 over 8192, 2 sequences, e4m3: 343 us,
+// 752 TFLOP/s; a prompt of 4096: 223 us, 616 TFLOP/s. What bounds it: one thread per
 // row takes a tile's 64 scores through a chain of load, maximum, exponentials and
 // store that two warps per scheduler do not hide; then a line's set-up (queries,
 // the first tile, the epilogue).

@@ -6,7 +6,7 @@ K and V are codes (int8 or e4m3) in pages of ``page_size`` tokens with one
 fp32 scale per page and KV head; a value is code * scale. Sequence b's slot s
 is row ``s % page_size`` of page ``page_table[b, s // page_size]`` (int32; an
 entry outside the pool has no memory: nothing is stored there, and its slots
-are no keys). The new tokens of a batch are packed: sequence b brings rows
+are no keys; an expanded table, one row for all sequences, can be read). The new tokens of a batch are packed: sequence b brings rows
 ``cu_tokens[b] .. cu_tokens[b+1]-1`` and holds ``seq_lens[b]`` tokens in all,
 these included, which are its last ones. ``max_tokens`` bounds the tokens of
 one sequence; the index tensors stay on the device, so a captured call can be
