@@ -154,7 +154,9 @@ class PagedQwen3Cache(Cache):
         the last ones), in every layer; their slots are written again by the next
         tokens. A pruned prompt can only be forgotten as a whole: which of its
         positions a layer kept is not known here."""
-        keep = max_length if max_length >= 0 else max(self.seen[0] + max_length, 0)
+        keep = int(max_length)
+        if keep < 0:
+            keep = max(self.seen[0] + keep, 0)
         drop = [max(n - keep, 0) for n in self.seen]
         if not any(drop):
             return

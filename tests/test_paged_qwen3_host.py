@@ -152,3 +152,13 @@ def test_a_refused_append_counts_nothing(monkeypatch):
     monkeypatch.setattr(paged, "paged_append", lambda *a, **kw: calls.append((a[5].tolist(), a[6])))
     c.store(1, x, x, 5)
     assert calls == [([9, 9], 3)] and c.held == [10, 9] and c.seen == [10, 15] and c.pruned == [0, 15]
+
+
+def test_lengths_given_as_tensors_and_empty_caches():
+    c = _cache()
+    c.crop(torch.tensor(4))
+    assert c.held == c.seen == [4, 4] and all(type(n) is int for n in c.held + c.seen)
+    c.reset()
+    c.reorder_cache(torch.tensor([1, 1]))
+    c.batch_repeat_interleave(2)
+    assert c.batch == 4 and c.held == [0, 0] and c.seq_lens.shape == (2, 4)
