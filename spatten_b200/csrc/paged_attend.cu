@@ -28,7 +28,7 @@
 //  * s = (q' . codes) (sm_scale log2(e) k_scale / that power) in fp32, p =
 //    2^(s - m) with a reference m that follows the row's maximum (updated when it is
 //    exceeded by more than kSlack); l sums p in fp32.
-//  * P is rounded to f16 for the second product (2^-12 of each weight, as much as
+//  * P is rounded to f16 for the second product (2^-11 of each weight, as much as
 //    an fp16 output's own rounding: 2.7e-4 off the 64-bit result where fp32 weights
 //    are 2.0e-4; a second f16 term would double that product), after v_scale has gone
 //    into it: w = 2^(s + log2 v_scale - M), M a second reference
