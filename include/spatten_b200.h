@@ -374,6 +374,119 @@ typedef struct {
 int spatten_paged_read(const spatten_paged_read_args* a, void* stream);
 
 /*
+ * Trees of drafted tokens: the new tokens of sequence b form a tree (or
+ * several), parents[row] (int32 [T]) being the place of a token's parent among
+ * its sequence's new tokens (0 for the first), which comes before its own; any
+ * other value makes it a child of the cached tokens. Writes
+ *   tree[row]      the new tokens that it sees (itself and its ancestors) as
+ *                  bits: bit j & 31 of word j >> 5 of its tree_words words (row
+ *                  stride tree_stride words) is new token j; and
+ *   positions[row] = seq_lens[b] - n_b + its depth (optional): what
+ *                  spatten_paged_append rotates by.
+ * for the first max_tokens (at most 1024, and 32 * tree_words) tokens of each
+ * sequence; other rows are left alone. One call serves every layer of a step.
+ */
+typedef struct {
+  int B, T, max_tokens;
+  const int32_t* cu_tokens;
+  const int32_t* seq_lens;
+  const int32_t* parents;
+  int32_t* tree;
+  int64_t tree_stride;
+  int tree_words;
+  int32_t* positions;
+} spatten_paged_tree_args;
+
+int spatten_paged_tree(const spatten_paged_tree_args* a, void* stream);
+
+/*
+ * spatten_paged_attend with more beside it:
+ *  * tree (optional, int32 [T, tree_words] with row stride tree_stride; 32 *
+ *    tree_words >= max_tokens): a row sees the slots before its sequence's new
+ *    tokens, and of these the ones whose bits are set in its words (whether
+ *    before or behind it; bits from n_b on count as clear);
+ *  * weight, position (optional, together; fp32 and int32 [num_pages, G,
+ *    page_size] beside the pool): the softmax weights that the call's rows give
+ *    a slot, summed in fp32 over the rows and the H / G heads of its KV head, are
+ *    added to its weight. The slots of the new tokens start from 0 and take
+ *    positions[row] (int32 [T]; NULL: the slot) as their position. The slots
+ *    of a page without memory have none. Two sequences of one call must not
+ *    share pages then. A NaN among a head's scores makes its weights NaN.
+ */
+typedef struct {
+  spatten_paged_attend_args attend;
+  const int32_t* tree;
+  int64_t tree_stride;
+  int tree_words;
+  float* weight;
+  int32_t* position;
+  const int32_t* positions;
+} spatten_paged_attend_ext_args;
+
+size_t spatten_paged_attend_ext_workspace_size(const spatten_paged_attend_ext_args* a);
+int spatten_paged_attend_ext(const spatten_paged_attend_ext_args* a, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/*
+ * Eviction by accumulated attention weight, the cascade's token pruning
+ * (spatten_bert.py:136-150) on a cache: a sequence of more than `keep` tokens
+ * keeps the tokens at the `recent` newest positions (position > newest -
+ * recent; no more than `keep`, which then are the ones of the largest weight)
+ * and of the others those of the largest weight, ties to the lower slot. With
+ * per_head each KV head chooses by its own weights and positions (the heads then
+ * hold different tokens in a slot); else by the sum of the heads' weights, rounded
+ * to fp32, and the first head's positions. A weight that is NaN or negative
+ * counts as 0.
+ * Kept tokens in slots before `keep` stay; those behind move into the free
+ * slots before it, both in ascending order, with their weights and positions. In
+ * the page that they come to their codes are round(code * S_old / S), S the larger
+ * of that page's scale (0 if none of its tokens stays) and the one that the
+ * largest moved magnitude needs; where S grew its other codes are rounded again as
+ * in spatten_paged_append. new_lens[b] (int32, may be seq_lens) = keep, or
+ * seq_lens[b] where that is not above it. A sequence with a slot that has no
+ * memory is left as it is. Sequences must not share pages that are moved into.
+ * At most 2^20 slots in a page-table row; 1 <= keep, 0 <= recent.
+ */
+typedef struct {
+  spatten_paged_cache cache;
+  int B;
+  const int32_t* seq_lens;
+  float* weight;
+  int32_t* position;
+  int keep, recent, per_head;
+  int32_t* new_lens;
+} spatten_paged_evict_args;
+
+size_t spatten_paged_evict_workspace_size(const spatten_paged_evict_args* a);
+int spatten_paged_evict(const spatten_paged_evict_args* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Keeps the accepted ones of the new tokens: accepted[b] (int32 [B, n_accepted],
+ * row stride accepted_stride) lists places among sequence b's new tokens in
+ * ascending order and ends at the first entry that is not above the one before
+ * it, is no new token, or whose slot has no memory (-1 behind a short list). The
+ * j-th accepted token moves to slot seq_lens[b] - n_b + j (rounded to that page's
+ * scale as in spatten_paged_evict), and with it, where given, its weight and
+ * position; new_lens[b] = seq_lens[b] - n_b + the list's length. cu_tokens as in
+ * spatten_paged_append (no rows are read; T is not needed). new_lens must not
+ * overlap seq_lens. Sequences must not share pages of the new tokens.
+ */
+typedef struct {
+  spatten_paged_cache cache;
+  int B;
+  const int32_t* cu_tokens;
+  const int32_t* seq_lens;
+  const int32_t* accepted;
+  int64_t accepted_stride;
+  int n_accepted;
+  float* weight;
+  int32_t* position;
+  int32_t* new_lens;
+} spatten_paged_keep_args;
+
+int spatten_paged_keep(const spatten_paged_keep_args* a, void* stream);
+
+/*
  * Fused Q/K/V projection of the active heads, with the quantisation the
  * attention kernel reads. Replaces, per layer of the cascade:
  *   slice_linear_weights (module.py:12-34): index_select of the active heads'

@@ -121,6 +121,38 @@ class PagedReadArgs(ctypes.Structure):
     ]
 
 
+class PagedTreeArgs(ctypes.Structure):
+    """Mirror of spatten_paged_tree_args (include/spatten_b200.h)."""
+    _fields_ = [
+        ("B", c_int), ("T", c_int), ("max_tokens", c_int), ("cu_tokens", c_vp), ("seq_lens", c_vp), ("parents", c_vp),
+        ("tree", c_vp), ("tree_stride", c_i64), ("tree_words", c_int), ("positions", c_vp),
+    ]
+
+
+class PagedAttendExtArgs(ctypes.Structure):
+    """Mirror of spatten_paged_attend_ext_args (include/spatten_b200.h)."""
+    _fields_ = [
+        ("attend", PagedAttendArgs), ("tree", c_vp), ("tree_stride", c_i64), ("tree_words", c_int),
+        ("weight", c_vp), ("position", c_vp), ("positions", c_vp),
+    ]
+
+
+class PagedEvictArgs(ctypes.Structure):
+    """Mirror of spatten_paged_evict_args (include/spatten_b200.h)."""
+    _fields_ = [
+        ("cache", PagedCache), ("B", c_int), ("seq_lens", c_vp), ("weight", c_vp), ("position", c_vp),
+        ("keep", c_int), ("recent", c_int), ("per_head", c_int), ("new_lens", c_vp),
+    ]
+
+
+class PagedKeepArgs(ctypes.Structure):
+    """Mirror of spatten_paged_keep_args (include/spatten_b200.h)."""
+    _fields_ = [
+        ("cache", PagedCache), ("B", c_int), ("cu_tokens", c_vp), ("seq_lens", c_vp), ("accepted", c_vp),
+        ("accepted_stride", c_i64), ("n_accepted", c_int), ("weight", c_vp), ("position", c_vp), ("new_lens", c_vp),
+    ]
+
+
 class CompactOutProjArgs(ctypes.Structure):
     """Mirror of spatten_compact_out_proj_args (include/spatten_b200.h)."""
     _fields_ = [
@@ -152,6 +184,12 @@ SIGNATURES = {
     "spatten_paged_attend_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(PagedAttendArgs)]),
     "spatten_paged_attend": (c_int, [ctypes.POINTER(PagedAttendArgs), c_vp, ctypes.c_size_t, c_vp]),
     "spatten_paged_read": (c_int, [ctypes.POINTER(PagedReadArgs), c_vp]),
+    "spatten_paged_tree": (c_int, [ctypes.POINTER(PagedTreeArgs), c_vp]),
+    "spatten_paged_attend_ext_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(PagedAttendExtArgs)]),
+    "spatten_paged_attend_ext": (c_int, [ctypes.POINTER(PagedAttendExtArgs), c_vp, ctypes.c_size_t, c_vp]),
+    "spatten_paged_evict_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(PagedEvictArgs)]),
+    "spatten_paged_evict": (c_int, [ctypes.POINTER(PagedEvictArgs), c_vp, ctypes.c_size_t, c_vp]),
+    "spatten_paged_keep": (c_int, [ctypes.POINTER(PagedKeepArgs), c_vp]),
     "spatten_qkv_proj": (c_int, [ctypes.POINTER(QkvProjArgs), c_vp]),
     "spatten_qk_norm_rope": (c_int, [ctypes.POINTER(QkNormRopeArgs), c_vp]),
     "spatten_compact_out_proj": (c_int, [ctypes.POINTER(CompactOutProjArgs), c_vp]),

@@ -578,6 +578,31 @@ static int check_out_rows(const char* who, const char* name, const void* x, int6
   return SPATTEN_OK;
 }
 
+// words of a tree's bits for the new tokens
+static int check_tree(const char* who, const void* tree, int64_t stride, int words, int T, int max_tokens) {
+  if (!tree || !aligned(tree, 4)) return fail(SPATTEN_ERR_INVALID, "%s: tree null or not 4-byte aligned", who);
+  if (words < 1 || (int64_t)words * 32 < max_tokens)
+    return fail(SPATTEN_ERR_INVALID, "%s: %d words of tree for %d tokens", who, words, max_tokens);
+  if (T > 1 && stride < 0) return fail(SPATTEN_ERR_INVALID, "%s: negative stride of tree", who);
+  return SPATTEN_OK;
+}
+
+// accumulated weights and positions: both or neither
+static int check_weights(const char* who, const float* weight, const int32_t* position) {
+  if (!weight != !position) return fail(SPATTEN_ERR_INVALID, "%s: one of weight, position", who);
+  if (!aligned(weight, 4) || !aligned(position, 4))
+    return fail(SPATTEN_ERR_INVALID, "%s: weight/position not 4-byte aligned", who);
+  return SPATTEN_OK;
+}
+
+static int check_workspace(const char* who, const void* ws, size_t bytes, size_t need) {
+  if (need == 0) return SPATTEN_OK;
+  if (!ws || bytes < need)
+    return fail(SPATTEN_ERR_INVALID, "%s: workspace of %zu bytes needed, %zu given", who, need, bytes);
+  if (!aligned(ws, 256)) return fail(SPATTEN_ERR_INVALID, "%s: workspace not 256-byte aligned", who);
+  return SPATTEN_OK;
+}
+
 int spatten_paged_append(const spatten_paged_append_args* a, void* stream) {
   static const char* who = "paged_append";
   if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
@@ -662,12 +687,8 @@ int spatten_paged_attend(const spatten_paged_attend_args* a, void* workspace, si
   if (p.b.B == 0 || p.b.max_tokens == 0) return ok();
   if (int e = check_rows(who, "q", a->q, a->q_st, a->q_sh)) return e;
   if (int e = check_out_rows(who, "out", a->out, a->o_st, a->o_sh, a->T, a->H, p.c.D)) return e;
-  const size_t need = align256(spatten::paged_attend_workspace(p, sm_count()));
-  if (need > 0) {
-    if (!workspace || workspace_bytes < need)
-      return fail(SPATTEN_ERR_INVALID, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
-    if (!aligned(workspace, 256)) return fail(SPATTEN_ERR_INVALID, "%s: workspace not 256-byte aligned", who);
-  }
+  if (int e = check_workspace(who, workspace, workspace_bytes, align256(spatten::paged_attend_workspace(p, sm_count()))))
+    return e;
   return cuda_status(spatten::launch_paged_attend(p, a->dtype, a->cache.kv_type, workspace, sm_count(),
                                                   (cudaStream_t)stream),
                      "paged_attend launch");
@@ -695,6 +716,134 @@ int spatten_paged_read(const spatten_paged_read_args* a, void* stream) {
   p.k_out = a->k_out; p.v_out = a->v_out;
   return cuda_status(spatten::launch_paged_read(p, a->dtype, a->cache.kv_type, (cudaStream_t)stream),
                      "paged_read launch");
+}
+
+int spatten_paged_tree(const spatten_paged_tree_args* a, void* stream) {
+  static const char* who = "paged_tree";
+  if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
+  spatten::PagedTreeParams p;
+  if (int e = fill_paged_batch(who, SPATTEN_DTYPE_F16, a->B, 1, a->T, a->max_tokens, a->cu_tokens, a->seq_lens, p.b))
+    return e;
+  if (p.b.B == 0 || p.b.max_tokens == 0) return ok();
+  if (p.b.max_tokens > spatten::kTreeTokens)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: trees of up to %d tokens (at most %d)", who, p.b.max_tokens,
+                spatten::kTreeTokens);
+  if (int e = check_tree(who, a->tree, a->tree_stride, a->tree_words, a->T, p.b.max_tokens)) return e;
+  if (a->T > 1 && a->tree_stride < a->tree_words)
+    return fail(SPATTEN_ERR_INVALID, "%s: rows of tree overlap", who);
+  if (!a->parents || !aligned(a->parents, 4) || !aligned(a->positions, 4))
+    return fail(SPATTEN_ERR_INVALID, "%s: null parents, or parents/positions not 4-byte aligned", who);
+  p.parents = a->parents;
+  p.tree = reinterpret_cast<uint32_t*>(a->tree); p.tree_st = a->tree_stride; p.words = a->tree_words;
+  p.positions = a->positions;
+  return cuda_status(spatten::launch_paged_tree(p, (cudaStream_t)stream), "paged_tree launch");
+}
+
+static int fill_paged_attend_ext(const spatten_paged_attend_ext_args* a, spatten::PagedWeighParams& p) {
+  static const char* who = "paged_attend_ext";
+  if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
+  if (int e = fill_paged_attend(&a->attend, p.a)) return e;
+  if (p.a.b.B == 0 || p.a.b.max_tokens == 0) return SPATTEN_OK;
+  if (a->tree) {
+    if (int e = check_tree(who, a->tree, a->tree_stride, a->tree_words, a->attend.T, p.a.b.max_tokens)) return e;
+    p.a.tree = reinterpret_cast<const uint32_t*>(a->tree);
+    p.a.tree_st = a->tree_stride; p.a.words = a->tree_words;
+  }
+  if (int e = check_weights(who, a->weight, a->position)) return e;
+  if (a->positions && (!a->weight || !aligned(a->positions, 4)))
+    return fail(SPATTEN_ERR_INVALID, "%s: positions without weight, or not 4-byte aligned", who);
+  p.weight = a->weight; p.position = a->position; p.positions = a->positions;
+  return SPATTEN_OK;
+}
+
+// the attention's part, and the rows' statistics
+static size_t attend_ext_part(const spatten::PagedWeighParams& p) {
+  return align256(spatten::paged_attend_workspace(p.a, sm_count()));
+}
+static size_t attend_ext_bytes(const spatten::PagedWeighParams& p) {
+  return attend_ext_part(p) + (p.weight ? align256((size_t)p.a.b.T * p.a.b.H * sizeof(float2)) : 0);
+}
+
+size_t spatten_paged_attend_ext_workspace_size(const spatten_paged_attend_ext_args* a) {
+  spatten::PagedWeighParams p;
+  if (fill_paged_attend_ext(a, p) != SPATTEN_OK || p.a.b.B == 0 || p.a.b.max_tokens == 0) return 0;
+  return attend_ext_bytes(p);
+}
+
+int spatten_paged_attend_ext(const spatten_paged_attend_ext_args* a, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  static const char* who = "paged_attend_ext";
+  spatten::PagedWeighParams p;
+  if (int e = fill_paged_attend_ext(a, p)) return e;
+  if (p.a.b.B == 0 || p.a.b.max_tokens == 0) return ok();
+  const spatten_paged_attend_args& t = a->attend;
+  if (int e = check_rows(who, "q", t.q, t.q_st, t.q_sh)) return e;
+  if (int e = check_out_rows(who, "out", t.out, t.o_st, t.o_sh, t.T, t.H, p.a.c.D)) return e;
+  if (int e = check_workspace(who, workspace, workspace_bytes, attend_ext_bytes(p))) return e;
+  if (p.weight) p.a.stat = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + attend_ext_part(p));
+  cudaError_t e = spatten::launch_paged_attend(p.a, t.dtype, t.cache.kv_type, workspace, sm_count(),
+                                               (cudaStream_t)stream);
+  if (e == cudaSuccess && p.weight)
+    e = spatten::launch_paged_weigh(p, t.dtype, t.cache.kv_type, (cudaStream_t)stream);
+  return cuda_status(e, "paged_attend_ext launch");
+}
+
+static int fill_paged_evict(const spatten_paged_evict_args* a, spatten::PagedEvictParams& p) {
+  static const char* who = "paged_evict";
+  if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
+  if (int e = fill_paged_cache(who, a->cache, a->B, true, p.c)) return e;
+  if (a->B < 0 || a->keep < 1 || a->recent < 0)
+    return fail(SPATTEN_ERR_INVALID, "%s: B=%d keep=%d recent=%d (need >= 0, >= 1, >= 0)", who, a->B, a->keep,
+                a->recent);
+  if (a->B > 65535) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: B=%d (at most 65535)", who, a->B);
+  if (p.c.G > 32767) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: %d KV heads", who, p.c.G);
+  if ((int64_t)p.c.max_pages * p.c.page > spatten::kEvictSlots)
+    return fail(SPATTEN_ERR_UNSUPPORTED, "%s: page table of %lld slots (at most %d)", who,
+                (long long)p.c.max_pages * p.c.page, spatten::kEvictSlots);
+  p.B = a->B; p.lens = a->seq_lens; p.weight = a->weight; p.position = a->position;
+  p.keep = a->keep; p.recent = a->recent; p.per_head = a->per_head != 0; p.new_lens = a->new_lens;
+  return SPATTEN_OK;
+}
+
+size_t spatten_paged_evict_workspace_size(const spatten_paged_evict_args* a) {
+  spatten::PagedEvictParams p;
+  if (fill_paged_evict(a, p) != SPATTEN_OK || p.B == 0) return 0;
+  return align256(spatten::paged_evict_workspace(p));
+}
+
+int spatten_paged_evict(const spatten_paged_evict_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  static const char* who = "paged_evict";
+  spatten::PagedEvictParams p;
+  if (int e = fill_paged_evict(a, p)) return e;
+  if (p.B == 0) return ok();
+  if (!p.weight) return fail(SPATTEN_ERR_INVALID, "%s: null weight", who);
+  if (int e = check_weights(who, p.weight, p.position)) return e;
+  if (!p.lens || !p.new_lens || !aligned(p.lens, 4) || !aligned(p.new_lens, 4))
+    return fail(SPATTEN_ERR_INVALID, "%s: null or misaligned seq_lens/new_lens", who);
+  if (int e = check_workspace(who, workspace, workspace_bytes, align256(spatten::paged_evict_workspace(p)))) return e;
+  return cuda_status(spatten::launch_paged_evict(p, a->cache.kv_type, workspace, sm_count(), (cudaStream_t)stream),
+                     "paged_evict launch");
+}
+
+int spatten_paged_keep(const spatten_paged_keep_args* a, void* stream) {
+  static const char* who = "paged_keep";
+  if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
+  spatten::PagedKeepParams p;
+  if (int e = fill_paged_cache(who, a->cache, a->B, true, p.c)) return e;
+  const int any = 1 << 30;  // rows: none are read
+  if (int e = fill_paged_batch(who, SPATTEN_DTYPE_F16, a->B, 0, any, any, a->cu_tokens, a->seq_lens, p.b)) return e;
+  if (a->n_accepted < 0) return fail(SPATTEN_ERR_INVALID, "%s: n_accepted=%d", who, a->n_accepted);
+  if (p.b.B == 0) return ok();
+  if (a->n_accepted > 0 && (!a->accepted || !aligned(a->accepted, 4) || a->accepted_stride < 0))
+    return fail(SPATTEN_ERR_INVALID, "%s: accepted null, misaligned or of a negative stride", who);
+  if (int e = check_weights(who, a->weight, a->position)) return e;
+  if (!a->new_lens || !aligned(a->new_lens, 4))
+    return fail(SPATTEN_ERR_INVALID, "%s: null or misaligned new_lens", who);
+  if (a->new_lens < a->seq_lens + a->B && a->seq_lens < a->new_lens + a->B)
+    return fail(SPATTEN_ERR_INVALID, "%s: new_lens overlaps seq_lens", who);
+  p.accepted = a->accepted; p.accepted_st = a->accepted_stride; p.A = a->n_accepted;
+  p.weight = a->weight; p.position = a->position; p.new_lens = a->new_lens;
+  return cuda_status(spatten::launch_paged_keep(p, a->cache.kv_type, (cudaStream_t)stream), "paged_keep launch");
 }
 
 }  // extern "C"

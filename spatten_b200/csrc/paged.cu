@@ -33,21 +33,6 @@ SPATTEN_DEV float max_abs_nan(float a, float x, float y) {
   return r;
 }
 
-// The scale that a block whose largest finite magnitude is `amax` needs.
-template <int KV>
-SPATTEN_DEV float scale_for(float amax) {
-  if constexpr (KV == kKvInt8) {
-    return div127_rn(amax);
-  } else {
-    if (amax == 0.f) return 0.f;
-    // amax = m 2^e, m in [1, 2): 448 = 1.75 * 2^8, so k = e - 8, or e - 7 for m > 1.75
-    const uint32_t u = __float_as_uint(amax);
-    const int e = (int)(u >> 23) - 127;  // -127 for subnormals, which the floor below covers
-    const int k = max(e - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0), -126);
-    return __uint_as_float((uint32_t)(k + 127) << 23);
-  }
-}
-
 // Eight finite values over the block's scale (not 0), as codes; rc = 1 / s.
 // int8: x rc (1 - 2^-20) and x rc (1 + 2^-20) enclose the rounded x / s, whose
 // rounding is theirs where they agree; where one of the eight disagrees (near a
@@ -85,25 +70,6 @@ SPATTEN_DEV uint2 encode8(const float2 (&x)[4], float s, float rc) {
     for (int j = 0; j < 2; ++j) {
       const float2 a = __fmul2_rn(x[2 * j], r2), b = __fmul2_rn(x[2 * j + 1], r2);
       w[j] = f32x2_to_e4m3x2(a.x, a.y) | (f32x2_to_e4m3x2(b.x, b.y) << 16);
-    }
-  }
-  return make_uint2(w[0], w[1]);
-}
-
-// Eight earlier codes under a grown scale: round(code * ratio).
-template <int KV>
-SPATTEN_DEV uint2 rescale8(uint2 c, float ratio) {
-  uint32_t w[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    float f[4];
-    codes4_to_f32<KV>(j ? c.y : c.x, f);
-    if constexpr (KV == kKvInt8) {
-      w[j] = 0u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[j] |= ((uint32_t)__float2int_rn(f[i] * ratio) & 0xFFu) << (8 * i);
-    } else {
-      w[j] = f32x2_to_e4m3x2(f[0] * ratio, f[1] * ratio) | (f32x2_to_e4m3x2(f[2] * ratio, f[3] * ratio) << 16);
     }
   }
   return make_uint2(w[0], w[1]);

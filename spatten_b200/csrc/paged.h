@@ -1,5 +1,7 @@
-// Paged 8-bit KV cache: append (paged.cu), read back (paged.cu) and attention
-// over it (paged_attend.cu).
+// Paged 8-bit KV cache: append (paged.cu), read back (paged.cu), attention over
+// it (paged_attend.cu, paged_attend_tc.cu), the weights that it gives the cached
+// tokens (paged_weigh.cu), trees of drafted tokens (paged_tree.cu), and tokens that
+// leave the cache (paged_evict.cu).
 #pragma once
 #include <cuda_runtime.h>
 #include <stddef.h>
@@ -60,6 +62,50 @@ struct PagedAttendParams {
   // the launch serves sequences with more than rows_over and at most rows_upto
   // query rows per KV head
   int64_t rows_over, rows_upto;
+  // beside the causal form:
+  const uint32_t* tree = nullptr;  // or null: bits of the new tokens that a row sees, [T, words]
+  int64_t tree_st = 0;
+  int words = 0;
+  float2* stat = nullptr;          // or null: [T, H] reference m of a row's exponentials, 1 / their sum
+};
+
+// The weights that a call's rows give the cached tokens (after the attention).
+struct PagedWeighParams {
+  PagedAttendParams a;      // its stat is read
+  float* weight;            // [P, G, page]
+  int32_t* position;        // [P, G, page]
+  const int32_t* positions; // or null: [T]
+};
+
+struct PagedTreeParams {
+  PagedBatch b;
+  const int32_t* parents;   // [T]
+  uint32_t* tree;           // [T, words]
+  int64_t tree_st;
+  int words;
+  int32_t* positions;       // or null: [T]
+};
+
+struct PagedEvictParams {
+  PagedCache c;
+  int B;
+  const int32_t* lens;
+  float* weight;
+  int32_t* position;
+  int keep, recent;
+  bool per_head;
+  int32_t* new_lens;
+};
+
+struct PagedKeepParams {
+  PagedCache c;
+  PagedBatch b;
+  const int32_t* accepted;  // [B, A], row stride accepted_st
+  int64_t accepted_st;
+  int A;
+  float* weight;            // or null
+  int32_t* position;
+  int32_t* new_lens;
 };
 
 struct PagedReadParams {
@@ -86,5 +132,12 @@ cudaError_t launch_paged_attend_tc(const PagedAttendParams& p, int dtype, int kv
 cudaError_t read_paged_device_error(unsigned int* code, bool reset);
 cudaError_t launch_paged_attend(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,
                                 cudaStream_t st);
+cudaError_t launch_paged_weigh(const PagedWeighParams& p, int dtype, int kv, cudaStream_t st);
+constexpr int kTreeTokens = 1024;  // new tokens of a sequence whose tree is laid out
+cudaError_t launch_paged_tree(const PagedTreeParams& p, cudaStream_t st);
+constexpr int kEvictSlots = 1 << 20;  // slots of a sequence that is chosen from
+size_t paged_evict_workspace(const PagedEvictParams& p);
+cudaError_t launch_paged_evict(const PagedEvictParams& p, int kv, void* ws, int n_sm, cudaStream_t st);
+cudaError_t launch_paged_keep(const PagedKeepParams& p, int kv, cudaStream_t st);
 
 }  // namespace spatten

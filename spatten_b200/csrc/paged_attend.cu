@@ -275,7 +275,8 @@ SPATTEN_DEV void read_v(uint32_t (&v)[D / 32], uint32_t blk, const LaneOffsets<D
   }
 }
 
-template <int KV, int D, int NB>
+// EXT: with a tree's masks or with the rows' statistics as results.
+template <int KV, int D, int NB, bool EXT>
 __global__ void __launch_bounds__(32 * kWarps, Shape<D, NB>::kCtas)
 paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf16) {
   using SH = Shape<D, NB>;
@@ -393,8 +394,9 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     const uint32_t t0 = few ? v0 * chunk : max(v0, lead) - lead, t1 = few ? min(KT, v1 * chunk) : max(v1, lead) - lead;
     const int nrows = sq.n * R, r0 = rt * ROWS;
     // slots that the tile's last and first row see
-    const int lim_max = min(sq.old + min((r0 + ROWS - 1) / R, sq.n - 1) + 1, sq.len);
-    const int lim_min = min(sq.old + r0 / R + 1, sq.len);
+    const bool tree = EXT && p.tree;
+    const int lim_max = min(sq.old + (tree ? sq.n : min((r0 + ROWS - 1) / R, sq.n - 1) + 1), sq.len);
+    const int lim_min = min(sq.old + (tree ? 0 : r0 / R + 1), sq.len);
     const uint32_t t_end = min(t1, (uint32_t)(max(lim_max, 0) + kKeys - 1) / kKeys);
 
     // queries: row gid of each 8-row block, all dims of it in the four lanes of gid
@@ -495,7 +497,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
 #pragma unroll
       for (int j = 0; j < 2; ++j) {  // this lane's rows of the products: 2 tig, 2 tig + 1
         cq[nb][j] = __shfl_sync(0xffffffffu, qs.factor, (2 * tig + j) * 4);
-        lim[nb][j] = min(sq.old + (r0 + nb * 8 + 2 * tig + j) / R + 1, sq.len);
+        lim[nb][j] = tree ? lim_max : min(sq.old + (r0 + nb * 8 + 2 * tig + j) / R + 1, sq.len);
         m[nb][j] = M[nb][j] = kNone;
         l[nb][j] = 0.f;
       }
@@ -537,6 +539,17 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               if (none || slot0 + gid + 4 * (i & 2) >= lim[nb][i & 1]) s[nb][i] = -INFINITY;
+          if (tree) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const int row = min(r0 + nb * 8 + 2 * tig + c, nrows - 1);
+                const uint32_t sees = tree_bits(p.tree + (sq.begin + row / R) * p.tree_st, p.words, slot0 - sq.old);
+                if (!((sees >> gid) & 1u)) s[nb][c] = -INFINITY;
+                if (!((sees >> (gid + 8)) & 1u)) s[nb][2 + c] = -INFINITY;
+              }
+          }
         }
         // p = 2^(s - m), and w = 2^(s + log2 v_scale - M)
         float top[NB][2], topw[NB][2];  // largest s, and s + log2 v_scale, of this lane
@@ -656,6 +669,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         v.x = bf16 ? pack2<__nv_bfloat16>(acc.x * inv, acc.y * inv) : pack2<__half>(acc.x * inv, acc.y * inv);
         v.y = bf16 ? pack2<__nv_bfloat16>(acc.z * inv, acc.w * inv) : pack2<__half>(acc.z * inv, acc.w * inv);
         *reinterpret_cast<uint2*>(op) = v;
+        if (EXT && p.stat && d == 0)
+          p.stat[(int64_t)(sq.begin + r / R) * p.b.H + g * R + r % R] = row_stat(mm, ll);
       } else {
         *reinterpret_cast<float4*>(ws.o + ((int64_t)slot * ROWS + row) * D + d) = acc;
         if (d == 0) ws.ml[(int64_t)slot * ROWS + row] = make_float4(mm, ll, MM, 0.f);
@@ -692,7 +707,7 @@ int grid_ctas(const PagedAttendParams& p, int n_sm) {
   return (int)fmin((double)wave, fmax(1.0, ceil(units_bound(p) / kWarps)));
 }
 
-template <int KV, int D, int NB>
+template <int KV, int D, int NB, bool EXT>
 cudaError_t attend_launch(const PagedAttendParams& p, bool bf16, const Workspace& ws, int ctas, cudaStream_t st) {
   using SH = Shape<D, NB>;
   const size_t smem = SH::kRing + (size_t)(p.b.B + 1) * sizeof(uint32_t);
@@ -701,20 +716,24 @@ cudaError_t attend_launch(const PagedAttendParams& p, bool bf16, const Workspace
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
-    e = cudaFuncSetAttribute(paged_attend_kernel<KV, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(paged_attend_kernel<KV, D, NB, EXT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              SH::kRing + (kMaxBatch + 1) * (int)sizeof(uint32_t));
     if (e != cudaSuccess) return e;
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  e = launch_dependent(paged_attend_kernel<KV, D, NB>, dim3(ctas), 32 * kWarps, smem, st, p, ws, bf16);
+  e = launch_dependent(paged_attend_kernel<KV, D, NB, EXT>, dim3(ctas), 32 * kWarps, smem, st, p, ws, bf16);
   if (e != cudaSuccess) return e;
   return launch_paged_join<D, SH::kRows>(p, ws, ctas, bf16, st);
 }
 
 template <int KV, int D>
 cudaError_t attend_rows(const PagedAttendParams& p, bool bf16, const Workspace& ws, int ctas, cudaStream_t st) {
-  return row_block(p) == 8 ? attend_launch<KV, D, 1>(p, bf16, ws, ctas, st)
-                           : attend_launch<KV, D, 2>(p, bf16, ws, ctas, st);
+  const bool ext = p.tree || p.stat;
+  if (row_block(p) == 8)
+    return ext ? attend_launch<KV, D, 1, true>(p, bf16, ws, ctas, st)
+               : attend_launch<KV, D, 1, false>(p, bf16, ws, ctas, st);
+  return ext ? attend_launch<KV, D, 2, true>(p, bf16, ws, ctas, st)
+             : attend_launch<KV, D, 2, false>(p, bf16, ws, ctas, st);
 }
 
 template <int KV>

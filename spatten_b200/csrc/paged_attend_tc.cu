@@ -130,6 +130,7 @@ struct Segments {
   const uint32_t* pre;
   uint32_t u, u1;
   int b, R;
+  bool tree;  // every row may see all new tokens (its line counts as in the causal form)
   // the current segment
   PagedSeq sq;
   int g, r0, nrows, lim_max, t0, t1;
@@ -169,7 +170,7 @@ struct Segments {
     whole = first && v1 == line;
     r0 = lo * kRowsCta;
     nrows = sq.n * R;
-    lim_max = max(min(sq.old + min((r0 + kRowsCta - 1) / R, sq.n - 1) + 1, sq.len), 0);
+    lim_max = max(min(sq.old + (tree ? sq.n : min((r0 + kRowsCta - 1) / R, sq.n - 1) + 1), sq.len), 0);
     const int kt = (lim_max + kKeys - 1) / kKeys;
     t0 = min(tile(v0), kt);
     t1 = v1 == line ? kt : min(tile(v1), kt);
@@ -178,7 +179,8 @@ struct Segments {
   }
 };
 
-template <int KV, int D>
+// EXT: with a tree's masks or with the rows' statistics as results.
+template <int KV, int D, bool EXT>
 __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const PagedAttendParams p, const PagedPartials ws,
                                                                       const bool bf16) {
   using L = Lay<D>;
@@ -252,6 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
   const uint32_t per = U / ctas, more = U % ctas;
   Segments seg{p, pre};
   seg.R = R;
+  seg.tree = EXT && p.tree;
   seg.b = 0;
   seg.u = seg.u1 = 0;
   if (cta < ctas) {
@@ -320,7 +323,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         __syncwarp();
         mbar_arrive_elect(q_full[rt]);
       }
-      const int lim = live ? min(seg.sq.old + i + 1, seg.sq.len) : 0;
+      const bool tree = EXT && p.tree;
+      const int lim = live ? (tree ? seg.lim_max : min(seg.sq.old + i + 1, seg.sq.len)) : 0;
+      const int all = tree ? min(lim, seg.sq.old) : lim;  // slots that the row sees whatever its mask
       float m = -INFINITY, M = -INFINITY, l = 0.f;
       if (!used) kv += max(nt, 0);
       for (int t = seg.t0; used && t < seg.t1; ++t, ++kv) {
@@ -339,12 +344,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         float a[4] = {cq * ks.x, cq * ks.y, cq * ks.z, cq * ks.w};
         const float lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w};
         const int key0 = t * kKeys;
-        const bool odd = key0 + kKeys > lim || have != 15u || !(fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) >= 0.f);
+        const bool odd = key0 + kKeys > all || have != 15u || !(fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) >= 0.f);
         if (__builtin_expect(__any_sync(0xffffffffu, odd), 0)) {  // masked keys, factors below 0 or NaN: t itself
 #pragma unroll
           for (int k = 0; k < kKeys; ++k) {
             s[k] *= a[k >> 4];
             if (key0 + k >= lim || !((have >> (k >> 4)) & 1u)) s[k] = -INFINITY;
+          }
+          if (tree && live) {
+            const uint32_t* words = p.tree + (seg.sq.begin + i) * p.tree_st;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t sees = tree_bits(words, p.words, key0 + 32 * h - seg.sq.old);
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (!((sees >> k) & 1u)) s[32 * h + k] = -INFINITY;
+            }
           }
           a[0] = a[1] = a[2] = a[3] = 1.f;
         }
@@ -462,6 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
                   make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
           }
         }
+        if (EXT && p.stat && live && seg.whole) p.stat[(int64_t)(seg.sq.begin + i) * p.b.H + h] = row_stat(m, l);
         if (live && !seg.whole) ws.ml[slot * kRowsCta + rt * kRowTile + row] = make_float4(m, l, M, 0.f);
         tc_fence_before();
       }
@@ -679,6 +695,7 @@ __global__ void __launch_bounds__(32 * (D / 16)) paged_join_rows_kernel(const Pa
     M = Mn;
   }
   const float inv = paged_normaliser(m, l, M);
+  if (p.stat && dim == 0) p.stat[(int64_t)(cut.begin + r / R) * p.b.H + cut.g * R + r % R] = row_stat(m, l);
   uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(cut.begin + r / R) * p.o_st +
                  (int64_t)(cut.g * R + r % R) * p.o_sh + 16 * dim;
 #pragma unroll
@@ -692,27 +709,33 @@ __global__ void __launch_bounds__(32 * (D / 16)) paged_join_rows_kernel(const Pa
   }
 }
 
-template <int KV, int D>
-cudaError_t tc_launch(const PagedAttendParams& p, bool bf16, const PagedPartials& ws, int ctas, cudaStream_t st) {
+template <int KV, int D, bool EXT>
+cudaError_t tc_launch_as(const PagedAttendParams& p, bool bf16, const PagedPartials& ws, int ctas, cudaStream_t st) {
   static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
-    e = cudaFuncSetAttribute(paged_attend_tc_kernel<KV, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(paged_attend_tc_kernel<KV, D, EXT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              Lay<D>::bytes(kMaxBatch));
     if (e != cudaSuccess) return e;
     // the split of the registers holds for this launch allocation only: setmaxnreg.inc would wait for
     // registers that the block does not hold
     cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, paged_attend_tc_kernel<KV, D>);
+    e = cudaFuncGetAttributes(&fa, paged_attend_tc_kernel<KV, D, EXT>);
     if (e != cudaSuccess) return e;
     if ((fa.numRegs + 7) / 8 * 8 != kRegs) return cudaErrorInvalidConfiguration;
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  e = launch_dependent(paged_attend_tc_kernel<KV, D>, dim3(ctas), kThreads, Lay<D>::bytes(p.b.B), st, p, ws, bf16);
+  e = launch_dependent(paged_attend_tc_kernel<KV, D, EXT>, dim3(ctas), kThreads, Lay<D>::bytes(p.b.B), st, p, ws, bf16);
   if (e != cudaSuccess) return e;
   return launch_dependent(paged_join_rows_kernel<D>, dim3(ctas, kRowsCta / 32), 32 * (D / 16), 0, st, p, ws, bf16);
+}
+
+template <int KV, int D>
+cudaError_t tc_launch(const PagedAttendParams& p, bool bf16, const PagedPartials& ws, int ctas, cudaStream_t st) {
+  return p.tree || p.stat ? tc_launch_as<KV, D, true>(p, bf16, ws, ctas, st)
+                          : tc_launch_as<KV, D, false>(p, bf16, ws, ctas, st);
 }
 
 }  // namespace

@@ -67,6 +67,19 @@ SPATTEN_DEV int paged_page(const PagedCache& c, int b, int pi) {
   return (pid >= 0 && pid < c.P) ? pid : -1;
 }
 
+// Bits j0 .. j0 + 31 of a row's words: whether the row sees the new tokens j0, ..;
+// those before 0 are cached tokens, which every row sees.
+SPATTEN_DEV uint32_t tree_bits(const uint32_t* w, int words, int j0) {
+  const int i = j0 >> 5;
+  auto word = [&](int k) { return k < 0 ? 0xFFFFFFFFu : k < words ? *(w + k) : 0u; };
+  return __funnelshift_r(word(i), word(i + 1), j0 & 31);
+}
+
+// The statistics of a finished row, for the weights it gave: w = 2^(s - x) y.
+SPATTEN_DEV float2 row_stat(float m, float l) {
+  return make_float2(m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.f / l);
+}
+
 // Two e4m3 codes (low byte first) as f16x2; every e4m3 value is an f16.
 SPATTEN_DEV uint32_t e4m3x2_to_f16x2(uint32_t two) {
   uint32_t r;
@@ -81,6 +94,21 @@ SPATTEN_DEV uint32_t f32x2_to_e4m3x2(float lo, float hi) {
   return r;
 }
 
+// The scale that a block whose largest finite magnitude is `amax` needs.
+template <int KV>
+SPATTEN_DEV float scale_for(float amax) {
+  if constexpr (KV == kKvInt8) {
+    return div127_rn(amax);
+  } else {
+    if (amax == 0.f) return 0.f;
+    // amax = m 2^e, m in [1, 2): 448 = 1.75 * 2^8, so k = e - 8, or e - 7 for m > 1.75
+    const uint32_t u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 127;  // -127 for subnormals, which the floor below covers
+    const int k = max(e - 8 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0), -126);
+    return __uint_as_float((uint32_t)(k + 127) << 23);
+  }
+}
+
 // Four codes (a 32-bit word, lowest byte first) as floats.
 template <int KV>
 SPATTEN_DEV void codes4_to_f32(uint32_t w, float (&f)[4]) {
@@ -93,6 +121,25 @@ SPATTEN_DEV void codes4_to_f32(uint32_t w, float (&f)[4]) {
     const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
     f[0] = x.x; f[1] = x.y; f[2] = y.x; f[3] = y.y;
   }
+}
+
+// Eight earlier codes under a grown scale: round(code * ratio).
+template <int KV>
+SPATTEN_DEV uint2 rescale8(uint2 c, float ratio) {
+  uint32_t w[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    float f[4];
+    codes4_to_f32<KV>(j ? c.y : c.x, f);
+    if constexpr (KV == kKvInt8) {
+      w[j] = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[j] |= ((uint32_t)__float2int_rn(f[i] * ratio) & 0xFFu) << (8 * i);
+    } else {
+      w[j] = f32x2_to_e4m3x2(f[0] * ratio, f[1] * ratio) | (f32x2_to_e4m3x2(f[2] * ratio, f[3] * ratio) << 16);
+    }
+  }
+  return make_uint2(w[0], w[1]);
 }
 
 // A query row as f16 for the product with the codes, times the power of two that

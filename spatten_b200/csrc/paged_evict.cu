@@ -1,0 +1,689 @@
+// Tokens that leave the paged 8-bit KV cache: eviction by accumulated attention
+// weight (spatten_paged_evict), and the rejected ones among drafted tokens
+// (spatten_paged_keep).
+//
+// Eviction. A sequence of more than `keep` slots keeps the tokens of the `recent`
+// newest positions, then those of the largest weight, ties to the lower slot. Its
+// kept tokens in slots behind `keep` move into the free slots before it, both in
+// ascending order. Nothing else moves: what is read (slots from `keep` on) and what is
+// written (slots before) are apart, so every written block is a CTA of its own, and
+// a token is rounded again only when it moves. Two launches:
+//
+// paged_select_kernel: a cluster of CTAs per sequence (or per sequence and KV head),
+// each holding the ordered keys of a run of slots in shared memory. The keep-th
+// largest key by radix rounds of 11 bits, whose histograms are summed over the
+// cluster; then the kept, the free and the moving slots as bits, a word per 32 slots,
+// whose prefix sums number them.
+//
+// paged_move_kernel: a CTA per block (page, KV head, K or V) of the first `keep`
+// slots. A token's codes under the block's scale S' are round(code * S / S') with S'
+// the larger of the block's scale (0 where it keeps nothing) and the one that the
+// largest moved magnitude needs; where S' grew, the kept codes are rounded likewise, as
+// appending does.
+#include <atomic>
+#include <cooperative_groups.h>
+
+#include "kernels.h"
+#include "paged_dev.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace spatten {
+namespace {
+
+constexpr float kMaxFinite = 3.402823466e38f;
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
+
+// ---------------------------------------------------------------- moving rows
+
+template <int D, int PAGE>
+struct MoveShape {
+  static constexpr int LPR = D / 16;                                 // lanes per row
+  static constexpr int NT = PAGE * LPR < 256 ? PAGE * LPR : 256;     // threads
+  static constexpr int RPP = NT / LPR;                               // rows per pass
+  static constexpr int PASSES = PAGE / RPP;                          // at most 4
+};
+
+// The rows of one block that tokens move into.
+template <int PAGE>
+struct MoveRows {
+  uint32_t src[PAGE];  // row of the pool, kNoRow: none
+  float scale[PAGE];   // its scale
+  uint32_t red[8];
+};
+
+template <int KV>
+SPATTEN_DEV float row_amax(uint4 c) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float f[4];
+    codes4_to_f32<KV>(w[i], f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(f[e]));
+  }
+  return m;
+}
+
+template <int KV>
+SPATTEN_DEV uint4 rescale16(uint4 c, float ratio) {
+  const uint2 a = rescale8<KV>(make_uint2(c.x, c.y), ratio), b = rescale8<KV>(make_uint2(c.z, c.w), ratio);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+// Moves m's rows into the block at `dst` (the rows before `end` that get none keep
+// their tokens, if `kept` says that there are any). All threads of the CTA; every
+// source is read before anything is written.
+template <int KV, int D, int PAGE>
+SPATTEN_DEV void move_block(MoveRows<PAGE>& m, const uint8_t* pool, uint8_t* dst, float* sp, float s_was, bool kept,
+                            int end) {
+  using S = MoveShape<D, PAGE>;
+  const int tid = threadIdx.x, lane = tid & 31, li = tid % S::LPR, rt = tid / S::LPR;
+  uint4 c[S::PASSES];
+  float amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < S::PASSES; ++j) {
+    const uint32_t row = m.src[j * S::RPP + rt];
+    c[j] = make_uint4(0u, 0u, 0u, 0u);
+    if (row != kNoRow) c[j] = *reinterpret_cast<const uint4*>(pool + (uint64_t)row * D + li * 16);
+  }
+#pragma unroll
+  for (int j = 0; j < S::PASSES; ++j) {
+    const int r = j * S::RPP + rt;
+    if (m.src[r] != kNoRow) amax = fmaxf(amax, fminf(row_amax<KV>(c[j]) * m.scale[r], kMaxFinite));
+  }
+  const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));  // magnitudes order as integers
+  if (lane == 0) m.red[tid >> 5] = top;
+  __syncthreads();
+  uint32_t all = 0u;
+#pragma unroll
+  for (int w = 0; w < S::NT / 32; ++w) all = max(all, m.red[w]);
+  const float s_old = kept ? s_was : 0.f, s = fmaxf(s_old, scale_for<KV>(__uint_as_float(all)));
+#pragma unroll
+  for (int j = 0; j < S::PASSES; ++j) {
+    const int r = j * S::RPP + rt;
+    uint4* to = reinterpret_cast<uint4*>(dst + r * D + li * 16);
+    if (m.src[r] != kNoRow) {
+      const float was = m.scale[r];
+      *to = s == was ? c[j] : s > 0.f ? rescale16<KV>(c[j], __fdiv_rn(was, s)) : make_uint4(0u, 0u, 0u, 0u);
+    } else if (r < end && s > s_old && kept) {
+      *to = rescale16<KV>(*to, __fdiv_rn(s_old, s));
+    }
+  }
+  if (tid == 0) *sp = s;
+}
+
+// ---------------------------------------------------------------- eviction
+
+// What the selection leaves for the moves, per sequence (and KV head): `moves`
+// tokens, the i-th from slot src[i] to slot dst[i]; first[j]: moves into blocks before j.
+struct EvictPlan {
+  int32_t* head;    // [lines][4]: moves, new length
+  int32_t* first;   // [lines][blocks + 1]
+  int32_t* dst;     // [lines][cap]
+  int32_t* src;     // [lines][cap]
+  float* edge;      // [B][G][2]: scales of the block of slot `keep` before the moves
+  int lines_per_b, blocks, cap;
+};
+
+constexpr int kSelThreads = 512, kBins = 2048;
+constexpr int kMaxKeys = 40960;  // of a CTA in shared memory; the others are read again
+
+struct SelShared {
+  uint32_t hist[2][kBins];
+  uint32_t scan[kSelThreads / 32 + 1];
+  uint32_t red[kSelThreads / 32][8];
+  uint32_t xch[8][8];   // what the cluster's other CTAs read, one row per exchange
+  uint32_t at[3];
+};
+
+// Sum over the CTA's threads before this one, and the sum of all.
+SPATTEN_DEV uint32_t block_scan(SelShared& sh, uint32_t x, uint32_t& total) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t y = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
+  }
+  __syncthreads();
+  if (lane == 31) sh.scan[warp] = y;
+  __syncthreads();
+  uint32_t before = 0u;
+  total = 0u;
+#pragma unroll
+  for (int w = 0; w < kSelThreads / 32; ++w) {
+    if (w < warp) before += sh.scan[w];
+    total += sh.scan[w];
+  }
+  return before + y - x;
+}
+
+// The lowest m bits that are set in t.
+SPATTEN_DEV uint32_t lowest_bits(uint32_t t, uint32_t m) {
+  while ((uint32_t)__popc(t) > m) t ^= 1u << (31 - __clz(t));
+  return t;
+}
+
+__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEvictParams p, const EvictPlan plan,
+                                                                   int run, int cached) {
+  extern __shared__ __align__(16) uint8_t dsm[];
+  SelShared& sh = *reinterpret_cast<SelShared*>(dsm);
+  uint32_t* keys = reinterpret_cast<uint32_t*>(dsm + sizeof(SelShared));  // [cached]
+  uint32_t* prot = keys + cached;                                          // [run / 32]: recent
+  uint32_t* kept = prot + run / 32;                                        // [run / 32]
+  uint32_t* ties = kept + run / 32;                                        // [run / 32]
+  grid_dependents();
+  grid_wait();
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = (int)cl.block_rank(), CL = (int)cl.num_blocks();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.z, hl = blockIdx.y;
+  const int G = p.c.G, page = p.c.page, page_log = __ffs(page) - 1, keep = p.keep;
+  const int64_t line = (int64_t)b * plan.lines_per_b + hl;
+  const int len = *(p.lens + b);
+  int32_t* const head = plan.head + line * 4;
+  if (len <= keep || (int64_t)len > (int64_t)p.c.max_pages * page) {  // (the same for the whole cluster)
+    if (rank == 0 && tid == 0) {
+      head[0] = 0;
+      head[1] = len;
+    }
+    return;
+  }
+  const int lo = min(rank * run, len), n = min(run, len - lo), words = (n + 31) / 32;
+
+  auto row_of = [&](int slot) {  // -1: no memory
+    const int pid = paged_page(p.c, b, slot >> page_log);
+    return pid < 0 ? (int64_t)-1 : ((int64_t)pid * G + hl) * page + (slot & (page - 1));
+  };
+  auto load_key = [&](int i) -> uint32_t {  // weights order as integers; negative ones and NaN count as 0
+    const int64_t row = row_of(lo + i);
+    if (row < 0) return 0u;
+    float w;
+    if (p.per_head) {
+      w = p.weight[row];
+    } else {
+      double sum = 0.0;
+      for (int g = 0; g < G; ++g) sum += (double)p.weight[row + (int64_t)g * page];
+      w = (float)sum;
+    }
+    return w > 0.f ? __float_as_uint(w) : 0u;
+  };
+  auto key = [&](int i) { return i < cached ? keys[i] : load_key(i); };
+
+  // keys, the newest position, whether every slot has memory
+  int newest = INT_MIN;
+  bool hole = false;
+  for (int i = tid; i < n; i += kSelThreads) {
+    const int64_t row = row_of(lo + i);
+    hole |= row < 0;
+    if (p.recent > 0 && row >= 0) newest = max(newest, p.position[row]);
+    if (i < cached) keys[i] = load_key(i);
+  }
+  {
+    const int top = __reduce_max_sync(0xffffffffu, newest);
+    const bool any = __any_sync(0xffffffffu, hole);
+    if (lane == 0) {
+      sh.red[warp][0] = (uint32_t)top;
+      sh.red[warp][1] = any;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int m = INT_MIN;
+      uint32_t h = 0u;
+      for (int w = 0; w < kSelThreads / 32; ++w) {
+        m = max(m, (int)sh.red[w][0]);
+        h |= sh.red[w][1];
+      }
+      sh.xch[0][0] = (uint32_t)m;
+      sh.xch[0][1] = h;
+    }
+    cl.sync();
+    uint32_t h = 0u;
+    newest = INT_MIN;
+    for (int r = 0; r < CL; ++r) {
+      const uint32_t* x = cl.map_shared_rank(&sh.xch[0][0], r);
+      newest = max(newest, (int)x[0]);
+      h |= x[1];
+    }
+    if (h) {  // left as it is
+      if (rank == 0 && tid == 0) {
+        head[0] = 0;
+        head[1] = len;
+      }
+      cl.sync();
+      return;
+    }
+  }
+  // the recent ones; how many they are, and the range of the keys of both classes
+  {
+    uint32_t cnt = 0u, lo0 = 0xFFFFFFFFu, hi0 = 0u, lo1 = 0xFFFFFFFFu, hi1 = 0u;
+    for (int base = 0; base < words * 32; base += kSelThreads) {
+      const int i = base + tid;
+      bool r = false;
+      if (i < n) {
+        if (p.recent > 0) r = (int64_t)p.position[row_of(lo + i)] > (int64_t)newest - p.recent;
+        const uint32_t k = key(i);
+        if (r) {
+          lo1 = min(lo1, k);
+          hi1 = max(hi1, k);
+        } else {
+          lo0 = min(lo0, k);
+          hi0 = max(hi0, k);
+        }
+      }
+      const uint32_t m = __ballot_sync(0xffffffffu, r);
+      if (lane == 0 && i < words * 32) {
+        prot[i >> 5] = m;
+        cnt += __popc(m);
+      }
+    }
+    lo0 = __reduce_min_sync(0xffffffffu, lo0);
+    hi0 = __reduce_max_sync(0xffffffffu, hi0);
+    lo1 = __reduce_min_sync(0xffffffffu, lo1);
+    hi1 = __reduce_max_sync(0xffffffffu, hi1);
+    if (lane == 0) {
+      sh.red[warp][0] = cnt;
+      sh.red[warp][1] = lo0;
+      sh.red[warp][2] = hi0;
+      sh.red[warp][3] = lo1;
+      sh.red[warp][4] = hi1;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      uint32_t x[5] = {0u, 0xFFFFFFFFu, 0u, 0xFFFFFFFFu, 0u};
+      for (int w = 0; w < kSelThreads / 32; ++w) {
+        x[0] += sh.red[w][0];
+        x[1] = min(x[1], sh.red[w][1]);
+        x[2] = max(x[2], sh.red[w][2]);
+        x[3] = min(x[3], sh.red[w][3]);
+        x[4] = max(x[4], sh.red[w][4]);
+      }
+      for (int i = 0; i < 5; ++i) sh.xch[1][i] = x[i];
+    }
+    cl.sync();
+  }
+  uint32_t recents = 0u, k_lo = 0xFFFFFFFFu, k_hi = 0u;
+  for (int r = 0; r < CL; ++r) recents += cl.map_shared_rank(&sh.xch[1][0], r)[0];
+  const bool cls = recents >= (uint32_t)keep;  // the class that is chosen from: the recent ones, or the others
+  for (int r = 0; r < CL; ++r) {
+    const uint32_t* x = cl.map_shared_rank(&sh.xch[1][0], r);
+    k_lo = min(k_lo, x[cls ? 3 : 1]);
+    k_hi = max(k_hi, x[cls ? 4 : 2]);
+  }
+  uint32_t need = cls ? keep : keep - recents;  // of the class; its largest keys
+  // radix rounds: keys above k_hi are kept, the need-th largest lies in [k_lo, k_hi]
+  bool whole = false, every = false;  // no ties: the class's keys above k_hi are kept; all of its keys are
+  for (int round = 0; !whole; ++round) {
+    const uint32_t span = k_hi - k_lo;
+    const int shift = span < (uint32_t)kBins ? 0 : 32 - __clz(span) - 11;
+    uint32_t* hist = sh.hist[round & 1];
+    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0u;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSelThreads) {
+      const uint32_t k = key(i);
+      if (((prot[i >> 5] >> (i & 31)) & 1u) == (uint32_t)cls && k >= k_lo && k <= k_hi) atomicAdd(&hist[(k - k_lo) >> shift], 1u);
+    }
+    cl.sync();
+    // bins from the top: thread t takes the bins kBins - 1 - 4 t ..
+    constexpr int PER = kBins / kSelThreads;
+    uint32_t c[PER], mine = 0u;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      c[j] = 0u;
+      for (int r = 0; r < CL; ++r) c[j] += cl.map_shared_rank(hist, r)[kBins - 1 - (tid * PER + j)];
+      mine += c[j];
+    }
+    uint32_t total;
+    uint32_t above = block_scan(sh, mine, total);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (above < need && need <= above + c[j]) {
+        sh.at[0] = kBins - 1 - (tid * PER + j);
+        sh.at[1] = above;
+        sh.at[2] = c[j];
+      }
+      above += c[j];
+    }
+    __syncthreads();
+    const uint32_t bin = sh.at[0], in = sh.at[2];
+    need -= sh.at[1];
+    const uint32_t b_lo = k_lo + (bin << shift);
+    const uint32_t b_hi = min(k_hi, b_lo + ((1u << shift) - 1u));
+    __syncthreads();  // sh.at is read
+    if (need == in) {  // all of the bin are kept
+      whole = true;
+      every = b_lo == 0u;
+      k_hi = b_lo - 1u;
+    } else {
+      k_lo = b_lo;
+      k_hi = b_hi;
+      if (shift == 0) break;  // one key: `need` of those that have it
+    }
+  }
+  // kept for sure, and the ones of the border's key
+  uint32_t n_ties = 0u;
+  for (int base = 0; base < words * 32; base += kSelThreads) {
+    const int i = base + tid;
+    bool sure = false, tie = false;
+    if (i < n) {
+      const bool mine = ((prot[i >> 5] >> (i & 31)) & 1u) == (uint32_t)cls;
+      const uint32_t k = key(i);
+      sure = mine ? every || k > k_hi : !cls;  // (chosen among the others: all recent ones stay)
+      tie = mine && !whole && k == k_hi;
+    }
+    const uint32_t ms = __ballot_sync(0xffffffffu, sure), mt = __ballot_sync(0xffffffffu, tie);
+    if (lane == 0 && i < words * 32) {
+      kept[i >> 5] = ms;
+      ties[i >> 5] = mt;
+      n_ties += __popc(mt);
+    }
+  }
+  {
+    uint32_t total;
+    block_scan(sh, n_ties, total);
+    if (tid == 0) sh.xch[2][0] = total;
+    cl.sync();
+  }
+  uint32_t before = 0u;
+  for (int r = 0; r < rank; ++r) before += cl.map_shared_rank(&sh.xch[2][0], r)[0];
+  uint32_t left = whole || before >= need ? 0u : need - before;  // ties that this CTA's slots may still keep
+  uint32_t n_dst = 0u, n_src = 0u;
+  for (int base = 0; base < words; base += kSelThreads) {
+    const int w = base + tid;
+    const uint32_t t = w < words ? ties[w] : 0u;
+    uint32_t total;
+    const uint32_t at = block_scan(sh, __popc(t), total);
+    if (w < words) {
+      const uint32_t k = kept[w] | (at < left ? lowest_bits(t, left - at) : 0u);
+      kept[w] = k;
+      const int s0 = lo + 32 * w;  // slots before `keep` of the word
+      const uint32_t front = s0 + 32 <= keep ? 0xFFFFFFFFu : s0 >= keep ? 0u : (1u << (keep - s0)) - 1u;
+      n_dst += __popc(front & ~k);
+      n_src += __popc(k & ~front);
+    }
+    left -= min(left, total);
+  }
+  {
+    uint32_t td, ts;
+    block_scan(sh, n_dst, td);
+    block_scan(sh, n_src, ts);
+    if (tid == 0) {
+      sh.xch[3][0] = td;
+      sh.xch[3][1] = ts;
+    }
+    cl.sync();
+  }
+  uint32_t d0 = 0u, s0 = 0u, moves = 0u;
+  for (int r = 0; r < CL; ++r) {
+    const uint32_t* x = cl.map_shared_rank(&sh.xch[3][0], r);
+    if (r < rank) {
+      d0 += x[0];
+      s0 += x[1];
+    }
+    moves += x[0];
+  }
+  int32_t* const dst = plan.dst + line * plan.cap;
+  int32_t* const src = plan.src + line * plan.cap;
+  int32_t* const first = plan.first + line * (plan.blocks + 1);
+  for (int base = 0; base < words; base += kSelThreads) {
+    const int w = base + tid;
+    const int at = lo + 32 * w;
+    const uint32_t k = w < words ? kept[w] : 0u;
+    const uint32_t front = w >= words || at >= keep ? 0u : at + 32 <= keep ? 0xFFFFFFFFu : (1u << (keep - at)) - 1u;
+    uint32_t free = front & ~k, move = w < words ? k & ~front : 0u, td, ts;
+    uint32_t d = d0 + block_scan(sh, __popc(free), td), s = s0 + block_scan(sh, __popc(move), ts);
+    d0 += td;
+    s0 += ts;
+    if (front)
+      for (int o = 0; o < 32; o += 16)  // (pages are multiples of 16)
+        if (((at + o) & (page - 1)) == 0 && at + o < keep) first[(at + o) >> page_log] = d + __popc(free & ((1u << o) - 1u));
+    for (; free; free &= free - 1u) dst[d++] = at + __ffs(free) - 1;
+    for (; move; move &= move - 1u) src[s++] = at + __ffs(move) - 1;
+  }
+  if (rank == 0) {
+    if (tid == 0) {
+      head[0] = (int)moves;
+      head[1] = keep;
+      first[plan.blocks] = (int)moves;
+    }
+    // the block of slot `keep` may change its scale while others read its tokens
+    const int g0 = p.per_head ? hl : 0, g1 = p.per_head ? hl + 1 : G;
+    for (int g = g0 + tid; g < g1; g += kSelThreads) {
+      const int64_t blk = (int64_t)paged_page(p.c, b, keep >> page_log) * G + g;
+      float* e = plan.edge + ((int64_t)b * G + g) * 2;
+      e[0] = p.c.k_scale[blk];
+      e[1] = p.c.v_scale[blk];
+    }
+  }
+  cl.sync();  // no CTA leaves while its shared memory is read
+}
+
+template <int KV, int D, int PAGE>
+__global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_move_kernel(const PagedEvictParams p,
+                                                                           const EvictPlan plan) {
+  using S = MoveShape<D, PAGE>;
+  __shared__ MoveRows<PAGE> m;
+  grid_dependents();
+  grid_wait();
+  const int b = blockIdx.z, G = p.c.G, tid = threadIdx.x, blk = blockIdx.x;
+  const bool isk = (int)blockIdx.y < G;
+  const int g = isk ? blockIdx.y : blockIdx.y - G;
+  const int64_t line = (int64_t)b * plan.lines_per_b + (p.per_head ? g : 0);
+  if (blk == 0 && blockIdx.y == 0 && tid == 0) p.new_lens[b] = plan.head[line * 4 + 1];
+  if (plan.head[line * 4] == 0) return;
+  const int32_t* first = plan.first + line * (plan.blocks + 1);
+  const int f0 = first[blk], f1 = first[blk + 1];
+  if (f1 <= f0) return;
+  const int end = min(p.keep - blk * PAGE, PAGE), edge = p.keep / PAGE;
+  const float edge_scale = plan.edge[((int64_t)b * G + g) * 2 + (isk ? 0 : 1)];
+  float* const scales = isk ? p.c.k_scale : p.c.v_scale;
+  uint8_t* const pool = isk ? p.c.k : p.c.v;
+  for (int r = tid; r < PAGE; r += S::NT) m.src[r] = kNoRow;
+  __syncthreads();
+  const int64_t to = (int64_t)paged_page(p.c, b, blk) * G + g;
+  for (int i = f0 + tid; i < f1; i += S::NT) {
+    const int d = plan.dst[line * plan.cap + i] - blk * PAGE, s = plan.src[line * plan.cap + i];
+    const int64_t from = (int64_t)paged_page(p.c, b, s / PAGE) * G + g, row = from * PAGE + s % PAGE;
+    m.src[d] = (uint32_t)row;
+    m.scale[d] = s / PAGE == edge ? edge_scale : scales[from];
+    if (isk) {
+      p.weight[to * PAGE + d] = p.weight[row];
+      p.position[to * PAGE + d] = p.position[row];
+    }
+  }
+  const float was = blk == edge ? edge_scale : scales[to];
+  __syncthreads();
+  move_block<KV, D, PAGE>(m, pool, pool + to * (PAGE * D), scales + to, was, f1 - f0 < end, end);
+}
+
+// ---------------------------------------------------------------- accepted tokens
+
+// A CTA per (K or V head, sequence) walks the blocks that accepted tokens move into, in
+// order: what it reads lies at or behind what it writes.
+template <int KV, int D, int PAGE>
+__global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_keep_kernel(const PagedKeepParams p) {
+  using S = MoveShape<D, PAGE>;
+  __shared__ MoveRows<PAGE> m;
+  __shared__ int stop, moved, fixed;
+  grid_dependents();
+  grid_wait();
+  const int b = blockIdx.y, G = p.c.G, tid = threadIdx.x;
+  const bool isk = (int)blockIdx.x < G;
+  const int g = isk ? blockIdx.x : blockIdx.x - G;
+  const PagedSeq sq = paged_seq(p.b, p.c, b);
+  const int32_t* acc = p.accepted + (int64_t)b * p.accepted_st;
+  // the list ends at the first entry that is not above the one before it, is no new token, or has no memory
+  if (tid == 0) stop = p.A;
+  __syncthreads();
+  for (int j = tid; j < p.A; j += S::NT) {
+    const int a = acc[j], slot = sq.old + a;
+    if (a <= (j ? acc[j - 1] : -1) || a >= sq.n || slot < 0 || slot >= sq.len || paged_page(p.c, b, slot / PAGE) < 0)
+      atomicMin(&stop, j);
+  }
+  __syncthreads();
+  const int count = stop;
+  if (blockIdx.x == 0 && tid == 0) p.new_lens[b] = sq.n == 0 ? *(p.b.lens + b) : max(sq.old + count, 0);
+  if (tid == 0) fixed = count;
+  __syncthreads();
+  for (int j = tid; j < count; j += S::NT)
+    if (acc[j] != j) atomicMin(&fixed, j);
+  __syncthreads();
+  if (fixed >= count) return;
+  float* const scales = isk ? p.c.k_scale : p.c.v_scale;
+  uint8_t* const pool = isk ? p.c.k : p.c.v;
+  const int slot0 = sq.old + fixed, slot1 = sq.old + count;  // slots that tokens move into
+  for (int blk = slot0 / PAGE; blk * PAGE < slot1; ++blk) {
+    const int lo = max(slot0 - blk * PAGE, 0), hi = min(slot1 - blk * PAGE, PAGE);
+    const int pid = paged_page(p.c, b, blk);
+    if (pid < 0) continue;  // (no page here: nothing to write to)
+    const int64_t to = (int64_t)pid * G + g;
+    for (int r = tid; r < PAGE; r += S::NT) {
+      m.src[r] = kNoRow;
+      if (r >= lo && r < hi) {
+        const int s = sq.old + acc[blk * PAGE + r - sq.old];
+        const int64_t from = (int64_t)paged_page(p.c, b, s / PAGE) * G + g, row = from * PAGE + s % PAGE;
+        m.src[r] = (uint32_t)row;
+        m.scale[r] = scales[from];
+      }
+    }
+    const float was = scales[to];
+    __syncthreads();
+    if (isk && p.weight) {  // a row per thread, read before any is written
+      const int r = lo + tid;
+      const float w = r < hi ? p.weight[m.src[r]] : 0.f;
+      const int x = r < hi ? p.position[m.src[r]] : 0;
+      __syncthreads();
+      if (r < hi) {
+        p.weight[to * PAGE + r] = w;
+        p.position[to * PAGE + r] = x;
+      }
+    }
+    move_block<KV, D, PAGE>(m, pool, pool + to * (PAGE * D), scales + to, was, lo > 0, lo);
+    __syncthreads();  // the block is written, its list read
+  }
+}
+
+struct EvictSplit {
+  int cluster, run, cached;
+  size_t smem;
+};
+
+EvictSplit split_for(const PagedEvictParams& p, int n_sm) {
+  (void)n_sm;
+  const int64_t slots = (int64_t)p.c.max_pages * p.c.page;
+  EvictSplit s;
+  s.cluster = slots <= 4096 ? 1 : slots <= 8192 ? 2 : slots <= 16384 ? 4 : 8;
+  s.run = (int)((slots + s.cluster - 1) / s.cluster + 31) / 32 * 32;
+  s.cached = s.run < kMaxKeys ? s.run : kMaxKeys;
+  s.smem = sizeof(SelShared) + (size_t)s.cached * 4 + (size_t)s.run / 32 * 12;
+  return s;
+}
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// plan (pointers null) and bytes
+size_t plan_for(const PagedEvictParams& p, void* ws, EvictPlan& x) {
+  const int64_t slots = (int64_t)p.c.max_pages * p.c.page;
+  x.lines_per_b = p.per_head ? p.c.G : 1;
+  const int64_t kept = p.keep < slots ? p.keep : slots;
+  x.blocks = (int)((kept + p.c.page - 1) / p.c.page);
+  x.cap = (int)(kept < slots - kept ? kept : slots - kept);
+  const size_t lines = (size_t)p.B * x.lines_per_b;
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* r = w + at;
+    at += align256(bytes);
+    return w ? r : nullptr;
+  };
+  x.head = reinterpret_cast<int32_t*>(take(lines * 16));
+  x.first = reinterpret_cast<int32_t*>(take(lines * (x.blocks + 1) * 4));
+  x.dst = reinterpret_cast<int32_t*>(take(lines * x.cap * 4));
+  x.src = reinterpret_cast<int32_t*>(take(lines * x.cap * 4));
+  x.edge = reinterpret_cast<float*>(take((size_t)p.B * p.c.G * 8));
+  return at;
+}
+
+template <int KV, int D, int PAGE>
+cudaError_t move_launch(const PagedEvictParams& p, const EvictPlan& plan, cudaStream_t st) {
+  return launch_dependent(paged_move_kernel<KV, D, PAGE>, dim3(plan.blocks, 2 * p.c.G, p.B), MoveShape<D, PAGE>::NT, 0,
+                          st, p, plan);
+}
+template <int KV, int D, int PAGE>
+cudaError_t keep_launch(const PagedKeepParams& p, cudaStream_t st) {
+  return launch_dependent(paged_keep_kernel<KV, D, PAGE>, dim3(2 * p.c.G, p.b.B), MoveShape<D, PAGE>::NT, 0, st, p);
+}
+
+// f(KV, D, PAGE) as constants
+template <typename F>
+cudaError_t with_shape(int kv, int D, int page, F f) {
+  auto pages = [&](auto k, auto d) {
+    switch (page) {
+      case 16: return f(k, d, std::integral_constant<int, 16>{});
+      case 32: return f(k, d, std::integral_constant<int, 32>{});
+      case 64: return f(k, d, std::integral_constant<int, 64>{});
+      case 128: return f(k, d, std::integral_constant<int, 128>{});
+      default: return cudaErrorInvalidValue;
+    }
+  };
+  auto dims = [&](auto k) {
+    if (D == 128) return pages(k, std::integral_constant<int, 128>{});
+    if (D == 64) return pages(k, std::integral_constant<int, 64>{});
+    return cudaErrorInvalidValue;
+  };
+  return kv == kKvInt8 ? dims(std::integral_constant<int, kKvInt8>{}) : dims(std::integral_constant<int, kKvE4m3>{});
+}
+
+cudaError_t select_launch(const PagedEvictParams& p, const EvictPlan& plan, int n_sm, cudaStream_t st) {
+  const EvictSplit s = split_for(p, n_sm);
+  static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
+    e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)(sizeof(SelShared) + kMaxKeys * 4 + kEvictSlots / 8 / 32 * 12));
+    if (e != cudaSuccess) return e;
+    if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(s.cluster, plan.lines_per_b, p.B);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = s.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = s.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, paged_select_kernel, p, plan, s.run, s.cached);
+}
+
+}  // namespace
+
+size_t paged_evict_workspace(const PagedEvictParams& p) {
+  EvictPlan x;
+  return plan_for(p, nullptr, x);
+}
+
+cudaError_t launch_paged_evict(const PagedEvictParams& p, int kv, void* ws, int n_sm, cudaStream_t st) {
+  EvictPlan plan;
+  plan_for(p, ws, plan);
+  const cudaError_t e = select_launch(p, plan, n_sm, st);
+  if (e != cudaSuccess) return e;
+  return with_shape(kv, p.c.D, p.c.page, [&](auto k, auto d, auto page) {
+    return move_launch<decltype(k)::value, decltype(d)::value, decltype(page)::value>(p, plan, st);
+  });
+}
+
+cudaError_t launch_paged_keep(const PagedKeepParams& p, int kv, cudaStream_t st) {
+  return with_shape(kv, p.c.D, p.c.page, [&](auto k, auto d, auto page) {
+    return keep_launch<decltype(k)::value, decltype(d)::value, decltype(page)::value>(p, st);
+  });
+}
+
+}  // namespace spatten

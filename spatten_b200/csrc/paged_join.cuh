@@ -132,6 +132,7 @@ paged_join_kernel(const PagedAttendParams p, const PagedPartials ws, const bool 
   if (live && part0 == 0) {
     const int r = cut.row0 + row;
     const float inv = paged_normaliser(m, l, M);
+    if (p.stat && lane == 0) p.stat[(int64_t)(cut.begin + r / R) * p.b.H + cut.g * R + r % R] = row_stat(m, l);
     uint16_t* op = static_cast<uint16_t*>(p.out) + (int64_t)(cut.begin + r / R) * p.o_st +
                    (int64_t)(cut.g * R + r % R) * p.o_sh + lane * E;
 #pragma unroll

@@ -20,6 +20,19 @@ replayed with other lengths, pages and contents.
 * ``paged_read`` -- cached tokens back in 16 bits: the ones that a cascade
   keeps (``topk_indices``), or whole sequences.
 
+Trees of drafted tokens, checked in one pass:
+
+* ``paged_tree`` -- from the drafted tokens' parents the bits of the new tokens
+  that each of them sees (for ``paged_attention``) and their positions (for
+  ``paged_append``), once per step for all layers;
+* ``paged_keep`` -- of the new tokens the accepted ones stay.
+
+A cache of bounded length, the cascade's token pruning while a model generates:
+
+* ``new_paged_weights(cache)`` -> ``PagedWeights``, in which ``paged_attention``
+  accumulates the attention weight of every cached token;
+* ``paged_evict`` -- the recent tokens and those of the largest weight stay.
+
 Rows behind ``cu_tokens[-1]`` (a padded batch) are neither read nor written.
 """
 import math
@@ -76,6 +89,29 @@ def new_paged_cache(num_pages, kv_heads, head_dim, page_size=64, kv_dtype=torch.
     k, v = (torch.zeros(shape, dtype=torch.int8, device=device).view(kv_dtype) for _ in range(2))
     ks, vs = (torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
     return PagedKVCache(k, v, ks, vs)
+
+
+class PagedWeights(namedtuple("PagedWeights", "weight position")):
+    """Beside a pool: the attention weight that each cached token has gathered,
+    fp32 [P, G, page], and its position, int32 [P, G, page]; contiguous."""
+
+
+def new_paged_weights(cache):
+    """No weight and position 0 everywhere; a slot's start with the first
+    ``paged_attention`` call that has its token among the new ones."""
+    shape, dev = cache.k.shape[:3], cache.k.device
+    return PagedWeights(torch.zeros(shape, dtype=torch.float32, device=dev),
+                        torch.zeros(shape, dtype=torch.int32, device=dev))
+
+
+def _weights(a, weights, dev, shape):
+    """The weights beside a pool of ``shape`` into ``a``; their checks."""
+    for t, name, dt in zip(weights, ("weight", "position"), (torch.float32, torch.int32)):
+        if t.get_device() != dev:
+            raise ValueError(f"weights.{name}: on {t.device}, the cache is on cuda:{dev}")
+        if t.dtype != dt or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"weights.{name}: need a contiguous {dt} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    a.weight, a.position = weights[0].data_ptr(), weights[1].data_ptr()
 
 
 def _index(t, name, dev, dim, dtype=torch.int32):
@@ -193,14 +229,46 @@ def paged_append(cache, k, v, page_table, cu_tokens, seq_lens, max_tokens, q=Non
     return q_out
 
 
-def paged_attention(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_scale=None, out=None):
+def paged_tree(parents, cu_tokens, seq_lens, max_tokens):
+    """Bits and positions of trees of drafted tokens: ``parents`` int32 [T]
+    holds, per new token, its parent's place among its sequence's new tokens
+    (which comes before its own), or -1 for a child of the cached tokens.
+    Returns (tree int32 [T, ceil(max_tokens / 32)], positions int32 [T]): bit j
+    of a row's words is set if it sees new token j (itself and its ancestors);
+    its position is that of the sequence's first new token plus its depth.
+    At most 1024 tokens per sequence."""
+    dev = parents.get_device()
+    if dev < 0:
+        raise ValueError("paged_tree: CUDA tensors expected (no CPU path)")
+    a = N.PagedTreeArgs()
+    a.B, a.seq_lens = seq_lens.shape[0], _index(seq_lens, "seq_lens", dev, 1)
+    a.parents = _index(parents, "parents", dev, 1)
+    _fill_tokens(a, dev, cu_tokens, parents.shape[0], max_tokens)
+    a.tree_words = a.tree_stride = max(-(-a.max_tokens // 32), 1)
+    tree, positions = parents.new_empty((a.T, a.tree_words)), parents.new_empty((a.T,))
+    a.tree, a.positions = tree.data_ptr(), positions.data_ptr()
+    _call(N.lib.spatten_paged_tree, dev, a)
+    return tree, positions
+
+
+def paged_attention(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_scale=None, out=None, tree=None,
+                    weights=None, positions=None):
     """Causal attention of the new tokens' queries q [T, H, D] over the cache
     -> [T, H, D]: query i of sequence b sees slots ``n < seq_lens[b] - n_b + i
     + 1`` (its own among them, appended before); 0 where it sees none. GQA as
     in HF's ``repeat_kv``. ``out`` rows behind the last sequence keep what they
-    held."""
-    a = N.PagedAttendArgs()
-    dev, (_, _, _, D) = _fill(a, cache, page_table, seq_lens)
+    held.
+
+    ``tree`` (int32 [T, >= max_tokens / 32], e.g. of ``paged_tree``): a query
+    sees every slot before its sequence's new tokens, and of these the ones
+    whose bits its row has. ``weights``: the softmax weight that the queries
+    give each cached token, summed over the query heads of its KV head, is
+    added to ``weights.weight``; the new tokens' own start at 0, and their
+    ``weights.position`` becomes ``positions`` (int32 [T]; default: the slot).
+    Sequences must not share pages then."""
+    ext = N.PagedAttendExtArgs() if tree is not None or weights is not None else None
+    a = N.PagedAttendArgs() if ext is None else ext.attend
+    dev, (P, G, page, D) = _fill(a, cache, page_table, seq_lens)
     shape, dt = (q.shape[0], q.shape[1], D), q.dtype
     if dt not in _DT:
         raise TypeError(f"q: dtype {dt} (need float16 or bfloat16)")
@@ -211,10 +279,82 @@ def paged_attention(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_sc
         out = q.new_empty(shape)
     a.out, a.o_st, a.o_sh = _rows(out, "out", dev, dt, shape)
     a.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-    n = N.lib.spatten_paged_attend_workspace_size(a)
+    if tree is not None:
+        ext.tree = _index(tree, "tree", dev, 2)
+        if tree.shape[0] != shape[0]:
+            raise ValueError(f"tree: {tree.shape[0]} rows for {shape[0]}")
+        if 32 * tree.shape[1] < min(a.max_tokens, a.T):
+            raise ValueError(f"tree: {tree.shape[1]} words of 32 tokens for {a.max_tokens}")
+        ext.tree_words, ext.tree_stride = tree.shape[1], tree.stride()[0]
+    if weights is not None:
+        _weights(ext, weights, dev, (P, G, page))
+    if positions is not None:
+        if weights is None:
+            raise ValueError("positions without weights")
+        ext.positions = _index(positions, "positions", dev, 1)
+        if positions.shape[0] != shape[0]:
+            raise ValueError(f"positions: {positions.shape[0]} for {shape[0]} rows")
+    if ext is None:
+        size, call = N.lib.spatten_paged_attend_workspace_size, N.lib.spatten_paged_attend
+    else:
+        a, size, call = ext, N.lib.spatten_paged_attend_ext_workspace_size, N.lib.spatten_paged_attend_ext
+    n = size(a)
     ws = q.new_empty((n,), dtype=torch.uint8) if n else None
-    _call(N.lib.spatten_paged_attend, dev, a, ws.data_ptr() if n else None, n)
+    _call(call, dev, a, ws.data_ptr() if n else None, n)
     return out
+
+
+def paged_evict(cache, weights, page_table, seq_lens, keep, recent=0, per_head=False):
+    """Sequences of more than ``keep`` tokens keep that many: those of the
+    ``recent`` newest positions, then those of the largest accumulated weight
+    (``weights``, see ``paged_attention``), ties to the lower slot. One choice
+    for all KV heads, by the sum of their weights (rounded to fp32), or with
+    ``per_head`` each head's own (its slots then hold other tokens than the
+    other heads'). Returns the sequences' new lengths, int32 [B].
+
+    Kept tokens in the first ``keep`` slots stay; the others move, with their
+    weights and positions, into the slots that became free, both in ascending
+    order: from then on slots are not in order of position, so later
+    ``paged_append`` and ``paged_attention`` calls need ``positions``. A moved
+    token is rounded to the scale of its new page, which grows as in
+    ``paged_append``. Sequences with slots that have no memory are left as they
+    are; sequences must not share the pages that tokens move into."""
+    a = N.PagedEvictArgs()
+    dev, (P, G, page, _) = _fill(a, cache, page_table, seq_lens)
+    _weights(a, weights, dev, (P, G, page))
+    a.keep, a.recent, a.per_head = int(keep), int(recent), bool(per_head)
+    new_lens = torch.empty_like(seq_lens, memory_format=torch.contiguous_format)
+    a.new_lens = new_lens.data_ptr()
+    n = N.lib.spatten_paged_evict_workspace_size(a)
+    ws = cache.k.new_empty((n,), dtype=torch.uint8) if n else None
+    _call(N.lib.spatten_paged_evict, dev, a, ws.data_ptr() if n else None, n)
+    return new_lens
+
+
+def paged_keep(cache, page_table, cu_tokens, seq_lens, accepted, weights=None):
+    """Of the new tokens the accepted ones stay: ``accepted`` int32 [B, A] lists
+    their places among their sequence's new tokens in ascending order, -1 behind
+    a short list (it ends at the first entry that is not above the one before
+    it, or no new token). They move to the front of the new tokens' slots in
+    that order, with their ``weights`` where given, rounded to the scales of
+    the pages they come to. Returns the sequences' new lengths, int32 [B].
+    Sequences must not share the pages of the new tokens."""
+    a = N.PagedKeepArgs()
+    dev, (P, G, page, _) = _fill(a, cache, page_table, seq_lens)
+    a.cu_tokens = _index(cu_tokens, "cu_tokens", dev, 1)
+    if cu_tokens.shape[0] != a.B + 1:
+        raise ValueError(f"cu_tokens: {cu_tokens.shape[0]} entries for {a.B} sequences")
+    a.accepted = _index(accepted, "accepted", dev, 2)
+    rows, a.n_accepted = accepted.shape
+    if rows != a.B:
+        raise ValueError(f"accepted: {rows} rows for {a.B} sequences")
+    a.accepted_stride = accepted.stride()[0]
+    if weights is not None:
+        _weights(a, weights, dev, (P, G, page))
+    new_lens = torch.empty_like(seq_lens, memory_format=torch.contiguous_format)
+    a.new_lens = new_lens.data_ptr()
+    _call(N.lib.spatten_paged_keep, dev, a)
+    return new_lens
 
 
 def paged_read(cache, page_table, seq_lens, idx=None, n_tokens=None, dtype=torch.bfloat16):
@@ -242,4 +382,5 @@ def paged_read(cache, page_table, seq_lens, idx=None, n_tokens=None, dtype=torch
     return k, v
 
 
-__all__ = ["PagedKVCache", "new_paged_cache", "paged_append", "paged_attention", "paged_read"]
+__all__ = ["PagedKVCache", "PagedWeights", "new_paged_cache", "new_paged_weights", "paged_append", "paged_attention",
+           "paged_evict", "paged_keep", "paged_read", "paged_tree"]
