@@ -756,12 +756,17 @@ static int fill_paged_attend_ext(const spatten_paged_attend_ext_args* a, spatten
   return SPATTEN_OK;
 }
 
-// the attention's part, and the rows' statistics
+// the attention's part, the rows' statistics, and scores
 static size_t attend_ext_part(const spatten::PagedWeighParams& p) {
   return align256(spatten::paged_attend_workspace(p.a, sm_count()));
 }
+static size_t attend_ext_stats(const spatten::PagedWeighParams& p) {
+  return align256((size_t)p.a.b.T * p.a.b.H * sizeof(float2));
+}
 static size_t attend_ext_bytes(const spatten::PagedWeighParams& p) {
-  return attend_ext_part(p) + (p.weight ? align256((size_t)p.a.b.T * p.a.b.H * sizeof(float2)) : 0);
+  if (!p.weight) return attend_ext_part(p);
+  return attend_ext_part(p) + attend_ext_stats(p) +
+         align256((size_t)p.a.b.B * p.a.c.G * p.a.c.max_pages * p.a.c.page * spatten::paged_attend_score_rows(p.a) * 4);
 }
 
 size_t spatten_paged_attend_ext_workspace_size(const spatten_paged_attend_ext_args* a) {
@@ -780,7 +785,13 @@ int spatten_paged_attend_ext(const spatten_paged_attend_ext_args* a, void* works
   if (int e = check_rows(who, "q", t.q, t.q_st, t.q_sh)) return e;
   if (int e = check_out_rows(who, "out", t.out, t.o_st, t.o_sh, t.T, t.H, p.a.c.D)) return e;
   if (int e = check_workspace(who, workspace, workspace_bytes, attend_ext_bytes(p))) return e;
-  if (p.weight) p.a.stat = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + attend_ext_part(p));
+  if (p.weight) {
+    uint8_t* w = static_cast<uint8_t*>(workspace) + attend_ext_part(p);
+    p.a.score_rows = spatten::paged_attend_score_rows(p.a);
+    p.rows_over = p.a.score_rows ? spatten::kScoreRows : 0;
+    p.a.stat = reinterpret_cast<float2*>(w);
+    if (p.a.score_rows) p.a.score = reinterpret_cast<float*>(w + attend_ext_stats(p));
+  }
   cudaError_t e = spatten::launch_paged_attend(p.a, t.dtype, t.cache.kv_type, workspace, sm_count(),
                                                (cudaStream_t)stream);
   if (e == cudaSuccess && p.weight)

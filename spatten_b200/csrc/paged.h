@@ -67,7 +67,12 @@ struct PagedAttendParams {
   int64_t tree_st = 0;
   int words = 0;
   float2* stat = nullptr;          // or null: [T, H] reference m of a row's exponentials, 1 / their sum
+  // or null: scores (log2) of sequences of at most kScoreRows query rows per KV
+  // head, [B, G, slots, score_rows], where an unmasked place's page has memory
+  float* score = nullptr;
+  int score_rows = 0;
 };
+constexpr int kScoreRows = 8;
 
 // The weights that a call's rows give the cached tokens (after the attention).
 struct PagedWeighParams {
@@ -75,6 +80,7 @@ struct PagedWeighParams {
   float* weight;            // [P, G, page]
   int32_t* position;        // [P, G, page]
   const int32_t* positions; // or null: [T]
+  int rows_over;            // sequences of at most as many rows have their scores kept
 };
 
 struct PagedTreeParams {
@@ -132,6 +138,7 @@ cudaError_t launch_paged_attend_tc(const PagedAttendParams& p, int dtype, int kv
 cudaError_t read_paged_device_error(unsigned int* code, bool reset);
 cudaError_t launch_paged_attend(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,
                                 cudaStream_t st);
+int paged_attend_score_rows(const PagedAttendParams& p);  // scores kept per slot; 0: none
 cudaError_t launch_paged_weigh(const PagedWeighParams& p, int dtype, int kv, cudaStream_t st);
 constexpr int kTreeTokens = 1024;  // new tokens of a sequence whose tree is laid out
 cudaError_t launch_paged_tree(const PagedTreeParams& p, cudaStream_t st);

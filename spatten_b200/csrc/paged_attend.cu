@@ -395,6 +395,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     const int nrows = sq.n * R, r0 = rt * ROWS;
     // slots that the tile's last and first row see
     const bool tree = EXT && p.tree;
+    float* const score = EXT && p.score && nrows <= kScoreRows
+                             ? p.score + ((int64_t)b * G + g) * p.c.max_pages * page * p.score_rows : nullptr;
     const int lim_max = min(sq.old + (tree ? sq.n : min((r0 + ROWS - 1) / R, sq.n - 1) + 1), sq.len);
     const int lim_min = min(sq.old + (tree ? 0 : r0 / R + 1), sq.len);
     const uint32_t t_end = min(t1, (uint32_t)(max(lim_max, 0) + kKeys - 1) / kKeys);
@@ -549,6 +551,17 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
                 if (!((sees >> gid) & 1u)) s[nb][c] = -INFINITY;
                 if (!((sees >> (gid + 8)) & 1u)) s[nb][2 + c] = -INFINITY;
               }
+          }
+        }
+        if constexpr (EXT && NB == 1) {
+          if (score && 2 * tig < p.score_rows && !none) {
+            float* to = score + (int64_t)(slot0 + gid) * p.score_rows + 2 * tig;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (slot0 + gid + 8 * h >= lim_max) break;
+              if (p.score_rows == 1) to[8 * h] = s[0][2 * h];
+              else *reinterpret_cast<float2*>(to + 8 * h * p.score_rows) = make_float2(s[0][2 * h], s[0][2 * h + 1]);
+            }
           }
         }
         // p = 2^(s - m), and w = 2^(s + log2 v_scale - M)
@@ -779,6 +792,18 @@ Plan plan_for(const PagedAttendParams& p) {
 }
 
 }  // namespace
+
+// The scores of a step are kept where a sequence has at most kScoreRows rows: 4 bytes
+// a row and slot, written and read once, instead of the keys' D bytes read again; up to 1 GiB
+// of them.
+int paged_attend_score_rows(const PagedAttendParams& p) {
+  const Plan x = plan_for(p);
+  if (!x.use_few || row_block(x.few) != kScoreRows) return 0;
+  const int64_t most = (int64_t)p.b.max_tokens * (p.b.H / p.c.G);
+  int rows = 1;
+  while (rows < most && rows < kScoreRows) rows *= 2;
+  return (double)p.b.B * p.c.G * p.c.max_pages * p.c.page * rows * 4 <= (double)(1 << 30) ? rows : 0;
+}
 
 bool paged_attend_fits(const PagedAttendParams& p) { return units_bound(plan_for(p).few) < 4e9; }
 
