@@ -85,14 +85,16 @@ const char* spatten_last_error(void) { return g_err.c_str(); }
 
 int spatten_device_error(unsigned int* code, int reset) {
   if (!code) return fail(SPATTEN_ERR_INVALID, "device_error: null output");
-  unsigned int proj = 0, out = 0, paged = 0;
+  unsigned int proj = 0, out = 0, paged = 0, weigh = 0;
   if (int e = cuda_status(spatten::read_device_error(code, reset != 0), "device_error read")) return e;
   if (int e = cuda_status(spatten::read_proj_device_error(&proj, reset != 0), "device_error read")) return e;
   if (int e = cuda_status(spatten::read_out_proj_device_error(&out, reset != 0), "device_error read")) return e;
   if (int e = cuda_status(spatten::read_paged_device_error(&paged, reset != 0), "device_error read")) return e;
+  if (int e = cuda_status(spatten::read_paged_weigh_error(&weigh, reset != 0), "device_error read")) return e;
   if (*code == 0) *code = proj;
   if (*code == 0) *code = out;
   if (*code == 0) *code = paged;
+  if (*code == 0) *code = weigh;
   return ok();
 }
 
@@ -753,26 +755,31 @@ static int fill_paged_attend_ext(const spatten_paged_attend_ext_args* a, spatten
   if (a->positions && (!a->weight || !aligned(a->positions, 4)))
     return fail(SPATTEN_ERR_INVALID, "%s: positions without weight, or not 4-byte aligned", who);
   p.weight = a->weight; p.position = a->position; p.positions = a->positions;
+  if (p.weight) p.a.score_rows = spatten::paged_attend_score_rows(p.a);
+  p.rows_over = p.a.score_rows ? spatten::kScoreRows : 0;
   return SPATTEN_OK;
 }
 
-// the attention's part, the rows' statistics, and scores
-static size_t attend_ext_part(const spatten::PagedWeighParams& p) {
-  return align256(spatten::paged_attend_workspace(p.a, sm_count()));
-}
-static size_t attend_ext_stats(const spatten::PagedWeighParams& p) {
-  return align256((size_t)p.a.b.T * p.a.b.H * sizeof(float2));
-}
-static size_t attend_ext_bytes(const spatten::PagedWeighParams& p) {
-  if (!p.weight) return attend_ext_part(p);
-  return attend_ext_part(p) + attend_ext_stats(p) +
-         align256((size_t)p.a.b.B * p.a.c.G * p.a.c.max_pages * p.a.c.page * spatten::paged_attend_score_rows(p.a) * 4);
+// The workspace: the attention's part, and for the weights the rows' statistics, the
+// scores that the attention keeps, and what the other rows need.
+struct AttendExtParts {
+  size_t stats, scores, weigh, bytes;
+};
+static AttendExtParts attend_ext_parts(const spatten::PagedWeighParams& p) {
+  AttendExtParts x;
+  x.stats = align256(spatten::paged_attend_workspace(p.a, sm_count()));
+  x.scores = x.weigh = x.bytes = x.stats;
+  if (!p.weight) return x;
+  x.scores += align256((size_t)p.a.b.T * p.a.b.H * sizeof(float2));
+  x.weigh = x.scores + align256((size_t)p.a.b.B * p.a.c.G * p.a.c.max_pages * p.a.c.page * p.a.score_rows * 4);
+  x.bytes = x.weigh + align256(spatten::paged_weigh_workspace(p));
+  return x;
 }
 
 size_t spatten_paged_attend_ext_workspace_size(const spatten_paged_attend_ext_args* a) {
   spatten::PagedWeighParams p;
   if (fill_paged_attend_ext(a, p) != SPATTEN_OK || p.a.b.B == 0 || p.a.b.max_tokens == 0) return 0;
-  return attend_ext_bytes(p);
+  return attend_ext_parts(p).bytes;
 }
 
 int spatten_paged_attend_ext(const spatten_paged_attend_ext_args* a, void* workspace, size_t workspace_bytes,
@@ -784,18 +791,17 @@ int spatten_paged_attend_ext(const spatten_paged_attend_ext_args* a, void* works
   const spatten_paged_attend_args& t = a->attend;
   if (int e = check_rows(who, "q", t.q, t.q_st, t.q_sh)) return e;
   if (int e = check_out_rows(who, "out", t.out, t.o_st, t.o_sh, t.T, t.H, p.a.c.D)) return e;
-  if (int e = check_workspace(who, workspace, workspace_bytes, attend_ext_bytes(p))) return e;
+  const AttendExtParts parts = attend_ext_parts(p);
+  if (int e = check_workspace(who, workspace, workspace_bytes, parts.bytes)) return e;
+  uint8_t* const w = static_cast<uint8_t*>(workspace);
   if (p.weight) {
-    uint8_t* w = static_cast<uint8_t*>(workspace) + attend_ext_part(p);
-    p.a.score_rows = spatten::paged_attend_score_rows(p.a);
-    p.rows_over = p.a.score_rows ? spatten::kScoreRows : 0;
-    p.a.stat = reinterpret_cast<float2*>(w);
-    if (p.a.score_rows) p.a.score = reinterpret_cast<float*>(w + attend_ext_stats(p));
+    p.a.stat = reinterpret_cast<float2*>(w + parts.stats);
+    if (p.a.score_rows) p.a.score = reinterpret_cast<float*>(w + parts.scores);
   }
   cudaError_t e = spatten::launch_paged_attend(p.a, t.dtype, t.cache.kv_type, workspace, sm_count(),
                                                (cudaStream_t)stream);
   if (e == cudaSuccess && p.weight)
-    e = spatten::launch_paged_weigh(p, t.dtype, t.cache.kv_type, (cudaStream_t)stream);
+    e = spatten::launch_paged_weigh(p, t.dtype, t.cache.kv_type, w + parts.weigh, sm_count(), (cudaStream_t)stream);
   return cuda_status(e, "paged_attend_ext launch");
 }
 

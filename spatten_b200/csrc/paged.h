@@ -139,7 +139,9 @@ cudaError_t read_paged_device_error(unsigned int* code, bool reset);
 cudaError_t launch_paged_attend(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,
                                 cudaStream_t st);
 int paged_attend_score_rows(const PagedAttendParams& p);  // scores kept per slot; 0: none
-cudaError_t launch_paged_weigh(const PagedWeighParams& p, int dtype, int kv, cudaStream_t st);
+size_t paged_weigh_workspace(const PagedWeighParams& p);
+cudaError_t launch_paged_weigh(const PagedWeighParams& p, int dtype, int kv, void* ws, int n_sm, cudaStream_t st);
+cudaError_t read_paged_weigh_error(unsigned int* code, bool reset);
 constexpr int kTreeTokens = 1024;  // new tokens of a sequence whose tree is laid out
 cudaError_t launch_paged_tree(const PagedTreeParams& p, cudaStream_t st);
 constexpr int kEvictSlots = 1 << 20;  // slots of a sequence that is chosen from
