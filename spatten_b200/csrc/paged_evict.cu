@@ -127,8 +127,8 @@ struct EvictPlan {
   int lines_per_b, blocks, cap;
 };
 
-constexpr int kSelThreads = 512, kBins = 2048;
-constexpr int kMaxKeys = 40960;  // of a CTA in shared memory; the others are read again
+constexpr int kSelThreads = 1024, kBins = 2048, kFly = 8;
+constexpr int kMaxWords = 40960;  // of a CTA's keys (and positions) in shared memory; the others are read again
 
 struct SelShared {
   uint32_t hist[2][kBins];
@@ -137,6 +137,9 @@ struct SelShared {
   uint32_t xch[8][8];   // what the cluster's other CTAs read, one row per exchange
   uint32_t at[3];
 };
+
+constexpr size_t kMostShared = sizeof(SelShared) + kMaxWords * 4 + kEvictSlots / 8 / 32 * 12;
+static_assert(kMostShared <= 227 * 1024, "a CTA's shared memory");
 
 // Sum over the CTA's threads before this one, and the sum of all.
 SPATTEN_DEV uint32_t block_scan(SelShared& sh, uint32_t x, uint32_t& total) {
@@ -171,7 +174,8 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
   extern __shared__ __align__(16) uint8_t dsm[];
   SelShared& sh = *reinterpret_cast<SelShared*>(dsm);
   uint32_t* keys = reinterpret_cast<uint32_t*>(dsm + sizeof(SelShared));  // [cached]
-  uint32_t* prot = keys + cached;                                          // [run / 32]: recent
+  int* posn = reinterpret_cast<int*>(keys + cached);                       // [cached] where recent > 0
+  uint32_t* prot = keys + (p.recent > 0 ? 2 : 1) * cached;                 // [run / 32]: recent
   uint32_t* kept = prot + run / 32;                                        // [run / 32]
   uint32_t* ties = kept + run / 32;                                        // [run / 32]
   grid_dependents();
@@ -192,33 +196,78 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
   }
   const int lo = min(rank * run, len), n = min(run, len - lo), words = (n + 31) / 32;
 
-  auto row_of = [&](int slot) {  // -1: no memory
-    const int pid = paged_page(p.c, b, slot >> page_log);
-    return pid < 0 ? (int64_t)-1 : ((int64_t)pid * G + hl) * page + (slot & (page - 1));
-  };
-  auto load_key = [&](int i) -> uint32_t {  // weights order as integers; negative ones and NaN count as 0
-    const int64_t row = row_of(lo + i);
-    if (row < 0) return 0u;
-    float w;
-    if (p.per_head) {
-      w = p.weight[row];
-    } else {
-      double sum = 0.0;
-      for (int g = 0; g < G; ++g) sum += (double)p.weight[row + (int64_t)g * page];
-      w = (float)sum;
+  // Slots i of this CTA's run, kFly of them at once: ordered keys (weights order as
+  // integers; negative ones and NaN count as 0), positions, and whether they have memory.
+  auto load = [&](const int (&i)[kFly], uint32_t (&k)[kFly], int (&pos)[kFly]) {
+    int64_t row[kFly];
+    bool all = true;
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      const int slot = lo + i[u], pid = i[u] < n ? paged_page(p.c, b, slot >> page_log) : 0;
+      all &= pid >= 0;
+      row[u] = ((int64_t)max(pid, 0) * G + hl) * page + (slot & (page - 1));
     }
-    return w > 0.f ? __float_as_uint(w) : 0u;
+    double sum[kFly];
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      k[u] = 0u;
+      pos[u] = 0;
+      sum[u] = 0.0;
+      if (i[u] < n && p.recent > 0) pos[u] = p.position[row[u]];
+      if (i[u] < n && p.per_head) sum[u] = p.weight[row[u]];
+    }
+    if (!p.per_head) {
+#pragma unroll 2
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int u = 0; u < kFly; ++u)
+          if (i[u] < n) sum[u] += (double)p.weight[row[u] + (int64_t)g * page];
+    }
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      const float w = (float)sum[u];
+      if (w > 0.f) k[u] = __float_as_uint(w);
+    }
+    return all;
   };
-  auto key = [&](int i) { return i < cached ? keys[i] : load_key(i); };
+  auto reload = [&](int at, int& pos) {  // of one that the shared memory did not hold
+    int i[kFly], x[kFly];
+    uint32_t k[kFly];
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) i[u] = u == 0 ? at : n;
+    load(i, k, x);
+    pos = x[0];
+    return k[0];
+  };
+  auto key = [&](int i) {
+    int pos;
+    return i < cached ? keys[i] : reload(i, pos);
+  };
+  auto position = [&](int i) {
+    int pos;
+    if (i < cached) return posn[i];
+    reload(i, pos);
+    return pos;
+  };
 
   // keys, the newest position, whether every slot has memory
   int newest = INT_MIN;
   bool hole = false;
-  for (int i = tid; i < n; i += kSelThreads) {
-    const int64_t row = row_of(lo + i);
-    hole |= row < 0;
-    if (p.recent > 0 && row >= 0) newest = max(newest, p.position[row]);
-    if (i < cached) keys[i] = load_key(i);
+  for (int base = tid; base < n; base += kSelThreads * kFly) {
+    int i[kFly], pos[kFly];
+    uint32_t k[kFly];
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) i[u] = base + u * kSelThreads;
+    hole |= !load(i, k, pos);
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      if (i[u] >= n) break;
+      newest = max(newest, pos[u]);
+      if (i[u] < cached) {
+        keys[i[u]] = k[u];
+        if (p.recent > 0) posn[i[u]] = pos[u];
+      }
+    }
   }
   {
     const int top = __reduce_max_sync(0xffffffffu, newest);
@@ -262,7 +311,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
       const int i = base + tid;
       bool r = false;
       if (i < n) {
-        if (p.recent > 0) r = (int64_t)p.position[row_of(lo + i)] > (int64_t)newest - p.recent;
+        if (p.recent > 0) r = (int64_t)position(i) > (int64_t)newest - p.recent;
         const uint32_t k = key(i);
         if (r) {
           lo1 = min(lo1, k);
@@ -570,13 +619,15 @@ struct EvictSplit {
 };
 
 EvictSplit split_for(const PagedEvictParams& p, int n_sm) {
-  (void)n_sm;
   const int64_t slots = (int64_t)p.c.max_pages * p.c.page;
   EvictSplit s;
-  s.cluster = slots <= 4096 ? 1 : slots <= 8192 ? 2 : slots <= 16384 ? 4 : 8;
+  const int64_t lines = (int64_t)p.B * (p.per_head ? p.c.G : 1);
+  s.cluster = 1;
+  while (s.cluster < 8 && slots > (int64_t)s.cluster * (lines * s.cluster < n_sm ? 2048 : 16384)) s.cluster *= 2;
   s.run = (int)((slots + s.cluster - 1) / s.cluster + 31) / 32 * 32;
-  s.cached = s.run < kMaxKeys ? s.run : kMaxKeys;
-  s.smem = sizeof(SelShared) + (size_t)s.cached * 4 + (size_t)s.run / 32 * 12;
+  const int arrays = p.recent > 0 ? 2 : 1;
+  s.cached = s.run < kMaxWords / arrays ? s.run : kMaxWords / arrays;
+  s.smem = sizeof(SelShared) + (size_t)s.cached * arrays * 4 + (size_t)s.run / 32 * 12;
   return s;
 }
 
@@ -643,7 +694,7 @@ cudaError_t select_launch(const PagedEvictParams& p, const EvictPlan& plan, int 
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
     e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(sizeof(SelShared) + kMaxKeys * 4 + kEvictSlots / 8 / 32 * 12));
+                             (int)kMostShared);
     if (e != cudaSuccess) return e;
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }

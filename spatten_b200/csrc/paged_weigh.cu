@@ -60,43 +60,56 @@ SPATTEN_DEV void add_weight(const PagedWeighParams& p, const WeighSlot& x, int g
   if (x.fresh) p.position[row] = x.position;
 }
 
-// A thread per slot, all heads.
+// A thread per slot, all heads, whose rows' statistics lie in shared memory.
+constexpr int kStatHeads = 64;
+
 template <int ROWS>
 __global__ void __launch_bounds__(kSlotThreads) paged_weigh_scores_kernel(const PagedWeighParams p) {
+  __shared__ float2 stat[kStatHeads][ROWS];
   grid_dependents();
   grid_wait();
   const PagedAttendParams& a = p.a;
-  const int b = blockIdx.y, G = a.c.G, R = a.b.H / G;
+  const int b = blockIdx.y, G = a.c.G, R = a.b.H / G, page = a.c.page;
   const PagedSeq sq = paged_seq(a.b, a.c, b);
   const int slot = blockIdx.x * kSlotThreads + threadIdx.x, lim = min(sq.old + sq.n, sq.len), nrows = sq.n * R;
-  if (sq.n == 0 || slot >= lim || nrows > p.rows_over) return;
-  WeighSlot x;
-  if (!weigh_slot(p, sq, b, slot, x)) return;
-  const int64_t slots = (int64_t)a.c.max_pages * a.c.page;
+  if (sq.n == 0 || (int)(blockIdx.x * kSlotThreads) >= lim || nrows > p.rows_over) return;
+  WeighSlot x = {};
+  const bool live = slot < lim && weigh_slot(p, sq, b, slot, x);
+  const int64_t slots = (int64_t)a.c.max_pages * page;
   const float* src = a.score + ((int64_t)b * G * slots + slot) * ROWS;
-#pragma unroll 4
-  for (int g = 0; g < G; ++g) {
-    float s[ROWS];
-    const float* at = src + g * slots * ROWS;
-    if constexpr (ROWS >= 4) {
-#pragma unroll
-      for (int i = 0; i < ROWS; i += 4) {
-        const float4 y = *reinterpret_cast<const float4*>(at + i);
-        s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < ROWS; ++i) s[i] = at[i];
+  for (int g0 = 0; g0 < G; g0 += kStatHeads) {
+    const int heads = min(G - g0, kStatHeads);
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * ROWS; i += kSlotThreads) {
+      const int g = i / ROWS, r = i % ROWS;  // (a row that there is not has no weight: its score is another's)
+      stat[g][r] = r < nrows ? a.stat[(int64_t)(sq.begin + r / R) * a.b.H + (g0 + g) * R + r % R] : make_float2(0.f, 0.f);
     }
-    const float before = x.fresh ? 0.f : p.weight[x.row + (int64_t)g * a.c.page];
-    float add = 0.f;
+    __syncthreads();
+    if (!live) continue;
+#pragma unroll 4
+    for (int h = 0; h < heads; ++h) {
+      const int g = g0 + h;
+      float s[ROWS];
+      const float* at = src + g * slots * ROWS;
+      if constexpr (ROWS >= 4) {
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-      if (i < nrows) {
-        const float2 y = a.stat[(int64_t)(sq.begin + i / R) * a.b.H + g * R + i % R];
-        add += fast_exp2(s[i] - y.x) * y.y;
+        for (int i = 0; i < ROWS; i += 4) {
+          const float4 y = *reinterpret_cast<const float4*>(at + i);
+          s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) s[i] = at[i];
       }
-    add_weight(p, x, g, before, add);
+      const float before = x.fresh ? 0.f : p.weight[x.row + (int64_t)g * page];
+      float add = 0.f;
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const float2 y = stat[h][i];
+        if (i < nrows) add += fast_exp2(s[i] - y.x) * y.y;
+      }
+      add_weight(p, x, g, before, add);
+    }
   }
 }
 
