@@ -7,7 +7,9 @@
 // kept tokens in slots behind `keep` move into the free slots before it, both in
 // ascending order. Nothing else moves: what is read (slots from `keep` on) and what is
 // written (slots before) are apart, so every written block is a CTA of its own, and
-// a token is rounded again only when it moves. Two launches:
+// a token is rounded again only when it moves. Three launches:
+//
+// paged_rank_kernel: the slots' keys, out of the pages.
 //
 // paged_select_kernel: a cluster of CTAs per sequence (or per sequence and KV head),
 // each holding the ordered keys of a run of slots in shared memory. The keep-th
@@ -15,8 +17,7 @@
 // cluster; then the kept, the free and the moving slots as bits, a word per 32 slots,
 // whose prefix sums number them.
 //
-// paged_move_kernel: a CTA per block (page, KV head, K or V) of the first `keep`
-// slots. A token's codes under the block's scale S' are round(code * S / S') with S'
+// paged_move_kernel: a CTA per few blocks (page, KV head) of the first `keep` slots. A token's codes under the block's scale S' are round(code * S / S') with S'
 // the larger of the block's scale (0 where it keeps nothing) and the one that the
 // largest moved magnitude needs; where S' grew, the kept codes are rounded likewise, as
 // appending does.
@@ -47,9 +48,9 @@ struct MoveShape {
 // The rows of one block that tokens move into.
 template <int PAGE>
 struct MoveRows {
-  uint32_t src[PAGE];  // row of the pool, kNoRow: none
-  float scale[PAGE];   // its scale
-  uint32_t red[8];
+  uint32_t src[PAGE];     // row of the pools, kNoRow: none
+  float scale[2][PAGE];   // its scales, K's and V's
+  uint32_t red[2][8];
 };
 
 template <int KV>
@@ -72,46 +73,54 @@ SPATTEN_DEV uint4 rescale16(uint4 c, float ratio) {
   return make_uint4(a.x, a.y, b.x, b.y);
 }
 
-// Moves m's rows into the block at `dst` (the rows before `end` that get none keep
-// their tokens, if `kept` says that there are any). All threads of the CTA; every
-// source is read before anything is written.
+// Moves m's rows into block `to` of K and of V, whose scales were `was` (the rows before
+// `end` that get none keep their tokens, if `kept` says that there are any). All
+// threads of the CTA; every source is read before anything is written.
 template <int KV, int D, int PAGE>
-SPATTEN_DEV void move_block(MoveRows<PAGE>& m, const uint8_t* pool, uint8_t* dst, float* sp, float s_was, bool kept,
-                            int end) {
+SPATTEN_DEV void move_block(MoveRows<PAGE>& m, const PagedCache& pc, int64_t to, float2 was, bool kept, int end) {
   using S = MoveShape<D, PAGE>;
   const int tid = threadIdx.x, lane = tid & 31, li = tid % S::LPR, rt = tid / S::LPR;
-  uint4 c[S::PASSES];
-  float amax = 0.f;
+  uint8_t* const pool[2] = {pc.k, pc.v};
+  uint4 c[2][S::PASSES];
 #pragma unroll
-  for (int j = 0; j < S::PASSES; ++j) {
-    const uint32_t row = m.src[j * S::RPP + rt];
-    c[j] = make_uint4(0u, 0u, 0u, 0u);
-    if (row != kNoRow) c[j] = *reinterpret_cast<const uint4*>(pool + (uint64_t)row * D + li * 16);
-  }
+  for (int v = 0; v < 2; ++v)
 #pragma unroll
-  for (int j = 0; j < S::PASSES; ++j) {
-    const int r = j * S::RPP + rt;
-    if (m.src[r] != kNoRow) amax = fmaxf(amax, fminf(row_amax<KV>(c[j]) * m.scale[r], kMaxFinite));
-  }
-  const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));  // magnitudes order as integers
-  if (lane == 0) m.red[tid >> 5] = top;
-  __syncthreads();
-  uint32_t all = 0u;
-#pragma unroll
-  for (int w = 0; w < S::NT / 32; ++w) all = max(all, m.red[w]);
-  const float s_old = kept ? s_was : 0.f, s = fmaxf(s_old, scale_for<KV>(__uint_as_float(all)));
-#pragma unroll
-  for (int j = 0; j < S::PASSES; ++j) {
-    const int r = j * S::RPP + rt;
-    uint4* to = reinterpret_cast<uint4*>(dst + r * D + li * 16);
-    if (m.src[r] != kNoRow) {
-      const float was = m.scale[r];
-      *to = s == was ? c[j] : s > 0.f ? rescale16<KV>(c[j], __fdiv_rn(was, s)) : make_uint4(0u, 0u, 0u, 0u);
-    } else if (r < end && s > s_old && kept) {
-      *to = rescale16<KV>(*to, __fdiv_rn(s_old, s));
+    for (int j = 0; j < S::PASSES; ++j) {
+      const uint32_t row = m.src[j * S::RPP + rt];
+      c[v][j] = make_uint4(0u, 0u, 0u, 0u);
+      if (row != kNoRow) c[v][j] = *reinterpret_cast<const uint4*>(pool[v] + (uint64_t)row * D + li * 16);
     }
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < S::PASSES; ++j) {
+      const int r = j * S::RPP + rt;
+      if (m.src[r] != kNoRow) amax = fmaxf(amax, fminf(row_amax<KV>(c[v][j]) * m.scale[v][r], kMaxFinite));
+    }
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));  // magnitudes order as integers
+    if (lane == 0) m.red[v][tid >> 5] = top;
   }
-  if (tid == 0) *sp = s;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    uint32_t all = 0u;
+#pragma unroll
+    for (int w = 0; w < S::NT / 32; ++w) all = max(all, m.red[v][w]);
+    const float s_old = kept ? (v ? was.y : was.x) : 0.f, s = fmaxf(s_old, scale_for<KV>(__uint_as_float(all)));
+#pragma unroll
+    for (int j = 0; j < S::PASSES; ++j) {
+      const int r = j * S::RPP + rt;
+      uint4* at = reinterpret_cast<uint4*>(pool[v] + (to * PAGE + r) * D + li * 16);
+      if (m.src[r] != kNoRow) {
+        const float from = m.scale[v][r];
+        *at = s == from ? c[v][j] : s > 0.f ? rescale16<KV>(c[v][j], __fdiv_rn(from, s)) : make_uint4(0u, 0u, 0u, 0u);
+      } else if (r < end && s > s_old && kept) {
+        *at = rescale16<KV>(*at, __fdiv_rn(s_old, s));
+      }
+    }
+    if (tid == 0) (v ? pc.v_scale : pc.k_scale)[to] = s;
+  }
 }
 
 // ---------------------------------------------------------------- eviction
@@ -124,24 +133,54 @@ struct EvictPlan {
   int32_t* dst;     // [lines][cap]
   int32_t* src;     // [lines][cap]
   float* edge;      // [B][G][2]: scales of the block of slot `keep` before the moves
-  int lines_per_b, blocks, cap;
+  uint32_t* key;    // [lines][pitch]: weights in the order of integers, kNoKey: no memory
+  int32_t* place;   // [lines][pitch] positions, where recent > 0
+  int lines_per_b, blocks, cap, pitch;
 };
 
-constexpr int kSelThreads = 1024, kBins = 2048, kFly = 8;
-constexpr int kMaxWords = 40960;  // of a CTA's keys (and positions) in shared memory; the others are read again
+// Keys of the slots, a thread each. Weights that are not negative order as integers;
+// negative ones and NaN count as 0.
+constexpr uint32_t kNoKey = 0xFFFFFFFFu;
+constexpr int kRankThreads = 256;
+
+__global__ void __launch_bounds__(kRankThreads) paged_rank_kernel(const PagedEvictParams p, const EvictPlan plan) {
+  grid_dependents();
+  grid_wait();
+  const int b = blockIdx.z, hl = blockIdx.y, slot = blockIdx.x * kRankThreads + threadIdx.x;
+  const int len = *(p.lens + b), G = p.c.G, page = p.c.page;
+  if (len <= p.keep || slot >= len || (int64_t)len > (int64_t)p.c.max_pages * page) return;
+  const int pid = paged_page(p.c, b, slot / page);
+  const int64_t row = ((int64_t)max(pid, 0) * G + hl) * page + slot % page;
+  float w;
+  if (p.per_head) {
+    w = p.weight[row];
+  } else {
+    double sum = 0.0;
+#pragma unroll 8
+    for (int g = 0; g < G; ++g) sum += (double)p.weight[row + (int64_t)g * page];
+    w = (float)sum;
+  }
+  const int64_t at = ((int64_t)b * plan.lines_per_b + hl) * plan.pitch + slot;
+  plan.key[at] = pid < 0 ? kNoKey : w > 0.f ? __float_as_uint(w) : 0u;
+  if (p.recent > 0) plan.place[at] = p.position[row];
+}
+
+constexpr int kSelThreads = 1024, kBins = 2048;
+constexpr int kMaxWords = 40960;  // of a CTA's keys in shared memory; longer runs are read from the workspace
 
 struct SelShared {
   uint32_t hist[2][kBins];
-  uint32_t scan[kSelThreads / 32 + 1];
+  uint32_t xch[4][8];   // what the cluster's other CTAs read, a row per exchange (16-byte aligned)
   uint32_t red[kSelThreads / 32][8];
-  uint32_t xch[8][8];   // what the cluster's other CTAs read, one row per exchange
-  uint32_t at[3];
+  uint32_t scan[kSelThreads / 32];
+  uint32_t at[4];
 };
 
 constexpr size_t kMostShared = sizeof(SelShared) + kMaxWords * 4 + kEvictSlots / 8 / 32 * 12;
 static_assert(kMostShared <= 227 * 1024, "a CTA's shared memory");
 
 // Sum over the CTA's threads before this one, and the sum of all.
+template <int NT>
 SPATTEN_DEV uint32_t block_scan(SelShared& sh, uint32_t x, uint32_t& total) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t y = x;
@@ -156,7 +195,7 @@ SPATTEN_DEV uint32_t block_scan(SelShared& sh, uint32_t x, uint32_t& total) {
   uint32_t before = 0u;
   total = 0u;
 #pragma unroll
-  for (int w = 0; w < kSelThreads / 32; ++w) {
+  for (int w = 0; w < NT / 32; ++w) {
     if (w < warp) before += sh.scan[w];
     total += sh.scan[w];
   }
@@ -169,13 +208,18 @@ SPATTEN_DEV uint32_t lowest_bits(uint32_t t, uint32_t m) {
   return t;
 }
 
-__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEvictParams p, const EvictPlan plan,
+// The largest cluster, whose loops over CTAs are unrolled: their loads from the
+// others' shared memory go out together.
+constexpr int kCluster = 8;
+
+// CACHED: a run's keys (and positions) fit the shared memory.
+template <bool CACHED, int NT>
+__global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams p, const EvictPlan plan,
                                                                    int run, int cached) {
   extern __shared__ __align__(16) uint8_t dsm[];
   SelShared& sh = *reinterpret_cast<SelShared*>(dsm);
   uint32_t* keys = reinterpret_cast<uint32_t*>(dsm + sizeof(SelShared));  // [cached]
-  int* posn = reinterpret_cast<int*>(keys + cached);                       // [cached] where recent > 0
-  uint32_t* prot = keys + (p.recent > 0 ? 2 : 1) * cached;                 // [run / 32]: recent
+  uint32_t* prot = keys + cached;                                          // [run / 32]: recent
   uint32_t* kept = prot + run / 32;                                        // [run / 32]
   uint32_t* ties = kept + run / 32;                                        // [run / 32]
   grid_dependents();
@@ -196,77 +240,29 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
   }
   const int lo = min(rank * run, len), n = min(run, len - lo), words = (n + 31) / 32;
 
-  // Slots i of this CTA's run, kFly of them at once: ordered keys (weights order as
-  // integers; negative ones and NaN count as 0), positions, and whether they have memory.
-  auto load = [&](const int (&i)[kFly], uint32_t (&k)[kFly], int (&pos)[kFly]) {
-    int64_t row[kFly];
-    bool all = true;
-#pragma unroll
-    for (int u = 0; u < kFly; ++u) {
-      const int slot = lo + i[u], pid = i[u] < n ? paged_page(p.c, b, slot >> page_log) : 0;
-      all &= pid >= 0;
-      row[u] = ((int64_t)max(pid, 0) * G + hl) * page + (slot & (page - 1));
-    }
-    double sum[kFly];
-#pragma unroll
-    for (int u = 0; u < kFly; ++u) {
-      k[u] = 0u;
-      pos[u] = 0;
-      sum[u] = 0.0;
-      if (i[u] < n && p.recent > 0) pos[u] = p.position[row[u]];
-      if (i[u] < n && p.per_head) sum[u] = p.weight[row[u]];
-    }
-    if (!p.per_head) {
-#pragma unroll 2
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int u = 0; u < kFly; ++u)
-          if (i[u] < n) sum[u] += (double)p.weight[row[u] + (int64_t)g * page];
-    }
-#pragma unroll
-    for (int u = 0; u < kFly; ++u) {
-      const float w = (float)sum[u];
-      if (w > 0.f) k[u] = __float_as_uint(w);
-    }
-    return all;
-  };
-  auto reload = [&](int at, int& pos) {  // of one that the shared memory did not hold
-    int i[kFly], x[kFly];
-    uint32_t k[kFly];
-#pragma unroll
-    for (int u = 0; u < kFly; ++u) i[u] = u == 0 ? at : n;
-    load(i, k, x);
-    pos = x[0];
-    return k[0];
-  };
-  auto key = [&](int i) {
-    int pos;
-    return i < cached ? keys[i] : reload(i, pos);
-  };
-  auto position = [&](int i) {
-    int pos;
-    if (i < cached) return posn[i];
-    reload(i, pos);
-    return pos;
-  };
+  const uint32_t* const key_at = plan.key + line * plan.pitch + lo;
+  const int32_t* const place_at = plan.place + line * plan.pitch + lo;
+  auto key = [&](int i) { return CACHED ? keys[i] : key_at[i]; };
 
-  // keys, the newest position, whether every slot has memory
+  // keys, the newest position, whether every slot has memory (pitch and runs are multiples of 32)
   int newest = INT_MIN;
   bool hole = false;
-  for (int base = tid; base < n; base += kSelThreads * kFly) {
-    int i[kFly], pos[kFly];
-    uint32_t k[kFly];
+#pragma unroll 4
+  for (int i = 4 * tid; i < n; i += 4 * NT) {
+    const uint4 k = *reinterpret_cast<const uint4*>(key_at + i);
+    const uint32_t x[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-    for (int u = 0; u < kFly; ++u) i[u] = base + u * kSelThreads;
-    hole |= !load(i, k, pos);
+    for (int j = 0; j < 4; ++j) hole |= i + j < n && x[j] == kNoKey;
+    if (CACHED) *reinterpret_cast<uint4*>(keys + i) = k;
+  }
+  if (p.recent > 0) {
+#pragma unroll 4
+    for (int i = 4 * tid; i < n; i += 4 * NT) {
+      const int4 k = *reinterpret_cast<const int4*>(place_at + i);
+      const int x[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-    for (int u = 0; u < kFly; ++u) {
-      if (i[u] >= n) break;
-      newest = max(newest, pos[u]);
-      if (i[u] < cached) {
-        keys[i[u]] = k[u];
-        if (p.recent > 0) posn[i[u]] = pos[u];
-      }
+      for (int j = 0; j < 4; ++j)
+        if (i + j < n) newest = max(newest, x[j]);
     }
   }
   {
@@ -280,7 +276,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
     if (tid == 0) {
       int m = INT_MIN;
       uint32_t h = 0u;
-      for (int w = 0; w < kSelThreads / 32; ++w) {
+      for (int w = 0; w < NT / 32; ++w) {
         m = max(m, (int)sh.red[w][0]);
         h |= sh.red[w][1];
       }
@@ -290,10 +286,12 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
     cl.sync();
     uint32_t h = 0u;
     newest = INT_MIN;
-    for (int r = 0; r < CL; ++r) {
-      const uint32_t* x = cl.map_shared_rank(&sh.xch[0][0], r);
-      newest = max(newest, (int)x[0]);
-      h |= x[1];
+#pragma unroll
+    for (int r = 0; r < kCluster; ++r) {
+      if (r >= CL) continue;
+      const uint2 x = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.xch[0][0], r));
+      newest = max(newest, (int)x.x);
+      h |= x.y;
     }
     if (h) {  // left as it is
       if (rank == 0 && tid == 0) {
@@ -307,11 +305,12 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
   // the recent ones; how many they are, and the range of the keys of both classes
   {
     uint32_t cnt = 0u, lo0 = 0xFFFFFFFFu, hi0 = 0u, lo1 = 0xFFFFFFFFu, hi1 = 0u;
-    for (int base = 0; base < words * 32; base += kSelThreads) {
+#pragma unroll 4
+    for (int base = 0; base < words * 32; base += NT) {
       const int i = base + tid;
       bool r = false;
       if (i < n) {
-        if (p.recent > 0) r = (int64_t)position(i) > (int64_t)newest - p.recent;
+        if (p.recent > 0) r = (int64_t)place_at[i] > (int64_t)newest - p.recent;
         const uint32_t k = key(i);
         if (r) {
           lo1 = min(lo1, k);
@@ -341,24 +340,34 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
     __syncthreads();
     if (tid == 0) {
       uint32_t x[5] = {0u, 0xFFFFFFFFu, 0u, 0xFFFFFFFFu, 0u};
-      for (int w = 0; w < kSelThreads / 32; ++w) {
+#pragma unroll 8
+      for (int w = 0; w < NT / 32; ++w) {
         x[0] += sh.red[w][0];
         x[1] = min(x[1], sh.red[w][1]);
         x[2] = max(x[2], sh.red[w][2]);
         x[3] = min(x[3], sh.red[w][3]);
         x[4] = max(x[4], sh.red[w][4]);
       }
+#pragma unroll
       for (int i = 0; i < 5; ++i) sh.xch[1][i] = x[i];
     }
     cl.sync();
   }
-  uint32_t recents = 0u, k_lo = 0xFFFFFFFFu, k_hi = 0u;
-  for (int r = 0; r < CL; ++r) recents += cl.map_shared_rank(&sh.xch[1][0], r)[0];
+  uint32_t recents = 0u, r_lo = 0xFFFFFFFFu, r_hi = 0u, k_lo = 0xFFFFFFFFu, k_hi = 0u;
+#pragma unroll
+  for (int r = 0; r < kCluster; ++r) {
+    if (r >= CL) continue;
+    const uint4 x = *reinterpret_cast<const uint4*>(cl.map_shared_rank(&sh.xch[1][0], r));
+    recents += x.x;
+    k_lo = min(k_lo, x.y);
+    k_hi = max(k_hi, x.z);
+    r_lo = min(r_lo, x.w);
+    r_hi = max(r_hi, *cl.map_shared_rank(&sh.xch[1][4], r));
+  }
   const bool cls = recents >= (uint32_t)keep;  // the class that is chosen from: the recent ones, or the others
-  for (int r = 0; r < CL; ++r) {
-    const uint32_t* x = cl.map_shared_rank(&sh.xch[1][0], r);
-    k_lo = min(k_lo, x[cls ? 3 : 1]);
-    k_hi = max(k_hi, x[cls ? 4 : 2]);
+  if (cls) {
+    k_lo = r_lo;
+    k_hi = r_hi;
   }
   uint32_t need = cls ? keep : keep - recents;  // of the class; its largest keys
   // radix rounds: keys above k_hi are kept, the need-th largest lies in [k_lo, k_hi]
@@ -367,24 +376,34 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
     const uint32_t span = k_hi - k_lo;
     const int shift = span < (uint32_t)kBins ? 0 : 32 - __clz(span) - 11;
     uint32_t* hist = sh.hist[round & 1];
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0u;
+    for (int i = tid; i < kBins; i += NT) hist[i] = 0u;
     __syncthreads();
-    for (int i = tid; i < n; i += kSelThreads) {
+#pragma unroll 4
+    for (int i = tid; i < n; i += NT) {
       const uint32_t k = key(i);
       if (((prot[i >> 5] >> (i & 31)) & 1u) == (uint32_t)cls && k >= k_lo && k <= k_hi) atomicAdd(&hist[(k - k_lo) >> shift], 1u);
     }
     cl.sync();
-    // bins from the top: thread t takes the bins kBins - 1 - 4 t ..
-    constexpr int PER = kBins / kSelThreads;
+    // bins from the top: thread t takes the PER bins that end at kBins - 1 - PER t
+    constexpr int PER = kBins / NT;
     uint32_t c[PER], mine = 0u;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      c[j] = 0u;
-      for (int r = 0; r < CL; ++r) c[j] += cl.map_shared_rank(hist, r)[kBins - 1 - (tid * PER + j)];
-      mine += c[j];
+    for (int j = 0; j < PER; ++j) c[j] = 0u;
+#pragma unroll
+    for (int r = 0; r < kCluster; ++r) {
+      if (r >= CL) continue;
+      const uint2* x = reinterpret_cast<const uint2*>(cl.map_shared_rank(hist, r) + kBins - PER - PER * tid);
+#pragma unroll
+      for (int j = 0; j < PER; j += 2) {
+        const uint2 y = x[j / 2];
+        c[PER - 1 - j] += y.x;
+        c[PER - 2 - j] += y.y;
+      }
     }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) mine += c[j];
     uint32_t total;
-    uint32_t above = block_scan(sh, mine, total);
+    uint32_t above = block_scan<NT>(sh, mine, total);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       if (above < need && need <= above + c[j]) {
@@ -412,7 +431,8 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
   }
   // kept for sure, and the ones of the border's key
   uint32_t n_ties = 0u;
-  for (int base = 0; base < words * 32; base += kSelThreads) {
+#pragma unroll 2
+  for (int base = 0; base < words * 32; base += NT) {
     const int i = base + tid;
     bool sure = false, tie = false;
     if (i < n) {
@@ -430,19 +450,21 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
   }
   {
     uint32_t total;
-    block_scan(sh, n_ties, total);
+    block_scan<NT>(sh, n_ties, total);
     if (tid == 0) sh.xch[2][0] = total;
     cl.sync();
   }
   uint32_t before = 0u;
-  for (int r = 0; r < rank; ++r) before += cl.map_shared_rank(&sh.xch[2][0], r)[0];
+#pragma unroll
+  for (int r = 0; r < kCluster; ++r)
+    if (r < rank) before += *cl.map_shared_rank(&sh.xch[2][0], r);
   uint32_t left = whole || before >= need ? 0u : need - before;  // ties that this CTA's slots may still keep
   uint32_t n_dst = 0u, n_src = 0u;
-  for (int base = 0; base < words; base += kSelThreads) {
+  for (int base = 0; base < words; base += NT) {
     const int w = base + tid;
     const uint32_t t = w < words ? ties[w] : 0u;
     uint32_t total;
-    const uint32_t at = block_scan(sh, __popc(t), total);
+    const uint32_t at = block_scan<NT>(sh, __popc(t), total);
     if (w < words) {
       const uint32_t k = kept[w] | (at < left ? lowest_bits(t, left - at) : 0u);
       kept[w] = k;
@@ -455,8 +477,8 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
   }
   {
     uint32_t td, ts;
-    block_scan(sh, n_dst, td);
-    block_scan(sh, n_src, ts);
+    block_scan<NT>(sh, n_dst, td);
+    block_scan<NT>(sh, n_src, ts);
     if (tid == 0) {
       sh.xch[3][0] = td;
       sh.xch[3][1] = ts;
@@ -464,31 +486,43 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
     cl.sync();
   }
   uint32_t d0 = 0u, s0 = 0u, moves = 0u;
-  for (int r = 0; r < CL; ++r) {
-    const uint32_t* x = cl.map_shared_rank(&sh.xch[3][0], r);
+#pragma unroll
+  for (int r = 0; r < kCluster; ++r) {
+    if (r >= CL) continue;
+    const uint2 x = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.xch[3][0], r));
     if (r < rank) {
-      d0 += x[0];
-      s0 += x[1];
+      d0 += x.x;
+      s0 += x.y;
     }
-    moves += x[0];
+    moves += x.x;
   }
   int32_t* const dst = plan.dst + line * plan.cap;
   int32_t* const src = plan.src + line * plan.cap;
   int32_t* const first = plan.first + line * (plan.blocks + 1);
-  for (int base = 0; base < words; base += kSelThreads) {
-    const int w = base + tid;
+  auto front_of = [&](int w) {  // slots before `keep` of a word
     const int at = lo + 32 * w;
-    const uint32_t k = w < words ? kept[w] : 0u;
-    const uint32_t front = w >= words || at >= keep ? 0u : at + 32 <= keep ? 0xFFFFFFFFu : (1u << (keep - at)) - 1u;
-    uint32_t free = front & ~k, move = w < words ? k & ~front : 0u, td, ts;
-    uint32_t d = d0 + block_scan(sh, __popc(free), td), s = s0 + block_scan(sh, __popc(move), ts);
+    return at + 32 <= keep ? 0xFFFFFFFFu : at >= keep ? 0u : (1u << (keep - at)) - 1u;
+  };
+  for (int base = 0; base < words; base += NT) {  // numbers of the words' first free and moving slots
+    const int w = base + tid;
+    const uint32_t k = w < words ? kept[w] : 0u, front = w < words ? front_of(w) : 0u;
+    uint32_t td, ts;
+    const uint32_t d = d0 + block_scan<NT>(sh, __popc(front & ~k), td), s = s0 + block_scan<NT>(sh, __popc(k & ~front), ts);
     d0 += td;
     s0 += ts;
-    if (front)
-      for (int o = 0; o < 32; o += 16)  // (pages are multiples of 16)
-        if (((at + o) & (page - 1)) == 0 && at + o < keep) first[(at + o) >> page_log] = d + __popc(free & ((1u << o) - 1u));
-    for (; free; free &= free - 1u) dst[d++] = at + __ffs(free) - 1;
-    for (; move; move &= move - 1u) src[s++] = at + __ffs(move) - 1;
+    if (w < words) {
+      prot[w] = d;
+      ties[w] = s;
+    }
+  }
+  __syncthreads();
+  for (int w = warp; w < words; w += NT / 32) {  // a slot per lane
+    const int slot = lo + 32 * w + lane;
+    const uint32_t k = kept[w], front = front_of(w), free = front & ~k, move = k & ~front, before_me = (1u << lane) - 1u;
+    const uint32_t d = prot[w] + __popc(free & before_me);
+    if ((free >> lane) & 1u) dst[d] = slot;
+    if ((move >> lane) & 1u) src[ties[w] + __popc(move & before_me)] = slot;
+    if (slot < keep && (slot & (page - 1)) == 0) first[slot >> page_log] = d;
   }
   if (rank == 0) {
     if (tid == 0) {
@@ -498,7 +532,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
     }
     // the block of slot `keep` may change its scale while others read its tokens
     const int g0 = p.per_head ? hl : 0, g1 = p.per_head ? hl + 1 : G;
-    for (int g = g0 + tid; g < g1; g += kSelThreads) {
+    for (int g = g0 + tid; g < g1; g += NT) {
       const int64_t blk = (int64_t)paged_page(p.c, b, keep >> page_log) * G + g;
       float* e = plan.edge + ((int64_t)b * G + g) * 2;
       e[0] = p.c.k_scale[blk];
@@ -508,6 +542,10 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedEv
   cl.sync();  // no CTA leaves while its shared memory is read
 }
 
+// A CTA takes kMoveBlocks blocks of a KV head, K and V: most of them may keep what they
+// have, and a CTA for each took longer to find that out than the moves.
+constexpr int kMoveBlocks = 4;
+
 template <int KV, int D, int PAGE>
 __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_move_kernel(const PagedEvictParams p,
                                                                            const EvictPlan plan) {
@@ -515,40 +553,54 @@ __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_move_kernel(cons
   __shared__ MoveRows<PAGE> m;
   grid_dependents();
   grid_wait();
-  const int b = blockIdx.z, G = p.c.G, tid = threadIdx.x, blk = blockIdx.x;
-  const bool isk = (int)blockIdx.y < G;
-  const int g = isk ? blockIdx.y : blockIdx.y - G;
+  const int b = blockIdx.z, g = blockIdx.y, G = p.c.G, tid = threadIdx.x, blk0 = blockIdx.x * kMoveBlocks;
   const int64_t line = (int64_t)b * plan.lines_per_b + (p.per_head ? g : 0);
-  if (blk == 0 && blockIdx.y == 0 && tid == 0) p.new_lens[b] = plan.head[line * 4 + 1];
+  if (blk0 == 0 && g == 0 && tid == 0) p.new_lens[b] = plan.head[line * 4 + 1];
   if (plan.head[line * 4] == 0) return;
-  const int32_t* first = plan.first + line * (plan.blocks + 1);
-  const int f0 = first[blk], f1 = first[blk + 1];
-  if (f1 <= f0) return;
-  const int end = min(p.keep - blk * PAGE, PAGE), edge = p.keep / PAGE;
-  const float edge_scale = plan.edge[((int64_t)b * G + g) * 2 + (isk ? 0 : 1)];
-  float* const scales = isk ? p.c.k_scale : p.c.v_scale;
-  uint8_t* const pool = isk ? p.c.k : p.c.v;
-  for (int r = tid; r < PAGE; r += S::NT) m.src[r] = kNoRow;
-  __syncthreads();
-  const int64_t to = (int64_t)paged_page(p.c, b, blk) * G + g;
-  for (int i = f0 + tid; i < f1; i += S::NT) {
-    const int d = plan.dst[line * plan.cap + i] - blk * PAGE, s = plan.src[line * plan.cap + i];
-    const int64_t from = (int64_t)paged_page(p.c, b, s / PAGE) * G + g, row = from * PAGE + s % PAGE;
-    m.src[d] = (uint32_t)row;
-    m.scale[d] = s / PAGE == edge ? edge_scale : scales[from];
-    if (isk) {
+  const int32_t* first = plan.first + line * (plan.blocks + 1) + blk0;
+  int f[kMoveBlocks + 1];
+#pragma unroll
+  for (int i = 0; i <= kMoveBlocks; ++i) f[i] = first[min(i, plan.blocks - blk0)];
+  const int edge = p.keep / PAGE;
+#pragma unroll 1
+  for (int i = 0; i < kMoveBlocks; ++i) {
+    const int blk = blk0 + i, f0 = f[0], f1 = f[1];
+#pragma unroll
+    for (int k = 0; k < kMoveBlocks; ++k) f[k] = f[k + 1];
+    if (f1 <= f0) continue;
+    const int end = min(p.keep - blk * PAGE, PAGE);
+    __syncthreads();  // the block before is through with m
+    for (int r = tid; r < PAGE; r += S::NT) m.src[r] = kNoRow;
+    __syncthreads();
+    const int64_t to = (int64_t)paged_page(p.c, b, blk) * G + g;
+    int d = 0;  // a move per thread
+    int64_t from = 0;
+    bool at_edge = false;
+    const bool mine = f0 + tid < f1;
+    if (mine) {
+      const int s = plan.src[line * plan.cap + f0 + tid];
+      d = plan.dst[line * plan.cap + f0 + tid] - blk * PAGE;
+      from = (int64_t)paged_page(p.c, b, s / PAGE) * G + g;
+      at_edge = s / PAGE == edge;
+      const int64_t row = from * PAGE + s % PAGE;
+      m.src[d] = (uint32_t)row;
       p.weight[to * PAGE + d] = p.weight[row];
       p.position[to * PAGE + d] = p.position[row];
     }
+    const float2 edge_scale = *reinterpret_cast<const float2*>(plan.edge + ((int64_t)b * G + g) * 2);
+    if (mine) {
+      m.scale[0][d] = at_edge ? edge_scale.x : p.c.k_scale[from];
+      m.scale[1][d] = at_edge ? edge_scale.y : p.c.v_scale[from];
+    }
+    const float2 was = blk == edge ? edge_scale : make_float2(p.c.k_scale[to], p.c.v_scale[to]);
+    __syncthreads();
+    move_block<KV, D, PAGE>(m, p.c, to, was, f1 - f0 < end, end);
   }
-  const float was = blk == edge ? edge_scale : scales[to];
-  __syncthreads();
-  move_block<KV, D, PAGE>(m, pool, pool + to * (PAGE * D), scales + to, was, f1 - f0 < end, end);
 }
 
 // ---------------------------------------------------------------- accepted tokens
 
-// A CTA per (K or V head, sequence) walks the blocks that accepted tokens move into, in
+// A CTA per (KV head, sequence) walks the blocks that accepted tokens move into, in
 // order: what it reads lies at or behind what it writes.
 template <int KV, int D, int PAGE>
 __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_keep_kernel(const PagedKeepParams p) {
@@ -557,9 +609,7 @@ __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_keep_kernel(cons
   __shared__ int stop, moved, fixed;
   grid_dependents();
   grid_wait();
-  const int b = blockIdx.y, G = p.c.G, tid = threadIdx.x;
-  const bool isk = (int)blockIdx.x < G;
-  const int g = isk ? blockIdx.x : blockIdx.x - G;
+  const int b = blockIdx.y, g = blockIdx.x, G = p.c.G, tid = threadIdx.x;
   const PagedSeq sq = paged_seq(p.b, p.c, b);
   const int32_t* acc = p.accepted + (int64_t)b * p.accepted_st;
   // the list ends at the first entry that is not above the one before it, is no new token, or has no memory
@@ -579,8 +629,6 @@ __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_keep_kernel(cons
     if (acc[j] != j) atomicMin(&fixed, j);
   __syncthreads();
   if (fixed >= count) return;
-  float* const scales = isk ? p.c.k_scale : p.c.v_scale;
-  uint8_t* const pool = isk ? p.c.k : p.c.v;
   const int slot0 = sq.old + fixed, slot1 = sq.old + count;  // slots that tokens move into
   for (int blk = slot0 / PAGE; blk * PAGE < slot1; ++blk) {
     const int lo = max(slot0 - blk * PAGE, 0), hi = min(slot1 - blk * PAGE, PAGE);
@@ -593,12 +641,13 @@ __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_keep_kernel(cons
         const int s = sq.old + acc[blk * PAGE + r - sq.old];
         const int64_t from = (int64_t)paged_page(p.c, b, s / PAGE) * G + g, row = from * PAGE + s % PAGE;
         m.src[r] = (uint32_t)row;
-        m.scale[r] = scales[from];
+        m.scale[0][r] = p.c.k_scale[from];
+        m.scale[1][r] = p.c.v_scale[from];
       }
     }
-    const float was = scales[to];
+    const float2 was = make_float2(p.c.k_scale[to], p.c.v_scale[to]);
     __syncthreads();
-    if (isk && p.weight) {  // a row per thread, read before any is written
+    if (p.weight) {  // a row per thread, read before any is written
       const int r = lo + tid;
       const float w = r < hi ? p.weight[m.src[r]] : 0.f;
       const int x = r < hi ? p.position[m.src[r]] : 0;
@@ -608,13 +657,13 @@ __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_keep_kernel(cons
         p.position[to * PAGE + r] = x;
       }
     }
-    move_block<KV, D, PAGE>(m, pool, pool + to * (PAGE * D), scales + to, was, lo > 0, lo);
+    move_block<KV, D, PAGE>(m, p.c, to, was, lo > 0, lo);
     __syncthreads();  // the block is written, its list read
   }
 }
 
 struct EvictSplit {
-  int cluster, run, cached;
+  int cluster, run, cached, threads;
   size_t smem;
 };
 
@@ -623,11 +672,11 @@ EvictSplit split_for(const PagedEvictParams& p, int n_sm) {
   EvictSplit s;
   const int64_t lines = (int64_t)p.B * (p.per_head ? p.c.G : 1);
   s.cluster = 1;
-  while (s.cluster < 8 && slots > (int64_t)s.cluster * (lines * s.cluster < n_sm ? 2048 : 16384)) s.cluster *= 2;
+  while (s.cluster < kCluster && slots > (int64_t)s.cluster * (lines * s.cluster < n_sm ? 2048 : 16384)) s.cluster *= 2;
   s.run = (int)((slots + s.cluster - 1) / s.cluster + 31) / 32 * 32;
-  const int arrays = p.recent > 0 ? 2 : 1;
-  s.cached = s.run < kMaxWords / arrays ? s.run : kMaxWords / arrays;
-  s.smem = sizeof(SelShared) + (size_t)s.cached * arrays * 4 + (size_t)s.run / 32 * 12;
+  s.cached = s.run <= kMaxWords ? s.run : 0;
+  s.threads = lines * s.cluster > n_sm && s.run <= 16384 ? 512 : 1024;
+  s.smem = sizeof(SelShared) + (size_t)s.cached * 4 + (size_t)s.run / 32 * 12;
   return s;
 }
 
@@ -653,17 +702,21 @@ size_t plan_for(const PagedEvictParams& p, void* ws, EvictPlan& x) {
   x.dst = reinterpret_cast<int32_t*>(take(lines * x.cap * 4));
   x.src = reinterpret_cast<int32_t*>(take(lines * x.cap * 4));
   x.edge = reinterpret_cast<float*>(take((size_t)p.B * p.c.G * 8));
+  x.pitch = (int)((slots + 31) / 32 * 32);
+  x.key = reinterpret_cast<uint32_t*>(take(lines * x.pitch * 4));
+  x.place = reinterpret_cast<int32_t*>(take(p.recent > 0 ? lines * x.pitch * 4 : 0));
   return at;
 }
 
 template <int KV, int D, int PAGE>
 cudaError_t move_launch(const PagedEvictParams& p, const EvictPlan& plan, cudaStream_t st) {
-  return launch_dependent(paged_move_kernel<KV, D, PAGE>, dim3(plan.blocks, 2 * p.c.G, p.B), MoveShape<D, PAGE>::NT, 0,
-                          st, p, plan);
+  return launch_dependent(paged_move_kernel<KV, D, PAGE>,
+                          dim3((plan.blocks + kMoveBlocks - 1) / kMoveBlocks, p.c.G, p.B), MoveShape<D, PAGE>::NT, 0, st, p,
+                          plan);
 }
 template <int KV, int D, int PAGE>
 cudaError_t keep_launch(const PagedKeepParams& p, cudaStream_t st) {
-  return launch_dependent(paged_keep_kernel<KV, D, PAGE>, dim3(2 * p.c.G, p.b.B), MoveShape<D, PAGE>::NT, 0, st, p);
+  return launch_dependent(paged_keep_kernel<KV, D, PAGE>, dim3(p.c.G, p.b.B), MoveShape<D, PAGE>::NT, 0, st, p);
 }
 
 // f(KV, D, PAGE) as constants
@@ -686,21 +739,21 @@ cudaError_t with_shape(int kv, int D, int page, F f) {
   return kv == kKvInt8 ? dims(std::integral_constant<int, kKvInt8>{}) : dims(std::integral_constant<int, kKvE4m3>{});
 }
 
-cudaError_t select_launch(const PagedEvictParams& p, const EvictPlan& plan, int n_sm, cudaStream_t st) {
-  const EvictSplit s = split_for(p, n_sm);
+template <bool CACHED, int NT>
+cudaError_t select_launch(const PagedEvictParams& p, const EvictPlan& plan, const EvictSplit& s, cudaStream_t st) {
   static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
-    e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(paged_select_kernel<CACHED, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)kMostShared);
     if (e != cudaSuccess) return e;
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(s.cluster, plan.lines_per_b, p.B);
-  cfg.blockDim = dim3(kSelThreads);
+  cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = s.smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2] = {};
@@ -711,7 +764,7 @@ cudaError_t select_launch(const PagedEvictParams& p, const EvictPlan& plan, int 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, paged_select_kernel, p, plan, s.run, s.cached);
+  return cudaLaunchKernelEx(&cfg, paged_select_kernel<CACHED, NT>, p, plan, s.run, s.cached);
 }
 
 }  // namespace
@@ -724,7 +777,12 @@ size_t paged_evict_workspace(const PagedEvictParams& p) {
 cudaError_t launch_paged_evict(const PagedEvictParams& p, int kv, void* ws, int n_sm, cudaStream_t st) {
   EvictPlan plan;
   plan_for(p, ws, plan);
-  const cudaError_t e = select_launch(p, plan, n_sm, st);
+  const dim3 slots((unsigned)((plan.pitch + kRankThreads - 1) / kRankThreads), plan.lines_per_b, p.B);
+  cudaError_t e = launch_dependent(paged_rank_kernel, slots, kRankThreads, 0, st, p, plan);
+  if (e != cudaSuccess) return e;
+  const EvictSplit s = split_for(p, n_sm);
+  if (s.cached == 0) e = select_launch<false, 1024>(p, plan, s, st);
+  else e = s.threads == 1024 ? select_launch<true, 1024>(p, plan, s, st) : select_launch<true, 512>(p, plan, s, st);
   if (e != cudaSuccess) return e;
   return with_shape(kv, p.c.D, p.c.page, [&](auto k, auto d, auto page) {
     return move_launch<decltype(k)::value, decltype(d)::value, decltype(page)::value>(p, plan, st);
