@@ -406,7 +406,7 @@ int spatten_paged_tree(const spatten_paged_tree_args* a, void* stream);
  *    tokens, and of these the ones whose bits are set in its words (whether
  *    before or behind it; bits from n_b on count as clear);
  *  * weight, position (optional, together; fp32 and int32 [num_pages, G,
- *    page_size] beside the pool): the softmax weights that the call's rows give
+ *    page_size] beside the pool, 16-byte aligned): the softmax weights that the call's rows give
  *    a slot, summed in fp32 over the rows and the H / G heads of its KV head, are
  *    added to its weight. The slots of the new tokens start from 0 and take
  *    positions[row] (int32 [T]; NULL: the slot) as their position. The slots

@@ -592,8 +592,8 @@ static int check_tree(const char* who, const void* tree, int64_t stride, int wor
 // accumulated weights and positions: both or neither
 static int check_weights(const char* who, const float* weight, const int32_t* position) {
   if (!weight != !position) return fail(SPATTEN_ERR_INVALID, "%s: one of weight, position", who);
-  if (!aligned(weight, 4) || !aligned(position, 4))
-    return fail(SPATTEN_ERR_INVALID, "%s: weight/position not 4-byte aligned", who);
+  if (!aligned(weight, 16) || !aligned(position, 16))
+    return fail(SPATTEN_ERR_INVALID, "%s: weight/position not 16-byte aligned", who);
   return SPATTEN_OK;
 }
 

@@ -775,6 +775,15 @@ namespace {
 // own, so that single tokens beside a prompt's piece keep the kernel made for
 // them (512 new tokens over 4096 take 63 us, 47 single ones over 4000 76, together
 // 150).
+//
+// A tree's rows (which are many for the tokens they come from) stay here while their
+// work, in tiles of 16 rows x 16 keys over the whole page table, is small: at 32 / 8
+// heads x 128 (int8) 26 tokens of one sequence over 777 keys (2744 tiles) take 28.5 us
+// there and 15.3 here, over 3000 (10528) 30.3 and 22.5, over 6000 (21000) 35.3 and 32.4, 64
+// tokens over 3000 (24064) 35.4 and 37.1, of four sequences over 777 26.6 and 28.7 with
+// 26 tokens (10976) and 36 and 64 with 64 over 1500 (48128).
+constexpr double kFewTiles = 12000;
+
 struct Plan {
   PagedAttendParams tc, few;
   bool use_tc, use_few;
@@ -785,6 +794,8 @@ Plan plan_for(const PagedAttendParams& p) {
   x.tc.rows_over = x.few.rows_over = 0;
   x.tc.rows_upto = x.few.rows_upto = INT64_MAX;
   if (!paged_attend_tc_takes(p)) return x;
+  const double lines = ((double)p.b.T * (p.b.H / p.c.G) / 16 + p.b.B) * p.c.G;
+  if (p.tree && lines * p.c.max_pages * (p.c.page / 16) <= kFewTiles) return x;
   x.use_tc = true;
   x.use_few = p.b.B > 1 && p.b.T < (int64_t)p.b.B * p.b.max_tokens;
   if (x.use_few) x.tc.rows_over = x.few.rows_upto = kTcRows;

@@ -33,94 +33,112 @@ namespace {
 
 using namespace sm100;
 
-// ---------------------------------------------------------------- few rows: kept scores
+// ---------------------------------------------------------------- slots
 
-constexpr int kSlotThreads = 256;
+// The kernels that write weights: a thread takes four slots (of one page), so that it
+// has 16 bytes of their weights in each access, and a CTA a group of heads.
+constexpr int kSlotThreads = 256, kQuad = 4, kSlotsCta = kSlotThreads * kQuad;
 
-// A slot's weights: what all its heads share.
-struct WeighSlot {
-  int64_t row;   // of head 0
-  bool fresh;    // a new token's
-  int position;
+struct WeighSlots {
+  int slot, lim;  // the first one; the sequence's end
+  int old;        // slots from here on are new tokens'
+  int64_t row;    // of head 0
+
+  // false: no memory, or behind the end
+  SPATTEN_DEV bool set(const PagedWeighParams& p, const PagedSeq& sq, int b, int first) {
+    const PagedCache& c = p.a.c;
+    slot = first;
+    lim = min(sq.old + sq.n, sq.len);
+    old = sq.old;
+    if (slot >= lim) return false;
+    const int pid = paged_page(c, b, slot / c.page);
+    row = (int64_t)max(pid, 0) * c.G * c.page + slot % c.page;
+    return pid >= 0;
+  }
+  SPATTEN_DEV bool plain() const { return slot + kQuad <= min(lim, old); }  // earlier tokens' all
+  // A head's weights before the call (their bytes; finish() knows which count).
+  SPATTEN_DEV float4 before(const PagedWeighParams& p, int g) const {
+    return *reinterpret_cast<const float4*>(p.weight + row + (int64_t)g * p.a.c.page);
+  }
+  SPATTEN_DEV void finish(const PagedWeighParams& p, const PagedSeq& sq, int g, float4 was, const float (&add)[kQuad]) const {
+    const int64_t at = row + (int64_t)g * p.a.c.page;
+    if (plain()) {
+      *reinterpret_cast<float4*>(p.weight + at) = make_float4(was.x + add[0], was.y + add[1], was.z + add[2], was.w + add[3]);
+      return;
+    }
+    const float w[kQuad] = {was.x, was.y, was.z, was.w};
+#pragma unroll
+    for (int i = 0; i < kQuad; ++i) {
+      if (slot + i >= lim) break;
+      const bool fresh = slot + i >= old;
+      p.weight[at + i] = (fresh ? 0.f : w[i]) + add[i];
+      if (fresh) p.position[at + i] = p.positions ? p.positions[sq.begin + slot + i - old] : slot + i;
+    }
+  }
 };
 
-SPATTEN_DEV bool weigh_slot(const PagedWeighParams& p, const PagedSeq& sq, int b, int slot, WeighSlot& x) {
-  const PagedCache& c = p.a.c;
-  const int pid = paged_page(c, b, slot / c.page);
-  if (pid < 0) return false;
-  x.row = (int64_t)pid * c.G * c.page + slot % c.page;
-  x.fresh = slot >= sq.old;
-  x.position = x.fresh && p.positions ? p.positions[sq.begin + slot - sq.old] : slot;
-  return true;
+// Slots x sequences x groups of heads; groups of `heads`, smaller where the CTAs are few.
+dim3 slot_grid(const PagedWeighParams& p, int n_sm, int& heads) {
+  const int64_t slots = (int64_t)p.a.c.max_pages * p.a.c.page, G = p.a.c.G;
+  const int64_t ctas = (slots + kSlotsCta - 1) / kSlotsCta;
+  heads = 8;
+  while (heads > 1 && ctas * p.a.b.B * ((G + heads - 1) / heads) < 4 * n_sm) heads /= 2;
+  return dim3((unsigned)ctas, p.a.b.B, (unsigned)((G + heads - 1) / heads));
 }
 
-SPATTEN_DEV void add_weight(const PagedWeighParams& p, const WeighSlot& x, int g, float before, float add) {
-  const int64_t row = x.row + (int64_t)g * p.a.c.page;
-  p.weight[row] = before + add;
-  if (x.fresh) p.position[row] = x.position;
-}
-
-// A thread per slot, all heads, whose rows' statistics lie in shared memory.
-constexpr int kStatHeads = 64;
+// ---------------------------------------------------------------- few rows: kept scores
 
 template <int ROWS>
-__global__ void __launch_bounds__(kSlotThreads) paged_weigh_scores_kernel(const PagedWeighParams p) {
-  __shared__ float2 stat[kStatHeads][ROWS];
+__global__ void __launch_bounds__(kSlotThreads) paged_weigh_scores_kernel(const PagedWeighParams p, int heads) {
+  __shared__ float2 stat[8][ROWS];
   grid_dependents();
   grid_wait();
   const PagedAttendParams& a = p.a;
-  const int b = blockIdx.y, G = a.c.G, R = a.b.H / G, page = a.c.page;
+  const int b = blockIdx.y, G = a.c.G, R = a.b.H / G, g0 = blockIdx.z * heads, tid = threadIdx.x;
   const PagedSeq sq = paged_seq(a.b, a.c, b);
-  const int slot = blockIdx.x * kSlotThreads + threadIdx.x, lim = min(sq.old + sq.n, sq.len), nrows = sq.n * R;
-  if (sq.n == 0 || (int)(blockIdx.x * kSlotThreads) >= lim || nrows > p.rows_over) return;
-  WeighSlot x = {};
-  const bool live = slot < lim && weigh_slot(p, sq, b, slot, x);
-  const int64_t slots = (int64_t)a.c.max_pages * page;
-  const float* src = a.score + ((int64_t)b * G * slots + slot) * ROWS;
-  for (int g0 = 0; g0 < G; g0 += kStatHeads) {
-    const int heads = min(G - g0, kStatHeads);
-    __syncthreads();
-    for (int i = threadIdx.x; i < heads * ROWS; i += kSlotThreads) {
-      const int g = i / ROWS, r = i % ROWS;  // (a row that there is not has no weight: its score is another's)
-      stat[g][r] = r < nrows ? a.stat[(int64_t)(sq.begin + r / R) * a.b.H + (g0 + g) * R + r % R] : make_float2(0.f, 0.f);
+  const int nrows = sq.n * R;
+  if (sq.n == 0 || nrows > p.rows_over) return;
+  WeighSlots x;
+  const bool live = x.set(p, sq, b, blockIdx.x * kSlotsCta + kQuad * tid);
+  if (tid < heads * ROWS && g0 + tid / ROWS < G) {
+    const int g = g0 + tid / ROWS, r = tid % ROWS;
+    if (r < nrows) stat[tid / ROWS][r] = a.stat[(int64_t)(sq.begin + r / R) * a.b.H + g * R + r % R];
+  }
+  __syncthreads();
+  if (!live) return;
+  const int64_t slots = (int64_t)a.c.max_pages * a.c.page;
+  const float* src = a.score + ((int64_t)b * G * slots + x.slot) * ROWS;
+#pragma unroll 2
+  for (int h = 0; h < min(heads, G - g0); ++h) {
+    const int g = g0 + h;
+    float s[kQuad * ROWS];
+    const float4* at = reinterpret_cast<const float4*>(src + g * slots * ROWS);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const float4 y = at[i];
+      s[4 * i] = y.x; s[4 * i + 1] = y.y; s[4 * i + 2] = y.z; s[4 * i + 3] = y.w;
     }
-    __syncthreads();
-    if (!live) continue;
-#pragma unroll 4
-    for (int h = 0; h < heads; ++h) {
-      const int g = g0 + h;
-      float s[ROWS];
-      const float* at = src + g * slots * ROWS;
-      if constexpr (ROWS >= 4) {
+    const float4 was = x.before(p, g);
+    float add[kQuad] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < ROWS; i += 4) {
-          const float4 y = *reinterpret_cast<const float4*>(at + i);
-          s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
-        }
-      } else {
+    for (int r = 0; r < ROWS; ++r)
+      if (r < nrows) {
+        const float2 y = stat[h][r];
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) s[i] = at[i];
+        for (int i = 0; i < kQuad; ++i) add[i] += fast_exp2(s[i * ROWS + r] - y.x) * y.y;
       }
-      const float before = x.fresh ? 0.f : p.weight[x.row + (int64_t)g * page];
-      float add = 0.f;
-#pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        const float2 y = stat[h][i];
-        if (i < nrows) add += fast_exp2(s[i] - y.x) * y.y;
-      }
-      add_weight(p, x, g, before, add);
-    }
+    x.finish(p, sq, g, was, add);
   }
 }
 
-cudaError_t scores_launch(const PagedWeighParams& p, cudaStream_t st) {
-  const int64_t slots = (int64_t)p.a.c.max_pages * p.a.c.page;
-  const dim3 grid((unsigned)((slots + kSlotThreads - 1) / kSlotThreads), p.a.b.B);
+cudaError_t scores_launch(const PagedWeighParams& p, int n_sm, cudaStream_t st) {
+  int heads;
+  const dim3 grid = slot_grid(p, n_sm, heads);
   switch (p.a.score_rows) {
-    case 1: return launch_dependent(paged_weigh_scores_kernel<1>, grid, kSlotThreads, 0, st, p);
-    case 2: return launch_dependent(paged_weigh_scores_kernel<2>, grid, kSlotThreads, 0, st, p);
-    case 4: return launch_dependent(paged_weigh_scores_kernel<4>, grid, kSlotThreads, 0, st, p);
-    case 8: return launch_dependent(paged_weigh_scores_kernel<8>, grid, kSlotThreads, 0, st, p);
+    case 1: return launch_dependent(paged_weigh_scores_kernel<1>, grid, kSlotThreads, 0, st, p, heads);
+    case 2: return launch_dependent(paged_weigh_scores_kernel<2>, grid, kSlotThreads, 0, st, p, heads);
+    case 4: return launch_dependent(paged_weigh_scores_kernel<4>, grid, kSlotThreads, 0, st, p, heads);
+    case 8: return launch_dependent(paged_weigh_scores_kernel<8>, grid, kSlotThreads, 0, st, p, heads);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -532,27 +550,34 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
   }
 }
 
-// The chunks' sums into the weights, a thread per slot, all heads.
-__global__ void __launch_bounds__(kSlotThreads) paged_weigh_sum_kernel(const PagedWeighParams p, const WeighPlan w) {
+// The chunks' sums into the weights.
+__global__ void __launch_bounds__(kSlotThreads) paged_weigh_sum_kernel(const PagedWeighParams p, const WeighPlan w,
+                                                                       int heads) {
   grid_dependents();
   grid_wait();
   const PagedAttendParams& a = p.a;
-  const int b = blockIdx.y, G = a.c.G, R = a.b.H / G;
+  const int b = blockIdx.y, G = a.c.G, R = a.b.H / G, g0 = blockIdx.z * heads;
   const PagedSeq sq = paged_seq(a.b, a.c, b);
-  const int slot = blockIdx.x * kSlotThreads + threadIdx.x, lim = Items::limit(sq), nrows = sq.n * R;
-  if (slot >= lim || nrows <= p.rows_over) return;
-  WeighSlot x;
-  if (!weigh_slot(p, sq, b, slot, x)) return;
-  // chunks with a row that sees the slot
-  const int c0 = a.tree || slot < sq.old ? 0 : (int)((int64_t)(slot - sq.old) * R / w.chunk);
+  const int nrows = sq.n * R;
+  WeighSlots x;
+  if (nrows <= p.rows_over || !x.set(p, sq, b, blockIdx.x * kSlotsCta + kQuad * threadIdx.x)) return;
   const int c1 = (nrows + w.chunk - 1) / w.chunk;
   const int64_t slots = (int64_t)a.c.max_pages * a.c.page;
+#pragma unroll 2
+  for (int h = 0; h < min(heads, G - g0); ++h) {
+    const int g = g0 + h;
+    const float4 was = x.before(p, g);
+    float add[kQuad] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int g = 0; g < G; ++g) {
-    const float before = x.fresh ? 0.f : p.weight[x.row + (int64_t)g * a.c.page];
-    float add = 0.f;
-    for (int c = c0; c < c1; ++c) add += w.partial[(((int64_t)c * a.b.B + b) * G + g) * slots + slot];
-    add_weight(p, x, g, before, add);
+    for (int c = 0; c < c1; ++c) {
+      const float4 y = *reinterpret_cast<const float4*>(w.partial + (((int64_t)c * a.b.B + b) * G + g) * slots + x.slot);
+      const float part[kQuad] = {y.x, y.y, y.z, y.w};
+      // a chunk of which no row sees a slot has left nothing for it
+      const int64_t seen = a.tree ? INT64_MAX : (int64_t)x.old + ((int64_t)min((c + 1) * w.chunk, nrows) - 1) / R + 1;
+#pragma unroll
+      for (int i = 0; i < kQuad; ++i) add[i] += x.slot + i < seen ? part[i] : 0.f;
+    }
+    x.finish(p, sq, g, was, add);
   }
 }
 
@@ -597,8 +622,9 @@ cudaError_t tc_launch(const PagedWeighParams& p, bool bf16, const WeighPlan& w, 
   e = launch_dependent(paged_weigh_tc_kernel<KV, D>, dim3((unsigned)std::min(2.0 * n_sm, items)), kThreads,
                        Lay<D>::bytes(a.b.B), st, p, w);
   if (e != cudaSuccess) return e;
-  return launch_dependent(paged_weigh_sum_kernel, dim3((unsigned)((slots + kSlotThreads - 1) / kSlotThreads), a.b.B),
-                          kSlotThreads, 0, st, p, w);
+  int heads;
+  const dim3 grid = slot_grid(p, n_sm, heads);
+  return launch_dependent(paged_weigh_sum_kernel, grid, kSlotThreads, 0, st, p, w, heads);
 }
 
 bool many_rows(const PagedWeighParams& p) { return most_rows(p) > p.rows_over; }
@@ -613,7 +639,7 @@ size_t paged_weigh_workspace(const PagedWeighParams& p) {
 cudaError_t launch_paged_weigh(const PagedWeighParams& p, int dtype, int kv, void* ws, int n_sm, cudaStream_t st) {
   if (dtype != kF16 && dtype != kBF16) return cudaErrorInvalidValue;
   if (p.a.score) {
-    const cudaError_t e = scores_launch(p, st);
+    const cudaError_t e = scores_launch(p, n_sm, st);
     if (e != cudaSuccess) return e;
   }
   if (!many_rows(p)) return cudaSuccess;
