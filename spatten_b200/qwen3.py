@@ -31,7 +31,10 @@ attention core with the progressive sparse attention kernel:
   keys and values of every layer go into a paged 8-bit cache (``paged.py``), and
   later forwards (a token, a few, or the next piece of a prompt) append to it and
   attend over it: QK-norm, RoPE and the append in one launch, the attention in
-  two. A layer that pruned its keys keeps attending over the ones it kept.
+  two. A layer that pruned its keys keeps attending over the ones it kept. With
+  ``keep_tokens`` the cascade goes on while it generates: a full layer forgets
+  the tokens of the least accumulated attention. Trees of drafted tokens are
+  checked in one forward (``draft_tree``, ``accept``).
 
 Unpadded batches only (the HF attention mask is not read: the mask is the
 causal one). The cascade state is shared by all layers of a model
@@ -106,21 +109,35 @@ class PagedQwen3Cache(Cache):
     each layer's pool, sequence b's pages in a row; the layers share one page
     table. Layers may hold different numbers of tokens (token pruning).
 
+    ``keep_tokens``: the layers keep account of the attention weight that each
+    token gathers, and one that has no room for the next tokens keeps the
+    ``recent_tokens`` newest and of the others those of the largest weight,
+    ``keep_tokens`` in all (``paged_evict``), and goes on; so a text may be longer
+    than ``max_tokens``. ``None``: a full cache refuses.
+
     HF's generation modes that change a cache are served: drafted tokens
     (``crop``), beams (``reorder_cache``), and changes of the batch
     (``batch_repeat_interleave``, ``batch_select_indices``)."""
 
-    def __init__(self, config, batch, max_tokens, page_size=64, kv_dtype=torch.int8, device="cuda"):
+    def __init__(self, config, batch, max_tokens, page_size=64, kv_dtype=torch.int8, device="cuda", keep_tokens=None,
+                 recent_tokens=0):
         super().__init__(layers=[])
         L, G, D = config.num_hidden_layers, config.num_key_value_heads, config.head_dim
         self.batch, self.max_tokens = batch, int(max_tokens)
+        self.keep_tokens, self.recent_tokens = keep_tokens, int(recent_tokens)
+        if keep_tokens is not None and not 1 <= keep_tokens < self.max_tokens:
+            raise ValueError(f"PagedQwen3Cache: keep_tokens {keep_tokens} of {self.max_tokens}")
+        if not 0 <= self.recent_tokens <= (keep_tokens or 0):
+            raise ValueError(f"PagedQwen3Cache: {recent_tokens} recent tokens among {keep_tokens}")
         mp = -(-self.max_tokens // page_size)
         self.pools = [paged.new_paged_cache(batch * mp, G, D, page_size, kv_dtype, device) for _ in range(L)]
+        self.weights = [paged.new_paged_weights(p) for p in self.pools] if keep_tokens is not None else [None] * L
+        self.tree = None  # (bits, positions, tokens per sequence, positions before) of drafted tokens
         self.page_table = self._pages(batch, mp, device)
         self.seq_lens = torch.zeros((L, batch), dtype=torch.int32, device=device)
         self.held = [0] * L  # slots of each layer, as the host counts them
         self.seen = [0] * L  # positions each layer has been given (kept or not)
-        self.pruned = [0] * L  # positions of a prompt of which each layer kept only some (0: all kept)
+        self.pruned = [0] * L  # positions of which each layer kept only some (0: all kept)
 
     @staticmethod
     def _pages(batch, per_sequence, device):
@@ -145,6 +162,7 @@ class PagedQwen3Cache(Cache):
 
     def reset(self):
         """Forget every token; the pools stay."""
+        self.tree = None
         self.seq_lens.zero_()
         L = len(self.pools)
         self.held, self.seen, self.pruned = [0] * L, [0] * L, [0] * L
@@ -152,8 +170,10 @@ class PagedQwen3Cache(Cache):
     def crop(self, max_length):
         """Forget the positions from ``max_length`` on (negative: that many of
         the last ones), in every layer; their slots are written again by the next
-        tokens. A pruned prompt can only be forgotten as a whole: which of its
-        positions a layer kept is not known here."""
+        tokens. Positions of which a layer kept only some (a pruned prompt, or what
+        there was at an eviction) can only be forgotten as a whole: which it kept is
+        not known here."""
+        self._no_tree("crop")
         keep = int(max_length)
         if keep < 0:
             keep = max(self.seen[0] + keep, 0)
@@ -164,7 +184,7 @@ class PagedQwen3Cache(Cache):
             return self.reset()
         for n, d, fixed in zip(self.seen, drop, self.pruned):
             if d and n - d < fixed:
-                raise NotImplementedError(f"PagedQwen3Cache: crop to {keep} inside a pruned prompt of {fixed} tokens")
+                raise NotImplementedError(f"PagedQwen3Cache: crop to {keep} inside {fixed} pruned tokens")
         if len(set(drop)) == 1:
             self.seq_lens.sub_(drop[0])
         else:  # layers that were given different numbers of tokens
@@ -188,6 +208,7 @@ class PagedQwen3Cache(Cache):
     def reorder_cache(self, beam_idx):
         """Sequence b becomes a copy of sequence beam_idx[b], on pages of its own
         (the next tokens of two beams differ)."""
+        self._no_tree("reorder_cache")
         rows = self._rows_of(beam_idx)
         if len(rows) != self.batch:
             raise ValueError(f"PagedQwen3Cache: {len(rows)} beams for {self.batch} sequences")
@@ -196,17 +217,21 @@ class PagedQwen3Cache(Cache):
             return
         dev = self.seq_lens.device
         dst, src = torch.tensor([moved, [rows[b] for b in moved]], device=dev)
-        for pool, held in zip(self.pools, self.held):
-            for t in pool:
+        for pool, w, held in zip(self.pools, self.weights, self.held):
+            for t in (*pool, *(w or ())):
                 t = self._by_sequence(t, -(-held // pool.k.shape[2]))
                 t.index_copy_(0, dst, t.index_select(0, src))
         self.seq_lens.index_copy_(1, dst, self.seq_lens.index_select(1, src))
 
     def _select(self, rows):
         """Sequence b of a new batch is a copy of sequence rows[b]."""
+        self._no_tree("a change of the batch")
         idx = torch.tensor(rows, device=self.seq_lens.device)
-        self.pools = [paged.PagedKVCache(*(self._by_sequence(t).index_select(0, idx).flatten(0, 1).view(t.dtype)
-                                           for t in pool)) for pool in self.pools]
+
+        def select(t):
+            return self._by_sequence(t).index_select(0, idx).flatten(0, 1).view(t.dtype)
+        self.pools = [paged.PagedKVCache(*map(select, pool)) for pool in self.pools]
+        self.weights = [w and paged.PagedWeights(*map(select, w)) for w in self.weights]
         self.seq_lens = self.seq_lens.index_select(1, idx)
         self.batch = len(rows)
         self.page_table = self._pages(self.batch, self.page_table.shape[1], idx.device)
@@ -229,9 +254,12 @@ class PagedQwen3Cache(Cache):
         """``paged_append`` of n tokens per sequence (rows k, v, packed by cu =
         ``packed(n)``) to one layer, counted as ``seen`` more positions; nothing
         counts when the call is refused."""
-        held = self.held[layer_idx] + n
-        if held > self.max_tokens:
-            raise ValueError(f"PagedQwen3Cache: {self.held[layer_idx]} + {n} tokens, room for {self.max_tokens}")
+        before = self.held[layer_idx]
+        if before + n > self.max_tokens:
+            if self.keep_tokens is None or self.keep_tokens + n > self.max_tokens or before <= self.keep_tokens:
+                raise ValueError(f"PagedQwen3Cache: {before} + {n} tokens, room for {self.max_tokens}")
+            before = self._evict(layer_idx)
+        held = before + n
         lens = self.seq_lens[layer_idx]
         lens.add_(n)
         try:
@@ -245,13 +273,77 @@ class PagedQwen3Cache(Cache):
             self.pruned[layer_idx] = self.seen[layer_idx]
         return q
 
-    def store(self, layer_idx, k, v, seen):
+    def _evict(self, layer_idx):
+        """Cut a layer to ``keep_tokens``; returns the slots it holds."""
+        lens = self.seq_lens[layer_idx]
+        lens.copy_(paged.paged_evict(self.pools[layer_idx], self.weights[layer_idx], self.page_table, lens,
+                                     self.keep_tokens, recent=self.recent_tokens))
+        self.held[layer_idx] = self.keep_tokens
+        self.pruned[layer_idx] = self.seen[layer_idx]
+        return self.keep_tokens
+
+    def positions(self, layer_idx, S):
+        """Positions int32 [batch * S] of the next S tokens of each sequence."""
+        first = self.seen[layer_idx]
+        return torch.arange(first, first + S, dtype=torch.int32, device=self.seq_lens.device).repeat(self.batch)
+
+    def store(self, layer_idx, k, v, seen, importance=None, positions=None):
         """Append finished (normed and rotated) keys and values [B, K, G, D];
-        ``seen``: the positions that they were chosen from."""
+        ``seen``: the positions that they were chosen from. With ``keep_tokens``
+        their attention weights (fp32 [B, K], spread over the KV heads; default
+        0) and positions ([B, K]; default: the next ones) start as given."""
         B, K, G, D = k.shape
         if B != self.batch:
             raise ValueError(f"PagedQwen3Cache: batch {B}, made for {self.batch}")
+        if positions is None and self.keep_tokens is not None:
+            positions = self.positions(layer_idx, K).view(B, K)
         self.append(layer_idx, K, seen, self.packed(K), k.reshape(B * K, G, D), v.reshape(B * K, G, D))
+        if self.keep_tokens is not None:
+            page = self.pools[layer_idx].k.shape[2]
+            slot = torch.arange(self.held[layer_idx] - K, self.held[layer_idx], device=k.device)
+            weight, position = (self._by_sequence(t) for t in self.weights[layer_idx])  # [B, pages, G, page]
+            weight[:, slot // page, :, slot % page] = 0.0 if importance is None else (importance.t() / G)[..., None]
+            position[:, slot // page, :, slot % page] = positions.t().to(torch.int32)[..., None]
+
+    def _no_tree(self, what):
+        if self.tree is not None:
+            raise RuntimeError(f"PagedQwen3Cache: {what} before the drafted tree's tokens were accepted")
+
+    def draft_tree(self, parents):
+        """The next forward's tokens [B, S] are a tree (or several): ``parents``
+        [B, S] holds the place of each one's parent among them, before its own, or
+        -1 for a child of the text so far. Returns their positions, int64 [B, S],
+        for the model's ``position_ids``; ``accept`` has to follow that forward."""
+        self._no_tree("another tree")
+        B, S = parents.shape
+        if B != self.batch or S < 1:
+            raise ValueError(f"PagedQwen3Cache: parents of {B} sequences x {S} tokens, made for {self.batch}")
+        if len(set(self.seen)) > 1 or self.seen[0] == 0:
+            raise ValueError("PagedQwen3Cache: a drafted tree follows a prompt")
+        dev = self.seq_lens.device
+        lens = torch.full((B,), self.seen[0] + S, dtype=torch.int32, device=dev)
+        bits, positions = paged.paged_tree(parents.to(dev, torch.int32).reshape(-1), self.packed(S), lens, S)
+        self.tree = bits, positions, S, self.seen[0]
+        return positions.view(B, S).long()
+
+    def accept(self, paths):
+        """Of the drafted tree's tokens the ones at ``paths`` (per sequence their
+        places, ascending, equally many for each) stay, in every layer."""
+        if self.tree is None or any(n != self.tree[3] + self.tree[2] for n in self.seen):
+            raise RuntimeError("PagedQwen3Cache: no forward of a drafted tree")
+        S = self.tree[2]
+        paths = [[int(i) for i in p] for p in paths]
+        if len(paths) != self.batch or len(set(map(len, paths))) != 1:
+            raise ValueError(f"PagedQwen3Cache: need as many accepted tokens for each of {self.batch} sequences")
+        if any(p != sorted(set(p)) or (p and not 0 <= p[0] <= p[-1] < S) for p in paths):
+            raise ValueError(f"PagedQwen3Cache: accepted places {paths} of {S} tokens (need them ascending)")
+        accepted = torch.tensor(paths, dtype=torch.int32, device=self.seq_lens.device).view(self.batch, -1)
+        gone, cu = S - accepted.shape[1], self.packed(S)
+        for pool, w, lens in zip(self.pools, self.weights, self.seq_lens):
+            lens.copy_(paged.paged_keep(pool, self.page_table, cu, lens, accepted, weights=w))
+        self.held = [n - gone for n in self.held]
+        self.seen = [n - gone for n in self.seen]
+        self.tree = None
 
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
         """HF's form of ``store`` ([B, G, K, D]); only a prefill's first call may
@@ -323,12 +415,19 @@ class SpattenQwen3Attention(Qwen3Attention):
         cos, sin = position_embeddings  # [B or 1, S, d]: a row per token
         rows = torch.arange(cos.shape[0] * S, dtype=torch.int32, device=q.device)
         positions = rows if cos.shape[0] == B else rows.repeat(B)
-        cu = cache.packed(S)
+        cu, more = cache.packed(S), {}
+        if cache.tree is not None:
+            more["tree"], at, drafted, before = cache.tree
+            if S != drafted or cache.seen[self.layer_idx] != before:
+                raise RuntimeError(f"PagedQwen3Cache: {S} tokens after a drafted tree of {drafted} that was not accepted")
+        if cache.keep_tokens is not None:
+            more["weights"] = cache.weights[self.layer_idx]
+            more["positions"] = at if cache.tree is not None else cache.positions(self.layer_idx, S)
         q = cache.append(self.layer_idx, S, S, cu, k, v, q=q, cos=cos.reshape(-1, d), sin=sin.reshape(-1, d),
                          positions=positions, q_norm_w=self.q_norm.weight, k_norm_w=self.k_norm.weight,
                          eps=self.q_norm.variance_epsilon)
         out = paged.paged_attention(q, cache.pools[self.layer_idx], cache.page_table, cu,
-                                    cache.seq_lens[self.layer_idx], S, sm_scale=self.scaling)
+                                    cache.seq_lens[self.layer_idx], S, sm_scale=self.scaling, **more)
         return self.o_proj(out.view(B, S, H * d)), None
 
     @torch.no_grad()
@@ -396,7 +495,9 @@ class SpattenQwen3Attention(Qwen3Attention):
         st.kept_per_layer.append(K)
 
         if isinstance(past_key_values, PagedQwen3Cache):
-            past_key_values.store(self.layer_idx, k, v, S)
+            # this layer's own weights: what it added to the cascade's
+            past_key_values.store(self.layer_idx, k, v, S, positions=pos,
+                                  importance=cum if st.cumulative is None else cum - st.cumulative)
         elif past_key_values is not None:
             # the cache concatenates into a new contiguous [B, Hkv, K, d] tensor
             # itself: the head-major views go in as they are (one copy, not two)

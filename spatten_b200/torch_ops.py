@@ -19,6 +19,18 @@ registries -- finds them under the ``spatten`` namespace:
   Tensor page_table, Tensor cu_tokens, Tensor seq_lens, int max_tokens, float sm_scale) -> Tensor``
 * ``spatten::paged_read(Tensor k_pool, Tensor v_pool, Tensor k_scale, Tensor v_scale, Tensor page_table,
   Tensor seq_lens, Tensor idx) -> (Tensor k, Tensor v)`` (bf16)
+* ``spatten::paged_tree(Tensor parents, Tensor cu_tokens, Tensor seq_lens, int max_tokens)
+  -> (Tensor tree, Tensor positions)``
+* ``spatten::paged_tree_attention(Tensor q, Tensor k_pool, Tensor v_pool, Tensor k_scale, Tensor v_scale,
+  Tensor page_table, Tensor cu_tokens, Tensor seq_lens, Tensor tree, int max_tokens, float sm_scale) -> Tensor``
+* ``spatten::paged_weighing_attention(Tensor q, Tensor k_pool, Tensor v_pool, Tensor k_scale, Tensor v_scale,
+  Tensor(a!) weight, Tensor(b!) position, Tensor page_table, Tensor cu_tokens, Tensor seq_lens, Tensor positions,
+  int max_tokens, float sm_scale) -> Tensor`` (causal attention that accumulates its weights)
+* ``spatten::paged_evict(Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor(c!) k_scale, Tensor(d!) v_scale,
+  Tensor(e!) weight, Tensor(f!) position, Tensor page_table, Tensor seq_lens, int keep, int recent, bool per_head)
+  -> Tensor`` (new lengths)
+* ``spatten::paged_keep(Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor(c!) k_scale, Tensor(d!) v_scale,
+  Tensor page_table, Tensor cu_tokens, Tensor seq_lens, Tensor accepted) -> Tensor`` (new lengths)
 
 CUDA tensors only, like the rest of the package. Importing this module
 registers the ops once.
@@ -83,3 +95,45 @@ def paged_read(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor
                page_table: torch.Tensor, seq_lens: torch.Tensor, idx: torch.Tensor
                ) -> tuple[torch.Tensor, torch.Tensor]:
     return _pd.paged_read(_pd.PagedKVCache(k_pool, v_pool, k_scale, v_scale), page_table, seq_lens, idx=idx)
+
+
+@torch.library.custom_op("spatten::paged_tree", mutates_args=())
+def paged_tree(parents: torch.Tensor, cu_tokens: torch.Tensor, seq_lens: torch.Tensor, max_tokens: int
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    return _pd.paged_tree(parents, cu_tokens, seq_lens, max_tokens)
+
+
+@torch.library.custom_op("spatten::paged_tree_attention", mutates_args=())
+def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+                         v_scale: torch.Tensor, page_table: torch.Tensor, cu_tokens: torch.Tensor,
+                         seq_lens: torch.Tensor, tree: torch.Tensor, max_tokens: int, sm_scale: float) -> torch.Tensor:
+    return _pd.paged_attention(q, _pd.PagedKVCache(k_pool, v_pool, k_scale, v_scale), page_table, cu_tokens,
+                               seq_lens, max_tokens, sm_scale=sm_scale, tree=tree)
+
+
+@torch.library.custom_op("spatten::paged_weighing_attention", mutates_args=("weight", "position"))
+def paged_weighing_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+                             v_scale: torch.Tensor, weight: torch.Tensor, position: torch.Tensor,
+                             page_table: torch.Tensor, cu_tokens: torch.Tensor, seq_lens: torch.Tensor,
+                             positions: torch.Tensor, max_tokens: int, sm_scale: float) -> torch.Tensor:
+    return _pd.paged_attention(q, _pd.PagedKVCache(k_pool, v_pool, k_scale, v_scale), page_table, cu_tokens,
+                               seq_lens, max_tokens, sm_scale=sm_scale, weights=_pd.PagedWeights(weight, position),
+                               positions=positions)
+
+
+_POOL = ("k_pool", "v_pool", "k_scale", "v_scale")
+
+
+@torch.library.custom_op("spatten::paged_evict", mutates_args=_POOL + ("weight", "position"))
+def paged_evict(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                weight: torch.Tensor, position: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                keep: int, recent: int, per_head: bool) -> torch.Tensor:
+    return _pd.paged_evict(_pd.PagedKVCache(k_pool, v_pool, k_scale, v_scale), _pd.PagedWeights(weight, position),
+                           page_table, seq_lens, keep, recent=recent, per_head=per_head)
+
+
+@torch.library.custom_op("spatten::paged_keep", mutates_args=_POOL)
+def paged_keep(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+               page_table: torch.Tensor, cu_tokens: torch.Tensor, seq_lens: torch.Tensor, accepted: torch.Tensor
+               ) -> torch.Tensor:
+    return _pd.paged_keep(_pd.PagedKVCache(k_pool, v_pool, k_scale, v_scale), page_table, cu_tokens, seq_lens, accepted)
