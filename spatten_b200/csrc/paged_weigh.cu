@@ -438,34 +438,39 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
         const float4* cst = reinterpret_cast<const float4*>(sm + L::oC + cs * kConstBytes);
         const int r0 = t * kTileRows;
         const int sees = it.sq.old + (a.tree ? 0 : r0 / R + 1);  // slots before it are seen by every row of the tile
+        auto weights2 = [&](int k) {  // of rows 2 k and 2 k + 1
+          const float4 c = cst[k];
+          const float2 y = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), __fmul2_rn(make_float2(c.x, c.y), ks2),
+                                      make_float2(c.z, c.w));
+          return make_float2(fast_exp2(y.x), fast_exp2(y.y));
+        };
         if (last < sees) {
 #pragma unroll
-          for (int k = 0; k < kTileRows / 2; ++k) {
-            const float4 c = cst[k];
-            float2 x2 = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), __fmul2_rn(make_float2(c.x, c.y), ks2),
-                                   make_float2(c.z, c.w));
-            x2.x = fast_exp2(x2.x);
-            x2.y = fast_exp2(x2.y);
-            sum = __fadd2_rn(sum, x2);
+          for (int k = 0; k < kTileRows / 2; ++k) sum = __fadd2_rn(sum, weights2(k));
+        } else if (!a.tree) {
+          // the first row of the tile that sees the key
+          const int64_t first = max((int64_t)(slot - it.sq.old) * R - r0, (int64_t)0);
+          if (__any_sync(0xffffffffu, first < kTileRows)) {
+            const int f = (int)min(first, (int64_t)kTileRows);
+#pragma unroll
+            for (int k = 0; k < kTileRows / 2; ++k) {
+              const float2 y = weights2(k);
+              sum = __fadd2_rn(sum, make_float2(2 * k >= f ? y.x : 0.f, 2 * k + 1 >= f ? y.y : 0.f));
+            }
           }
         } else {
           const int j = slot - it.sq.old;  // the key's place among the new tokens
-          const int64_t first = (int64_t)j * R - r0;  // the causal form's first row that sees it
+          const bool none = (j >> 5) >= a.words;
 #pragma unroll
-          for (int k = 0; k < kTileRows; ++k) {
-            bool see = j < 0;
-            if (!see) {
-              if (a.tree) {
-                const int i = (r0 + k) / R;
-                see = i < it.sq.n && (j >> 5) < a.words &&
-                      ((*(a.tree + (it.sq.begin + i) * a.tree_st + (j >> 5)) >> (j & 31)) & 1u);
-              } else {
-                see = k >= first;
-              }
+          for (int k = 0; k < kTileRows / 2; ++k) {
+            const float2 y = weights2(k);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int i = min((r0 + 2 * k + h) / R, it.sq.n - 1);  // (rows behind the last one weigh nothing)
+              bool see = j < 0;
+              if (!see && !none) see = (*(a.tree + (it.sq.begin + i) * a.tree_st + (j >> 5)) >> (j & 31)) & 1u;
+              if (see) (h ? sum.y : sum.x) += h ? y.y : y.x;
             }
-            const float* c = reinterpret_cast<const float*>(cst + (k >> 1)) + (k & 1);
-            const float x1 = fast_exp2(fmaf(s[k], c[0] * ks, c[2]));
-            if (see) (k & 1 ? sum.y : sum.x) += x1;
           }
         }
         __syncwarp();
