@@ -12,11 +12,12 @@
 // the keys again would take 2.1 GB.
 //
 // More: the scores are computed again, on the tensor cores, with the keys as rows:
-//   S^T [128 keys x 64 rows] = K codes . Q'^T   (kind::f16, fp32 in tensor memory),
+//   S^T [128 keys x 128 rows] = K codes . Q'^T   (kind::f16, fp32 in tensor memory),
 // so that a thread owns a key and the sum over rows needs no exchange.
 // paged_weigh_rows_kernel lays the query rows out once (f16 as the attention's, in
 // the layout that the MMAs read, and two numbers a row: cq, its scores' factor, and
-// b = log2(1 / l) - m, so that p = 2^(S (cq k_scale) + b)); paged_weigh_tc_kernel
+// b = log2(1 / l) - m, so that p = 2^(S (cq k_scale) + b), cq mostly the same for a
+// tile); paged_weigh_tc_kernel
 // takes 256 keys x a chunk of the rows at a time; the last kernel adds the chunks up.
 // Bound by the exponentials, one per (row, key).
 #include <algorithm>
@@ -145,36 +146,37 @@ cudaError_t scores_launch(const PagedWeighParams& p, int n_sm, cudaStream_t st) 
 
 // ---------------------------------------------------------------- many rows: tensor cores
 
-constexpr int kKeys = 256, kTileRows = 64, kFoldTiles = 8;
-constexpr int kSumWarps = 8, kThreads = 32 * (kSumWarps + 2);
-constexpr int kConsts = 4;               // tiles' row constants in shared memory
-constexpr int kConstBytes = kTileRows * 8;
+constexpr int kKeys = 256, kTileRows = 128, kGroup = 32, kFoldTiles = 4;
+constexpr int kSumWarps = 16, kWideWarps = 4, kThreads = 32 * (kSumWarps + kWideWarps + 2);
+constexpr int kRing = 2;    // tiles of query rows, blocks of keys in shared memory
+constexpr int kConsts = 4;  // tiles' row constants
+constexpr int kConstBytes = kTileRows * 8 + 16;  // b and cq of the rows, the cq that all have (0: each its own)
 constexpr unsigned kErr = 0x500;
 
 // What the main kernel works on, in the workspace.
 struct WeighPlan {
-  uint8_t* tiles;     // [G][tiles_g] records: 64 query rows, then their constants
-  float* partial;     // [chunks][B][G][slots]
+  uint8_t* tiles;     // [G][tiles_g] records: 128 query rows, then their constants
+  float* partial;     // [chunks][2][B][G][slots]: of the chunk's even and odd 64 rows
   int64_t tiles_g;
   int chunk, chunks;  // rows of a chunk (a multiple of kTileRows), chunks of a sequence at most
 };
 
 template <int D>
 struct Lay {
-  static constexpr int kRing = D == 128 ? 2 : 4;            // tiles of query rows
   static constexpr int kQBytes = kTileRows * D * 2;
   static constexpr int kRecord = kQBytes + kConstBytes;
-  static constexpr int oK = 0;                               // [2][D / 64][128][128 B]
   static constexpr int kKHalf = 128 * D * 2;
-  static constexpr int oQ = oK + 2 * kKHalf;                 // [ring][D / 64][64][128 B]
-  static constexpr int oC = oQ + kRing * kQBytes;            // [kConsts][32][cq, cq, b, b]
-  static constexpr int oBar = oC + kConsts * kConstBytes;
-  static constexpr int kBars = 2 * kRing + 2 * kConsts + 2 + 2 + 1 + 1;
+  static constexpr int oK = 0;                               // [ring][2][D / 64][128][128 B]
+  static constexpr int oQ = oK + kRing * 2 * kKHalf;         // [ring][D / 64][128][128 B]
+  static constexpr int oC = oQ + kRing * kQBytes;            // [kConsts]
+  static constexpr int oScale = oC + kConsts * kConstBytes;  // [ring][256] scales of the keys
+  static constexpr int oBar = oScale + kRing * kKeys * 4;
+  static constexpr int kBars = 4 * kRing + 2 * kConsts + 4 + 1;
   static constexpr int oTmem = oBar + kBars * 8;
   static constexpr int oAbort = oTmem + 4;
-  static constexpr int oScan = (oAbort + 4 + 7) & ~7;        // [10] 64-bit
-  static constexpr int oPre = oScan + 8 * (kThreads / 32);   // [B + 1]
-  static constexpr int bytes(int B) { return oPre + (B + 1) * 4 + 1024; }
+  static constexpr int oScan = (oAbort + 4 + 7) & ~7;        // [warps] 64-bit
+  static constexpr int oPre = oScan + 8 * (kThreads / 32);   // [pairs + 1]
+  static constexpr int bytes(int B) { return oPre + ((B + 1) / 2 + 1) * 4 + 1024; }
 };
 
 // First record of sequence b: records of sequences whose rows are apart are apart.
@@ -197,9 +199,11 @@ __global__ void __launch_bounds__(256) paged_weigh_rows_kernel(const PagedWeighP
     return bf16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u))
                 : __half22float2(*reinterpret_cast<const __half2*>(&x));
   };
-  uint4 x[kTileRows / RPP];
+  constexpr int STEPS = kTileRows / RPP;
+  uint4 x[STEPS];
+  float top[STEPS], most = 0.f;  // the rows' largest magnitudes, that of the finite rows of the tile
 #pragma unroll
-  for (int k = 0; k < kTileRows / RPP; ++k) {
+  for (int k = 0; k < STEPS; ++k) {
     const int r = t * kTileRows + k * RPP + tid / LQ;
     x[k] = make_uint4(0u, 0u, 0u, 0u);
     if (r < nrows)
@@ -207,36 +211,58 @@ __global__ void __launch_bounds__(256) paged_weigh_rows_kernel(const PagedWeighP
                                              (int64_t)(g * R + r % R) * a.q_sh + 8 * li);
   }
 #pragma unroll
-  for (int k = 0; k < kTileRows / RPP; ++k) {
-    const int y = k * RPP + tid / LQ, r = t * kTileRows + y;
+  for (int k = 0; k < STEPS; ++k) {
     const uint32_t in[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-    float top = 0.f;
+    float m = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 f = pair(in[j]);
-      top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-      if (!(f.x == f.x && f.y == f.y)) top = INFINITY;  // fmaxf drops a NaN
+      m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+      if (!(f.x == f.x && f.y == f.y)) m = INFINITY;  // fmaxf drops a NaN
     }
 #pragma unroll
-    for (int d = LQ / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const QueryScale qs = query_scale(top, a.scale_log2);
+    for (int d = LQ / 2; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    top[k] = m;
+    if (m < INFINITY) most = fmaxf(most, m);
+  }
+  __shared__ float red[8];
+  most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+  if ((tid & 31) == 0) red[tid >> 5] = most;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = fmaxf(most, red[i]);
+  // One power of two for the tile, so that the sums need one number a row instead of two: where
+  // each row reaches 2^-12 of the largest magnitude, what f16 drops of it is below 2^-28 of
+  // the row's own largest.
+  bool far = false;
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) far |= top[k] > 0.f && top[k] < most * 0x1p-12f;
+  const bool common = !__syncthreads_or(far);
+  float* const consts = reinterpret_cast<float*>(rec + L::kQBytes);
+  const QueryScale all = query_scale(most, a.scale_log2);
+  if (tid == 0) consts[2 * kTileRows] = common ? all.factor : 0.f;
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const int y = k * RPP + tid / LQ, r = t * kTileRows + y;
+    const uint32_t in[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+    const QueryScale own = query_scale(top[k], a.scale_log2);  // (its factor is NaN for a row that is not finite)
+    const float up = top[k] < INFINITY ? (common ? all.up : own.up) : 0.f;
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 f = pair(in[j]);
-      o[j] = pack2<__half>(f.x * qs.up, f.y * qs.up);
+      o[j] = up > 0.f ? pack2<__half>(f.x * up, f.y * up) : 0u;
     }
     *reinterpret_cast<uint4*>(rec + (li >> 3) * (kTileRows * 128) + y * 128 + (((li & 7) ^ (y & 7)) << 4)) =
         make_uint4(o[0], o[1], o[2], o[3]);
     if (li == 0) {
-      float2 c = make_float2(0.f, -INFINITY);  // no row: no weight
+      float2 c = make_float2(-INFINITY, 0.f);  // no row: no weight
       if (r < nrows) {
         const float2 s = a.stat[(int64_t)(sq.begin + r / R) * a.b.H + g * R + r % R];
-        c = make_float2(qs.factor, log2f(s.y) - s.x);
+        c = make_float2(top[k] < INFINITY ? log2f(s.y) - s.x : NAN, common ? all.factor : own.factor);
       }
-      float* to = reinterpret_cast<float*>(rec + L::kQBytes) + (y >> 1) * 4 + (y & 1);
-      to[0] = c.x;
-      to[2] = c.y;
+      consts[y] = c.x;
+      consts[kTileRows + y] = c.y;
     }
   }
 }
@@ -245,6 +271,16 @@ SPATTEN_DEV void bulk_load(uint32_t dst, const void* src, uint32_t bytes, SBar b
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar.a)
                : "memory");
+}
+
+// Waits for the loads under way; r, which one of them fills, is used behind this only.
+SPATTEN_DEV void tmem_wait_ld32(float (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+               "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+               "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+               "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+               ::"memory");
 }
 
 // Four codes in order as two f16 pairs.
@@ -267,37 +303,54 @@ SPATTEN_DEV uint2 widen4(uint32_t w) {
 struct Items {
   const PagedWeighParams& p;
   const WeighPlan& w;
-  const uint32_t* pre;
+  const uint32_t* pre;  // items before each pair of sequences
+  int R;
   uint32_t next_item, total;
-  // the item
+  // the sequence: its items, its blocks of keys and chunks of rows
+  uint32_t from, to, kt, ch;
   PagedSeq sq;
-  int b, g, c, k0, lim, nrows, t0, t1;  // row tiles [t0, t1)
+  int b, lim, nrows;
+  // the item: row tiles [t0, t1)
+  int g, c, k0, t0, t1;
 
   static SPATTEN_DEV int limit(const PagedSeq& s) { return max(min(s.old + s.n, s.len), 0); }
   static SPATTEN_DEV unsigned long long count(const PagedWeighParams& p, const WeighPlan& w, int b) {
+    if (b >= p.a.b.B) return 0;
     const PagedSeq s = paged_seq(p.a.b, p.a.c, b);
     const int R = p.a.b.H / p.a.c.G, rows = s.n * R;
     if (rows <= p.rows_over) return 0;
     return (unsigned long long)p.a.c.G * ((rows + w.chunk - 1) / w.chunk) * ((limit(s) + kKeys - 1) / kKeys);
   }
+  SPATTEN_DEV Items(const PagedWeighParams& p, const WeighPlan& w, const uint32_t* pre, uint32_t first, uint32_t total)
+      : p(p), w(w), pre(pre), R(p.a.b.H / p.a.c.G), next_item(first), total(total), from(0), to(0) {}
   SPATTEN_DEV bool next() {
     while (next_item < total) {
       const uint32_t u = next_item;
       next_item += gridDim.x;
-      int lo = 0;
-      for (int hi = p.a.b.B; hi - lo > 1;) {  // the sequence of item u
-        const int mid = (lo + hi) >> 1;
-        if (pre[mid] <= u) lo = mid; else hi = mid;
+      if (u < from || u >= to) {
+        int lo = 0;
+        for (int hi = (p.a.b.B + 1) / 2; hi - lo > 1;) {  // the pair of item u
+          const int mid = (lo + hi) >> 1;
+          if (pre[mid] <= u) lo = mid; else hi = mid;
+        }
+        b = 2 * lo;
+        from = pre[lo];
+        to = from + (uint32_t)count(p, w, b);
+        if (u >= to) {
+          ++b;
+          from = to;
+          to = pre[lo + 1];
+        }
+        sq = paged_seq(p.a.b, p.a.c, b);
+        lim = limit(sq);
+        nrows = sq.n * R;
+        kt = (lim + kKeys - 1) / kKeys;
+        ch = (nrows + w.chunk - 1) / w.chunk;
       }
-      b = lo;
-      sq = paged_seq(p.a.b, p.a.c, b);
-      const int R = p.a.b.H / p.a.c.G;
-      lim = limit(sq);
-      nrows = sq.n * R;
-      const uint32_t kt = (lim + kKeys - 1) / kKeys, ch = (nrows + w.chunk - 1) / w.chunk, x = u - pre[b];
-      k0 = (int)(x % kt) * kKeys;
-      c = (int)(x / kt % ch);
-      g = (int)(x / kt / ch);
+      const uint32_t x = (u - from) / kt;
+      k0 = (int)(u - from - x * kt) * kKeys;
+      g = (int)(x / ch);
+      c = (int)(x - g * ch);
       t0 = c * (w.chunk / kTileRows);
       t1 = min(t0 + w.chunk / kTileRows, (nrows + kTileRows - 1) / kTileRows);
       if (!p.a.tree && k0 > sq.old) t0 = max(t0, (int)min((int64_t)(k0 - sq.old) * R / kTileRows, (int64_t)INT_MAX));
@@ -308,19 +361,18 @@ struct Items {
 };
 
 template <int KV, int D>
-__global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const PagedWeighParams p, const WeighPlan w) {
+__global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const PagedWeighParams p, const WeighPlan w) {
   using L = Lay<D>;
-  constexpr int RING = L::kRing;
   extern __shared__ uint8_t smem_raw[];
   grid_dependents();
   grid_wait();
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const uint32_t bars = smem_u32(sm + L::oBar);
-  const SBarArr q_full{bars}, q_empty{bars + 8 * RING}, c_full{bars + 16 * RING},
-      c_empty{bars + 16 * RING + 8 * kConsts}, s_full{bars + 16 * RING + 16 * kConsts},
-      s_empty{bars + 16 * RING + 16 * kConsts + 16}, rest{bars + 16 * RING + 16 * kConsts + 32};
-  const SBar k_full = rest[0], drain = rest[1];
+  const SBarArr q_full{bars}, q_empty{bars + 8 * kRing}, k_full{bars + 16 * kRing}, k_empty{bars + 24 * kRing},
+      c_full{bars + 32 * kRing}, c_empty{bars + 32 * kRing + 8 * kConsts}, s_full{bars + 32 * kRing + 16 * kConsts},
+      s_empty{bars + 32 * kRing + 16 * kConsts + 16}, rest{bars + 32 * kRing + 16 * kConsts + 32};
+  const SBar drain = rest[0];
   volatile int* abort = reinterpret_cast<volatile int*>(sm + L::oAbort);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + L::oTmem);
   uint32_t* pre = reinterpret_cast<uint32_t*>(sm + L::oPre);
@@ -329,9 +381,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.c.G, R = a.b.H / G;
 
   if (tid == 0) {
-    for (int i = 0; i < RING; ++i) {
+    for (int i = 0; i < kRing; ++i) {
       mbar_init(q_full[i], 1);
       mbar_init(q_empty[i], 1);
+      mbar_init(k_full[i], kWideWarps);
+      mbar_init(k_empty[i], kSumWarps + 1);  // the scales are read, and the products done
     }
     for (int i = 0; i < kConsts; ++i) {
       mbar_init(c_full[i], 1);
@@ -341,20 +395,20 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
       mbar_init(s_full[i], 1);
       mbar_init(s_empty[i], kSumWarps);
     }
-    mbar_init(k_full, kSumWarps);
     mbar_init(drain, 1);
     fence_barrier_init();
     *abort = 0;
     pre[0] = 0;
   }
-  if (warp == kSumWarps + 1) {
-    tmem_alloc(tslot, 256);
+  if (warp == kSumWarps + kWideWarps + 1) {
+    tmem_alloc(tslot, 512);
     tmem_relinquish();
   }
   unsigned long long U = 0;
-  for (int base = 0; base < a.b.B; base += kThreads) {
-    const int b = base + tid;
-    unsigned long long x = b < a.b.B ? Items::count(p, w, b) : 0;
+  const int pairs = (a.b.B + 1) / 2;
+  for (int base = 0; base < pairs; base += kThreads) {
+    const int i = base + tid;
+    unsigned long long x = i < pairs ? Items::count(p, w, 2 * i) + Items::count(p, w, 2 * i + 1) : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long y = __shfl_up_sync(0xffffffffu, x, o);
@@ -363,11 +417,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
     if (lane == 31) scan[warp] = x;
     __syncthreads();
     unsigned long long front = U;
-    for (int i = 0; i < kThreads / 32; ++i) {
-      if (i < warp) front += scan[i];
-      U += scan[i];
+    for (int k = 0; k < kThreads / 32; ++k) {
+      if (k < warp) front += scan[k];
+      U += scan[k];
     }
-    if (b < a.b.B) pre[b + 1] = (uint32_t)(front + x);
+    if (i < pairs) pre[i + 1] = (uint32_t)(front + x);
     __syncthreads();
   }
   tc_fence_before();
@@ -375,105 +429,92 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
   tc_fence_after();
   const uint32_t tmem = *tslot;
   // (the attention's host check leaves 32 bits for sequences that share no rows)
-  Items it{p, w, pre, blockIdx.x, U >> 32 ? 0u : (uint32_t)U};
+  Items it(p, w, pre, blockIdx.x, U >> 32 ? 0u : (uint32_t)U);
 
   if (warp < kSumWarps) {
-    // ------------------------------------------------------------ keys to f16, sums of the weights
-    constexpr int CH = D / 16, KPS = 32 * kSumWarps / CH, STEPS = kKeys / KPS;  // chunks of a key, keys of a step
-    const int col = CH == 8 ? (tid & 3) + ((tid >> 1) & 4) : tid & 3;
-    const int key = CH == 8 ? ((tid >> 2) & 1) + 2 * (tid >> 4) : tid >> 2;
-    const int page = a.c.page, page_log = __ffs(page) - 1;
-    const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * kTileRows;
-    uint32_t n = 0;  // tiles
+    // ------------------------------------------------------------ sums of the weights
+    // a thread takes a key and half of a tile's rows (four warps per scheduler hide one
+    // another's latencies, which two did not)
+    constexpr int kHalf = kTileRows / 2;
+    const int side = warp >> 3, key = tid & (kKeys - 1);
+    const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + ((warp >> 2) & 1) * kTileRows + side * kHalf;
+    uint32_t n = 0, items = 0;  // tiles, blocks of keys
     bool alive = true;
     while (alive && it.next()) {
-      // (the item before is through: its last scores were there)
-      int pid[STEPS];
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int slot = it.k0 + key + KPS * i;
-        pid[i] = slot < it.lim ? paged_page(a.c, it.b, slot >> page_log) : -1;
-      }
-      const int slot = it.k0 + tid;
-      const int pid_s = slot < it.lim ? paged_page(a.c, it.b, slot >> page_log) : -1;
-      uint4 x[STEPS];
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int at = (it.k0 + key + KPS * i) & (page - 1);
-        x[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (pid[i] >= 0)
-          x[i] = *reinterpret_cast<const uint4*>(a.c.k + (((int64_t)pid[i] * G + it.g) * page + at) * D + col * 16);
-      }
-      const float ks = pid_s >= 0 ? a.c.k_scale[(int64_t)pid_s * G + it.g] : 0.f;
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int row = key + KPS * i;
-        const uint2 e = widen4<KV>(x[i].x), f = widen4<KV>(x[i].y), h = widen4<KV>(x[i].z), o = widen4<KV>(x[i].w);
-        uint8_t* dst = sm + L::oK + (row >> 7) * L::kKHalf + (col >> 2) * (128 * 128) + (row & 127) * 128;
-        const int sub = (col & 3) * 2;
-        *reinterpret_cast<uint4*>(dst + ((sub ^ (row & 7)) << 4)) = make_uint4(e.x, e.y, f.x, f.y);
-        *reinterpret_cast<uint4*>(dst + (((sub + 1) ^ (row & 7)) << 4)) = make_uint4(h.x, h.y, o.x, o.y);
-      }
-      fence_proxy_async_smem();
+      const uint32_t kb = items % kRing;
+      if (!__all_sync(0xffffffffu, mbar_wait(k_full[kb], (items / kRing) & 1, kErr | 8, abort))) break;
+      const float ks = *reinterpret_cast<const float*>(sm + L::oScale + (kb * kKeys + key) * 4);
       __syncwarp();
-      mbar_arrive_elect(k_full);
-
-      const float2 ks2 = make_float2(ks, ks);
+      mbar_arrive_elect(k_empty[kb]);
+      ++items;
+      const int slot = it.k0 + key;
       float total = 0.f;
       float2 sum = make_float2(0.f, 0.f);
-      const int last = min(it.k0 + (warp << 5) + 31, it.lim - 1);  // key of the warp
+      const int last = min(it.k0 + (key | 31), it.lim - 1);  // key of the warp
       for (int t = it.t0; t < it.t1; ++t, ++n) {
         const uint32_t buf = n & 1, cs = n % kConsts;
         bool ok = mbar_wait(s_full[buf], (n >> 1) & 1, kErr | 1, abort);
         ok = ok && mbar_wait(c_full[cs], (n / kConsts) & 1, kErr | 2, abort);
         if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
         tc_fence_after();
-        float s[kTileRows];
-        tmem_ld32f(ts + buf * 128, s);
-        tmem_ld32f(ts + buf * 128 + 32, s + 32);
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        mbar_arrive_elect(s_empty[buf]);
-        const float4* cst = reinterpret_cast<const float4*>(sm + L::oC + cs * kConstBytes);
-        const int r0 = t * kTileRows;
-        const int sees = it.sq.old + (a.tree ? 0 : r0 / R + 1);  // slots before it are seen by every row of the tile
-        auto weights2 = [&](int k) {  // of rows 2 k and 2 k + 1
-          const float4 c = cst[k];
-          const float2 y = __ffma2_rn(make_float2(s[2 * k], s[2 * k + 1]), __fmul2_rn(make_float2(c.x, c.y), ks2),
-                                      make_float2(c.z, c.w));
-          return make_float2(fast_exp2(y.x), fast_exp2(y.y));
-        };
-        if (last < sees) {
+        const int r0 = t * kTileRows + side * kHalf, groups = (min(kHalf, it.nrows - r0) + kGroup - 1) / kGroup;
+        // whether every row of the half sees the warp's keys: row r0 sees slots up to sq.old + r0 / R
+        const bool seen = last < it.sq.old || (!a.tree && (int64_t)(last - it.sq.old) * it.R <= r0);
+        // the first row of the half that sees the key, in the causal form
+        const int f = a.tree || seen ? 0
+                          : (int)min(max((int64_t)(slot - it.sq.old) * R - r0, (int64_t)0), (int64_t)kHalf);
+        const bool some = groups > 0 && __any_sync(0xffffffffu, f < kHalf);
+        const float* cst = reinterpret_cast<const float*>(sm + L::oC + cs * kConstBytes);
+        const float4* bs = reinterpret_cast<const float4*>(cst + side * kHalf);
+        const float cq = cst[2 * kTileRows];
+        const float2 f2 = make_float2(cq * ks, cq * ks);
+        // (loops that are not unrolled keep the roles' code within the instruction caches)
+        if (some && seen && cq != 0.f) {
+#pragma unroll 1
+          for (int q = 0; q < groups; ++q) {
+            float s[kGroup];
+            tmem_ld32f(ts + buf * 2 * kTileRows + q * kGroup, s);
+            tmem_wait_ld32(s);
 #pragma unroll
-          for (int k = 0; k < kTileRows / 2; ++k) sum = __fadd2_rn(sum, weights2(k));
-        } else if (!a.tree) {
-          // the first row of the tile that sees the key
-          const int64_t first = max((int64_t)(slot - it.sq.old) * R - r0, (int64_t)0);
-          if (__any_sync(0xffffffffu, first < kTileRows)) {
-            const int f = (int)min(first, (int64_t)kTileRows);
-#pragma unroll
-            for (int k = 0; k < kTileRows / 2; ++k) {
-              const float2 y = weights2(k);
-              sum = __fadd2_rn(sum, make_float2(2 * k >= f ? y.x : 0.f, 2 * k + 1 >= f ? y.y : 0.f));
+            for (int k = 0; k < kGroup / 4; ++k) {
+              const float4 b = bs[q * (kGroup / 4) + k];
+              float2 y = __ffma2_rn(make_float2(s[4 * k], s[4 * k + 1]), f2, make_float2(b.x, b.y));
+              float2 z = __ffma2_rn(make_float2(s[4 * k + 2], s[4 * k + 3]), f2, make_float2(b.z, b.w));
+              y = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+              z = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+              sum = __fadd2_rn(sum, __fadd2_rn(y, z));
             }
           }
-        } else {
+        } else if (some) {
           const int j = slot - it.sq.old;  // the key's place among the new tokens
-          const bool none = (j >> 5) >= a.words;
+#pragma unroll 1
+          for (int q = 0; q < groups; ++q) {
+            uint32_t sees;  // rows of the group that see the key
+            if (!a.tree) {
+              const int first = f - q * kGroup;
+              sees = first <= 0 ? 0xFFFFFFFFu : first >= kGroup ? 0u : 0xFFFFFFFFu << first;
+            } else {
+              sees = j < 0 ? 0xFFFFFFFFu : 0u;
+              for (int k = 0; j >= 0 && (j >> 5) < a.words && k < kGroup; ++k) {
+                const int i = min((r0 + q * kGroup + k) / it.R, it.sq.n - 1);  // (rows behind the last weigh nothing)
+                sees |= ((*(a.tree + (it.sq.begin + i) * a.tree_st + (j >> 5)) >> (j & 31)) & 1u) << k;
+              }
+            }
+            float s[kGroup];
+            tmem_ld32f(ts + buf * 2 * kTileRows + q * kGroup, s);
+            tmem_wait_ld32(s);
+            __syncwarp();
 #pragma unroll
-          for (int k = 0; k < kTileRows / 2; ++k) {
-            const float2 y = weights2(k);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int i = min((r0 + 2 * k + h) / R, it.sq.n - 1);  // (rows behind the last one weigh nothing)
-              bool see = j < 0;
-              if (!see && !none) see = (*(a.tree + (it.sq.begin + i) * a.tree_st + (j >> 5)) >> (j & 31)) & 1u;
-              if (see) (h ? sum.y : sum.x) += h ? y.y : y.x;
+            for (int k = 0; k < kGroup; ++k) {
+              const int r = side * kHalf + q * kGroup + k;
+              const float y = fast_exp2(fmaf(s[k], cst[kTileRows + r] * ks, cst[r]));
+              if ((sees >> k) & 1u) (k & 1 ? sum.y : sum.x) += y;
             }
           }
         }
+        tc_fence_before();
         __syncwarp();
+        mbar_arrive_elect(s_empty[buf]);
         mbar_arrive_elect(c_empty[cs]);
         if ((t + 1 - it.t0) % kFoldTiles == 0) {
           total += sum.x + sum.y;
@@ -481,9 +522,64 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
         }
       }
       if (alive && slot < it.lim)
-        w.partial[(((int64_t)it.c * a.b.B + it.b) * G + it.g) * a.c.max_pages * page + slot] = total + (sum.x + sum.y);
+        w.partial[((((int64_t)it.c * 2 + side) * a.b.B + it.b) * G + it.g) * a.c.max_pages * a.c.page + slot] =
+            total + (sum.x + sum.y);
     }
-  } else if (warp == kSumWarps) {
+  } else if (warp < kSumWarps + kWideWarps) {
+    // ------------------------------------------------------------ keys to f16
+    constexpr int CH = D / 16, KPS = 32 * kWideWarps / CH, STEPS = kKeys / KPS, FLY = 8;  // chunks of a key, keys of a step
+    const int x = tid - 32 * kSumWarps;
+    const int col = CH == 8 ? (x & 3) + ((x >> 1) & 4) : x & 3;
+    const int key = CH == 8 ? ((x >> 2) & 1) + 2 * (x >> 4) : x >> 2;
+    const int page = a.c.page, page_log = __ffs(page) - 1;
+    uint32_t items = 0;
+    while (it.next()) {
+      const uint32_t kb = items % kRing;
+      auto page_of = [&](int i) {
+        const int slot = it.k0 + i;
+        return slot < it.lim ? paged_page(a.c, it.b, slot >> page_log) : -1;
+      };
+      float ks[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int q = page_of(x + 128 * i);
+        ks[i] = q >= 0 ? a.c.k_scale[(int64_t)q * G + it.g] : 0.f;
+      }
+      bool ok = true;
+#pragma unroll 1
+      for (int s0 = 0; s0 < STEPS; s0 += FLY) {
+        int pid[FLY];
+#pragma unroll
+        for (int i = 0; i < FLY; ++i) pid[i] = page_of(key + KPS * (s0 + i));
+        uint4 c[FLY];
+#pragma unroll
+        for (int i = 0; i < FLY; ++i) {
+          const int at = (it.k0 + key + KPS * (s0 + i)) & (page - 1);
+          c[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (pid[i] >= 0)
+            c[i] = *reinterpret_cast<const uint4*>(a.c.k + (((int64_t)pid[i] * G + it.g) * page + at) * D + col * 16);
+        }
+        if (s0 == 0) ok = mbar_wait(k_empty[kb], ((items / kRing) & 1) ^ 1, kErr | 9, abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+        for (int i = 0; i < FLY; ++i) {
+          const int row = key + KPS * (s0 + i);
+          const uint2 e = widen4<KV>(c[i].x), f = widen4<KV>(c[i].y), h = widen4<KV>(c[i].z), o = widen4<KV>(c[i].w);
+          uint8_t* dst = sm + L::oK + (kb * 2 + (row >> 7)) * L::kKHalf + (col >> 2) * (128 * 128) + (row & 127) * 128;
+          const int sub = (col & 3) * 2;
+          *reinterpret_cast<uint4*>(dst + ((sub ^ (row & 7)) << 4)) = make_uint4(e.x, e.y, f.x, f.y);
+          *reinterpret_cast<uint4*>(dst + (((sub + 1) ^ (row & 7)) << 4)) = make_uint4(h.x, h.y, o.x, o.y);
+        }
+      }
+      if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) *reinterpret_cast<float*>(sm + L::oScale + (kb * kKeys + x + 128 * i) * 4) = ks[i];
+      fence_proxy_async_smem();
+      __syncwarp();
+      mbar_arrive_elect(k_full[kb]);
+      ++items;
+    }
+  } else if (warp == kSumWarps + kWideWarps) {
     // ------------------------------------------------------------ query rows
     if (lane == 0) {
       uint32_t n = 0;
@@ -492,8 +588,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
       while (ok && it.next()) {
         const uint8_t* rec = w.tiles + (it.g * w.tiles_g + first_tile(it.sq, R, it.b)) * (int64_t)L::kRecord;
         for (int t = it.t0; t < it.t1; ++t) {
-          const uint32_t qs = n % RING, cs = n % kConsts;
-          ok = mbar_wait(q_empty[qs], ((n / RING) & 1) ^ 1, kErr | 3, abort) &&
+          const uint32_t qs = n % kRing, cs = n % kConsts;
+          ok = mbar_wait(q_empty[qs], ((n / kRing) & 1) ^ 1, kErr | 3, abort) &&
                mbar_wait(c_empty[cs], ((n / kConsts) & 1) ^ 1, kErr | 4, abort);
           if (!ok) break;
           const uint8_t* src = rec + (int64_t)t * L::kRecord;
@@ -507,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
       // no copy is under way when the CTA leaves (they are long done unless a wait ran out)
       const long long start = clock64();
       for (uint32_t i = n > (uint32_t)kConsts ? n - kConsts : 0; i < n; ++i) {
-        while (i + RING >= n && !mbar_try_wait(q_full[i % RING], (i / RING) & 1) && clock64() - start < kWaitLimitCycles) {
+        while (i + kRing >= n && !mbar_try_wait(q_full[i % kRing], (i / kRing) & 1) && clock64() - start < kWaitLimitCycles) {
         }
         while (!mbar_try_wait(c_full[i % kConsts], (i / kConsts) & 1) && clock64() - start < kWaitLimitCycles) {
         }
@@ -520,25 +616,29 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
       uint32_t n = 0, items = 0;
       bool ok = true;
       while (ok && it.next()) {
-        ok = mbar_wait(k_full, items++ & 1, kErr | 5, abort);
+        const uint32_t kb = items % kRing;
+        ok = mbar_wait(k_full[kb], (items / kRing) & 1, kErr | 5, abort);
         for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
-          const uint32_t qs = n % RING, buf = n & 1;
+          const uint32_t qs = n % kRing, buf = n & 1;
           ok = mbar_wait(s_empty[buf], ((n >> 1) & 1) ^ 1, kErr | 6, abort) &&
-               mbar_wait(q_full[qs], (n / RING) & 1, kErr | 7, abort);
+               mbar_wait(q_full[qs], (n / kRing) & 1, kErr | 7, abort);
           if (!ok) break;
           tc_fence_after();
           const uint64_t q = smem_desc_sw128(smem_u32(sm + L::oQ + qs * L::kQBytes), 16, 1024);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint64_t k = smem_desc_sw128(smem_u32(sm + L::oK + h * L::kKHalf), 16, 1024);
+            const uint64_t k = smem_desc_sw128(smem_u32(sm + L::oK + (kb * 2 + h) * L::kKHalf), 16, 1024);
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i)  // the descriptors' addresses count 16 bytes
-              mma_f16(tmem + buf * 128 + h * kTileRows, k + (((i >> 2) * (128 * 128) + (i & 3) * 32) >> 4),
-                      q + (((i >> 2) * (kTileRows * 128) + (i & 3) * 32) >> 4), idesc, i > 0);
+            for (int i = 0; i < D / 16; ++i) {  // the descriptors' addresses count 16 bytes
+              const uint32_t at = ((i >> 2) * (128 * 128) + (i & 3) * 32) >> 4;
+              mma_f16(tmem + (buf * 2 + h) * kTileRows, k + at, q + at, idesc, i > 0);
+            }
           }
           mma_commit(s_full[buf]);
           mma_commit(q_empty[qs]);
         }
+        if (ok) mma_commit(k_empty[kb]);
+        ++items;
       }
       // every MMA issued has completed before the tensor memory is freed
       mma_commit(drain);
@@ -549,9 +649,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_weigh_tc_kernel(const Paged
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kSumWarps + 1) {
+  if (warp == kSumWarps + kWideWarps + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -573,10 +673,11 @@ __global__ void __launch_bounds__(kSlotThreads) paged_weigh_sum_kernel(const Pag
     const int g = g0 + h;
     const float4 was = x.before(p, g);
     float add[kQuad] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 2
     for (int c = 0; c < c1; ++c) {
-      const float4 y = *reinterpret_cast<const float4*>(w.partial + (((int64_t)c * a.b.B + b) * G + g) * slots + x.slot);
-      const float part[kQuad] = {y.x, y.y, y.z, y.w};
+      const float* at = w.partial + (((int64_t)c * 2 * a.b.B + b) * G + g) * slots + x.slot;
+      const float4 y = *reinterpret_cast<const float4*>(at), z = *reinterpret_cast<const float4*>(at + a.b.B * G * slots);
+      const float part[kQuad] = {y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w};
       // a chunk of which no row sees a slot has left nothing for it
       const int64_t seen = a.tree ? INT64_MAX : (int64_t)x.old + ((int64_t)min((c + 1) * w.chunk, nrows) - 1) / R + 1;
 #pragma unroll
@@ -594,7 +695,7 @@ int64_t most_rows(const PagedWeighParams& p) { return (int64_t)p.a.b.max_tokens 
 size_t plan_for(const PagedWeighParams& p, void* ws, WeighPlan& x) {
   const PagedAttendParams& a = p.a;
   const int64_t rows = most_rows(p), slots = (int64_t)a.c.max_pages * a.c.page;
-  const int64_t fit = std::max<int64_t>(1, ((int64_t)1 << 28) / std::max<int64_t>(1, slots * a.b.B * a.c.G));
+  const int64_t fit = std::max<int64_t>(1, ((int64_t)1 << 27) / std::max<int64_t>(1, slots * a.b.B * a.c.G));
   const int64_t most = std::min<int64_t>(std::min<int64_t>(8, fit), (rows + 511) / 512);
   x.chunk = (int)((rows + most * kTileRows - 1) / (most * kTileRows) * kTileRows);
   x.chunks = (int)((rows + x.chunk - 1) / x.chunk);
@@ -603,7 +704,7 @@ size_t plan_for(const PagedWeighParams& p, void* ws, WeighPlan& x) {
   const size_t tiles = align256((size_t)x.tiles_g * a.c.G * (a.c.D == 128 ? Lay<128>::kRecord : Lay<64>::kRecord));
   x.tiles = w;
   x.partial = reinterpret_cast<float*>(w + (w ? tiles : 0));
-  return tiles + align256((size_t)x.chunks * a.b.B * a.c.G * slots * sizeof(float));
+  return tiles + align256((size_t)x.chunks * 2 * a.b.B * a.c.G * slots * sizeof(float));
 }
 
 template <int KV, int D>
@@ -624,7 +725,7 @@ cudaError_t tc_launch(const PagedWeighParams& p, bool bf16, const WeighPlan& w, 
   if (e != cudaSuccess) return e;
   const int64_t slots = (int64_t)a.c.max_pages * a.c.page;
   const double items = (double)a.b.B * a.c.G * w.chunks * ((slots + kKeys - 1) / kKeys);
-  e = launch_dependent(paged_weigh_tc_kernel<KV, D>, dim3((unsigned)std::min(2.0 * n_sm, items)), kThreads,
+  e = launch_dependent(paged_weigh_tc_kernel<KV, D>, dim3((unsigned)std::min((double)n_sm, items)), kThreads,
                        Lay<D>::bytes(a.b.B), st, p, w);
   if (e != cudaSuccess) return e;
   int heads;
