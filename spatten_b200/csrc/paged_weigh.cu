@@ -170,7 +170,8 @@ struct Lay {
   static constexpr int oQ = oK + kRing * 2 * kKHalf;         // [ring][D / 64][128][128 B]
   static constexpr int oC = oQ + kRing * kQBytes;            // [kConsts]
   static constexpr int oScale = oC + kConsts * kConstBytes;  // [ring][256] scales of the keys
-  static constexpr int oBar = oScale + kRing * kKeys * 4;
+  static constexpr int oItem = oScale + kRing * kKeys * 4;   // [ring] Item
+  static constexpr int oBar = oItem + kRing * 64;
   static constexpr int kBars = 4 * kRing + 2 * kConsts + 4 + 1;
   static constexpr int oTmem = oBar + kBars * 8;
   static constexpr int oAbort = oTmem + 4;
@@ -298,8 +299,18 @@ SPATTEN_DEV uint2 widen4(uint32_t w) {
   }
 }
 
+// What the sums and the products have to know of a block of keys. The warps that widen
+// it leave it beside it: working it out took each of the others a quarter of an item's time.
+struct Item {
+  int t0, t1;            // row tiles; none: the last item is behind
+  int k0, lim;           // first slot, end of the sequence
+  int old, n, begin;     // of its PagedSeq
+  int nrows;
+  int64_t partial;       // where the sums of the first key's even rows go
+};
+static_assert(sizeof(Item) <= 64, "two of them in Lay");
+
 // The items of a CTA: 256 keys of a (sequence, KV head) by a chunk of its rows.
-// Every role walks them by itself.
 struct Items {
   const PagedWeighParams& p;
   const WeighPlan& w;
@@ -440,9 +451,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
     const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + ((warp >> 2) & 1) * kTileRows + side * kHalf;
     uint32_t n = 0, items = 0;  // tiles, blocks of keys
     bool alive = true;
-    while (alive && it.next()) {
+    while (alive) {
       const uint32_t kb = items % kRing;
       if (!__all_sync(0xffffffffu, mbar_wait(k_full[kb], (items / kRing) & 1, kErr | 8, abort))) break;
+      const Item it = *reinterpret_cast<const Item*>(sm + L::oItem + kb * 64);
+      if (it.t0 == it.t1) break;
       const float ks = *reinterpret_cast<const float*>(sm + L::oScale + (kb * kKeys + key) * 4);
       __syncwarp();
       mbar_arrive_elect(k_empty[kb]);
@@ -459,10 +472,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
         tc_fence_after();
         const int r0 = t * kTileRows + side * kHalf, groups = (min(kHalf, it.nrows - r0) + kGroup - 1) / kGroup;
         // whether every row of the half sees the warp's keys: row r0 sees slots up to sq.old + r0 / R
-        const bool seen = last < it.sq.old || (!a.tree && (int64_t)(last - it.sq.old) * it.R <= r0);
+        const bool seen = last < it.old || (!a.tree && (int64_t)(last - it.old) * R <= r0);
         // the first row of the half that sees the key, in the causal form
         const int f = a.tree || seen ? 0
-                          : (int)min(max((int64_t)(slot - it.sq.old) * R - r0, (int64_t)0), (int64_t)kHalf);
+                          : (int)min(max((int64_t)(slot - it.old) * R - r0, (int64_t)0), (int64_t)kHalf);
         const bool some = groups > 0 && __any_sync(0xffffffffu, f < kHalf);
         const float* cst = reinterpret_cast<const float*>(sm + L::oC + cs * kConstBytes);
         const float4* bs = reinterpret_cast<const float4*>(cst + side * kHalf);
@@ -486,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
             }
           }
         } else if (some) {
-          const int j = slot - it.sq.old;  // the key's place among the new tokens
+          const int j = slot - it.old;  // the key's place among the new tokens
 #pragma unroll 1
           for (int q = 0; q < groups; ++q) {
             uint32_t sees;  // rows of the group that see the key
@@ -496,8 +509,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
             } else {
               sees = j < 0 ? 0xFFFFFFFFu : 0u;
               for (int k = 0; j >= 0 && (j >> 5) < a.words && k < kGroup; ++k) {
-                const int i = min((r0 + q * kGroup + k) / it.R, it.sq.n - 1);  // (rows behind the last weigh nothing)
-                sees |= ((*(a.tree + (it.sq.begin + i) * a.tree_st + (j >> 5)) >> (j & 31)) & 1u) << k;
+                const int i = min((r0 + q * kGroup + k) / R, it.n - 1);  // (rows behind the last weigh nothing)
+                sees |= ((*(a.tree + (it.begin + i) * a.tree_st + (j >> 5)) >> (j & 31)) & 1u) << k;
               }
             }
             float s[kGroup];
@@ -522,8 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
         }
       }
       if (alive && slot < it.lim)
-        w.partial[((((int64_t)it.c * 2 + side) * a.b.B + it.b) * G + it.g) * a.c.max_pages * a.c.page + slot] =
-            total + (sum.x + sum.y);
+        w.partial[it.partial + (side ? (int64_t)a.b.B * G * a.c.max_pages * a.c.page : 0) + key] = total + (sum.x + sum.y);
     }
   } else if (warp < kSumWarps + kWideWarps) {
     // ------------------------------------------------------------ keys to f16
@@ -533,8 +545,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
     const int key = CH == 8 ? ((x >> 2) & 1) + 2 * (x >> 4) : x >> 2;
     const int page = a.c.page, page_log = __ffs(page) - 1;
     uint32_t items = 0;
-    while (it.next()) {
+    for (bool ok = true; ok; ++items) {
       const uint32_t kb = items % kRing;
+      Item* const item = reinterpret_cast<Item*>(sm + L::oItem + kb * 64);
+      if (!it.next()) {
+        ok = mbar_wait(k_empty[kb], ((items / kRing) & 1) ^ 1, kErr | 9, abort);
+        if (__all_sync(0xffffffffu, ok)) {
+          if (x == 0) item->t0 = item->t1 = 0;
+          __syncwarp();
+          mbar_arrive_elect(k_full[kb]);
+        }
+        break;
+      }
       auto page_of = [&](int i) {
         const int slot = it.k0 + i;
         return slot < it.lim ? paged_page(a.c, it.b, slot >> page_log) : -1;
@@ -545,7 +567,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
         const int q = page_of(x + 128 * i);
         ks[i] = q >= 0 ? a.c.k_scale[(int64_t)q * G + it.g] : 0.f;
       }
-      bool ok = true;
 #pragma unroll 1
       for (int s0 = 0; s0 < STEPS; s0 += FLY) {
         int pid[FLY];
@@ -560,7 +581,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
             c[i] = *reinterpret_cast<const uint4*>(a.c.k + (((int64_t)pid[i] * G + it.g) * page + at) * D + col * 16);
         }
         if (s0 == 0) ok = mbar_wait(k_empty[kb], ((items / kRing) & 1) ^ 1, kErr | 9, abort);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
 #pragma unroll
         for (int i = 0; i < FLY; ++i) {
           const int row = key + KPS * (s0 + i);
@@ -571,13 +593,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
           *reinterpret_cast<uint4*>(dst + (((sub + 1) ^ (row & 7)) << 4)) = make_uint4(h.x, h.y, o.x, o.y);
         }
       }
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!ok) break;
+      if (x == 0) {
+        item->t0 = it.t0; item->t1 = it.t1; item->k0 = it.k0; item->lim = it.lim;
+        item->old = it.sq.old; item->n = it.sq.n; item->begin = it.sq.begin; item->nrows = it.nrows;
+        item->partial = (((int64_t)it.c * 2 * a.b.B + it.b) * G + it.g) * a.c.max_pages * page + it.k0;
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) *reinterpret_cast<float*>(sm + L::oScale + (kb * kKeys + x + 128 * i) * 4) = ks[i];
       fence_proxy_async_smem();
       __syncwarp();
       mbar_arrive_elect(k_full[kb]);
-      ++items;
     }
   } else if (warp == kSumWarps + kWideWarps) {
     // ------------------------------------------------------------ query rows
@@ -615,10 +641,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
       constexpr uint32_t idesc = instr_desc(1, 0, 0, 0, 128, kTileRows);
       uint32_t n = 0, items = 0;
       bool ok = true;
-      while (ok && it.next()) {
+      while (ok) {
         const uint32_t kb = items % kRing;
         ok = mbar_wait(k_full[kb], (items / kRing) & 1, kErr | 5, abort);
-        for (int t = it.t0; t < it.t1 && ok; ++t, ++n) {
+        if (!ok) break;
+        const int2 tiles = *reinterpret_cast<const int2*>(sm + L::oItem + kb * 64);
+        if (tiles.x == tiles.y) break;
+        for (int t = tiles.x; t < tiles.y && ok; ++t, ++n) {
           const uint32_t qs = n % kRing, buf = n & 1;
           ok = mbar_wait(s_empty[buf], ((n >> 1) & 1) ^ 1, kErr | 6, abort) &&
                mbar_wait(q_full[qs], (n / kRing) & 1, kErr | 7, abort);
