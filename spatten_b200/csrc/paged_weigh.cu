@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kSlotThreads) paged_weigh_scores_kernel(const 
     const float4* at = reinterpret_cast<const float4*>(src + g * slots * ROWS);
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const float4 y = at[i];
+      const float4 y = __ldcs(at + i);  // (read once)
       s[4 * i] = y.x; s[4 * i + 1] = y.y; s[4 * i + 2] = y.z; s[4 * i + 3] = y.w;
     }
     const float4 was = x.before(p, g);
@@ -540,6 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
   } else if (warp < kSumWarps + kWideWarps) {
     // ------------------------------------------------------------ keys to f16
     constexpr int CH = D / 16, KPS = 32 * kWideWarps / CH, STEPS = kKeys / KPS, FLY = 8;  // chunks of a key, keys of a step
+    static_assert(STEPS == FLY || STEPS == 2 * FLY, "one or two rounds");
     const int x = tid - 32 * kSumWarps;
     const int col = CH == 8 ? (x & 3) + ((x >> 1) & 4) : x & 3;
     const int key = CH == 8 ? ((x >> 2) & 1) + 2 * (x >> 4) : x >> 2;
@@ -567,33 +568,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
         const int q = page_of(x + 128 * i);
         ks[i] = q >= 0 ? a.c.k_scale[(int64_t)q * G + it.g] : 0.f;
       }
+      int pid[FLY];
+      uint4 c[FLY];
+      auto fetch = [&](int i, int step) {
+        const int at = (it.k0 + key + KPS * step) & (page - 1);
+        c[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (pid[i] >= 0)
+          c[i] = *reinterpret_cast<const uint4*>(a.c.k + (((int64_t)pid[i] * G + it.g) * page + at) * D + col * 16);
+      };
+#pragma unroll
+      for (int i = 0; i < FLY; ++i) pid[i] = page_of(key + KPS * i);
+#pragma unroll
+      for (int i = 0; i < FLY; ++i) fetch(i, i);
+      if (STEPS > FLY) {
+#pragma unroll
+        for (int i = 0; i < FLY; ++i) pid[i] = page_of(key + KPS * (FLY + i));
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(k_empty[kb], ((items / kRing) & 1) ^ 1, kErr | 9, abort));
+      if (!ok) break;
 #pragma unroll 1
       for (int s0 = 0; s0 < STEPS; s0 += FLY) {
-        int pid[FLY];
-#pragma unroll
-        for (int i = 0; i < FLY; ++i) pid[i] = page_of(key + KPS * (s0 + i));
-        uint4 c[FLY];
-#pragma unroll
-        for (int i = 0; i < FLY; ++i) {
-          const int at = (it.k0 + key + KPS * (s0 + i)) & (page - 1);
-          c[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (pid[i] >= 0)
-            c[i] = *reinterpret_cast<const uint4*>(a.c.k + (((int64_t)pid[i] * G + it.g) * page + at) * D + col * 16);
-        }
-        if (s0 == 0) ok = mbar_wait(k_empty[kb], ((items / kRing) & 1) ^ 1, kErr | 9, abort);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
 #pragma unroll
         for (int i = 0; i < FLY; ++i) {
           const int row = key + KPS * (s0 + i);
           const uint2 e = widen4<KV>(c[i].x), f = widen4<KV>(c[i].y), h = widen4<KV>(c[i].z), o = widen4<KV>(c[i].w);
+          if (s0 + FLY < STEPS) fetch(i, s0 + FLY + i);  // the next ones, under the other widenings
           uint8_t* dst = sm + L::oK + (kb * 2 + (row >> 7)) * L::kKHalf + (col >> 2) * (128 * 128) + (row & 127) * 128;
           const int sub = (col & 3) * 2;
           *reinterpret_cast<uint4*>(dst + ((sub ^ (row & 7)) << 4)) = make_uint4(e.x, e.y, f.x, f.y);
           *reinterpret_cast<uint4*>(dst + (((sub + 1) ^ (row & 7)) << 4)) = make_uint4(h.x, h.y, o.x, o.y);
         }
       }
-      if (!ok) break;
       if (x == 0) {
         item->t0 = it.t0; item->t1 = it.t1; item->k0 = it.k0; item->lim = it.lim;
         item->old = it.sq.old; item->n = it.sq.n; item->begin = it.sq.begin; item->nrows = it.nrows;
