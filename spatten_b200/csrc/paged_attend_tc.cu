@@ -346,21 +346,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attend_tc_kernel(const Page
         const int key0 = t * kKeys;
         const bool odd = key0 + kKeys > all || have != 15u || !(fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) >= 0.f);
         if (__builtin_expect(__any_sync(0xffffffffu, odd), 0)) {  // masked keys, factors below 0 or NaN: t itself
+          // the keys that the row sees, as bits (few instructions: this path is met once a line, and comes
+          // from beyond the instruction caches)
+          uint32_t sees[2];
 #pragma unroll
-          for (int k = 0; k < kKeys; ++k) {
-            s[k] *= a[k >> 4];
-            if (key0 + k >= lim || !((have >> (k >> 4)) & 1u)) s[k] = -INFINITY;
+          for (int h = 0; h < 2; ++h) {
+            const int left = lim - key0 - 32 * h;
+            sees[h] = left >= 32 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << left) - 1u;
+            sees[h] &= ((have >> (2 * h)) & 1u ? 0xFFFFu : 0u) | ((have >> (2 * h + 1)) & 1u ? 0xFFFF0000u : 0u);
+            if (tree && live)
+              sees[h] &= tree_bits(p.tree + (seg.sq.begin + i) * p.tree_st, p.words, key0 + 32 * h - seg.sq.old);
           }
-          if (tree && live) {
-            const uint32_t* words = p.tree + (seg.sq.begin + i) * p.tree_st;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t sees = tree_bits(words, p.words, key0 + 32 * h - seg.sq.old);
-#pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (!((sees >> k) & 1u)) s[32 * h + k] = -INFINITY;
-            }
-          }
+          for (int k = 0; k < kKeys; ++k) s[k] = (sees[k >> 5] >> (k & 31)) & 1u ? s[k] * a[k >> 4] : -INFINITY;
           a[0] = a[1] = a[2] = a[3] = 1.f;
         }
         float top = -INFINITY, topw = -INFINITY;
