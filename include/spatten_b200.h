@@ -411,7 +411,7 @@ int spatten_paged_tree(const spatten_paged_tree_args* a, void* stream);
  *    added to its weight. The slots of the new tokens start from 0 and take
  *    positions[row] (int32 [T]; NULL: the slot) as their position. The slots
  *    of a page without memory have none. Two sequences of one call must not
- *    share pages then. A NaN among a head's scores makes its weights NaN.
+ *    share pages, nor claim the same rows, then. A NaN among a head's scores makes its weights NaN.
  */
 typedef struct {
   spatten_paged_attend_args attend;

@@ -188,9 +188,10 @@ struct SelShared {
 constexpr size_t kMostShared = sizeof(SelShared) + kMaxWords * 4 + kEvictSlots / 8 / 32 * 12;
 static_assert(kMostShared <= 227 * 1024, "a CTA's shared memory");
 
-// Sum over the CTA's threads before this one, and the sum of all.
+// Sum over the CTA's threads before this one, and the sum of all. (The selection runs each
+// part of its code once, so its size is time: nothing in it is unrolled without need.)
 template <int NT>
-SPATTEN_DEV uint32_t block_scan(SelShared& sh, uint32_t x, uint32_t& total) {
+__device__ __noinline__ uint2 block_scan(SelShared& sh, uint32_t x) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t y = x;
 #pragma unroll
@@ -201,14 +202,8 @@ SPATTEN_DEV uint32_t block_scan(SelShared& sh, uint32_t x, uint32_t& total) {
   __syncthreads();
   if (lane == 31) sh.scan[warp] = y;
   __syncthreads();
-  uint32_t before = 0u;
-  total = 0u;
-#pragma unroll
-  for (int w = 0; w < NT / 32; ++w) {
-    if (w < warp) before += sh.scan[w];
-    total += sh.scan[w];
-  }
-  return before + y - x;
+  const uint32_t v = lane < NT / 32 ? sh.scan[lane] : 0u;
+  return make_uint2(__reduce_add_sync(0xffffffffu, lane < warp ? v : 0u) + y - x, __reduce_add_sync(0xffffffffu, v));
 }
 
 // The lowest m bits that are set in t.
@@ -256,7 +251,7 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
   // keys, the newest position, whether every slot has memory (pitch and runs are multiples of 32)
   int newest = INT_MIN;
   bool hole = false;
-#pragma unroll 4
+#pragma unroll 2
   for (int i = 4 * tid; i < n; i += 4 * NT) {
     const uint4 k = *reinterpret_cast<const uint4*>(key_at + i);
     const uint32_t x[4] = {k.x, k.y, k.z, k.w};
@@ -265,7 +260,7 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
     if (CACHED) *reinterpret_cast<uint4*>(keys + i) = k;
   }
   if (p.recent > 0) {
-#pragma unroll 4
+#pragma unroll 2
     for (int i = 4 * tid; i < n; i += 4 * NT) {
       const int4 k = *reinterpret_cast<const int4*>(place_at + i);
       const int x[4] = {k.x, k.y, k.z, k.w};
@@ -282,26 +277,20 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
       sh.red[warp][1] = any;
     }
     __syncthreads();
-    if (tid == 0) {
-      int m = INT_MIN;
-      uint32_t h = 0u;
-      for (int w = 0; w < NT / 32; ++w) {
-        m = max(m, (int)sh.red[w][0]);
-        h |= sh.red[w][1];
+    if (warp == 0) {
+      const bool in = lane < NT / 32;
+      const int m = __reduce_max_sync(0xffffffffu, in ? (int)sh.red[lane][0] : INT_MIN);
+      const uint32_t h = __reduce_max_sync(0xffffffffu, in ? sh.red[lane][1] : 0u);
+      if (lane == 0) {
+        sh.xch[0][0] = (uint32_t)m;
+        sh.xch[0][1] = h;
       }
-      sh.xch[0][0] = (uint32_t)m;
-      sh.xch[0][1] = h;
     }
     cl.sync();
-    uint32_t h = 0u;
-    newest = INT_MIN;
-#pragma unroll
-    for (int r = 0; r < kCluster; ++r) {
-      if (r >= CL) continue;
-      const uint2 x = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.xch[0][0], r));
-      newest = max(newest, (int)x.x);
-      h |= x.y;
-    }
+    const uint2 x = lane < CL ? *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.xch[0][0], lane))
+                              : make_uint2((uint32_t)INT_MIN, 0u);
+    newest = __reduce_max_sync(0xffffffffu, (int)x.x);
+    const uint32_t h = __reduce_max_sync(0xffffffffu, x.y);
     if (h) {  // left as it is
       if (rank == 0 && tid == 0) {
         head[0] = 0;
@@ -314,7 +303,7 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
   // the recent ones; how many they are, and the range of the keys of both classes
   {
     uint32_t cnt = 0u, lo0 = 0xFFFFFFFFu, hi0 = 0u, lo1 = 0xFFFFFFFFu, hi1 = 0u;
-#pragma unroll 4
+#pragma unroll 2
     for (int base = 0; base < words * 32; base += NT) {
       const int i = base + tid;
       bool r = false;
@@ -347,36 +336,30 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
       sh.red[warp][4] = hi1;
     }
     __syncthreads();
-    if (tid == 0) {
-      uint32_t x[5] = {0u, 0xFFFFFFFFu, 0u, 0xFFFFFFFFu, 0u};
-#pragma unroll 8
-      for (int w = 0; w < NT / 32; ++w) {
-        x[0] += sh.red[w][0];
-        x[1] = min(x[1], sh.red[w][1]);
-        x[2] = max(x[2], sh.red[w][2]);
-        x[3] = min(x[3], sh.red[w][3]);
-        x[4] = max(x[4], sh.red[w][4]);
-      }
+    if (warp == 0) {
+      const bool in = lane < NT / 32;
 #pragma unroll
-      for (int i = 0; i < 5; ++i) sh.xch[1][i] = x[i];
+      for (int i = 0; i < 5; ++i) {
+        const uint32_t v = in ? sh.red[lane][i] : (i & 1 ? 0xFFFFFFFFu : 0u);
+        const uint32_t y = i == 0 ? __reduce_add_sync(0xffffffffu, v)
+                                  : i & 1 ? __reduce_min_sync(0xffffffffu, v) : __reduce_max_sync(0xffffffffu, v);
+        if (lane == 0) sh.xch[1][i] = y;
+      }
     }
     cl.sync();
   }
-  uint32_t recents = 0u, r_lo = 0xFFFFFFFFu, r_hi = 0u, k_lo = 0xFFFFFFFFu, k_hi = 0u;
-#pragma unroll
-  for (int r = 0; r < kCluster; ++r) {
-    if (r >= CL) continue;
-    const uint4 x = *reinterpret_cast<const uint4*>(cl.map_shared_rank(&sh.xch[1][0], r));
-    recents += x.x;
-    k_lo = min(k_lo, x.y);
-    k_hi = max(k_hi, x.z);
-    r_lo = min(r_lo, x.w);
-    r_hi = max(r_hi, *cl.map_shared_rank(&sh.xch[1][4], r));
+  uint4 range = make_uint4(0u, 0xFFFFFFFFu, 0u, 0xFFFFFFFFu);
+  uint32_t r_hi = 0u;
+  if (lane < CL) {
+    range = *reinterpret_cast<const uint4*>(cl.map_shared_rank(&sh.xch[1][0], lane));
+    r_hi = *cl.map_shared_rank(&sh.xch[1][4], lane);
   }
+  const uint32_t recents = __reduce_add_sync(0xffffffffu, range.x);
+  uint32_t k_lo = __reduce_min_sync(0xffffffffu, range.y), k_hi = __reduce_max_sync(0xffffffffu, range.z);
   const bool cls = recents >= (uint32_t)keep;  // the class that is chosen from: the recent ones, or the others
   if (cls) {
-    k_lo = r_lo;
-    k_hi = r_hi;
+    k_lo = __reduce_min_sync(0xffffffffu, range.w);
+    k_hi = __reduce_max_sync(0xffffffffu, r_hi);
   }
   uint32_t need = cls ? keep : keep - recents;  // of the class; its largest keys
   // radix rounds: keys above k_hi are kept, the need-th largest lies in [k_lo, k_hi]
@@ -387,7 +370,7 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
     uint32_t* hist = sh.hist[round & 1];
     for (int i = tid; i < kBins; i += NT) hist[i] = 0u;
     __syncthreads();
-#pragma unroll 4
+#pragma unroll 2
     for (int i = tid; i < n; i += NT) {
       const uint32_t k = key(i);
       if (((prot[i >> 5] >> (i & 31)) & 1u) == (uint32_t)cls && k >= k_lo && k <= k_hi) atomicAdd(&hist[(k - k_lo) >> shift], 1u);
@@ -411,8 +394,7 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) mine += c[j];
-    uint32_t total;
-    uint32_t above = block_scan<NT>(sh, mine, total);
+    uint32_t above = block_scan<NT>(sh, mine).x;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       if (above < need && need <= above + c[j]) {
@@ -458,22 +440,18 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
     }
   }
   {
-    uint32_t total;
-    block_scan<NT>(sh, n_ties, total);
+    const uint32_t total = block_scan<NT>(sh, n_ties).y;
     if (tid == 0) sh.xch[2][0] = total;
     cl.sync();
   }
-  uint32_t before = 0u;
-#pragma unroll
-  for (int r = 0; r < kCluster; ++r)
-    if (r < rank) before += *cl.map_shared_rank(&sh.xch[2][0], r);
+  const uint32_t before = __reduce_add_sync(0xffffffffu, lane < rank ? *cl.map_shared_rank(&sh.xch[2][0], lane) : 0u);
   uint32_t left = whole || before >= need ? 0u : need - before;  // ties that this CTA's slots may still keep
   uint32_t n_dst = 0u, n_src = 0u;
   for (int base = 0; base < words; base += NT) {
     const int w = base + tid;
     const uint32_t t = w < words ? ties[w] : 0u;
-    uint32_t total;
-    const uint32_t at = block_scan<NT>(sh, __popc(t), total);
+    const uint2 ties_at = block_scan<NT>(sh, __popc(t));
+    const uint32_t at = ties_at.x;
     if (w < words) {
       const uint32_t k = kept[w] | (at < left ? lowest_bits(t, left - at) : 0u);
       kept[w] = k;
@@ -482,29 +460,20 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
       n_dst += __popc(front & ~k);
       n_src += __popc(k & ~front);
     }
-    left -= min(left, total);
+    left -= min(left, ties_at.y);
   }
   {
-    uint32_t td, ts;
-    block_scan<NT>(sh, n_dst, td);
-    block_scan<NT>(sh, n_src, ts);
+    const uint32_t td = block_scan<NT>(sh, n_dst).y, ts = block_scan<NT>(sh, n_src).y;
     if (tid == 0) {
       sh.xch[3][0] = td;
       sh.xch[3][1] = ts;
     }
     cl.sync();
   }
-  uint32_t d0 = 0u, s0 = 0u, moves = 0u;
-#pragma unroll
-  for (int r = 0; r < kCluster; ++r) {
-    if (r >= CL) continue;
-    const uint2 x = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.xch[3][0], r));
-    if (r < rank) {
-      d0 += x.x;
-      s0 += x.y;
-    }
-    moves += x.x;
-  }
+  const uint2 counts = lane < CL ? *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.xch[3][0], lane)) : make_uint2(0u, 0u);
+  const uint32_t moves = __reduce_add_sync(0xffffffffu, counts.x);
+  uint32_t d0 = __reduce_add_sync(0xffffffffu, lane < rank ? counts.x : 0u);
+  uint32_t s0 = __reduce_add_sync(0xffffffffu, lane < rank ? counts.y : 0u);
   int32_t* const dst = plan.dst + line * plan.cap;
   int32_t* const src = plan.src + line * plan.cap;
   int32_t* const first = plan.first + line * (plan.blocks + 1);
@@ -515,14 +484,13 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
   for (int base = 0; base < words; base += NT) {  // numbers of the words' first free and moving slots
     const int w = base + tid;
     const uint32_t k = w < words ? kept[w] : 0u, front = w < words ? front_of(w) : 0u;
-    uint32_t td, ts;
-    const uint32_t d = d0 + block_scan<NT>(sh, __popc(front & ~k), td), s = s0 + block_scan<NT>(sh, __popc(k & ~front), ts);
-    d0 += td;
-    s0 += ts;
+    const uint2 d = block_scan<NT>(sh, __popc(front & ~k)), s = block_scan<NT>(sh, __popc(k & ~front));
     if (w < words) {
-      prot[w] = d;
-      ties[w] = s;
+      prot[w] = d0 + d.x;
+      ties[w] = s0 + s.x;
     }
+    d0 += d.y;
+    s0 += s.y;
   }
   __syncthreads();
   for (int w = warp; w < words; w += NT / 32) {  // a slot per lane

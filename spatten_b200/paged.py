@@ -44,6 +44,7 @@ from . import _native as N
 
 _DT = {torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
 _KV = {torch.int8: N.KV_INT8, torch.float8_e4m3fn: N.KV_E4M3}
+_INT_MAX = 2 ** 31 - 1
 
 
 class PagedKVCache(namedtuple("PagedKVCache", "k v k_scale v_scale")):
@@ -233,7 +234,7 @@ def paged_tree(parents, cu_tokens, seq_lens, max_tokens):
     """Bits and positions of trees of drafted tokens: ``parents`` int32 [T]
     holds, per new token, its parent's place among its sequence's new tokens
     (which comes before its own), or -1 for a child of the cached tokens.
-    Returns (tree int32 [T, ceil(max_tokens / 32)], positions int32 [T]): bit j
+    Returns (tree int32 [T, ceil(min(max_tokens, T) / 32)], positions int32 [T]): bit j
     of a row's words is set if it sees new token j (itself and its ancestors);
     its position is that of the sequence's first new token plus its depth.
     At most 1024 tokens per sequence."""
@@ -244,7 +245,7 @@ def paged_tree(parents, cu_tokens, seq_lens, max_tokens):
     a.B, a.seq_lens = seq_lens.shape[0], _index(seq_lens, "seq_lens", dev, 1)
     a.parents = _index(parents, "parents", dev, 1)
     _fill_tokens(a, dev, cu_tokens, parents.shape[0], max_tokens)
-    a.tree_words = a.tree_stride = max(-(-a.max_tokens // 32), 1)
+    a.tree_words = a.tree_stride = max(-(-min(a.max_tokens, a.T) // 32), 1)
     tree, positions = parents.new_empty((a.T, a.tree_words)), parents.new_empty((a.T,))
     a.tree, a.positions = tree.data_ptr(), positions.data_ptr()
     _call(N.lib.spatten_paged_tree, dev, a)
@@ -265,7 +266,7 @@ def paged_attention(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_sc
     give each cached token, summed over the query heads of its KV head, is
     added to ``weights.weight``; the new tokens' own start at 0, and their
     ``weights.position`` becomes ``positions`` (int32 [T]; default: the slot).
-    Sequences must not share pages then."""
+    Sequences must not share pages, nor claim the same rows, then."""
     ext = N.PagedAttendExtArgs() if tree is not None or weights is not None else None
     a = N.PagedAttendArgs() if ext is None else ext.attend
     dev, (P, G, page, D) = _fill(a, cache, page_table, seq_lens)
@@ -322,7 +323,7 @@ def paged_evict(cache, weights, page_table, seq_lens, keep, recent=0, per_head=F
     a = N.PagedEvictArgs()
     dev, (P, G, page, _) = _fill(a, cache, page_table, seq_lens)
     _weights(a, weights, dev, (P, G, page))
-    a.keep, a.recent, a.per_head = int(keep), int(recent), bool(per_head)
+    a.keep, a.recent, a.per_head = min(int(keep), _INT_MAX), min(int(recent), _INT_MAX), bool(per_head)
     new_lens = torch.empty_like(seq_lens, memory_format=torch.contiguous_format)
     a.new_lens = new_lens.data_ptr()
     n = N.lib.spatten_paged_evict_workspace_size(a)

@@ -282,6 +282,51 @@ def test_weights_of_extreme_rows(n):
     assert abs(float(got[3].sum()) - 2 * n) < 1e-3 * n
 
 
+@pytest.mark.parametrize("n,R", [(1, 2), (3, 4), (80, 2)])
+@pytest.mark.parametrize("scale", [None, 0.0, -0.25])
+def test_weights_of_rows_far_apart(n, R, scale):
+    """Query rows whose magnitudes lie 2^40 apart, some of zeros; a scale of 0 or below it."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(18)
+    G, D, page, L = 2, 128, 32, 300
+    cache, table = _filled(E4, 12, G, page, D, g), _table(1, 10, 12, g)
+    q = torch.randn(n, G * R, D, generator=g)
+    q *= 2.0 ** torch.randint(-35, 4, (n, G * R, 1), generator=g)
+    q[n // 2, 0] = 0
+    q = q.to(BF16).cuda()
+    w = _weights(cache, g)
+    before = paged.PagedWeights(*(t.clone() for t in w))
+    args = (q, cache, table.cuda(), _i32([0, n]), _i32([L]), n)
+    out = paged.paged_attention(*args, sm_scale=scale, weights=w)
+    _check(out, q, cache, table, [0, n], [L], D ** -0.5 if scale is None else scale, None, before, w)
+
+
+def test_expanded_words_and_lists():
+    """One mask, one list of accepted tokens for all; limits beyond any length."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(20)
+    G, D, page, n = 1, 64, 16, 4
+    cu, lens = _cum([n] * 3), [n + 9, n + 30, n]
+    cache, table = _filled(I8, 12, G, page, D, g), _table(3, 4, 12, g)
+    q = torch.randn(cu[-1], 2, D, generator=g).to(F16).cuda()
+    mask = _i32([[5]])  # tokens 0 and 2
+    out = paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), n, tree=mask.expand(cu[-1], 1))
+    _check(out, q, cache, table, cu, lens, D ** -0.5, {t: frozenset((0, 2)) for t in range(cu[-1])})
+    before = _cpu(cache)
+    got = paged.paged_keep(cache, table.cuda(), _i32(cu), _i32(lens), _i32([[0, 2, -1]]).expand(3, 3))
+    moves, new = OT.keep(before, table, cu, lens, [[0, 2, -1]] * 3)
+    assert got.tolist() == new
+    _check_moved(cache, before, table, moves, new)
+    w = _weights(cache, g)
+    was = [t.clone() for t in (*cache, *w)]
+    assert paged.paged_evict(cache, w, table.cuda(), got, 2 ** 40, recent=2 ** 40).tolist() == new
+    assert all(torch.equal(a, b) for a, b in zip(was, (*cache, *w)))
+    moves = _evicted(cache, w, table, new, 5, recent=2 ** 31 - 1)
+    assert moves[1][0]
+    tree, pos = paged.paged_tree(_i32([-1] * 5), _i32([0, 5]), _i32([5]), 1 << 28)
+    assert tree.tolist() == [[1], [2], [4], [8], [16]] and pos.tolist() == [0] * 5
+
+
 def test_weights_long_and_offsets_past_32_bits():
     """A pool whose codes and weights lie beyond 2^32 bytes, pages at its end."""
     from spatten_b200 import paged
