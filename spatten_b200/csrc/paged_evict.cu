@@ -191,7 +191,7 @@ static_assert(kMostShared <= 227 * 1024, "a CTA's shared memory");
 // Sum over the CTA's threads before this one, and the sum of all. (The selection runs each
 // part of its code once, so its size is time: nothing in it is unrolled without need.)
 template <int NT>
-__device__ __noinline__ uint2 block_scan(SelShared& sh, uint32_t x) {
+SPATTEN_DEV uint2 block_scan(SelShared& sh, uint32_t x) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t y = x;
 #pragma unroll

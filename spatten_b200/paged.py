@@ -58,10 +58,9 @@ class PagedKVCache(namedtuple("PagedKVCache", "k v k_scale v_scale")):
     @property
     def native(self):
         """(device index, shape of the pool, C form without a page table)."""
-        try:
-            return self._native
-        except AttributeError:
-            pass
+        got = self.__dict__.get("_native")
+        if got is not None:
+            return got
         k, v, ks, vs = self
         dev, dt, shape = k.get_device(), k.dtype, k.shape
         if dev < 0:
@@ -107,23 +106,39 @@ def new_paged_weights(cache):
 
 def _weights(a, weights, dev, shape):
     """The weights beside a pool of ``shape`` into ``a``; their checks."""
-    for t, name, dt in zip(weights, ("weight", "position"), (torch.float32, torch.int32)):
-        if t.get_device() != dev:
-            raise ValueError(f"weights.{name}: on {t.device}, the cache is on cuda:{dev}")
-        if t.dtype != dt or t.shape != shape or not t.is_contiguous():
-            raise ValueError(f"weights.{name}: need a contiguous {dt} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    a.weight, a.position = weights[0].data_ptr(), weights[1].data_ptr()
+    w, p = weights
+    if w.get_device() != dev or p.get_device() != dev:
+        raise ValueError(f"weights.weight / position: on {w.device} and {p.device}, the cache is on cuda:{dev}")
+    if w.dtype is not torch.float32 or w.shape != shape or not w.is_contiguous():
+        raise ValueError(f"weights.weight: need a contiguous float32 {tuple(shape)}, got {w.dtype} {tuple(w.shape)}")
+    if p.dtype is not torch.int32 or p.shape != shape or not p.is_contiguous():
+        raise ValueError(f"weights.position: need a contiguous int32 {tuple(shape)}, got {p.dtype} {tuple(p.shape)}")
+    a.weight, a.position = w.data_ptr(), p.data_ptr()
 
 
 def _index(t, name, dev, dim, dtype=torch.int32):
     """Pointer of an index tensor; its checks."""
     if t.get_device() != dev:
         raise ValueError(f"{name}: on {t.device}, the cache is on cuda:{dev}")
-    if t.dtype != dtype or t.dim() != dim:
+    st = t.stride()
+    if t.dtype is not dtype or len(st) != dim:
         raise ValueError(f"{name}: {t.dtype} of {t.dim()} dimensions (need {dtype} of {dim})")
-    if t.stride()[-1] != 1 and t.shape[-1] > 1:
+    if st[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: last dimension must be contiguous")
     return t.data_ptr()
+
+
+def _like(q, shape):
+    """Uninitialised [T, heads, D] of q's type (its own shape, where it is contiguous, costs least)."""
+    return torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+
+
+def _scratch(n, t):
+    """n bytes of workspace (a multiple of 256) beside an int32 tensor, and their address."""
+    if not n:
+        return None, None
+    ws = t.new_empty((n // 4,))
+    return ws, ws.data_ptr()
 
 
 def _fill(a, cache, page_table, seq_lens):
@@ -277,7 +292,7 @@ def paged_attention(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_sc
     _fill_tokens(a, dev, cu_tokens, shape[0], max_tokens)
     a.q, a.q_st, a.q_sh = _rows(q, "q", dev, dt, shape)
     if out is None:
-        out = q.new_empty(shape)
+        out = _like(q, shape)
     a.out, a.o_st, a.o_sh = _rows(out, "out", dev, dt, shape)
     a.sm_scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
     if tree is not None:
@@ -300,8 +315,8 @@ def paged_attention(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_sc
     else:
         a, size, call = ext, N.lib.spatten_paged_attend_ext_workspace_size, N.lib.spatten_paged_attend_ext
     n = size(a)
-    ws = q.new_empty((n,), dtype=torch.uint8) if n else None
-    _call(call, dev, a, ws.data_ptr() if n else None, n)
+    ws, at = _scratch(n, seq_lens)
+    _call(call, dev, a, at, n)
     return out
 
 
@@ -327,8 +342,8 @@ def paged_evict(cache, weights, page_table, seq_lens, keep, recent=0, per_head=F
     new_lens = torch.empty_like(seq_lens, memory_format=torch.contiguous_format)
     a.new_lens = new_lens.data_ptr()
     n = N.lib.spatten_paged_evict_workspace_size(a)
-    ws = cache.k.new_empty((n,), dtype=torch.uint8) if n else None
-    _call(N.lib.spatten_paged_evict, dev, a, ws.data_ptr() if n else None, n)
+    ws, at = _scratch(n, seq_lens)
+    _call(N.lib.spatten_paged_evict, dev, a, at, n)
     return new_lens
 
 
