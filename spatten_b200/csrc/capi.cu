@@ -755,6 +755,7 @@ static int fill_paged_attend_ext(const spatten_paged_attend_ext_args* a, spatten
   if (a->positions && (!a->weight || !aligned(a->positions, 4)))
     return fail(SPATTEN_ERR_INVALID, "%s: positions without weight, or not 4-byte aligned", who);
   p.weight = a->weight; p.position = a->position; p.positions = a->positions;
+  p.a.by_pool = spatten::slot_places(p.a, true) < spatten::slot_places(p.a, false);
   if (p.weight) p.a.score_rows = spatten::paged_attend_score_rows(p.a);
   p.rows_over = p.a.score_rows ? spatten::kScoreRows : 0;
   return SPATTEN_OK;
@@ -771,7 +772,7 @@ static AttendExtParts attend_ext_parts(const spatten::PagedWeighParams& p) {
   x.scores = x.weigh = x.bytes = x.stats;
   if (!p.weight) return x;
   x.scores += align256((size_t)p.a.b.T * p.a.b.H * sizeof(float2));
-  x.weigh = x.scores + align256((size_t)p.a.b.B * p.a.c.G * p.a.c.max_pages * p.a.c.page * p.a.score_rows * 4);
+  x.weigh = x.scores + align256((size_t)spatten::slot_places(p.a, p.a.by_pool) * p.a.score_rows * 4);
   x.bytes = x.weigh + align256(spatten::paged_weigh_workspace(p));
   return x;
 }

@@ -68,11 +68,18 @@ struct PagedAttendParams {
   int words = 0;
   float2* stat = nullptr;          // or null: [T, H] reference m of a row's exponentials, 1 / their sum
   // or null: scores (log2) of sequences of at most kScoreRows query rows per KV
-  // head, [B, G, slots, score_rows], where an unmasked place's page has memory
+  // head, [slot_place][score_rows], where an unmasked place's page has memory
   float* score = nullptr;
   int score_rows = 0;
+  bool by_pool = false;            // see slot_places
 };
 constexpr int kScoreRows = 8;
+
+// What a call keeps for each of its slots (of which sequences share none) lies by
+// sequence and slot, [B, G, slots], or like the pool, [P, G, page]: whichever is smaller.
+inline int64_t slot_places(const PagedAttendParams& p, bool by_pool) {
+  return by_pool ? (int64_t)p.c.P * p.c.G * p.c.page : (int64_t)p.b.B * p.c.G * p.c.max_pages * p.c.page;
+}
 
 // The weights that a call's rows give the cached tokens (after the attention).
 struct PagedWeighParams {

@@ -396,7 +396,8 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     // slots that the tile's last and first row see
     const bool tree = EXT && p.tree;
     float* const score = EXT && p.score && nrows <= kScoreRows
-                             ? p.score + ((int64_t)b * G + g) * p.c.max_pages * page * p.score_rows : nullptr;
+                             ? p.score + (p.by_pool ? 0 : ((int64_t)b * G + g) * p.c.max_pages * page * p.score_rows)
+                             : nullptr;
     const int lim_max = min(sq.old + (tree ? sq.n : min((r0 + ROWS - 1) / R, sq.n - 1) + 1), sq.len);
     const int lim_min = min(sq.old + (tree ? 0 : r0 / R + 1), sq.len);
     const uint32_t t_end = min(t1, (uint32_t)(max(lim_max, 0) + kKeys - 1) / kKeys);
@@ -428,6 +429,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     };
     const uint32_t ring = smem_u32(dsm) + warp * ST * SH::kStageBytes;
     uint32_t row_l = kNoRow, have_l = 0, have_n = 0;  // have: tiles with memory, a bit per lane
+    uint32_t row_s = kNoRow;  // the tiles' rows when their scores are kept
     int pid_n = -1;
     float ks_l = 0.f, vs_l = 0.f, ks_n = 0.f, vs_n = 0.f;
     // tile j on its way into slot j % ST (an empty group past the end)
@@ -519,6 +521,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         const int slot0 = tile_slot(j), at = j % AHEAD;
         if (at == 0) {
           have_l = have_n;
+          if constexpr (EXT && NB == 1) row_s = row_l;
           ks_l = ks_n;
           vs_l = vs_n > 0.f ? fmaxf(log2f(vs_n), kNoScale) : kNoScale;  // log2 of the scale
         }
@@ -554,8 +557,9 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
           }
         }
         if constexpr (EXT && NB == 1) {
+          const uint32_t row = __shfl_sync(0xffffffffu, row_s, at);
           if (score && 2 * tig < p.score_rows && !none) {
-            float* to = score + (int64_t)(slot0 + gid) * p.score_rows + 2 * tig;
+            float* to = score + (int64_t)((p.by_pool ? row : (uint32_t)slot0) + gid) * p.score_rows + 2 * tig;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (slot0 + gid + 8 * h >= lim_max) break;
@@ -813,7 +817,7 @@ int paged_attend_score_rows(const PagedAttendParams& p) {
   const int64_t most = (int64_t)p.b.max_tokens * (p.b.H / p.c.G);
   int rows = 1;
   while (rows < most && rows < kScoreRows) rows *= 2;
-  return (double)p.b.B * p.c.G * p.c.max_pages * p.c.page * rows * 4 <= (double)(1 << 30) ? rows : 0;
+  return (double)slot_places(p, p.by_pool) * rows * 4 <= (double)(1 << 30) ? rows : 0;
 }
 
 bool paged_attend_fits(const PagedAttendParams& p) { return units_bound(plan_for(p).few) < 4e9; }

@@ -563,7 +563,7 @@ template <int KV, int D, int PAGE>
 __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_keep_kernel(const PagedKeepParams p) {
   using S = MoveShape<D, PAGE>;
   __shared__ MoveRows<PAGE> m;
-  __shared__ int stop, moved, fixed;
+  __shared__ int stop, fixed;
   grid_dependents();
   grid_wait();
   const int b = blockIdx.y, g = blockIdx.x, G = p.c.G, tid = threadIdx.x;

@@ -78,6 +78,16 @@ struct WeighSlots {
   }
 };
 
+// Where what is kept for a slot lies: of head 0, and from a head to the next.
+struct SlotPlaces {
+  int64_t first, head;
+  SPATTEN_DEV SlotPlaces(const PagedAttendParams& a, int b, int slot, int64_t row) {
+    const int64_t slots = (int64_t)a.c.max_pages * a.c.page;
+    first = a.by_pool ? row : (int64_t)b * a.c.G * slots + slot;
+    head = a.by_pool ? a.c.page : slots;
+  }
+};
+
 // Slots x sequences x groups of heads; groups of `heads`, smaller where the CTAs are few.
 dim3 slot_grid(const PagedWeighParams& p, int n_sm, int& heads) {
   const int64_t slots = (int64_t)p.a.c.max_pages * p.a.c.page, G = p.a.c.G;
@@ -107,13 +117,13 @@ __global__ void __launch_bounds__(kSlotThreads) paged_weigh_scores_kernel(const 
   }
   __syncthreads();
   if (!live) return;
-  const int64_t slots = (int64_t)a.c.max_pages * a.c.page;
-  const float* src = a.score + ((int64_t)b * G * slots + x.slot) * ROWS;
+  const SlotPlaces place(a, b, x.slot, x.row);
+  const float* src = a.score + place.first * ROWS;
 #pragma unroll 2
   for (int h = 0; h < min(heads, G - g0); ++h) {
     const int g = g0 + h;
     float s[kQuad * ROWS];
-    const float4* at = reinterpret_cast<const float4*>(src + g * slots * ROWS);
+    const float4* at = reinterpret_cast<const float4*>(src + g * place.head * ROWS);
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const float4 y = __ldcs(at + i);  // (read once)
@@ -152,11 +162,13 @@ constexpr int kRing = 2;    // tiles of query rows, blocks of keys in shared mem
 constexpr int kConsts = 4;  // tiles' row constants
 constexpr int kConstBytes = kTileRows * 8 + 16;  // b and cq of the rows, the cq that all have (0: each its own)
 constexpr unsigned kErr = 0x500;
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;
 
 // What the main kernel works on, in the workspace.
 struct WeighPlan {
   uint8_t* tiles;     // [G][tiles_g] records: 128 query rows, then their constants
-  float* partial;     // [chunks][2][B][G][slots]: of the chunk's even and odd 64 rows
+  float* partial;     // [chunks][2][places]: sums of the even and the odd 64 rows of a chunk's tiles
+  int64_t places;     // slot_places
   int64_t tiles_g;
   int chunk, chunks;  // rows of a chunk (a multiple of kTileRows), chunks of a sequence at most
 };
@@ -170,7 +182,8 @@ struct Lay {
   static constexpr int oQ = oK + kRing * 2 * kKHalf;         // [ring][D / 64][128][128 B]
   static constexpr int oC = oQ + kRing * kQBytes;            // [kConsts]
   static constexpr int oScale = oC + kConsts * kConstBytes;  // [ring][256] scales of the keys
-  static constexpr int oItem = oScale + kRing * kKeys * 4;   // [ring] Item
+  static constexpr int oRow = oScale + kRing * kKeys * 4;    // [ring][256] rows of the pool
+  static constexpr int oItem = oRow + kRing * kKeys * 4;     // [ring] Item
   static constexpr int oBar = oItem + kRing * 64;
   static constexpr int kBars = 4 * kRing + 2 * kConsts + 4 + 1;
   static constexpr int oTmem = oBar + kBars * 8;
@@ -306,7 +319,7 @@ struct Item {
   int k0, lim;           // first slot, end of the sequence
   int old, n, begin;     // of its PagedSeq
   int nrows;
-  int64_t partial;       // where the sums of the first key's even rows go
+  int64_t partial;       // where the even rows' sums go, of the first slot or of row 0 of the pool
 };
 static_assert(sizeof(Item) <= 64, "two of them in Lay");
 
@@ -457,6 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
       const Item it = *reinterpret_cast<const Item*>(sm + L::oItem + kb * 64);
       if (it.t0 == it.t1) break;
       const float ks = *reinterpret_cast<const float*>(sm + L::oScale + (kb * kKeys + key) * 4);
+      const uint32_t row = *reinterpret_cast<const uint32_t*>(sm + L::oRow + (kb * kKeys + key) * 4);
       __syncwarp();
       mbar_arrive_elect(k_empty[kb]);
       ++items;
@@ -534,8 +548,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
           sum = make_float2(0.f, 0.f);
         }
       }
-      if (alive && slot < it.lim)
-        w.partial[it.partial + (side ? (int64_t)a.b.B * G * a.c.max_pages * a.c.page : 0) + key] = total + (sum.x + sum.y);
+      if (alive && row != kNoRow)  // (a slot of the sequence, with memory)
+        w.partial[it.partial + (side ? w.places : 0) + (a.by_pool ? row : (uint32_t)key)] = total + (sum.x + sum.y);
     }
   } else if (warp < kSumWarps + kWideWarps) {
     // ------------------------------------------------------------ keys to f16
@@ -563,12 +577,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
         return slot < it.lim ? paged_page(a.c, it.b, slot >> page_log) : -1;
       };
       float ks[2];
+      uint32_t rows[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int q = page_of(x + 128 * i);
         ks[i] = q >= 0 ? a.c.k_scale[(int64_t)q * G + it.g] : 0.f;
+        rows[i] = q >= 0 ? ((uint32_t)q * G + it.g) * page + ((it.k0 + x + 128 * i) & (page - 1)) : kNoRow;
       }
-      int pid[FLY];
+      int pid[FLY] = {};
       uint4 c[FLY];
       auto fetch = [&](int i, int step) {
         const int at = (it.k0 + key + KPS * step) & (page - 1);
@@ -602,10 +618,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weigh_tc_kernel(const Paged
       if (x == 0) {
         item->t0 = it.t0; item->t1 = it.t1; item->k0 = it.k0; item->lim = it.lim;
         item->old = it.sq.old; item->n = it.sq.n; item->begin = it.sq.begin; item->nrows = it.nrows;
-        item->partial = (((int64_t)it.c * 2 * a.b.B + it.b) * G + it.g) * a.c.max_pages * page + it.k0;
+        item->partial = 2 * it.c * w.places +
+                        (a.by_pool ? 0 : ((int64_t)it.b * G + it.g) * a.c.max_pages * page + it.k0);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) *reinterpret_cast<float*>(sm + L::oScale + (kb * kKeys + x + 128 * i) * 4) = ks[i];
+      for (int i = 0; i < 2; ++i) {
+        *reinterpret_cast<float*>(sm + L::oScale + (kb * kKeys + x + 128 * i) * 4) = ks[i];
+        *reinterpret_cast<uint32_t*>(sm + L::oRow + (kb * kKeys + x + 128 * i) * 4) = rows[i];
+      }
       fence_proxy_async_smem();
       __syncwarp();
       mbar_arrive_elect(k_full[kb]);
@@ -701,7 +721,7 @@ __global__ void __launch_bounds__(kSlotThreads) paged_weigh_sum_kernel(const Pag
   WeighSlots x;
   if (nrows <= p.rows_over || !x.set(p, sq, b, blockIdx.x * kSlotsCta + kQuad * threadIdx.x)) return;
   const int c1 = (nrows + w.chunk - 1) / w.chunk;
-  const int64_t slots = (int64_t)a.c.max_pages * a.c.page;
+  const SlotPlaces place(a, b, x.slot, x.row);
 #pragma unroll 2
   for (int h = 0; h < min(heads, G - g0); ++h) {
     const int g = g0 + h;
@@ -709,8 +729,8 @@ __global__ void __launch_bounds__(kSlotThreads) paged_weigh_sum_kernel(const Pag
     float add[kQuad] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
     for (int c = 0; c < c1; ++c) {
-      const float* at = w.partial + (((int64_t)c * 2 * a.b.B + b) * G + g) * slots + x.slot;
-      const float4 y = *reinterpret_cast<const float4*>(at), z = *reinterpret_cast<const float4*>(at + a.b.B * G * slots);
+      const float* at = w.partial + 2 * c * w.places + place.first + g * place.head;
+      const float4 y = *reinterpret_cast<const float4*>(at), z = *reinterpret_cast<const float4*>(at + w.places);
       const float part[kQuad] = {y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w};
       // a chunk of which no row sees a slot has left nothing for it
       const int64_t seen = a.tree ? INT64_MAX : (int64_t)x.old + ((int64_t)min((c + 1) * w.chunk, nrows) - 1) / R + 1;
@@ -728,8 +748,9 @@ int64_t most_rows(const PagedWeighParams& p) { return (int64_t)p.a.b.max_tokens 
 // Chunks of at least 512 rows, up to eight of them, in at most 1 GiB of sums.
 size_t plan_for(const PagedWeighParams& p, void* ws, WeighPlan& x) {
   const PagedAttendParams& a = p.a;
-  const int64_t rows = most_rows(p), slots = (int64_t)a.c.max_pages * a.c.page;
-  const int64_t fit = std::max<int64_t>(1, ((int64_t)1 << 27) / std::max<int64_t>(1, slots * a.b.B * a.c.G));
+  const int64_t rows = most_rows(p);
+  x.places = slot_places(a, a.by_pool);
+  const int64_t fit = std::max<int64_t>(1, ((int64_t)1 << 27) / x.places);
   const int64_t most = std::min<int64_t>(std::min<int64_t>(8, fit), (rows + 511) / 512);
   x.chunk = (int)((rows + most * kTileRows - 1) / (most * kTileRows) * kTileRows);
   x.chunks = (int)((rows + x.chunk - 1) / x.chunk);
@@ -738,7 +759,7 @@ size_t plan_for(const PagedWeighParams& p, void* ws, WeighPlan& x) {
   const size_t tiles = align256((size_t)x.tiles_g * a.c.G * (a.c.D == 128 ? Lay<128>::kRecord : Lay<64>::kRecord));
   x.tiles = w;
   x.partial = reinterpret_cast<float*>(w + (w ? tiles : 0));
-  return tiles + align256((size_t)x.chunks * 2 * a.b.B * a.c.G * slots * sizeof(float));
+  return tiles + align256((size_t)x.chunks * 2 * x.places * sizeof(float));
 }
 
 template <int KV, int D>

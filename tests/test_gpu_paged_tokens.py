@@ -301,6 +301,24 @@ def test_weights_of_rows_far_apart(n, R, scale):
     _check(out, q, cache, table, [0, n], [L], D ** -0.5 if scale is None else scale, None, before, w)
 
 
+@pytest.mark.parametrize("news,R", [([1, 1, 1], 4), ([1, 1, 1], 1), ([3, 7, 1], 3), ([60, 1, 2], 2), ([90, 70, 130], 1)])
+def test_weights_with_a_table_wider_than_the_pool(news, R):
+    """Most of the page table has no memory: what a call keeps lies like the pool."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(21)
+    G, D, page, lens = 2, 64, 16, [n + 70 for n in news]
+    mp = max(lens) // page + 1
+    cache = _filled(I8, 3 * mp, G, page, D, g)
+    table = torch.cat([_table(3, mp, 3 * mp, g), torch.full((3, 500), -1, dtype=torch.int32)], 1)
+    table[1, 2] = -1  # and a hole
+    w, cu = _weights(cache, g), _cum(news)
+    for _ in range(2):
+        q = torch.randn(cu[-1], G * R, D, generator=g).to(BF16).cuda()
+        before = paged.PagedWeights(*(t.clone() for t in w))
+        out = paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), max(news), weights=w)
+        _check(out, q, cache, table, cu, lens, D ** -0.5, None, before, w)
+
+
 def test_expanded_words_and_lists():
     """One mask, one list of accepted tokens for all; limits beyond any length."""
     from spatten_b200 import paged
