@@ -61,7 +61,7 @@ SPATTEN_DEV float row_amax(uint4 c) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float f[4];
-    codes4_to_f32<KV>(w[i], f);
+    codes4_to_f32_alu<KV>(w[i], f);
 #pragma unroll
     for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(f[e]));
   }
