@@ -31,9 +31,12 @@
 // in one shared-memory buffer a tile's exponentials had to wait for the product of
 // the tile before (512 new tokens over 32768: 376 us instead of 320).
 //
-// 512 new tokens over 32768 (32 heads, 8 KV heads, D = 128, int8): 320 us, 854
-// TFLOP/s, 0.51 of the measured bf16 rate; 1024 over 8192, 2 sequences, e4m3: 343 us,
-// 752 TFLOP/s; a prompt of 4096: 223 us, 616 TFLOP/s. What bounds it: one thread per
+// 512 new tokens over 32768 (32 heads, 8 KV heads, D = 128, int8): 319 us, 857
+// TFLOP/s, 0.51 of the measured bf16 rate; 1024 over 8192, 2 sequences, e4m3: 313 us,
+// 823 TFLOP/s; a prompt of 4096: 215 us, 640 TFLOP/s; 16 trees of up to 64 tokens over
+// up to 8192 keys: 173 us (causal rows: 157). Code that runs once a line counts: with the
+// masked tiles' path in twice the instructions the trees took 210 us, the second of
+// these 343. What bounds it: one thread per
 // row takes a tile's 64 scores through a chain of load, maximum, exponentials and
 // store that two warps per scheduler do not hide; then a line's set-up (queries,
 // the first tile, the epilogue).

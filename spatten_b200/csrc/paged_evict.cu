@@ -17,10 +17,16 @@
 // cluster; then the kept, the free and the moving slots as bits, a word per 32 slots,
 // whose prefix sums number them.
 //
-// paged_move_kernel: a CTA per block (page, KV head) of the first `keep` slots. A token's codes under the block's scale S' are round(code * S / S') with S'
-// the larger of the block's scale (0 where it keeps nothing) and the one that the
+// paged_move_kernel: a CTA per block (page, KV head) of the first `keep` slots. A
+// token's codes under the block's scale S' are round(code * S / S') with S' the larger of the block's scale (0 where it keeps nothing) and the one that the
 // largest moved magnitude needs; where S' grew, the kept codes are rounded likewise, as
 // appending does.
+//
+// Bound by latency, the chain of loads and of cluster barriers: 131001 slots of one
+// sequence cut to 65536 62 us (the moved codes alone are 134 MB, 21 us), 48 sequences of up
+// to 5000 slots cut to 4096 by head 72 us, 16 of 1088 cut to 1024 25 us. With the keys
+// gathered by the selection itself (8 CTAs for the longest case) that took 123 us of its
+// own; the selection's code, which runs once, is kept small (28 -> 25 us).
 #include <atomic>
 #include <cooperative_groups.h>
 
@@ -520,8 +526,8 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
 }
 
 // A CTA per block (page, KV head), K and V together: most of the time is the chain of
-// loads plan, page, codes. (Four blocks a CTA one after the other, 256 threads: 82 us
-// instead of 73 for 48 sequences of up to 5000 tokens by head.)
+// loads plan, page, codes. (Four blocks a CTA one after the other, 256 threads: the
+// 72 us above were 82.)
 template <int KV, int D, int PAGE>
 __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_move_kernel(const PagedEvictParams p,
                                                                            const EvictPlan plan) {
@@ -558,7 +564,8 @@ __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_move_kernel(cons
 // ---------------------------------------------------------------- accepted tokens
 
 // A CTA per (KV head, sequence) walks the blocks that accepted tokens move into, in
-// order: what it reads lies at or behind what it writes.
+// order: what it reads lies at or behind what it writes. Accepted branches are short, so the
+// walk is a block or two: one sequence 3.8 us, 64 5.4 us, the chain of loads.
 template <int KV, int D, int PAGE>
 __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_keep_kernel(const PagedKeepParams p) {
   using S = MoveShape<D, PAGE>;
