@@ -404,7 +404,7 @@ int spatten_paged_tree(const spatten_paged_tree_args* a, void* stream);
  *  * tree (optional, int32 [T, tree_words] with row stride tree_stride; 32 *
  *    tree_words >= max_tokens): a row sees the slots before its sequence's new
  *    tokens, and of these the ones whose bits are set in its words (whether
- *    before or behind it; bits from n_b on count as clear);
+ *    before or behind it; bits from n_b or max_tokens on count as clear);
  *  * weight, position (optional, together; fp32 and int32 [num_pages, G,
  *    page_size] beside the pool, 16-byte aligned): the softmax weights that the call's rows give
  *    a slot, summed in fp32 over the rows and the H / G heads of its KV head, are

@@ -59,8 +59,8 @@ def attend(q, cache, table, cu, lens, sm_scale, sees=None, max_tokens=None):
                 seen = slot < old + i + 1
             else:
                 seen = slot < old
-                for j in sees.get(t, ()):
-                    if j < n and 0 <= old + j < L:
+                for j in sees.get(t, ()):  # (tokens behind max_tokens are not the call's)
+                    if j < (n if max_tokens is None else min(n, max_tokens)) and 0 <= old + j < L:
                         seen[old + j] = True
             seen = seen & has
             if not seen.any():

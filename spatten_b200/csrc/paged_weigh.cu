@@ -201,13 +201,15 @@ struct Lay {
   static constexpr int bytes(int B) { return oPre + ((B + 1) / 2 + 1) * 4 + 1024; }
 };
 
+constexpr int kRowThreads = 512;
+
 // First record of sequence b: records of sequences whose rows are apart are apart.
 SPATTEN_DEV int64_t first_tile(const PagedSeq& s, int R, int b) { return (int64_t)s.begin * R / kTileRows + b; }
 
 template <int D>
-__global__ void __launch_bounds__(256) paged_weigh_rows_kernel(const PagedWeighParams p, const WeighPlan w, bool bf16) {
+__global__ void __launch_bounds__(kRowThreads) paged_weigh_rows_kernel(const PagedWeighParams p, const WeighPlan w, bool bf16) {
   using L = Lay<D>;
-  constexpr int LQ = D / 8, RPP = 256 / LQ;  // lanes of a row, rows of a pass
+  constexpr int LQ = D / 8, RPP = kRowThreads / LQ;  // lanes of a row, rows of a pass
   grid_dependents();
   grid_wait();
   const PagedAttendParams& a = p.a;
@@ -247,12 +249,12 @@ __global__ void __launch_bounds__(256) paged_weigh_rows_kernel(const PagedWeighP
     top[k] = m;
     if (m < INFINITY) most = fmaxf(most, m);
   }
-  __shared__ float red[8];
+  __shared__ float red[kRowThreads / 32];
   most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
   if ((tid & 31) == 0) red[tid >> 5] = most;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) most = fmaxf(most, red[i]);
+  for (int i = 0; i < kRowThreads / 32; ++i) most = fmaxf(most, red[i]);
   // One power of two for the tile, so that the sums need one number a row instead of two: where
   // each row reaches 2^-12 of the largest magnitude, what f16 drops of it is below 2^-28 of
   // the row's own largest.
@@ -784,7 +786,7 @@ cudaError_t tc_launch(const PagedWeighParams& p, bool bf16, const WeighPlan& w, 
   }
   const PagedAttendParams& a = p.a;
   const dim3 tiles((unsigned)((most_rows(p) + kTileRows - 1) / kTileRows), a.c.G, a.b.B);
-  e = launch_dependent(paged_weigh_rows_kernel<D>, tiles, 256, 0, st, p, w, bf16);
+  e = launch_dependent(paged_weigh_rows_kernel<D>, tiles, kRowThreads, 0, st, p, w, bf16);
   if (e != cudaSuccess) return e;
   const int64_t slots = (int64_t)a.c.max_pages * a.c.page;
   const double items = (double)a.b.B * a.c.G * w.chunks * ((slots + kKeys - 1) / kKeys);

@@ -319,6 +319,69 @@ def test_weights_with_a_table_wider_than_the_pool(news, R):
         _check(out, q, cache, table, cu, lens, D ** -0.5, None, before, w)
 
 
+@pytest.mark.parametrize("B,R,G", [(5000, 16, 1), (8192, 2, 1), (3, 1, 12), (700, 9, 3)])
+def test_weights_of_many_sequences_and_heads(B, R, G):
+    """Each row gives a weight of 1 in all; the output is the plain call's."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(25)
+    D, page = 64, 16
+    lens = [rng % 61 + 1 for rng in torch.randint(0, 1 << 20, (B,), generator=g).tolist()]
+    cache = _filled(E4, 4 * B, G, page, D, g)
+    table = torch.arange(4 * B, dtype=torch.int32).view(B, 4).cuda()
+    q = torch.randn(B, G * R, D, generator=g).to(BF16).cuda()
+    w = _weights(cache, g)
+    args = (q, cache, table, _i32(list(range(B + 1))), _i32(lens), 1)
+    before = w.weight.clone()
+    out = paged.paged_attention(*args, weights=w)
+    assert torch.equal(out, paged.paged_attention(*args))
+    slot = torch.arange(64, device="cuda")
+    held = (slot < args[4][:, None]).view(B, 4, 1, page)
+    old = (slot < args[4][:, None] - 1).view(B, 4, 1, page)
+    now, was = w.weight.view(B, 4, G, page).double(), before.view(B, 4, G, page).double()
+    gained = torch.where(held, now - torch.where(old, was, torch.zeros_like(was)), torch.zeros_like(now)).sum((1, 3))
+    assert torch.allclose(gained, torch.full_like(gained, R), rtol=1e-3, atol=1e-3)  # (differences of rounded sums)
+    assert torch.equal(now[~held.expand_as(now)], was[~held.expand_as(was)])
+
+
+@pytest.mark.parametrize("n,R,L", [(600, 64, 700), (1100, 8, 2500)])
+def test_weights_of_very_many_rows(n, R, L):
+    """Chunks of thousands of rows."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(26)
+    G, D, page = 1, 64, 64
+    mp = -(-L // page)
+    cache, table = _filled(I8, mp, G, page, D, g, spread=False), _table(1, mp, mp, g)
+    q = torch.randn(n, R, D, generator=g).to(F16).cuda()
+    w = paged.new_paged_weights(cache)
+    paged.paged_attention(q, cache, table.cuda(), _i32([0, n]), _i32([L]), n, weights=w)
+    at = table[0].long().cuda()
+    k = (cache.k[at, 0].double() * cache.k_scale[at, 0, None, None].double()).reshape(-1, D)[:L]
+    want = torch.zeros(L, dtype=torch.float64, device="cuda")
+    late = torch.arange(L, device="cuda")[None] > torch.arange(n, device="cuda")[:, None] + L - n
+    for h in range(R):
+        want += torch.softmax((q[:, h].double() @ k.T * D ** -0.5).masked_fill(late, float("-inf")), -1).sum(0)
+    got = w.weight[at, 0].view(-1)[:L].double()
+    assert ((got - want).abs() <= want * 4 * 2.0 ** -16 + 1e-30).all()
+
+
+@pytest.mark.parametrize("n,R", [(6, 1), (40, 4)])
+def test_trees_of_odd_batches(n, R):
+    """Fewer tokens held than rows, more rows than max_tokens, a table that is too short."""
+    from spatten_b200 import paged
+    g, rng = torch.Generator().manual_seed(27), random.Random(27)
+    G, D, page = 2, 64, 16
+    news, lens = [n, n + 3, n, 0], [n - 3, n + 20, n + 50, 7]
+    cu = _cum(news)
+    cache, table = _filled(I8, 30, G, page, D, g), _table(4, 5, 30, g)
+    sees = {t: frozenset(j for j in range(64) if rng.random() < 0.5) for t in range(cu[-1])}
+    tree = OT.words(sees, cu[-1], 2).cuda()
+    q = torch.randn(cu[-1], G * R, D, generator=g).to(F16).cuda()
+    w = _weights(cache, g)
+    before = paged.PagedWeights(*(t.clone() for t in w))
+    out = paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), n, tree=tree, weights=w)
+    _check(out, q, cache, table, cu, lens, D ** -0.5, sees, before, w, max_tokens=n)
+
+
 def test_expanded_words_and_lists():
     """One mask, one list of accepted tokens for all; limits beyond any length."""
     from spatten_b200 import paged
