@@ -757,7 +757,7 @@ static int fill_paged_attend_ext(const spatten_paged_attend_ext_args* a, spatten
   p.weight = a->weight; p.position = a->position; p.positions = a->positions;
   p.a.by_pool = spatten::slot_places(p.a, true) < spatten::slot_places(p.a, false);
   if (p.weight) p.a.score_rows = spatten::paged_attend_score_rows(p.a);
-  p.rows_over = p.a.score_rows ? spatten::kScoreRows : 0;
+  p.rows_over = p.a.score_rows;
   return SPATTEN_OK;
 }
 

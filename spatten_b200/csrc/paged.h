@@ -67,13 +67,13 @@ struct PagedAttendParams {
   int64_t tree_st = 0;
   int words = 0;
   float2* stat = nullptr;          // or null: [T, H] reference m of a row's exponentials, 1 / their sum
-  // or null: scores (log2) of sequences of at most kScoreRows query rows per KV
+  // or null: scores (log2) of sequences of at most score_rows query rows per KV
   // head, [slot_place][score_rows], where an unmasked place's page has memory
   float* score = nullptr;
   int score_rows = 0;
   bool by_pool = false;            // see slot_places
 };
-constexpr int kScoreRows = 8;
+constexpr int kScoreRows = 32;   // at most
 
 // What a call keeps for each of its slots (of which sequences share none) lies by
 // sequence and slot, [B, G, slots], or like the pool, [P, G, page]: whichever is smaller.

@@ -395,7 +395,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
     const int nrows = sq.n * R, r0 = rt * ROWS;
     // slots that the tile's last and first row see
     const bool tree = EXT && p.tree;
-    float* const score = EXT && p.score && nrows <= kScoreRows
+    float* const score = EXT && p.score && nrows <= p.score_rows
                              ? p.score + (p.by_pool ? 0 : ((int64_t)b * G + g) * p.c.max_pages * page * p.score_rows)
                              : nullptr;
     const int lim_max = min(sq.old + (tree ? sq.n : min((r0 + ROWS - 1) / R, sq.n - 1) + 1), sq.len);
@@ -521,7 +521,7 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
         const int slot0 = tile_slot(j), at = j % AHEAD;
         if (at == 0) {
           have_l = have_n;
-          if constexpr (EXT && NB == 1) row_s = row_l;
+          if constexpr (EXT) row_s = row_l;
           ks_l = ks_n;
           vs_l = vs_n > 0.f ? fmaxf(log2f(vs_n), kNoScale) : kNoScale;  // log2 of the scale
         }
@@ -556,15 +556,18 @@ paged_attend_kernel(const PagedAttendParams p, const Workspace ws, const bool bf
               }
           }
         }
-        if constexpr (EXT && NB == 1) {
+        if constexpr (EXT) {
           const uint32_t row = __shfl_sync(0xffffffffu, row_s, at);
-          if (score && 2 * tig < p.score_rows && !none) {
-            float* to = score + (int64_t)((p.by_pool ? row : (uint32_t)slot0) + gid) * p.score_rows + 2 * tig;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const int r = r0 + 8 * nb + 2 * tig;  // (with r + 1 below score_rows, a power of two, or that is 1)
+            if (!score || r >= nrows || none) break;
+            float* to = score + (int64_t)((p.by_pool ? row : (uint32_t)slot0) + gid) * p.score_rows + r;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (slot0 + gid + 8 * h >= lim_max) break;
-              if (p.score_rows == 1) to[8 * h] = s[0][2 * h];
-              else *reinterpret_cast<float2*>(to + 8 * h * p.score_rows) = make_float2(s[0][2 * h], s[0][2 * h + 1]);
+              if (p.score_rows == 1) to[8 * h] = s[nb][2 * h];
+              else *reinterpret_cast<float2*>(to + 8 * h * p.score_rows) = make_float2(s[nb][2 * h], s[nb][2 * h + 1]);
             }
           }
         }
@@ -808,15 +811,17 @@ Plan plan_for(const PagedAttendParams& p) {
 
 }  // namespace
 
-// The scores of a step are kept where a sequence has at most kScoreRows rows: 4 bytes
-// a row and slot, written and read once, instead of the keys' D bytes read again; up to 1 GiB
-// of them.
+// The scores of a step or of a few drafted tokens are kept: 4 bytes a row and slot, written
+// and read once, instead of the keys' D bytes read again and three launches (24 sequences of
+// 7 drafted tokens over 2000 keys, 21 rows: 42 us with the attention's 23.5, 62 so). Up to
+// kScoreRows rows and 1 GiB; beside the tcgen05 launch 8, as most of what is left there is
+// single tokens.
 int paged_attend_score_rows(const PagedAttendParams& p) {
   const Plan x = plan_for(p);
-  if (!x.use_few || row_block(x.few) != kScoreRows) return 0;
-  const int64_t most = (int64_t)p.b.max_tokens * (p.b.H / p.c.G);
+  const int64_t all = (int64_t)p.b.max_tokens * (p.b.H / p.c.G), most = x.use_tc ? 8 : all;
+  if (!x.use_few || most > kScoreRows || (x.use_tc && row_block(x.few) != 8)) return 0;
   int rows = 1;
-  while (rows < most && rows < kScoreRows) rows *= 2;
+  while (rows < most) rows *= 2;
   return (double)slot_places(p, p.by_pool) * rows * 4 <= (double)(1 << 30) ? rows : 0;
 }
 

@@ -7,7 +7,8 @@
 // positions. Two ways, by the query rows that a sequence has per KV head:
 //
 // Up to kScoreRows: the attention has kept its scores (4 bytes a row and slot), and
-// paged_weigh_scores_kernel turns them into weights. For 64 sequences x 8 heads x 32768
+// paged_weigh_scores_kernel (paged_weigh_rowed_kernel beyond 8 rows) turns them into weights.
+// For 64 sequences x 8 heads x 32768
 // keys with 4 rows the scores and weights are 670 MB to write and read; reading the keys
 // again would take 2.1 GB (2806 us with a kernel that did, 830 to 880 now, the attention alone
 // 665 to 690; the scores' kernel by itself 64 us = 5.5 TB/s, what is left is the
@@ -97,9 +98,9 @@ struct SlotPlaces {
 };
 
 // Slots x sequences x groups of heads; groups of `heads`, smaller where the CTAs are few.
-dim3 slot_grid(const PagedWeighParams& p, int n_sm, int& heads) {
+dim3 slot_grid(const PagedWeighParams& p, int n_sm, int per_cta, int& heads) {
   const int64_t slots = (int64_t)p.a.c.max_pages * p.a.c.page, G = p.a.c.G;
-  const int64_t ctas = (slots + kSlotsCta - 1) / kSlotsCta;
+  const int64_t ctas = (slots + per_cta - 1) / per_cta;
   heads = 8;
   while (heads > 1 && ctas * p.a.b.B * ((G + heads - 1) / heads) < 4 * n_sm) heads /= 2;
   return dim3((unsigned)ctas, p.a.b.B, (unsigned)((G + heads - 1) / heads));
@@ -119,6 +120,7 @@ __global__ void __launch_bounds__(kSlotThreads) paged_weigh_scores_kernel(const 
   if (sq.n == 0 || nrows > p.rows_over) return;
   WeighSlots x;
   const bool live = x.set(p, sq, b, blockIdx.x * kSlotsCta + kQuad * tid);
+  static_assert(8 * ROWS <= kSlotThreads, "a row's statistics per thread");
   if (tid < heads * ROWS && g0 + tid / ROWS < G) {
     const int g = g0 + tid / ROWS, r = tid % ROWS;
     if (r < nrows) stat[tid / ROWS][r] = a.stat[(int64_t)(sq.begin + r / R) * a.b.H + g * R + r % R];
@@ -130,15 +132,15 @@ __global__ void __launch_bounds__(kSlotThreads) paged_weigh_scores_kernel(const 
 #pragma unroll 2
   for (int h = 0; h < min(heads, G - g0); ++h) {
     const int g = g0 + h;
-    float s[kQuad * ROWS];
     const float4* at = reinterpret_cast<const float4*>(src + g * place.head * ROWS);
+    const float4 was = x.before(p, g);
+    float add[kQuad] = {0.f, 0.f, 0.f, 0.f};
+    float s[kQuad * ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const float4 y = __ldcs(at + i);  // (read once)
       s[4 * i] = y.x; s[4 * i + 1] = y.y; s[4 * i + 2] = y.z; s[4 * i + 3] = y.w;
     }
-    const float4 was = x.before(p, g);
-    float add[kQuad] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
       if (r < nrows) {
@@ -150,14 +152,73 @@ __global__ void __launch_bounds__(kSlotThreads) paged_weigh_scores_kernel(const 
   }
 }
 
+// 16 or 32 rows a slot: four rows a thread, so that a slot's scores are read whole (four
+// slots a thread as above: 50 us for the 42 at 24 sequences of 7 drafted tokens over 2000).
+constexpr int kRowedSlots = 64;  // of a CTA
+
+template <int ROWS>
+__global__ void __launch_bounds__(kSlotThreads) paged_weigh_rowed_kernel(const PagedWeighParams p, int heads) {
+  constexpr int L = ROWS / 4, SPP = kSlotThreads / L;  // threads of a slot, slots of a pass
+  __shared__ float2 stat[8][ROWS];
+  grid_dependents();
+  grid_wait();
+  const PagedAttendParams& a = p.a;
+  const int b = blockIdx.y, G = a.c.G, R = a.b.H / G, g0 = blockIdx.z * heads, tid = threadIdx.x, li = tid % L;
+  const PagedSeq sq = paged_seq(a.b, a.c, b);
+  const int nrows = sq.n * R, first = blockIdx.x * kRowedSlots, lim = min(sq.old + sq.n, sq.len);
+  if (sq.n == 0 || nrows > p.rows_over || first >= lim) return;  // (the CTA as one)
+  static_assert(8 * ROWS <= kSlotThreads, "a row's statistics per thread");
+  if (tid < heads * ROWS && g0 + tid / ROWS < G) {
+    const int g = g0 + tid / ROWS, r = tid % ROWS;
+    stat[tid / ROWS][r] = r < nrows ? a.stat[(int64_t)(sq.begin + r / R) * a.b.H + g * R + r % R] : make_float2(0.f, 0.f);
+  }
+  __syncthreads();
+  // the attention's tiles of rows store each up to the last slot that one of them sees
+  int sees[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sees[k] = 4 * li + k >= nrows ? 0 : a.tree ? INT_MAX : sq.old + (4 * li + k) / R + 1;
+  // (little code, which runs a few times, and many warps)
+#pragma unroll 1
+  for (int s0 = 0; s0 < kRowedSlots; s0 += SPP) {
+    const int slot = first + s0 + tid / L;
+    const int pid = slot < lim ? paged_page(a.c, b, slot / a.c.page) : -1;
+    const int64_t row = (int64_t)max(pid, 0) * G * a.c.page + slot % a.c.page;
+    const SlotPlaces place(a, b, slot, row);
+#pragma unroll 1
+    for (int h = 0; h < min(heads, G - g0); ++h) {
+      const int g = g0 + h;
+      const int64_t at = row + (int64_t)g * a.c.page;
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (pid >= 0 && 4 * li < nrows)
+        y = __ldcs(reinterpret_cast<const float4*>(a.score + (place.first + g * place.head) * ROWS) + li);
+      const float before = pid >= 0 && li == 0 && slot < sq.old ? p.weight[at] : 0.f;
+      const float s[4] = {y.x, y.y, y.z, y.w};
+      float add = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 z = stat[h][4 * li + k];
+        if (slot < sees[k]) add += fast_exp2(s[k] - z.x) * z.y;
+      }
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) add += __shfl_xor_sync(0xffffffffu, add, o);
+      if (pid >= 0 && li == 0) {
+        p.weight[at] = before + add;
+        if (slot >= sq.old) p.position[at] = p.positions ? p.positions[sq.begin + slot - sq.old] : slot;
+      }
+    }
+  }
+}
+
 cudaError_t scores_launch(const PagedWeighParams& p, int n_sm, cudaStream_t st) {
   int heads;
-  const dim3 grid = slot_grid(p, n_sm, heads);
+  const dim3 grid = slot_grid(p, n_sm, p.a.score_rows > 8 ? kRowedSlots : kSlotsCta, heads);
   switch (p.a.score_rows) {
     case 1: return launch_dependent(paged_weigh_scores_kernel<1>, grid, kSlotThreads, 0, st, p, heads);
     case 2: return launch_dependent(paged_weigh_scores_kernel<2>, grid, kSlotThreads, 0, st, p, heads);
     case 4: return launch_dependent(paged_weigh_scores_kernel<4>, grid, kSlotThreads, 0, st, p, heads);
     case 8: return launch_dependent(paged_weigh_scores_kernel<8>, grid, kSlotThreads, 0, st, p, heads);
+    case 16: return launch_dependent(paged_weigh_rowed_kernel<16>, grid, kSlotThreads, 0, st, p, heads);
+    case 32: return launch_dependent(paged_weigh_rowed_kernel<32>, grid, kSlotThreads, 0, st, p, heads);
     default: return cudaErrorInvalidValue;
   }
 }
@@ -755,13 +816,15 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 int64_t most_rows(const PagedWeighParams& p) { return (int64_t)p.a.b.max_tokens * (p.a.b.H / p.a.c.G); }
 
-// Chunks of at least 512 rows, up to eight of them, in at most 1 GiB of sums.
+// Chunks of 768 rows, up to eight of them, in at most 1 GiB of sums: an item's keys cost
+// about as much to widen as two tiles of rows to multiply and sum (1024 new tokens over 8192, 2
+// sequences: 313, 279, 263, 259 and 262 us with 256, 384, 512, 768 and 1024 rows).
 size_t plan_for(const PagedWeighParams& p, void* ws, WeighPlan& x) {
   const PagedAttendParams& a = p.a;
   const int64_t rows = most_rows(p);
   x.places = slot_places(a, a.by_pool);
   const int64_t fit = std::max<int64_t>(1, ((int64_t)1 << 27) / x.places);
-  const int64_t most = std::min<int64_t>(std::min<int64_t>(8, fit), (rows + 511) / 512);
+  const int64_t most = std::min<int64_t>(std::min<int64_t>(8, fit), (rows + 767) / 768);
   x.chunk = (int)((rows + most * kTileRows - 1) / (most * kTileRows) * kTileRows);
   x.chunks = (int)((rows + x.chunk - 1) / x.chunk);
   x.tiles_g = (int64_t)a.b.T * (a.b.H / a.c.G) / kTileRows + a.b.B + 1;
@@ -794,7 +857,7 @@ cudaError_t tc_launch(const PagedWeighParams& p, bool bf16, const WeighPlan& w, 
                        Lay<D>::bytes(a.b.B), st, p, w);
   if (e != cudaSuccess) return e;
   int heads;
-  const dim3 grid = slot_grid(p, n_sm, heads);
+  const dim3 grid = slot_grid(p, n_sm, kSlotsCta, heads);
   return launch_dependent(paged_weigh_sum_kernel, grid, kSlotThreads, 0, st, p, w, heads);
 }
 
