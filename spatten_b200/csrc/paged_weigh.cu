@@ -274,11 +274,23 @@ __global__ void __launch_bounds__(kRowThreads) paged_weigh_rows_kernel(const Pag
   grid_dependents();
   grid_wait();
   const PagedAttendParams& a = p.a;
-  const int b = blockIdx.z, g = blockIdx.y, t = blockIdx.x, R = a.b.H / a.c.G, tid = threadIdx.x;
+  // whose record this is (a CTA for each of the longest sequence's tiles in every sequence would be
+  // half a million where one prompt of 8192 tokens is among 256 sequences)
+  __shared__ int owner;
+  const int g = blockIdx.y, R = a.b.H / a.c.G, tid = threadIdx.x;
+  if (tid == 0) owner = -1;
+  __syncthreads();
+  for (int i = tid; i < a.b.B; i += kRowThreads) {
+    const PagedSeq s = paged_seq(a.b, a.c, i);
+    const int64_t at = (int64_t)blockIdx.x - first_tile(s, R, i);
+    if (s.n * R > p.rows_over && at >= 0 && at * kTileRows < s.n * R) atomicMax(&owner, i);
+  }
+  __syncthreads();
+  const int b = owner;
+  if (b < 0) return;
   const PagedSeq sq = paged_seq(a.b, a.c, b);
-  const int nrows = sq.n * R;
-  if (nrows <= p.rows_over || t * kTileRows >= nrows) return;
-  uint8_t* rec = w.tiles + (g * w.tiles_g + first_tile(sq, R, b) + t) * (int64_t)L::kRecord;
+  const int nrows = sq.n * R, t = (int)(blockIdx.x - first_tile(sq, R, b));
+  uint8_t* rec = w.tiles + (g * w.tiles_g + blockIdx.x) * (int64_t)L::kRecord;
   const int li = tid % LQ;
   auto pair = [&](uint32_t x) {
     return bf16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u))
@@ -816,7 +828,7 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 int64_t most_rows(const PagedWeighParams& p) { return (int64_t)p.a.b.max_tokens * (p.a.b.H / p.a.c.G); }
 
-// Chunks of 768 rows, up to eight of them, in at most 1 GiB of sums: an item's keys cost
+// Chunks of 768 rows, up to 32 of them, in at most 1 GiB of sums: an item's keys cost
 // about as much to widen as two tiles of rows to multiply and sum (1024 new tokens over 8192, 2
 // sequences: 313, 279, 263, 259 and 262 us with 256, 384, 512, 768 and 1024 rows).
 size_t plan_for(const PagedWeighParams& p, void* ws, WeighPlan& x) {
@@ -824,7 +836,7 @@ size_t plan_for(const PagedWeighParams& p, void* ws, WeighPlan& x) {
   const int64_t rows = most_rows(p);
   x.places = slot_places(a, a.by_pool);
   const int64_t fit = std::max<int64_t>(1, ((int64_t)1 << 27) / x.places);
-  const int64_t most = std::min<int64_t>(std::min<int64_t>(8, fit), (rows + 767) / 768);
+  const int64_t most = std::min<int64_t>(std::min<int64_t>(32, fit), (rows + 767) / 768);
   x.chunk = (int)((rows + most * kTileRows - 1) / (most * kTileRows) * kTileRows);
   x.chunks = (int)((rows + x.chunk - 1) / x.chunk);
   x.tiles_g = (int64_t)a.b.T * (a.b.H / a.c.G) / kTileRows + a.b.B + 1;
@@ -848,7 +860,7 @@ cudaError_t tc_launch(const PagedWeighParams& p, bool bf16, const WeighPlan& w, 
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   const PagedAttendParams& a = p.a;
-  const dim3 tiles((unsigned)((most_rows(p) + kTileRows - 1) / kTileRows), a.c.G, a.b.B);
+  const dim3 tiles((unsigned)w.tiles_g, a.c.G);
   e = launch_dependent(paged_weigh_rows_kernel<D>, tiles, kRowThreads, 0, st, p, w, bf16);
   if (e != cudaSuccess) return e;
   const int64_t slots = (int64_t)a.c.max_pages * a.c.page;
