@@ -814,7 +814,6 @@ static int fill_paged_evict(const spatten_paged_evict_args* a, spatten::PagedEvi
     return fail(SPATTEN_ERR_INVALID, "%s: B=%d keep=%d recent=%d (need >= 0, >= 1, >= 0)", who, a->B, a->keep,
                 a->recent);
   if (a->B > 65535) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: B=%d (at most 65535)", who, a->B);
-  if (p.c.G > 32767) return fail(SPATTEN_ERR_UNSUPPORTED, "%s: %d KV heads", who, p.c.G);
   if ((int64_t)p.c.max_pages * p.c.page > spatten::kEvictSlots)
     return fail(SPATTEN_ERR_UNSUPPORTED, "%s: page table of %lld slots (at most %d)", who,
                 (long long)p.c.max_pages * p.c.page, spatten::kEvictSlots);

@@ -24,8 +24,8 @@
 // tile); paged_weigh_tc_kernel
 // takes 256 keys x a chunk of the rows at a time; the last kernel adds the chunks up.
 // Bound by the exponentials, one per (row, key): 1024 new tokens over 8192, 2 sequences, 16
-// / 8 heads, e4m3: 95 us for 185 million of them, 61 % of the conversion pipe's cycles
-// while an SM has work, tensor pipe 31 %; 271 us with the attention, which takes 152.
+// / 8 heads, e4m3: 92 us for 185 million of them, 64 % of the conversion pipe's cycles
+// while an SM has work, tensor pipe 33 %; 259 us with the attention, which takes 152.
 // What it took: the keys widened a block ahead by warps of their own (four warps that sum per
 // scheduler instead of two CTAs that do everything by turns), and code that fits the
 // instruction caches: the same kernel with its rare paths unrolled took 145 us.
