@@ -137,7 +137,8 @@ int paged_attend_max_batch();  // sequences of one call
 bool paged_attend_fits(const PagedAttendParams& p);  // units of work count in 32 bits
 size_t paged_attend_workspace(const PagedAttendParams& p, int n_sm);
 // the tcgen05 path (paged_attend_tc.cu), for many query rows per KV head
-constexpr int kTcRows = 64;  // it takes sequences with more rows than this
+constexpr int kTcRows = 64;       // it takes sequences with more rows than this,
+constexpr int kTcRowsAlike = 48;  // or this where all have as many
 bool paged_attend_tc_takes(const PagedAttendParams& p);
 size_t paged_attend_tc_workspace(const PagedAttendParams& p, int n_sm);
 cudaError_t launch_paged_attend_tc(const PagedAttendParams& p, int dtype, int kv, void* ws, int n_sm,

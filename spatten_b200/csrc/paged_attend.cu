@@ -19,7 +19,7 @@
 // rate. One sequence of 131001, 53 us = 5.0 TB/s; 48 ragged ones of up to 8192, 79 us
 // = 5.2 TB/s. One of 777 takes 8.8 us, which is the chain of dependent loads and the
 // second launch. Beyond 16 rows each row tile walks the keys by itself: 32 sequences
-// over 8192 keys of e4m3 take 100, 184, 274 and 379 us at 16, 32, 48 and 64 rows (the
+// over 8192 keys of e4m3 take 100, 183, 267 and 358 us at 16, 32, 48 and 64 rows (the
 // cache's bytes once: 82 us).
 //
 // Numerics:
@@ -770,26 +770,32 @@ int paged_attend_max_batch() { return kMaxBatch; }
 namespace {
 
 // Which kernels a call takes. Sequences of more than kTcRows query rows per KV
-// head (pieces of prompts) go to the tcgen05 kernel, the others to the one above.
-// 64 rows (8 KV heads x 128, int8) take 40 us there and 43 us here at 4 sequences
-// over 4096 keys, 61 and 71 us at one over 32768, 349 and 476 us at 32 over 8192, but
-// 49 and 44 us at 16 over 1000 (e4m3) and 24 and 15 us at one over 800; 96 rows 40
-// and 57, 60 and 94, 331 and 702, 50 and 56, 24 and 15 us. So the sides meet at 40
-// rows where sequences are many and long and beyond 128 where they are few and short;
-// the border is in between, as lengths are not known on the host, which
+// head (pieces of prompts) go to the tcgen05 kernel, the others to the one above; of more
+// than kTcRowsAlike where all of the call's have as many.
+// At 32 / 8 heads x 128, 32 sequences over 8192 keys take at 32, 48 and 64 rows 235, 343
+// and 452 us here, 291 there from 33 on (int8); 183, 267 and 358, and 287 (e4m3). 64 rows
+// take 36 us there and 43 us here at 4 sequences over 4096 keys, 57 and 71 us at one over
+// 32768, 42 and 50 us at 16 over 1000 (e4m3). Lengths are not known on the host, which
 // knows the largest sequence's rows only. Where
 // the rows show that some must be shorter, both are launched and each serves its
 // own, so that single tokens beside a prompt's piece keep the kernel made for
 // them (512 new tokens over 4096 take 63 us, 47 single ones over 4000 76, together
-// 150).
+// 150); for a few rows more that does not pay (24 trees of 3 to 17 tokens, 9 to 51 rows,
+// over 20 to 4096 keys: 55 us in both, 25 here), hence the two borders.
 //
-// A tree's rows (which are many for the tokens they come from) stay here while their
-// work, in tiles of 16 rows x 16 keys over the whole page table, is small: at 32 / 8
-// heads x 128 (int8) 26 tokens of one sequence over 777 keys (2744 tiles) take 28.5 us
-// there and 15.3 here, over 3000 (10528) 30.3 and 22.5, over 6000 (21000) 35.3 and 32.4, 64
-// tokens over 3000 (24064) 35.4 and 37.1, of four sequences over 777 26.6 and 28.7 with
-// 26 tokens (10976) and 36 and 64 with 64 over 1500 (48128).
-constexpr double kFewTiles = 12000;
+// Trees (whose rows are many for the tokens they come from) and calls of up to kFewRows
+// rows stay here while their work is small: tiles of 16 rows x 16 keys over the
+// whole page table, a row tile's set-up counted as kTileCost of them. At 32 / 8 heads x
+// 128 (int8), that work, the time there and here: 64 rows of one sequence over
+// 800 keys 3100, 25.8 and 14.4 us, 96 over 1500 6776, 27.5 and 16.3, 64 of four over 777
+// 12320, 23.7 and 19.4, of one over 6000 16040, 30.8 and 24.1, of 16 over 300 28800, 29.2
+// and 32.0; trees of 26 tokens of one over 3000 keys
+// 12780, 29.7 and 23.5, of 64 over 1500 16456, 34.8 and 28.0, of 26 of four sequences over 777
+// 18480, 25.6 and 29.9, of 64 of two over 777 20944, 30.7 and 32.1, of 64 of four over 1500 65824,
+// 35.5 and 67.7. Longer pieces take the tcgen05 kernel even so: a prompt's
+// bits do not change with the width of its page table.
+constexpr int kFewRows = 128;
+constexpr double kFewTiles = 17500, kTileCost = 25;
 
 struct Plan {
   PagedAttendParams tc, few;
@@ -802,7 +808,9 @@ Plan plan_for(const PagedAttendParams& p) {
   x.tc.rows_upto = x.few.rows_upto = INT64_MAX;
   if (!paged_attend_tc_takes(p)) return x;
   const double lines = ((double)p.b.T * (p.b.H / p.c.G) / 16 + p.b.B) * p.c.G;
-  if (p.tree && lines * p.c.max_pages * (p.c.page / 16) <= kFewTiles) return x;
+  if ((p.tree || (int64_t)p.b.max_tokens * (p.b.H / p.c.G) <= kFewRows) &&
+      lines * ((double)p.c.max_pages * (p.c.page / 16) + kTileCost) <= kFewTiles)
+    return x;
   x.use_tc = true;
   x.use_few = p.b.B > 1 && p.b.T < (int64_t)p.b.B * p.b.max_tokens;
   if (x.use_few) x.tc.rows_over = x.few.rows_upto = kTcRows;

@@ -743,7 +743,8 @@ cudaError_t tc_launch(const PagedAttendParams& p, bool bf16, const PagedPartials
 
 bool paged_attend_tc_takes(const PagedAttendParams& p) {
   const int R = p.b.H / p.c.G;
-  if ((int64_t)p.b.max_tokens * R <= kTcRows || p.b.B > kMaxBatch) return false;
+  const bool alike = p.b.T >= (int64_t)p.b.B * p.b.max_tokens;
+  if ((int64_t)p.b.max_tokens * R <= (alike ? kTcRowsAlike : kTcRows) || p.b.B > kMaxBatch) return false;
   const double lines = (double)p.b.T * R / kRowsCta + p.b.B;  // at most
   return lines * p.c.G * ((double)p.c.max_pages * p.c.page + p.b.max_tokens + kRowsCta + kLineCost) < 4e9;
 }

@@ -42,6 +42,12 @@ def _weights(cache, g):
     return w
 
 
+def _wide(table, page):
+    """The table with columns behind the sequences' (300000 slots: calls of more than a few
+    query rows go to the tcgen05 kernel, which small work over a narrow table does not)."""
+    return torch.cat([table, torch.full((table.shape[0], 300000 // page), -1, dtype=torch.int32)], 1)
+
+
 def _check(out, q, cache, table, cu, lens, sm, sees, before=None, after=None, positions=None, max_tokens=None):
     """Outputs, and with the pools ``before`` and ``after`` the weights and positions."""
     c = _cpu(cache)
@@ -129,7 +135,8 @@ TREES = [
 
 @pytest.mark.parametrize("kv,dt,D,page,G,R,news,lens", TREES)
 @pytest.mark.parametrize("weigh", [False, True])
-def test_tree_attention(kv, dt, D, page, G, R, news, lens, weigh):
+@pytest.mark.parametrize("wide", [False, True])
+def test_tree_attention(kv, dt, D, page, G, R, news, lens, weigh, wide):
     """Trees of paged_tree, over contexts that end anywhere in a page or tile."""
     from spatten_b200 import paged
     g, rng = torch.Generator().manual_seed(len(news) + D), random.Random(5)
@@ -137,6 +144,7 @@ def test_tree_attention(kv, dt, D, page, G, R, news, lens, weigh):
     B, cu = len(lens), _cum(news)
     P = B * mp + 2
     cache, table = _filled(kv, P, G, page, D, g), _table(B, mp, P, g)
+    table = _wide(table, page) if wide else table
     parents = [p for n in news for p in _random_tree(n, rng)]
     tree, pos = paged.paged_tree(_i32(parents), _i32(cu), _i32(lens), max(news))
     sees, _ = OT.tree(parents, cu, lens, max(news))
@@ -149,7 +157,8 @@ def test_tree_attention(kv, dt, D, page, G, R, news, lens, weigh):
 
 
 @pytest.mark.parametrize("R,n", [(1, 5), (4, 40)])
-def test_masks_of_any_bits(R, n):
+@pytest.mark.parametrize("far", [False, True])
+def test_masks_of_any_bits(R, n, far):
     """Words that name later tokens, none at all (an empty row, over an empty context
     too), bits behind the sequence's tokens, wide strided words; pages without
     memory in the context and among the new tokens."""
@@ -161,6 +170,7 @@ def test_masks_of_any_bits(R, n):
     mp = max(lens) // page + 2
     cache, table = _filled(I8, 30, G, page, D, g), _table(4, mp, 30, g)
     table[1, 1], table[2, 0], table[3, (n + 2) // page] = -1, 99, -5
+    table = _wide(table, page) if far else table
     sees = {t: frozenset(j for j in range(64) if rng.random() < 0.4) for t in range(cu[-1])}
     for t in (0, 2, cu[1], cu[2] + 1):
         sees[t] = frozenset()
@@ -193,6 +203,25 @@ def test_chain_is_causal(news, R):
     assert pos.tolist() == [61 + i for n in news for i in range(n)]
     a, b = paged.paged_attention(q, cache, *args), paged.paged_attention(q, cache, *args, tree=tree)
     assert torch.allclose(a.float(), b.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+
+
+@pytest.mark.parametrize("kv", [I8, E4])
+@pytest.mark.parametrize("R,n", [(4, 12), (7, 7), (4, 16), (1, 65), (4, 32), (3, 43), (16, 5)])
+@pytest.mark.parametrize("wide,weigh", [(False, False), (True, False), (True, True)])
+def test_causal_on_either_side_of_the_kernels(kv, R, n, wide, weigh):
+    """48 to 129 query rows per KV head, over narrow and wide page tables, beside shorter ones."""
+    from spatten_b200 import paged
+    g = torch.Generator().manual_seed(R * n)
+    G, D, page, news, lens = 2, 128, 32, [n, 1, n - 1, 0, n], [n, 100, n + 33, 70, 450]
+    cu, mp, B = _cum(news), 15, 5
+    cache, table = _filled(kv, B * mp, G, page, D, g), _table(B, mp, B * mp, g)
+    table = _wide(table, page) if wide else table
+    q = torch.randn(cu[-1], G * R, D, generator=g).to(BF16).cuda()
+    w = _weights(cache, g) if weigh else None
+    before = paged.PagedWeights(*(t.clone() for t in w)) if weigh else None
+    out = paged.paged_attention(q, cache, table.cuda(), _i32(cu), _i32(lens), n, weights=w)
+    sees = {cu[b] + i: frozenset(range(i + 1)) for b in range(B) for i in range(news[b])}
+    _check(out, q, cache, table, cu, lens, D ** -0.5, sees, before, w)
 
 
 # ------------------------------------------------------------------ weights
