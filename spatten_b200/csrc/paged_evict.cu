@@ -121,7 +121,10 @@ SPATTEN_DEV void move_block(MoveRows<PAGE>& m, const PagedCache& pc, int64_t to,
       uint4* at = reinterpret_cast<uint4*>(pool[v] + (to * PAGE + r) * D + li * 16);
       if (m.src[r] != kNoRow) {
         const float from = m.scale[v][r];
-        *at = s == from ? c[v][j] : s > 0.f ? rescale16<KV>(c[v][j], __fdiv_rn(from, s)) : make_uint4(0u, 0u, 0u, 0u);
+        // (a row of zeros asks for no scale of its own, so its ratio may overflow: 0 inf would be a NaN)
+        *at = s == from ? c[v][j]
+              : s > 0.f ? rescale16<KV>(c[v][j], fminf(__fdiv_rn(from, s), kMaxFinite))
+                        : make_uint4(0u, 0u, 0u, 0u);
       } else if (r < end && s > s_old && kept) {
         *at = rescale16<KV>(*at, __fdiv_rn(s_old, s));
       }
