@@ -25,16 +25,23 @@ registries -- finds them under the ``spatten`` namespace:
   Tensor page_table, Tensor cu_tokens, Tensor seq_lens, Tensor tree, int max_tokens, float sm_scale) -> Tensor``
 * ``spatten::paged_weighing_attention(Tensor q, Tensor k_pool, Tensor v_pool, Tensor k_scale, Tensor v_scale,
   Tensor(a!) weight, Tensor(b!) position, Tensor page_table, Tensor cu_tokens, Tensor seq_lens, Tensor positions,
-  int max_tokens, float sm_scale) -> Tensor`` (causal attention that accumulates its weights)
+  int max_tokens, float sm_scale, Tensor? tree=None) -> Tensor`` (attention that accumulates its weights; causal, or
+  under a tree's bits)
 * ``spatten::paged_evict(Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor(c!) k_scale, Tensor(d!) v_scale,
   Tensor(e!) weight, Tensor(f!) position, Tensor page_table, Tensor seq_lens, int keep, int recent, bool per_head)
   -> Tensor`` (new lengths)
 * ``spatten::paged_keep(Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor(c!) k_scale, Tensor(d!) v_scale,
-  Tensor page_table, Tensor cu_tokens, Tensor seq_lens, Tensor accepted) -> Tensor`` (new lengths)
+  Tensor page_table, Tensor cu_tokens, Tensor seq_lens, Tensor accepted) -> Tensor`` (new lengths; for a cache
+  without accumulated weights)
+* ``spatten::paged_keep_weighed(Tensor(a!) k_pool, Tensor(b!) v_pool, Tensor(c!) k_scale, Tensor(d!) v_scale,
+  Tensor(e!) weight, Tensor(f!) position, Tensor page_table, Tensor cu_tokens, Tensor seq_lens, Tensor accepted)
+  -> Tensor`` (the same with the tokens' weights and positions moving along)
 
 CUDA tensors only, like the rest of the package. Importing this module
 registers the ops once.
 """
+from typing import Optional
+
 import torch
 
 from . import paged as _pd
@@ -115,10 +122,11 @@ def paged_tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
 def paged_weighing_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
                              v_scale: torch.Tensor, weight: torch.Tensor, position: torch.Tensor,
                              page_table: torch.Tensor, cu_tokens: torch.Tensor, seq_lens: torch.Tensor,
-                             positions: torch.Tensor, max_tokens: int, sm_scale: float) -> torch.Tensor:
+                             positions: torch.Tensor, max_tokens: int, sm_scale: float,
+                             tree: Optional[torch.Tensor] = None) -> torch.Tensor:
     return _pd.paged_attention(q, _pd.PagedKVCache(k_pool, v_pool, k_scale, v_scale), page_table, cu_tokens,
-                               seq_lens, max_tokens, sm_scale=sm_scale, weights=_pd.PagedWeights(weight, position),
-                               positions=positions)
+                               seq_lens, max_tokens, sm_scale=sm_scale, tree=tree,
+                               weights=_pd.PagedWeights(weight, position), positions=positions)
 
 
 _POOL = ("k_pool", "v_pool", "k_scale", "v_scale")
@@ -137,3 +145,11 @@ def paged_keep(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor
                page_table: torch.Tensor, cu_tokens: torch.Tensor, seq_lens: torch.Tensor, accepted: torch.Tensor
                ) -> torch.Tensor:
     return _pd.paged_keep(_pd.PagedKVCache(k_pool, v_pool, k_scale, v_scale), page_table, cu_tokens, seq_lens, accepted)
+
+
+@torch.library.custom_op("spatten::paged_keep_weighed", mutates_args=_POOL + ("weight", "position"))
+def paged_keep_weighed(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                       weight: torch.Tensor, position: torch.Tensor, page_table: torch.Tensor, cu_tokens: torch.Tensor,
+                       seq_lens: torch.Tensor, accepted: torch.Tensor) -> torch.Tensor:
+    return _pd.paged_keep(_pd.PagedKVCache(k_pool, v_pool, k_scale, v_scale), page_table, cu_tokens, seq_lens, accepted,
+                          weights=_pd.PagedWeights(weight, position))
