@@ -282,6 +282,11 @@ def paged_attention(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_sc
     added to ``weights.weight``; the new tokens' own start at 0, and their
     ``weights.position`` becomes ``positions`` (int32 [T]; default: the slot).
     Sequences must not share pages, nor claim the same rows, then."""
+    return _attend(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_scale, out, tree, weights, positions)
+
+
+def _attend(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_scale=None, out=None, tree=None, weights=None,
+            positions=None):
     ext = N.PagedAttendExtArgs() if tree is not None or weights is not None else None
     a = N.PagedAttendArgs() if ext is None else ext.attend
     dev, (P, G, page, D) = _fill(a, cache, page_table, seq_lens)

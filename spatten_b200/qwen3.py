@@ -132,6 +132,7 @@ class PagedQwen3Cache(Cache):
         mp = -(-self.max_tokens // page_size)
         self.pools = [paged.new_paged_cache(batch * mp, G, D, page_size, kv_dtype, device) for _ in range(L)]
         self.weights = [paged.new_paged_weights(p) for p in self.pools] if keep_tokens is not None else [None] * L
+        self.asked = [None] * L  # queries [B, S, H, D] of a layer's last forward and their scale, where accounts need them
         self.tree = None  # (bits, positions, tokens per sequence, positions before) of drafted tokens
         self.page_table = self._pages(batch, mp, device)
         self.seq_lens = torch.zeros((L, batch), dtype=torch.int32, device=device)
@@ -165,6 +166,7 @@ class PagedQwen3Cache(Cache):
         self.tree = None
         self.seq_lens.zero_()
         L = len(self.pools)
+        self.asked = [None] * L
         self.held, self.seen, self.pruned = [0] * L, [0] * L, [0] * L
 
     def crop(self, max_length):
@@ -268,6 +270,7 @@ class PagedQwen3Cache(Cache):
             lens.sub_(n)
             raise
         self.held[layer_idx] = held
+        self.asked[layer_idx] = None
         self.seen[layer_idx] += seen
         if n < seen:
             self.pruned[layer_idx] = self.seen[layer_idx]
@@ -281,6 +284,20 @@ class PagedQwen3Cache(Cache):
         self.held[layer_idx] = self.keep_tokens
         self.pruned[layer_idx] = self.seen[layer_idx]
         return self.keep_tokens
+
+    def note(self, layer_idx, q, S, sm_scale):
+        """The queries [B * S, H, D] that a forward of a drafted tree asked a layer with: what they give the
+        cached tokens counts once it is known which of them stay (``accept``)."""
+        if self.keep_tokens is not None and self.tree is not None:
+            self.asked[layer_idx] = q.view(self.batch, S, *q.shape[1:]), sm_scale
+
+    def _account(self, layer_idx, q, sm_scale, weights, positions=None):
+        """Adds what the queries [B, n, H, D] of a layer's last n tokens give its cached ones to ``weights``."""
+        B, n, H, D = q.shape
+        if q.is_cuda:
+            q.record_stream(torch.cuda.current_stream(q.device))
+        paged._attend(q.reshape(B * n, H, D), self.pools[layer_idx], self.page_table, self.packed(n),
+                      self.seq_lens[layer_idx], n, sm_scale=sm_scale, weights=weights, positions=positions)
 
     def positions(self, layer_idx, S):
         """Positions int32 [batch * S] of the next S tokens of each sequence."""
@@ -328,7 +345,9 @@ class PagedQwen3Cache(Cache):
 
     def accept(self, paths):
         """Of the drafted tree's tokens the ones at ``paths`` (per sequence their
-        places, ascending, equally many for each) stay, in every layer."""
+        places, ascending, equally many for each) stay, in every layer. With
+        ``keep_tokens`` the accepted ones' attention weights are added here, as if the
+        text had been given without a draft: the rejected ones' never count."""
         if self.tree is None or any(n != self.tree[3] + self.tree[2] for n in self.seen):
             raise RuntimeError("PagedQwen3Cache: no forward of a drafted tree")
         S = self.tree[2]
@@ -339,11 +358,17 @@ class PagedQwen3Cache(Cache):
             raise ValueError(f"PagedQwen3Cache: accepted places {paths} of {S} tokens (need them ascending)")
         accepted = torch.tensor(paths, dtype=torch.int32, device=self.seq_lens.device).view(self.batch, -1)
         gone, cu = S - accepted.shape[1], self.packed(S)
-        for pool, w, lens in zip(self.pools, self.weights, self.seq_lens):
-            lens.copy_(paged.paged_keep(pool, self.page_table, cu, lens, accepted, weights=w))
+        for pool, lens in zip(self.pools, self.seq_lens):  # (the new tokens have no weights yet)
+            lens.copy_(paged.paged_keep(pool, self.page_table, cu, lens, accepted))
         self.held = [n - gone for n in self.held]
-        self.seen = [n - gone for n in self.seen]
-        self.tree = None
+        before, self.tree = self.tree[3], None
+        for i, asked in enumerate(self.asked):
+            self.seen[i] = before
+            if asked is not None and S > gone:
+                q = asked[0][torch.arange(self.batch, device=accepted.device)[:, None], accepted.long()]
+                self._account(i, q, asked[1], self.weights[i], self.positions(i, S - gone))
+            self.asked[i] = None
+            self.seen[i] = before + S - gone
 
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
         """HF's form of ``store`` ([B, G, K, D]); only a prefill's first call may
@@ -417,17 +442,17 @@ class SpattenQwen3Attention(Qwen3Attention):
         positions = rows if cos.shape[0] == B else rows.repeat(B)
         cu, more = cache.packed(S), {}
         if cache.tree is not None:
-            more["tree"], at, drafted, before = cache.tree
+            more["tree"], _, drafted, before = cache.tree
             if S != drafted or cache.seen[self.layer_idx] != before:
                 raise RuntimeError(f"PagedQwen3Cache: {S} tokens after a drafted tree of {drafted} that was not accepted")
-        if cache.keep_tokens is not None:
-            more["weights"] = cache.weights[self.layer_idx]
-            more["positions"] = at if cache.tree is not None else cache.positions(self.layer_idx, S)
+        elif cache.keep_tokens is not None:
+            more["weights"], more["positions"] = cache.weights[self.layer_idx], cache.positions(self.layer_idx, S)
         q = cache.append(self.layer_idx, S, S, cu, k, v, q=q, cos=cos.reshape(-1, d), sin=sin.reshape(-1, d),
                          positions=positions, q_norm_w=self.q_norm.weight, k_norm_w=self.k_norm.weight,
                          eps=self.q_norm.variance_epsilon)
         out = paged.paged_attention(q, cache.pools[self.layer_idx], cache.page_table, cu,
                                     cache.seq_lens[self.layer_idx], S, sm_scale=self.scaling, **more)
+        cache.note(self.layer_idx, q, S, self.scaling)
         return self.o_proj(out.view(B, S, H * d)), None
 
     @torch.no_grad()

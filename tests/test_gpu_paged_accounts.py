@@ -1,0 +1,87 @@
+"""What PagedQwen3Cache(keep_tokens=...) counts while tokens are drafted: the attention
+weights of the text's tokens and no others, to the bounds of
+tests/test_gpu_paged_tokens.py where a call is compared with the oracle."""
+import pytest
+import torch
+
+from oracle import paged_tokens as OT
+from tests.test_gpu_paged import BF16, E4, I8, U, _cpu
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+
+
+@pytest.fixture()
+def lm(qwen3_model):
+    from transformers import Qwen3ForCausalLM
+    from spatten_b200.qwen3 import patch_qwen3
+    torch.manual_seed(0)
+    return patch_qwen3(Qwen3ForCausalLM(qwen3_model.config).to("cuda", BF16).eval())
+
+
+def _ids(B, n, seed):
+    return torch.randint(0, 1000, (B, n), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def _totals(cache, lm, tokens):
+    """Each token of the text gives a weight of 1 per query head, in every layer: a layer's
+    weights add up to them (fp32 sums of at most 2^8 rounded terms each, 2^-16)."""
+    H = lm.config.num_attention_heads
+    for w, n in zip(cache.weights, cache.held):
+        by_seq = w.weight.view(cache.batch, -1, *w.weight.shape[1:]).transpose(2, 3).flatten(1, 2)[:, :n]
+        total = by_seq.double().sum((1, 2))
+        assert torch.allclose(total, torch.full_like(total, tokens * H), rtol=2.0 ** -12), (total.tolist(), tokens * H)
+
+
+PARENTS = [-1, 0, 0, 1, 1, 2, 5, 6, -1]
+
+
+@pytest.mark.parametrize("kv,B", [(I8, 1), (E4, 2)])
+def test_rejected_drafts_of_a_tree_do_not_count(lm, kv, B):
+    """Over a text that a tree's accepted branch continued, each layer's weights are
+    those of before and what the oracle gives for the accepted tokens' queries."""
+    from spatten_b200.qwen3 import PagedQwen3Cache
+    cache = PagedQwen3Cache(lm.config, B, 120, page_size=16, kv_dtype=kv, keep_tokens=60, recent_tokens=8)
+    G, H, D = lm.config.num_key_value_heads, lm.config.num_attention_heads, lm.config.head_dim
+    with torch.no_grad():
+        lm(input_ids=_ids(B, 45, 1), past_key_values=cache, use_cache=True)
+        seen = 45
+        for step, path in enumerate(([0, 2, 5, 6], [], [8], [0, 1, 4], [0, 2, 5])):
+            _totals(cache, lm, seen)
+            pos = cache.draft_tree(torch.tensor([PARENTS] * B))
+            lm(input_ids=_ids(B, 9, step + 2), position_ids=pos, past_key_values=cache, use_cache=True)
+            before = [w.weight.double().cpu().clone() for w in cache.weights]
+            queries = [q[:, path].float().cpu() for q, _ in cache.asked]
+            cache.accept([path] * B)
+            seen, n = seen + len(path), len(path)
+            assert cache.held == [seen] * len(cache.held)
+            table, cu = cache.page_table.cpu(), [b * n for b in range(B + 1)]
+            for i, (w, q) in enumerate(zip(cache.weights, queries)):
+                want = before[i].view(B, -1, G, 16).transpose(2, 3).flatten(1, 2)[:, :seen - n]  # [B, slots, G]
+                _, _, _, add, err = OT.attend(q.reshape(B * n, H, D), _cpu(cache.pools[i]), table, cu, [seen] * B, D ** -0.5)
+                got = w.weight.double().cpu().view(B, -1, G, 16).transpose(2, 3).flatten(1, 2)[:, :seen]
+                at = w.position.cpu().view(B, -1, G, 16).transpose(2, 3).flatten(1, 2)[:, :seen]
+                assert (at == torch.arange(seen)[None, :, None]).all()
+                for b in range(B):
+                    total = torch.cat([want[b], torch.zeros(n, G).double()]) + (add[b].T if n else 0)
+                    tol = 2 * D * U * (err[b].T if n else 0) + total * (3 * 2.0 ** -16) + 1e-37
+                    assert ((got[b] - total).abs() <= tol).all()
+        _totals(cache, lm, seen)
+
+
+def test_a_text_continued_by_trees_weighs_its_tokens(lm):
+    from spatten_b200.qwen3 import PagedQwen3Cache
+    cache = PagedQwen3Cache(lm.config, 2, 120, page_size=16, keep_tokens=60, recent_tokens=8)
+    with torch.no_grad():
+        lm(input_ids=_ids(2, 30, 1), past_key_values=cache, use_cache=True)
+        for step in range(3):
+            pos = cache.draft_tree(torch.tensor([PARENTS] * 2))
+            lm(input_ids=_ids(2, 9, step + 2), position_ids=pos, past_key_values=cache, use_cache=True)
+            cache.accept([[0, 1, 3], [0, 2, 5]])
+            lm(input_ids=_ids(2, 1, step + 9), past_key_values=cache, use_cache=True)
+    _totals(cache, lm, 42)
