@@ -119,6 +119,10 @@ class PagedQwen3Cache(Cache):
     (``crop``), beams (``reorder_cache``), and changes of the batch
     (``batch_repeat_interleave``, ``batch_select_indices``)."""
 
+    # tokens of a forward that accounts can be taken back for: drafts are fewer, and more are
+    # a piece of the text (64 tokens of 32 x 128 are 0.5 MB a layer and sequence)
+    drafted = 64
+
     def __init__(self, config, batch, max_tokens, page_size=64, kv_dtype=torch.int8, device="cuda", keep_tokens=None,
                  recent_tokens=0):
         super().__init__(layers=[])
@@ -132,7 +136,7 @@ class PagedQwen3Cache(Cache):
         mp = -(-self.max_tokens // page_size)
         self.pools = [paged.new_paged_cache(batch * mp, G, D, page_size, kv_dtype, device) for _ in range(L)]
         self.weights = [paged.new_paged_weights(p) for p in self.pools] if keep_tokens is not None else [None] * L
-        self.asked = [None] * L  # queries [B, S, H, D] of a layer's last forward and their scale, where accounts need them
+        self.asked = [None] * L  # queries [B, n, H, D] of the last n tokens of a layer's last forward, and their scale
         self.tree = None  # (bits, positions, tokens per sequence, positions before) of drafted tokens
         self.page_table = self._pages(batch, mp, device)
         self.seq_lens = torch.zeros((L, batch), dtype=torch.int32, device=device)
@@ -174,7 +178,9 @@ class PagedQwen3Cache(Cache):
         the last ones), in every layer; their slots are written again by the next
         tokens. Positions of which a layer kept only some (a pruned prompt, or what
         there was at an eviction) can only be forgotten as a whole: which it kept is
-        not known here."""
+        not known here. With ``keep_tokens`` the attention weight that the forgotten ones
+        gave the others goes too, up to its rounding, for as many as were among the last
+        ``drafted`` (64) tokens of the last forward; that of earlier ones stays."""
         self._no_tree("crop")
         keep = int(max_length)
         if keep < 0:
@@ -187,6 +193,9 @@ class PagedQwen3Cache(Cache):
         for n, d, fixed in zip(self.seen, drop, self.pruned):
             if d and n - d < fixed:
                 raise NotImplementedError(f"PagedQwen3Cache: crop to {keep} inside {fixed} pruned tokens")
+        for i, d in enumerate(drop):
+            if d:
+                self._take_back(i, d)
         if len(set(drop)) == 1:
             self.seq_lens.sub_(drop[0])
         else:  # layers that were given different numbers of tokens
@@ -224,6 +233,11 @@ class PagedQwen3Cache(Cache):
                 t = self._by_sequence(t, -(-held // pool.k.shape[2]))
                 t.index_copy_(0, dst, t.index_select(0, src))
         self.seq_lens.index_copy_(1, dst, self.seq_lens.index_select(1, src))
+        self._ask_for(torch.tensor(rows, device=dev))
+
+    def _ask_for(self, idx):
+        """The noted queries of sequences idx."""
+        self.asked = [a and (a[0].index_select(0, idx), a[1]) for a in self.asked]
 
     def _select(self, rows):
         """Sequence b of a new batch is a copy of sequence rows[b]."""
@@ -235,6 +249,7 @@ class PagedQwen3Cache(Cache):
         self.pools = [paged.PagedKVCache(*map(select, pool)) for pool in self.pools]
         self.weights = [w and paged.PagedWeights(*map(select, w)) for w in self.weights]
         self.seq_lens = self.seq_lens.index_select(1, idx)
+        self._ask_for(idx)
         self.batch = len(rows)
         self.page_table = self._pages(self.batch, self.page_table.shape[1], idx.device)
 
@@ -285,11 +300,13 @@ class PagedQwen3Cache(Cache):
         self.pruned[layer_idx] = self.seen[layer_idx]
         return self.keep_tokens
 
-    def note(self, layer_idx, q, S, sm_scale):
-        """The queries [B * S, H, D] that a forward of a drafted tree asked a layer with: what they give the
-        cached tokens counts once it is known which of them stay (``accept``)."""
-        if self.keep_tokens is not None and self.tree is not None:
-            self.asked[layer_idx] = q.view(self.batch, S, *q.shape[1:]), sm_scale
+    def note(self, layer_idx, q, sm_scale):
+        """The queries [B, S, H, D] that a forward asked a layer with. Those of a drafted tree count
+        once it is known which of them stay (``accept``), others until they are cropped."""
+        if self.keep_tokens is not None:
+            if self.tree is None and q.shape[1] > self.drafted:
+                q = q[:, -self.drafted:].clone()
+            self.asked[layer_idx] = q, sm_scale
 
     def _account(self, layer_idx, q, sm_scale, weights, positions=None):
         """Adds what the queries [B, n, H, D] of a layer's last n tokens give its cached ones to ``weights``."""
@@ -298,6 +315,17 @@ class PagedQwen3Cache(Cache):
             q.record_stream(torch.cuda.current_stream(q.device))
         paged._attend(q.reshape(B * n, H, D), self.pools[layer_idx], self.page_table, self.packed(n),
                       self.seq_lens[layer_idx], n, sm_scale=sm_scale, weights=weights, positions=positions)
+
+    def _take_back(self, layer_idx, n):
+        """Before a layer's last n tokens leave: what they gave the others leaves with them."""
+        if self.asked[layer_idx] is None:
+            return
+        q, sm_scale = self.asked[layer_idx]
+        stay = max(q.shape[1] - n, 0)
+        gone = paged.new_paged_weights(self.pools[layer_idx])
+        self._account(layer_idx, q[:, stay:], sm_scale, gone)
+        self.weights[layer_idx].weight.sub_(gone.weight)  # (of the slots that are let go: anything)
+        self.asked[layer_idx] = (q[:, :stay], sm_scale) if stay else None
 
     def positions(self, layer_idx, S):
         """Positions int32 [batch * S] of the next S tokens of each sequence."""
@@ -367,7 +395,9 @@ class PagedQwen3Cache(Cache):
             if asked is not None and S > gone:
                 q = asked[0][torch.arange(self.batch, device=accepted.device)[:, None], accepted.long()]
                 self._account(i, q, asked[1], self.weights[i], self.positions(i, S - gone))
-            self.asked[i] = None
+                self.note(i, q, asked[1])
+            else:
+                self.asked[i] = None
             self.seen[i] = before + S - gone
 
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
@@ -452,7 +482,7 @@ class SpattenQwen3Attention(Qwen3Attention):
                          eps=self.q_norm.variance_epsilon)
         out = paged.paged_attention(q, cache.pools[self.layer_idx], cache.page_table, cu,
                                     cache.seq_lens[self.layer_idx], S, sm_scale=self.scaling, **more)
-        cache.note(self.layer_idx, q, S, self.scaling)
+        cache.note(self.layer_idx, q.view(B, S, H, d), self.scaling)
         return self.o_proj(out.view(B, S, H * d)), None
 
     @torch.no_grad()
@@ -523,6 +553,11 @@ class SpattenQwen3Attention(Qwen3Attention):
             # this layer's own weights: what it added to the cascade's
             past_key_values.store(self.layer_idx, k, v, S, positions=pos,
                                   importance=cum if st.cumulative is None else cum - st.cumulative)
+            if K == S and past_key_values.keep_tokens is not None:  # (else it cannot be cropped into)
+                if q8 is not None:
+                    last = slice(-past_key_values.drafted, None)
+                    q = (q8[:, :, last] * qs[:, :, last, None]).transpose(1, 2).to(v.dtype)
+                past_key_values.note(self.layer_idx, q, self.scaling)
         elif past_key_values is not None:
             # the cache concatenates into a new contiguous [B, Hkv, K, d] tensor
             # itself: the head-major views go in as they are (one copy, not two)

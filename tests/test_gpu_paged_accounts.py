@@ -85,3 +85,75 @@ def test_a_text_continued_by_trees_weighs_its_tokens(lm):
             cache.accept([[0, 1, 3], [0, 2, 5]])
             lm(input_ids=_ids(2, 1, step + 9), past_key_values=cache, use_cache=True)
     _totals(cache, lm, 42)
+
+
+@pytest.mark.parametrize("kv,B,n,stay", [(I8, 1, 6, 2), (E4, 2, 6, 5), (I8, 2, 1, 0), (E4, 1, 64, 1), (I8, 1, 90, 40)])
+def test_cropped_drafts_do_not_count(lm, kv, B, n, stay):
+    """n drafted tokens of which the last are cropped: each layer's weights are those of
+    before and what the oracle gives for the queries that stay. What was added and taken
+    back again leaves its rounding twice."""
+    from spatten_b200.qwen3 import PagedQwen3Cache
+    cache = PagedQwen3Cache(lm.config, B, 200, page_size=16, kv_dtype=kv, keep_tokens=150)
+    G, H, D, old = lm.config.num_key_value_heads, lm.config.num_attention_heads, lm.config.head_dim, 45
+    flat = lambda w: w.double().cpu().view(B, -1, G, 16).transpose(2, 3).flatten(1, 2)  # noqa: E731  [B, slots, G]
+    with torch.no_grad():
+        lm(input_ids=_ids(B, old, 1), past_key_values=cache, use_cache=True)
+        before = [flat(w.weight) for w in cache.weights]
+        lm(input_ids=_ids(B, n, 2), past_key_values=cache, use_cache=True)
+        queries = [q.float().cpu() for q, _ in cache.asked]
+        m = queries[0].shape[1]
+        assert m == min(n, 64) and n - stay <= m
+        cache.crop(stay - n if n == 6 else old + stay)  # (a negative length: that many of the last)
+        assert cache.get_seq_length() == old + stay
+    _totals(cache, lm, old + stay)
+    table, held = cache.page_table.cpu(), old + n
+    for i, (w, q) in enumerate(zip(cache.weights, queries)):
+        cu = [b * m for b in range(B + 1)]
+        args = _cpu(cache.pools[i]), table, cu
+        _, _, _, all_of, err = OT.attend(q.reshape(B * m, H, D), *args, [held] * B, D ** -0.5)
+        gone = q[:, m - (n - stay):].reshape(-1, H, D)
+        _, _, _, out_of, _ = OT.attend(gone, *args[:2], [b * (n - stay) for b in range(B + 1)], [held] * B, D ** -0.5)
+        got = flat(w.weight)[:, :old]
+        for b in range(B if n <= 64 else 0):  # (of more, the first ones' queries are not at hand: the totals)
+            want = before[i][b, :old] + (all_of[b] - out_of[b])[:, :old].T
+            most = before[i][b, :old] + all_of[b][:, :old].T
+            tol = 4 * D * U * err[b][:, :old].T + most * (6 * 2.0 ** -16) + 1e-37
+            assert ((got[b] - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_drafts_of_generate_do_not_count(lm, quant):
+    """HF's drafted tokens, the first ones in the prompt's own forward."""
+    from spatten_b200.qwen3 import PagedQwen3Cache
+    for layer in lm.model.layers:
+        layer.self_attn.enable_prog_quant = quant
+    ids = torch.randint(0, 50, (1, 10), generator=torch.Generator().manual_seed(1)).repeat(1, 4).cuda()
+    cache, dropped = PagedQwen3Cache(lm.config, 1, 128, page_size=16, keep_tokens=100), []
+    crop = cache.crop
+
+    def counted(length):
+        dropped.append(cache.get_seq_length() - length)
+        crop(length)
+        _totals(cache, lm, length)
+    cache.crop = counted
+    lm.generate(ids, attention_mask=torch.ones_like(ids), past_key_values=cache, max_new_tokens=30, min_new_tokens=30,
+                do_sample=False, eos_token_id=999, pad_token_id=0, prompt_lookup_num_tokens=4)
+    assert dropped[0] > 0 and sum(d > 0 for d in dropped) > 3
+
+
+def test_noted_queries_follow_their_sequences(lm):
+    """A crop after the batch was reordered and selected from; a second one takes what is left."""
+    from spatten_b200.qwen3 import PagedQwen3Cache
+    cache = PagedQwen3Cache(lm.config, 3, 64, page_size=16, keep_tokens=60)
+    with torch.no_grad():
+        lm(input_ids=_ids(3, 20, 1), past_key_values=cache, use_cache=True)
+        lm(input_ids=_ids(3, 6, 2), past_key_values=cache, use_cache=True)
+        cache.reorder_cache(torch.tensor([2, 0, 0]))
+        cache.batch_select_indices(torch.tensor([0, 2]))
+        cache.batch_repeat_interleave(2)
+        for n in (24, 21, 20):
+            cache.crop(n)
+            _totals(cache, lm, n)
+        assert cache.asked == [None] * len(cache.asked)
+        lm(input_ids=_ids(4, 5, 3), past_key_values=cache, use_cache=True)
+    _totals(cache, lm, 25)
