@@ -352,13 +352,15 @@ class PagedQwen3Cache(Cache):
 
     def _no_tree(self, what):
         if self.tree is not None:
-            raise RuntimeError(f"PagedQwen3Cache: {what} before the drafted tree's tokens were accepted")
+            raise RuntimeError(f"PagedQwen3Cache: {what} before the drafted tree's tokens were accepted (accept) or given up "
+                               "(drop_tree)")
 
     def draft_tree(self, parents):
         """The next forward's tokens [B, S] are a tree (or several): ``parents``
         [B, S] holds the place of each one's parent among them, before its own, or
         -1 for a child of the text so far. Returns their positions, int64 [B, S],
-        for the model's ``position_ids``; ``accept`` has to follow that forward."""
+        for the model's ``position_ids``; ``accept`` has to follow that forward, or
+        ``drop_tree``."""
         self._no_tree("another tree")
         B, S = parents.shape
         if B != self.batch or S < 1:
@@ -399,6 +401,18 @@ class PagedQwen3Cache(Cache):
             else:
                 self.asked[i] = None
             self.seen[i] = before + S - gone
+
+    def drop_tree(self):
+        """Give a drafted tree up, if there is one: before its forward, after it, or where that
+        failed on the way. Its tokens leave the layers that they had come to."""
+        if self.tree is None:
+            return
+        before, self.tree = self.tree[3], None
+        for i, n in enumerate(self.seen):
+            if n > before:
+                self.seq_lens[i].sub_(n - before)
+                self.held[i] -= n - before
+                self.seen[i], self.asked[i] = before, None
 
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
         """HF's form of ``store`` ([B, G, K, D]); only a prefill's first call may

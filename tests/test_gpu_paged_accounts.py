@@ -157,3 +157,29 @@ def test_noted_queries_follow_their_sequences(lm):
         assert cache.asked == [None] * len(cache.asked)
         lm(input_ids=_ids(4, 5, 3), past_key_values=cache, use_cache=True)
     _totals(cache, lm, 25)
+
+
+def test_a_tree_given_up_leaves_the_accounts(lm):
+    """After its forward, or when a layer raises."""
+    from spatten_b200.qwen3 import PagedQwen3Cache
+    cache = PagedQwen3Cache(lm.config, 1, 120, page_size=16, keep_tokens=60)
+    attn = lm.model.layers[1].self_attn
+    with torch.no_grad():
+        lm(input_ids=_ids(1, 30, 1), past_key_values=cache, use_cache=True)
+        before = [[t.clone() for t in w] for w in cache.weights]
+        for fails in (False, True):
+            pos = cache.draft_tree(torch.tensor([PARENTS]))
+            o_proj = attn.o_proj
+            attn.o_proj = None if fails else o_proj  # (no module)
+            try:
+                lm(input_ids=_ids(1, 9, 2), position_ids=pos, past_key_values=cache, use_cache=True)
+                assert not fails
+            except TypeError:
+                assert fails and cache.seen == [39, 39, 30]
+            attn.o_proj = o_proj
+            cache.drop_tree()
+            assert cache.held == cache.seen == [30] * 3
+            for w, was in zip(cache.weights, before):
+                assert all(torch.equal(a, b) for a, b in zip(w, was))
+        lm(input_ids=_ids(1, 3, 3), past_key_values=cache, use_cache=True)
+    _totals(cache, lm, 33)
