@@ -137,7 +137,7 @@ class PagedQwen3Cache(Cache):
         self.pools = [paged.new_paged_cache(batch * mp, G, D, page_size, kv_dtype, device) for _ in range(L)]
         self.weights = [paged.new_paged_weights(p) for p in self.pools] if keep_tokens is not None else [None] * L
         self.asked = [None] * L  # queries [B, n, H, D] of the last n tokens of a layer's last forward, and their scale
-        self.tree = None  # (bits, positions, tokens per sequence, positions before) of drafted tokens
+        self.tree = None  # (bits, parents, tokens per sequence, positions before) of drafted tokens
         self.page_table = self._pages(batch, mp, device)
         self.seq_lens = torch.zeros((L, batch), dtype=torch.int32, device=device)
         self.held = [0] * L  # slots of each layer, as the host counts them
@@ -369,13 +369,15 @@ class PagedQwen3Cache(Cache):
             raise ValueError("PagedQwen3Cache: a drafted tree follows a prompt")
         dev = self.seq_lens.device
         lens = torch.full((B,), self.seen[0] + S, dtype=torch.int32, device=dev)
-        bits, positions = paged.paged_tree(parents.to(dev, torch.int32).reshape(-1), self.packed(S), lens, S)
-        self.tree = bits, positions, S, self.seen[0]
+        parents = parents.to(dev, torch.int32, copy=True)
+        bits, positions = paged.paged_tree(parents.reshape(-1), self.packed(S), lens, S)
+        self.tree = bits, parents, S, self.seen[0]
         return positions.view(B, S).long()
 
     def accept(self, paths):
         """Of the drafted tree's tokens the ones at ``paths`` (per sequence their
-        places, ascending, equally many for each) stay, in every layer. With
+        places, ascending, equally many for each) stay, in every layer: a branch from the
+        text on, each of them one position behind the one before it. With
         ``keep_tokens`` the accepted ones' attention weights are added here, as if the
         text had been given without a draft: the rejected ones' never count."""
         if self.tree is None or any(n != self.tree[3] + self.tree[2] for n in self.seen):
@@ -386,6 +388,13 @@ class PagedQwen3Cache(Cache):
             raise ValueError(f"PagedQwen3Cache: need as many accepted tokens for each of {self.batch} sequences")
         if any(p != sorted(set(p)) or (p and not 0 <= p[0] <= p[-1] < S) for p in paths):
             raise ValueError(f"PagedQwen3Cache: accepted places {paths} of {S} tokens (need them ascending)")
+        for up, path in zip(self.tree[1].tolist(), paths):
+            depth = []
+            for i, a in enumerate(up):  # (as paged_tree: another value makes a child of the text)
+                depth.append(depth[a] + 1 if 0 <= a < i else 0)
+            if [depth[i] for i in path] != list(range(len(path))):
+                raise ValueError(f"PagedQwen3Cache: accepted places {path} are {[depth[i] for i in path]} positions behind "
+                                 "the text (need a branch: 0, 1, ..)")
         accepted = torch.tensor(paths, dtype=torch.int32, device=self.seq_lens.device).view(self.batch, -1)
         gone, cu = S - accepted.shape[1], self.packed(S)
         for pool, lens in zip(self.pools, self.seq_lens):  # (the new tokens have no weights yet)

@@ -46,3 +46,19 @@ def test_a_tree_that_evicted_can_be_given_up(monkeypatch):
     assert c.held == [10, 16] and c.seen == [16, 16] and c.seq_lens[:, 0].tolist() == [10, 16]
     _forward(c, 1)
     assert c.held == [11, 17] and c.seen == [17, 17]
+
+
+def test_accepted_places_continue_the_text(monkeypatch):
+    """Places whose positions skip or repeat are no branch."""
+    c, calls = _qwen(monkeypatch)
+    parents = torch.tensor([[-1, 0, 0, 1, 7, 3], [-1, 0, 1, -5, 3, 4]])
+    _forward(c, 5)
+    c.draft_tree(parents)
+    parents.zero_()  # the cache has its own
+    _forward(c, 6)
+    for bad in ([[1], [0]], [[0], [1]], [[0, 3], [0, 1]], [[0, 4], [0, 1]], [[0, 1, 2], [0, 1, 2]], [[0, 1], [0, 3]]):
+        with pytest.raises(ValueError, match="branch"):
+            c.accept(bad)
+    assert c.tree is not None and c.seen == [11, 11] and not any(x[0] == "keep" for x in calls)
+    c.accept([[0, 1, 3], [3, 4, 5]])
+    assert calls[-1] == ("keep", [[0, 1, 3], [3, 4, 5]], False) and c.seen == [8, 8]
