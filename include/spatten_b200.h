@@ -321,6 +321,8 @@ typedef struct {
 } spatten_paged_append_args;
 
 int spatten_paged_append(const spatten_paged_append_args* a, void* stream);
+/* What spatten_paged_append would refuse, without a launch: its status. */
+int spatten_paged_append_check(const spatten_paged_append_args* a);
 
 /*
  * Attention of the new tokens' queries over the cache: query i of sequence b

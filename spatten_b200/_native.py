@@ -181,6 +181,7 @@ SIGNATURES = {
     "spatten_decode_importance": (c_int, [ctypes.POINTER(DecodeArgs), c_vp, ctypes.c_size_t, c_vp]),
     "spatten_decode_attend": (c_int, [ctypes.POINTER(DecodeArgs), c_vp, ctypes.c_size_t, c_vp]),
     "spatten_paged_append": (c_int, [ctypes.POINTER(PagedAppendArgs), c_vp]),
+    "spatten_paged_append_check": (c_int, [ctypes.POINTER(PagedAppendArgs)]),
     "spatten_paged_attend_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(PagedAttendArgs)]),
     "spatten_paged_attend": (c_int, [ctypes.POINTER(PagedAttendArgs), c_vp, ctypes.c_size_t, c_vp]),
     "spatten_paged_read": (c_int, [ctypes.POINTER(PagedReadArgs), c_vp]),

@@ -605,14 +605,13 @@ static int check_workspace(const char* who, const void* ws, size_t bytes, size_t
   return SPATTEN_OK;
 }
 
-int spatten_paged_append(const spatten_paged_append_args* a, void* stream) {
+static int fill_paged_append(const spatten_paged_append_args* a, spatten::PagedAppendParams& p) {
   static const char* who = "paged_append";
   if (!a) return fail(SPATTEN_ERR_INVALID, "%s: null args", who);
-  spatten::PagedAppendParams p;
   if (int e = fill_paged_cache(who, a->cache, a->B, true, p.c)) return e;
   if (int e = fill_paged_batch(who, a->dtype, a->B, a->H, a->T, a->max_tokens, a->cu_tokens, a->seq_lens, p.b))
     return e;
-  if (p.b.B == 0 || p.b.max_tokens == 0) return ok();
+  if (p.b.B == 0 || p.b.max_tokens == 0) return SPATTEN_OK;
   if (p.b.max_tokens / p.c.page + 2 > 65535)
     return fail(SPATTEN_ERR_UNSUPPORTED, "%s: more than 65533 pages of new tokens in one sequence", who);
   if (int e = check_rows(who, "k", a->k, a->k_st, a->k_sh)) return e;
@@ -648,6 +647,19 @@ int spatten_paged_append(const spatten_paged_append_args* a, void* stream) {
   p.cos = a->cos; p.sin = a->sin;
   p.cs_f32 = a->cs_dtype == SPATTEN_DTYPE_F32; p.cs_rows = a->cs_rows; p.cs_st = a->cs_stride;
   p.positions = a->positions;
+  return SPATTEN_OK;
+}
+
+int spatten_paged_append_check(const spatten_paged_append_args* a) {
+  spatten::PagedAppendParams p;
+  if (int e = fill_paged_append(a, p)) return e;
+  return ok();
+}
+
+int spatten_paged_append(const spatten_paged_append_args* a, void* stream) {
+  spatten::PagedAppendParams p;
+  if (int e = fill_paged_append(a, p)) return e;
+  if (p.b.B == 0 || p.b.max_tokens == 0) return ok();
   return cuda_status(spatten::launch_paged_append(p, a->dtype, a->cache.kv_type, (cudaStream_t)stream),
                      "paged_append launch");
 }

@@ -198,6 +198,20 @@ def paged_append(cache, k, v, page_table, cu_tokens, seq_lens, max_tokens, q=Non
     the tables, clamped to them. The arithmetic is fp32, rounded once. A page's
     scale only grows; where it does, its earlier codes are rounded again.
     Two sequences must not append into the same page in one call."""
+    dev, a, q_out = _append_args(cache, k, v, page_table, cu_tokens, seq_lens, max_tokens, q, cos, sin, positions,
+                                 q_norm_w, k_norm_w, eps, q_out)
+    _call(N.lib.spatten_paged_append, dev, a)
+    return q_out
+
+
+def _check_append(*args, **kw):
+    """Raises what ``paged_append`` would with these arguments; does nothing else."""
+    N.check(N.lib.spatten_paged_append_check(_append_args(*args, **kw)[1]))
+
+
+def _append_args(cache, k, v, page_table, cu_tokens, seq_lens, max_tokens, q=None, cos=None, sin=None,
+                 positions=None, q_norm_w=None, k_norm_w=None, eps=1e-6, q_out=None):
+    """(device index, the call's arguments, q_out); their checks."""
     a = N.PagedAppendArgs()
     dev, (_, G, _, D) = _fill(a, cache, page_table, seq_lens)
     dt, T = k.dtype, k.shape[0]
@@ -241,8 +255,7 @@ def paged_append(cache, k, v, page_table, cu_tokens, seq_lens, max_tokens, q=Non
                 raise ValueError(f"positions: {positions.shape[0]} for {T} rows")
     elif positions is not None:
         raise ValueError("positions without cos / sin")
-    _call(N.lib.spatten_paged_append, dev, a)
-    return q_out
+    return dev, a, q_out
 
 
 def paged_tree(parents, cu_tokens, seq_lens, max_tokens):

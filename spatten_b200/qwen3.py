@@ -275,6 +275,8 @@ class PagedQwen3Cache(Cache):
         if before + n > self.max_tokens:
             if self.keep_tokens is None or self.keep_tokens + n > self.max_tokens or before <= self.keep_tokens:
                 raise ValueError(f"PagedQwen3Cache: {before} + {n} tokens, room for {self.max_tokens}")
+            if self.seq_lens.is_cuda:  # (elsewhere the eviction itself refuses)
+                paged._check_append(self.pools[layer_idx], k, v, self.page_table, cu, self.seq_lens[layer_idx], n, **kw)
             before = self._evict(layer_idx)
         held = before + n
         lens = self.seq_lens[layer_idx]

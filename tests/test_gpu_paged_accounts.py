@@ -183,3 +183,26 @@ def test_a_tree_given_up_leaves_the_accounts(lm):
                 assert all(torch.equal(a, b) for a, b in zip(w, was))
         lm(input_ids=_ids(1, 3, 3), past_key_values=cache, use_cache=True)
     _totals(cache, lm, 33)
+
+
+def test_a_refused_append_forgets_nothing(lm):
+    """A full cache evicts only for tokens that it can take."""
+    from spatten_b200.qwen3 import PagedQwen3Cache
+    cache = PagedQwen3Cache(lm.config, 1, 48, page_size=16, keep_tokens=30)
+    G, D = lm.config.num_key_value_heads, lm.config.head_dim
+    with torch.no_grad():
+        lm(input_ids=_ids(1, 48, 1), past_key_values=cache, use_cache=True)
+    was = [t.clone().view(I8) for i in range(3) for t in (*cache.pools[i], *cache.weights[i])]
+    good = torch.zeros(2, G, D, dtype=BF16, device="cuda")
+    shifted = torch.zeros(2 * G * D + 1, dtype=BF16, device="cuda")[1:].view(2, G, D)  # not 16-byte aligned
+    cos = torch.zeros(2, D, dtype=BF16, device="cuda")
+    for k, kw in ((good.float(), {}), (good[:1], {}), (good[..., :64], {}), (good.cpu(), {}), (shifted, {}),
+                  (good, dict(cos=cos)), (good, dict(cos=cos, sin=cos.float())), (good, dict(q_norm_w=cos[0])),
+                  (good, dict(k_norm_w=good[0, 0], eps=-1.0))):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            cache.append(0, 2, 2, cache.packed(2), k, good, **kw)
+    assert cache.held == cache.seen == [48] * 3 and cache.pruned == [0] * 3 and (cache.seq_lens == 48).all()
+    for t, old in zip([t.view(I8) for i in range(3) for t in (*cache.pools[i], *cache.weights[i])], was):
+        assert torch.equal(t, old)
+    cache.append(0, 2, 2, cache.packed(2), good, good)
+    assert cache.held == [32, 48, 48] and cache.pruned[0] == 48
