@@ -771,11 +771,14 @@ namespace {
 
 // Which kernels a call takes. Sequences of more than kTcRows query rows per KV
 // head (pieces of prompts) go to the tcgen05 kernel, the others to the one above; of more
-// than kTcRowsAlike where all of the call's have as many.
+// than kTcRowsAlike where all of the call's have as many. Causal calls go by these counts
+// alone, so that their bits do not change with the width of the page table.
 // At 32 / 8 heads x 128, 32 sequences over 8192 keys take at 32, 48 and 64 rows 235, 343
-// and 452 us here, 291 there from 33 on (int8); 183, 267 and 358, and 287 (e4m3). 64 rows
+// and 452 us here, 291 there from 33 on (int8); 183, 267 and 358, and 287 (e4m3): the border
+// for sequences alike is where e4m3's sides meet, int8's do at about 40. 64 rows
 // take 36 us there and 43 us here at 4 sequences over 4096 keys, 57 and 71 us at one over
-// 32768, 42 and 50 us at 16 over 1000 (e4m3). Lengths are not known on the host, which
+// 32768, 42 and 50 us at 16 over 1000 (e4m3), but 26 and 14 us at one over 800 (int8). Lengths
+// are not known on the host, which
 // knows the largest sequence's rows only. Where
 // the rows show that some must be shorter, both are launched and each serves its
 // own, so that single tokens beside a prompt's piece keep the kernel made for
@@ -783,18 +786,14 @@ namespace {
 // 150); for a few rows more that does not pay (24 trees of 3 to 17 tokens, 9 to 51 rows,
 // over 20 to 4096 keys: 55 us in both, 25 here), hence the two borders.
 //
-// Trees (whose rows are many for the tokens they come from) and calls of up to kFewRows
-// rows stay here while their work is small: tiles of 16 rows x 16 keys over the
-// whole page table, a row tile's set-up counted as kTileCost of them. At 32 / 8 heads x
-// 128 (int8), that work, the time there and here: 64 rows of one sequence over
-// 800 keys 3100, 25.8 and 14.4 us, 96 over 1500 6776, 27.5 and 16.3, 64 of four over 777
-// 12320, 23.7 and 19.4, of one over 6000 16040, 30.8 and 24.1, of 16 over 300 28800, 29.2
-// and 32.0; trees of 26 tokens of one over 3000 keys
+// Trees, whose rows are many for the tokens they come from, stay here while their work is
+// small: tiles of 16 rows x 16 keys over the
+// whole page table (whatever the sequences hold of it), a row tile's set-up counted as kTileCost
+// of them. At 32 / 8 heads x
+// 128 (int8), that work, the time there and here: trees of 26 tokens of one over 3000 keys
 // 12780, 29.7 and 23.5, of 64 over 1500 16456, 34.8 and 28.0, of 26 of four sequences over 777
 // 18480, 25.6 and 29.9, of 64 of two over 777 20944, 30.7 and 32.1, of 64 of four over 1500 65824,
-// 35.5 and 67.7. Longer pieces take the tcgen05 kernel even so: a prompt's
-// bits do not change with the width of its page table.
-constexpr int kFewRows = 128;
+// 35.5 and 67.7. (Measured for those heads and D alone.)
 constexpr double kFewTiles = 17500, kTileCost = 25;
 
 struct Plan {
@@ -808,9 +807,7 @@ Plan plan_for(const PagedAttendParams& p) {
   x.tc.rows_upto = x.few.rows_upto = INT64_MAX;
   if (!paged_attend_tc_takes(p)) return x;
   const double lines = ((double)p.b.T * (p.b.H / p.c.G) / 16 + p.b.B) * p.c.G;
-  if ((p.tree || (int64_t)p.b.max_tokens * (p.b.H / p.c.G) <= kFewRows) &&
-      lines * ((double)p.c.max_pages * (p.c.page / 16) + kTileCost) <= kFewTiles)
-    return x;
+  if (p.tree && lines * ((double)p.c.max_pages * (p.c.page / 16) + kTileCost) <= kFewTiles) return x;
   x.use_tc = true;
   x.use_few = p.b.B > 1 && p.b.T < (int64_t)p.b.B * p.b.max_tokens;
   if (x.use_few) x.tc.rows_over = x.few.rows_upto = kTcRows;
