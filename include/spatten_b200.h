@@ -446,7 +446,8 @@ int spatten_paged_attend_ext(const spatten_paged_attend_ext_args* a, void* works
  * largest moved magnitude needs; where S grew its other codes are rounded again as
  * in spatten_paged_append. new_lens[b] (int32, may be seq_lens) = keep, or
  * seq_lens[b] where that is not above it. A sequence with a slot that has no
- * memory is left as it is. Sequences must not share pages that are moved into.
+ * memory, or with more slots than the pool, is left as it is. Sequences must not
+ * share pages that are moved into.
  * At most 2^20 slots in a page-table row; 1 <= keep, 0 <= recent.
  */
 typedef struct {

@@ -136,17 +136,32 @@ SPATTEN_DEV void move_block(MoveRows<PAGE>& m, const PagedCache& pc, int64_t to,
 // ---------------------------------------------------------------- eviction
 
 // What the selection leaves for the moves, per sequence (and KV head): `moves`
-// tokens, the i-th from slot src[i] to slot dst[i]; first[j]: moves into blocks before j.
+// tokens, the i-th from slot src[base + i] to slot dst[base + i]; first[j]: moves into blocks before j.
+//
+// The page tables may have many times the slots of the pool (256 sequences x 8 heads, tables of
+// 131072 slots beside a pool of 1.3 million: 2.2 GB for what lies by slot). Then by_pool: keys and
+// positions lie like the pool (sequences that share a page have the same there), and the lists'
+// places are taken as they are needed, at most one for each slot of the pool, as no two tokens move
+// to the same (a call that breaks that rule leaves the sequences alone that find no place).
 struct EvictPlan {
-  int32_t* head;    // [lines][4]: moves, new length
+  uint32_t* head;   // [lines][4]: moves, new length, base
   int32_t* first;   // [lines][blocks + 1]
-  int32_t* dst;     // [lines][cap]
-  int32_t* src;     // [lines][cap]
+  int32_t* dst;     // [room]
+  int32_t* src;     // [room]
+  unsigned long long* used;  // by_pool: places taken
   float* edge;      // [B][G][2]: scales of the block of slot `keep` before the moves
-  uint32_t* key;    // [lines][pitch]: weights in the order of integers, kNoKey: no memory
-  int32_t* place;   // [lines][pitch] positions, where recent > 0
-  int lines_per_b, blocks, cap, pitch;
+  uint32_t* key;    // [lines][pitch] or [P][lines_per_b][page]: weights in the order of integers, kNoKey: no memory
+  int32_t* place;   // the same of positions, where recent > 0
+  int64_t room;
+  int lines_per_b, blocks, cap, pitch, usable;  // usable: slots that a sequence may hold
+  bool by_pool;
 };
+
+// Where a slot's key lies when they lie like the pool; negative: no memory.
+SPATTEN_DEV int64_t pooled_key(const PagedCache& c, const EvictPlan& plan, int b, int hl, int slot, int page_log) {
+  const int pid = paged_page(c, b, slot >> page_log);
+  return pid < 0 ? -1 : (((int64_t)pid * plan.lines_per_b + hl) << page_log) + (slot & (c.page - 1));
+}
 
 // Keys of the slots, four of a page a thread. Weights that are not negative order as
 // integers; negative ones and NaN count as 0.
@@ -158,7 +173,8 @@ __global__ void __launch_bounds__(kRankThreads) paged_rank_kernel(const PagedEvi
   grid_wait();
   const int b = blockIdx.z, hl = blockIdx.y, slot = blockIdx.x * kRankSlots + 4 * threadIdx.x;
   const int len = *(p.lens + b), G = p.c.G, page = p.c.page;
-  if (len <= p.keep || slot >= len || (int64_t)len > (int64_t)p.c.max_pages * page) return;
+  if (plan.by_pool && blockIdx.x == 0 && b == 0 && hl == 0 && threadIdx.x == 0) *plan.used = 0;
+  if (len <= p.keep || slot >= len || len > plan.usable) return;
   const int pid = paged_page(p.c, b, slot / page);
   const int64_t row = ((int64_t)max(pid, 0) * G + hl) * page + slot % page;
   float w[4];
@@ -178,7 +194,9 @@ __global__ void __launch_bounds__(kRankThreads) paged_rank_kernel(const PagedEvi
   uint32_t k[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) k[i] = pid < 0 ? kNoKey : w[i] > 0.f ? __float_as_uint(w[i]) : 0u;
-  const int64_t at = ((int64_t)b * plan.lines_per_b + hl) * plan.pitch + slot;
+  const int64_t at = plan.by_pool ? ((int64_t)pid * plan.lines_per_b + hl) * page + slot % page
+                                  : ((int64_t)b * plan.lines_per_b + hl) * plan.pitch + slot;
+  if (at < 0) return;  // (no memory, and no place for its key)
   *reinterpret_cast<uint4*>(plan.key + at) = make_uint4(k[0], k[1], k[2], k[3]);
   if (p.recent > 0) *reinterpret_cast<int4*>(plan.place + at) = *reinterpret_cast<const int4*>(p.position + row);
 }
@@ -225,8 +243,8 @@ SPATTEN_DEV uint32_t lowest_bits(uint32_t t, uint32_t m) {
 // others' shared memory go out together.
 constexpr int kCluster = 8;
 
-// CACHED: a run's keys (and positions) fit the shared memory.
-template <bool CACHED, int NT>
+// CACHED: a run's keys (and positions) fit the shared memory. POOL: plan.by_pool.
+template <bool CACHED, int NT, bool POOL>
 __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams p, const EvictPlan plan,
                                                                    int run, int cached) {
   extern __shared__ __align__(16) uint8_t dsm[];
@@ -243,26 +261,34 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
   const int G = p.c.G, page = p.c.page, page_log = __ffs(page) - 1, keep = p.keep;
   const int64_t line = (int64_t)b * plan.lines_per_b + hl;
   const int len = *(p.lens + b);
-  int32_t* const head = plan.head + line * 4;
-  if (len <= keep || (int64_t)len > (int64_t)p.c.max_pages * page) {  // (the same for the whole cluster)
+  uint32_t* const head = plan.head + line * 4;
+  auto leave_alone = [&]() {
     if (rank == 0 && tid == 0) {
-      head[0] = 0;
-      head[1] = len;
+      head[0] = 0u;
+      head[1] = (uint32_t)len;
     }
+  };
+  if (len <= keep || len > plan.usable) {  // (the same for the whole cluster)
+    leave_alone();
     return;
   }
-  const int lo = min(rank * run, len), n = min(run, len - lo), words = (n + 31) / 32;
+  // tables that are wider than the pool: the CTAs share the sequence's own slots (48 by head in tables
+  // of ten times their slots: 151 us, 175 in runs of the table's)
+  int part = run;
+  if constexpr (POOL) part = min(run, (((len + CL - 1) >> (__ffs(CL) - 1)) + 31) / 32 * 32);  // (CL: 1 to 8)
+  const int lo = min(rank * part, len), n = min(part, len - lo), words = (n + 31) / 32;
 
-  const uint32_t* const key_at = plan.key + line * plan.pitch + lo;
-  const int32_t* const place_at = plan.place + line * plan.pitch + lo;
-  auto key = [&](int i) { return CACHED ? keys[i] : key_at[i]; };
+  auto at = [&](int i) { return POOL ? pooled_key(p.c, plan, b, hl, lo + i, page_log) : line * plan.pitch + lo + i; };
+  auto key = [&](int i) { return CACHED ? keys[i] : plan.key[at(i)]; };
 
   // keys, the newest position, whether every slot has memory (pitch and runs are multiples of 32)
   int newest = INT_MIN;
   bool hole = false;
 #pragma unroll 2
   for (int i = 4 * tid; i < n; i += 4 * NT) {
-    const uint4 k = *reinterpret_cast<const uint4*>(key_at + i);
+    const int64_t from = at(i);
+    uint4 k = make_uint4(kNoKey, kNoKey, kNoKey, kNoKey);
+    if (!POOL || from >= 0) k = *reinterpret_cast<const uint4*>(plan.key + from);
     const uint32_t x[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) hole |= i + j < n && x[j] == kNoKey;
@@ -271,7 +297,9 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
   if (p.recent > 0) {
 #pragma unroll 2
     for (int i = 4 * tid; i < n; i += 4 * NT) {
-      const int4 k = *reinterpret_cast<const int4*>(place_at + i);
+      const int64_t from = at(i);
+      int4 k = make_int4(INT_MIN, INT_MIN, INT_MIN, INT_MIN);
+      if (!POOL || from >= 0) k = *reinterpret_cast<const int4*>(plan.place + from);
       const int x[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -300,11 +328,8 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
                               : make_uint2((uint32_t)INT_MIN, 0u);
     newest = __reduce_max_sync(0xffffffffu, (int)x.x);
     const uint32_t h = __reduce_max_sync(0xffffffffu, x.y);
-    if (h) {  // left as it is
-      if (rank == 0 && tid == 0) {
-        head[0] = 0;
-        head[1] = len;
-      }
+    if (h) {
+      leave_alone();
       cl.sync();
       return;
     }
@@ -317,7 +342,7 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
       const int i = base + tid;
       bool r = false;
       if (i < n) {
-        if (p.recent > 0) r = (int64_t)place_at[i] > (int64_t)newest - p.recent;
+        if (p.recent > 0) r = (int64_t)plan.place[at(i)] > (int64_t)newest - p.recent;
         const uint32_t k = key(i);
         if (r) {
           lo1 = min(lo1, k);
@@ -483,8 +508,24 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
   const uint32_t moves = __reduce_add_sync(0xffffffffu, counts.x);
   uint32_t d0 = __reduce_add_sync(0xffffffffu, lane < rank ? counts.x : 0u);
   uint32_t s0 = __reduce_add_sync(0xffffffffu, lane < rank ? counts.y : 0u);
-  int32_t* const dst = plan.dst + line * plan.cap;
-  int32_t* const src = plan.src + line * plan.cap;
+  uint32_t base = (uint32_t)(line * plan.cap);
+  if (POOL) {
+    if (rank == 0 && tid == 0) {
+      const unsigned long long first_place = atomicAdd(plan.used, (unsigned long long)moves);
+      sh.xch[0][0] = (uint32_t)first_place;
+      sh.xch[0][1] = first_place + moves <= (unsigned long long)plan.room;
+    }
+    cl.sync();
+    const uint2 x = *reinterpret_cast<const uint2*>(cl.map_shared_rank(&sh.xch[0][0], 0));
+    if (!x.y) {
+      leave_alone();
+      cl.sync();
+      return;
+    }
+    base = x.x;
+  }
+  int32_t* const dst = plan.dst + base;
+  int32_t* const src = plan.src + base;
   int32_t* const first = plan.first + line * (plan.blocks + 1);
   auto front_of = [&](int w) {  // slots before `keep` of a word
     const int at = lo + 32 * w;
@@ -512,8 +553,9 @@ __global__ void __launch_bounds__(NT) paged_select_kernel(const PagedEvictParams
   }
   if (rank == 0) {
     if (tid == 0) {
-      head[0] = (int)moves;
-      head[1] = keep;
+      head[0] = moves;
+      head[1] = (uint32_t)keep;
+      head[2] = base;
       first[plan.blocks] = (int)moves;
     }
     // the block of slot `keep` may change its scale while others read its tokens
@@ -539,8 +581,8 @@ __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_move_kernel(cons
   grid_wait();
   const int b = blockIdx.z, g = blockIdx.y, G = p.c.G, tid = threadIdx.x, blk = blockIdx.x;
   const int64_t line = (int64_t)b * plan.lines_per_b + (p.per_head ? g : 0);
-  const int2 head = *reinterpret_cast<const int2*>(plan.head + line * 4);
-  if (blk == 0 && g == 0 && tid == 0) p.new_lens[b] = head.y;
+  const uint4 head = *reinterpret_cast<const uint4*>(plan.head + line * 4);
+  if (blk == 0 && g == 0 && tid == 0) p.new_lens[b] = (int)head.y;
   if (head.x == 0) return;
   const int32_t* first = plan.first + line * (plan.blocks + 1) + blk;
   const int f0 = first[0], f1 = first[1];
@@ -551,7 +593,7 @@ __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_move_kernel(cons
   __syncthreads();
   const float2 edge_scale = *reinterpret_cast<const float2*>(plan.edge + ((int64_t)b * G + g) * 2);
   if (f0 + tid < f1) {  // a move per thread
-    const int s = plan.src[line * plan.cap + f0 + tid], d = plan.dst[line * plan.cap + f0 + tid] - blk * PAGE;
+    const int s = plan.src[head.z + f0 + tid], d = plan.dst[head.z + f0 + tid] - blk * PAGE;
     const int64_t from = (int64_t)paged_page(p.c, b, s / PAGE) * G + g, row = from * PAGE + s % PAGE;
     m.src[d] = (uint32_t)row;
     m.scale[0][d] = s / PAGE == edge ? edge_scale.x : p.c.k_scale[from];
@@ -629,13 +671,18 @@ __global__ void __launch_bounds__(MoveShape<D, PAGE>::NT) paged_keep_kernel(cons
   }
 }
 
+// Slots that a sequence may hold: those of its table, and no more than the pool has.
+int64_t usable_slots(const PagedEvictParams& p) {
+  return (int64_t)(p.c.max_pages < p.c.P ? p.c.max_pages : p.c.P) * p.c.page;
+}
+
 struct EvictSplit {
   int cluster, run, cached, threads;
   size_t smem;
 };
 
 EvictSplit split_for(const PagedEvictParams& p, int n_sm) {
-  const int64_t slots = (int64_t)p.c.max_pages * p.c.page;
+  const int64_t slots = usable_slots(p);
   EvictSplit s;
   const int64_t lines = (int64_t)p.B * (p.per_head ? p.c.G : 1);
   s.cluster = 1;
@@ -651,7 +698,9 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // plan (pointers null) and bytes
 size_t plan_for(const PagedEvictParams& p, void* ws, EvictPlan& x) {
-  const int64_t slots = (int64_t)p.c.max_pages * p.c.page;
+  const int64_t slots = usable_slots(p), pool = (int64_t)p.c.P * p.c.page;
+  x.usable = (int)slots;
+  x.by_pool = pool < (int64_t)p.B * p.c.max_pages * p.c.page;
   x.lines_per_b = p.per_head ? p.c.G : 1;
   const int64_t kept = p.keep < slots ? p.keep : slots;
   x.blocks = (int)((kept + p.c.page - 1) / p.c.page);
@@ -664,14 +713,18 @@ size_t plan_for(const PagedEvictParams& p, void* ws, EvictPlan& x) {
     at += align256(bytes);
     return w ? r : nullptr;
   };
-  x.head = reinterpret_cast<int32_t*>(take(lines * 16));
+  x.head = reinterpret_cast<uint32_t*>(take(lines * 16));
+  x.used = reinterpret_cast<unsigned long long*>(take(8));
   x.first = reinterpret_cast<int32_t*>(take(lines * (x.blocks + 1) * 4));
-  x.dst = reinterpret_cast<int32_t*>(take(lines * x.cap * 4));
-  x.src = reinterpret_cast<int32_t*>(take(lines * x.cap * 4));
+  x.room = (int64_t)lines * x.cap;  // (fewer than 2^32: the pool has fewer rows)
+  if (x.by_pool && x.room > x.lines_per_b * pool) x.room = x.lines_per_b * pool;
+  x.dst = reinterpret_cast<int32_t*>(take(x.room * 4));
+  x.src = reinterpret_cast<int32_t*>(take(x.room * 4));
   x.edge = reinterpret_cast<float*>(take((size_t)p.B * p.c.G * 8));
   x.pitch = (int)((slots + 31) / 32 * 32);
-  x.key = reinterpret_cast<uint32_t*>(take(lines * x.pitch * 4));
-  x.place = reinterpret_cast<int32_t*>(take(p.recent > 0 ? lines * x.pitch * 4 : 0));
+  const size_t keys = (x.by_pool ? (size_t)x.lines_per_b * pool : lines * x.pitch) * 4;
+  x.key = reinterpret_cast<uint32_t*>(take(keys));
+  x.place = reinterpret_cast<int32_t*>(take(p.recent > 0 ? keys : 0));
   return at;
 }
 
@@ -705,14 +758,14 @@ cudaError_t with_shape(int kv, int D, int page, F f) {
   return kv == kKvInt8 ? dims(std::integral_constant<int, kKvInt8>{}) : dims(std::integral_constant<int, kKvE4m3>{});
 }
 
-template <bool CACHED, int NT>
-cudaError_t select_launch(const PagedEvictParams& p, const EvictPlan& plan, const EvictSplit& s, cudaStream_t st) {
+template <bool CACHED, int NT, bool POOL>
+cudaError_t select_launch_as(const PagedEvictParams& p, const EvictPlan& plan, const EvictSplit& s, cudaStream_t st) {
   static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !((allowed.load(std::memory_order_relaxed) >> dev) & 1)) {
-    e = cudaFuncSetAttribute(paged_select_kernel<CACHED, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(paged_select_kernel<CACHED, NT, POOL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)kMostShared);
     if (e != cudaSuccess) return e;
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
@@ -730,7 +783,13 @@ cudaError_t select_launch(const PagedEvictParams& p, const EvictPlan& plan, cons
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, paged_select_kernel<CACHED, NT>, p, plan, s.run, s.cached);
+  return cudaLaunchKernelEx(&cfg, paged_select_kernel<CACHED, NT, POOL>, p, plan, s.run, s.cached);
+}
+
+template <bool CACHED, int NT>
+cudaError_t select_launch(const PagedEvictParams& p, const EvictPlan& plan, const EvictSplit& s, cudaStream_t st) {
+  return plan.by_pool ? select_launch_as<CACHED, NT, true>(p, plan, s, st)
+                      : select_launch_as<CACHED, NT, false>(p, plan, s, st);
 }
 
 }  // namespace

@@ -351,8 +351,9 @@ def paged_evict(cache, weights, page_table, seq_lens, keep, recent=0, per_head=F
     order: from then on slots are not in order of position, so later
     ``paged_append`` and ``paged_attention`` calls need ``positions``. A moved
     token is rounded to the scale of its new page, which grows as in
-    ``paged_append``. Sequences with slots that have no memory are left as they
-    are; sequences must not share the pages that tokens move into."""
+    ``paged_append``. Sequences with slots that have no memory, or more slots
+    than the pool, are left as they are; sequences must not share the pages that
+    tokens move into."""
     a = N.PagedEvictArgs()
     dev, (P, G, page, _) = _fill(a, cache, page_table, seq_lens)
     _weights(a, weights, dev, (P, G, page))
