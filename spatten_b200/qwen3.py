@@ -558,8 +558,11 @@ class SpattenQwen3Attention(Qwen3Attention):
         qh = q.permute(0, 2, 1, 3) if q is not None else None  # [B, H, S, d] views
         kh = k.permute(0, 2, 1, 3)   # [B, Hkv, K, d]
         vh = v.permute(0, 2, 1, 3)
+        # a cache that keeps accounts is given this layer's own weights, whole: as a difference of the
+        # cascade's fp32 sums over layers they would lose the bits that those have no room for
+        own = isinstance(past_key_values, PagedQwen3Cache) and past_key_values.keep_tokens is not None
         common = dict(sm_scale=self.scaling, v_thr=v_thr, v_prune_count=v_count, key_limit=key_limit,
-                      tok_in=st.cumulative, want_tok=True, out=out.permute(0, 2, 1, 3))
+                      tok_in=None if own else st.cumulative, want_tok=True, out=out.permute(0, 2, 1, 3))
         if self.enable_prog_quant:
             if q8 is None:
                 q8, qs = quant_q_int8(qh)
@@ -569,16 +572,16 @@ class SpattenQwen3Attention(Qwen3Attention):
             self.last_refetch = r.refetch
         else:
             r = prog_attn(qh, kh, vh, mode=N.MODE_DENSE, **common)
-        cum = r.token_importance
+        importance = cum = r.token_importance
+        if own and st.cumulative is not None:
+            cum = st.cumulative + importance  # (the sum that the kernel would have made)
         self.kept_positions = pos
         self.token_importance = cum
         st.kept_per_layer.append(K)
 
         if isinstance(past_key_values, PagedQwen3Cache):
-            # this layer's own weights: what it added to the cascade's
-            past_key_values.store(self.layer_idx, k, v, S, positions=pos,
-                                  importance=cum if st.cumulative is None else cum - st.cumulative)
-            if K == S and past_key_values.keep_tokens is not None:  # (else it cannot be cropped into)
+            past_key_values.store(self.layer_idx, k, v, S, positions=pos, importance=importance)
+            if K == S and own:  # (else it cannot be cropped into)
                 if q8 is not None:
                     last = slice(-past_key_values.drafted, None)
                     q = (q8[:, :, last] * qs[:, :, last, None]).transpose(1, 2).to(v.dtype)

@@ -206,3 +206,30 @@ def test_a_refused_append_forgets_nothing(lm):
         assert torch.equal(t, old)
     cache.append(0, 2, 2, cache.packed(2), good, good)
     assert cache.held == [32, 48, 48] and cache.pruned[0] == 48
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_a_prompts_weights_are_the_layers_own(lm, quant):
+    """Whatever the layers before gathered, to the bit; and the cascade's sums are those of a
+    model without such a cache."""
+    from spatten_b200.qwen3 import PagedQwen3Cache
+    attn = lm.model.layers[1].self_attn
+    attn.enable_prog_quant = quant
+    S, hidden = 40, lm.config.hidden_size
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(1, S, hidden, generator=g).to(BF16).cuda()
+    rope = lm.model.rotary_emb(x, torch.arange(S, device="cuda")[None])
+    past = torch.exp(4 * torch.randn(1, S, generator=g)).cuda() * 1e4
+    want, sums = None, None
+    for cumulative, cached in ((None, True), (past, True), (past, False)):
+        attn.cascade.positions = torch.arange(S, device="cuda")[None]
+        attn.cascade.cumulative = cumulative
+        cache = PagedQwen3Cache(lm.config, 1, 64, page_size=16, keep_tokens=40) if cached else None
+        attn(x, rope, past_key_values=cache)
+        if cached:
+            got = cache.weights[1].weight.clone()
+            assert want is None or torch.equal(got, want)
+            want = got
+        if cumulative is not None:
+            assert sums is None or torch.equal(attn.token_importance, sums)
+            sums = attn.token_importance
