@@ -329,8 +329,8 @@ __global__ void __launch_bounds__(kRowThreads) paged_weigh_rows_kernel(const Pag
 #pragma unroll
   for (int i = 0; i < kRowThreads / 32; ++i) most = fmaxf(most, red[i]);
   // One power of two for the tile, so that the sums need one number a row instead of two: where
-  // each row reaches 2^-12 of the largest magnitude, what f16 drops of it is below 2^-28 of
-  // the row's own largest.
+  // each row reaches 2^-12 of the largest magnitude, which goes to 2^14 or more, its own largest is 4
+  // or more: what f16 drops of it, at most half its smallest step 2^-24, is below 2^-27 of that.
   bool far = false;
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) far |= top[k] > 0.f && top[k] < most * 0x1p-12f;
@@ -828,7 +828,8 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 int64_t most_rows(const PagedWeighParams& p) { return (int64_t)p.a.b.max_tokens * (p.a.b.H / p.a.c.G); }
 
-// Chunks of 768 rows, up to 32 of them, in at most 1 GiB of sums: an item's keys cost
+// Chunks of 768 rows, up to 32 of them, in at most 1 GiB of sums (8 bytes a chunk and place; one
+// chunk there is always, whatever the places): an item's keys cost
 // about as much to widen as two tiles of rows to multiply and sum (1024 new tokens over 8192, 2
 // sequences: 313, 279, 263, 259 and 262 us with 256, 384, 512, 768 and 1024 rows).
 size_t plan_for(const PagedWeighParams& p, void* ws, WeighPlan& x) {

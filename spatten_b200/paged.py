@@ -264,8 +264,10 @@ def paged_tree(parents, cu_tokens, seq_lens, max_tokens):
     (which comes before its own), or -1 for a child of the cached tokens.
     Returns (tree int32 [T, ceil(min(max_tokens, T) / 32)], positions int32 [T]): bit j
     of a row's words is set if it sees new token j (itself and its ancestors);
-    its position is that of the sequence's first new token plus its depth.
-    At most 1024 tokens per sequence."""
+    its position is that of the sequence's first new token, ``seq_lens`` less
+    the new tokens, plus its depth (after an eviction, which leaves the cache
+    shorter than the text: pass the text's lengths). At most 1024 tokens per
+    sequence."""
     dev = parents.get_device()
     if dev < 0:
         raise ValueError("paged_tree: CUDA tensors expected (no CPU path)")
@@ -292,7 +294,8 @@ def paged_attention(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_sc
     sees every slot before its sequence's new tokens, and of these the ones
     whose bits its row has. ``weights``: the softmax weight that the queries
     give each cached token, summed over the query heads of its KV head, is
-    added to ``weights.weight``; the new tokens' own start at 0, and their
+    added to ``weights.weight`` (all rows count, also drafts that are rejected
+    later); the new tokens' own start at 0, and their
     ``weights.position`` becomes ``positions`` (int32 [T]; default: the slot).
     Sequences must not share pages, nor claim the same rows, then."""
     return _attend(q, cache, page_table, cu_tokens, seq_lens, max_tokens, sm_scale, out, tree, weights, positions)

@@ -34,7 +34,7 @@ attention core with the progressive sparse attention kernel:
   two. A layer that pruned its keys keeps attending over the ones it kept. With
   ``keep_tokens`` the cascade goes on while it generates: a full layer forgets
   the tokens of the least accumulated attention. Trees of drafted tokens are
-  checked in one forward (``draft_tree``, ``accept``).
+  checked in one forward (``draft_tree``, ``accept`` or ``drop_tree``).
 
 Unpadded batches only (the HF attention mask is not read: the mask is the
 causal one). The cascade state is shared by all layers of a model
