@@ -140,6 +140,8 @@ def test_weights_past_2_32_bytes(n, R):
     from oracle import paged_tokens as OT
     from spatten_b200 import paged
     torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 100e9:
+        pytest.skip("needs 77 GB of a GPU's memory")
     g = torch.Generator().manual_seed(81)
     G, D, page, L, mp = 1, 64, 128, 700, 7
     P = (1 << 30) // page + 100
